@@ -215,7 +215,7 @@ def _held(a, least, threshold):
     step a time would never move else."""
     big = a.amax(1, keepdim=True)
     # (Up to 2^-20 above a power of two counts as that power.)
-    top = _exponents(big * (1 - 2.0 ** -21))
+    top = _exponents(big * (1 - 2.0 ** -20))
     step = torch.exp2((torch.maximum(_exponents(a), top + least) - 3).to(a.dtype))
     return torch.floor(a / step + threshold * 2.0 ** -17) * step, top
 
