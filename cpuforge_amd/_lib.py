@@ -44,6 +44,12 @@ class LinearC(C.Structure):
                 ("y", _vp), ("xs", _vp), ("dy", _vp), ("gw", _vp), ("ga", _vp), ("gb", _vp)]
 
 
+class AdamwTensorC(C.Structure):
+    """`cfops_adamw_tensor` (include/cfops.h)."""
+    _fields_ = [("p", _vp), ("g", _vp), ("m", _vp), ("v", _vp), ("state8", _vp), ("n", _sz),
+                ("weight_decay", C.c_float)]
+
+
 SIGNATURES = {
     "cfattn_create": (C.c_int, [C.c_int, C.POINTER(_vp)]),
     "cfattn_destroy": (C.c_int, [_vp]),
@@ -101,6 +107,15 @@ SIGNATURES = {
     "cfops_adamw_update": (C.c_int, [_vp] * 5 + [_sz, C.c_uint64] + [C.c_float] * 5 + [_vp]),
     "cfops_adamw_update_multi": (C.c_int, [_vp, _sz] + [C.POINTER(_vp)] * 4 + [C.POINTER(_sz), _fp, C.c_uint64]
                                  + [C.c_float] * 4 + [_vp]),
+    "cfops_lm_head_logprobs": (C.c_int, [_vp] * 4 + [_sz] * 3 + [_vp] * 4),
+    "cfops_lm_head_logprobs_backward": (C.c_int, [_vp] * 6 + [_sz] * 3 + [_vp] * 3),
+    "cfops_preference_loss": (C.c_int, [_vp] * 4 + [_sz, _vp, _sz, C.c_int] + [C.c_double] * 3 + [C.c_int]
+                              + [_vp] * 4),
+    "cfops_policy_loss": (C.c_int, [_vp] * 6 + [_sz, _vp, _sz, C.c_int] + [C.c_double] * 3 + [C.c_int] + [_vp] * 3),
+    "cfops_adamw8_state_bytes": (_sz, [_sz]),
+    "cfops_adamw8_update_multi": (C.c_int, [_vp, _sz, C.POINTER(AdamwTensorC), C.c_uint64] + [C.c_float] * 4 + [_vp]),
+    "cfops_adamw8_pack_multi": (C.c_int, [_vp, _sz, C.POINTER(AdamwTensorC), _vp]),
+    "cfops_adamw8_unpack_multi": (C.c_int, [_vp, _sz, C.POINTER(AdamwTensorC), _vp]),
     # include/cfio.h
     "cfio_bf16_to_f32": (C.c_int, [_vp, _vp, _vp, _sz, _vp]),
     "cfio_f16_to_f32": (C.c_int, [_vp, _vp, _vp, _sz, _vp]),

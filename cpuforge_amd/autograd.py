@@ -183,6 +183,78 @@ class LMHeadCEDevFn(torch.autograd.Function):
         return (dhn * g).view(ctx.shape), (dhead * g if ctx.has_dhead else None), None
 
 
+class LMHeadLogprobsFn(torch.autograd.Function):
+    """The targets' log-probabilities under logits = hn head^T and the block
+    that ops.ce_check reads (ops.lm_head_logprobs)."""
+
+    @staticmethod
+    def forward(ctx, hn, head, targets):
+        d = hn.shape[-1]
+        h2, head2, tg = _flat(hn, d), head.contiguous(), targets.contiguous().view(-1)
+        t, vocab = h2.shape[0], head2.shape[0]
+        logp, lse = _empty(tg, tg)
+        result = P.ce_result_buffer(hn.device)
+        P.lm_head_logprobs(h2, head2, tg, t, d, vocab, logp, lse, result)
+        ctx.save_for_backward(h2, head2, tg, lse)
+        ctx.shape = hn.shape
+        ctx.mark_non_differentiable(result)
+        ctx.set_materialize_grads(False)
+        return logp.view(targets.shape), result
+
+    @staticmethod
+    def backward(ctx, g, _g_result):
+        h2, head, tg, lse = ctx.saved_tensors
+        need_hn, need_head = ctx.needs_input_grad[:2]
+        if g is None or not (need_hn or need_head):
+            return None, None, None
+        dhn = torch.empty_like(h2) if need_hn else None
+        dhead = torch.zeros_like(head) if need_head else None
+        P.lm_head_logprobs_backward(h2, head, tg, lse, g.contiguous().view(-1), h2.shape[0], h2.shape[1],
+                                    head.shape[0], dhn, dhead)
+        return None if dhn is None else dhn.view(ctx.shape), dhead, None
+
+
+class PreferenceLossFn(torch.autograd.Function):
+    """ops.preference_loss; its forward already forms dlogp."""
+
+    @staticmethod
+    def forward(ctx, logp, ref_logp, targets, offsets, kw):
+        lp = logp.contiguous()
+        dlogp = torch.zeros_like(lp)
+        rewards = torch.empty(offsets.numel() - 1, device=lp.device, dtype=torch.float32)
+        result = torch.empty(P.PREFERENCE_RESULT_WORDS, dtype=torch.int32, device=lp.device)
+        P.preference_loss(lp, _c(ref_logp), _c(targets), offsets, dlogp, rewards, result, **kw)
+        ctx.save_for_backward(dlogp)
+        ctx.mark_non_differentiable(rewards, result)
+        return P.preference_result(result).loss.clone(), rewards, result
+
+    @staticmethod
+    def backward(ctx, g, *_):
+        return ctx.saved_tensors[0] * g, None, None, None, None
+
+
+class PolicyLossFn(torch.autograd.Function):
+    """ops.policy_loss; its forward already forms dlogp."""
+
+    @staticmethod
+    def forward(ctx, logp, old_logp, ref_logp, advantages, targets, offsets, kw):
+        lp = logp.contiguous()
+        dlogp = torch.zeros_like(lp)
+        result = torch.empty(P.POLICY_RESULT_WORDS, dtype=torch.int32, device=lp.device)
+        P.policy_loss(lp, _c(old_logp), _c(ref_logp), _c(advantages), _c(targets), offsets, dlogp, result, **kw)
+        ctx.save_for_backward(dlogp)
+        ctx.mark_non_differentiable(result)
+        return P.policy_result(result).loss.clone(), result
+
+    @staticmethod
+    def backward(ctx, g, _):
+        return (ctx.saved_tensors[0] * g, *(None,) * 6)
+
+
+def _c(t):
+    return None if t is None else t.detach().contiguous()
+
+
 def rmsnorm(x, w, eps):
     return RMSNormFn.apply(x, w, eps)
 
@@ -209,3 +281,20 @@ def lm_head_ce(hn, head, targets):
 def lm_head_ce_dev(hn, head, targets):
     """(loss, cfops_ce_result block): the loss with no host wait."""
     return LMHeadCEDevFn.apply(hn, head, targets)
+
+
+def lm_head_logprobs(hn, head, targets):
+    """(log-probabilities of the targets, shaped as they are; 0 where the target
+    is ops.IGNORE_INDEX, and the block whose target check ops.ce_check runs)."""
+    return LMHeadLogprobsFn.apply(hn, head, targets)
+
+
+def preference_loss(logp, ref_logp, targets, offsets, **kw):
+    """(loss, rewards [2 * pairs], result block) of ops.preference_loss, whose
+    keywords it takes; logp's gradient is the loss's."""
+    return PreferenceLossFn.apply(logp, ref_logp, targets, offsets, kw)
+
+
+def policy_loss(logp, old_logp, ref_logp, advantages, targets, offsets, **kw):
+    """(loss, result block) of ops.policy_loss, whose keywords it takes."""
+    return PolicyLossFn.apply(logp, old_logp, ref_logp, advantages, targets, offsets, kw)

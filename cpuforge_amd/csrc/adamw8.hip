@@ -1,0 +1,310 @@
+// AdamW over many tensors whose moments are held in 8 bits or in 32
+// (cfops_adamw8_update_multi of include/cfops.h).
+//
+// An 8-bit state holds blocks of 256 consecutive values of a tensor.  With E
+// the block's power of two, its largest magnitude in (2^E, 2^(E+1)]:
+//   m: sign, 4 exponent, 3 mantissa bits; the binade [2^E, 2^(E+1)) is exponent
+//      field 14, fields 1 and up are normal, field 0 subnormal; 0x7f is NaN;
+//   v: 5 exponent, 3 mantissa bits; [2^E, 2^(E+1)) is field 30; 0xff is infinity.
+// E is held as a byte, E + 127.  A power of two costs a float code none of its
+// bits (an absmax scale would round the block's values once more), and a state
+// that is read, given as f32 and packed again is the same state.
+//
+// Rounding: up or down by the value's fraction of a step against 17 bits that
+// are a function of its index and the step count.  beta2 = 0.999 moves v by a
+// thousandth of itself a step and beta1 = 0.95 m by a twentieth, less than half a
+// step of three mantissa bits (1/16 to 1/8): rounded to nearest such a moment would
+// never move; so the mean of its roundings is the value.  A positive v is
+// never held as zero: the update divides by its root.
+// m' = b1 m + (1-b1) g and v' are formed in f64 (products of a held value, at most
+// four significant bits, and of f32s: one rounding in 53 bits), since a rounding
+// to 8 bits goes by what lies below f32; the update itself is f32 on (float)m'
+// and (float)v', not on the held values.
+//
+// What bounds it: HBM, 16 bytes a value a step (p read and written, g read, two
+// bytes read and written) against 28 with f32 states.
+#include <algorithm>
+
+#include "adamw_math.hpp"
+#include "cfattn_common.hpp"
+#include "cfops_kernels.hpp"
+
+namespace cfattn {
+namespace {
+
+constexpr int kBlock = 4096;  // values of a workgroup: 16 blocks, one to 16 lanes
+
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// The layout of a state of n values: codes of m and of v, a byte for every value
+// of whole blocks, then a byte for every block's exponent of m and of v.
+struct State8 {
+    uint8_t *m, *v, *em, *ev;
+};
+__device__ __forceinline__ State8 state8(uint8_t* s, long n) {
+    const long nb = (n + 255) / 256;
+    return {s, s + nb * 256, s + nb * 512, s + nb * 513};
+}
+
+__device__ __forceinline__ double pow2(int e) { return __builtin_bit_cast(double, (uint64_t)(uint32_t)(e + 1023) << 52); }
+__device__ __forceinline__ uint32_t hi_word(double a) { return (uint32_t)(__builtin_bit_cast(uint64_t, a) >> 32); }
+
+// A code's magnitude in units of 2^(E + 113) (m) or 2^(E + 97) (v): its fields are
+// an f32's, subnormals with them.
+__device__ __forceinline__ float code_unit(uint32_t c) { return __builtin_bit_cast(float, c << 20); }
+constexpr int kUnitM = -14, kUnitV = -30;  // of 2^byte
+
+__device__ __forceinline__ double decode_m(uint32_t c, double unit) {
+    const float y = code_unit(c & 0x7f);
+    const double x = (double)((c & 0x80) ? -y : y) * unit;
+    return (c & 0x7f) == 0x7f ? __builtin_nan("") : x;
+}
+__device__ __forceinline__ double decode_v(uint32_t c, double unit) {
+    return c == 0xff ? __builtin_inf() : (double)code_unit(c) * unit;
+}
+
+// The code of magnitude a; `least` is E's biased exponent of the first normal
+// binade and `low` its power of two.  r: 17 bits, the rounding threshold.  In the
+// high word of a double lie its exponent, the three mantissa bits of a code and
+// the 17 below them.  Below the first normal binade the steps are that binade's:
+// the sum with its power of two has them.
+__device__ __forceinline__ uint32_t encode(double a, uint32_t least, double low, uint32_t r) {
+    const bool normal = hi_word(a) >> 20 >= least;
+    const uint32_t u = (hi_word(normal ? a : a + low) + r) >> 17;
+    return u - (least << 3) + (normal ? 8 : 0);
+}
+
+// What f32 does not hold.
+__device__ __forceinline__ bool odd(uint32_t hi) { return (hi & 0x7fffffff) >= (1023u + 128) << 20; }
+
+// Byte of a block's exponent, from the largest high word of its magnitudes (up to
+// 2^-20 above a power of two counts as that power).
+__device__ __forceinline__ int exponent_byte(uint32_t hi) {
+    return max(0, (int)(hi >> 20) - 1023 + 127 - ((hi & 0xfffff) == 0));
+}
+
+// Largest of 16 lanes.
+__device__ __forceinline__ uint32_t max16(uint32_t x) {
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o));
+    return x;
+}
+
+// Two rounds of a 32-bit multiplicative mix.
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+    x = (x ^ (x >> 16)) * 0xA511E9B3u;
+    x = (x ^ (x >> 15)) * 0x63D83595u;
+    return x ^ (x >> 16);
+}
+
+// The tensor that workgroup b falls in.
+__device__ __forceinline__ const Adamw8Tensor& find(const Adamw8Args& a, long b) {
+    int lo = 0, hi = a.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (a.t[mid].block0 <= b)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return a.t[lo];
+}
+
+// Four consecutive values p[i..i+3] of n, those at or past n as zeros.
+__device__ __forceinline__ float4 load4(const float* p, long i, long n, bool vec) {
+    if (vec && i + 3 < n) return *reinterpret_cast<const float4*>(p + i);
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (i < n) x.x = p[i];
+    if (i + 1 < n) x.y = p[i + 1];
+    if (i + 2 < n) x.z = p[i + 2];
+    if (i + 3 < n) x.w = p[i + 3];
+    return x;
+}
+__device__ __forceinline__ void store4(float* p, long i, long n, bool vec, const float4& x) {
+    if (vec && i + 3 < n) {
+        *reinterpret_cast<float4*>(p + i) = x;
+        return;
+    }
+    if (i < n) p[i] = x.x;
+    if (i + 1 < n) p[i + 1] = x.y;
+    if (i + 2 < n) p[i + 2] = x.z;
+    if (i + 3 < n) p[i + 3] = x.w;
+}
+
+// Codes of a block's 16 values of this lane, four to a word.
+__device__ __forceinline__ void encode_block(const double (&m)[16], const double (&v)[16], const uint32_t (&r)[16],
+                                             uint32_t (&cm)[4], uint32_t (&cv)[4], int& em, int& ev) {
+    uint32_t tm = 0, tv = 0;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const uint32_t hm = hi_word(m[e]) & 0x7fffffff, hv = hi_word(v[e]) & 0x7fffffff;
+        tm = max(tm, odd(hm) ? 0u : hm);
+        tv = max(tv, odd(hv) ? 0u : hv);
+    }
+    em = exponent_byte(max16(tm));
+    ev = exponent_byte(max16(tv));
+    // Biased exponents of the first normal binades: E - 13 and E - 29.
+    const uint32_t lm = (uint32_t)(em - 127 - 13 + 1023), lv = (uint32_t)(ev - 127 - 29 + 1023);
+    const double wm = pow2(em - 127 - 13), wv = pow2(ev - 127 - 29);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        cm[j] = cv[j] = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int e = 4 * j + k;
+            const uint32_t hm = hi_word(m[e]);
+            uint32_t c = odd(hm) ? 0x7fu : encode(__builtin_fabs(m[e]), lm, wm, r[e] & 0x1ffff);
+            c |= (hm >> 31) << 7;
+            cm[j] |= c << (8 * k);
+            c = odd(hi_word(v[e])) ? 0xffu : encode(__builtin_fabs(v[e]), lv, wv, r[e] >> 15);
+            if (v[e] != 0.0) c = max(c, 1u);
+            cv[j] |= c << (8 * k);
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void adamw8_kernel(const Adamw8Args a) {
+    const Adamw8Tensor& t = find(a, blockIdx.x);
+    const long e0 = ((long)blockIdx.x - t.block0) * kBlock;
+    const float ob1 = 1.0f - a.beta1, ob2 = 1.0f - a.beta2;
+    if (!t.state8) {  // 32-bit states
+        const long e1 = min(e0 + kBlock, t.n);
+        for (long i = e0 + 4 * threadIdx.x; i < e1; i += 1024) {
+            float4 p = load4(t.p, i, t.n, t.vec), m = load4(t.m, i, t.n, t.vec), v = load4(t.v, i, t.n, t.vec);
+            const float4 g = load4(t.g, i, t.n, t.vec);
+            adamw_one(p.x, g.x, m.x, v.x, a.lr, a.beta1, a.beta2, ob1, ob2, a.eps, t.weight_decay, a.bc1, a.bc2);
+            adamw_one(p.y, g.y, m.y, v.y, a.lr, a.beta1, a.beta2, ob1, ob2, a.eps, t.weight_decay, a.bc1, a.bc2);
+            adamw_one(p.z, g.z, m.z, v.z, a.lr, a.beta1, a.beta2, ob1, ob2, a.eps, t.weight_decay, a.bc1, a.bc2);
+            adamw_one(p.w, g.w, m.w, v.w, a.lr, a.beta1, a.beta2, ob1, ob2, a.eps, t.weight_decay, a.bc1, a.bc2);
+            store4(t.p, i, t.n, t.vec, p);
+            store4(t.m, i, t.n, t.vec, m);
+            store4(t.v, i, t.n, t.vec, v);
+        }
+        return;
+    }
+    // 16 lanes to a block; of each run of 64 values a lane has four.
+    const long b = e0 / 256 + threadIdx.x / 16;
+    if (b * 256 >= t.n) return;  // (whole groups of 16 lanes)
+    const State8 s = state8(t.state8, t.n);
+    const long i0 = b * 256 + 4 * (threadIdx.x % 16);
+    uint32_t cm[4], cv[4];
+    float p[16], g[16];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        cm[j] = *reinterpret_cast<const uint32_t*>(s.m + i0 + 64 * j);
+        cv[j] = *reinterpret_cast<const uint32_t*>(s.v + i0 + 64 * j);
+        const float4 x = load4(t.p, i0 + 64 * j, t.n, t.vec), y = load4(t.g, i0 + 64 * j, t.n, t.vec);
+        p[4 * j] = x.x, p[4 * j + 1] = x.y, p[4 * j + 2] = x.z, p[4 * j + 3] = x.w;
+        g[4 * j] = y.x, g[4 * j + 1] = y.y, g[4 * j + 2] = y.z, g[4 * j + 3] = y.w;
+    }
+    const double um = pow2(s.em[b] + kUnitM), uv = pow2(s.ev[b] + kUnitV);
+    const double b1 = a.beta1, b2 = a.beta2, d1 = ob1, d2 = ob2;
+    double m[16], v[16];
+    uint32_t r[16];
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const uint32_t km = cm[e / 4] >> (8 * (e % 4)) & 0xff, kv = cv[e / 4] >> (8 * (e % 4)) & 0xff;
+        const double gd = g[e];
+        m[e] = fma(d1, gd, b1 * decode_m(km, um));
+        v[e] = fma(d2 * gd, gd, b2 * decode_v(kv, uv));
+        const float mf = (float)m[e], vf = (float)v[e];
+        const float upd = mf * a.c1 / (sqrtf(vf) * a.c2 + a.eps) + t.weight_decay * p[e];
+        p[e] -= a.lr * upd;
+        r[e] = mix((uint32_t)(i0 + 64 * (e / 4) + e % 4) + a.key);
+    }
+    int em, ev;
+    encode_block(m, v, r, cm, cv, em, ev);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        store4(t.p, i0 + 64 * j, t.n, t.vec, make_float4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]));
+        *reinterpret_cast<uint32_t*>(s.m + i0 + 64 * j) = cm[j];
+        *reinterpret_cast<uint32_t*>(s.v + i0 + 64 * j) = cv[j];
+    }
+    if (threadIdx.x % 16 == 0) {
+        s.em[b] = (uint8_t)em;
+        s.ev[b] = (uint8_t)ev;
+    }
+}
+
+// f32 moments into an 8-bit state, each to the nearest of its steps, and back.
+template <bool PACK>
+__global__ __launch_bounds__(256) void adamw8_convert_kernel(const Adamw8Args a) {
+    const Adamw8Tensor& t = find(a, blockIdx.x);
+    const long b = ((long)blockIdx.x - t.block0) * (kBlock / 256) + threadIdx.x / 16;
+    if (b * 256 >= t.n) return;
+    const State8 s = state8(t.state8, t.n);
+    const long i0 = b * 256 + 4 * (threadIdx.x % 16);
+    uint32_t cm[4], cv[4];
+    if constexpr (PACK) {
+        double m[16], v[16];
+        uint32_t r[16];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float4 x = load4(t.m, i0 + 64 * j, t.n, t.vec), y = load4(t.v, i0 + 64 * j, t.n, t.vec);
+            m[4 * j] = x.x, m[4 * j + 1] = x.y, m[4 * j + 2] = x.z, m[4 * j + 3] = x.w;
+            v[4 * j] = y.x, v[4 * j + 1] = y.y, v[4 * j + 2] = y.z, v[4 * j + 3] = y.w;
+#pragma unroll
+            for (int k = 0; k < 4; k++) r[4 * j + k] = 1u << 16 | 1u << 31;
+        }
+        int em, ev;
+        encode_block(m, v, r, cm, cv, em, ev);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            *reinterpret_cast<uint32_t*>(s.m + i0 + 64 * j) = cm[j];
+            *reinterpret_cast<uint32_t*>(s.v + i0 + 64 * j) = cv[j];
+        }
+        if (threadIdx.x % 16 == 0) {
+            s.em[b] = (uint8_t)em;
+            s.ev[b] = (uint8_t)ev;
+        }
+    } else {
+        const double um = pow2(s.em[b] + kUnitM), uv = pow2(s.ev[b] + kUnitV);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            cm[j] = *reinterpret_cast<const uint32_t*>(s.m + i0 + 64 * j);
+            cv[j] = *reinterpret_cast<const uint32_t*>(s.v + i0 + 64 * j);
+            float m[4], v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                m[k] = (float)decode_m(cm[j] >> (8 * k) & 0xff, um);
+                v[k] = (float)decode_v(cv[j] >> (8 * k) & 0xff, uv);
+            }
+            store4(t.m, i0 + 64 * j, t.n, t.vec, make_float4(m[0], m[1], m[2], m[3]));
+            store4(t.v, i0 + 64 * j, t.n, t.vec, make_float4(v[0], v[1], v[2], v[3]));
+        }
+    }
+}
+
+}  // namespace
+
+size_t adamw8_state_bytes(size_t n) { return (n + 255) / 256 * 514; }
+
+uint32_t adamw8_key(uint64_t t) {
+    auto mix32 = [](uint32_t x) {
+        x = (x ^ (x >> 16)) * 0xA511E9B3u;
+        x = (x ^ (x >> 15)) * 0x63D83595u;
+        return x ^ (x >> 16);
+    };
+    return mix32((uint32_t)t * 0x9E3779B1u + 0x7F4A7C15u);
+}
+
+hipError_t launch_adamw8(Adamw8Args a, Adamw8Op op, hipStream_t st) {
+    long blocks = 0;
+    for (int i = 0; i < a.count; i++) {
+        Adamw8Tensor& t = a.t[i];
+        const bool pg = op != Adamw8Op::kUpdate || (aligned16(t.p) && aligned16(t.g));
+        const bool mv = (op == Adamw8Op::kUpdate && t.state8) || (aligned16(t.m) && aligned16(t.v));
+        t.vec = pg && mv;
+        t.block0 = blocks;
+        blocks += (t.n + kBlock - 1) / kBlock;
+    }
+    if (blocks == 0) return hipSuccess;
+    if (blocks > 0xffffffL) return hipErrorInvalidConfiguration;  // fewer than 2^32 threads
+    const auto kernel = op == Adamw8Op::kUpdate ? adamw8_kernel
+                        : op == Adamw8Op::kPack ? adamw8_convert_kernel<true>
+                                                : adamw8_convert_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace cfattn

@@ -1,12 +1,13 @@
 // C ABI of the layer ops (declared in include/cfops.h).
 //
 // Host-side plumbing only: argument checks, scratch from the context's pool
-// and dispatch to the gfx950 kernels of gemm_f32.hip, lora.hip and
-// layer_ops.hip.  There is no CPU compute path.
+// and dispatch to the gfx950 kernels of gemm_f32.hip, lora.hip, layer_ops.hip,
+// head_logp.hip, seq_loss.hip and adamw8.hip.  There is no CPU compute path.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstddef>
 #include <cstdint>
 #include <cstring>
@@ -61,22 +62,19 @@ int gemm(cfattn_ctx* c, int kind, const float* a, const float* b, float* out, si
     return launch_gemm(c, g, st);
 }
 
-// Whether a buffer that one tensor's update writes shares memory with any of
-// another's (a parameter under two names, or beside a view of itself).
-bool adamw_overlaps(const cfattn::AdamwArgs& a) {
-    struct Range {
-        uintptr_t lo, hi;
-        bool written;
-    } r[4 * cfattn::kAdamwBatch];
-    int n = 0;
-    for (int i = 0; i < a.count; i++) {
-        const cfattn::AdamwTensor& t = a.t[i];
-        const float* const ptr[4] = {t.p, t.m, t.v, t.g};
-        for (int j = 0; j < 4; j++) {
-            const uintptr_t lo = reinterpret_cast<uintptr_t>(ptr[j]);
-            r[n++] = {lo, lo + (size_t)t.n * sizeof(float), j < 3};
-        }
-    }
+// Memory that one tensor's update reads or writes.
+struct Range {
+    uintptr_t lo, hi;
+    bool written;
+};
+Range range(const void* p, size_t bytes, bool written) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+    return {lo, lo + bytes, written};
+}
+
+// Whether one of the ranges that is written shares memory with any other (a
+// parameter under two names, or beside a view of itself).  Sorts them.
+bool overlaps(Range* r, int n) {
     std::sort(r, r + n, [](const Range& x, const Range& y) { return x.lo < y.lo; });
     uintptr_t end = 0, end_written = 0;
     for (int i = 0; i < n; i++) {
@@ -85,6 +83,37 @@ bool adamw_overlaps(const cfattn::AdamwArgs& a) {
         if (r[i].written) end_written = std::max(end_written, r[i].hi);
     }
     return false;
+}
+
+bool adamw_overlaps(const cfattn::AdamwArgs& a) {
+    Range r[4 * cfattn::kAdamwBatch];
+    int n = 0;
+    for (int i = 0; i < a.count; i++) {
+        const cfattn::AdamwTensor& t = a.t[i];
+        const float* const ptr[4] = {t.p, t.m, t.v, t.g};
+        for (int j = 0; j < 4; j++) r[n++] = range(ptr[j], (size_t)t.n * sizeof(float), j < 3);
+    }
+    return overlaps(r, n);
+}
+
+bool adamw8_overlaps(const cfattn::Adamw8Args& a, cfattn::Adamw8Op op) {
+    using cfattn::Adamw8Op;
+    Range r[4 * cfattn::kAdamw8Batch];
+    int n = 0;
+    for (int i = 0; i < a.count; i++) {
+        const cfattn::Adamw8Tensor& t = a.t[i];
+        const size_t bytes = (size_t)t.n * sizeof(float);
+        if (t.state8) r[n++] = range(t.state8, cfattn::adamw8_state_bytes((size_t)t.n), op != Adamw8Op::kUnpack);
+        if (op == Adamw8Op::kUpdate) {
+            r[n++] = range(t.p, bytes, true);
+            r[n++] = range(t.g, bytes, false);
+        }
+        if (op != Adamw8Op::kUpdate || !t.state8) {
+            r[n++] = range(t.m, bytes, op != Adamw8Op::kPack);
+            r[n++] = range(t.v, bytes, op != Adamw8Op::kPack);
+        }
+    }
+    return overlaps(r, n);
 }
 
 int check_linears(cfattn_ctx* c, size_t t, size_t in, const cfops_linear* lin, size_t n) {
@@ -463,6 +492,213 @@ int cfops_adamw_update_multi(cfattn_ctx* c, size_t count, float* const* p, const
         }
     }
     return CFATTN_OK;
+}
+
+// ---------------------------------------- preference and policy training
+
+namespace {
+
+int check_logprobs(cfattn_ctx* c, size_t t, size_t d, size_t vocab) {
+    if (d == 0 || vocab == 0) return fail(c, CFATTN_ERR_ARG, "d and vocab must be positive");
+    // (A launch with a workgroup of 256 threads to each row has fewer than 2^32.)
+    if (t >= (size_t)1 << 24 || !fits_int(d) || !fits_int(vocab))
+        return fail(c, CFATTN_ERR_UNSUPPORTED, "t=%zu not below 2^24, or d=%zu, vocab=%zu above 2^31", t, d, vocab);
+    return CFATTN_OK;
+}
+
+// Scratch of the log-probabilities: the scored rows, their hidden states (in the
+// backward over them their gradients), and the logits of a chunk of them.
+struct LogpRows {
+    int *idx, *count;
+    float *hn, *logits;
+    size_t chunk;
+};
+int logp_rows(cfattn_ctx* c, size_t t, size_t d, size_t vocab, LogpRows& r) {
+    // A chunk's logits fit the head's limit, its rows a launch of workgroups.
+    r.chunk = std::min<size_t>(c->head_chunk_bytes / (vocab * sizeof(float)), (size_t)1 << 22);
+    r.chunk = std::min(std::max<size_t>(r.chunk, 1), t);
+    int rc = CFATTN_OK;
+    if (!(r.count = static_cast<int*>(slot(c, cfattn_ctx::OPS_IDX, (t + 4) * sizeof(int), &rc)))) return rc;
+    r.idx = r.count + 4;
+    if (!(r.hn = static_cast<float*>(slot(c, cfattn_ctx::OPS_ROWS, t * d * sizeof(float), &rc)))) return rc;
+    r.logits = static_cast<float*>(slot(c, cfattn_ctx::OPS_LOGITS, r.chunk * vocab * sizeof(float), &rc));
+    return r.logits ? CFATTN_OK : rc;
+}
+
+int check_sequences(cfattn_ctx* c, size_t rows, size_t seqs) {
+    // (A launch has fewer than 2^32 threads, a workgroup to each sequence or pair.)
+    if (!fits_int(rows) || seqs > (size_t)1 << 22)
+        return fail(c, CFATTN_ERR_UNSUPPORTED, "rows=%zu above 2^31 or sequences=%zu above 2^22", rows, seqs);
+    return CFATTN_OK;
+}
+
+int adamw8_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors, cfattn::Adamw8Op op,
+                 cfattn::Adamw8Args& a, hipStream_t st) {
+    using cfattn::Adamw8Op;
+    if (count && !tensors) return fail(c, CFATTN_ERR_ARG, "null array");
+    for (size_t i = 0; i < count; i++) {
+        const cfops_adamw_tensor& x = tensors[i];
+        if (x.n == 0 || (op != Adamw8Op::kUpdate && !x.state8)) continue;
+        if ((op == Adamw8Op::kUpdate && (!x.p || !x.g)) ||
+            ((op != Adamw8Op::kUpdate || !x.state8) && (!x.m || !x.v)))
+            return fail(c, CFATTN_ERR_ARG, "null buffer");
+        if (reinterpret_cast<uintptr_t>(x.state8) % 16)
+            return fail(c, CFATTN_ERR_ARG, "state8 must be 16-byte aligned");
+    }
+    a.count = 0;
+    for (size_t i = 0; i < count; i++) {
+        const cfops_adamw_tensor& x = tensors[i];
+        if (x.n && (op == Adamw8Op::kUpdate || x.state8))
+            a.t[a.count++] = {x.p, x.g, x.m, x.v, x.state8, (long)x.n, x.weight_decay, 0, 0};
+        if (a.count == cfattn::kAdamw8Batch || (i + 1 == count && a.count)) {
+            // Tensors of one launch are updated side by side.
+            const int step = adamw8_overlaps(a, op) ? 1 : a.count;
+            for (int k = 0; k < a.count; k += step) {
+                cfattn::Adamw8Args b = a;
+                std::copy(a.t + k, a.t + k + step, b.t);
+                b.count = step;
+                CF_HIP(c, cfattn::launch_adamw8(b, op, st), "adamw launch");
+            }
+            a.count = 0;
+        }
+    }
+    return CFATTN_OK;
+}
+
+}  // namespace
+
+int cfops_lm_head_logprobs(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets, size_t t,
+                           size_t d, size_t vocab, float* logp, float* lse, cfops_ce_result* result, void* stream) {
+    CF_LOCK(c, stream);
+    if (!result) return fail(c, CFATTN_ERR_ARG, "null result");
+    CF_TRY(check_logprobs(c, t, d, vocab));
+    if (!head || (t && (!hn || !targets || !logp || !lse))) return fail(c, CFATTN_ERR_ARG, "null buffer");
+    const hipStream_t st = to_stream(stream);
+    LogpRows rows{};
+    CF_TRY(logp_rows(c, t, d, vocab, rows));
+    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, logp, lse, result, st),
+           "log-probability launch");
+    if (t == 0) return CFATTN_OK;
+    CF_HIP(c, cfattn::launch_logp_gather(hn, rows.idx, rows.count, rows.hn, t, d, st), "log-probability launch");
+    for (size_t j0 = 0; j0 < t; j0 += rows.chunk) {
+        const size_t nr = std::min(t - j0, rows.chunk);
+        CF_TRY(gemm(c, CFOPS_NT, rows.hn + j0 * d, head, rows.logits, nr, d, vocab, false, st));
+        CF_HIP(c, cfattn::launch_logp_rows(rows.logits, targets, rows.idx, rows.count, logp, lse, j0, nr, vocab, st),
+               "log-probability launch");
+    }
+    CF_HIP(c, cfattn::launch_logp_finish(targets, logp, t, result, st), "log-probability launch");
+    return CFATTN_OK;
+}
+
+int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets,
+                                    const float* lse, const float* dlogp, size_t t, size_t d, size_t vocab,
+                                    float* dhn, float* dhead, void* stream) {
+    CF_LOCK(c, stream);
+    CF_TRY(check_logprobs(c, t, d, vocab));
+    if (t == 0 || (!dhn && !dhead)) return CFATTN_OK;
+    if (!hn || !head || !targets || !lse || !dlogp) return fail(c, CFATTN_ERR_ARG, "null buffer");
+    const hipStream_t st = to_stream(stream);
+    LogpRows rows{};
+    CF_TRY(logp_rows(c, t, d, vocab, rows));
+    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, nullptr, nullptr, nullptr, st),
+           "log-probability launch");
+    CF_HIP(c, cfattn::launch_logp_gather(hn, rows.idx, rows.count, rows.hn, t, d, st), "log-probability launch");
+    for (size_t j0 = 0; j0 < t; j0 += rows.chunk) {
+        const size_t nr = std::min(t - j0, rows.chunk);
+        float* h = rows.hn + j0 * d;
+        CF_TRY(gemm(c, CFOPS_NT, h, head, rows.logits, nr, d, vocab, false, st));
+        CF_HIP(c, cfattn::launch_logp_grad_rows(rows.logits, targets, rows.idx, rows.count, lse, dlogp, j0, nr, vocab,
+                                                st),
+               "log-probability launch");
+        if (dhead) CF_TRY(gemm(c, CFOPS_TN, rows.logits, h, dhead, vocab, nr, d, true, st));
+        if (dhn) CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, h, nr, vocab, d, false, st));
+    }
+    if (dhn)
+        CF_HIP(c, cfattn::launch_logp_scatter(rows.hn, rows.idx, rows.count, dhn, t, d, st), "log-probability launch");
+    return CFATTN_OK;
+}
+
+static_assert(sizeof(cfops_preference_result) == sizeof(cfattn::PreferenceResult) &&
+                  sizeof(cfops_policy_result) == sizeof(cfattn::PolicyResult) &&
+                  offsetof(cfops_policy_result, clipped) == offsetof(cfattn::PolicyResult, clipped),
+              "the results are the kernels' blocks");
+
+int cfops_preference_loss(cfattn_ctx* c, const float* logp, const float* ref_logp, const int64_t* targets,
+                          size_t rows, const int64_t* offsets, size_t pairs, int form, double beta, double margin,
+                          double label_smoothing, int length_mean, float* dlogp, float* rewards,
+                          cfops_preference_result* result, void* stream) {
+    CF_LOCK(c, stream);
+    if (pairs == 0) return fail(c, CFATTN_ERR_ARG, "pairs must be positive");
+    if (!offsets || !result || (rows && (!logp || !dlogp)) || !rewards) return fail(c, CFATTN_ERR_ARG, "null buffer");
+    if (form != CFOPS_PREFERENCE_SIGMOID && form != CFOPS_PREFERENCE_HINGE && form != CFOPS_PREFERENCE_SQUARED)
+        return fail(c, CFATTN_ERR_ARG, "unknown preference form %d", form);
+    if (!(label_smoothing >= 0.0 && label_smoothing < 1.0) ||
+        (form != CFOPS_PREFERENCE_SIGMOID && label_smoothing != 0.0))
+        return fail(c, CFATTN_ERR_ARG, "label_smoothing must be in [0, 1), and 0 for the hinge and squared forms");
+    CF_TRY(check_sequences(c, rows, pairs));
+    int rc = CFATTN_OK;
+    void* scratch = slot(c, cfattn_ctx::OPS_SEQ, cfattn::preference_scratch_bytes(pairs), &rc);
+    if (!scratch) return rc;
+    cfattn::PreferenceArgs a{};
+    a.logp = logp, a.ref_logp = ref_logp, a.targets = targets, a.offsets = offsets, a.rows = (long)rows;
+    a.pairs = (long)pairs, a.form = form, a.length_mean = length_mean != 0, a.beta = beta, a.margin = margin;
+    a.label_smoothing = label_smoothing, a.dlogp = dlogp, a.rewards = rewards;
+    a.result = reinterpret_cast<cfattn::PreferenceResult*>(result);
+    CF_HIP(c, cfattn::launch_preference(a, scratch, to_stream(stream)), "preference loss launch");
+    return CFATTN_OK;
+}
+
+int cfops_policy_loss(cfattn_ctx* c, const float* logp, const float* old_logp, const float* ref_logp,
+                      const float* advantages, const int64_t* targets, size_t rows, const int64_t* offsets,
+                      size_t seqs, int per_token, double clip_low, double clip_high, double kl_coef, int reduction,
+                      float* dlogp, cfops_policy_result* result, void* stream) {
+    CF_LOCK(c, stream);
+    if (seqs == 0) return fail(c, CFATTN_ERR_ARG, "sequences must be positive");
+    if (!offsets || !result || (rows && (!logp || !dlogp)) || ((rows || !per_token) && !advantages))
+        return fail(c, CFATTN_ERR_ARG, "null buffer");
+    if (!(clip_low >= 0.0 && clip_low <= 1.0 && clip_high >= 0.0))
+        return fail(c, CFATTN_ERR_ARG, "clip_low must be in [0, 1] and clip_high not negative");
+    if (reduction != CFOPS_POLICY_TOKEN_MEAN && reduction != CFOPS_POLICY_SEQUENCE_MEAN)
+        return fail(c, CFATTN_ERR_ARG, "unknown reduction %d", reduction);
+    CF_TRY(check_sequences(c, rows, seqs));
+    int rc = CFATTN_OK;
+    void* scratch = slot(c, cfattn_ctx::OPS_SEQ, cfattn::policy_scratch_bytes(seqs), &rc);
+    if (!scratch) return rc;
+    cfattn::PolicyArgs a{};
+    a.logp = logp, a.old_logp = old_logp, a.ref_logp = ref_logp, a.advantages = advantages, a.targets = targets;
+    a.offsets = offsets, a.rows = (long)rows, a.seqs = (long)seqs, a.per_token = per_token != 0;
+    a.sequence_mean = reduction == CFOPS_POLICY_SEQUENCE_MEAN, a.low = 1.0 - clip_low, a.high = 1.0 + clip_high;
+    a.log_low = std::log1p(-clip_low), a.log_high = std::log1p(clip_high), a.kl_coef = kl_coef, a.dlogp = dlogp;
+    a.result = reinterpret_cast<cfattn::PolicyResult*>(result);
+    CF_HIP(c, cfattn::launch_policy(a, scratch, to_stream(stream)), "policy loss launch");
+    return CFATTN_OK;
+}
+
+size_t cfops_adamw8_state_bytes(size_t n) { return cfattn::adamw8_state_bytes(n); }
+
+int cfops_adamw8_update_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors, uint64_t t, float lr,
+                              float beta1, float beta2, float eps, void* stream) {
+    CF_LOCK(c, stream);
+    cfattn::Adamw8Args a{};
+    a.lr = lr, a.beta1 = beta1, a.beta2 = beta2, a.eps = eps;
+    a.bc1 = 1.0f - powi_f32(beta1, (int)(int32_t)t);
+    a.bc2 = 1.0f - powi_f32(beta2, (int)(int32_t)t);
+    a.c1 = (float)(1.0 / (1.0 - std::pow((double)beta1, (double)t)));
+    a.c2 = (float)(1.0 / std::sqrt(1.0 - std::pow((double)beta2, (double)t)));
+    a.key = cfattn::adamw8_key(t);
+    return adamw8_multi(c, count, tensors, cfattn::Adamw8Op::kUpdate, a, to_stream(stream));
+}
+
+int cfops_adamw8_pack_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors, void* stream) {
+    CF_LOCK(c, stream);
+    cfattn::Adamw8Args a{};
+    return adamw8_multi(c, count, tensors, cfattn::Adamw8Op::kPack, a, to_stream(stream));
+}
+
+int cfops_adamw8_unpack_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors, void* stream) {
+    CF_LOCK(c, stream);
+    cfattn::Adamw8Args a{};
+    return adamw8_multi(c, count, tensors, cfattn::Adamw8Op::kUnpack, a, to_stream(stream));
 }
 
 }  // extern "C"

@@ -114,4 +114,89 @@ struct LoraGrad {
 size_t lora_grad_plan(LoraGrad& g);
 hipError_t launch_lora_grad(const LoraGrad& g, hipStream_t st);
 
+// AdamW over tensors whose moments are held in 8 bits (state8) or 32 (m, v)
+// (adamw8.hip); none empty.  Update reads and writes p and the state; pack and
+// unpack convert between m, v and state8.
+constexpr int kAdamw8Batch = 60;
+struct Adamw8Tensor {
+    float* p;
+    const float* g;
+    float *m, *v;
+    uint8_t* state8;
+    long n;
+    float weight_decay;
+    int vec;      // set by launch_adamw8, as block0
+    long block0;
+};
+struct Adamw8Args {
+    Adamw8Tensor t[kAdamw8Batch];
+    int count;
+    float lr, beta1, beta2, eps, bc1, bc2;  // 32-bit states, as AdamwArgs
+    float c1, c2;                           // 1 / bc1, 1 / sqrt(bc2)
+    uint32_t key;                           // adamw8_key(t)
+};
+enum class Adamw8Op { kUpdate, kPack, kUnpack };
+size_t adamw8_state_bytes(size_t n);
+uint32_t adamw8_key(uint64_t t);
+hipError_t launch_adamw8(Adamw8Args a, Adamw8Op op, hipStream_t st);
+
+// Losses over packed sequences (seq_loss.hip); at least one pair or sequence.
+struct PreferenceResult {
+    int bad_seq;  // first sequence whose offsets do not rise within the rows, or INT_MAX
+    float loss, accuracy, margin;
+};
+struct PreferenceArgs {
+    const float *logp, *ref_logp;  // ref_logp may be null
+    const int64_t *targets, *offsets;  // targets may be null: every row is scored
+    long rows, pairs;
+    int form, length_mean;
+    double beta, margin, label_smoothing;
+    float *dlogp, *rewards;
+    PreferenceResult* result;
+    double* terms;  // set by launch_preference
+};
+size_t preference_scratch_bytes(size_t pairs);
+hipError_t launch_preference(PreferenceArgs a, void* scratch, hipStream_t st);
+
+struct PolicyResult {
+    int n_scored, bad_seq;
+    float loss, kl, clipped;
+};
+struct PolicyArgs {
+    const float *logp, *old_logp, *ref_logp, *advantages;  // old_logp, ref_logp may be null
+    const int64_t *targets, *offsets;
+    long rows, seqs;
+    int per_token, sequence_mean;
+    double low, high, log_low, log_high, kl_coef;  // the ratio's borders and their logarithms
+    float* dlogp;
+    PolicyResult* result;
+    double* terms;  // set by launch_policy, as counts
+    int* counts;
+};
+size_t policy_scratch_bytes(size_t seqs);
+hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st);
+
+// Log-probabilities of the targets (head_logp.hip).  Rows whose target is within
+// the vocabulary are scored; `idx` and `count` (device memory) name them in
+// order, and the kernels below work on scored rows [j0, j0 + nrows), of which
+// `logits` holds the logits; those at or past *count are zeros in what they
+// write, or not written.  The other arrays are indexed by row.
+//   select:    idx and count, the result block (CeMisc; or null), and logp and
+//              lse (or null) of the rows that are not scored;
+//   gather:    the scored rows of hn side by side;   scatter: back, other rows 0;
+//   rows:      logp and lse;   grad_rows: the logits become their gradients;
+//   finish:    the mean of -logp, summed in f64 in row order.
+hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, float* logp,
+                              float* lse, void* misc, hipStream_t st);
+hipError_t launch_logp_gather(const float* hn, const int* idx, const int* count, float* out, size_t rows, size_t d,
+                              hipStream_t st);
+hipError_t launch_logp_scatter(const float* in, const int* idx, const int* count, float* dhn, size_t rows, size_t d,
+                               hipStream_t st);
+hipError_t launch_logp_rows(const float* logits, const int64_t* targets, const int* idx, const int* count, float* logp,
+                            float* lse, size_t j0, size_t nrows, size_t vocab, hipStream_t st);
+hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const int* idx, const int* count,
+                                 const float* lse, const float* dlogp, size_t j0, size_t nrows, size_t vocab,
+                                 hipStream_t st);
+hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t rows, void* misc, hipStream_t st);
+
 }  // namespace cfattn

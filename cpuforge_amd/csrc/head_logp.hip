@@ -1,0 +1,199 @@
+// Log-probabilities of the targets under logits = hn . head^T, and their
+// gradient (cfops_lm_head_logprobs of include/cfops.h), over rows of logits:
+//   lse = log sum_v exp(x_v),  logp = x_target - lse,
+//   d x_v = dlogp ((v == target) - exp(x_v - lse)).
+#include <limits.h>
+
+#include "cfattn_common.hpp"
+#include "cfops_kernels.hpp"
+
+namespace cfattn {
+namespace {
+
+constexpr long kIgnoreIndex = -100;  // crates/core/src/ops/loss.rs:4
+
+// A running maximum and the sum of exp(x - maximum).
+struct MaxSum {
+    float m, s;
+};
+__device__ __forceinline__ MaxSum merge(const MaxSum& a, const MaxSum& b) {
+    const float m = fmaxf(a.m, b.m);
+    // (An empty side has m = -inf and s = 0.)
+    const float sa = a.s == 0.0f ? 0.0f : a.s * expf(a.m - m), sb = b.s == 0.0f ? 0.0f : b.s * expf(b.m - m);
+    return {m, sa + sb};
+}
+
+// The scored rows (targets within the vocabulary): idx[0..n) in row order, n
+// at *count; the result's counts; logp and lse of the other rows, 0 where the
+// target is ignored and NaN where it is out of range.  One workgroup: 1024
+// targets a round, their places from a scan.
+__global__ __launch_bounds__(1024) void logp_select_kernel(const int64_t* __restrict__ targets, long rows, long vocab,
+                                                           int* __restrict__ idx, int* __restrict__ count,
+                                                           float* __restrict__ logp, float* __restrict__ lse,
+                                                           CeMisc* __restrict__ misc) {
+    __shared__ int wave_n[16], bad_row;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x == 0) bad_row = INT_MAX;
+    __syncthreads();
+    int n = 0, ignored = 0;
+    for (long r0 = 0; r0 < rows; r0 += 1024) {
+        const long r = r0 + threadIdx.x;
+        const int64_t t = r < rows ? targets[r] : kIgnoreIndex;
+        const bool scored = t >= 0 && t < vocab;
+        if (r < rows && !scored) {
+            ignored += t == kIgnoreIndex;
+            if (t != kIgnoreIndex) atomicMin(&bad_row, (int)r);
+            if (logp) logp[r] = lse[r] = t == kIgnoreIndex ? 0.0f : __builtin_nanf("");
+        }
+        const unsigned long long m = __ballot(scored);
+        if (lane == 0) wave_n[wave] = __popcll(m);
+        __syncthreads();
+        int at = n;
+        for (int w = 0; w < 16; w++) {
+            at += w < wave ? wave_n[w] : 0;
+            n += wave_n[w];
+        }
+        if (scored) idx[at + __popcll(m & ((1ull << lane) - 1))] = (int)r;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) ignored += __shfl_xor(ignored, o);
+    if (lane == 0) wave_n[wave] = ignored;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        *count = n;
+        if (misc) {
+            int all = 0;
+            for (int w = 0; w < 16; w++) all += wave_n[w];
+            *misc = {(int)(rows - all), bad_row, 0.0f};
+        }
+    }
+}
+
+// out[j] = hn[idx[j]], zeros from row n on.
+__global__ __launch_bounds__(256) void logp_gather_kernel(const float* __restrict__ hn, const int* __restrict__ idx,
+                                                          const int* __restrict__ count, float* __restrict__ out,
+                                                          long d) {
+    const long j = blockIdx.x;
+    const float* x = j < *count ? hn + (long)idx[j] * d : nullptr;
+    for (long i = threadIdx.x; i < d; i += 256) out[j * d + i] = x ? x[i] : 0.0f;
+}
+
+// dhn[idx[j]] = in[j] for j < n, the other rows zeros.
+__global__ __launch_bounds__(256) void logp_scatter_kernel(const float* __restrict__ in, const int* __restrict__ idx,
+                                                           const int* __restrict__ count, float* __restrict__ dhn,
+                                                           long d) {
+    // The place of row blockIdx.x among the ascending idx.
+    const int r = blockIdx.x, n = *count;
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (idx[mid] < r)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    const float* x = lo < n && idx[lo] == r ? in + (long)lo * d : nullptr;
+    for (long i = threadIdx.x; i < d; i += 256) dhn[r * d + i] = x ? x[i] : 0.0f;
+}
+
+// One scored row to a workgroup: `logits` holds those of scored rows [j0, ..).
+__global__ __launch_bounds__(512) void logp_rows_kernel(const float* __restrict__ logits,
+                                                        const int64_t* __restrict__ targets,
+                                                        const int* __restrict__ idx, const int* __restrict__ count,
+                                                        float* __restrict__ logp, float* __restrict__ lse, int j0,
+                                                        long vocab) {
+    __shared__ MaxSum red[8];
+    const int j = j0 + blockIdx.x;
+    if (j >= *count) return;
+    const long r = idx[j], t = targets[r];
+    const float* x = logits + (long)blockIdx.x * vocab;
+    float m = -INFINITY;
+    for (long i = threadIdx.x; i < vocab; i += 512) m = fmaxf(m, x[i]);
+    float s = 0.0f;
+    for (long i = threadIdx.x; i < vocab; i += 512) s += expf(x[i] - m);
+    MaxSum a{m, s};
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) a = merge(a, {__shfl_xor(a.m, o), __shfl_xor(a.s, o)});
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 8; i++) a = merge(a, red[i]);
+        const float l = a.m + logf(a.s);
+        lse[r] = l;
+        logp[r] = x[t] - l;
+    }
+}
+
+// dlogits over the logits of scored rows [j0, ..); zeros from row n on.
+__global__ __launch_bounds__(512) void logp_grad_rows_kernel(float* __restrict__ logits,
+                                                             const int64_t* __restrict__ targets,
+                                                             const int* __restrict__ idx,
+                                                             const int* __restrict__ count,
+                                                             const float* __restrict__ lse,
+                                                             const float* __restrict__ dlogp, int j0, long vocab) {
+    const int j = j0 + blockIdx.x;
+    const bool scored = j < *count;
+    const long r = scored ? idx[j] : 0, t = scored ? targets[r] : -1;
+    float* x = logits + (long)blockIdx.x * vocab;
+    const float g = scored ? dlogp[r] : 0.0f, l = scored ? lse[r] : 0.0f;
+    for (long i = threadIdx.x; i < vocab; i += 512)
+        x[i] = !scored ? 0.0f : i == t ? -g * expm1f(x[i] - l) : -g * expf(x[i] - l);
+}
+
+// The mean of -logp over the scored rows, summed in f64 in a fixed order.
+__global__ __launch_bounds__(256) void logp_finish_kernel(const int64_t* __restrict__ targets,
+                                                          const float* __restrict__ logp, long rows,
+                                                          CeMisc* __restrict__ m) {
+    __shared__ double sp[256];
+    double s = 0.0;
+    for (long r = threadIdx.x; r < rows; r += 256)
+        if (targets[r] != kIgnoreIndex) s -= (double)logp[r];
+    sp[threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double tot = 0.0;
+        for (int i = 0; i < 256; i++) tot += sp[i];
+        const int n = m->n_valid;
+        m->loss = n > 0 ? (float)(tot / (double)n) : 0.0f;
+    }
+}
+
+}  // namespace
+
+hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, float* logp,
+                              float* lse, void* misc, hipStream_t st) {
+    hipLaunchKernelGGL(logp_select_kernel, dim3(1), dim3(1024), 0, st, targets, (long)rows, (long)vocab, idx, count,
+                       logp, lse, static_cast<CeMisc*>(misc));
+    return hipGetLastError();
+}
+hipError_t launch_logp_gather(const float* hn, const int* idx, const int* count, float* out, size_t rows, size_t d,
+                              hipStream_t st) {
+    hipLaunchKernelGGL(logp_gather_kernel, dim3((unsigned)rows), dim3(256), 0, st, hn, idx, count, out, (long)d);
+    return hipGetLastError();
+}
+hipError_t launch_logp_scatter(const float* in, const int* idx, const int* count, float* dhn, size_t rows, size_t d,
+                               hipStream_t st) {
+    hipLaunchKernelGGL(logp_scatter_kernel, dim3((unsigned)rows), dim3(256), 0, st, in, idx, count, dhn, (long)d);
+    return hipGetLastError();
+}
+hipError_t launch_logp_rows(const float* logits, const int64_t* targets, const int* idx, const int* count, float* logp,
+                            float* lse, size_t j0, size_t nrows, size_t vocab, hipStream_t st) {
+    hipLaunchKernelGGL(logp_rows_kernel, dim3((unsigned)nrows), dim3(512), 0, st, logits, targets, idx, count, logp,
+                       lse, (int)j0, (long)vocab);
+    return hipGetLastError();
+}
+hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const int* idx, const int* count,
+                                 const float* lse, const float* dlogp, size_t j0, size_t nrows, size_t vocab,
+                                 hipStream_t st) {
+    hipLaunchKernelGGL(logp_grad_rows_kernel, dim3((unsigned)nrows), dim3(512), 0, st, logits, targets, idx, count,
+                       lse, dlogp, (int)j0, (long)vocab);
+    return hipGetLastError();
+}
+hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t rows, void* misc, hipStream_t st) {
+    hipLaunchKernelGGL(logp_finish_kernel, dim3(1), dim3(256), 0, st, targets, logp, (long)rows,
+                       static_cast<CeMisc*>(misc));
+    return hipGetLastError();
+}
+
+}  // namespace cfattn

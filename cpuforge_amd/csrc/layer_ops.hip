@@ -13,6 +13,7 @@
 
 #include <algorithm>
 
+#include "adamw_math.hpp"
 #include "cfattn_common.hpp"
 #include "cfops_kernels.hpp"
 
@@ -705,19 +706,6 @@ hipError_t launch_ce_finish(const int64_t* targets, const float* row_loss, size_
 }
 
 // ------------------------------------------------------------------- AdamW
-// optim.rs:21-29 with every product and sum rounded on its own:
-//   m = b1*m + (1-b1)*g,  v = b2*v + ((1-b2)*g)*g,
-//   p -= lr * ((m/bc1) / (sqrt(v/bc2) + eps) + wd*p).
-__device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v, float lr, float b1, float b2, float ob1,
-                                          float ob2, float eps, float wd, float bc1, float bc2) {
-    m = radd(rmul(b1, m), rmul(ob1, g));
-    v = radd(rmul(b2, v), rmul(rmul(ob2, g), g));
-    const float mhat = rdiv(m, bc1);
-    const float vhat = rdiv(v, bc2);
-    const float upd = radd(rdiv(mhat, radd(rsqrt_cr(vhat), eps)), rmul(wd, p));
-    p = rsub(p, rmul(lr, upd));
-}
-
 // Up to kAdamwBatch tensors in one launch: a block updates kAdamwBlock elements
 // of the tensor it falls in (AdamwTensor::block0 counts blocks).  HBM-bound (28
 // bytes an element, 6.8 TB/s on 16.8M elements); a model's adapters are small

@@ -15,12 +15,19 @@ the holder of device memory and the current HIP stream:
     adamw_update                        crates/train/src/optim.rs:9-30
       (adamw_update_multi: many tensors, optim.rs:48-61)
 
+Training on preferences and rewards has no reference counterpart:
+
+    lm_head_logprobs(_backward)         the targets' log-probabilities
+    preference_loss, policy_loss        losses over them, with their gradients
+    adamw8_update_multi                 AdamW with its moments in 8 bits
+
 Misuse the reference would panic on raises `ShapeError` (an AssertionError);
 library failures raise `CfattnError`.
 """
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
@@ -277,3 +284,198 @@ def adamw_update_multi(ps, gs, ms, vs, t, lr, beta1, beta2, eps, weight_decays, 
         arrs.append((C.c_void_p * k)(*[x.data_ptr() for x in ts]))
     _call(ctx, "cfops_adamw_update_multi", k, *arrs, (C.c_size_t * k)(*sizes), (C.c_float * k)(*weight_decays),
           int(t), float(lr), float(beta1), float(beta2), float(eps), _stream())
+
+
+# ---------------------------------- log-probabilities through the LM head
+def _result(t: torch.Tensor, words: int) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int32 or t.numel() < words \
+            or not t.is_contiguous():
+        raise TypeError(f"result must be a contiguous int32 device tensor of {words} words")
+    return t.data_ptr()
+
+
+def lm_head_logprobs(hn, head, targets, t, d, vocab, logp, lse, result, ctx: Context | None = None) -> None:
+    """logits = hn . head^T (never held whole); lse [t] is their log-sum-exp and
+    logp [t] the targets' logits less it, both 0 where the target is
+    IGNORE_INDEX (all overwritten).  `result` (ce_result_buffer) gets the mean
+    of -logp (ce_result_loss) and the first row whose target is out of range,
+    which ce_check reports; such a row's logp is NaN.  No host wait."""
+    ctx = ctx or default_context()
+    _call(ctx, "cfops_lm_head_logprobs", _f32(hn, "hn", t * d), _f32(head, "head", vocab * d), _targets(targets, t),
+          t, d, vocab, _f32(logp, "logp", t), _f32(lse, "lse", t), _result(result, CE_RESULT_WORDS), _stream())
+
+
+def lm_head_logprobs_backward(hn, head, targets, lse, dlogp, t, d, vocab, dhn=None, dhead=None,
+                              ctx: Context | None = None) -> None:
+    """From the gradient dlogp of logp and the forward's lse: dhn (overwritten)
+    and dhead += dlogits^T . hn, each when given.  The logits are formed again."""
+    ctx = ctx or default_context()
+    _call(ctx, "cfops_lm_head_logprobs_backward", _f32(hn, "hn", t * d), _f32(head, "head", vocab * d),
+          _targets(targets, t), _f32(lse, "lse", t), _f32(dlogp, "dlogp", t), t, d, vocab, _opt(dhn, "dhn", t * d),
+          _opt(dhead, "dhead", vocab * d), _stream())
+
+
+# ------------------------------------------- losses over packed sequences
+PREFERENCE_FORMS = {"sigmoid": 0, "hinge": 1, "squared": 2}
+POLICY_REDUCTIONS = {"token": 0, "sequence": 1}
+PREFERENCE_RESULT_WORDS, POLICY_RESULT_WORDS = 4, 5
+
+
+class PreferenceResult(NamedTuple):
+    """Views of a cfops_preference_result block, 0-d device tensors."""
+    loss: torch.Tensor
+    accuracy: torch.Tensor
+    margin: torch.Tensor
+
+
+class PolicyResult(NamedTuple):
+    """Views of a cfops_policy_result block, 0-d device tensors."""
+    loss: torch.Tensor
+    kl: torch.Tensor
+    clipped: torch.Tensor
+    n_scored: torch.Tensor
+
+
+def preference_result(result: torch.Tensor) -> PreferenceResult:
+    return PreferenceResult(*result.view(torch.float32)[1:4].unbind())
+
+
+def policy_result(result: torch.Tensor) -> PolicyResult:
+    return PolicyResult(*result.view(torch.float32)[2:5].unbind(), result[0])
+
+
+def _bad_seq(bad: int) -> None:
+    if bad != _NO_BAD_ROW:
+        raise _lib.CfattnError(_lib.ERR_ARG, f"offsets of sequence {bad} do not rise within the rows")
+
+
+def preference_check(result: torch.Tensor) -> None:
+    """Waits for `result` and raises where a sequence's offsets do not rise
+    within the rows."""
+    _bad_seq(int(result[0].item()))
+
+
+def policy_check(result: torch.Tensor) -> None:
+    _bad_seq(int(result[1].item()))
+
+
+def _offsets(t: torch.Tensor) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int64 or not t.is_contiguous():
+        raise TypeError("offsets must be a contiguous int64 device tensor")
+    return t.data_ptr()
+
+
+def preference_loss(logp, ref_logp, targets, offsets, dlogp, rewards, result, *, beta: float, form: str = "sigmoid",
+                    margin: float = 0.0, label_smoothing: float = 0.0, length_mean: bool = False,
+                    ctx: Context | None = None) -> None:
+    """The mean loss of pairs of sequences and its gradient dlogp.  Sequence i
+    is rows [offsets[i], offsets[i + 1]) of logp; 2j is the chosen and 2j + 1
+    the rejected one of pair j.  A reward is beta times the sum (length_mean:
+    the mean) of logp - ref_logp over a sequence's scored rows, those whose
+    target is not IGNORE_INDEX (targets None: all; ref_logp None: of logp).
+    With z = chosen - rejected reward - margin:
+        "sigmoid"  -(1 - s) log sigmoid(z) - s log sigmoid(-z), s = label_smoothing
+        "hinge"    max(0, 1 - z)
+        "squared"  (z - 1/2)^2
+    rewards [2 * pairs] and `result` (at least PREFERENCE_RESULT_WORDS int32; see
+    preference_result, preference_check) are overwritten, and dlogp in the rows
+    of sequences.  No host wait."""
+    ctx = ctx or default_context()
+    rows, entries = logp.numel(), offsets.numel()
+    if entries % 2 == 0:
+        raise _lib.ShapeError(_lib.ERR_SHAPE, f"offsets of pairs have an odd number of entries, got {entries}")
+    if form not in PREFERENCE_FORMS:
+        raise ValueError(f"unknown preference form {form!r}")
+    tp = None if targets is None else _targets(targets, rows)
+    _call(ctx, "cfops_preference_loss", _f32(logp, "logp"), _opt(ref_logp, "ref_logp", rows), tp, rows,
+          _offsets(offsets), entries // 2, PREFERENCE_FORMS[form], float(beta), float(margin), float(label_smoothing),
+          int(length_mean), _f32(dlogp, "dlogp", rows), _f32(rewards, "rewards", entries - 1),
+          _result(result, PREFERENCE_RESULT_WORDS), _stream())
+
+
+def policy_loss(logp, old_logp, ref_logp, advantages, targets, offsets, dlogp, result, *, clip_low: float,
+                clip_high: float, kl_coef: float = 0.0, reduction: str = "token", per_token: bool | None = None,
+                ctx: Context | None = None) -> None:
+    """The clipped policy loss of sequences (as in preference_loss) and its
+    gradient dlogp: with r = exp(logp - old_logp) (None: r = 1) and the
+    advantage A of its sequence (advantages [sequences]) or of the row ([rows];
+    per_token says which where the two numbers are the same), a scored row's
+    loss is
+        -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef k,
+        k = exp(ref_logp - logp) - (ref_logp - logp) - 1  (ref_logp None: none),
+    averaged over the scored rows ("token") or over the sequences' means
+    ("sequence").  `result` (at least POLICY_RESULT_WORDS int32; see
+    policy_result, policy_check) is overwritten, and dlogp in the rows of
+    sequences.  No host wait."""
+    ctx = ctx or default_context()
+    rows, seqs = logp.numel(), offsets.numel() - 1
+    if reduction not in POLICY_REDUCTIONS:
+        raise ValueError(f"unknown reduction {reduction!r}")
+    if per_token is None:
+        per_token = advantages.numel() != seqs
+    tp = None if targets is None else _targets(targets, rows)
+    _call(ctx, "cfops_policy_loss", _f32(logp, "logp"), _opt(old_logp, "old_logp", rows),
+          _opt(ref_logp, "ref_logp", rows), _f32(advantages, "advantages", rows if per_token else seqs), tp, rows,
+          _offsets(offsets), seqs, int(per_token), float(clip_low), float(clip_high), float(kl_coef),
+          POLICY_REDUCTIONS[reduction], _f32(dlogp, "dlogp", rows), _result(result, POLICY_RESULT_WORDS), _stream())
+
+
+# ------------------------------------------- AdamW with states in 8 bits
+def adamw8_state(n: int, device="cuda") -> torch.Tensor:
+    """An 8-bit state of n values (cfops_adamw_tensor), zero moments."""
+    return torch.zeros(_lib.lib().cfops_adamw8_state_bytes(int(n)), dtype=torch.uint8, device=device)
+
+
+def _state8(s: torch.Tensor, n: int) -> int:
+    if not isinstance(s, torch.Tensor) or not s.is_cuda or s.dtype != torch.uint8 or not s.is_contiguous():
+        raise TypeError("state8 must be a contiguous uint8 device tensor")
+    want = _lib.lib().cfops_adamw8_state_bytes(n)
+    if s.numel() != want:
+        raise _lib.ShapeError(_lib.ERR_SHAPE, f"assertion `left == right` failed: state8.len() = {s.numel()}, "
+                                              f"expected {want}")
+    return s.data_ptr()
+
+
+class Adamw8Tensors:
+    """The tensors of adamw8_update_multi, checked once: a list of dicts of p,
+    g, weight_decay and either m and v or state8 (adamw8_state; with m and v
+    too, they are what adamw8_pack_multi reads and adamw8_unpack_multi writes).
+    It keeps the tensors alive; a table may be passed any number of times."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        self.table = (_lib.AdamwTensorC * len(self.tensors))()
+        for c, t in zip(self.table, self.tensors):
+            p, g, m, v, s = (t.get(k) for k in ("p", "g", "m", "v", "state8"))
+            if s is None and (m is None or v is None):
+                raise ValueError("a tensor needs m and v, or state8")
+            of = next((x for x in (p, m, v) if x is not None), None)
+            if of is None:
+                raise ValueError("a tensor needs p, or m and v")
+            n = of.numel()
+            c.p, c.g, c.m, c.v = (_opt(x, k, n) for x, k in ((p, "p"), (g, "g"), (m, "m"), (v, "v")))
+            c.state8 = None if s is None else _state8(s, n)
+            c.n, c.weight_decay = n, float(t.get("weight_decay", 0.0))
+
+
+def _adamw8(name, tensors, ctx, *args):
+    ctx = ctx or default_context()
+    table = tensors if isinstance(tensors, Adamw8Tensors) else Adamw8Tensors(tensors)
+    _call(ctx, name, len(table.tensors), table.table, *args, _stream())
+
+
+def adamw8_update_multi(tensors, t, lr, beta1, beta2, eps, ctx: Context | None = None) -> None:
+    """One AdamW step (t 1-based) of many tensors (Adamw8Tensors, or a list it
+    takes), those with a state8 with their moments held in 8 bits, the others
+    as adamw_update.  In place, in few launches."""
+    _adamw8("cfops_adamw8_update_multi", tensors, ctx, int(t), float(lr), float(beta1), float(beta2), float(eps))
+
+
+def adamw8_pack_multi(tensors, ctx: Context | None = None) -> None:
+    """The f32 moments m and v of the tensors that have a state8 into it."""
+    _adamw8("cfops_adamw8_pack_multi", tensors, ctx)
+
+
+def adamw8_unpack_multi(tensors, ctx: Context | None = None) -> None:
+    """The moments that 8-bit states stand for, into m and v."""
+    _adamw8("cfops_adamw8_unpack_multi", tensors, ctx)

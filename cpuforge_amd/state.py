@@ -10,7 +10,9 @@ model has LoRA adapters, "lora_rank", "lora_alpha", "lora_targets".  A model
 is any object with `named_params()` (visit_params order,
 crates/model/src/model.rs:179-208), `lora_cfg` (None or rank / alpha /
 targets) and `add_lora(rank, alpha, targets, seed)`; the optimizer is
-`cpuforge_amd.optim.AdamW`.  Errors raise `FormatError` with the reference's
+`cpuforge_amd.optim.AdamW`; moments it holds in 8 bits are stored as the f32
+values they stand for (and packed again, to the same states, by the first
+update after a load).  Errors raise `FormatError` with the reference's
 message.
 """
 from __future__ import annotations
@@ -68,7 +70,8 @@ def save_state(path, model, opt, step: int, consumed: int) -> None:
         shape = list(p.shape)
         owned.append((f"p.{name}", shape, p.detach()))
         if name in opt.state:
-            m, v = opt.state[name]
+            s = opt.state[name]
+            m, v = s if isinstance(s, tuple) else s.moments()
         else:
             m = v = torch.zeros_like(p)
         owned.append((f"m.{name}", shape, m))

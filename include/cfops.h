@@ -166,6 +166,108 @@ int cfops_adamw_update_multi(cfattn_ctx* ctx, size_t count, float* const* p, con
                              float* const* v, const size_t* n, const float* weight_decay, uint64_t t, float lr,
                              float beta1, float beta2, float eps, void* stream);
 
+/* ---- preference and policy training ---------------------------------------
+ * No reference counterpart (the reference trains on cross-entropy alone):
+ * log-probabilities of the targets through the LM head, the losses that start
+ * from them, and AdamW with its moments in 8 bits.  Queued on `stream` with no
+ * host wait; results are blocks in device memory. */
+
+/* logits = hn . head^T; lse[r] = log sum_v exp(logits[r][v]); logp[r] =
+ * logits[r][targets[r]] - lse[r], both 0 where the target is
+ * CFOPS_IGNORE_INDEX.  hn [t, d], head [vocab, d]; logp, lse [t] and the block
+ * `result` (device memory) are overwritten: result->loss is the mean of -logp
+ * over the scored rows, result->bad_row names the first row whose target is
+ * outside [0, vocab) (such a row's logp and lse are NaN), as
+ * cfops_lm_head_ce_dev's does.  The logits are never held whole.  d and vocab
+ * must be positive, t below 2^24. */
+int cfops_lm_head_logprobs(cfattn_ctx* ctx, const float* hn, const float* head, const int64_t* targets, size_t t,
+                           size_t d, size_t vocab, float* logp, float* lse, cfops_ce_result* result, void* stream);
+/* From the gradient dlogp [t] of logp, and lse as the forward wrote it: dhn
+ * [t, d] (overwritten; NULL: not wanted) and, when dhead is non-null, dhead
+ * [vocab, d] += dlogits^T . hn.  The logits are formed again.  Rows that are not
+ * scored, or have a target out of range, have no gradient, and their hn, lse
+ * and dlogp do not matter. */
+int cfops_lm_head_logprobs_backward(cfattn_ctx* ctx, const float* hn, const float* head, const int64_t* targets,
+                                    const float* lse, const float* dlogp, size_t t, size_t d, size_t vocab,
+                                    float* dhn, float* dhead, void* stream);
+
+/* Rows of packed sequences: sequence i is rows [offsets[i], offsets[i + 1]) of
+ * logp (int64 in device memory, rising within [0, rows]).  A row whose target
+ * is CFOPS_IGNORE_INDEX is not scored (targets NULL: every row is): its inputs
+ * are not read, its gradient is 0.  Rows of no sequence keep their dlogp.
+ * Where offsets do not rise within [0, rows] they are not followed: the
+ * sequence counts as empty, the loss is NaN and the block's bad_seq names the
+ * first one (INT32_MAX: none). */
+typedef struct cfops_preference_result {
+    int32_t bad_seq;
+    float loss;     /* the mean over the pairs */
+    float accuracy; /* share of pairs whose chosen sequence has the larger reward */
+    float margin;   /* mean difference of their rewards */
+} cfops_preference_result;
+enum { CFOPS_PREFERENCE_SIGMOID = 0, CFOPS_PREFERENCE_HINGE = 1, CFOPS_PREFERENCE_SQUARED = 2 };
+/* Sequence 2j is the chosen and 2j + 1 the rejected one of pair j; offsets has
+ * 2 * pairs + 1 entries.  A sequence's reward is beta times the sum over its
+ * scored rows (length_mean != 0: the mean; 0 with none) of logp - ref_logp
+ * (ref_logp NULL: of logp); z = reward(chosen) - reward(rejected) - margin:
+ *   SIGMOID  -(1 - s) log sigmoid(z) - s log sigmoid(-z), s = label_smoothing
+ *   HINGE    max(0, 1 - z)
+ *   SQUARED  (z - 1/2)^2
+ * rewards [2 * pairs] and dlogp, the gradient of the mean loss, are
+ * overwritten.  label_smoothing is in [0, 1) and 0 for the other forms. */
+int cfops_preference_loss(cfattn_ctx* ctx, const float* logp, const float* ref_logp, const int64_t* targets,
+                          size_t rows, const int64_t* offsets, size_t pairs, int form, double beta, double margin,
+                          double label_smoothing, int length_mean, float* dlogp, float* rewards,
+                          cfops_preference_result* result, void* stream);
+
+typedef struct cfops_policy_result {
+    int32_t n_scored;
+    int32_t bad_seq;
+    float loss;
+    float kl;      /* the KL estimate under the loss's weights (0 without ref_logp) */
+    float clipped; /* share of scored rows whose ratio is cut */
+} cfops_policy_result;
+enum { CFOPS_POLICY_TOKEN_MEAN = 0, CFOPS_POLICY_SEQUENCE_MEAN = 1 };
+/* With r = exp(logp - old_logp) (old_logp NULL: r = 1, for one step on fresh
+ * samples) and A the row's advantage, a scored row's loss is
+ *   -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef k,
+ *   k = exp(x) - x - 1, x = ref_logp - logp (ref_logp NULL: no KL term),
+ * weighted 1 / N over all N scored rows (TOKEN_MEAN) or 1 / (M n_i) for the
+ * n_i scored rows of one of the M sequences that have any (SEQUENCE_MEAN).
+ * advantages: one a row (per_token != 0) or one a sequence.  offsets has seqs +
+ * 1 entries.  dlogp is overwritten. */
+int cfops_policy_loss(cfattn_ctx* ctx, const float* logp, const float* old_logp, const float* ref_logp,
+                      const float* advantages, const int64_t* targets, size_t rows, const int64_t* offsets,
+                      size_t seqs, int per_token, double clip_low, double clip_high, double kl_coef, int reduction,
+                      float* dlogp, cfops_policy_result* result, void* stream);
+
+/* AdamW over many tensors, each with its moments in 32 bits (m and v, updated as
+ * cfops_adamw_update does, bit for bit) or, where state8 is non-null, in 8: a
+ * buffer of cfops_adamw8_state_bytes(n) bytes, 16-byte aligned; zeroed, it
+ * holds zeros.  It holds blocks of 256 values, each with a power of two of its own
+ * for either moment: m as sign, 4 exponent and 3 mantissa bits, v as 5 and 3.
+ * A moment is rounded up or down by its fraction of a step against a threshold
+ * that is a function of its index and t, so that the mean of its roundings is its
+ * value; a positive v is never held as zero; what f32 does not hold is held as
+ * NaN (m) and infinity (v).  The update itself is f32, from the new moments
+ * before they are rounded.  Tensors that share memory are updated in order. */
+typedef struct cfops_adamw_tensor {
+    float* p;
+    const float* g;
+    float* m;       /* update: not read where state8 is non-null */
+    float* v;
+    uint8_t* state8;
+    size_t n;
+    float weight_decay;
+} cfops_adamw_tensor;
+size_t cfops_adamw8_state_bytes(size_t n);
+int cfops_adamw8_update_multi(cfattn_ctx* ctx, size_t count, const cfops_adamw_tensor* tensors, uint64_t t, float lr,
+                              float beta1, float beta2, float eps, void* stream);
+/* f32 moments m and v of the tensors that have a state8 into it, each to the
+ * nearest of its steps, and back.  An unpacked state packs to the same values.
+ * (p, g and weight_decay are not read.) */
+int cfops_adamw8_pack_multi(cfattn_ctx* ctx, size_t count, const cfops_adamw_tensor* tensors, void* stream);
+int cfops_adamw8_unpack_multi(cfattn_ctx* ctx, size_t count, const cfops_adamw_tensor* tensors, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,285 @@
+"""GPU tests of the targets' log-probabilities through the LM head and their
+gradients (cfops_lm_head_logprobs, _backward) against 64 bits."""
+import pytest
+import torch
+
+from cpuforge_amd import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+IGN = -100
+U = 2.0 ** -24  # half a step of f32
+
+
+def inputs(t, d, vocab, seed, masked=0.3, std=None):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    hn = torch.randn(t, d, generator=g, device=DEV)
+    head = torch.randn(vocab, d, generator=g, device=DEV) * (std or 2.0 / d ** 0.5)
+    tg = torch.randint(0, vocab, (t,), generator=g, device=DEV)
+    tg[torch.rand(t, generator=g, device=DEV) < masked] = IGN
+    return hn, head, tg, torch.randn(t, generator=g, device=DEV)
+
+
+def forward(hn, head, tg, check=True):
+    from cpuforge_amd import ops as P
+    t, d = hn.shape
+    logp, lse = (torch.full((t,), 77.0, device=DEV) for _ in range(2))
+    res = P.ce_result_buffer(DEV)
+    P.lm_head_logprobs(hn, head, tg, t, d, head.shape[0], logp, lse, res)
+    if check:
+        P.ce_check(res, tg, head.shape[0])
+    return logp, lse, res
+
+
+def backward(hn, head, tg, lse, dlogp, want_head=True):
+    from cpuforge_amd import ops as P
+    dhn = torch.full_like(hn, 77.0)
+    dhead = torch.ones_like(head) if want_head else None
+    P.lm_head_logprobs_backward(hn, head, tg, lse, dlogp, *hn.shape, head.shape[0], dhn, dhead)
+    return dhn, dhead
+
+
+def reference(hn, head, tg, dlogp):
+    """(logp, lse, dhn, dhead, dlogits) in 64 bits, and a bound on a logit's
+    error: the f32 products' (2^-22 of |hn| . |head|; their operands hold 22 bits
+    or more, and their sums are f32)."""
+    x = hn.double() @ head.double().T
+    off = 2.0 ** -22 * (hn.abs().double() @ head.abs().double().T).amax(1)
+    use = tg != IGN
+    ti = tg.clamp(min=0)
+    lse = torch.where(use, torch.logsumexp(x, 1), 0.0)
+    logp = torch.where(use, x.gather(1, ti[:, None])[:, 0] - lse, 0.0)
+    dx = torch.zeros_like(x).scatter_(1, ti[:, None], 1.0) - torch.softmax(x, 1)
+    dx = torch.where(use[:, None], dx * torch.where(use, dlogp.double(), 0.0)[:, None], 0.0)
+    return logp, lse, dx @ head.double(), dx.T @ hn.double(), dx, off, x
+
+
+def check(hn, head, tg, dlogp):
+    vocab = head.shape[0]
+    logp, lse, res = forward(hn, head, tg)
+    w_logp, w_lse, w_dhn, w_dhead, dx, off, x = reference(hn, head, tg, dlogp)
+    # A sum of exp over the vocabulary in f32: its longest chain of additions, and
+    # each term's rounded argument (up to 2^-24 of the largest difference) and exp.
+    chain = vocab / 512 + 24 + 8
+    spread = (x.amax(1) - x.amin(1)).clamp(max=104.0)
+    tol = off + U * (chain + spread + w_lse.abs() * 2)
+    use = tg != IGN
+    assert bool(((lse - w_lse).abs() <= torch.where(use, tol, 0.0)).all()), (lse - w_lse).abs().max()
+    tol2 = tol + off + U * (w_logp.abs() + 2 * w_lse.abs())
+    assert bool(((logp - w_logp).abs() <= torch.where(use, tol2, 0.0)).all()), (logp - w_logp).abs().max()
+    n = int(use.sum())
+    assert int(res[0]) == n and int(res[1]) == 2 ** 31 - 1
+    mean = -float(w_logp.sum()) / max(n, 1)
+    assert abs(float(res.view(torch.float32)[2]) - mean) <= float(tol2.max()) + 2.0 ** -23 * abs(mean)
+    dhn, dhead = backward(hn, head, tg, lse, dlogp)
+    # exp(x - lse): the errors of both, the difference's rounding and exp's, on
+    # every dlogit; then products of 22-bit operands in f32 sums.
+    p = dx.abs() + torch.zeros_like(dx).scatter_(1, tg.clamp(min=0)[:, None], 1.0) * (dlogp.abs() * use).double()[:, None]
+    rel = (off + tol + U * (spread + 8))[:, None] + 2.0 ** -21 + U * vocab ** 0.5
+    floor = 2.0 ** -36 * dlogp.abs().double()[:, None] * use[:, None]  # dlogits below their row's 2^-36
+    e = p * rel + floor
+    assert bool(((dhn - w_dhn).abs() <= e @ head.abs().double() + 1e-37).all()), (dhn - w_dhn).abs().max()
+    assert not dhn[~use].any()
+    tol_h = e.T @ hn.abs().double() + 2.0 ** -24 * (1 + w_dhead.abs()) + U * hn.shape[0] ** 0.5 * (p.T @ hn.abs().double())
+    assert bool(((dhead - 1 - w_dhead).abs() <= tol_h + 1e-37).all()), (dhead - 1 - w_dhead).abs().max()
+    assert torch.equal(backward(hn, head, tg, lse, dlogp, False)[0], dhn)
+
+
+SHAPES = [(1, 1, 1), (1, 64, 5), (3, 7, 130), (1, 576, 4097), (5, 576, 2000), (16, 100, 1000), (17, 576, 1000),
+          (64, 33, 4099), (65, 31, 257), (130, 100, 257), (256, 64, 512), (257, 576, 3001), (300, 65, 50),
+          (700, 128, 900), (513, 576, 8192), (1000, 16, 20000)]
+
+
+@pytest.mark.parametrize("t,d,vocab", SHAPES)
+def test_log_probabilities_and_gradients_match_64_bits(t, d, vocab):
+    print(t, d, vocab, flush=True)
+    check(*inputs(t, d, vocab, t + d + vocab))
+
+
+@pytest.mark.parametrize("masked", [0.0, 0.97, 1.0])
+@pytest.mark.parametrize("t", [9, 400])
+def test_masks(t, masked):
+    hn, head, tg, g = inputs(t, 96, 777, 5, masked)
+    check(hn, head, tg, g)
+    logp, lse, _ = forward(hn, head, tg)
+    dhn, dhead = backward(hn, head, tg, lse, g)
+    # What is not scored is not read.
+    off = tg == IGN
+    hn2, lse2, g2 = hn.clone(), lse.clone(), g.clone()
+    hn2[off], lse2[off], g2[off] = float("nan"), float("inf"), float("nan")
+    logp2, lse3, _ = forward(hn2, head, tg)
+    dhn2, dhead2 = backward(hn2, head, tg, lse2, g2)
+    assert torch.equal(logp, logp2) and torch.equal(lse, lse3)
+    assert torch.equal(dhn, dhn2) and torch.equal(dhead, dhead2)
+
+
+@pytest.mark.parametrize("t", [4, 300])
+def test_large_and_small_logits(t):
+    """Logits of +-300 (one weight row far above the others), rows of tiny and
+    of zero hidden states, weights over a wide range."""
+    hn, head, tg, g = inputs(t, 96, 1500, 6)
+    head *= torch.logspace(-6, 0, 1500, device=DEV)[:, None]
+    head[700] *= 1e3
+    hn[0] *= 1e-20
+    hn[1] = 0.0
+    hn[2] *= 30.0
+    tg[:4] = torch.tensor([3, 700, 701, 5], device=DEV)
+    check(hn, head, tg, g)
+
+
+@pytest.mark.parametrize("t", [4, 300])
+def test_targets_out_of_range(t):
+    from cpuforge_amd import ops as P
+    hn, head, tg, g = inputs(t, 64, 900, 7, 0.0)
+    want_logp, want_lse, _ = forward(hn, head, tg)
+    good_dhn, _ = backward(hn, head, tg, want_lse, g)
+    bad = tg.clone()
+    bad[1], bad[3] = 900, -1
+    logp, lse, res = forward(hn, head, bad, check=False)
+    with pytest.raises(_lib.CfattnError, match="target 900 out of range for vocab 900"):
+        P.ce_check(res, bad, 900)
+    keep = torch.ones(t, dtype=torch.bool, device=DEV)
+    keep[1] = keep[3] = False
+    assert torch.equal(logp[keep], want_logp[keep]) and bool(torch.isnan(logp[~keep]).all())
+    assert torch.equal(lse[keep], want_lse[keep])
+    dhn, dhead = backward(hn, head, bad, lse, g)
+    assert not dhn[~keep].any() and bool(torch.isfinite(dhead).all())
+    # (The rows' order in a product decides no bits of another row.)
+    assert torch.equal(dhn[keep], good_dhn[keep])
+
+
+@pytest.mark.parametrize("t", [4, 300])
+def test_a_row_that_is_not_finite_stays_alone(t):
+    hn, head, tg, g = inputs(t, 64, 900, 8, 0.0)
+    logp, lse, _ = forward(hn, head, tg)
+    dhn, _ = backward(hn, head, tg, lse, g, False)
+    hn2 = hn.clone()
+    hn2[2, 5] = float("nan")
+    logp2, lse2, _ = forward(hn2, head, tg)
+    dhn2, _ = backward(hn2, head, tg, lse2, g, False)
+    keep = torch.arange(t, device=DEV) != 2
+    assert bool(torch.isnan(logp2[2])) and bool(torch.isnan(lse2[2])) and bool(torch.isnan(dhn2[2]).any())
+    assert torch.equal(logp[keep], logp2[keep]) and torch.equal(dhn[keep], dhn2[keep])
+
+
+def test_no_rows():
+    from cpuforge_amd import ops as P
+    e = torch.empty(0, device=DEV)
+    head = torch.randn(10, 4, device=DEV)
+    tg = torch.empty(0, dtype=torch.int64, device=DEV)
+    res = P.ce_result_buffer(DEV)
+    P.lm_head_logprobs(e, head, tg, 0, 4, 10, e, e, res)
+    assert res.tolist() == [0, 2 ** 31 - 1, 0]
+    dhead = torch.ones_like(head)
+    P.lm_head_logprobs_backward(e, head, tg, e, e, 0, 4, 10, e, dhead)
+    assert bool((dhead == 1).all())
+
+
+def test_refusals():
+    from cpuforge_amd import ops as P
+    hn, head, tg, g = inputs(4, 8, 10, 1)
+    res = P.ce_result_buffer(DEV)
+    x = torch.zeros(4, device=DEV)
+    with pytest.raises(_lib.ShapeError):
+        P.lm_head_logprobs(hn, head, tg[:3], 4, 8, 10, x, x, res)
+    with pytest.raises(_lib.ShapeError):
+        P.lm_head_logprobs(hn, head, tg, 4, 8, 11, x, x, res)
+    with pytest.raises(TypeError):
+        P.lm_head_logprobs(hn, head, tg.int(), 4, 8, 10, x, x, res)
+    with pytest.raises(TypeError):
+        P.lm_head_logprobs(hn, head, tg, 4, 8, 10, x, x, res[:2])
+    with pytest.raises(TypeError):
+        P.lm_head_logprobs(hn.half(), head, tg, 4, 8, 10, x, x, res)
+    with pytest.raises(ValueError):
+        P.lm_head_logprobs(hn, head.T.contiguous().T, tg, 4, 8, 10, x, x, res)
+    with pytest.raises(_lib.CfattnError, match="positive"):
+        P.lm_head_logprobs(hn[:, :0].contiguous(), head[:, :0].contiguous(), tg, 4, 0, 10, x, x, res)
+
+
+def test_rows_in_chunks_and_repeated_calls_agree():
+    """A limit that cuts the backward's rows into chunks changes no bit of the rows'
+    gradients, nor does a second run."""
+    from cpuforge_amd import ops as P
+    hn, head, tg, g = inputs(700, 96, 2000, 12)
+    _, lse, _ = forward(hn, head, tg)
+    dhn, dhead = backward(hn, head, tg, lse, g)
+    again = backward(hn, head, tg, lse, g)
+    assert torch.equal(dhn, again[0]) and torch.equal(dhead, again[1])
+    P.set_head_chunk_limit(300 * 2000 * 4)
+    try:
+        logp2, lse2, _ = forward(hn, head, tg)
+        dhn2, dhead2 = backward(hn, head, tg, lse2, g)
+    finally:
+        P.set_head_chunk_limit(512 << 20)
+    w = reference(hn, head, tg, g)
+    assert bool(((dhn2 - w[2]).abs() <= 2 * (dhn - w[2]).abs().max()).all())
+    assert bool(((dhead2 - dhead).abs() <= 2.0 ** -20 * dhead.abs().max()).all())
+
+
+def test_captured_step_replays():
+    from cpuforge_amd import ops as P
+    hn, head, tg, g = inputs(300, 96, 3001, 13)
+    t, d, vocab = 300, 96, 3001
+
+    def bufs():
+        return [torch.zeros(t, device=DEV), torch.zeros(t, device=DEV), P.ce_result_buffer(DEV), torch.zeros_like(hn),
+                torch.zeros_like(head)]
+
+    def step(b):
+        P.lm_head_logprobs(hn, head, tg, t, d, vocab, b[0], b[1], b[2])
+        b[4].zero_()
+        P.lm_head_logprobs_backward(hn, head, tg, b[1], g, t, d, vocab, b[3], b[4])
+    a, b = bufs(), bufs()
+    step(b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(a)
+    for i in range(4):
+        hn.mul_(1.01)
+        tg.copy_(tg.roll(1))
+        graph.replay()
+        torch.cuda.synchronize()
+        step(b)
+        assert all(torch.equal(x, y) for x, y in zip(a, b)), i
+    # Outgrown scratch of the graph's stays: a larger eager call, then a replay.
+    forward(*inputs(900, 128, 5000, 14)[:3])
+    graph.replay()
+    step(b)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_autograd():
+    from cpuforge_amd import autograd as A
+    hn, head, tg, g = inputs(60, 48, 500, 15)
+    h3 = hn.view(4, 15, 48).requires_grad_()
+    w = head.clone().requires_grad_()
+    logp, res = A.lm_head_logprobs(h3, w, tg.view(4, 15))
+    assert logp.shape == (4, 15) and not res.requires_grad
+    dh, dw = torch.autograd.grad(logp, (h3, w), g.view(4, 15))
+    _, lse, _ = forward(hn, head, tg)
+    want = backward(hn, head, tg, lse, g)
+    assert torch.equal(dh.view(60, 48), want[0])
+    assert bool(((dw - (want[1] - 1)).abs() <= 2.0 ** -22 * (1 + dw.abs())).all())
+    (only,) = torch.autograd.grad(A.lm_head_logprobs(h3.detach(), w, tg.view(4, 15))[0], w, g.view(4, 15))
+    assert torch.equal(only, dw)
+
+
+def test_against_differences():
+    """The gradient against central differences of the 64-bit formula."""
+    hn, head, tg, g = inputs(6, 10, 40, 16, 0.2)
+    _, lse, _ = forward(hn, head, tg)
+    dhn, dhead = backward(hn, head, tg, lse, g)
+
+    def f(h, w):
+        return float((reference(h, w, tg, g)[0] * g.double()).sum())
+    h64, w64 = hn.double(), head.double()
+    for arr, got, at in ((h64, dhn, (0, 3)), (h64, dhn, (4, 9)), (w64, dhead - 1, (3, 2)), (w64, dhead - 1, (39, 0))):
+        eps = 1e-6
+        keep = float(arr[at])
+        arr[at] = keep + eps
+        up = f(h64, w64)
+        arr[at] = keep - eps
+        down = f(h64, w64)
+        arr[at] = keep
+        num = (up - down) / (2 * eps)
+        assert abs(float(got[at]) - num) <= 1e-5 * (1 + abs(num))
