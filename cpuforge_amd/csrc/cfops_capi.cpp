@@ -27,6 +27,14 @@ constexpr size_t kGemmWorkspace = (size_t)32 << 20;
 
 bool fits_int(size_t x) { return x <= (size_t)INT_MAX; }
 
+// A slot's buffer as T*.
+template <typename T>
+int take(cfattn_ctx* c, int s, size_t bytes, T*& p) {
+    int rc = CFATTN_OK;
+    p = static_cast<T*>(slot(c, s, bytes, &rc));
+    return p ? CFATTN_OK : rc;
+}
+
 int launch_gemm(cfattn_ctx* c, const cfattn::GemmF32& g, hipStream_t st) {
     int rc = CFATTN_OK;
     float* ws = static_cast<float*>(slot(c, cfattn_ctx::OPS_WS, kGemmWorkspace, &rc));
@@ -506,8 +514,11 @@ int check_logprobs(cfattn_ctx* c, size_t t, size_t d, size_t vocab) {
     return CFATTN_OK;
 }
 
-// Scratch of the log-probabilities: the scored rows, their hidden states (in the
-// backward over them their gradients), and the logits of a chunk of them.
+// From how many rows on the log-probabilities' products run on packed operands.
+constexpr size_t kHeadRows = 64;
+
+// Scratch of the log-probabilities of few rows: the scored rows, their hidden
+// states (in the backward over them their gradients), and the logits of a chunk.
 struct LogpRows {
     int *idx, *count;
     float *hn, *logits;
@@ -517,12 +528,83 @@ int logp_rows(cfattn_ctx* c, size_t t, size_t d, size_t vocab, LogpRows& r) {
     // A chunk's logits fit the head's limit, its rows a launch of workgroups.
     r.chunk = std::min<size_t>(c->head_chunk_bytes / (vocab * sizeof(float)), (size_t)1 << 22);
     r.chunk = std::min(std::max<size_t>(r.chunk, 1), t);
-    int rc = CFATTN_OK;
-    if (!(r.count = static_cast<int*>(slot(c, cfattn_ctx::OPS_IDX, (t + 4) * sizeof(int), &rc)))) return rc;
+    CF_TRY(take(c, cfattn_ctx::OPS_IDX, (t + 4) * sizeof(int), r.count));
     r.idx = r.count + 4;
-    if (!(r.hn = static_cast<float*>(slot(c, cfattn_ctx::OPS_ROWS, t * d * sizeof(float), &rc)))) return rc;
-    r.logits = static_cast<float*>(slot(c, cfattn_ctx::OPS_LOGITS, r.chunk * vocab * sizeof(float), &rc));
-    return r.logits ? CFATTN_OK : rc;
+    CF_TRY(take(c, cfattn_ctx::OPS_ROWS, t * d * sizeof(float), r.hn));
+    return take(c, cfattn_ctx::OPS_LOGITS, r.chunk * vocab * sizeof(float), r.logits);
+}
+
+// Scratch of those of many rows (head_plan).
+struct LogpHead {
+    cfattn::HeadPlan plan;
+    int *idx, *count, *exponents;
+    char *rows, *packed;
+    float* scale;
+};
+int logp_head(cfattn_ctx* c, size_t t, size_t d, size_t vocab, LogpHead& h) {
+    h.plan = cfattn::head_plan(t, d, vocab, c->head_chunk_bytes);
+    CF_TRY(take(c, cfattn_ctx::OPS_IDX, (t + 4 + h.plan.v_pad / 32) * sizeof(int), h.count));
+    h.idx = h.count + 4;
+    h.exponents = h.idx + t;
+    CF_TRY(take(c, cfattn_ctx::OPS_ROWS, h.plan.rows_bytes + h.plan.t_pad * sizeof(float), h.rows));
+    h.scale = reinterpret_cast<float*>(h.rows + h.plan.rows_bytes);
+    return take(c, cfattn_ctx::OPS_HEAD, h.plan.head_bytes, h.packed);
+}
+
+int logprobs_many(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets, size_t t, size_t d,
+                  size_t vocab, float* logp, float* lse, void* result, hipStream_t st) {
+    LogpHead h{};
+    CF_TRY(logp_head(c, t, d, vocab, h));
+    char* stats = nullptr;
+    CF_TRY(take(c, cfattn_ctx::OPS_STATS, h.plan.stats_bytes + h.plan.t_pad * sizeof(float), stats));
+    float* xt = reinterpret_cast<float*>(stats + h.plan.stats_bytes);
+    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, h.idx, h.count, logp, lse, result, st),
+           "log-probability launch");
+    CF_HIP(c, cfattn::launch_head_pack(h.plan, hn, h.idx, h.count, head, d, vocab, h.rows, h.scale, h.packed, nullptr,
+                                       h.exponents, nullptr, st),
+           "log-probability launch");
+    CF_HIP(c, cfattn::launch_head_stats(h.plan, h.rows, h.scale, h.packed, h.exponents, targets, h.idx, h.count, vocab,
+                                        stats, xt, logp, lse, st),
+           "log-probability launch");
+    return CFATTN_OK;
+}
+
+int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets,
+                           const float* lse, const float* dlogp, size_t t, size_t d, size_t vocab, float* dhn,
+                           float* dhead, hipStream_t st) {
+    LogpHead h{};
+    CF_TRY(logp_head(c, t, d, vocab, h));
+    char *back = nullptr, *grad = nullptr;
+    float *part = nullptr, *dlogits = nullptr, *gathered = nullptr;
+    if (dhn) {
+        CF_TRY(take(c, cfattn_ctx::OPS_BACK, h.plan.back_bytes, back));
+        CF_TRY(take(c, cfattn_ctx::OPS_LOGITS, h.plan.grad_bytes, grad));
+        CF_TRY(take(c, cfattn_ctx::OPS_PART, h.plan.part_bytes, part));
+    }
+    if (dhead) {
+        const size_t floats = h.plan.chunk * vocab;
+        CF_TRY(take(c, cfattn_ctx::OPS_DLOGITS, (floats + t * d) * sizeof(float), dlogits));
+        gathered = dlogits + floats;
+    }
+    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, h.idx, h.count, nullptr, nullptr, nullptr, st),
+           "log-probability launch");
+    CF_HIP(c, cfattn::launch_head_pack(h.plan, hn, h.idx, h.count, head, d, vocab, h.rows, h.scale, h.packed, back,
+                                       h.exponents, h.count + 1, st),
+           "log-probability launch");
+    if (dhead)
+        CF_HIP(c, cfattn::launch_logp_gather(hn, h.idx, h.count, gathered, t, d, st), "log-probability launch");
+    if (dhn) CF_HIP(c, cfattn::launch_head_zero_rows(targets, t, vocab, dhn, d, st), "log-probability launch");
+    for (size_t j0 = 0; j0 < t; j0 += h.plan.chunk) {
+        CF_HIP(c, cfattn::launch_head_grad(h.plan, h.rows, h.scale, h.packed, back, h.exponents, h.count + 1, targets,
+                                           h.idx, h.count, lse, dlogp, j0, d, vocab, grad, dlogits, part, dhn, st),
+               "log-probability launch");
+        if (!dhead) continue;
+        const size_t nr = std::min(t - j0, h.plan.chunk);
+        CF_HIP(c, cfattn::launch_head_zero_tail(h.plan, h.count, j0, nr, vocab, dlogits, st),
+               "log-probability launch");
+        CF_TRY(gemm(c, CFOPS_TN, dlogits, gathered + j0 * d, dhead, vocab, nr, d, true, st));
+    }
+    return CFATTN_OK;
 }
 
 int check_sequences(cfattn_ctx* c, size_t rows, size_t seqs) {
@@ -574,6 +656,11 @@ int cfops_lm_head_logprobs(cfattn_ctx* c, const float* hn, const float* head, co
     CF_TRY(check_logprobs(c, t, d, vocab));
     if (!head || (t && (!hn || !targets || !logp || !lse))) return fail(c, CFATTN_ERR_ARG, "null buffer");
     const hipStream_t st = to_stream(stream);
+    if (t >= kHeadRows) {
+        CF_TRY(logprobs_many(c, hn, head, targets, t, d, vocab, logp, lse, result, st));
+        CF_HIP(c, cfattn::launch_logp_finish(targets, logp, t, result, st), "log-probability launch");
+        return CFATTN_OK;
+    }
     LogpRows rows{};
     CF_TRY(logp_rows(c, t, d, vocab, rows));
     CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, logp, lse, result, st),
@@ -598,6 +685,7 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
     if (t == 0 || (!dhn && !dhead)) return CFATTN_OK;
     if (!hn || !head || !targets || !lse || !dlogp) return fail(c, CFATTN_ERR_ARG, "null buffer");
     const hipStream_t st = to_stream(stream);
+    if (t >= kHeadRows) return logprobs_backward_many(c, hn, head, targets, lse, dlogp, t, d, vocab, dhn, dhead, st);
     LogpRows rows{};
     CF_TRY(logp_rows(c, t, d, vocab, rows));
     CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, nullptr, nullptr, nullptr, st),

@@ -61,7 +61,8 @@ __global__ __launch_bounds__(1024) void logp_select_kernel(const int64_t* __rest
     if (lane == 0) wave_n[wave] = ignored;
     __syncthreads();
     if (threadIdx.x == 0) {
-        *count = n;
+        count[0] = n;
+        count[1] = INT_MIN;  // the largest exponent that head_gemm.hip's pack finds
         if (misc) {
             int all = 0;
             for (int w = 0; w < 16; w++) all += wave_n[w];
