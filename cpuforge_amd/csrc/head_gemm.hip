@@ -23,6 +23,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cfattn_common.hpp"
 #include "cfops_kernels.hpp"
@@ -36,6 +37,7 @@ constexpr int kFrag = 1024;        // bytes of an operand of one MFMA
 constexpr int kBN = 128;           // tokens of a tile
 constexpr int kWgs = 512;          // two workgroups to a CU
 constexpr int kStages = 3;
+constexpr int kGroup = 8;          // token tiles
 constexpr float kTop = 32768.0f;   // of a dlogit over dlogp
 
 __device__ __forceinline__ float exp2i(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
@@ -117,41 +119,67 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const float* __restrict_
 // [32 columns][16 rows][piece].  There lane l holds column l % 32 and of 16 rows
 // those that it holds of a product's 32 x 32 result: 4 (l / 32) + 0..3 and the
 // same eight on.
-template <bool BACK>
-__global__ __launch_bounds__(256) void pack_head_kernel(const float* __restrict__ head, char* __restrict__ out,
-                                                        char* __restrict__ back, int* __restrict__ exponents,
-                                                        int* __restrict__ largest, int vocab, int d, int k16, int v16,
-                                                        int vec) {
-    __shared__ float red[4];
-    __shared__ uint32_t tile[4][32][33];
+// A wave takes the pairs of operands (32 columns) w, w + NW, ..; with U > 0 at most U
+// of them, which stay in registers between the largest value and the pieces.  (The 32
+// rows of 2048 columns that each workgroup has read are 0.5 GB on all CUs together:
+// read again, they came from HBM again, 640 us for 128256 x 2048 at 3.3 TB/s of one
+// read and one write.)
+template <bool BACK, int NW, int U>
+__global__ __launch_bounds__(64 * NW) void pack_head_kernel(const float* __restrict__ head, char* __restrict__ out,
+                                                            char* __restrict__ back, int* __restrict__ exponents,
+                                                            int* __restrict__ largest, int vocab, int d, int k16,
+                                                            int v16, int vec) {
+    __shared__ float red[NW];
+    __shared__ uint32_t tile[BACK ? NW : 1][32][33];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * 32, r = r0 + (lane & 31);
     const float* row = r < vocab ? head + (long)r * d : nullptr;
     const bool v = vec && row;
-    float top = 0.0f, x[8];
-    for (int s = wave; s < k16; s += 4) {
-        load8(x, row, 16 * s + 8 * (lane >> 5), d, v);
+    const int c = 8 * (lane >> 5), pairs = (k16 + 1) / 2;
+    float top = 0.0f, x[U ? U : 1][2][8];
+    auto load = [&](float (&y)[2][8], int s) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) top = fmaxf(top, finite_abs(x[i]));
+        for (int q = 0; q < 2; q++) {
+            const bool in = 2 * s + q < k16;
+            load8(y[q], in ? row : nullptr, 16 * (2 * s + q) + c, d, v && in);
+        }
+    };
+    auto widen = [&](const float (&y)[2][8]) {
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, finite_abs(y[q][i]));
+    };
+    if constexpr (U > 0) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (wave + u * NW < pairs) load(x[u], wave + u * NW);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (wave + u * NW < pairs) widen(x[u]);
+    } else {
+        for (int s = wave; s < pairs; s += NW) {
+            load(x[0], s);
+            widen(x[0]);
+        }
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     if (lane == 0) red[wave] = top;
     __syncthreads();
-    const int e = group_exponent(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+#pragma unroll
+    for (int w = 0; w < NW; w++) top = fmaxf(top, red[w]);
+    const int e = group_exponent(top);
     if (threadIdx.x == 0) {
         exponents[blockIdx.x] = e;
         if (BACK) atomicMax(largest, e);
     }
     const float sc = exp2i(-e);
-    // Two operands (32 columns) a round.
-    for (int s = 2 * wave; s < k16; s += 8) {
+    auto store = [&](const float (&y)[2][8], int s) {
 #pragma unroll
         for (int q = 0; q < 2; q++) {
-            if (!BACK && s + q >= k16) break;
-            const int c = 8 * (lane >> 5);
-            load8(x, s + q < k16 ? row : nullptr, 16 * (s + q) + c, d, v && s + q < k16);
-            const Pieces p = split8(x, sc);
-            if (s + q < k16) store_pieces(out + ((long)blockIdx.x * k16 + s + q) * 2 * kFrag, lane, p);
+            const Pieces p = split8(y[q], sc);
+            if (2 * s + q < k16)
+                store_pieces(out + ((long)blockIdx.x * k16 + 2 * s + q) * 2 * kFrag, lane, p);
             if constexpr (BACK)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
@@ -173,9 +201,19 @@ __global__ __launch_bounds__(256) void pack_head_kernel(const float* __restrict_
                     p.h[i] = __builtin_bit_cast(_Float16, (uint16_t)u);
                     p.l[i] = __builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
                 }
-                store_pieces(back + ((long)(s / 2) * v16 + blockIdx.x * 2 + q) * 2 * kFrag, lane, p);
+                store_pieces(back + ((long)s * v16 + blockIdx.x * 2 + q) * 2 * kFrag, lane, p);
             }
             __builtin_amdgcn_wave_barrier();
+        }
+    };
+    if constexpr (U > 0) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (wave + u * NW < pairs) store(x[u], wave + u * NW);
+    } else {
+        for (int s = wave; s < pairs; s += NW) {
+            load(x[0], s);
+            store(x[0], s);
         }
     }
 }
@@ -248,9 +286,20 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
     const int o0 = (int)((long)outer * xcd / 8), o1 = (int)((long)outer * (xcd + 1) / 8);
     const uint32_t lds0 = lds_offset(lds), voff = lane * 16;
     for (int item = local; item < (o1 - o0) * inner; item += kWgs / 8) {
-        const int o = wave_uniform(o0 + item / inner), in = wave_uniform(item % inner);
-        const int tm = E == Epi::kPartial ? wave_uniform(in % g.mt) : o;
-        const int tt = E == Epi::kPartial ? wave_uniform(in / g.mt) : in;
+        // Stats and grad: kGroup token tiles with every tile along a of the XCD, then the
+        // next ones: what 64 workgroups read at a time is near a square, and the tokens'
+        // operands stay in the XCD's L2.
+        int o, tm, tt;
+        if constexpr (E == Epi::kPartial) {
+            o = wave_uniform(o0 + item / inner);
+            tm = wave_uniform(item % inner % g.mt);
+            tt = wave_uniform(item % inner / g.mt);
+        } else {
+            const int grp = item / ((o1 - o0) * kGroup), left = item - grp * (o1 - o0) * kGroup;
+            const int w = min(kGroup, nt - grp * kGroup);
+            o = tm = wave_uniform(o0 + left / w);
+            tt = wave_uniform(grp * kGroup + left % w);
+        }
         int k0 = 0, k1 = g.k16;
         if constexpr (E == Epi::kPartial) {
             k0 = wave_uniform((int)((long)g.k16 * o / splits));
@@ -377,7 +426,13 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
 #pragma unroll
                     for (int i = 0; i < MB; i++)
 #pragma unroll
-                        for (int q = 0; q < 16; q++) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], c[i], -m));
+                        for (int q = 0; q < 16; q += 4) {
+                            float x[4];
+#pragma unroll
+                            for (int z = 0; z < 4; z++) x[z] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][q + z], c[i], -m));
+                            sum += (x[0] + x[1]) + (x[2] + x[3]);
+                            __builtin_amdgcn_sched_barrier(0);  // (all at once take more registers than there are)
+                        }
                     sum = sum_halves(sum);
                     if (scored && hh == 0) g.stats[(long)(m0 / (32 * MB)) * g.ld + g.j0 + col] = make_float2(m, sum);
                 } else {
@@ -525,14 +580,31 @@ hipError_t launch_head_pack(const HeadPlan& p, const float* hn, const int* idx, 
                        (int)d, p.k16, d % 4 == 0 && aligned16(hn));
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 grid((unsigned)(p.v_pad / 32));
-    const int vec = d % 4 == 0 && aligned16(head);
+    const int vec = d % 4 == 0 && aligned16(head), pairs = (p.k16 + 1) / 2;
+    auto pack = [&](auto b, auto nw, auto u) {
+        constexpr int kNw = decltype(nw)::value;
+        hipLaunchKernelGGL((pack_head_kernel<decltype(b)::value, kNw, decltype(u)::value>),
+                           dim3((unsigned)(p.v_pad / 32)), dim3(64 * kNw), 0, st, head, packed, back, exponents,
+                           largest, (int)vocab, (int)d, p.k16, (int)(p.v_pad / 16), vec);
+    };
+    using std::integral_constant;
+    auto sized = [&](auto b) {
+        // The fewest registers that hold the rows.
+        if (pairs <= 8)
+            pack(b, integral_constant<int, 8>{}, integral_constant<int, 1>{});
+        else if (pairs <= 24)
+            pack(b, integral_constant<int, 8>{}, integral_constant<int, 3>{});
+        else if (pairs <= 64)
+            pack(b, integral_constant<int, 16>{}, integral_constant<int, 4>{});
+        else if (pairs <= 128)
+            pack(b, integral_constant<int, 16>{}, integral_constant<int, 8>{});
+        else
+            pack(b, integral_constant<int, 8>{}, integral_constant<int, 0>{});
+    };
     if (back)
-        hipLaunchKernelGGL(pack_head_kernel<true>, grid, dim3(256), 0, st, head, packed, back, exponents, largest,
-                           (int)vocab, (int)d, p.k16, (int)(p.v_pad / 16), vec);
+        sized(std::true_type{});
     else
-        hipLaunchKernelGGL(pack_head_kernel<false>, grid, dim3(256), 0, st, head, packed, back, exponents, largest,
-                           (int)vocab, (int)d, p.k16, (int)(p.v_pad / 16), vec);
+        sized(std::false_type{});
     return hipGetLastError();
 }
 
