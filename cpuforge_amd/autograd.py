@@ -183,6 +183,11 @@ class LMHeadCEDevFn(torch.autograd.Function):
         return (dhn * g).view(ctx.shape), (dhead * g if ctx.has_dhead else None), None
 
 
+#: Most bytes that lm_head_logprobs keeps from its forward for its backward
+#: (about 4 tokens * vocab + 4 d * vocab); above, the logits are formed again.
+LOGPROBS_KEEP_LIMIT = 8 << 30
+
+
 class LMHeadLogprobsFn(torch.autograd.Function):
     """The targets' log-probabilities under logits = hn head^T and the block
     that ops.ce_check reads (ops.lm_head_logprobs)."""
@@ -194,8 +199,13 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         t, vocab = h2.shape[0], head2.shape[0]
         logp, lse = _empty(tg, tg)
         result = P.ce_result_buffer(hn.device)
-        P.lm_head_logprobs(h2, head2, tg, t, d, vocab, logp, lse, result)
-        ctx.save_for_backward(h2, head2, tg, lse)
+        keep = None
+        if any(ctx.needs_input_grad):
+            n = P.lm_head_logprobs_keep_bytes(t, d, vocab)
+            if 0 < n <= LOGPROBS_KEEP_LIMIT:
+                keep = torch.empty(n, dtype=torch.uint8, device=hn.device)
+        P.lm_head_logprobs(h2, head2, tg, t, d, vocab, logp, lse, result, keep)
+        ctx.save_for_backward(h2, head2, tg, lse, keep)
         ctx.shape = hn.shape
         ctx.mark_non_differentiable(result)
         ctx.set_materialize_grads(False)
@@ -203,14 +213,14 @@ class LMHeadLogprobsFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g, _g_result):
-        h2, head, tg, lse = ctx.saved_tensors
+        h2, head, tg, lse, keep = ctx.saved_tensors
         need_hn, need_head = ctx.needs_input_grad[:2]
         if g is None or not (need_hn or need_head):
             return None, None, None
         dhn = torch.empty_like(h2) if need_hn else None
         dhead = torch.zeros_like(head) if need_head else None
         P.lm_head_logprobs_backward(h2, head, tg, lse, g.contiguous().view(-1), h2.shape[0], h2.shape[1],
-                                    head.shape[0], dhn, dhead)
+                                    head.shape[0], dhn, dhead, keep)
         return None if dhn is None else dhn.view(ctx.shape), dhead, None
 
 

@@ -534,75 +534,111 @@ int logp_rows(cfattn_ctx* c, size_t t, size_t d, size_t vocab, LogpRows& r) {
     return take(c, cfattn_ctx::OPS_LOGITS, r.chunk * vocab * sizeof(float), r.logits);
 }
 
-// Scratch of those of many rows (head_plan).
-struct LogpHead {
-    cfattn::HeadPlan plan;
-    int *idx, *count, *exponents;
-    char *rows, *packed;
-    float* scale;
+// Buffers of those of many rows: what a backward reads lies in `keep` where the
+// caller holds it, else in scratch.
+size_t align_up(size_t x) { return (x + 1023) / 1024 * 1024; }
+struct KeepLayout {
+    size_t keep, back, factor, bytes;  // offsets; count, idx and exponents come first
 };
-int logp_head(cfattn_ctx* c, size_t t, size_t d, size_t vocab, LogpHead& h) {
-    h.plan = cfattn::head_plan(t, d, vocab, c->head_chunk_bytes);
-    CF_TRY(take(c, cfattn_ctx::OPS_IDX, (t + 4 + h.plan.v_pad / 32) * sizeof(int), h.count));
-    h.idx = h.count + 4;
-    h.exponents = h.idx + t;
-    CF_TRY(take(c, cfattn_ctx::OPS_ROWS, h.plan.rows_bytes + h.plan.t_pad * sizeof(float), h.rows));
-    h.scale = reinterpret_cast<float*>(h.rows + h.plan.rows_bytes);
-    return take(c, cfattn_ctx::OPS_HEAD, h.plan.head_bytes, h.packed);
+KeepLayout keep_layout(const cfattn::HeadPlan& p, size_t t) {
+    KeepLayout l{};
+    l.keep = align_up((4 + t + p.v_pad / 32) * sizeof(int));
+    l.back = l.keep + align_up(p.keep_bytes);
+    l.factor = l.back + align_up(p.back_bytes);
+    l.bytes = l.factor + align_up(p.factor_bytes);
+    return l;
+}
+void keep_at(const cfattn::HeadPlan& p, size_t t, char* base, cfattn::HeadBuffers& b) {
+    const KeepLayout l = keep_layout(p, t);
+    b.count = reinterpret_cast<int*>(base);
+    b.idx = b.count + 4;
+    b.exponents = b.idx + t;
+    b.keep = base + l.keep;
+    b.back = base + l.back;
+    b.factor = reinterpret_cast<float*>(base + l.factor);
+}
+
+// The forward's scratch; with no keep, the small parts of it are scratch too.
+int head_scratch(cfattn_ctx* c, const cfattn::HeadPlan& p, size_t t, cfattn::HeadBuffers& b) {
+    char *rows = nullptr, *stats = nullptr;
+    CF_TRY(take(c, cfattn_ctx::OPS_ROWS, p.rows_bytes + p.t_pad * sizeof(float), rows));
+    b.rows = rows;
+    b.scale = reinterpret_cast<float*>(rows + p.rows_bytes);
+    CF_TRY(take(c, cfattn_ctx::OPS_STATS, p.stats_bytes + p.chunk * sizeof(float), stats));
+    b.stats = stats;
+    b.xt = reinterpret_cast<float*>(stats + p.stats_bytes);
+    CF_TRY(take(c, cfattn_ctx::OPS_HEAD, p.head_bytes, b.packed));
+    if (b.count) return CFATTN_OK;
+    CF_TRY(take(c, cfattn_ctx::OPS_IDX, (4 + t + p.v_pad / 32) * sizeof(int), b.count));
+    b.idx = b.count + 4;
+    b.exponents = b.idx + t;
+    return CFATTN_OK;
+}
+
+int check_keep(cfattn_ctx* c, const void* keep, size_t have, size_t need) {
+    if (reinterpret_cast<uintptr_t>(keep) % 16) return fail(c, CFATTN_ERR_ARG, "keep must be 16-byte aligned");
+    if (have < need) return fail(c, CFATTN_ERR_ARG, "keep holds %zu bytes, %zu are needed", have, need);
+    return CFATTN_OK;
 }
 
 int logprobs_many(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets, size_t t, size_t d,
-                  size_t vocab, float* logp, float* lse, void* result, hipStream_t st) {
-    LogpHead h{};
-    CF_TRY(logp_head(c, t, d, vocab, h));
-    char* stats = nullptr;
-    CF_TRY(take(c, cfattn_ctx::OPS_STATS, h.plan.stats_bytes + h.plan.t_pad * sizeof(float), stats));
-    float* xt = reinterpret_cast<float*>(stats + h.plan.stats_bytes);
-    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, h.idx, h.count, logp, lse, result, st),
+                  size_t vocab, float* logp, float* lse, void* result, void* keep, size_t keep_bytes,
+                  hipStream_t st) {
+    const cfattn::HeadPlan p = cfattn::head_plan(t, d, vocab, SIZE_MAX);
+    cfattn::HeadBuffers b{};
+    if (keep) {
+        CF_TRY(check_keep(c, keep, keep_bytes, keep_layout(p, t).bytes));
+        keep_at(p, t, static_cast<char*>(keep), b);
+    }
+    CF_TRY(head_scratch(c, p, t, b));
+    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, b.idx, b.count, logp, lse, result, st),
            "log-probability launch");
-    CF_HIP(c, cfattn::launch_head_pack(h.plan, hn, h.idx, h.count, head, d, vocab, h.rows, h.scale, h.packed, nullptr,
-                                       h.exponents, nullptr, st),
-           "log-probability launch");
-    CF_HIP(c, cfattn::launch_head_stats(h.plan, h.rows, h.scale, h.packed, h.exponents, targets, h.idx, h.count, vocab,
-                                        stats, xt, logp, lse, st),
-           "log-probability launch");
+    CF_HIP(c, cfattn::launch_head_pack(p, b, hn, head, d, vocab, st), "log-probability launch");
+    CF_HIP(c, cfattn::launch_head_stats(p, b, targets, 0, vocab, logp, lse, st), "log-probability launch");
     return CFATTN_OK;
 }
 
 int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets,
-                           const float* lse, const float* dlogp, size_t t, size_t d, size_t vocab, float* dhn,
-                           float* dhead, hipStream_t st) {
-    LogpHead h{};
-    CF_TRY(logp_head(c, t, d, vocab, h));
-    char *back = nullptr, *grad = nullptr;
-    float *part = nullptr, *dlogits = nullptr, *gathered = nullptr;
+                           const float* dlogp, size_t t, size_t d, size_t vocab, float* dhn, float* dhead,
+                           const void* keep, size_t keep_bytes, hipStream_t st) {
+    const cfattn::HeadPlan p = cfattn::head_plan(t, d, vocab, keep ? SIZE_MAX : c->head_chunk_bytes);
+    cfattn::HeadBuffers b{};
+    if (keep) {
+        CF_TRY(check_keep(c, keep, keep_bytes, keep_layout(p, t).bytes));
+        keep_at(p, t, static_cast<char*>(const_cast<void*>(keep)), b);
+    } else {
+        CF_TRY(head_scratch(c, p, t, b));
+        CF_TRY(take(c, cfattn_ctx::OPS_LOGITS, p.keep_bytes, b.keep));
+        CF_TRY(take(c, cfattn_ctx::OPS_BACK, p.back_bytes + p.factor_bytes, b.back));
+        b.factor = reinterpret_cast<float*>(b.back + p.back_bytes);
+        CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, b.idx, b.count, nullptr, nullptr, nullptr, st),
+               "log-probability launch");
+        CF_HIP(c, cfattn::launch_head_pack(p, b, hn, head, d, vocab, st), "log-probability launch");
+    }
     if (dhn) {
-        CF_TRY(take(c, cfattn_ctx::OPS_BACK, h.plan.back_bytes, back));
-        CF_TRY(take(c, cfattn_ctx::OPS_LOGITS, h.plan.grad_bytes, grad));
-        CF_TRY(take(c, cfattn_ctx::OPS_PART, h.plan.part_bytes, part));
+        CF_TRY(take(c, cfattn_ctx::OPS_PART, p.part_bytes, b.part));
+        CF_HIP(c, cfattn::launch_head_zero_rows(targets, t, vocab, dhn, d, st), "log-probability launch");
     }
+    // The head's gradient is an f32 product over dlogits that fit the head's limit.
+    const size_t pass = std::min(p.chunk, std::max<size_t>(c->head_chunk_bytes / (vocab * sizeof(float)) / 128 * 128, 128));
+    float *dlogits = nullptr, *gathered = nullptr;
     if (dhead) {
-        const size_t floats = h.plan.chunk * vocab;
-        CF_TRY(take(c, cfattn_ctx::OPS_DLOGITS, (floats + t * d) * sizeof(float), dlogits));
-        gathered = dlogits + floats;
+        CF_TRY(take(c, cfattn_ctx::OPS_DLOGITS, (pass * vocab + t * d) * sizeof(float), dlogits));
+        gathered = dlogits + pass * vocab;
+        CF_HIP(c, cfattn::launch_logp_gather(hn, b.idx, b.count, gathered, t, d, st), "log-probability launch");
     }
-    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, h.idx, h.count, nullptr, nullptr, nullptr, st),
-           "log-probability launch");
-    CF_HIP(c, cfattn::launch_head_pack(h.plan, hn, h.idx, h.count, head, d, vocab, h.rows, h.scale, h.packed, back,
-                                       h.exponents, h.count + 1, st),
-           "log-probability launch");
-    if (dhead)
-        CF_HIP(c, cfattn::launch_logp_gather(hn, h.idx, h.count, gathered, t, d, st), "log-probability launch");
-    if (dhn) CF_HIP(c, cfattn::launch_head_zero_rows(targets, t, vocab, dhn, d, st), "log-probability launch");
-    for (size_t j0 = 0; j0 < t; j0 += h.plan.chunk) {
-        CF_HIP(c, cfattn::launch_head_grad(h.plan, h.rows, h.scale, h.packed, back, h.exponents, h.count + 1, targets,
-                                           h.idx, h.count, lse, dlogp, j0, d, vocab, grad, dlogits, part, dhn, st),
-               "log-probability launch");
-        if (!dhead) continue;
-        const size_t nr = std::min(t - j0, h.plan.chunk);
-        CF_HIP(c, cfattn::launch_head_zero_tail(h.plan, h.count, j0, nr, vocab, dlogits, st),
-               "log-probability launch");
-        CF_TRY(gemm(c, CFOPS_TN, dlogits, gathered + j0 * d, dhead, vocab, nr, d, true, st));
+    for (size_t j0 = 0; j0 < t; j0 += p.chunk) {
+        if (!keep)
+            CF_HIP(c, cfattn::launch_head_stats(p, b, targets, j0, vocab, nullptr, nullptr, st),
+                   "log-probability launch");
+        if (dhn)
+            CF_HIP(c, cfattn::launch_head_dhn(p, b, targets, head, dlogp, j0, d, dhn, st), "log-probability launch");
+        for (size_t i = 0; dhead && i < p.chunk && j0 + i < t; i += pass) {
+            const size_t nr = std::min({t - j0 - i, p.chunk - i, pass});
+            CF_HIP(c, cfattn::launch_head_dlogits(p, b, targets, dlogp, j0, i, nr, vocab, dlogits, st),
+                   "log-probability launch");
+            CF_TRY(gemm(c, CFOPS_TN, dlogits, gathered + (j0 + i) * d, dhead, vocab, nr, d, true, st));
+        }
     }
     return CFATTN_OK;
 }
@@ -649,15 +685,21 @@ int adamw8_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors,
 
 }  // namespace
 
+size_t cfops_lm_head_logprobs_keep_bytes(size_t t, size_t d, size_t vocab) {
+    if (t < kHeadRows || t >= (size_t)1 << 24 || d == 0 || vocab == 0 || !fits_int(d) || !fits_int(vocab)) return 0;
+    return keep_layout(cfattn::head_plan(t, d, vocab, SIZE_MAX), t).bytes;
+}
+
 int cfops_lm_head_logprobs(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets, size_t t,
-                           size_t d, size_t vocab, float* logp, float* lse, cfops_ce_result* result, void* stream) {
+                           size_t d, size_t vocab, float* logp, float* lse, cfops_ce_result* result, void* keep,
+                           size_t keep_bytes, void* stream) {
     CF_LOCK(c, stream);
     if (!result) return fail(c, CFATTN_ERR_ARG, "null result");
     CF_TRY(check_logprobs(c, t, d, vocab));
     if (!head || (t && (!hn || !targets || !logp || !lse))) return fail(c, CFATTN_ERR_ARG, "null buffer");
     const hipStream_t st = to_stream(stream);
     if (t >= kHeadRows) {
-        CF_TRY(logprobs_many(c, hn, head, targets, t, d, vocab, logp, lse, result, st));
+        CF_TRY(logprobs_many(c, hn, head, targets, t, d, vocab, logp, lse, result, keep, keep_bytes, st));
         CF_HIP(c, cfattn::launch_logp_finish(targets, logp, t, result, st), "log-probability launch");
         return CFATTN_OK;
     }
@@ -679,13 +721,14 @@ int cfops_lm_head_logprobs(cfattn_ctx* c, const float* hn, const float* head, co
 
 int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets,
                                     const float* lse, const float* dlogp, size_t t, size_t d, size_t vocab,
-                                    float* dhn, float* dhead, void* stream) {
+                                    float* dhn, float* dhead, const void* keep, size_t keep_bytes, void* stream) {
     CF_LOCK(c, stream);
     CF_TRY(check_logprobs(c, t, d, vocab));
     if (t == 0 || (!dhn && !dhead)) return CFATTN_OK;
     if (!hn || !head || !targets || !lse || !dlogp) return fail(c, CFATTN_ERR_ARG, "null buffer");
     const hipStream_t st = to_stream(stream);
-    if (t >= kHeadRows) return logprobs_backward_many(c, hn, head, targets, lse, dlogp, t, d, vocab, dhn, dhead, st);
+    if (t >= kHeadRows)
+        return logprobs_backward_many(c, hn, head, targets, dlogp, t, d, vocab, dhn, dhead, keep, keep_bytes, st);
     LogpRows rows{};
     CF_TRY(logp_rows(c, t, d, vocab, rows));
     CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, nullptr, nullptr, nullptr, st),

@@ -200,34 +200,37 @@ hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const in
 hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t rows, void* misc, hipStream_t st);
 
 // The same for many rows, on packed f16 operands (head_gemm.hip), the logits only
-// in registers.  A plan holds the sizes of the buffers that its functions take:
-//   pack:   the scored rows of hn (rows, and scale [t_pad]) and the head (packed,
-//           exponents [v_pad / 32]; with `back` non-null also that and *largest,
-//           which select has reset) as operands;
-//   stats:  logp and lse of the scored rows (stats, xt [t_pad]);
-//   grad:   of scored rows [j0, j0 + chunk), j0 a multiple of chunk: dhn (or
-//           null) from `grad` and `part`, and dlogits [chunk][vocab] (or null), of
-//           which zero_tail clears the rows [.., rows) that grad leaves;
+// in registers.  A plan holds the sizes of the buffers, of which rows are in
+// chunks: those of stats, xt, keep and factor begin at the chunk's first scored row.
+//   pack:      rows, scale, packed and exponents, and with back non-null also that
+//              and count[1] (which select has reset);
+//   stats:     logp and lse (or null) of scored rows [j0, j0 + chunk), j0 a
+//              multiple of chunk; with keep non-null (and back packed) also that and
+//              factor, from which
+//   dhn:       their rows of dhn, and
+//   dlogits:   dlogits [rows][vocab] of those of them from `local` (a multiple of
+//              128) on, zeros behind the last scored one;
 //   zero_rows: dhn of the rows that are not scored.
 struct HeadPlan {
-    int k16;  // 16-k steps of a row
+    int k16, splits_max;  // 16-k steps of a row
     size_t t_pad, v_pad, d_pad, chunk;
-    size_t rows_bytes, head_bytes, back_bytes, stats_bytes, grad_bytes, part_bytes;
+    size_t rows_bytes, head_bytes, back_bytes, stats_bytes, keep_bytes, factor_bytes, part_bytes;
+};
+struct HeadBuffers {
+    int *idx, *count, *exponents;        // [t], [2], [v_pad / 32]
+    char *rows, *packed, *back, *keep;   // operands
+    float *scale, *xt, *factor, *part;   // scale [t_pad], xt [chunk]
+    void* stats;
 };
 HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes);
-hipError_t launch_head_pack(const HeadPlan& p, const float* hn, const int* idx, const int* count, const float* head,
-                            size_t d, size_t vocab, char* rows, float* scale, char* packed, char* back, int* exponents,
-                            int* largest, hipStream_t st);
-hipError_t launch_head_stats(const HeadPlan& p, const char* rows, const float* scale, const char* packed,
-                             const int* exponents, const int64_t* targets, const int* idx, const int* count,
-                             size_t vocab, void* stats, float* xt, float* logp, float* lse, hipStream_t st);
-hipError_t launch_head_grad(const HeadPlan& p, const char* rows, const float* scale, const char* packed,
-                            const char* back, const int* exponents, const int* largest, const int64_t* targets,
-                            const int* idx, const int* count, const float* lse, const float* dlogp, size_t j0,
-                            size_t d, size_t vocab, char* grad, float* dlogits, float* part, float* dhn,
-                            hipStream_t st);
-hipError_t launch_head_zero_tail(const HeadPlan& p, const int* count, size_t j0, size_t rows, size_t vocab,
-                                 float* dlogits, hipStream_t st);
+hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float* hn, const float* head, size_t d,
+                            size_t vocab, hipStream_t st);
+hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, size_t j0, size_t vocab,
+                             float* logp, float* lse, hipStream_t st);
+hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* head,
+                           const float* dlogp, size_t j0, size_t d, float* dhn, hipStream_t st);
+hipError_t launch_head_dlogits(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* dlogp,
+                               size_t j0, size_t local, size_t rows, size_t vocab, float* dlogits, hipStream_t st);
 hipError_t launch_head_zero_rows(const int64_t* targets, size_t t, size_t vocab, float* dhn, size_t d,
                                  hipStream_t st);
 

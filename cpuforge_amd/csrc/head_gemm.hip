@@ -13,8 +13,16 @@
 // of a group's exponent: rows of hidden states have one each, 32 rows of the
 // head share one.  A logit's error is so bounded by 2^-22 sum |h_k w_k| and 2^-39 of
 // the largest |h| times the largest |w| of the 32 rows, which is no more than f32
-// sums leave.  The gradients of logits lie in [-1, 1] times their row's dlogp: they
-// are formed without it, times 2^15 at most, and it multiplies the row at the end.
+// sums leave.
+//
+// The hidden states' gradient, dlogp (head[target] - sum_v P_v head[v]), takes P
+// from the forward: beside its statistics that keeps, for each token and 128
+// rows of the head, exp(x - m) with m their largest logit, as pieces in the order
+// of the gradient's product (4 bytes a logit).  The product adds 128 rows at a time
+// and scales their sum by exp(m - lse), a factor of the result's own column:
+// nothing is rounded again, and no exponential or product is formed twice.  (The
+// logits formed again in the backward instead, 3686 x 576 x 49152: 0.81 ms, where
+// keeping them takes 0.2.)
 //
 // Packed operands: both are first written as MFMA operands (1 KiB: a lane's eight
 // f16, 64 lanes) of 32 rows and 16 k, the two pieces side by side, so a
@@ -85,55 +93,41 @@ __device__ __forceinline__ void load8(float (&x)[8], const float* row, int k, in
     }
 }
 
-// The scored rows of hn, 32 to a workgroup, as operands [32 rows][16 k][piece], and
-// each row's 2^e; rows from n on are zeros.
-__global__ __launch_bounds__(256) void pack_rows_kernel(const float* __restrict__ hn, const int* __restrict__ idx,
-                                                        const int* __restrict__ count, char* __restrict__ out,
-                                                        float* __restrict__ scale, int d, int k16, int vec) {
-    __shared__ float red[4][32];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.x * 32 + (lane & 31);
-    const int n = *count;
-    if ((int)blockIdx.x * 32 >= (n + kBN - 1) / kBN * kBN) return;
-    const float* row = j < n ? hn + (long)idx[j] * d : nullptr;
-    const bool v = vec && row;
-    float top = 0.0f, x[8];
-    for (int s = wave; s < k16; s += 4) {
-        load8(x, row, 16 * s + 8 * (lane >> 5), d, v);
-#pragma unroll
-        for (int i = 0; i < 8; i++) top = fmaxf(top, finite_abs(x[i]));
-    }
-    top = max_halves(top);
-    if (lane < 32) red[wave][lane] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0][lane & 31], red[1][lane & 31]), fmaxf(red[2][lane & 31], red[3][lane & 31]));
-    const int e = group_exponent(top);
-    if (wave == 0 && lane < 32) scale[j] = exp2i(e);
-    for (int s = wave; s < k16; s += 4) {
-        load8(x, row, 16 * s + 8 * (lane >> 5), d, v);
-        store_pieces(out + ((long)blockIdx.x * k16 + s) * 2 * kFrag, lane, split8(x, exp2i(-e)));
-    }
-}
+struct PackArgs {
+    const float *hn, *head;
+    const int *idx, *count;
+    char *rows, *packed, *back;
+    float* scale;
+    int *exponents, *largest;
+    int row_blocks, vocab, d, k16, v16, vec_rows, vec_head;
+};
 
-// 32 rows of the head to a workgroup, as operands [32 rows][16 k][piece] with
-// their e, and, for the hidden states' gradient, whose k are these rows, as
-// [32 columns][16 rows][piece].  There lane l holds column l % 32 and of 16 rows
-// those that it holds of a product's 32 x 32 result: 4 (l / 32) + 0..3 and the
-// same eight on.
+// 32 rows to a workgroup, as operands [32 rows][16 k][piece]: first the scored rows
+// of hn, each with its own 2^e, zeros from row n on; then the head's, with one e,
+// and, for the hidden states' gradient, whose k are these rows, as [32 columns][16
+// rows][piece] too.  There lane l holds column l % 32 and of 16 rows those that it
+// holds of a product's 32 x 32 result: 4 (l / 32) + 0..3 and the same eight on.
 // A wave takes the pairs of operands (32 columns) w, w + NW, ..; with U > 0 at most U
-// of them, which stay in registers between the largest value and the pieces.  (The 32
-// rows of 2048 columns that each workgroup has read are 0.5 GB on all CUs together:
-// read again, they came from HBM again, 640 us for 128256 x 2048 at 3.3 TB/s of one
-// read and one write.)
+// of them, which stay in registers between the largest value and the pieces.
+// Bound by HBM: 128256 x 2048 411 us, 5.1 TB/s of one read and one write.  (Read
+// twice, the second time came from HBM again, since the 32 rows of all workgroups in
+// flight are 0.5 GB: 640 us.)
 template <bool BACK, int NW, int U>
-__global__ __launch_bounds__(64 * NW) void pack_head_kernel(const float* __restrict__ head, char* __restrict__ out,
-                                                            char* __restrict__ back, int* __restrict__ exponents,
-                                                            int* __restrict__ largest, int vocab, int d, int k16,
-                                                            int v16, int vec) {
-    __shared__ float red[NW];
+__global__ __launch_bounds__(64 * NW) void pack_kernel(const PackArgs g) {
+    __shared__ float red[NW][32];
     __shared__ uint32_t tile[BACK ? NW : 1][32][33];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * 32, r = r0 + (lane & 31);
-    const float* row = r < vocab ? head + (long)r * d : nullptr;
-    const bool v = vec && row;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31;
+    const bool is_head = (int)blockIdx.x >= g.row_blocks;
+    const int blk = is_head ? blockIdx.x - g.row_blocks : blockIdx.x, r = blk * 32 + l32, k16 = g.k16, d = g.d;
+    const float* row = nullptr;
+    if (is_head) {
+        if (r < g.vocab) row = g.head + (long)r * d;
+    } else {
+        const int n = *g.count;
+        if (blk * 32 >= (n + kBN - 1) / kBN * kBN) return;
+        if (r < n) row = g.hn + (long)g.idx[r] * d;
+    }
+    const bool v = (is_head ? g.vec_head : g.vec_rows) && row;
     const int c = 8 * (lane >> 5), pairs = (k16 + 1) / 2;
     float top = 0.0f, x[U ? U : 1][2][8];
     auto load = [&](float (&y)[2][8], int s) {
@@ -162,34 +156,38 @@ __global__ __launch_bounds__(64 * NW) void pack_head_kernel(const float* __restr
             widen(x[0]);
         }
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if (lane == 0) red[wave] = top;
+    top = max_halves(top);
+    if (lane < 32) red[wave][lane] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; w++) top = fmaxf(top, red[w]);
+    for (int w = 0; w < NW; w++) top = fmaxf(top, red[w][l32]);
+    if (is_head)
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     const int e = group_exponent(top);
-    if (threadIdx.x == 0) {
-        exponents[blockIdx.x] = e;
-        if (BACK) atomicMax(largest, e);
+    if (is_head && threadIdx.x == 0) {
+        g.exponents[blk] = e;
+        if (BACK) atomicMax(g.largest, e);
     }
+    if (!is_head && threadIdx.x < 32) g.scale[r] = exp2i(e);
     const float sc = exp2i(-e);
+    char* out = is_head ? g.packed : g.rows;
     auto store = [&](const float (&y)[2][8], int s) {
 #pragma unroll
         for (int q = 0; q < 2; q++) {
             const Pieces p = split8(y[q], sc);
-            if (2 * s + q < k16)
-                store_pieces(out + ((long)blockIdx.x * k16 + 2 * s + q) * 2 * kFrag, lane, p);
+            if (2 * s + q < k16) store_pieces(out + ((long)blk * k16 + 2 * s + q) * 2 * kFrag, lane, p);
             if constexpr (BACK)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     // (Copies: a bit cast of a vector's element itself takes element 0.)
                     const _Float16 h = p.h[i], l = p.l[i];
-                    tile[wave][lane & 31][16 * q + c + i] = (uint32_t)__builtin_bit_cast(uint16_t, h) |
-                                                            (uint32_t)__builtin_bit_cast(uint16_t, l) << 16;
+                    tile[wave][l32][16 * q + c + i] = (uint32_t)__builtin_bit_cast(uint16_t, h) |
+                                                      (uint32_t)__builtin_bit_cast(uint16_t, l) << 16;
                 }
         }
         if constexpr (BACK) {
+            if (!is_head) return;
             // (A wave's own part of LDS: its own order of accesses is enough.)
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -197,11 +195,11 @@ __global__ __launch_bounds__(64 * NW) void pack_head_kernel(const float* __restr
                 Pieces p;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const uint32_t u = tile[wave][16 * q + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)][lane & 31];
+                    const uint32_t u = tile[wave][16 * q + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)][l32];
                     p.h[i] = __builtin_bit_cast(_Float16, (uint16_t)u);
                     p.l[i] = __builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
                 }
-                store_pieces(back + ((long)s * v16 + blockIdx.x * 2 + q) * 2 * kFrag, lane, p);
+                store_pieces(g.back + ((long)s * g.v16 + blk * 2 + q) * 2 * kFrag, lane, p);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -218,39 +216,31 @@ __global__ __launch_bounds__(64 * NW) void pack_head_kernel(const float* __restr
     }
 }
 
-enum class Epi { kStats, kGrad, kPartial };
-
 struct HeadArgs {
-    const char *a, *b;   // operands: rows of the result along a (BM to a tile), tokens along b
-    int k16;             // 16-k steps of an operand
-    int mt;              // tiles along a
-    const int* count;    // scored rows
-    int j0, chunk;       // this launch's: [j0, min(j0 + chunk, count))
-    // stats and grad: a is the head
-    const int* exponents;
+    const char *a, *b;  // operands: rows of the result along a (64 MB to a tile), tokens along b
+    int k16;            // 16-k steps of an operand
+    int mt;             // tiles along a
+    const int* count;   // scored rows
+    int j0, chunk;      // this launch's: [j0, min(j0 + chunk, count)); b, stats, keep and part start at j0
+    long ld;            // of stats, xt and factor
+    // statistics: a is the head
+    const int *exponents, *largest, *idx;
     const float* scale;
     const int64_t* targets;
-    const int* idx;
-    int vocab;
-    float2* stats;       // [128 rows of the head][ld]: max and sum of exp2, in log2 units
-    long ld;
-    float* xt;           // the targets' logits
-    // grad
-    const float* lse;
-    const float* dlogp;
-    const int* largest;
-    char* grad;          // [32 tokens][v16][piece]
-    int v16;
-    float* dlogits;      // or null: [chunk][vocab]
-    // partial: a is the head by columns, b the gradients
-    float* part;         // [split][chunk][BM * mt]
+    int vocab, v16;
+    float2* stats;      // [128 rows of the head][ld]: max and sum of exp2, in log2 units
+    float* xt;          // the targets' logits
+    char* keep;         // [32 tokens][v16][piece], or null
+    // gradient: a is the head by columns, b what statistics kept
+    const float* factor;  // [128 rows of the head][ld]
+    float* part;          // [split][chunk][64 MB mt]
     int splits_max;
 };
 
-// Splits of the hidden states' gradient's k (the vocabulary) over workgroups: a
-// multiple of the XCDs, so that one XCD's L2 holds what its workgroups share.  The
-// one with the least rounds of its share of the 64 workgroups of an XCD times its
-// length; a split's partial sums cost their way through memory.
+// Splits of the gradient's k (the vocabulary) over workgroups: a multiple of the
+// XCDs, so that one XCD's L2 holds what its workgroups share.  The one with the
+// least rounds of an XCD's share over its 64 workgroups times its length; a split's
+// partial sums cost their way through memory.
 __device__ __forceinline__ int splits_of(int tiles, int k16, int splits_max) {
     int best = 8;
     float least = INFINITY;
@@ -262,11 +252,11 @@ __device__ __forceinline__ int splits_of(int tiles, int k16, int splits_max) {
     return best;
 }
 
-// A tile of BM = 64 MB rows and kBN tokens to a workgroup of four waves, each 32 MB x 64;
+// A tile of 64 MB rows and kBN tokens to a workgroup of four waves, each 32 MB x 64;
 // two workgroups to a CU: one's epilogue runs beside the other's products.
-template <int MB, Epi E>
+template <int MB, bool GRAD>
 __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
-    constexpr int BM = 64 * MB, CH = 4 * MB + 8, STAGE = CH * kFrag, PER = CH / 4;
+    constexpr int BM = 64 * MB, CH = 4 * MB + 8, PER = CH / 4 + GRAD, STAGE = CH * kFrag + GRAD * 1024;
     static_assert(CH % 4 == 0, "whole loads a wave");
     __shared__ __attribute__((aligned(1024))) char lds[kStages * STAGE];
     const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
@@ -277,69 +267,71 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
     // Items of an XCD: a contiguous run of the tiles along a (of the splits), every
     // token tile with each.
     const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
-    int outer = g.mt, inner = nt, splits = 1;
-    if constexpr (E == Epi::kPartial) {
-        splits = wave_uniform(splits_of(g.mt * nt, g.k16, g.splits_max));
-        outer = splits;
+    int outer = g.mt, inner = nt;
+    if constexpr (GRAD) {
+        outer = wave_uniform(splits_of(g.mt * nt, g.k16, g.splits_max));
         inner = g.mt * nt;
     }
     const int o0 = (int)((long)outer * xcd / 8), o1 = (int)((long)outer * (xcd + 1) / 8);
     const uint32_t lds0 = lds_offset(lds), voff = lane * 16;
     for (int item = local; item < (o1 - o0) * inner; item += kWgs / 8) {
-        // Stats and grad: kGroup token tiles with every tile along a of the XCD, then the
-        // next ones: what 64 workgroups read at a time is near a square, and the tokens'
-        // operands stay in the XCD's L2.
-        int o, tm, tt;
-        if constexpr (E == Epi::kPartial) {
+        // Statistics: kGroup token tiles with every tile along a of the XCD, then the
+        // next ones: what 64 workgroups read at a time is near a square.
+        int o, tm, tt, k0 = 0, k1 = g.k16;
+        if constexpr (GRAD) {
             o = wave_uniform(o0 + item / inner);
             tm = wave_uniform(item % inner % g.mt);
             tt = wave_uniform(item % inner / g.mt);
+            // (Whole runs of 128 rows of the head.)
+            k0 = wave_uniform((int)((long)(g.k16 / 8) * o / outer) * 8);
+            k1 = wave_uniform((int)((long)(g.k16 / 8) * (o + 1) / outer) * 8);
         } else {
             const int grp = item / ((o1 - o0) * kGroup), left = item - grp * (o1 - o0) * kGroup;
             const int w = min(kGroup, nt - grp * kGroup);
             o = tm = wave_uniform(o0 + left / w);
             tt = wave_uniform(grp * kGroup + left % w);
         }
-        int k0 = 0, k1 = g.k16;
-        if constexpr (E == Epi::kPartial) {
-            k0 = wave_uniform((int)((long)g.k16 * o / splits));
-            k1 = wave_uniform((int)((long)g.k16 * (o + 1) / splits));
-        }
-        const char* src[PER];
+        const char* src[CH / 4];
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int c = PER * wave + i;  // the stage's KiB: operand c / 2, piece c % 2
+        for (int i = 0; i < CH / 4; i++) {
+            const int c = CH / 4 * wave + i;  // the stage's KiB: operand c / 2, piece c % 2
             const int blk = c / 2;
             const char* base = blk < 2 * MB ? g.a + ((long)(tm * 2 * MB + blk) * g.k16 + k0) * 2 * kFrag
                                             : g.b + ((long)(tt * 4 + blk - 2 * MB) * g.k16 + k0) * 2 * kFrag;
             src[i] = base + (c % 2) * kFrag;
         }
+        const int col0 = tt * kBN + wn * 64;  // this wave's first token
+        int kl = k0;                          // the next stage's k
         auto load = [&](uint32_t stage) {
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
-                lds_load16_so(src[i], voff, lds0 + stage + (PER * wave + i) * kFrag);
+            for (int i = 0; i < CH / 4; i++) {
+                lds_load16_so(src[i], voff, lds0 + stage + (CH / 4 * wave + i) * kFrag);
                 src[i] += 2 * kFrag;
             }
+            if constexpr (GRAD) {
+                // The factors of the stage's 128 rows for the wave's tokens.
+                lds_load4_so(g.factor + (long)(kl / 8) * g.ld + col0, lane * 4, lds0 + stage + CH * kFrag + wave * 256);
+                kl++;
+            }
         };
-        f32x16 acc[MB][2];
+        f32x16 acc[MB][2], tot[GRAD ? MB : 1][2];
 #pragma unroll
-        for (int i = 0; i < MB; i++) acc[i][0] = acc[i][1] = zero16();
+        for (int i = 0; i < MB; i++) {
+            acc[i][0] = acc[i][1] = zero16();
+            if constexpr (GRAD) tot[i][0] = tot[i][1] = zero16();
+        }
         // Every wave is done with the LDS of the item before, and with its stores
         // (they would count among the loads waited for below).
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         uint32_t cur = 0, nxt = 2 * STAGE;
-        load(0);
+        if (k0 < k1) load(0);  // (more splits than runs: some have none)
         if (k0 + 1 < k1) load(STAGE);
         for (int k = k0; k < k1; k++) {
-            if (k + 1 < k1) {
-                if constexpr (PER == 6)
-                    asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
-                else
-                    asm volatile("s_waitcnt vmcnt(5) lgkmcnt(0)" ::: "memory");
-            } else {
+            if (k + 1 < k1)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(PER) : "memory");
+            else
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            }
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             if (k + 2 < k1) load(nxt);
@@ -364,14 +356,28 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
 #pragma unroll
                     for (int j = 0; j < 2; j++)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][pa[q]], b[j][pb[q]], acc[i][j], 0, 0, 0);
+            if constexpr (GRAD) {
+                if (k % 8 != 7) continue;
+                const float* f = reinterpret_cast<const float*>(s + CH * kFrag + wave * 256);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float fj = f[32 * j + l32];
+#pragma unroll
+                    for (int i = 0; i < MB; i++) {
+#pragma unroll
+                        for (int q = 0; q < 16; q++) tot[i][j][q] = fmaf(acc[i][j][q], fj, tot[i][j][q]);
+                        acc[i][j] = zero16();
+                    }
+                }
+            }
         }
 
         const int m0 = tm * BM + wm * 32 * MB;  // this wave's first row
-        if constexpr (E == Epi::kPartial) {
+        if constexpr (GRAD) {
             const int rows = g.mt * BM;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const int col = tt * kBN + wn * 64 + 32 * j + l32;
+                const int col = col0 + 32 * j + l32;
                 float* out = g.part + ((long)o * g.chunk + col) * rows + m0 + 4 * hh;
                 if (col < n)
 #pragma unroll
@@ -379,139 +385,129 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
 #pragma unroll
                         for (int q = 0; q < 4; q++)
                             *reinterpret_cast<float4*>(out + 32 * i + 8 * q) =
-                                make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                                            acc[i][j][4 * q + 3]);
+                                make_float4(tot[i][j][4 * q], tot[i][j][4 * q + 1], tot[i][j][4 * q + 2],
+                                            tot[i][j][4 * q + 3]);
             }
-            continue;
         } else {
             const int live = g.vocab - m0;  // rows of the head in this wave's part
-            if (live <= 0 && E == Epi::kStats) continue;
             int e[MB];
 #pragma unroll
             for (int i = 0; i < MB; i++) e[i] = wave_uniform(g.exponents[m0 / 32 + i]);
+            const int big = g.keep ? wave_uniform(*g.largest) : 0;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const int col = tt * kBN + wn * 64 + 32 * j + l32;
+                const int col = col0 + 32 * j + l32;
                 const bool scored = col < n;
                 const long r = scored ? g.idx[g.j0 + col] : 0;
                 const int et = (int)(__builtin_bit_cast(uint32_t, g.scale[g.j0 + col]) >> 23) - 127;
                 // The target's row within this wave's part.
                 const long target = (scored ? g.targets[r] : -1) - m0;
-                const bool here = __any(target >= 0 && target < 32 * MB);
-                if constexpr (E == Epi::kStats) {
-                    if (live < 32 * MB)
-#pragma unroll
-                        for (int i = 0; i < MB; i++)
-#pragma unroll
-                            for (int q = 0; q < 16; q++)
-                                if (32 * i + 8 * (q >> 2) + 4 * hh + (q & 3) >= live) acc[i][j][q] = -INFINITY;
-                    if (here)
-#pragma unroll
-                        for (int i = 0; i < MB; i++)
-#pragma unroll
-                            for (int q = 0; q < 16; q++)
-                                if (32 * i + 8 * (q >> 2) + 4 * hh + (q & 3) == target)
-                                    g.xt[g.j0 + col] = acc[i][j][q] * pow2_clamped(e[i] + et);
-                    float c[MB], m = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < MB; i++) {
-                        c[i] = pow2_clamped(e[i] + et) * kLog2e;
-                        float t = acc[i][j][0];
-#pragma unroll
-                        for (int q = 1; q < 16; q++) t = fmaxf(t, acc[i][j][q]);
-                        m = fmaxf(m, t * c[i]);
-                    }
-                    m = max_halves(m);
-                    float sum = 0.0f;
+                if (live < 32 * MB)
 #pragma unroll
                     for (int i = 0; i < MB; i++)
 #pragma unroll
-                        for (int q = 0; q < 16; q += 4) {
-                            float x[4];
+                        for (int q = 0; q < 16; q++)
+                            if (32 * i + 8 * (q >> 2) + 4 * hh + (q & 3) >= live) acc[i][j][q] = -INFINITY;
+                if (__any(target >= 0 && target < 32 * MB))
 #pragma unroll
-                            for (int z = 0; z < 4; z++) x[z] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][q + z], c[i], -m));
-                            sum += (x[0] + x[1]) + (x[2] + x[3]);
-                            __builtin_amdgcn_sched_barrier(0);  // (all at once take more registers than there are)
-                        }
-                    sum = sum_halves(sum);
-                    if (scored && hh == 0) g.stats[(long)(m0 / (32 * MB)) * g.ld + g.j0 + col] = make_float2(m, sum);
-                } else {
-                    const float lse2 = (scored ? g.lse[r] : 0.0f) * kLog2e;
-                    const float dl = g.dlogits && scored ? g.dlogp[r] : 0.0f;
-                    const int big = wave_uniform(*g.largest);
+                    for (int i = 0; i < MB; i++)
 #pragma unroll
-                    for (int i = 0; i < MB; i++) {
-                        const float c = pow2_clamped(e[i] + et) * kLog2e;
-                        const float f = kTop * pow2_clamped(e[i] - big);
-                        float y[16];
+                        for (int q = 0; q < 16; q++)
+                            if (32 * i + 8 * (q >> 2) + 4 * hh + (q & 3) == target)
+                                g.xt[col] = acc[i][j][q] * pow2_clamped(e[i] + et);
+                float c[MB], m = -INFINITY;
 #pragma unroll
-                        for (int q = 0; q < 16; q++) {
-                            const int row = 32 * i + 8 * (q >> 2) + 4 * hh + (q & 3);
-                            float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][q], c, -lse2));
-                            if (here && row == target) p -= 1.0f;
-                            y[q] = scored && row < live ? p : 0.0f;
-                        }
-                        if (g.dlogits && col < g.chunk) {
-                            float* out = g.dlogits + (long)col * g.vocab + m0 + 32 * i + 4 * hh;
+                for (int i = 0; i < MB; i++) {
+                    c[i] = pow2_clamped(e[i] + et) * kLog2e;
+                    float t = acc[i][j][0];
 #pragma unroll
-                            for (int q = 0; q < 16; q++)
-                                if (32 * i + 8 * (q >> 2) + 4 * hh + (q & 3) < live)
-                                    out[8 * (q >> 2) + (q & 3)] = -dl * y[q];
-                        }
-                        if (!g.grad) continue;
+                    for (int q = 1; q < 16; q++) t = fmaxf(t, acc[i][j][q]);
+                    m = fmaxf(m, t * c[i]);
+                }
+                m = max_halves(m);
+                if (live <= 0) m = 0.0f;  // (its exponentials are zeros)
+                float sum = 0.0f;
 #pragma unroll
-                        for (int q = 0; q < 2; q++) {
-                            float x[8];
+                for (int i = 0; i < MB; i++) {
+                    float y[16];
 #pragma unroll
-                            for (int z = 0; z < 8; z++) x[z] = y[8 * q + z];
-                            store_pieces(g.grad + ((long)(tt * 4 + wn * 2 + j) * g.v16 + m0 / 16 + 2 * i + q) * 2 * kFrag,
-                                         lane, split8(x, f));
-                        }
+                    for (int q = 0; q < 16; q += 4) {
+#pragma unroll
+                        for (int z = 0; z < 4; z++)
+                            y[q + z] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][q + z], c[i], -m));
+                        sum += (y[q] + y[q + 1]) + (y[q + 2] + y[q + 3]);
+                        __builtin_amdgcn_sched_barrier(0);  // (all at once take more registers than there are)
+                    }
+                    if (!g.keep) continue;
+                    const float f = scored ? kTop * pow2_clamped(e[i] - big) : 0.0f;
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        float x[8];
+#pragma unroll
+                        for (int z = 0; z < 8; z++) x[z] = y[8 * q + z];
+                        store_pieces(g.keep + ((long)(col0 / 32 + j) * g.v16 + m0 / 16 + 2 * i + q) * 2 * kFrag, lane,
+                                     split8(x, f));
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
+                sum = sum_halves(sum);
+                if (scored && hh == 0 && live > 0) g.stats[(long)(m0 / (32 * MB)) * g.ld + col] = make_float2(m, sum);
             }
         }
     }
 }
 
-// lse and logp of scored row j from its parts' maxima and sums, a wave to a row.
-__global__ __launch_bounds__(256) void head_finish_kernel(const float2* __restrict__ stats, long ld, int parts,
-                                                          const float* __restrict__ xt, const int* __restrict__ idx,
-                                                          const int* __restrict__ count, float* __restrict__ logp,
-                                                          float* __restrict__ lse) {
-    // 16 rows to a workgroup: lane l has row l % 16, so that a part's are read side by side.
-    __shared__ float2 red[16][17];
-    const int c = threadIdx.x & 15, p0 = threadIdx.x >> 4, j = blockIdx.x * 16 + c, n = *count;
-    float m = -INFINITY, s = 0.0f;
-    if (j < n)
-        for (int p = p0; p < parts; p += 16) {
-            const float2 x = stats[p * ld + j];
-            const float t = fmaxf(m, x.x);
-            // (NaN sums pass through; an empty m is -inf beside a sum of 0.)
-            s = (s == 0.0f ? 0.0f : s * exp2f(m - t)) + x.y * exp2f(x.x - t);
-            m = t;
-        }
-    red[p0][c] = make_float2(m, s);
-    __syncthreads();
-    if (p0 || j >= n) return;
-    for (int p = 1; p < 16; p++) {
-        const float2 x = red[p][c];
-        const float t = fmaxf(m, x.x);
-        s = (s == 0.0f ? 0.0f : s * exp2f(m - t)) + (x.y == 0.0f ? 0.0f : x.y * exp2f(x.x - t));
-        m = t;
-    }
-    // Units of kLog2e as rounded: the quotient has the largest logit's own bits.
-    const double l = (double)m / (double)kLog2e + log((double)s);
-    const int r = idx[j];
-    lse[r] = (float)l;
-    logp[r] = (float)((double)xt[j] - l);
+// Sums of exp2 with their maxima.
+__device__ __forceinline__ float2 join(const float2& a, const float2& b) {
+    const float t = fmaxf(a.x, b.x);
+    // (A sum of 0 is an empty part's, beside -inf; a NaN sum passes through.)
+    return make_float2(t, (a.y == 0.0f ? 0.0f : a.y * exp2f(a.x - t)) + (b.y == 0.0f ? 0.0f : b.y * exp2f(b.x - t)));
 }
 
-// dhn of the chunk's scored rows: the splits' sums in order, times dlogp.
+// lse and logp (or null) of scored rows [j0, ..) from their parts' maxima and sums,
+// and what the gradient scales a part by (or null).  16 rows to a workgroup, lane l
+// has row l % 16, so that a part's are read side by side.
+__global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restrict__ stats, long ld, int parts,
+                                                           int all_parts, const float* __restrict__ xt,
+                                                           const int* __restrict__ idx, const int* __restrict__ count,
+                                                           int j0, int chunk, float* __restrict__ logp,
+                                                           float* __restrict__ lse, float* __restrict__ factor) {
+    __shared__ float2 red[16][16];
+    __shared__ float lse2[16];
+    const int c = threadIdx.x & 15, p0 = threadIdx.x >> 4, j = blockIdx.x * 16 + c;
+    const int n = min(*count - j0, chunk);
+    if ((int)blockIdx.x * 16 >= (n + kBN - 1) / kBN * kBN) return;
+    float2 a = make_float2(-INFINITY, 0.0f);
+    if (j < n)
+        for (int p = p0; p < parts; p += 64) a = join(a, stats[p * ld + j]);
+    a = join(a, make_float2(__shfl_xor(a.x, 16), __shfl_xor(a.y, 16)));
+    a = join(a, make_float2(__shfl_xor(a.x, 32), __shfl_xor(a.y, 32)));
+    if ((threadIdx.x & 63) < 16) red[threadIdx.x >> 6][c] = a;
+    __syncthreads();
+    if (p0 == 0) {
+        for (int w = 1; w < 16; w++) a = join(a, red[w][c]);
+        lse2[c] = a.x + log2f(a.y);
+        if (j < n && logp) {
+            // Units of kLog2e as rounded: the quotient has the largest logit's own bits.
+            const double l = (double)a.x / (double)kLog2e + log((double)a.y);
+            const int r = idx[j0 + j];
+            lse[r] = (float)l;
+            logp[r] = (float)((double)xt[j] - l);
+        }
+    }
+    if (!factor) return;
+    __syncthreads();
+    for (int p = p0; p < all_parts; p += 64)
+        factor[p * ld + j] = j < n && p < parts ? exp2f(stats[p * ld + j].x - lse2[c]) : 0.0f;
+}
+
+// dhn of scored rows [j0, ..): dlogp (head[target] - the splits' sums in order).
 __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __restrict__ part, int chunk, int rows,
                                                                int mt, int k16, int splits_max,
                                                                const int* __restrict__ idx,
                                                                const int* __restrict__ count, int j0,
+                                                               const int64_t* __restrict__ targets,
+                                                               const float* __restrict__ head,
                                                                const float* __restrict__ dlogp,
                                                                const int* __restrict__ largest,
                                                                float* __restrict__ dhn, int d) {
@@ -520,23 +516,59 @@ __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __re
     if (col >= n) return;
     const int splits = splits_of(mt * ((n + kBN - 1) / kBN), k16, splits_max);
     const long r = idx[j0 + col];
-    const float f = -dlogp[r];
-    const int big = *largest;
-    const float u = pow2_clamped(big - 15);
+    const float* w = head + targets[r] * d;
+    const float f = dlogp[r], u = pow2_clamped(*largest - 15);
     for (int i = threadIdx.x; i < d; i += 256) {
         float s = 0.0f;
         for (int p = 0; p < splits; p++) s += part[((long)p * chunk + col) * rows + i];
-        dhn[r * d + i] = f * (s * u);
+        dhn[r * d + i] = f * (w[i] - s * u);
     }
 }
 
-// Zeros in the rows of dlogits behind the last tile.
-__global__ __launch_bounds__(256) void head_zero_tail_kernel(const int* __restrict__ count, int j0, int chunk,
-                                                             float* __restrict__ dlogits, long vocab) {
-    const int n = max(min(*count - j0, chunk), 0);
-    const long r = blockIdx.x;
-    if (r < (n + kBN - 1) / kBN * kBN) return;
-    for (long i = threadIdx.x; i < vocab; i += 256) dlogits[r * vocab + i] = 0.0f;
+// dlogits [rows][vocab] of scored rows [j0, ..) from what statistics kept, zeros
+// from row n on: 32 rows and 128 columns to a workgroup, through LDS, so that
+// rows are written 512 bytes at a time.
+__global__ __launch_bounds__(256) void head_dlogits_kernel(const char* __restrict__ keep, int v16,
+                                                           const float* __restrict__ factor, long ld,
+                                                           const int* __restrict__ exponents,
+                                                           const int* __restrict__ largest,
+                                                           const int* __restrict__ idx,
+                                                           const int* __restrict__ count, int j0, int chunk, int nr,
+                                                           const int64_t* __restrict__ targets,
+                                                           const float* __restrict__ dlogp,
+                                                           float* __restrict__ dlogits, long vocab) {
+    __shared__ float tile[32][129];
+    __shared__ float grad[32];
+    __shared__ int target[32];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
+    const int n = min(*count - j0, chunk), t0 = blockIdx.y * 32;
+    const long v0 = (long)blockIdx.x * 128;
+    if (threadIdx.x < 32) {
+        const bool scored = t0 + (int)threadIdx.x < n;
+        const long r = scored ? idx[j0 + t0 + threadIdx.x] : 0;
+        grad[threadIdx.x] = scored ? dlogp[r] : 0.0f;
+        target[threadIdx.x] = scored ? (int)targets[r] : -1;
+    }
+    if (t0 < n) {
+        const float f = t0 + l32 < n ? factor[blockIdx.x * ld + t0 + l32] : 0.0f;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const int s = 2 * wave + q;  // 16 columns
+            const char* p = keep + ((long)blockIdx.y * v16 + blockIdx.x * 8 + s) * 2 * kFrag + lane * 16;
+            const f16x8 h = *reinterpret_cast<const f16x8*>(p), l = *reinterpret_cast<const f16x8*>(p + kFrag);
+            const float u = f * pow2_clamped(*largest - exponents[blockIdx.x * 4 + wave] - 15);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                tile[l32][16 * s + 8 * (i >> 2) + 4 * hh + (i & 3)] = ((float)h[i] + (float)l[i]) * u;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * 128; i += 256) {
+        const int r = i >> 7, c = i & 127;
+        if (t0 + r >= nr || v0 + c >= vocab) continue;
+        const float p = t0 + r < n ? tile[r][c] : 0.0f;
+        dlogits[(t0 + r) * vocab + v0 + c] = t0 + r < n ? grad[r] * ((v0 + c == target[r]) - p) : 0.0f;
+    }
 }
 
 // Zeros in the rows that are not scored.
@@ -550,9 +582,9 @@ __global__ __launch_bounds__(256) void head_zero_rows_kernel(const int64_t* __re
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 size_t up(size_t x, size_t to) { return (x + to - 1) / to * to; }
 
-// Blocks of 32 along the columns of the head, to a tile: three (192) to a wave's 96
-// or four (256), whichever pads less.
-int back_mb(size_t d) { return up(d, 192) < up(d, 256) ? 3 : 4; }
+// Blocks of 32 columns of the head of a wave in the gradient's product (its sums
+// take twice the registers): three where that pads little, else two.
+int back_mb(size_t d) { return 10 * up(d, 192) <= 11 * up(d, 128) ? 3 : 2; }
 constexpr int kSplitsMax = 32;
 
 }  // namespace
@@ -564,97 +596,93 @@ HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes) {
     p.t_pad = up(t, kBN);
     p.d_pad = up(d, 64 * back_mb(d));
     p.chunk = std::min(std::max<size_t>(chunk_bytes / (p.v_pad * 4) / kBN * kBN, kBN), p.t_pad);
+    p.splits_max = (int)std::min<size_t>(
+        kSplitsMax, std::max<size_t>(8, ((size_t)256 << 20) / (p.chunk * p.d_pad * sizeof(float)) / 8 * 8));
+    p.splits_max = (int)std::min<size_t>(p.splits_max, std::max<size_t>(8, p.v_pad / 256 / 8 * 8));
     p.rows_bytes = p.t_pad * p.k16 * 64;
     p.head_bytes = p.v_pad * p.k16 * 64;
     p.back_bytes = p.d_pad * p.v_pad * 4;
-    p.stats_bytes = (p.v_pad / 128) * p.t_pad * sizeof(float2);
-    p.grad_bytes = p.chunk * p.v_pad * 4;
-    p.part_bytes = (size_t)kSplitsMax * p.chunk * p.d_pad * sizeof(float);
+    p.stats_bytes = (p.v_pad / 128) * p.chunk * sizeof(float2);
+    p.keep_bytes = p.chunk * p.v_pad * 4;
+    p.factor_bytes = (p.v_pad / 128) * p.chunk * sizeof(float);
+    p.part_bytes = (size_t)p.splits_max * p.chunk * p.d_pad * sizeof(float);
     return p;
 }
 
-hipError_t launch_head_pack(const HeadPlan& p, const float* hn, const int* idx, const int* count, const float* head,
-                            size_t d, size_t vocab, char* rows, float* scale, char* packed, char* back, int* exponents,
-                            int* largest, hipStream_t st) {
-    hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)(p.t_pad / 32)), dim3(256), 0, st, hn, idx, count, rows, scale,
-                       (int)d, p.k16, d % 4 == 0 && aligned16(hn));
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    const int vec = d % 4 == 0 && aligned16(head), pairs = (p.k16 + 1) / 2;
-    auto pack = [&](auto b, auto nw, auto u) {
+hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float* hn, const float* head, size_t d,
+                            size_t vocab, hipStream_t st) {
+    PackArgs g{};
+    g.hn = hn, g.head = head, g.idx = b.idx, g.count = b.count, g.rows = b.rows, g.packed = b.packed, g.back = b.back;
+    g.scale = b.scale, g.exponents = b.exponents, g.largest = b.count + 1, g.row_blocks = (int)(p.t_pad / 32);
+    g.vocab = (int)vocab, g.d = (int)d, g.k16 = p.k16, g.v16 = (int)(p.v_pad / 16);
+    g.vec_rows = d % 4 == 0 && aligned16(hn), g.vec_head = d % 4 == 0 && aligned16(head);
+    const int pairs = (p.k16 + 1) / 2;
+    auto pack = [&](auto back, auto nw, auto u) {
         constexpr int kNw = decltype(nw)::value;
-        hipLaunchKernelGGL((pack_head_kernel<decltype(b)::value, kNw, decltype(u)::value>),
-                           dim3((unsigned)(p.v_pad / 32)), dim3(64 * kNw), 0, st, head, packed, back, exponents,
-                           largest, (int)vocab, (int)d, p.k16, (int)(p.v_pad / 16), vec);
+        hipLaunchKernelGGL((pack_kernel<decltype(back)::value, kNw, decltype(u)::value>),
+                           dim3((unsigned)((p.t_pad + p.v_pad) / 32)), dim3(64 * kNw), 0, st, g);
     };
     using std::integral_constant;
-    auto sized = [&](auto b) {
+    auto sized = [&](auto back) {
         // The fewest registers that hold the rows.
         if (pairs <= 8)
-            pack(b, integral_constant<int, 8>{}, integral_constant<int, 1>{});
+            pack(back, integral_constant<int, 8>{}, integral_constant<int, 1>{});
         else if (pairs <= 24)
-            pack(b, integral_constant<int, 8>{}, integral_constant<int, 3>{});
+            pack(back, integral_constant<int, 8>{}, integral_constant<int, 3>{});
         else if (pairs <= 64)
-            pack(b, integral_constant<int, 16>{}, integral_constant<int, 4>{});
-        else if (pairs <= 128)
-            pack(b, integral_constant<int, 16>{}, integral_constant<int, 8>{});
+            pack(back, integral_constant<int, 16>{}, integral_constant<int, 4>{});
         else
-            pack(b, integral_constant<int, 8>{}, integral_constant<int, 0>{});
+            pack(back, integral_constant<int, 8>{}, integral_constant<int, 0>{});
     };
-    if (back)
+    if (b.back)
         sized(std::true_type{});
     else
         sized(std::false_type{});
     return hipGetLastError();
 }
 
-hipError_t launch_head_stats(const HeadPlan& p, const char* rows, const float* scale, const char* packed,
-                             const int* exponents, const int64_t* targets, const int* idx, const int* count,
-                             size_t vocab, void* stats, float* xt, float* logp, float* lse, hipStream_t st) {
+hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, size_t j0, size_t vocab,
+                             float* logp, float* lse, hipStream_t st) {
     HeadArgs g{};
-    g.a = packed, g.b = rows, g.k16 = p.k16, g.mt = (int)(p.v_pad / 256), g.count = count, g.j0 = 0;
-    g.chunk = (int)p.t_pad, g.exponents = exponents, g.scale = scale, g.targets = targets, g.idx = idx;
-    g.vocab = (int)vocab, g.stats = static_cast<float2*>(stats), g.ld = (long)p.t_pad, g.xt = xt;
-    hipLaunchKernelGGL((head_gemm_kernel<4, Epi::kStats>), dim3(kWgs), dim3(256), 0, st, g);
+    g.a = b.packed, g.b = b.rows + j0 / 32 * p.k16 * 2 * kFrag, g.k16 = p.k16, g.mt = (int)(p.v_pad / 256);
+    g.count = b.count, g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.exponents = b.exponents;
+    g.largest = b.count + 1, g.idx = b.idx, g.scale = b.scale, g.targets = targets, g.vocab = (int)vocab;
+    g.v16 = (int)(p.v_pad / 16), g.stats = static_cast<float2*>(b.stats), g.xt = b.xt, g.keep = b.keep;
+    hipLaunchKernelGGL((head_gemm_kernel<4, false>), dim3(kWgs), dim3(256), 0, st, g);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)(p.t_pad / 16)), dim3(256), 0, st, g.stats, g.ld,
-                       (int)((vocab + 127) / 128), xt, idx, count, logp, lse);
+    hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)(p.chunk / 16)), dim3(1024), 0, st, g.stats, g.ld,
+                       (int)((vocab + 127) / 128), (int)(p.v_pad / 128), b.xt, b.idx, b.count, (int)j0, (int)p.chunk,
+                       logp, lse, b.keep ? b.factor : nullptr);
     return hipGetLastError();
 }
 
-hipError_t launch_head_grad(const HeadPlan& p, const char* rows, const float* scale, const char* packed,
-                            const char* back, const int* exponents, const int* largest, const int64_t* targets,
-                            const int* idx, const int* count, const float* lse, const float* dlogp, size_t j0,
-                            size_t d, size_t vocab, char* grad, float* dlogits, float* part, float* dhn,
-                            hipStream_t st) {
-    HeadArgs g{};
-    g.a = packed, g.b = rows + j0 / 32 * p.k16 * 2 * kFrag, g.k16 = p.k16, g.mt = (int)(p.v_pad / 256);
-    g.count = count, g.j0 = (int)j0, g.chunk = (int)p.chunk, g.exponents = exponents, g.scale = scale;
-    g.targets = targets, g.idx = idx, g.vocab = (int)vocab, g.lse = lse, g.dlogp = dlogp, g.largest = largest;
-    g.grad = dhn ? grad : nullptr, g.v16 = (int)(p.v_pad / 16), g.dlogits = dlogits;
-    hipLaunchKernelGGL((head_gemm_kernel<4, Epi::kGrad>), dim3(kWgs), dim3(256), 0, st, g);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !dhn) return e;
+hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* head,
+                           const float* dlogp, size_t j0, size_t d, float* dhn, hipStream_t st) {
     const int mb = back_mb(d);
-    HeadArgs h{};
-    h.a = back, h.b = grad, h.k16 = g.v16, h.mt = (int)(p.d_pad / (64 * mb)), h.count = count, h.j0 = (int)j0;
-    h.chunk = (int)p.chunk, h.part = part, h.splits_max = std::min(kSplitsMax, std::max(8, h.k16 / 4 / 8 * 8));
+    HeadArgs g{};
+    g.a = b.back, g.b = b.keep, g.k16 = (int)(p.v_pad / 16), g.mt = (int)(p.d_pad / (64 * mb)), g.count = b.count;
+    g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.factor = b.factor, g.part = b.part;
+    g.splits_max = p.splits_max;
     if (mb == 3)
-        hipLaunchKernelGGL((head_gemm_kernel<3, Epi::kPartial>), dim3(kWgs), dim3(256), 0, st, h);
+        hipLaunchKernelGGL((head_gemm_kernel<3, true>), dim3(kWgs), dim3(256), 0, st, g);
     else
-        hipLaunchKernelGGL((head_gemm_kernel<4, Epi::kPartial>), dim3(kWgs), dim3(256), 0, st, h);
-    e = hipGetLastError();
+        hipLaunchKernelGGL((head_gemm_kernel<2, true>), dim3(kWgs), dim3(256), 0, st, g);
+    hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(head_grad_reduce_kernel, dim3((unsigned)p.chunk), dim3(256), 0, st, part, (int)p.chunk,
-                       (int)p.d_pad, h.mt, h.k16, h.splits_max, idx, count, (int)j0, dlogp, largest, dhn, (int)d);
+    hipLaunchKernelGGL(head_grad_reduce_kernel, dim3((unsigned)p.chunk), dim3(256), 0, st, b.part, (int)p.chunk,
+                       (int)p.d_pad, g.mt, g.k16, g.splits_max, b.idx, b.count, (int)j0, targets, head, dlogp,
+                       b.count + 1, dhn, (int)d);
     return hipGetLastError();
 }
 
-hipError_t launch_head_zero_tail(const HeadPlan& p, const int* count, size_t j0, size_t rows, size_t vocab,
-                                 float* dlogits, hipStream_t st) {
-    hipLaunchKernelGGL(head_zero_tail_kernel, dim3((unsigned)rows), dim3(256), 0, st, count, (int)j0, (int)p.chunk,
-                       dlogits, (long)vocab);
+hipError_t launch_head_dlogits(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* dlogp,
+                               size_t j0, size_t local, size_t rows, size_t vocab, float* dlogits, hipStream_t st) {
+    // (Rows [local, local + rows) of those that statistics kept from row j0 on.)
+    hipLaunchKernelGGL(head_dlogits_kernel, dim3((unsigned)((vocab + 127) / 128), (unsigned)((rows + 31) / 32)),
+                       dim3(256), 0, st, b.keep + local * p.v_pad * 4, (int)(p.v_pad / 16), b.factor + local,
+                       (long)p.chunk, b.exponents, b.count + 1, b.idx, b.count, (int)(j0 + local), (int)rows,
+                       (int)rows, targets, dlogp, dlogits, (long)vocab);
     return hipGetLastError();
 }
 

@@ -143,18 +143,23 @@ __global__ __launch_bounds__(512) void logp_grad_rows_kernel(float* __restrict__
 }
 
 // The mean of -logp over the scored rows, summed in f64 in a fixed order.
-__global__ __launch_bounds__(256) void logp_finish_kernel(const int64_t* __restrict__ targets,
-                                                          const float* __restrict__ logp, long rows,
-                                                          CeMisc* __restrict__ m) {
-    __shared__ double sp[256];
+__global__ __launch_bounds__(1024) void logp_finish_kernel(const int64_t* __restrict__ targets,
+                                                           const float* __restrict__ logp, long rows,
+                                                           CeMisc* __restrict__ m) {
+    __shared__ double red[16];
     double s = 0.0;
-    for (long r = threadIdx.x; r < rows; r += 256)
-        if (targets[r] != kIgnoreIndex) s -= (double)logp[r];
-    sp[threadIdx.x] = s;
+#pragma unroll 4
+    for (long r = threadIdx.x; r < rows; r += 1024) {
+        const float x = logp[r];
+        s -= targets[r] != kIgnoreIndex ? (double)x : 0.0;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
         double tot = 0.0;
-        for (int i = 0; i < 256; i++) tot += sp[i];
+        for (int i = 0; i < 16; i++) tot += red[i];
         const int n = m->n_valid;
         m->loss = n > 0 ? (float)(tot / (double)n) : 0.0f;
     }
@@ -192,7 +197,7 @@ hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const in
     return hipGetLastError();
 }
 hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t rows, void* misc, hipStream_t st) {
-    hipLaunchKernelGGL(logp_finish_kernel, dim3(1), dim3(256), 0, st, targets, logp, (long)rows,
+    hipLaunchKernelGGL(logp_finish_kernel, dim3(1), dim3(1024), 0, st, targets, logp, (long)rows,
                        static_cast<CeMisc*>(misc));
     return hipGetLastError();
 }

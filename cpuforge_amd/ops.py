@@ -294,25 +294,43 @@ def _result(t: torch.Tensor, words: int) -> int:
     return t.data_ptr()
 
 
-def lm_head_logprobs(hn, head, targets, t, d, vocab, logp, lse, result, ctx: Context | None = None) -> None:
+def lm_head_logprobs(hn, head, targets, t, d, vocab, logp, lse, result, keep=None, ctx: Context | None = None) -> None:
     """logits = hn . head^T (never held whole); lse [t] is their log-sum-exp and
     logp [t] the targets' logits less it, both 0 where the target is
     IGNORE_INDEX (all overwritten).  `result` (ce_result_buffer) gets the mean
     of -logp (ce_result_loss) and the first row whose target is out of range,
-    which ce_check reports; such a row's logp is NaN.  No host wait."""
+    which ce_check reports; such a row's logp is NaN.  `keep` (a uint8 tensor of
+    lm_head_logprobs_keep_bytes, when given) takes what the backward reads.  No
+    host wait."""
     ctx = ctx or default_context()
     _call(ctx, "cfops_lm_head_logprobs", _f32(hn, "hn", t * d), _f32(head, "head", vocab * d), _targets(targets, t),
-          t, d, vocab, _f32(logp, "logp", t), _f32(lse, "lse", t), _result(result, CE_RESULT_WORDS), _stream())
+          t, d, vocab, _f32(logp, "logp", t), _f32(lse, "lse", t), _result(result, CE_RESULT_WORDS), *_keep(keep),
+          _stream())
 
 
-def lm_head_logprobs_backward(hn, head, targets, lse, dlogp, t, d, vocab, dhn=None, dhead=None,
+def lm_head_logprobs_backward(hn, head, targets, lse, dlogp, t, d, vocab, dhn=None, dhead=None, keep=None,
                               ctx: Context | None = None) -> None:
-    """From the gradient dlogp of logp and the forward's lse: dhn (overwritten)
-    and dhead += dlogits^T . hn, each when given.  The logits are formed again."""
+    """From the gradient dlogp of logp: dhn (overwritten) and dhead +=
+    dlogits^T . hn, each when given.  hn, head, targets, lse and keep are the
+    forward's; without keep the logits are formed again."""
     ctx = ctx or default_context()
     _call(ctx, "cfops_lm_head_logprobs_backward", _f32(hn, "hn", t * d), _f32(head, "head", vocab * d),
           _targets(targets, t), _f32(lse, "lse", t), _f32(dlogp, "dlogp", t), t, d, vocab, _opt(dhn, "dhn", t * d),
-          _opt(dhead, "dhead", vocab * d), _stream())
+          _opt(dhead, "dhead", vocab * d), *_keep(keep), _stream())
+
+
+def _keep(keep):
+    if keep is None:
+        return None, 0
+    if not isinstance(keep, torch.Tensor) or not keep.is_cuda or keep.dtype != torch.uint8 or not keep.is_contiguous():
+        raise TypeError("keep must be a contiguous uint8 device tensor")
+    return keep.data_ptr(), keep.numel()
+
+
+def lm_head_logprobs_keep_bytes(t: int, d: int, vocab: int) -> int:
+    """Size of lm_head_logprobs' keep (about 4 t vocab + 4 d vocab bytes), 0
+    where it uses none."""
+    return _lib.lib().cfops_lm_head_logprobs_keep_bytes(int(t), int(d), int(vocab))
 
 
 # ------------------------------------------- losses over packed sequences

@@ -179,17 +179,24 @@ int cfops_adamw_update_multi(cfattn_ctx* ctx, size_t count, float* const* p, con
  * over the scored rows, result->bad_row names the first row whose target is
  * outside [0, vocab) (such a row's logp and lse are NaN), as
  * cfops_lm_head_ce_dev's does.  The logits are never held whole.  d and vocab
- * must be positive, t below 2^24. */
+ * must be positive, t below 2^24.
+ * `keep` (device memory of keep_bytes, 16-byte aligned, or NULL) takes what a
+ * backward reads, so that it need not form the logits again: a buffer of
+ * cfops_lm_head_logprobs_keep_bytes(t, d, vocab), about 4 t vocab + 4 d vocab
+ * bytes; where that is 0 (few rows) it is not used. */
+size_t cfops_lm_head_logprobs_keep_bytes(size_t t, size_t d, size_t vocab);
 int cfops_lm_head_logprobs(cfattn_ctx* ctx, const float* hn, const float* head, const int64_t* targets, size_t t,
-                           size_t d, size_t vocab, float* logp, float* lse, cfops_ce_result* result, void* stream);
-/* From the gradient dlogp [t] of logp, and lse as the forward wrote it: dhn
- * [t, d] (overwritten; NULL: not wanted) and, when dhead is non-null, dhead
- * [vocab, d] += dlogits^T . hn.  The logits are formed again.  Rows that are not
- * scored, or have a target out of range, have no gradient, and their hn, lse
- * and dlogp do not matter. */
+                           size_t d, size_t vocab, float* logp, float* lse, cfops_ce_result* result, void* keep,
+                           size_t keep_bytes, void* stream);
+/* From the gradient dlogp [t] of logp: dhn [t, d] (overwritten; NULL: not wanted)
+ * and, when dhead is non-null, dhead [vocab, d] += dlogits^T . hn.  hn, head,
+ * targets and lse are the forward's, and so is keep (NULL: the logits are formed
+ * again, a chunk of rows that fit cfops_set_head_chunk_limit at a time).  Rows
+ * that are not scored, or have a target out of range, have no gradient, and
+ * their hn, lse and dlogp do not matter. */
 int cfops_lm_head_logprobs_backward(cfattn_ctx* ctx, const float* hn, const float* head, const int64_t* targets,
                                     const float* lse, const float* dlogp, size_t t, size_t d, size_t vocab,
-                                    float* dhn, float* dhead, void* stream);
+                                    float* dhn, float* dhead, const void* keep, size_t keep_bytes, void* stream);
 
 /* Rows of packed sequences: sequence i is rows [offsets[i], offsets[i + 1]) of
  * logp (int64 in device memory, rising within [0, rows]).  A row whose target

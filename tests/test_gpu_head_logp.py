@@ -20,23 +20,35 @@ def inputs(t, d, vocab, seed, masked=0.3, std=None):
     return hn, head, tg, torch.randn(t, generator=g, device=DEV)
 
 
-def forward(hn, head, tg, check=True):
+def forward(hn, head, tg, check=True, keep=None):
     from cpuforge_amd import ops as P
     t, d = hn.shape
     logp, lse = (torch.full((t,), 77.0, device=DEV) for _ in range(2))
     res = P.ce_result_buffer(DEV)
-    P.lm_head_logprobs(hn, head, tg, t, d, head.shape[0], logp, lse, res)
+    P.lm_head_logprobs(hn, head, tg, t, d, head.shape[0], logp, lse, res, keep)
     if check:
         P.ce_check(res, tg, head.shape[0])
     return logp, lse, res
 
 
-def backward(hn, head, tg, lse, dlogp, want_head=True):
+def backward(hn, head, tg, lse, dlogp, want_head=True, keep=None):
     from cpuforge_amd import ops as P
     dhn = torch.full_like(hn, 77.0)
     dhead = torch.ones_like(head) if want_head else None
-    P.lm_head_logprobs_backward(hn, head, tg, lse, dlogp, *hn.shape, head.shape[0], dhn, dhead)
+    P.lm_head_logprobs_backward(hn, head, tg, lse, dlogp, *hn.shape, head.shape[0], dhn, dhead, keep)
     return dhn, dhead
+
+
+def kept(hn, head, tg):
+    """A keep buffer as the forward leaves it, of bytes that are no numbers before."""
+    from cpuforge_amd import ops as P
+    n = P.lm_head_logprobs_keep_bytes(*hn.shape, head.shape[0])
+    if n == 0:
+        return None
+    keep = torch.full((n + 64,), 255, dtype=torch.uint8, device=DEV)
+    forward(hn, head, tg, False, keep[:n])
+    assert bool((keep[n:] == 255).all())
+    return keep[:n]
 
 
 def reference(hn, head, tg, dlogp):
@@ -71,18 +83,20 @@ def check(hn, head, tg, dlogp):
     assert int(res[0]) == n and int(res[1]) == 2 ** 31 - 1
     mean = -float(w_logp.sum()) / max(n, 1)
     assert abs(float(res.view(torch.float32)[2]) - mean) <= float(tol2.max()) + 2.0 ** -23 * abs(mean)
-    dhn, dhead = backward(hn, head, tg, lse, dlogp)
     # exp(x - lse): the errors of both, the difference's rounding and exp's, on
     # every dlogit; then products of 22-bit operands in f32 sums.
     p = dx.abs() + torch.zeros_like(dx).scatter_(1, tg.clamp(min=0)[:, None], 1.0) * (dlogp.abs() * use).double()[:, None]
     rel = (off + tol + U * (spread + 8))[:, None] + 2.0 ** -21 + U * vocab ** 0.5
     floor = 2.0 ** -36 * dlogp.abs().double()[:, None] * use[:, None]  # dlogits below their row's 2^-36
     e = p * rel + floor
-    assert bool(((dhn - w_dhn).abs() <= e @ head.abs().double() + 1e-37).all()), (dhn - w_dhn).abs().max()
-    assert not dhn[~use].any()
+    tol_n = e @ head.abs().double() + 1e-37
     tol_h = e.T @ hn.abs().double() + 2.0 ** -24 * (1 + w_dhead.abs()) + U * hn.shape[0] ** 0.5 * (p.T @ hn.abs().double())
-    assert bool(((dhead - 1 - w_dhead).abs() <= tol_h + 1e-37).all()), (dhead - 1 - w_dhead).abs().max()
-    assert torch.equal(backward(hn, head, tg, lse, dlogp, False)[0], dhn)
+    for keep in (None, kept(hn, head, tg)):
+        dhn, dhead = backward(hn, head, tg, lse, dlogp, keep=keep)
+        assert bool(((dhn - w_dhn).abs() <= tol_n).all()), (dhn - w_dhn).abs().max()
+        assert not dhn[~use].any()
+        assert bool(((dhead - 1 - w_dhead).abs() <= tol_h + 1e-37).all()), (dhead - 1 - w_dhead).abs().max()
+        assert torch.equal(backward(hn, head, tg, lse, dlogp, False, keep)[0], dhn)
 
 
 SHAPES = [(1, 1, 1), (1, 64, 5), (3, 7, 130), (1, 576, 4097), (5, 576, 2000), (16, 100, 1000), (17, 576, 1000),
@@ -192,6 +206,17 @@ def test_refusals():
         P.lm_head_logprobs(hn.half(), head, tg, 4, 8, 10, x, x, res)
     with pytest.raises(ValueError):
         P.lm_head_logprobs(hn, head.T.contiguous().T, tg, 4, 8, 10, x, x, res)
+    n = P.lm_head_logprobs_keep_bytes(300, 8, 10)
+    assert P.lm_head_logprobs_keep_bytes(4, 8, 10) == 0 and P.lm_head_logprobs_keep_bytes(300, 0, 10) == 0
+    big, tg3 = torch.zeros(300, 8, device=DEV), torch.zeros(300, dtype=torch.int64, device=DEV)
+    keep, y = torch.zeros(n + 16, dtype=torch.uint8, device=DEV), torch.zeros(300, device=DEV)
+    for bad, what in ((keep[:n - 1], "needed"), (keep[1:], "aligned")):
+        with pytest.raises(_lib.CfattnError, match=what):
+            P.lm_head_logprobs(big, head, tg3, 300, 8, 10, y, y, res, bad)
+        with pytest.raises(_lib.CfattnError, match=what):
+            P.lm_head_logprobs_backward(big, head, tg3, y, y, 300, 8, 10, big, None, bad)
+    with pytest.raises(TypeError):
+        P.lm_head_logprobs(big, head, tg3, 300, 8, 10, y, y, res, keep.float())
     with pytest.raises(_lib.CfattnError, match="positive"):
         P.lm_head_logprobs(hn[:, :0].contiguous(), head[:, :0].contiguous(), tg, 4, 0, 10, x, x, res)
 
@@ -257,11 +282,26 @@ def test_autograd():
     assert logp.shape == (4, 15) and not res.requires_grad
     dh, dw = torch.autograd.grad(logp, (h3, w), g.view(4, 15))
     _, lse, _ = forward(hn, head, tg)
-    want = backward(hn, head, tg, lse, g)
+    want = backward(hn, head, tg, lse, g, keep=kept(hn, head, tg))
     assert torch.equal(dh.view(60, 48), want[0])
     assert bool(((dw - (want[1] - 1)).abs() <= 2.0 ** -22 * (1 + dw.abs())).all())
     (only,) = torch.autograd.grad(A.lm_head_logprobs(h3.detach(), w, tg.view(4, 15))[0], w, g.view(4, 15))
     assert torch.equal(only, dw)
+
+
+def test_autograd_keeps_up_to_its_limit(monkeypatch):
+    """With and without what the forward keeps: the same gradients to f32 sums in
+    another order; a second backward of one graph gives the first one's."""
+    from cpuforge_amd import autograd as A
+    hn, head, tg, g = inputs(700, 96, 2000, 17)
+    hn.requires_grad_()
+    logp, _ = A.lm_head_logprobs(hn, head, tg)
+    (a,) = torch.autograd.grad(logp, hn, g, retain_graph=True)
+    (b,) = torch.autograd.grad(logp, hn, g)
+    assert torch.equal(a, b)
+    monkeypatch.setattr(A, "LOGPROBS_KEEP_LIMIT", 1000)
+    (c,) = torch.autograd.grad(A.lm_head_logprobs(hn, head, tg)[0], hn, g)
+    assert bool(((a - c).abs() <= 2.0 ** -20 * a.abs().max()).all())
 
 
 def test_against_differences():
