@@ -109,7 +109,7 @@ SIGNATURES = {
                                  + [C.c_float] * 4 + [_vp]),
     "cfops_lm_head_logprobs_keep_bytes": (_sz, [_sz] * 3),
     "cfops_lm_head_logprobs": (C.c_int, [_vp] * 4 + [_sz] * 3 + [_vp] * 4 + [_sz, _vp]),
-    "cfops_lm_head_logprobs_backward": (C.c_int, [_vp] * 6 + [_sz] * 3 + [_vp] * 3 + [_sz, _vp]),
+    "cfops_lm_head_logprobs_backward": (C.c_int, [_vp] * 6 + [_sz] * 3 + [_vp] * 2 + [C.c_int, _vp, _sz, _vp]),
     "cfops_preference_loss": (C.c_int, [_vp] * 4 + [_sz, _vp, _sz, C.c_int] + [C.c_double] * 3 + [C.c_int]
                               + [_vp] * 4),
     "cfops_policy_loss": (C.c_int, [_vp] * 6 + [_sz, _vp, _sz, C.c_int] + [C.c_double] * 3 + [C.c_int] + [_vp] * 3),

@@ -218,9 +218,9 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         if g is None or not (need_hn or need_head):
             return None, None, None
         dhn = torch.empty_like(h2) if need_hn else None
-        dhead = torch.zeros_like(head) if need_head else None
+        dhead = torch.empty_like(head) if need_head else None
         P.lm_head_logprobs_backward(h2, head, tg, lse, g.contiguous().view(-1), h2.shape[0], h2.shape[1],
-                                    head.shape[0], dhn, dhead, keep)
+                                    head.shape[0], dhn, dhead, keep, acc=False)
         return None if dhn is None else dhn.view(ctx.shape), dhead, None
 
 

@@ -600,7 +600,7 @@ int logprobs_many(cfattn_ctx* c, const float* hn, const float* head, const int64
 
 int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets,
                            const float* dlogp, size_t t, size_t d, size_t vocab, float* dhn, float* dhead,
-                           const void* keep, size_t keep_bytes, hipStream_t st) {
+                           bool acc, const void* keep, size_t keep_bytes, hipStream_t st) {
     const cfattn::HeadPlan p = cfattn::head_plan(t, d, vocab, keep ? SIZE_MAX : c->head_chunk_bytes);
     cfattn::HeadBuffers b{};
     if (keep) {
@@ -613,19 +613,30 @@ int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, co
         b.factor = reinterpret_cast<float*>(b.back + p.back_bytes);
         CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, b.idx, b.count, nullptr, nullptr, nullptr, st),
                "log-probability launch");
-        CF_HIP(c, cfattn::launch_head_pack(p, b, hn, head, d, vocab, st), "log-probability launch");
     }
+    // The head's gradient goes through dlogits that fit the head's limit.
+    const size_t pass =
+        std::min(p.chunk, std::max<size_t>(c->head_chunk_bytes / (p.v_pad * sizeof(float)) / 128 * 128, 128));
+    char* dlogits = nullptr;
+    unsigned* col_top = nullptr;
+    if (dhead) {
+        CF_TRY(take(c, cfattn_ctx::OPS_DLOGITS, pass * p.v_pad * sizeof(float) + vocab * sizeof(unsigned), dlogits));
+        col_top = reinterpret_cast<unsigned*>(dlogits + pass * p.v_pad * sizeof(float));
+        char* rows = nullptr;
+        CF_TRY(take(c, cfattn_ctx::OPS_ROWS_BACK, p.rows_back_bytes + p.t_pad * sizeof(float), rows));
+        b.rows_back = rows;
+        if (keep) {
+            // (A pack of the rows alone; their exponents come out the same.)
+            b.scale = reinterpret_cast<float*>(rows + p.rows_back_bytes);
+            cfattn::HeadBuffers only = b;
+            only.back = nullptr;
+            CF_HIP(c, cfattn::launch_head_pack(p, only, hn, nullptr, d, vocab, st), "log-probability launch");
+        }
+    }
+    if (!keep) CF_HIP(c, cfattn::launch_head_pack(p, b, hn, head, d, vocab, st), "log-probability launch");
     if (dhn) {
         CF_TRY(take(c, cfattn_ctx::OPS_PART, p.part_bytes, b.part));
         CF_HIP(c, cfattn::launch_head_zero_rows(targets, t, vocab, dhn, d, st), "log-probability launch");
-    }
-    // The head's gradient is an f32 product over dlogits that fit the head's limit.
-    const size_t pass = std::min(p.chunk, std::max<size_t>(c->head_chunk_bytes / (vocab * sizeof(float)) / 128 * 128, 128));
-    float *dlogits = nullptr, *gathered = nullptr;
-    if (dhead) {
-        CF_TRY(take(c, cfattn_ctx::OPS_DLOGITS, (pass * vocab + t * d) * sizeof(float), dlogits));
-        gathered = dlogits + pass * vocab;
-        CF_HIP(c, cfattn::launch_logp_gather(hn, b.idx, b.count, gathered, t, d, st), "log-probability launch");
     }
     for (size_t j0 = 0; j0 < t; j0 += p.chunk) {
         if (!keep)
@@ -633,12 +644,10 @@ int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, co
                    "log-probability launch");
         if (dhn)
             CF_HIP(c, cfattn::launch_head_dhn(p, b, targets, head, dlogp, j0, d, dhn, st), "log-probability launch");
-        for (size_t i = 0; dhead && i < p.chunk && j0 + i < t; i += pass) {
-            const size_t nr = std::min({t - j0 - i, p.chunk - i, pass});
-            CF_HIP(c, cfattn::launch_head_dlogits(p, b, targets, dlogp, j0, i, nr, vocab, dlogits, st),
+        for (size_t i = 0; dhead && i < p.chunk && j0 + i < t; i += pass)
+            CF_HIP(c, cfattn::launch_head_dhead(p, b, targets, dlogp, j0, i, std::min({t - j0 - i, p.chunk - i, pass}),
+                                                d, vocab, dlogits, col_top, dhead, acc || j0 + i, st),
                    "log-probability launch");
-            CF_TRY(gemm(c, CFOPS_TN, dlogits, gathered + (j0 + i) * d, dhead, vocab, nr, d, true, st));
-        }
     }
     return CFATTN_OK;
 }
@@ -721,14 +730,17 @@ int cfops_lm_head_logprobs(cfattn_ctx* c, const float* hn, const float* head, co
 
 int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets,
                                     const float* lse, const float* dlogp, size_t t, size_t d, size_t vocab,
-                                    float* dhn, float* dhead, const void* keep, size_t keep_bytes, void* stream) {
+                                    float* dhn, float* dhead, int acc, const void* keep, size_t keep_bytes,
+                                    void* stream) {
     CF_LOCK(c, stream);
     CF_TRY(check_logprobs(c, t, d, vocab));
+    if (t == 0 && !acc) return zero_grad(c, dhead, vocab * d, to_stream(stream));
     if (t == 0 || (!dhn && !dhead)) return CFATTN_OK;
     if (!hn || !head || !targets || !lse || !dlogp) return fail(c, CFATTN_ERR_ARG, "null buffer");
     const hipStream_t st = to_stream(stream);
     if (t >= kHeadRows)
-        return logprobs_backward_many(c, hn, head, targets, dlogp, t, d, vocab, dhn, dhead, keep, keep_bytes, st);
+        return logprobs_backward_many(c, hn, head, targets, dlogp, t, d, vocab, dhn, dhead, acc != 0, keep, keep_bytes,
+                                      st);
     LogpRows rows{};
     CF_TRY(logp_rows(c, t, d, vocab, rows));
     CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, nullptr, nullptr, nullptr, st),
@@ -741,7 +753,7 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
         CF_HIP(c, cfattn::launch_logp_grad_rows(rows.logits, targets, rows.idx, rows.count, lse, dlogp, j0, nr, vocab,
                                                 st),
                "log-probability launch");
-        if (dhead) CF_TRY(gemm(c, CFOPS_TN, rows.logits, h, dhead, vocab, nr, d, true, st));
+        if (dhead) CF_TRY(gemm(c, CFOPS_TN, rows.logits, h, dhead, vocab, nr, d, acc || j0, st));
         if (dhn) CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, h, nr, vocab, d, false, st));
     }
     if (dhn)

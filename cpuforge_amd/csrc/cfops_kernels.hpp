@@ -203,22 +203,23 @@ hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t 
 // in registers.  A plan holds the sizes of the buffers, of which rows are in
 // chunks: those of stats, xt, keep and factor begin at the chunk's first scored row.
 //   pack:      rows, scale, packed and exponents, and with back non-null also that
-//              and count[1] (which select has reset);
+//              and count[1] (which select has reset); with rows_back non-null that
+//              too; with head null only what is of rows (rows may be null then);
 //   stats:     logp and lse (or null) of scored rows [j0, j0 + chunk), j0 a
 //              multiple of chunk; with keep non-null (and back packed) also that and
 //              factor, from which
 //   dhn:       their rows of dhn, and
-//   dlogits:   dlogits [rows][vocab] of those of them from `local` (a multiple of
-//              128) on, zeros behind the last scored one;
+//   dhead:     what `rows` of them from `local` (a multiple of 128) on add to dhead
+//              (acc 0: give as dhead), in scratch of up(rows, 32) v_pad 4 bytes and vocab words;
 //   zero_rows: dhn of the rows that are not scored.
 struct HeadPlan {
     int k16, splits_max;  // 16-k steps of a row
     size_t t_pad, v_pad, d_pad, chunk;
-    size_t rows_bytes, head_bytes, back_bytes, stats_bytes, keep_bytes, factor_bytes, part_bytes;
+    size_t rows_bytes, head_bytes, back_bytes, stats_bytes, keep_bytes, factor_bytes, rows_back_bytes, part_bytes;
 };
 struct HeadBuffers {
     int *idx, *count, *exponents;        // [t], [2], [v_pad / 32]
-    char *rows, *packed, *back, *keep;   // operands
+    char *rows, *packed, *back, *keep, *rows_back;  // operands
     float *scale, *xt, *factor, *part;   // scale [t_pad], xt [chunk]
     void* stats;
 };
@@ -229,8 +230,9 @@ hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, const int6
                              float* logp, float* lse, hipStream_t st);
 hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* head,
                            const float* dlogp, size_t j0, size_t d, float* dhn, hipStream_t st);
-hipError_t launch_head_dlogits(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* dlogp,
-                               size_t j0, size_t local, size_t rows, size_t vocab, float* dlogits, hipStream_t st);
+hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* dlogp,
+                             size_t j0, size_t local, size_t rows, size_t d, size_t vocab, char* packed_dlogits,
+                             unsigned* col_top, float* dhead, int acc, hipStream_t st);
 hipError_t launch_head_zero_rows(const int64_t* targets, size_t t, size_t vocab, float* dhn, size_t d,
                                  hipStream_t st);
 

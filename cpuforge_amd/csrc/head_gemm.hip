@@ -34,6 +34,7 @@
 #include <type_traits>
 
 #include "cfattn_common.hpp"
+#include "cfattn_kernels.hpp"
 #include "cfops_kernels.hpp"
 
 namespace cfattn {
@@ -96,17 +97,17 @@ __device__ __forceinline__ void load8(float (&x)[8], const float* row, int k, in
 struct PackArgs {
     const float *hn, *head;
     const int *idx, *count;
-    char *rows, *packed, *back;
+    char *rows, *packed, *back, *rows_back;  // rows and rows_back may be null
     float* scale;
     int *exponents, *largest;
-    int row_blocks, vocab, d, k16, v16, vec_rows, vec_head;
+    int row_blocks, vocab, d, k16, v16, t16, vec_rows, vec_head;
 };
 
 // 32 rows to a workgroup, as operands [32 rows][16 k][piece]: first the scored rows
 // of hn, each with its own 2^e, zeros from row n on; then the head's, with one e,
-// and, for the hidden states' gradient, whose k are these rows, as [32 columns][16
-// rows][piece] too.  There lane l holds column l % 32 and of 16 rows those that it
-// holds of a product's 32 x 32 result: 4 (l / 32) + 0..3 and the same eight on.
+// and, for the gradients, whose k are these rows, as [32 columns][16 rows][piece]
+// too.  There lane l holds column l % 32 and of 16 rows those that it holds of a
+// product's 32 x 32 result: 4 (l / 32) + 0..3 and the same eight on.
 // A wave takes the pairs of operands (32 columns) w, w + NW, ..; with U > 0 at most U
 // of them, which stay in registers between the largest value and the pieces.
 // Bound by HBM: 128256 x 2048 411 us, 5.1 TB/s of one read and one write.  (Read
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(64 * NW) void pack_kernel(const PackArgs g) {
 #pragma unroll
         for (int q = 0; q < 2; q++) {
             const Pieces p = split8(y[q], sc);
-            if (2 * s + q < k16) store_pieces(out + ((long)blk * k16 + 2 * s + q) * 2 * kFrag, lane, p);
+            if (out && 2 * s + q < k16) store_pieces(out + ((long)blk * k16 + 2 * s + q) * 2 * kFrag, lane, p);
             if constexpr (BACK)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
@@ -187,7 +188,9 @@ __global__ __launch_bounds__(64 * NW) void pack_kernel(const PackArgs g) {
                 }
         }
         if constexpr (BACK) {
-            if (!is_head) return;
+            char* to = is_head ? g.back : g.rows_back;
+            if (!to) return;
+            const int steps = is_head ? g.v16 : g.t16;
             // (A wave's own part of LDS: its own order of accesses is enough.)
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -199,7 +202,7 @@ __global__ __launch_bounds__(64 * NW) void pack_kernel(const PackArgs g) {
                     p.h[i] = __builtin_bit_cast(_Float16, (uint16_t)u);
                     p.l[i] = __builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
                 }
-                store_pieces(g.back + ((long)s * g.v16 + blk * 2 + q) * 2 * kFrag, lane, p);
+                store_pieces(to + ((long)s * steps + blk * 2 + q) * 2 * kFrag, lane, p);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -216,10 +219,14 @@ __global__ __launch_bounds__(64 * NW) void pack_kernel(const PackArgs g) {
     }
 }
 
+enum class Product { kStats, kRows, kHead };
+
 struct HeadArgs {
-    const char *a, *b;  // operands: rows of the result along a (64 MB to a tile), tokens along b
-    int k16;            // 16-k steps of an operand
-    int mt;             // tiles along a
+    // Operands: rows of the result along a (64 MB to a tile), columns (kBN) along b: the
+    // scored rows, or (head) the columns of the head.
+    const char *a, *b;
+    int ka, kb;         // 16-k steps from one 32 rows of a (of b) to the next
+    int mt, nt;         // tiles along a, and (head) along b
     const int* count;   // scored rows
     int j0, chunk;      // this launch's: [j0, min(j0 + chunk, count)); b, stats, keep and part start at j0
     long ld;            // of stats, xt and factor
@@ -231,10 +238,14 @@ struct HeadArgs {
     float2* stats;      // [128 rows of the head][ld]: max and sum of exp2, in log2 units
     float* xt;          // the targets' logits
     char* keep;         // [32 tokens][v16][piece], or null
-    // gradient: a is the head by columns, b what statistics kept
+    // the rows' gradient: a is the head by columns, b what statistics kept
     const float* factor;  // [128 rows of the head][ld]
     float* part;          // [split][chunk][64 MB mt]
     int splits_max;
+    // the head's gradient: a is the dlogits by columns, b the rows by columns
+    const unsigned* col_top;  // [vocab]: a bound of the dlogits of a column, as f32 bits
+    float* dhead;
+    int d, acc;         // acc: added to dhead, else written
 };
 
 // Splits of the gradient's k (the vocabulary) over workgroups: a multiple of the
@@ -252,39 +263,40 @@ __device__ __forceinline__ int splits_of(int tiles, int k16, int splits_max) {
     return best;
 }
 
-// A tile of 64 MB rows and kBN tokens to a workgroup of four waves, each 32 MB x 64;
+// A tile of 64 MB rows and kBN columns to a workgroup of four waves, each 32 MB x 64;
 // two workgroups to a CU: one's epilogue runs beside the other's products.
-template <int MB, bool GRAD>
+template <int MB, Product P>
 __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
-    constexpr int BM = 64 * MB, CH = 4 * MB + 8, PER = CH / 4 + GRAD, STAGE = CH * kFrag + GRAD * 1024;
+    constexpr bool ROWS = P == Product::kRows;
+    constexpr int BM = 64 * MB, CH = 4 * MB + 8, PER = CH / 4 + ROWS, STAGE = CH * kFrag + ROWS * 1024;
     static_assert(CH % 4 == 0, "whole loads a wave");
     __shared__ __attribute__((aligned(1024))) char lds[kStages * STAGE];
     const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1, l32 = lane & 31, hh = lane >> 5;
-    const int n = min(wave_uniform(*g.count) - g.j0, g.chunk);
-    if (n <= 0) return;
-    const int nt = (n + kBN - 1) / kBN;
+    const int n = max(min(wave_uniform(*g.count) - g.j0, g.chunk), 0);
+    if (n == 0 && !(P == Product::kHead && !g.acc)) return;
+    const int nt = P == Product::kHead ? g.nt : (n + kBN - 1) / kBN;
     // Items of an XCD: a contiguous run of the tiles along a (of the splits), every
-    // token tile with each.
+    // tile along b with each.
     const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
     int outer = g.mt, inner = nt;
-    if constexpr (GRAD) {
-        outer = wave_uniform(splits_of(g.mt * nt, g.k16, g.splits_max));
+    if constexpr (ROWS) {
+        outer = wave_uniform(splits_of(g.mt * nt, g.ka, g.splits_max));
         inner = g.mt * nt;
     }
     const int o0 = (int)((long)outer * xcd / 8), o1 = (int)((long)outer * (xcd + 1) / 8);
     const uint32_t lds0 = lds_offset(lds), voff = lane * 16;
     for (int item = local; item < (o1 - o0) * inner; item += kWgs / 8) {
-        // Statistics: kGroup token tiles with every tile along a of the XCD, then the
-        // next ones: what 64 workgroups read at a time is near a square.
-        int o, tm, tt, k0 = 0, k1 = g.k16;
-        if constexpr (GRAD) {
+        // Without splits: kGroup tiles along b with every tile along a of the XCD, then
+        // the next ones: what 64 workgroups read at a time is near a square.
+        int o, tm, tt, k0 = 0, k1 = P == Product::kHead ? (n + 15) / 16 : g.ka;
+        if constexpr (ROWS) {
             o = wave_uniform(o0 + item / inner);
             tm = wave_uniform(item % inner % g.mt);
             tt = wave_uniform(item % inner / g.mt);
             // (Whole runs of 128 rows of the head.)
-            k0 = wave_uniform((int)((long)(g.k16 / 8) * o / outer) * 8);
-            k1 = wave_uniform((int)((long)(g.k16 / 8) * (o + 1) / outer) * 8);
+            k0 = wave_uniform((int)((long)(g.ka / 8) * o / outer) * 8);
+            k1 = wave_uniform((int)((long)(g.ka / 8) * (o + 1) / outer) * 8);
         } else {
             const int grp = item / ((o1 - o0) * kGroup), left = item - grp * (o1 - o0) * kGroup;
             const int w = min(kGroup, nt - grp * kGroup);
@@ -296,11 +308,11 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
         for (int i = 0; i < CH / 4; i++) {
             const int c = CH / 4 * wave + i;  // the stage's KiB: operand c / 2, piece c % 2
             const int blk = c / 2;
-            const char* base = blk < 2 * MB ? g.a + ((long)(tm * 2 * MB + blk) * g.k16 + k0) * 2 * kFrag
-                                            : g.b + ((long)(tt * 4 + blk - 2 * MB) * g.k16 + k0) * 2 * kFrag;
+            const char* base = blk < 2 * MB ? g.a + ((long)(tm * 2 * MB + blk) * g.ka + k0) * 2 * kFrag
+                                            : g.b + ((long)(tt * 4 + blk - 2 * MB) * g.kb + k0) * 2 * kFrag;
             src[i] = base + (c % 2) * kFrag;
         }
-        const int col0 = tt * kBN + wn * 64;  // this wave's first token
+        const int col0 = tt * kBN + wn * 64;  // this wave's first column
         int kl = k0;                          // the next stage's k
         auto load = [&](uint32_t stage) {
 #pragma unroll
@@ -308,17 +320,17 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
                 lds_load16_so(src[i], voff, lds0 + stage + (CH / 4 * wave + i) * kFrag);
                 src[i] += 2 * kFrag;
             }
-            if constexpr (GRAD) {
+            if constexpr (ROWS) {
                 // The factors of the stage's 128 rows for the wave's tokens.
                 lds_load4_so(g.factor + (long)(kl / 8) * g.ld + col0, lane * 4, lds0 + stage + CH * kFrag + wave * 256);
                 kl++;
             }
         };
-        f32x16 acc[MB][2], tot[GRAD ? MB : 1][2];
+        f32x16 acc[MB][2], tot[ROWS ? MB : 1][2];
 #pragma unroll
         for (int i = 0; i < MB; i++) {
             acc[i][0] = acc[i][1] = zero16();
-            if constexpr (GRAD) tot[i][0] = tot[i][1] = zero16();
+            if constexpr (ROWS) tot[i][0] = tot[i][1] = zero16();
         }
         // Every wave is done with the LDS of the item before, and with its stores
         // (they would count among the loads waited for below).
@@ -356,7 +368,7 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
 #pragma unroll
                     for (int j = 0; j < 2; j++)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][pa[q]], b[j][pb[q]], acc[i][j], 0, 0, 0);
-            if constexpr (GRAD) {
+            if constexpr (ROWS) {
                 if (k % 8 != 7) continue;
                 const float* f = reinterpret_cast<const float*>(s + CH * kFrag + wave * 256);
 #pragma unroll
@@ -373,7 +385,35 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
         }
 
         const int m0 = tm * BM + wm * 32 * MB;  // this wave's first row
-        if constexpr (GRAD) {
+        if constexpr (P == Product::kHead) {
+#pragma unroll
+            for (int i = 0; i < MB; i++) {
+                const int v0 = m0 + 32 * i + 4 * hh;
+                float u[16];
+#pragma unroll
+                for (int q = 0; q < 16; q++) {
+                    const int v = min(v0 + 8 * (q >> 2) + (q & 3), g.vocab - 1);
+                    u[q] = exp2i(group_exponent(__builtin_bit_cast(float, g.col_top[v])));
+                }
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int col = col0 + 32 * j + l32;
+                    float* out = g.dhead + (long)v0 * g.d + col;
+                    float old[16];
+                    // (All reads before the first write: they are in flight together.)
+#pragma unroll
+                    for (int q = 0; q < 16; q++) {
+                        const int r = 8 * (q >> 2) + (q & 3);
+                        old[q] = g.acc && col < g.d && v0 + r < g.vocab ? out[(long)r * g.d] : 0.0f;
+                    }
+#pragma unroll
+                    for (int q = 0; q < 16; q++) {
+                        const int r = 8 * (q >> 2) + (q & 3);
+                        if (col < g.d && v0 + r < g.vocab) out[(long)r * g.d] = fmaf(acc[i][j][q], u[q], old[q]);
+                    }
+                }
+            }
+        } else if constexpr (ROWS) {
             const int rows = g.mt * BM;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
@@ -525,49 +565,90 @@ __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __re
     }
 }
 
-// dlogits [rows][vocab] of scored rows [j0, ..) from what statistics kept, zeros
-// from row n on: 32 rows and 128 columns to a workgroup, through LDS, so that
-// rows are written 512 bytes at a time.
-__global__ __launch_bounds__(256) void head_dlogits_kernel(const char* __restrict__ keep, int v16,
-                                                           const float* __restrict__ factor, long ld,
-                                                           const int* __restrict__ exponents,
-                                                           const int* __restrict__ largest,
-                                                           const int* __restrict__ idx,
-                                                           const int* __restrict__ count, int j0, int chunk, int nr,
-                                                           const int64_t* __restrict__ targets,
-                                                           const float* __restrict__ dlogp,
-                                                           float* __restrict__ dlogits, long vocab) {
-    __shared__ float tile[32][129];
-    __shared__ float grad[32];
-    __shared__ int target[32];
+// What the head's gradient takes of what statistics kept, for scored rows [j0, ..).
+struct DlogitsArgs {
+    const char* keep;     // from row j0 on
+    const float* factor;
+    const int *exponents, *largest, *idx, *count;
+    const int64_t* targets;
+    const float *dlogp, *scale;
+    unsigned* col_top;
+    char* out;            // [32 columns][t16][piece]
+    long ld;
+    int v16, t16, j0, chunk, vocab;
+};
+
+// A bound of every column's dlogits times their rows' 2^e: a column's power of two is
+// its own, since a token that is rarely likely has gradients far below the others',
+// which an optimizer that divides by their size scales up.  From the upper pieces
+// (f16, to 2^-11): 128 columns and every 8th 32 rows to a workgroup.
+__global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
-    const int n = min(*count - j0, chunk), t0 = blockIdx.y * 32;
-    const long v0 = (long)blockIdx.x * 128;
-    if (threadIdx.x < 32) {
-        const bool scored = t0 + (int)threadIdx.x < n;
-        const long r = scored ? idx[j0 + t0 + threadIdx.x] : 0;
-        grad[threadIdx.x] = scored ? dlogp[r] : 0.0f;
-        target[threadIdx.x] = scored ? (int)targets[r] : -1;
-    }
-    if (t0 < n) {
-        const float f = t0 + l32 < n ? factor[blockIdx.x * ld + t0 + l32] : 0.0f;
+    const int n = min(*g.count - g.j0, g.chunk);
+    float top[2][8] = {};
+    const float u = pow2_clamped(*g.largest - g.exponents[blockIdx.x * 4 + wave] - 15);
+    for (int t0 = 32 * blockIdx.y; t0 < n; t0 += 32 * gridDim.y) {
+        const int j = t0 + l32;
+        if (j >= n) continue;
+        const float row = fabsf(g.dlogp[g.idx[g.j0 + j]]) * g.scale[g.j0 + j];
+        const float f = g.factor[blockIdx.x * g.ld + j] * u * row;
 #pragma unroll
         for (int q = 0; q < 2; q++) {
-            const int s = 2 * wave + q;  // 16 columns
-            const char* p = keep + ((long)blockIdx.y * v16 + blockIdx.x * 8 + s) * 2 * kFrag + lane * 16;
-            const f16x8 h = *reinterpret_cast<const f16x8*>(p), l = *reinterpret_cast<const f16x8*>(p + kFrag);
-            const float u = f * pow2_clamped(*largest - exponents[blockIdx.x * 4 + wave] - 15);
+            const f16x8 h = *reinterpret_cast<const f16x8*>(
+                g.keep + ((long)(t0 / 32) * g.v16 + blockIdx.x * 8 + 2 * wave + q) * 2 * kFrag + lane * 16);
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                tile[l32][16 * s + 8 * (i >> 2) + 4 * hh + (i & 3)] = ((float)h[i] + (float)l[i]) * u;
+            for (int i = 0; i < 8; i++) top[q][i] = fmaxf(top[q][i], finite_abs((float)h[i] * f));
+        }
+        // (One workgroup of the columns sees to a row's target.)
+        if (blockIdx.x == 0 && wave == 0 && hh == 0)
+            atomicMax(g.col_top + g.targets[g.idx[g.j0 + j]], __builtin_bit_cast(unsigned, finite_abs(row)));
+    }
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float x = top[q][i];
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+            const int v = blockIdx.x * 128 + 16 * (2 * wave + q) + 8 * (i >> 2) + 4 * hh + (i & 3);
+            if (l32 == 0 && v < g.vocab) atomicMax(g.col_top + v, __builtin_bit_cast(unsigned, x));
+        }
+}
+
+// The dlogits times their rows' 2^e as operands by columns: 32 rows and 128 columns
+// to a workgroup, turned round in LDS.
+__global__ __launch_bounds__(256) void head_pack_dlogits_kernel(const DlogitsArgs g) {
+    __shared__ float tile[32][129];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
+    const int n = min(*g.count - g.j0, g.chunk), t0 = blockIdx.y * 32, j = t0 + l32;
+    if (t0 >= n) return;
+    const bool scored = j < n;
+    const long r = scored ? g.idx[g.j0 + j] : 0;
+    const float row = scored ? g.dlogp[r] * g.scale[g.j0 + j] : 0.0f;
+    const float f = scored ? g.factor[blockIdx.x * g.ld + j] * pow2_clamped(*g.largest - g.exponents[blockIdx.x * 4 + wave] - 15) : 0.0f;
+    const int target = scored ? (int)g.targets[r] - (int)blockIdx.x * 128 : -1;
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+        const int s = 2 * wave + q;  // 16 columns
+        const char* p = g.keep + ((long)blockIdx.y * g.v16 + blockIdx.x * 8 + s) * 2 * kFrag + lane * 16;
+        const f16x8 h = *reinterpret_cast<const f16x8*>(p), l = *reinterpret_cast<const f16x8*>(p + kFrag);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int c = 16 * s + 8 * (i >> 2) + 4 * hh + (i & 3);
+            // (Rows from n on are zeros, whatever their factor.)
+            tile[l32][c] = scored ? row * ((c == target ? 1.0f : 0.0f) - ((float)h[i] + (float)l[i]) * f) : 0.0f;
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * 128; i += 256) {
-        const int r = i >> 7, c = i & 127;
-        if (t0 + r >= nr || v0 + c >= vocab) continue;
-        const float p = t0 + r < n ? tile[r][c] : 0.0f;
-        dlogits[(t0 + r) * vocab + v0 + c] = t0 + r < n ? grad[r] * ((v0 + c == target[r]) - p) : 0.0f;
+    const int v = blockIdx.x * 128 + 32 * wave + l32;
+    const float sc = exp2i(-group_exponent(v < g.vocab ? __builtin_bit_cast(float, g.col_top[v]) : 0.0f));
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = tile[16 * q + 8 * (i >> 2) + 4 * hh + (i & 3)][32 * wave + l32];
+        store_pieces(g.out + ((long)(blockIdx.x * 4 + wave) * g.t16 + blockIdx.y * 2 + q) * 2 * kFrag, lane,
+                     split8(x, sc));
     }
 }
 
@@ -605,6 +686,7 @@ HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes) {
     p.stats_bytes = (p.v_pad / 128) * p.chunk * sizeof(float2);
     p.keep_bytes = p.chunk * p.v_pad * 4;
     p.factor_bytes = (p.v_pad / 128) * p.chunk * sizeof(float);
+    p.rows_back_bytes = up(d, kBN) * p.t_pad * 4;
     p.part_bytes = (size_t)p.splits_max * p.chunk * p.d_pad * sizeof(float);
     return p;
 }
@@ -613,14 +695,16 @@ hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float
                             size_t vocab, hipStream_t st) {
     PackArgs g{};
     g.hn = hn, g.head = head, g.idx = b.idx, g.count = b.count, g.rows = b.rows, g.packed = b.packed, g.back = b.back;
+    g.rows_back = b.rows_back, g.t16 = (int)(p.t_pad / 16);
     g.scale = b.scale, g.exponents = b.exponents, g.largest = b.count + 1, g.row_blocks = (int)(p.t_pad / 32);
     g.vocab = (int)vocab, g.d = (int)d, g.k16 = p.k16, g.v16 = (int)(p.v_pad / 16);
     g.vec_rows = d % 4 == 0 && aligned16(hn), g.vec_head = d % 4 == 0 && aligned16(head);
+    const size_t blocks = (p.t_pad + (head ? p.v_pad : 0)) / 32;
     const int pairs = (p.k16 + 1) / 2;
     auto pack = [&](auto back, auto nw, auto u) {
         constexpr int kNw = decltype(nw)::value;
         hipLaunchKernelGGL((pack_kernel<decltype(back)::value, kNw, decltype(u)::value>),
-                           dim3((unsigned)((p.t_pad + p.v_pad) / 32)), dim3(64 * kNw), 0, st, g);
+                           dim3((unsigned)blocks), dim3(64 * kNw), 0, st, g);
     };
     using std::integral_constant;
     auto sized = [&](auto back) {
@@ -634,7 +718,7 @@ hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float
         else
             pack(back, integral_constant<int, 8>{}, integral_constant<int, 0>{});
     };
-    if (b.back)
+    if (b.back || b.rows_back)
         sized(std::true_type{});
     else
         sized(std::false_type{});
@@ -644,11 +728,11 @@ hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float
 hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, size_t j0, size_t vocab,
                              float* logp, float* lse, hipStream_t st) {
     HeadArgs g{};
-    g.a = b.packed, g.b = b.rows + j0 / 32 * p.k16 * 2 * kFrag, g.k16 = p.k16, g.mt = (int)(p.v_pad / 256);
+    g.a = b.packed, g.b = b.rows + j0 / 32 * p.k16 * 2 * kFrag, g.ka = g.kb = p.k16, g.mt = (int)(p.v_pad / 256);
     g.count = b.count, g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.exponents = b.exponents;
     g.largest = b.count + 1, g.idx = b.idx, g.scale = b.scale, g.targets = targets, g.vocab = (int)vocab;
     g.v16 = (int)(p.v_pad / 16), g.stats = static_cast<float2*>(b.stats), g.xt = b.xt, g.keep = b.keep;
-    hipLaunchKernelGGL((head_gemm_kernel<4, false>), dim3(kWgs), dim3(256), 0, st, g);
+    hipLaunchKernelGGL((head_gemm_kernel<4, Product::kStats>), dim3(kWgs), dim3(256), 0, st, g);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)(p.chunk / 16)), dim3(1024), 0, st, g.stats, g.ld,
@@ -661,28 +745,41 @@ hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, const int64_
                            const float* dlogp, size_t j0, size_t d, float* dhn, hipStream_t st) {
     const int mb = back_mb(d);
     HeadArgs g{};
-    g.a = b.back, g.b = b.keep, g.k16 = (int)(p.v_pad / 16), g.mt = (int)(p.d_pad / (64 * mb)), g.count = b.count;
+    g.a = b.back, g.b = b.keep, g.ka = g.kb = (int)(p.v_pad / 16), g.mt = (int)(p.d_pad / (64 * mb)), g.count = b.count;
     g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.factor = b.factor, g.part = b.part;
     g.splits_max = p.splits_max;
     if (mb == 3)
-        hipLaunchKernelGGL((head_gemm_kernel<3, true>), dim3(kWgs), dim3(256), 0, st, g);
+        hipLaunchKernelGGL((head_gemm_kernel<3, Product::kRows>), dim3(kWgs), dim3(256), 0, st, g);
     else
-        hipLaunchKernelGGL((head_gemm_kernel<2, true>), dim3(kWgs), dim3(256), 0, st, g);
+        hipLaunchKernelGGL((head_gemm_kernel<2, Product::kRows>), dim3(kWgs), dim3(256), 0, st, g);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(head_grad_reduce_kernel, dim3((unsigned)p.chunk), dim3(256), 0, st, b.part, (int)p.chunk,
-                       (int)p.d_pad, g.mt, g.k16, g.splits_max, b.idx, b.count, (int)j0, targets, head, dlogp,
+                       (int)p.d_pad, g.mt, g.ka, g.splits_max, b.idx, b.count, (int)j0, targets, head, dlogp,
                        b.count + 1, dhn, (int)d);
     return hipGetLastError();
 }
 
-hipError_t launch_head_dlogits(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* dlogp,
-                               size_t j0, size_t local, size_t rows, size_t vocab, float* dlogits, hipStream_t st) {
-    // (Rows [local, local + rows) of those that statistics kept from row j0 on.)
-    hipLaunchKernelGGL(head_dlogits_kernel, dim3((unsigned)((vocab + 127) / 128), (unsigned)((rows + 31) / 32)),
-                       dim3(256), 0, st, b.keep + local * p.v_pad * 4, (int)(p.v_pad / 16), b.factor + local,
-                       (long)p.chunk, b.exponents, b.count + 1, b.idx, b.count, (int)(j0 + local), (int)rows,
-                       (int)rows, targets, dlogp, dlogits, (long)vocab);
+hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* dlogp,
+                             size_t j0, size_t local, size_t rows, size_t d, size_t vocab, char* packed_dlogits,
+                             unsigned* col_top, float* dhead, int acc, hipStream_t st) {
+    DlogitsArgs g{};
+    g.keep = b.keep + local * p.v_pad * 4, g.factor = b.factor + local, g.exponents = b.exponents;
+    g.largest = b.count + 1, g.idx = b.idx, g.count = b.count, g.targets = targets, g.dlogp = dlogp;
+    g.scale = b.scale, g.col_top = col_top, g.out = packed_dlogits, g.ld = (long)p.chunk, g.v16 = (int)(p.v_pad / 16);
+    g.t16 = (int)(up(rows, 32) / 16), g.j0 = (int)(j0 + local), g.chunk = (int)rows, g.vocab = (int)vocab;
+    hipError_t e = launch_fill_zero(reinterpret_cast<float*>(col_top), vocab, st);
+    if (e != hipSuccess) return e;
+    const unsigned t32 = (unsigned)((rows + 31) / 32), v128 = (unsigned)(p.v_pad / 128);
+    hipLaunchKernelGGL(head_col_top_kernel, dim3(v128, std::min(t32, 8u)), dim3(256), 0, st, g);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    hipLaunchKernelGGL(head_pack_dlogits_kernel, dim3(v128, t32), dim3(256), 0, st, g);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    HeadArgs h{};
+    h.a = packed_dlogits, h.b = b.rows_back + (j0 + local) / 16 * 2 * kFrag, h.ka = g.t16, h.kb = (int)(p.t_pad / 16);
+    h.mt = (int)(p.v_pad / 256), h.nt = (int)((d + kBN - 1) / kBN), h.count = b.count, h.j0 = g.j0, h.chunk = g.chunk;
+    h.vocab = (int)vocab, h.col_top = col_top, h.dhead = dhead, h.d = (int)d, h.acc = acc;
+    hipLaunchKernelGGL((head_gemm_kernel<4, Product::kHead>), dim3(kWgs), dim3(256), 0, st, h);
     return hipGetLastError();
 }
 

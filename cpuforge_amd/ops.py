@@ -309,14 +309,14 @@ def lm_head_logprobs(hn, head, targets, t, d, vocab, logp, lse, result, keep=Non
 
 
 def lm_head_logprobs_backward(hn, head, targets, lse, dlogp, t, d, vocab, dhn=None, dhead=None, keep=None,
-                              ctx: Context | None = None) -> None:
+                              ctx: Context | None = None, acc: bool = True) -> None:
     """From the gradient dlogp of logp: dhn (overwritten) and dhead +=
-    dlogits^T . hn, each when given.  hn, head, targets, lse and keep are the
+    dlogits^T . hn (acc=False: overwritten), each when given.  hn, head, targets, lse and keep are the
     forward's; without keep the logits are formed again."""
     ctx = ctx or default_context()
     _call(ctx, "cfops_lm_head_logprobs_backward", _f32(hn, "hn", t * d), _f32(head, "head", vocab * d),
           _targets(targets, t), _f32(lse, "lse", t), _f32(dlogp, "dlogp", t), t, d, vocab, _opt(dhn, "dhn", t * d),
-          _opt(dhead, "dhead", vocab * d), *_keep(keep), _stream())
+          _opt(dhead, "dhead", vocab * d), int(acc), *_keep(keep), _stream())
 
 
 def _keep(keep):

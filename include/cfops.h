@@ -189,14 +189,15 @@ int cfops_lm_head_logprobs(cfattn_ctx* ctx, const float* hn, const float* head, 
                            size_t d, size_t vocab, float* logp, float* lse, cfops_ce_result* result, void* keep,
                            size_t keep_bytes, void* stream);
 /* From the gradient dlogp [t] of logp: dhn [t, d] (overwritten; NULL: not wanted)
- * and, when dhead is non-null, dhead [vocab, d] += dlogits^T . hn.  hn, head,
- * targets and lse are the forward's, and so is keep (NULL: the logits are formed
+ * and, when dhead is non-null, dhead [vocab, d] += dlogits^T . hn (acc == 0: =).
+ * hn, head, targets and lse are the forward's, and so is keep (NULL: the logits are formed
  * again, a chunk of rows that fit cfops_set_head_chunk_limit at a time).  Rows
  * that are not scored, or have a target out of range, have no gradient, and
  * their hn, lse and dlogp do not matter. */
 int cfops_lm_head_logprobs_backward(cfattn_ctx* ctx, const float* hn, const float* head, const int64_t* targets,
                                     const float* lse, const float* dlogp, size_t t, size_t d, size_t vocab,
-                                    float* dhn, float* dhead, const void* keep, size_t keep_bytes, void* stream);
+                                    float* dhn, float* dhead, int acc, const void* keep, size_t keep_bytes,
+                                    void* stream);
 
 /* Rows of packed sequences: sequence i is rows [offsets[i], offsets[i + 1]) of
  * logp (int64 in device memory, rising within [0, rows]).  A row whose target

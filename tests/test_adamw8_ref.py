@@ -48,7 +48,7 @@ def test_state_bytes():
 def test_null_contexts_are_refused():
     L = _lib.lib()
     assert L.cfops_lm_head_logprobs(None, None, None, None, 1, 1, 1, None, None, None, None, 0, None) == _lib.ERR_ARG
-    assert L.cfops_lm_head_logprobs_backward(None, None, None, None, None, None, 1, 1, 1, None, None, None, 0,
+    assert L.cfops_lm_head_logprobs_backward(None, None, None, None, None, None, 1, 1, 1, None, None, 1, None, 0,
                                              None) == _lib.ERR_ARG
     assert L.cfops_preference_loss(None, None, None, None, 1, None, 1, 0, 0.1, 0.0, 0.0, 0, None, None, None,
                                    None) == _lib.ERR_ARG

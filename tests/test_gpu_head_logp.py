@@ -31,11 +31,11 @@ def forward(hn, head, tg, check=True, keep=None):
     return logp, lse, res
 
 
-def backward(hn, head, tg, lse, dlogp, want_head=True, keep=None):
+def backward(hn, head, tg, lse, dlogp, want_head=True, keep=None, acc=True):
     from cpuforge_amd import ops as P
     dhn = torch.full_like(hn, 77.0)
     dhead = torch.ones_like(head) if want_head else None
-    P.lm_head_logprobs_backward(hn, head, tg, lse, dlogp, *hn.shape, head.shape[0], dhn, dhead, keep)
+    P.lm_head_logprobs_backward(hn, head, tg, lse, dlogp, *hn.shape, head.shape[0], dhn, dhead, keep, acc=acc)
     return dhn, dhead
 
 
@@ -97,6 +97,8 @@ def check(hn, head, tg, dlogp):
         assert not dhn[~use].any()
         assert bool(((dhead - 1 - w_dhead).abs() <= tol_h + 1e-37).all()), (dhead - 1 - w_dhead).abs().max()
         assert torch.equal(backward(hn, head, tg, lse, dlogp, False, keep)[0], dhn)
+        over = backward(hn, head, tg, lse, dlogp, True, keep, acc=False)[1]  # over ones
+        assert bool(((over - w_dhead).abs() <= tol_h + 1e-37).all())
 
 
 SHAPES = [(1, 1, 1), (1, 64, 5), (3, 7, 130), (1, 576, 4097), (5, 576, 2000), (16, 100, 1000), (17, 576, 1000),
@@ -187,6 +189,8 @@ def test_no_rows():
     dhead = torch.ones_like(head)
     P.lm_head_logprobs_backward(e, head, tg, e, e, 0, 4, 10, e, dhead)
     assert bool((dhead == 1).all())
+    P.lm_head_logprobs_backward(e, head, tg, e, e, 0, 4, 10, e, dhead, acc=False)
+    assert not dhead.any()
 
 
 def test_refusals():
@@ -284,7 +288,7 @@ def test_autograd():
     _, lse, _ = forward(hn, head, tg)
     want = backward(hn, head, tg, lse, g, keep=kept(hn, head, tg))
     assert torch.equal(dh.view(60, 48), want[0])
-    assert bool(((dw - (want[1] - 1)).abs() <= 2.0 ** -22 * (1 + dw.abs())).all())
+    assert torch.equal(dw, backward(hn, head, tg, lse, g, keep=kept(hn, head, tg), acc=False)[1])
     (only,) = torch.autograd.grad(A.lm_head_logprobs(h3.detach(), w, tg.view(4, 15))[0], w, g.view(4, 15))
     assert torch.equal(only, dw)
 
