@@ -63,14 +63,16 @@ __device__ __forceinline__ double decode_v(uint32_t c, double unit) {
     return c == 0xff ? __builtin_inf() : (double)code_unit(c) * unit;
 }
 
-// The code of magnitude a; `least` is E's biased exponent of the first normal
-// binade and `low` its power of two.  r: 17 bits, the rounding threshold.  In the
-// high word of a double lie its exponent, the three mantissa bits of a code and
-// the 17 below them.  Below the first normal binade the steps are that binade's:
-// the sum with its power of two has them.
-__device__ __forceinline__ uint32_t encode(double a, uint32_t least, double low, uint32_t r) {
-    const bool normal = hi_word(a) >> 20 >= least;
-    const uint32_t u = (hi_word(normal ? a : a + low) + r) >> 17;
+// The code of the magnitude whose high word is `hi`; `least` is the biased exponent
+// of the first normal binade.  r: 17 bits, the rounding threshold.  In the high word
+// of a double lie its exponent, the three mantissa bits of a code and the 17 below
+// them; what lies below those can carry nothing into the code.  Below the first
+// normal binade the steps are that binade's: the sum with its power of two has them.
+__device__ __forceinline__ uint32_t encode(uint32_t hi, uint32_t least, uint32_t r) {
+    const bool normal = hi >> 20 >= least;
+    const double a = __builtin_bit_cast(double, (uint64_t)hi << 32);
+    const double low = __builtin_bit_cast(double, (uint64_t)(least << 20) << 32);
+    const uint32_t u = ((normal ? hi : hi_word(a + low)) + r) >> 17;
     return u - (least << 3) + (normal ? 8 : 0);
 }
 
@@ -131,34 +133,34 @@ __device__ __forceinline__ void store4(float* p, long i, long n, bool vec, const
     if (i + 3 < n) p[i + 3] = x.w;
 }
 
-// Codes of a block's 16 values of this lane, four to a word.
-__device__ __forceinline__ void encode_block(const double (&m)[16], const double (&v)[16], const uint32_t (&r)[16],
+// Codes of a block's 16 values of this lane, four to a word, from their high words
+// (m with its sign); threshold(e) are the 32 bits of value e.
+template <typename F>
+__device__ __forceinline__ void encode_block(const uint32_t (&m)[16], const uint32_t (&v)[16], F threshold,
                                              uint32_t (&cm)[4], uint32_t (&cv)[4], int& em, int& ev) {
     uint32_t tm = 0, tv = 0;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-        const uint32_t hm = hi_word(m[e]) & 0x7fffffff, hv = hi_word(v[e]) & 0x7fffffff;
+        const uint32_t hm = m[e] & 0x7fffffff;
         tm = max(tm, odd(hm) ? 0u : hm);
-        tv = max(tv, odd(hv) ? 0u : hv);
+        tv = max(tv, odd(v[e]) ? 0u : v[e]);
     }
     em = exponent_byte(max16(tm));
     ev = exponent_byte(max16(tv));
     // Biased exponents of the first normal binades: E - 13 and E - 29.
     const uint32_t lm = (uint32_t)(em - 127 - 13 + 1023), lv = (uint32_t)(ev - 127 - 29 + 1023);
-    const double wm = pow2(em - 127 - 13), wv = pow2(ev - 127 - 29);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         cm[j] = cv[j] = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int e = 4 * j + k;
-            const uint32_t hm = hi_word(m[e]);
-            uint32_t c = odd(hm) ? 0x7fu : encode(__builtin_fabs(m[e]), lm, wm, r[e] & 0x1ffff);
-            c |= (hm >> 31) << 7;
+            const uint32_t r = threshold(e), hm = m[e] & 0x7fffffff;
+            uint32_t c = odd(hm) ? 0x7fu : encode(hm, lm, r & 0x1ffff);
+            c |= (m[e] >> 31) << 7;
             cm[j] |= c << (8 * k);
-            c = odd(hi_word(v[e])) ? 0xffu : encode(__builtin_fabs(v[e]), lv, wv, r[e] >> 15);
-            if (v[e] != 0.0) c = max(c, 1u);
-            cv[j] |= c << (8 * k);
+            c = odd(v[e]) ? 0xffu : encode(v[e], lv, r >> 15);
+            cv[j] |= max(c, v[e] ? 1u : 0u) << (8 * k);
         }
     }
 }
@@ -199,24 +201,31 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Adamw8Args a) {
     }
     const double um = pow2(s.em[b] + kUnitM), uv = pow2(s.ev[b] + kUnitV);
     const double b1 = a.beta1, b2 = a.beta2, d1 = ob1, d2 = ob2;
-    double m[16], v[16];
-    uint32_t r[16];
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-        const uint32_t km = cm[e / 4] >> (8 * (e % 4)) & 0xff, kv = cv[e / 4] >> (8 * (e % 4)) & 0xff;
-        const double gd = g[e];
-        m[e] = fma(d1, gd, b1 * decode_m(km, um));
-        v[e] = fma(d2 * gd, gd, b2 * decode_v(kv, uv));
-        const float mf = (float)m[e], vf = (float)v[e];
-        const float upd = mf * a.c1 / (sqrtf(vf) * a.c2 + a.eps) + t.weight_decay * p[e];
-        p[e] -= a.lr * upd;
-        r[e] = mix((uint32_t)(i0 + 64 * (e / 4) + e % 4) + a.key);
-    }
-    int em, ev;
-    encode_block(m, v, r, cm, cv, em, ev);
+    uint32_t m[16], v[16];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int e = 4 * j + k;
+            const double gd = g[e];
+            const double md = fma(d1, gd, b1 * decode_m(cm[j] >> (8 * k) & 0xff, um));
+            const double vd = fma(d2 * gd, gd, b2 * decode_v(cv[j] >> (8 * k) & 0xff, uv));
+            const float mf = (float)md, vf = (float)vd;
+            // (The instructions' square root and reciprocal, to a step of f32: what they are
+            // off by is 2^-23 of an update that is itself a thousandth of p or less.)
+            const float den = fmaf(__builtin_amdgcn_sqrtf(vf), a.c2, a.eps);
+            const float upd = fmaf(mf * a.c1, __builtin_amdgcn_rcpf(den), t.weight_decay * p[e]);
+            p[e] = fmaf(-a.lr, upd, p[e]);
+            m[e] = hi_word(md);
+            v[e] = hi_word(vd) & 0x7fffffff;
+        }
         store4(t.p, i0 + 64 * j, t.n, t.vec, make_float4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]));
+    }
+    int em, ev;
+    encode_block(
+        m, v, [&](int e) { return mix((uint32_t)(i0 + 64 * (e / 4) + e % 4) + a.key); }, cm, cv, em, ev);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
         *reinterpret_cast<uint32_t*>(s.m + i0 + 64 * j) = cm[j];
         *reinterpret_cast<uint32_t*>(s.v + i0 + 64 * j) = cv[j];
     }
@@ -236,18 +245,20 @@ __global__ __launch_bounds__(256) void adamw8_convert_kernel(const Adamw8Args a)
     const long i0 = b * 256 + 4 * (threadIdx.x % 16);
     uint32_t cm[4], cv[4];
     if constexpr (PACK) {
-        double m[16], v[16];
-        uint32_t r[16];
+        uint32_t m[16], v[16];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const float4 x = load4(t.m, i0 + 64 * j, t.n, t.vec), y = load4(t.v, i0 + 64 * j, t.n, t.vec);
-            m[4 * j] = x.x, m[4 * j + 1] = x.y, m[4 * j + 2] = x.z, m[4 * j + 3] = x.w;
-            v[4 * j] = y.x, v[4 * j + 1] = y.y, v[4 * j + 2] = y.z, v[4 * j + 3] = y.w;
+            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int k = 0; k < 4; k++) r[4 * j + k] = 1u << 16 | 1u << 31;
+            for (int k = 0; k < 4; k++) {
+                m[4 * j + k] = hi_word((double)xs[k]);
+                v[4 * j + k] = hi_word((double)ys[k]) & 0x7fffffff;
+            }
         }
         int em, ev;
-        encode_block(m, v, r, cm, cv, em, ev);
+        encode_block(
+            m, v, [](int) { return 1u << 16 | 1u << 31; }, cm, cv, em, ev);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             *reinterpret_cast<uint32_t*>(s.m + i0 + 64 * j) = cm[j];
