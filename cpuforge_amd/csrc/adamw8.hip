@@ -34,6 +34,11 @@ namespace {
 
 constexpr int kBlock = 4096;  // values of a workgroup: 16 blocks, one to 16 lanes
 
+template <int N>
+struct Args : Adamw8Step {
+    Adamw8Tensor t[N];
+};
+
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // The layout of a state of n values: codes of m and of v, a byte for every value
@@ -100,7 +105,8 @@ __device__ __forceinline__ uint32_t mix(uint32_t x) {
 }
 
 // The tensor that workgroup b falls in.
-__device__ __forceinline__ const Adamw8Tensor& find(const Adamw8Args& a, long b) {
+template <int N>
+__device__ __forceinline__ const Adamw8Tensor& find(const Args<N>& a, long b) {
     int lo = 0, hi = a.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -165,7 +171,8 @@ __device__ __forceinline__ void encode_block(const uint32_t (&m)[16], const uint
     }
 }
 
-__global__ __launch_bounds__(256) void adamw8_kernel(const Adamw8Args a) {
+template <int N>
+__global__ __launch_bounds__(256) void adamw8_kernel(const Args<N> a) {
     const Adamw8Tensor& t = find(a, blockIdx.x);
     const long e0 = ((long)blockIdx.x - t.block0) * kBlock;
     const float ob1 = 1.0f - a.beta1, ob2 = 1.0f - a.beta2;
@@ -236,8 +243,8 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Adamw8Args a) {
 }
 
 // f32 moments into an 8-bit state, each to the nearest of its steps, and back.
-template <bool PACK>
-__global__ __launch_bounds__(256) void adamw8_convert_kernel(const Adamw8Args a) {
+template <int N, bool PACK>
+__global__ __launch_bounds__(256) void adamw8_convert_kernel(const Args<N> a) {
     const Adamw8Tensor& t = find(a, blockIdx.x);
     const long b = ((long)blockIdx.x - t.block0) * (kBlock / 256) + threadIdx.x / 16;
     if (b * 256 >= t.n) return;
@@ -299,10 +306,22 @@ uint32_t adamw8_key(uint64_t t) {
     return mix32((uint32_t)t * 0x9E3779B1u + 0x7F4A7C15u);
 }
 
-hipError_t launch_adamw8(Adamw8Args a, Adamw8Op op, hipStream_t st) {
+template <int N>
+static hipError_t launch(const Adamw8Tensor* t, const Adamw8Step& step, Adamw8Op op, unsigned blocks, hipStream_t st) {
+    Args<N> a;
+    static_cast<Adamw8Step&>(a) = step;
+    std::copy(t, t + step.count, a.t);
+    const auto kernel = op == Adamw8Op::kUpdate ? adamw8_kernel<N>
+                        : op == Adamw8Op::kPack ? adamw8_convert_kernel<N, true>
+                                                : adamw8_convert_kernel<N, false>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_adamw8(Adamw8Tensor* tensors, const Adamw8Step& step, Adamw8Op op, hipStream_t st) {
     long blocks = 0;
-    for (int i = 0; i < a.count; i++) {
-        Adamw8Tensor& t = a.t[i];
+    for (int i = 0; i < step.count; i++) {
+        Adamw8Tensor& t = tensors[i];
         const bool pg = op != Adamw8Op::kUpdate || (aligned16(t.p) && aligned16(t.g));
         const bool mv = (op == Adamw8Op::kUpdate && t.state8) || (aligned16(t.m) && aligned16(t.v));
         t.vec = pg && mv;
@@ -311,11 +330,8 @@ hipError_t launch_adamw8(Adamw8Args a, Adamw8Op op, hipStream_t st) {
     }
     if (blocks == 0) return hipSuccess;
     if (blocks > 0xffffffL) return hipErrorInvalidConfiguration;  // fewer than 2^32 threads
-    const auto kernel = op == Adamw8Op::kUpdate ? adamw8_kernel
-                        : op == Adamw8Op::kPack ? adamw8_convert_kernel<true>
-                                                : adamw8_convert_kernel<false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
-    return hipGetLastError();
+    return step.count <= kAdamw8Few ? launch<kAdamw8Few>(tensors, step, op, (unsigned)blocks, st)
+                                    : launch<kAdamw8Batch>(tensors, step, op, (unsigned)blocks, st);
 }
 
 }  // namespace cfattn

@@ -104,12 +104,12 @@ bool adamw_overlaps(const cfattn::AdamwArgs& a) {
     return overlaps(r, n);
 }
 
-bool adamw8_overlaps(const cfattn::Adamw8Args& a, cfattn::Adamw8Op op) {
+bool adamw8_overlaps(const cfattn::Adamw8Tensor* ts, int count, cfattn::Adamw8Op op) {
     using cfattn::Adamw8Op;
     Range r[4 * cfattn::kAdamw8Batch];
     int n = 0;
-    for (int i = 0; i < a.count; i++) {
-        const cfattn::Adamw8Tensor& t = a.t[i];
+    for (int i = 0; i < count; i++) {
+        const cfattn::Adamw8Tensor& t = ts[i];
         const size_t bytes = (size_t)t.n * sizeof(float);
         if (t.state8) r[n++] = range(t.state8, cfattn::adamw8_state_bytes((size_t)t.n), op != Adamw8Op::kUnpack);
         if (op == Adamw8Op::kUpdate) {
@@ -660,7 +660,7 @@ int check_sequences(cfattn_ctx* c, size_t rows, size_t seqs) {
 }
 
 int adamw8_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors, cfattn::Adamw8Op op,
-                 cfattn::Adamw8Args& a, hipStream_t st) {
+                 cfattn::Adamw8Step step, hipStream_t st) {
     using cfattn::Adamw8Op;
     if (count && !tensors) return fail(c, CFATTN_ERR_ARG, "null array");
     for (size_t i = 0; i < count; i++) {
@@ -672,21 +672,18 @@ int adamw8_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors,
         if (reinterpret_cast<uintptr_t>(x.state8) % 16)
             return fail(c, CFATTN_ERR_ARG, "state8 must be 16-byte aligned");
     }
-    a.count = 0;
+    cfattn::Adamw8Tensor batch[cfattn::kAdamw8Batch];
+    int n = 0;
     for (size_t i = 0; i < count; i++) {
         const cfops_adamw_tensor& x = tensors[i];
         if (x.n && (op == Adamw8Op::kUpdate || x.state8))
-            a.t[a.count++] = {x.p, x.g, x.m, x.v, x.state8, (long)x.n, x.weight_decay, 0, 0};
-        if (a.count == cfattn::kAdamw8Batch || (i + 1 == count && a.count)) {
+            batch[n++] = {x.p, x.g, x.m, x.v, x.state8, (long)x.n, x.weight_decay, 0, 0};
+        if (n == cfattn::kAdamw8Batch || (i + 1 == count && n)) {
             // Tensors of one launch are updated side by side.
-            const int step = adamw8_overlaps(a, op) ? 1 : a.count;
-            for (int k = 0; k < a.count; k += step) {
-                cfattn::Adamw8Args b = a;
-                std::copy(a.t + k, a.t + k + step, b.t);
-                b.count = step;
-                CF_HIP(c, cfattn::launch_adamw8(b, op, st), "adamw launch");
-            }
-            a.count = 0;
+            step.count = n > 1 && adamw8_overlaps(batch, n, op) ? 1 : n;
+            for (int k = 0; k < n; k += step.count)
+                CF_HIP(c, cfattn::launch_adamw8(batch + k, step, op, st), "adamw launch");
+            n = 0;
         }
     }
     return CFATTN_OK;
@@ -822,7 +819,7 @@ size_t cfops_adamw8_state_bytes(size_t n) { return cfattn::adamw8_state_bytes(n)
 int cfops_adamw8_update_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors, uint64_t t, float lr,
                               float beta1, float beta2, float eps, void* stream) {
     CF_LOCK(c, stream);
-    cfattn::Adamw8Args a{};
+    cfattn::Adamw8Step a{};
     a.lr = lr, a.beta1 = beta1, a.beta2 = beta2, a.eps = eps;
     a.bc1 = 1.0f - powi_f32(beta1, (int)(int32_t)t);
     a.bc2 = 1.0f - powi_f32(beta2, (int)(int32_t)t);
@@ -834,14 +831,12 @@ int cfops_adamw8_update_multi(cfattn_ctx* c, size_t count, const cfops_adamw_ten
 
 int cfops_adamw8_pack_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors, void* stream) {
     CF_LOCK(c, stream);
-    cfattn::Adamw8Args a{};
-    return adamw8_multi(c, count, tensors, cfattn::Adamw8Op::kPack, a, to_stream(stream));
+    return adamw8_multi(c, count, tensors, cfattn::Adamw8Op::kPack, {}, to_stream(stream));
 }
 
 int cfops_adamw8_unpack_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors, void* stream) {
     CF_LOCK(c, stream);
-    cfattn::Adamw8Args a{};
-    return adamw8_multi(c, count, tensors, cfattn::Adamw8Op::kUnpack, a, to_stream(stream));
+    return adamw8_multi(c, count, tensors, cfattn::Adamw8Op::kUnpack, {}, to_stream(stream));
 }
 
 }  // extern "C"

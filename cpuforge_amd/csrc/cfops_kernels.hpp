@@ -117,7 +117,10 @@ hipError_t launch_lora_grad(const LoraGrad& g, hipStream_t st);
 // AdamW over tensors whose moments are held in 8 bits (state8) or 32 (m, v)
 // (adamw8.hip); none empty.  Update reads and writes p and the state; pack and
 // unpack convert between m, v and state8.
-constexpr int kAdamw8Batch = 60;
+// A launch takes up to kAdamw8Batch tensors as arguments (28 KiB of them; SmolLM-135M's
+// 420 adapters in batches of 60, 240 and 448: 89, 49 and 41 us), or up to
+// kAdamw8Few, which are a microsecond less to pass.
+constexpr int kAdamw8Batch = 448, kAdamw8Few = 16;
 struct Adamw8Tensor {
     float* p;
     const float* g;
@@ -128,8 +131,7 @@ struct Adamw8Tensor {
     int vec;      // set by launch_adamw8, as block0
     long block0;
 };
-struct Adamw8Args {
-    Adamw8Tensor t[kAdamw8Batch];
+struct Adamw8Step {
     int count;
     float lr, beta1, beta2, eps, bc1, bc2;  // 32-bit states, as AdamwArgs
     float c1, c2;                           // 1 / bc1, 1 / sqrt(bc2)
@@ -138,7 +140,7 @@ struct Adamw8Args {
 enum class Adamw8Op { kUpdate, kPack, kUnpack };
 size_t adamw8_state_bytes(size_t n);
 uint32_t adamw8_key(uint64_t t);
-hipError_t launch_adamw8(Adamw8Args a, Adamw8Op op, hipStream_t st);
+hipError_t launch_adamw8(Adamw8Tensor* t, const Adamw8Step& step, Adamw8Op op, hipStream_t st);
 
 // Losses over packed sequences (seq_loss.hip); at least one pair or sequence.
 struct PreferenceResult {
