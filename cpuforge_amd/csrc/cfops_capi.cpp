@@ -514,9 +514,6 @@ int check_logprobs(cfattn_ctx* c, size_t t, size_t d, size_t vocab) {
     return CFATTN_OK;
 }
 
-// From how many rows on the log-probabilities' products run on packed operands.
-constexpr size_t kHeadRows = 64;
-
 // Scratch of the log-probabilities of few rows: the scored rows, their hidden
 // states (in the backward over them their gradients), and the logits of a chunk.
 struct LogpRows {
@@ -692,7 +689,7 @@ int adamw8_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors,
 }  // namespace
 
 size_t cfops_lm_head_logprobs_keep_bytes(size_t t, size_t d, size_t vocab) {
-    if (t < kHeadRows || t >= (size_t)1 << 24 || d == 0 || vocab == 0 || !fits_int(d) || !fits_int(vocab)) return 0;
+    if (t <= cfattn::kLogpFew || t >= (size_t)1 << 24 || d == 0 || vocab == 0 || !fits_int(d) || !fits_int(vocab)) return 0;
     return keep_layout(cfattn::head_plan(t, d, vocab, SIZE_MAX), t).bytes;
 }
 
@@ -704,23 +701,18 @@ int cfops_lm_head_logprobs(cfattn_ctx* c, const float* hn, const float* head, co
     CF_TRY(check_logprobs(c, t, d, vocab));
     if (!head || (t && (!hn || !targets || !logp || !lse))) return fail(c, CFATTN_ERR_ARG, "null buffer");
     const hipStream_t st = to_stream(stream);
-    if (t >= kHeadRows) {
-        CF_TRY(logprobs_many(c, hn, head, targets, t, d, vocab, logp, lse, result, keep, keep_bytes, st));
-        CF_HIP(c, cfattn::launch_logp_finish(targets, logp, t, result, st), "log-probability launch");
+    if (t == 0) {
+        CF_HIP(c, cfattn::launch_ce_begin(targets, 0, result, st), "log-probability launch");
         return CFATTN_OK;
     }
-    LogpRows rows{};
-    CF_TRY(logp_rows(c, t, d, vocab, rows));
-    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, logp, lse, result, st),
-           "log-probability launch");
-    if (t == 0) return CFATTN_OK;
-    CF_HIP(c, cfattn::launch_logp_gather(hn, rows.idx, rows.count, rows.hn, t, d, st), "log-probability launch");
-    for (size_t j0 = 0; j0 < t; j0 += rows.chunk) {
-        const size_t nr = std::min(t - j0, rows.chunk);
-        CF_TRY(gemm(c, CFOPS_NT, rows.hn + j0 * d, head, rows.logits, nr, d, vocab, false, st));
-        CF_HIP(c, cfattn::launch_logp_rows(rows.logits, targets, rows.idx, rows.count, logp, lse, j0, nr, vocab, st),
+    if (t <= cfattn::kLogpFew) {
+        char* scratch = nullptr;
+        CF_TRY(take(c, cfattn_ctx::OPS_STATS, cfattn::logp_few_bytes(t, vocab), scratch));
+        CF_HIP(c, cfattn::launch_logp_few(hn, head, targets, t, d, vocab, logp, lse, result, scratch, st),
                "log-probability launch");
+        return CFATTN_OK;
     }
+    CF_TRY(logprobs_many(c, hn, head, targets, t, d, vocab, logp, lse, result, keep, keep_bytes, st));
     CF_HIP(c, cfattn::launch_logp_finish(targets, logp, t, result, st), "log-probability launch");
     return CFATTN_OK;
 }
@@ -735,7 +727,7 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
     if (t == 0 || (!dhn && !dhead)) return CFATTN_OK;
     if (!hn || !head || !targets || !lse || !dlogp) return fail(c, CFATTN_ERR_ARG, "null buffer");
     const hipStream_t st = to_stream(stream);
-    if (t >= kHeadRows)
+    if (t > cfattn::kLogpFew)
         return logprobs_backward_many(c, hn, head, targets, dlogp, t, d, vocab, dhn, dhead, acc != 0, keep, keep_bytes,
                                       st);
     LogpRows rows{};

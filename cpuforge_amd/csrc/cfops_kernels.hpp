@@ -118,7 +118,7 @@ hipError_t launch_lora_grad(const LoraGrad& g, hipStream_t st);
 // (adamw8.hip); none empty.  Update reads and writes p and the state; pack and
 // unpack convert between m, v and state8.
 // A launch takes up to kAdamw8Batch tensors as arguments (28 KiB of them; SmolLM-135M's
-// 420 adapters in batches of 60, 240 and 448: 89, 49 and 41 us), or up to
+// 420 adapters in batches of 60, 240 and 448: 89, 45 and 39 us), or up to
 // kAdamw8Few, which are a microsecond less to pass.
 constexpr int kAdamw8Batch = 448, kAdamw8Few = 16;
 struct Adamw8Tensor {
@@ -186,20 +186,24 @@ hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st);
 //   select:    idx, count[0], INT_MIN in count[1], the result block (CeMisc; or
 //              null), and logp and lse (or null) of the rows that are not scored;
 //   gather:    the scored rows of hn side by side;   scatter: back, other rows 0;
-//   rows:      logp and lse;   grad_rows: the logits become their gradients;
-//   finish:    the mean of -logp, summed in f64 in row order.
+//   grad_rows: the logits become their gradients;
+//   finish:    the mean of -logp, summed in f64 in a fixed order.
 hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, float* logp,
                               float* lse, void* misc, hipStream_t st);
 hipError_t launch_logp_gather(const float* hn, const int* idx, const int* count, float* out, size_t rows, size_t d,
                               hipStream_t st);
 hipError_t launch_logp_scatter(const float* in, const int* idx, const int* count, float* dhn, size_t rows, size_t d,
                                hipStream_t st);
-hipError_t launch_logp_rows(const float* logits, const int64_t* targets, const int* idx, const int* count, float* logp,
-                            float* lse, size_t j0, size_t nrows, size_t vocab, hipStream_t st);
 hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const int* idx, const int* count,
                                  const float* lse, const float* dlogp, size_t j0, size_t nrows, size_t vocab,
                                  hipStream_t st);
 hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t rows, void* misc, hipStream_t st);
+// All of the forward for at most kLogpFew rows in two launches, in scratch of
+// logp_few_bytes(t, vocab).
+constexpr size_t kLogpFew = 64;
+size_t logp_few_bytes(size_t t, size_t vocab);
+hipError_t launch_logp_few(const float* hn, const float* head, const int64_t* targets, size_t t, size_t d, size_t vocab,
+                           float* logp, float* lse, void* misc, void* scratch, hipStream_t st);
 
 // The same for many rows, on packed f16 operands (head_gemm.hip), the logits only
 // in registers.  A plan holds the sizes of the buffers, of which rows are in

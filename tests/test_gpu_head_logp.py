@@ -102,7 +102,7 @@ def check(hn, head, tg, dlogp):
 
 
 SHAPES = [(1, 1, 1), (1, 64, 5), (3, 7, 130), (1, 576, 4097), (5, 576, 2000), (16, 100, 1000), (17, 576, 1000),
-          (64, 33, 4099), (65, 31, 257), (130, 100, 257), (256, 64, 512), (257, 576, 3001), (300, 65, 50),
+          (15, 50, 63), (32, 576, 3000), (33, 40, 128), (64, 33, 4099), (64, 130, 66), (65, 31, 257), (130, 100, 257), (256, 64, 512), (257, 576, 3001), (300, 65, 50),
           (700, 128, 900), (513, 576, 8192), (1000, 16, 20000)]
 
 
