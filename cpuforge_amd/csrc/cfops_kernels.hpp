@@ -199,8 +199,11 @@ hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const in
                                  hipStream_t st);
 hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t rows, void* misc, hipStream_t st);
 // All of the forward for at most kLogpFew rows in two launches, in scratch of
-// logp_few_bytes(t, vocab).
-constexpr size_t kLogpFew = 64;
+// logp_few_bytes(t, vocab).  (us against the packed operands, 576 x 49152 and 2048 x
+// 128256: 32 rows 56 and 83, 415 and 631; 48 rows 88 and 85, 754 and 632; the
+// gradients' f32 products against theirs 128 and 183, 682 and 1167 at 32 rows, with
+// the forward's part of keeping 182 and 186, 1084 and 1176.)
+constexpr size_t kLogpFew = 32;
 size_t logp_few_bytes(size_t t, size_t vocab);
 hipError_t launch_logp_few(const float* hn, const float* head, const int64_t* targets, size_t t, size_t d, size_t vocab,
                            float* logp, float* lse, void* misc, void* scratch, hipStream_t st);

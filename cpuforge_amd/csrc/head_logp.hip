@@ -283,7 +283,8 @@ hipError_t launch_logp_few(const float* hn, const float* head, const int64_t* ta
     float* xt = static_cast<float*>(scratch);
     MaxSum* stats = reinterpret_cast<MaxSum*>(xt + kLogpFew);
     const unsigned parts = (unsigned)((vocab + kFewVocab - 1) / kFewVocab);
-    const auto kernel = t <= 16 ? logp_few_kernel<1> : t <= 32 ? logp_few_kernel<2> : logp_few_kernel<4>;
+    static_assert(kLogpFew == 32, "the tokens of a wave");
+    const auto kernel = t <= 16 ? logp_few_kernel<1> : logp_few_kernel<2>;
     hipLaunchKernelGGL(kernel, dim3(parts), dim3(256), 0, st, hn, head, targets, (int)t, (int)d, (int)vocab, stats, xt);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

@@ -31,26 +31,34 @@ __device__ __forceinline__ Span span(const int64_t* __restrict__ offsets, long i
     return {bad ? 0 : lo, bad ? 0 : hi, bad};
 }
 
-// Sum over a group of NW waves, every lane getting it, in a fixed order.
-template <int NW>
-__device__ __forceinline__ double group_sum(double x, double* red) {
+// Sums of K values over a group of NW waves, every lane getting them, in a fixed
+// order.  red: K * NW values, free again after the caller's next barrier.
+template <int NW, int K>
+__device__ __forceinline__ void group_sums(double (&x)[K], double* red) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+    for (int o = 32; o >= 1; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; k++) x[k] += __shfl_xor(x[k], o);
     if constexpr (NW > 1) {
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-        __syncthreads();
-        x = 0.0;
+        if ((threadIdx.x & 63) == 0)
 #pragma unroll
-        for (int i = 0; i < NW; i++) x += red[i];
+            for (int k = 0; k < K; k++) red[k * NW + (threadIdx.x >> 6)] = x[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            x[k] = 0.0;
+#pragma unroll
+            for (int i = 0; i < NW; i++) x[k] += red[k * NW + i];
+        }
     }
-    return x;
 }
 
-struct PairTerms {
-    double loss, margin;
-    int accurate;
-};
+__device__ __forceinline__ bool is_scored(const int64_t* __restrict__ targets, long r) {
+    return !targets || targets[r] != kIgnoreIndex;
+}
+
+constexpr int kRows = 2;  // rows of a lane whose loads are in flight together
 
 // log(1 + exp(x)).
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
@@ -76,19 +84,32 @@ template <int NW>
 __device__ __forceinline__ void one_pair(const PreferenceArgs& a, long pair, double* red) {
     const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
     const Span s[2] = {span(a.offsets, 2 * pair, a.rows), span(a.offsets, 2 * pair + 1, a.rows)};
+    double sums[4] = {};  // of either sequence, and its scored rows
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+        for (long r0 = s[k].lo + tid; r0 < s[k].hi; r0 += kRows * 64 * NW) {
+            float x[kRows], y[kRows];
+            bool use[kRows];
+#pragma unroll
+            for (int i = 0; i < kRows; i++) {
+                const long r = r0 + i * 64 * NW, at = min(r, s[k].hi - 1);
+                use[i] = is_scored(a.targets, at) && r < s[k].hi;
+                x[i] = a.logp[at];
+                y[i] = a.ref_logp ? a.ref_logp[at] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kRows; i++)
+                if (use[i]) {
+                    sums[k] += (double)x[i] - (double)y[i];
+                    sums[2 + k] += 1.0;
+                }
+        }
+    group_sums<NW>(sums, red);
     double reward[2], share[2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        double sum = 0.0, cnt = 0.0;
-        for (long r = s[k].lo + tid; r < s[k].hi; r += 64 * NW)
-            if (!a.targets || a.targets[r] != kIgnoreIndex) {
-                sum += (double)a.logp[r] - (a.ref_logp ? (double)a.ref_logp[r] : 0.0);
-                cnt += 1.0;
-            }
-        sum = group_sum<NW>(sum, red);
-        cnt = group_sum<NW>(cnt, red);
-        share[k] = a.length_mean ? a.beta / fmax(cnt, 1.0) : a.beta;
-        reward[k] = sum * share[k];
+        share[k] = a.length_mean ? a.beta / fmax(sums[2 + k], 1.0) : a.beta;
+        reward[k] = sums[k] * share[k];
     }
     double l, dz;
     preference_term(a, reward[0] - reward[1] - a.margin, l, dz);
@@ -96,8 +117,8 @@ __device__ __forceinline__ void one_pair(const PreferenceArgs& a, long pair, dou
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         const float d = (float)(k ? -dz * share[k] : dz * share[k]);
-        for (long r = s[k].lo + tid; r < s[k].hi; r += 64 * NW)
-            a.dlogp[r] = !a.targets || a.targets[r] != kIgnoreIndex ? d : 0.0f;
+#pragma unroll 4
+        for (long r = s[k].lo + tid; r < s[k].hi; r += 64 * NW) a.dlogp[r] = is_scored(a.targets, r) ? d : 0.0f;
     }
     if (tid == 0) {
         a.rewards[2 * pair] = (float)reward[0];
@@ -107,103 +128,132 @@ __device__ __forceinline__ void one_pair(const PreferenceArgs& a, long pair, dou
     }
 }
 
-// The result from the pairs' terms, by one workgroup of NW waves.
+// The first sequence whose offsets do not rise within the rows, by a workgroup of NW
+// waves (its barriers: two).
 template <int NW>
-__device__ __forceinline__ void preference_result(const PreferenceArgs& a, double* red) {
-    double loss = 0.0, margin = 0.0, accurate = 0.0;
-    int bad = INT_MAX;
-    for (long i = threadIdx.x; i < a.pairs; i += 64 * NW) {
-        loss += a.terms[2 * i];
-        margin += a.terms[2 * i + 1];
-        accurate += a.terms[2 * i + 1] > 0.0;
-        for (int k = 1; k >= 0; k--)
-            if (span(a.offsets, 2 * i + k, a.rows).bad) bad = min(bad, (int)(2 * i + k));
-    }
-    loss = group_sum<NW>(loss, red);
-    margin = group_sum<NW>(margin, red);
-    accurate = group_sum<NW>(accurate, red);
+__device__ __forceinline__ int first_bad(const int64_t* __restrict__ offsets, long seqs, long rows) {
     __shared__ int first;
     if (threadIdx.x == 0) first = INT_MAX;
     __syncthreads();
-    if (bad != INT_MAX) atomicMin(&first, bad);
+    for (long i = threadIdx.x; i < seqs; i += 64 * NW)
+        if (span(offsets, i, rows).bad) atomicMin(&first, (int)i);
     __syncthreads();
+    return first;
+}
+
+// The result from the pairs' terms, by one workgroup of NW waves.
+template <int NW>
+__device__ __forceinline__ void preference_result(const PreferenceArgs& a, double* red) {
+    double sums[3] = {};
+    for (long i = threadIdx.x; i < a.pairs; i += 64 * NW) {
+        sums[0] += a.terms[2 * i];
+        sums[1] += a.terms[2 * i + 1] > 0.0;
+        sums[2] += a.terms[2 * i + 1];
+    }
+    const int bad = first_bad<NW>(a.offsets, 2 * a.pairs, a.rows);
+    group_sums<NW>(sums, red);
     if (threadIdx.x == 0) {
-        const double n = fmax((double)a.pairs, 1.0);
-        *a.result = {first, (float)(loss / n), (float)(accurate / n), (float)(margin / n)};
+        const double n = (double)a.pairs;
+        *a.result = {bad, (float)(sums[0] / n), (float)(sums[1] / n), (float)(sums[2] / n)};
     }
 }
 
 __global__ __launch_bounds__(1024) void preference_small_kernel(const PreferenceArgs a) {
-    __shared__ double red[16];
+    __shared__ double red[3 * 16];
     for (long pair = threadIdx.x >> 6; pair < a.pairs; pair += 16) one_pair<1>(a, pair, red);
     __threadfence_block();
     __syncthreads();
     preference_result<16>(a, red);
 }
 __global__ __launch_bounds__(512) void preference_pair_kernel(const PreferenceArgs a) {
-    __shared__ double red[8];
+    __shared__ double red[4 * 8];
     one_pair<8>(a, blockIdx.x, red);
 }
 __global__ __launch_bounds__(1024) void preference_finish_kernel(const PreferenceArgs a) {
-    __shared__ double red[16];
+    __shared__ double red[3 * 16];
     preference_result<16>(a, red);
 }
 
 // ------------------------------------------------------------------- policy
 
-// Scored rows of a sequence, by one workgroup of four waves.
+// Scored rows of [lo, hi), by NW waves from lane `tid` on.
+template <int NW>
+__device__ __forceinline__ double count_rows(const PolicyArgs& a, const Span& s, int tid, double* red) {
+    double n[1] = {};
+    for (long r0 = s.lo + tid; r0 < s.hi; r0 += 8 * 64 * NW) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const long r = r0 + i * 64 * NW;
+            n[0] += is_scored(a.targets, min(r, s.hi - 1)) && r < s.hi;
+        }
+    }
+    group_sums<NW>(n, red);
+    return n[0];
+}
 __global__ __launch_bounds__(256) void policy_count_kernel(const PolicyArgs a) {
     __shared__ double red[4];
-    const Span s = span(a.offsets, blockIdx.x, a.rows);
-    double n = 0.0;
-    for (long r = s.lo + threadIdx.x; r < s.hi; r += 256) n += !a.targets || a.targets[r] != kIgnoreIndex;
-    n = group_sum<4>(n, red);
+    const double n = count_rows<4>(a, span(a.offsets, blockIdx.x, a.rows), threadIdx.x, red);
     if (threadIdx.x == 0) a.counts[blockIdx.x] = (int)n;
 }
 
 // N, the scored rows, and M, the sequences with any, by a workgroup of NW waves.
 template <int NW>
 __device__ __forceinline__ void totals(const PolicyArgs& a, double& n, double& m, double* red) {
-    n = m = 0.0;
+    double x[2] = {};
     for (long i = threadIdx.x; i < a.seqs; i += 64 * NW) {
         const int c = a.counts[i];
-        n += c;
-        m += c > 0;
+        x[0] += c;
+        x[1] += c > 0;
     }
-    n = group_sum<NW>(n, red);
-    m = group_sum<NW>(m, red);
+    group_sums<NW>(x, red);
+    n = x[0], m = x[1];
 }
 
-// Rows [r0, r1) of sequence `seq` whose scored rows weigh w: their gradients, and
-// their terms added to the lane's sums.
-__device__ __forceinline__ void policy_rows(const PolicyArgs& a, long seq, double w, long r, long r1, int step,
-                                            double& loss, double& kl, double& cuts) {
-    for (; r < r1; r += step) {
-        float d = 0.0f;
-        if (!a.targets || a.targets[r] != kIgnoreIndex) {
-            const double lp = a.logp[r];
-            const double adv = a.advantages[a.per_token ? r : seq];
-            const double diff = a.old_logp ? lp - (double)a.old_logp[r] : 0.0;
-            const double ratio = exp(diff);
-            // min(r A, clip(r) A) is the clipped one past the border on the side A
-            // pushes to.
-            const bool up = adv > 0.0 && diff > a.log_high, down = adv < 0.0 && diff < a.log_low;
-            double l = -ratio * adv, dl = l;
-            if (up || down) {
-                l = -(up ? a.high : a.low) * adv;
-                dl = 0.0;
-                cuts += 1.0;
-            }
-            if (a.ref_logp) {
-                const double x = (double)a.ref_logp[r] - lp, e = expm1(x);
-                kl += w * (e - x);
-                l += a.kl_coef * (e - x);
-                dl -= a.kl_coef * e;
-            }
-            loss += w * l;
-            d = (float)(dl * w);
+// One row's gradient, its terms added to the lane's sums (loss, KL, cut rows).
+__device__ __forceinline__ float policy_row(const PolicyArgs& a, double w, double lp, double old, double ref, double adv,
+                                            double (&sums)[3]) {
+    const double diff = a.old_logp ? lp - old : 0.0;
+    const double ratio = exp(diff);
+    // min(r A, clip(r) A) is the clipped one past the border on the side A pushes to.
+    const bool up = adv > 0.0 && diff > a.log_high, down = adv < 0.0 && diff < a.log_low;
+    double l = -ratio * adv, dl = l;
+    if (up || down) {
+        l = -(up ? a.high : a.low) * adv;
+        dl = 0.0;
+        sums[2] += 1.0;
+    }
+    if (a.ref_logp) {
+        const double x = ref - lp, e = expm1(x);
+        sums[1] += w * (e - x);
+        l += a.kl_coef * (e - x);
+        dl -= a.kl_coef * e;
+    }
+    sums[0] += w * l;
+    return (float)(dl * w);
+}
+
+// The rows of sequence `seq`, whose scored ones weigh w, from lane `tid` of NW waves on.
+template <int NW>
+__device__ __forceinline__ void policy_rows(const PolicyArgs& a, long seq, const Span& s, double w, int tid,
+                                            double (&sums)[3]) {
+    for (long r0 = s.lo + tid; r0 < s.hi; r0 += kRows * 64 * NW) {
+        float lp[kRows], old[kRows], ref[kRows], adv[kRows];
+        bool use[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; i++) {
+            const long r = min(r0 + i * 64 * NW, s.hi - 1);
+            use[i] = is_scored(a.targets, r);
+            lp[i] = a.logp[r];
+            old[i] = a.old_logp ? a.old_logp[r] : 0.0f;
+            ref[i] = a.ref_logp ? a.ref_logp[r] : 0.0f;
+            adv[i] = a.advantages[a.per_token ? r : seq];
         }
-        a.dlogp[r] = d;
+#pragma unroll
+        for (int i = 0; i < kRows; i++) {
+            const long r = r0 + i * 64 * NW;
+            if (r >= s.hi) break;
+            a.dlogp[r] = use[i] ? policy_row(a, w, lp[i], old[i], ref[i], adv[i], sums) : 0.0f;
+        }
     }
 }
 
@@ -213,71 +263,49 @@ __device__ __forceinline__ double row_weight(const PolicyArgs& a, long seq, doub
 }
 
 template <int NW>
-__device__ __forceinline__ void policy_result(const PolicyArgs& a, double loss, double kl, double cuts, double n,
-                                              double* red) {
-    loss = group_sum<NW>(loss, red);
-    kl = group_sum<NW>(kl, red);
-    cuts = group_sum<NW>(cuts, red);
-    __shared__ int first;
-    if (threadIdx.x == 0) first = INT_MAX;
-    __syncthreads();
-    for (long i = threadIdx.x; i < a.seqs; i += 64 * NW)
-        if (span(a.offsets, i, a.rows).bad) atomicMin(&first, (int)i);
-    __syncthreads();
+__device__ __forceinline__ void policy_result(const PolicyArgs& a, double (&sums)[3], double n, double* red) {
+    const int bad = first_bad<NW>(a.offsets, a.seqs, a.rows);
+    group_sums<NW>(sums, red);
     if (threadIdx.x == 0)
-        *a.result = {(int)n, first, first == INT_MAX ? (float)loss : __builtin_nanf(""), (float)kl,
-                     (float)(cuts / fmax(n, 1.0))};
+        *a.result = {(int)n, bad, bad == INT_MAX ? (float)sums[0] : __builtin_nanf(""), (float)sums[1],
+                     (float)(sums[2] / fmax(n, 1.0))};
 }
 
 // A wave to a sequence, one workgroup for all.
 __global__ __launch_bounds__(1024) void policy_small_kernel(const PolicyArgs a) {
-    __shared__ double red[16];
+    __shared__ double red[3 * 16];
     const int lane = threadIdx.x & 63;
     for (long i = threadIdx.x >> 6; i < a.seqs; i += 16) {
-        const Span s = span(a.offsets, i, a.rows);
-        double n = 0.0;
-        for (long r = s.lo + lane; r < s.hi; r += 64) n += !a.targets || a.targets[r] != kIgnoreIndex;
-        n = group_sum<1>(n, red);
+        const double n = count_rows<1>(a, span(a.offsets, i, a.rows), lane, red);
         if (lane == 0) a.counts[i] = (int)n;
     }
     __threadfence_block();
     __syncthreads();
-    double n, m, loss = 0.0, kl = 0.0, cuts = 0.0;
+    double n, m, sums[3] = {};
     totals<16>(a, n, m, red);
-    for (long i = threadIdx.x >> 6; i < a.seqs; i += 16) {
-        const Span s = span(a.offsets, i, a.rows);
-        policy_rows(a, i, row_weight(a, i, n, m), s.lo + lane, s.hi, 64, loss, kl, cuts);
-    }
-    policy_result<16>(a, loss, kl, cuts, n, red);
+    for (long i = threadIdx.x >> 6; i < a.seqs; i += 16)
+        policy_rows<1>(a, i, span(a.offsets, i, a.rows), row_weight(a, i, n, m), lane, sums);
+    policy_result<16>(a, sums, n, red);
 }
 
 // A workgroup to a sequence: its terms go to `terms`.
 __global__ __launch_bounds__(256) void policy_seq_kernel(const PolicyArgs a) {
-    __shared__ double red[4];
-    double n, m, loss = 0.0, kl = 0.0, cuts = 0.0;
+    __shared__ double red[3 * 4];
+    double n, m, sums[3] = {};
     totals<4>(a, n, m, red);
     const long i = blockIdx.x;
-    const Span s = span(a.offsets, i, a.rows);
-    policy_rows(a, i, row_weight(a, i, n, m), s.lo + threadIdx.x, s.hi, 256, loss, kl, cuts);
-    loss = group_sum<4>(loss, red);
-    kl = group_sum<4>(kl, red);
-    cuts = group_sum<4>(cuts, red);
-    if (threadIdx.x == 0) {
-        a.terms[3 * i] = loss;
-        a.terms[3 * i + 1] = kl;
-        a.terms[3 * i + 2] = cuts;
-    }
+    policy_rows<4>(a, i, span(a.offsets, i, a.rows), row_weight(a, i, n, m), threadIdx.x, sums);
+    group_sums<4>(sums, red);
+    if (threadIdx.x < 3) a.terms[3 * i + threadIdx.x] = threadIdx.x == 0 ? sums[0] : threadIdx.x == 1 ? sums[1] : sums[2];
 }
 __global__ __launch_bounds__(1024) void policy_finish_kernel(const PolicyArgs a) {
-    __shared__ double red[16];
-    double n, m, loss = 0.0, kl = 0.0, cuts = 0.0;
+    __shared__ double red[3 * 16];
+    double n, m, sums[3] = {};
     totals<16>(a, n, m, red);
-    for (long i = threadIdx.x; i < a.seqs; i += 1024) {
-        loss += a.terms[3 * i];
-        kl += a.terms[3 * i + 1];
-        cuts += a.terms[3 * i + 2];
-    }
-    policy_result<16>(a, loss, kl, cuts, n, red);
+    for (long i = threadIdx.x; i < a.seqs; i += 1024)
+#pragma unroll
+        for (int k = 0; k < 3; k++) sums[k] += a.terms[3 * i + k];
+    policy_result<16>(a, sums, n, red);
 }
 
 }  // namespace
