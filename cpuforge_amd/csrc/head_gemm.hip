@@ -64,6 +64,10 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a < INFINITY ? a : 0.0f;
 }
 
+__device__ __forceinline__ f32x16 mfma_f16(const f16x8& a, const f16x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
 struct Pieces {
     f16x8 h, l;
 };
@@ -326,6 +330,8 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
                 kl++;
             }
         };
+        // (A wave of a last tile whose columns all lie behind the last one forms nothing.)
+        const bool live_cols = P == Product::kHead || col0 < n;
         f32x16 acc[MB][2], tot[ROWS ? MB : 1][2];
 #pragma unroll
         for (int i = 0; i < MB; i++) {
@@ -362,15 +368,16 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
             }
             // (The order that shares an operand from one to the next: 1% less time.)
             constexpr int pa[3] = {1, 0, 0}, pb[3] = {0, 0, 1};
+            if (live_cols)
 #pragma unroll
-            for (int q = 0; q < 3; q++)
+                for (int q = 0; q < 3; q++)
 #pragma unroll
-                for (int i = 0; i < MB; i++)
+                    for (int i = 0; i < MB; i++)
 #pragma unroll
-                    for (int jj = 0; jj < 2; jj++) {
-                        const int j = (i + q) & 1 ? 1 - jj : jj;
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][pa[q]], b[j][pb[q]], acc[i][j], 0, 0, 0);
-                    }
+                        for (int jj = 0; jj < 2; jj++) {
+                            const int j = (i + q) & 1 ? 1 - jj : jj;
+                            acc[i][j] = mfma_f16(a[i][pa[q]], b[j][pb[q]], acc[i][j]);
+                        }
             if constexpr (ROWS) {
                 if (k % 8 != 7) continue;
                 const float* f = reinterpret_cast<const float*>(s + CH * kFrag + wave * 256);
@@ -432,6 +439,7 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
                                             tot[i][j][4 * q + 3]);
             }
         } else {
+            if (!live_cols) continue;
             const int live = g.vocab - m0;  // rows of the head in this wave's part
             int e[MB];
 #pragma unroll
@@ -443,21 +451,32 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
                 const bool scored = col < n;
                 const long r = scored ? g.idx[g.j0 + col] : 0;
                 const int et = (int)(__builtin_bit_cast(uint32_t, g.scale[g.j0 + col]) >> 23) - 127;
-                // The target's row within this wave's part.
+                // The target's row within this wave's part; the rows of q lie at 4 hh.
                 const long target = (scored ? g.targets[r] : -1) - m0;
-                if (live < 32 * MB)
+                const int at = (int)(target >= 0 && target < 32 * MB ? target : -1000) - 4 * hh;
+                if (live < 32 * MB) {
+                    const int end = live - 4 * hh;
 #pragma unroll
                     for (int i = 0; i < MB; i++)
 #pragma unroll
                         for (int q = 0; q < 16; q++)
-                            if (32 * i + 8 * (q >> 2) + 4 * hh + (q & 3) >= live) acc[i][j][q] = -INFINITY;
-                if (__any(target >= 0 && target < 32 * MB))
+                            if (32 * i + 8 * (q >> 2) + (q & 3) >= end) acc[i][j][q] = -INFINITY;
+                }
+                if (__any(at > -500)) {
+                    float x = 0.0f;
+                    bool hit = false;
+                    int et_i = 0;
 #pragma unroll
                     for (int i = 0; i < MB; i++)
 #pragma unroll
-                        for (int q = 0; q < 16; q++)
-                            if (32 * i + 8 * (q >> 2) + 4 * hh + (q & 3) == target)
-                                g.xt[col] = acc[i][j][q] * pow2_clamped(e[i] + et);
+                        for (int q = 0; q < 16; q++) {
+                            const bool here = 32 * i + 8 * (q >> 2) + (q & 3) == at;
+                            x = here ? acc[i][j][q] : x;
+                            hit |= here;
+                            if (q == 15) et_i = at >= 32 * i ? e[i] : et_i;
+                        }
+                    if (hit) g.xt[col] = x * pow2_clamped(et_i + et);
+                }
                 float c[MB], m = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < MB; i++) {
