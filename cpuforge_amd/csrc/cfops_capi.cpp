@@ -611,9 +611,10 @@ int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, co
         CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, b.idx, b.count, nullptr, nullptr, nullptr, st),
                "log-probability launch");
     }
-    // The head's gradient goes through dlogits that fit the head's limit.
-    const size_t pass =
-        std::min(p.chunk, std::max<size_t>(c->head_chunk_bytes / (p.v_pad * sizeof(float)) / 128 * 128, 128));
+    // The head's gradient goes through dlogits that fit the head's limit (and a launch
+    // with a row of workgroups to 32 rows).
+    const size_t pass = std::min({p.chunk, (size_t)1 << 20,
+                                  std::max<size_t>(c->head_chunk_bytes / (p.v_pad * sizeof(float)) / 128 * 128, 128)});
     char* dlogits = nullptr;
     unsigned* col_top = nullptr;
     if (dhead) {

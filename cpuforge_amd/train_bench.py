@@ -181,9 +181,28 @@ class SmolLM:
         """The parameters that train (TrainSpec)."""
         return [p for _, p in self.named_params() if p.requires_grad]
 
+    def hidden(self, tokens):
+        """The final norm's output [B, S, d]."""
+        return self._hidden_cfops(tokens) if self.backend == "cfops" else self._hidden_torch(tokens)
+
+    def logprobs(self, tokens, targets):
+        """The targets' log-probabilities [B, S], 0 where a target is
+        ops.IGNORE_INDEX (A.lm_head_logprobs; cfops backend, no host wait:
+        check_targets() reports a target out of range).  What a preference or
+        policy loss starts from."""
+        if self.backend != "cfops":
+            raise ValueError("log-probabilities need the cfops backend")
+        logp, res = A.lm_head_logprobs(self.hidden(tokens), self.embed, targets)
+        self._ce = (res, targets)
+        return logp
+
     def loss(self, tokens, targets):
         if self.backend == "cfops":
             return self._loss_cfops(tokens, targets)
+        logits = self.hidden(tokens) @ self.embed.t()
+        return F.cross_entropy(logits.view(-1, self.c["vocab"]).float(), targets.view(-1))
+
+    def _hidden_torch(self, tokens):
         c = self.c
         B, S = tokens.shape
         x = self.embed[tokens]
@@ -196,14 +215,12 @@ class SmolLM:
             x = x + layer["wo"](o.view(B, S, -1).to(self.dtype))
             n2 = rmsnorm(x, layer["mlp_norm"], c["eps"])
             x = x + layer["down"](F.silu(layer["gate"](n2)) * layer["up"](n2))
-        hn = rmsnorm(x, self.final_norm, c["eps"])
-        logits = hn @ self.embed.t()
-        return F.cross_entropy(logits.view(-1, c["vocab"]).float(), targets.view(-1))
+        return rmsnorm(x, self.final_norm, c["eps"])
 
-    def _loss_cfops(self, tokens, targets):
+    def _hidden_cfops(self, tokens):
         """Layer::forward (crates/model/src/layer.rs:90-143) per layer, then the
-        final norm and the tied LM head with its loss (model.rs:436-442), every
-        op but the gather and the residual adds in libcfattn.so."""
+        final norm, every op but the gather and the residual adds in
+        libcfattn.so."""
         c, cf = self.c, "cfops"
         B, S = tokens.shape
         x = self.embed[tokens]
@@ -218,7 +235,11 @@ class SmolLM:
             n2 = A.rmsnorm(x, layer["mlp_norm"], c["eps"])
             g, u = A.shared_input_linears(n2, [layer[n].spec() for n in ("gate", "up")])
             x = x + layer["down"](A.silu_mul(g, u), cf)
-        hn = A.rmsnorm(x, self.final_norm, c["eps"])
+        return A.rmsnorm(x, self.final_norm, c["eps"])
+
+    def _loss_cfops(self, tokens, targets):
+        """The tied LM head with its loss (model.rs:436-442)."""
+        hn = self._hidden_cfops(tokens)
         if self.ce_on_device:
             loss, res = A.lm_head_ce_dev(hn, self.embed, targets)
             self._ce = (res, targets)

@@ -103,7 +103,8 @@ def check(hn, head, tg, dlogp):
 
 SHAPES = [(1, 1, 1), (1, 64, 5), (3, 7, 130), (1, 576, 4097), (5, 576, 2000), (16, 100, 1000), (17, 576, 1000),
           (15, 50, 63), (32, 576, 3000), (33, 40, 128), (64, 33, 4099), (64, 130, 66), (65, 31, 257), (130, 100, 257), (256, 64, 512), (257, 576, 3001), (300, 65, 50),
-          (700, 128, 900), (513, 576, 8192), (1000, 16, 20000)]
+          (700, 128, 900), (513, 576, 8192), (1000, 16, 20000), (70, 1500, 300), (66, 2100, 300),
+          (40, 3, 7)]
 
 
 @pytest.mark.parametrize("t,d,vocab", SHAPES)
@@ -243,6 +244,18 @@ def test_rows_in_chunks_and_repeated_calls_agree():
     w = reference(hn, head, tg, g)
     assert bool(((dhn2 - w[2]).abs() <= 2 * (dhn - w[2]).abs().max()).all())
     assert bool(((dhead2 - dhead).abs() <= 2.0 ** -20 * dhead.abs().max()).all())
+    # With what the forward keeps, the head's gradient alone goes in passes.
+    keep = kept(hn, head, tg)
+    one = backward(hn, head, tg, lse, g, keep=keep)
+    P.set_head_chunk_limit(0)
+    try:
+        many = backward(hn, head, tg, lse, g, keep=keep)
+        over = backward(hn, head, tg, lse, g, keep=keep, acc=False)[1]
+    finally:
+        P.set_head_chunk_limit(512 << 20)
+    assert torch.equal(one[0], many[0])
+    assert bool(((many[1] - dhead).abs() <= 2.0 ** -20 * dhead.abs().max()).all())
+    assert bool(((many[1] - 1 - over).abs() <= 2.0 ** -20 * dhead.abs().max()).all())
 
 
 def test_captured_step_replays():
