@@ -508,9 +508,11 @@ namespace {
 
 int check_logprobs(cfattn_ctx* c, size_t t, size_t d, size_t vocab) {
     if (d == 0 || vocab == 0) return fail(c, CFATTN_ERR_ARG, "d and vocab must be positive");
-    // (A launch with a workgroup of 256 threads to each row has fewer than 2^32.)
-    if (t >= (size_t)1 << 24 || !fits_int(d) || !fits_int(vocab))
-        return fail(c, CFATTN_ERR_UNSUPPORTED, "t=%zu not below 2^24, or d=%zu, vocab=%zu above 2^31", t, d, vocab);
+    // (A launch with a workgroup of 256 threads to each row, or 1024 to 32 of the head, has
+    // fewer than 2^32.)
+    if (t >= (size_t)1 << 24 || !fits_int(d) || vocab >= (size_t)1 << 26)
+        return fail(c, CFATTN_ERR_UNSUPPORTED, "t=%zu not below 2^24, d=%zu above 2^31, or vocab=%zu not below 2^26", t,
+                    d, vocab);
     return CFATTN_OK;
 }
 
@@ -525,7 +527,7 @@ int logp_rows(cfattn_ctx* c, size_t t, size_t d, size_t vocab, LogpRows& r) {
     // A chunk's logits fit the head's limit, its rows a launch of workgroups.
     r.chunk = std::min<size_t>(c->head_chunk_bytes / (vocab * sizeof(float)), (size_t)1 << 22);
     r.chunk = std::min(std::max<size_t>(r.chunk, 1), t);
-    CF_TRY(take(c, cfattn_ctx::OPS_IDX, (t + 4) * sizeof(int), r.count));
+    CF_TRY(take(c, cfattn_ctx::OPS_IDX, (4 + 2 * t) * sizeof(int), r.count));
     r.idx = r.count + 4;
     CF_TRY(take(c, cfattn_ctx::OPS_ROWS, t * d * sizeof(float), r.hn));
     return take(c, cfattn_ctx::OPS_LOGITS, r.chunk * vocab * sizeof(float), r.logits);
@@ -539,7 +541,7 @@ struct KeepLayout {
 };
 KeepLayout keep_layout(const cfattn::HeadPlan& p, size_t t) {
     KeepLayout l{};
-    l.keep = align_up((4 + t + p.v_pad / 32) * sizeof(int));
+    l.keep = align_up((4 + 2 * t + p.v_pad / 32) * sizeof(int));
     l.back = l.keep + align_up(p.keep_bytes);
     l.factor = l.back + align_up(p.back_bytes);
     l.bytes = l.factor + align_up(p.factor_bytes);
@@ -549,7 +551,7 @@ void keep_at(const cfattn::HeadPlan& p, size_t t, char* base, cfattn::HeadBuffer
     const KeepLayout l = keep_layout(p, t);
     b.count = reinterpret_cast<int*>(base);
     b.idx = b.count + 4;
-    b.exponents = b.idx + t;
+    b.exponents = b.idx + 2 * t;
     b.keep = base + l.keep;
     b.back = base + l.back;
     b.factor = reinterpret_cast<float*>(base + l.factor);
@@ -566,9 +568,9 @@ int head_scratch(cfattn_ctx* c, const cfattn::HeadPlan& p, size_t t, cfattn::Hea
     b.xt = reinterpret_cast<float*>(stats + p.stats_bytes);
     CF_TRY(take(c, cfattn_ctx::OPS_HEAD, p.head_bytes, b.packed));
     if (b.count) return CFATTN_OK;
-    CF_TRY(take(c, cfattn_ctx::OPS_IDX, (4 + t + p.v_pad / 32) * sizeof(int), b.count));
+    CF_TRY(take(c, cfattn_ctx::OPS_IDX, (4 + 2 * t + p.v_pad / 32) * sizeof(int), b.count));
     b.idx = b.count + 4;
-    b.exponents = b.idx + t;
+    b.exponents = b.idx + 2 * t;
     return CFATTN_OK;
 }
 
@@ -588,10 +590,10 @@ int logprobs_many(cfattn_ctx* c, const float* hn, const float* head, const int64
         keep_at(p, t, static_cast<char*>(keep), b);
     }
     CF_TRY(head_scratch(c, p, t, b));
-    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, b.idx, b.count, logp, lse, result, st),
+    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, b.idx, b.count, p.tag, logp, lse, result, st),
            "log-probability launch");
     CF_HIP(c, cfattn::launch_head_pack(p, b, hn, head, d, vocab, st), "log-probability launch");
-    CF_HIP(c, cfattn::launch_head_stats(p, b, targets, 0, vocab, logp, lse, st), "log-probability launch");
+    CF_HIP(c, cfattn::launch_head_stats(p, b, t, 0, vocab, logp, lse, st), "log-probability launch");
     return CFATTN_OK;
 }
 
@@ -608,7 +610,7 @@ int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, co
         CF_TRY(take(c, cfattn_ctx::OPS_LOGITS, p.keep_bytes, b.keep));
         CF_TRY(take(c, cfattn_ctx::OPS_BACK, p.back_bytes + p.factor_bytes, b.back));
         b.factor = reinterpret_cast<float*>(b.back + p.back_bytes);
-        CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, b.idx, b.count, nullptr, nullptr, nullptr, st),
+        CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, b.idx, b.count, p.tag, nullptr, nullptr, nullptr, st),
                "log-probability launch");
     }
     // The head's gradient goes through dlogits that fit the head's limit (and a launch
@@ -634,16 +636,16 @@ int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, co
     if (!keep) CF_HIP(c, cfattn::launch_head_pack(p, b, hn, head, d, vocab, st), "log-probability launch");
     if (dhn) {
         CF_TRY(take(c, cfattn_ctx::OPS_PART, p.part_bytes, b.part));
-        CF_HIP(c, cfattn::launch_head_zero_rows(targets, t, vocab, dhn, d, st), "log-probability launch");
+        CF_HIP(c, cfattn::launch_head_zero_rows(p, b, t, dhn, d, st), "log-probability launch");
     }
     for (size_t j0 = 0; j0 < t; j0 += p.chunk) {
         if (!keep)
-            CF_HIP(c, cfattn::launch_head_stats(p, b, targets, j0, vocab, nullptr, nullptr, st),
+            CF_HIP(c, cfattn::launch_head_stats(p, b, t, j0, vocab, nullptr, nullptr, st),
                    "log-probability launch");
         if (dhn)
-            CF_HIP(c, cfattn::launch_head_dhn(p, b, targets, head, dlogp, j0, d, dhn, st), "log-probability launch");
+            CF_HIP(c, cfattn::launch_head_dhn(p, b, t, head, dlogp, j0, d, dhn, st), "log-probability launch");
         for (size_t i = 0; dhead && i < p.chunk && j0 + i < t; i += pass)
-            CF_HIP(c, cfattn::launch_head_dhead(p, b, targets, dlogp, j0, i, std::min({t - j0 - i, p.chunk - i, pass}),
+            CF_HIP(c, cfattn::launch_head_dhead(p, b, t, dlogp, j0, i, std::min({t - j0 - i, p.chunk - i, pass}),
                                                 d, vocab, dlogits, col_top, dhead, acc || j0 + i, st),
                    "log-probability launch");
     }
@@ -690,7 +692,9 @@ int adamw8_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors,
 }  // namespace
 
 size_t cfops_lm_head_logprobs_keep_bytes(size_t t, size_t d, size_t vocab) {
-    if (t <= cfattn::kLogpFew || t >= (size_t)1 << 24 || d == 0 || vocab == 0 || !fits_int(d) || !fits_int(vocab)) return 0;
+    if (t <= cfattn::kLogpFew || t >= (size_t)1 << 24 || d == 0 || vocab == 0 || !fits_int(d) ||
+        vocab >= (size_t)1 << 26)
+        return 0;
     return keep_layout(cfattn::head_plan(t, d, vocab, SIZE_MAX), t).bytes;
 }
 
@@ -733,7 +737,8 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
                                       st);
     LogpRows rows{};
     CF_TRY(logp_rows(c, t, d, vocab, rows));
-    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, nullptr, nullptr, nullptr, st),
+    CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, 0, nullptr, nullptr, nullptr,
+                                              st),
            "log-probability launch");
     CF_HIP(c, cfattn::launch_logp_gather(hn, rows.idx, rows.count, rows.hn, t, d, st), "log-probability launch");
     for (size_t j0 = 0; j0 < t; j0 += rows.chunk) {

@@ -183,13 +183,14 @@ hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st);
 // order, and the kernels below work on scored rows [j0, j0 + nrows), of which
 // `logits` holds the logits; those at or past *count are zeros in what they
 // write, or not written.  The other arrays are indexed by row.
-//   select:    idx, count[0], INT_MIN in count[1], the result block (CeMisc; or
-//              null), and logp and lse (or null) of the rows that are not scored;
+//   select:    idx and, from idx + rows on, their targets; count[0], INT_MIN in
+//              count[1], tag in count[2]; the result block (CeMisc; or null), and logp
+//              and lse (or null) of the rows that are not scored;
 //   gather:    the scored rows of hn side by side;   scatter: back, other rows 0;
 //   grad_rows: the logits become their gradients;
 //   finish:    the mean of -logp, summed in f64 in a fixed order.
-hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, float* logp,
-                              float* lse, void* misc, hipStream_t st);
+hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, int tag,
+                              float* logp, float* lse, void* misc, hipStream_t st);
 hipError_t launch_logp_gather(const float* hn, const int* idx, const int* count, float* out, size_t rows, size_t d,
                               hipStream_t st);
 hipError_t launch_logp_scatter(const float* in, const int* idx, const int* count, float* dhn, size_t rows, size_t d,
@@ -221,13 +222,15 @@ hipError_t launch_logp_few(const float* hn, const float* head, const int64_t* ta
 //   dhead:     what `rows` of them from `local` (a multiple of 128) on add to dhead
 //              (acc 0: give as dhead), in scratch of up(rows, 32) v_pad 4 bytes and vocab words;
 //   zero_rows: dhn of the rows that are not scored.
+// What a forward of other sizes kept (count[2] is not the plan's tag) counts as no
+// scored row, and gives NaN gradients.
 struct HeadPlan {
-    int k16, splits_max;  // 16-k steps of a row
+    int k16, splits_max, tag;  // 16-k steps of a row
     size_t t_pad, v_pad, d_pad, chunk;
     size_t rows_bytes, head_bytes, back_bytes, stats_bytes, keep_bytes, factor_bytes, rows_back_bytes, part_bytes;
 };
 struct HeadBuffers {
-    int *idx, *count, *exponents;        // [t], [2], [v_pad / 32]
+    int *idx, *count, *exponents;        // [2 t], [4], [v_pad / 32]
     char *rows, *packed, *back, *keep, *rows_back;  // operands
     float *scale, *xt, *factor, *part;   // scale [t_pad], xt [chunk]
     void* stats;
@@ -235,14 +238,14 @@ struct HeadBuffers {
 HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes);
 hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float* hn, const float* head, size_t d,
                             size_t vocab, hipStream_t st);
-hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, size_t j0, size_t vocab,
+hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, size_t t, size_t j0, size_t vocab,
                              float* logp, float* lse, hipStream_t st);
-hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* head,
+hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* head,
                            const float* dlogp, size_t j0, size_t d, float* dhn, hipStream_t st);
-hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* dlogp,
+hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* dlogp,
                              size_t j0, size_t local, size_t rows, size_t d, size_t vocab, char* packed_dlogits,
                              unsigned* col_top, float* dhead, int acc, hipStream_t st);
-hipError_t launch_head_zero_rows(const int64_t* targets, size_t t, size_t vocab, float* dhn, size_t d,
+hipError_t launch_head_zero_rows(const HeadPlan& p, const HeadBuffers& b, size_t t, float* dhn, size_t d,
                                  hipStream_t st);
 
 }  // namespace cfattn

@@ -29,6 +29,7 @@
 // stage goes to LDS by direct loads of whole KiB and is read without bank
 // conflicts, and no wave spends instructions on splitting.
 #include <hip/hip_runtime.h>
+#include <limits.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -98,13 +99,18 @@ __device__ __forceinline__ void load8(float (&x)[8], const float* row, int k, in
     }
 }
 
+// Scored rows of [j0, j0 + chunk); none where `count` is another plan's.
+__device__ __forceinline__ int scored_rows(const int* __restrict__ count, int tag, int j0, int chunk) {
+    return count[2] == tag ? max(min(count[0] - j0, chunk), 0) : 0;
+}
+
 struct PackArgs {
     const float *hn, *head;
     const int *idx, *count;
     char *rows, *packed, *back, *rows_back;  // rows and rows_back may be null
     float* scale;
     int *exponents, *largest;
-    int row_blocks, vocab, d, k16, v16, t16, vec_rows, vec_head;
+    int row_blocks, vocab, d, k16, v16, t16, vec_rows, vec_head, tag;
 };
 
 // 32 rows to a workgroup, as operands [32 rows][16 k][piece]: first the scored rows
@@ -128,7 +134,7 @@ __global__ __launch_bounds__(64 * NW) void pack_kernel(const PackArgs g) {
     if (is_head) {
         if (r < g.vocab) row = g.head + (long)r * d;
     } else {
-        const int n = *g.count;
+        const int n = scored_rows(g.count, g.tag, 0, INT_MAX);
         if (blk * 32 >= (n + kBN - 1) / kBN * kBN) return;
         if (r < n) row = g.hn + (long)g.idx[r] * d;
     }
@@ -232,12 +238,12 @@ struct HeadArgs {
     int ka, kb;         // 16-k steps from one 32 rows of a (of b) to the next
     int mt, nt;         // tiles along a, and (head) along b
     const int* count;   // scored rows
+    int tag;
     int j0, chunk;      // this launch's: [j0, min(j0 + chunk, count)); b, stats, keep and part start at j0
     long ld;            // of stats, xt and factor
     // statistics: a is the head
-    const int *exponents, *largest, *idx;
+    const int *exponents, *largest, *targets;  // targets: of scored rows
     const float* scale;
-    const int64_t* targets;
     int vocab, v16;
     float2* stats;      // [128 rows of the head][ld]: max and sum of exp2, in log2 units
     float* xt;          // the targets' logits
@@ -277,8 +283,9 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
     __shared__ __attribute__((aligned(1024))) char lds[kStages * STAGE];
     const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1, l32 = lane & 31, hh = lane >> 5;
-    const int n = max(min(wave_uniform(*g.count) - g.j0, g.chunk), 0);
-    if (n == 0 && !(P == Product::kHead && !g.acc)) return;
+    const int n = wave_uniform(scored_rows(g.count, g.tag, g.j0, g.chunk));
+    const bool other = P == Product::kHead && wave_uniform(g.count[2]) != g.tag;
+    if (n == 0 && !(P == Product::kHead && (!g.acc || other))) return;
     const int nt = P == Product::kHead ? g.nt : (n + kBN - 1) / kBN;
     // Items of an XCD: a contiguous run of the tiles along a (of the splits), every
     // tile along b with each.
@@ -403,7 +410,7 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
 #pragma unroll
                 for (int q = 0; q < 16; q++) {
                     const int v = min(v0 + 8 * (q >> 2) + (q & 3), g.vocab - 1);
-                    u[q] = exp2i(group_exponent(__builtin_bit_cast(float, g.col_top[v])));
+                    u[q] = other ? __builtin_nanf("") : exp2i(group_exponent(__builtin_bit_cast(float, g.col_top[v])));
                 }
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
@@ -449,11 +456,10 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
             for (int j = 0; j < 2; j++) {
                 const int col = col0 + 32 * j + l32;
                 const bool scored = col < n;
-                const long r = scored ? g.idx[g.j0 + col] : 0;
                 const int et = (int)(__builtin_bit_cast(uint32_t, g.scale[g.j0 + col]) >> 23) - 127;
                 // The target's row within this wave's part; the rows of q lie at 4 hh.
-                const long target = (scored ? g.targets[r] : -1) - m0;
-                const int at = (int)(target >= 0 && target < 32 * MB ? target : -1000) - 4 * hh;
+                const int target = (scored ? g.targets[g.j0 + col] : -1) - m0;
+                const int at = (target >= 0 && target < 32 * MB ? target : -1000) - 4 * hh;
                 if (live < 32 * MB) {
                     const int end = live - 4 * hh;
 #pragma unroll
@@ -532,12 +538,12 @@ __device__ __forceinline__ float2 join(const float2& a, const float2& b) {
 __global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restrict__ stats, long ld, int parts,
                                                            int all_parts, const float* __restrict__ xt,
                                                            const int* __restrict__ idx, const int* __restrict__ count,
-                                                           int j0, int chunk, float* __restrict__ logp,
+                                                           int tag, int j0, int chunk, float* __restrict__ logp,
                                                            float* __restrict__ lse, float* __restrict__ factor) {
     __shared__ float2 red[16][16];
     __shared__ float lse2[16];
     const int c = threadIdx.x & 15, p0 = threadIdx.x >> 4, j = blockIdx.x * 16 + c;
-    const int n = min(*count - j0, chunk);
+    const int n = scored_rows(count, tag, j0, chunk);
     if ((int)blockIdx.x * 16 >= (n + kBN - 1) / kBN * kBN) return;
     float2 a = make_float2(-INFINITY, 0.0f);
     if (j < n)
@@ -568,13 +574,13 @@ __global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restr
 __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __restrict__ part, int chunk, int rows,
                                                                int mt, int k16, int splits_max,
                                                                const int* __restrict__ idx,
-                                                               const int* __restrict__ count, int j0,
-                                                               const int64_t* __restrict__ targets,
+                                                               const int* __restrict__ targets,
+                                                               const int* __restrict__ count, int tag, int j0,
                                                                const float* __restrict__ head,
                                                                const float* __restrict__ dlogp,
                                                                const int* __restrict__ largest,
                                                                float* __restrict__ dhn, int d) {
-    const int n = min(*count - j0, chunk);
+    const int n = scored_rows(count, tag, j0, chunk);
     const int quads = (d + 3) / 4;
     const long at = (long)blockIdx.x * 256 + threadIdx.x;
     const int col = (int)(at / quads), i0 = (int)(at % quads) * 4;
@@ -591,7 +597,7 @@ __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __re
         for (int z = 0; z < 8; z++) s.x += x[z].x, s.y += x[z].y, s.z += x[z].z, s.w += x[z].w;
     }
     const long r = idx[j0 + col];
-    const float* w = head + targets[r] * d + i0;
+    const float* w = head + (long)targets[j0 + col] * d + i0;
     float* out = dhn + r * d + i0;
     const float f = dlogp[r], u = pow2_clamped(*largest - 15), t[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
@@ -603,13 +609,12 @@ __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __re
 struct DlogitsArgs {
     const char* keep;     // from row j0 on
     const float* factor;
-    const int *exponents, *largest, *idx, *count;
-    const int64_t* targets;
+    const int *exponents, *largest, *idx, *targets, *count;
     const float *dlogp, *scale;
     unsigned* col_top;
     char* out;            // [32 columns][t16][piece]
     long ld;
-    int v16, t16, j0, chunk, vocab;
+    int v16, t16, tag, j0, chunk, vocab;
 };
 
 // A bound of every column's dlogits times their rows' 2^e: a column's power of two is
@@ -618,7 +623,7 @@ struct DlogitsArgs {
 // (f16, to 2^-11): 128 columns and every 8th 32 rows to a workgroup.
 __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
-    const int n = min(*g.count - g.j0, g.chunk);
+    const int n = scored_rows(g.count, g.tag, g.j0, g.chunk);
     float top[2][8] = {};
     const float u = pow2_clamped(*g.largest - g.exponents[blockIdx.x * 4 + wave] - 15);
     for (int t0 = 32 * blockIdx.y; t0 < n; t0 += 32 * gridDim.y) {
@@ -635,7 +640,7 @@ __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) 
         }
         // (One workgroup of the columns sees to a row's target.)
         if (blockIdx.x == 0 && wave == 0 && hh == 0)
-            atomicMax(g.col_top + g.targets[g.idx[g.j0 + j]], __builtin_bit_cast(unsigned, finite_abs(row)));
+            atomicMax(g.col_top + g.targets[g.j0 + j], __builtin_bit_cast(unsigned, finite_abs(row)));
     }
 #pragma unroll
     for (int q = 0; q < 2; q++)
@@ -654,13 +659,13 @@ __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) 
 __global__ __launch_bounds__(256) void head_pack_dlogits_kernel(const DlogitsArgs g) {
     __shared__ float tile[32][129];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
-    const int n = min(*g.count - g.j0, g.chunk), t0 = blockIdx.y * 32, j = t0 + l32;
+    const int n = scored_rows(g.count, g.tag, g.j0, g.chunk), t0 = blockIdx.y * 32, j = t0 + l32;
     if (t0 >= n) return;
     const bool scored = j < n;
     const long r = scored ? g.idx[g.j0 + j] : 0;
     const float row = scored ? g.dlogp[r] * g.scale[g.j0 + j] : 0.0f;
     const float f = scored ? g.factor[blockIdx.x * g.ld + j] * pow2_clamped(*g.largest - g.exponents[blockIdx.x * 4 + wave] - 15) : 0.0f;
-    const int target = scored ? (int)g.targets[r] - (int)blockIdx.x * 128 : -1;
+    const int target = scored ? g.targets[g.j0 + j] - (int)blockIdx.x * 128 : -1;
 #pragma unroll
     for (int q = 0; q < 2; q++) {
         const int s = 2 * wave + q;  // 16 columns
@@ -686,12 +691,22 @@ __global__ __launch_bounds__(256) void head_pack_dlogits_kernel(const DlogitsArg
     }
 }
 
-// Zeros in the rows that are not scored.
-__global__ __launch_bounds__(256) void head_zero_rows_kernel(const int64_t* __restrict__ targets, long vocab,
+// Zeros in the rows that are not among the ascending idx.
+__global__ __launch_bounds__(256) void head_zero_rows_kernel(const int* __restrict__ idx,
+                                                             const int* __restrict__ count, int tag,
                                                              float* __restrict__ dhn, int d) {
-    const long r = blockIdx.x;
-    if (targets[r] >= 0 && targets[r] < vocab) return;
-    for (int i = threadIdx.x; i < d; i += 256) dhn[r * d + i] = 0.0f;
+    const int r = blockIdx.x, n = scored_rows(count, tag, 0, INT_MAX);
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (idx[mid] < r)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    if (lo < n && idx[lo] == r) return;
+    const float x = count[2] == tag ? 0.0f : __builtin_nanf("");
+    for (int i = threadIdx.x; i < d; i += 256) dhn[(long)r * d + i] = x;
 }
 
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -706,6 +721,7 @@ constexpr int kSplitsMax = 32;
 
 HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes) {
     HeadPlan p{};
+    p.tag = (int)((uint32_t)t * 0x9E3779B1u ^ (uint32_t)d * 0x85EBCA77u ^ (uint32_t)vocab * 0xC2B2AE3Du ^ 0x6C6F6770u);
     p.k16 = (int)((d + 15) / 16);
     p.v_pad = up(vocab, 256);
     p.t_pad = up(t, kBN);
@@ -733,6 +749,7 @@ hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float
     g.scale = b.scale, g.exponents = b.exponents, g.largest = b.count + 1, g.row_blocks = (int)(p.t_pad / 32);
     g.vocab = (int)vocab, g.d = (int)d, g.k16 = p.k16, g.v16 = (int)(p.v_pad / 16);
     g.vec_rows = d % 4 == 0 && aligned16(hn), g.vec_head = d % 4 == 0 && aligned16(head);
+    g.tag = p.tag;
     const size_t blocks = (p.t_pad + (head ? p.v_pad : 0)) / 32;
     const int pairs = (p.k16 + 1) / 2;
     auto pack = [&](auto back, auto nw, auto u) {
@@ -759,29 +776,29 @@ hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float
     return hipGetLastError();
 }
 
-hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, size_t j0, size_t vocab,
+hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, size_t t, size_t j0, size_t vocab,
                              float* logp, float* lse, hipStream_t st) {
     HeadArgs g{};
     g.a = b.packed, g.b = b.rows + j0 / 32 * p.k16 * 2 * kFrag, g.ka = g.kb = p.k16, g.mt = (int)(p.v_pad / 256);
     g.count = b.count, g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.exponents = b.exponents;
-    g.largest = b.count + 1, g.idx = b.idx, g.scale = b.scale, g.targets = targets, g.vocab = (int)vocab;
+    g.largest = b.count + 1, g.targets = b.idx + t, g.scale = b.scale, g.tag = p.tag, g.vocab = (int)vocab;
     g.v16 = (int)(p.v_pad / 16), g.stats = static_cast<float2*>(b.stats), g.xt = b.xt, g.keep = b.keep;
     hipLaunchKernelGGL((head_gemm_kernel<4, Product::kStats>), dim3(kWgs), dim3(256), 0, st, g);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)(p.chunk / 16)), dim3(1024), 0, st, g.stats, g.ld,
-                       (int)((vocab + 127) / 128), (int)(p.v_pad / 128), b.xt, b.idx, b.count, (int)j0, (int)p.chunk,
-                       logp, lse, b.keep ? b.factor : nullptr);
+                       (int)((vocab + 127) / 128), (int)(p.v_pad / 128), b.xt, b.idx, b.count, p.tag, (int)j0,
+                       (int)p.chunk, logp, lse, b.keep ? b.factor : nullptr);
     return hipGetLastError();
 }
 
-hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* head,
+hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* head,
                            const float* dlogp, size_t j0, size_t d, float* dhn, hipStream_t st) {
     const int mb = back_mb(d);
     HeadArgs g{};
     g.a = b.back, g.b = b.keep, g.ka = g.kb = (int)(p.v_pad / 16), g.mt = (int)(p.d_pad / (64 * mb)), g.count = b.count;
     g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.factor = b.factor, g.part = b.part;
-    g.splits_max = p.splits_max;
+    g.splits_max = p.splits_max, g.tag = p.tag;
     if (mb == 3)
         hipLaunchKernelGGL((head_gemm_kernel<3, Product::kRows>), dim3(kWgs), dim3(256), 0, st, g);
     else
@@ -790,17 +807,17 @@ hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, const int64_
     if (e != hipSuccess) return e;
     const size_t quads = p.chunk * ((d + 3) / 4);
     hipLaunchKernelGGL(head_grad_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, b.part, (int)p.chunk,
-                       (int)p.d_pad, g.mt, g.ka, g.splits_max, b.idx, b.count, (int)j0, targets, head, dlogp,
-                       b.count + 1, dhn, (int)d);
+                       (int)p.d_pad, g.mt, g.ka, g.splits_max, b.idx, b.idx + t, b.count, p.tag, (int)j0, head,
+                       dlogp, b.count + 1, dhn, (int)d);
     return hipGetLastError();
 }
 
-hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, const int64_t* targets, const float* dlogp,
+hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* dlogp,
                              size_t j0, size_t local, size_t rows, size_t d, size_t vocab, char* packed_dlogits,
                              unsigned* col_top, float* dhead, int acc, hipStream_t st) {
     DlogitsArgs g{};
     g.keep = b.keep + local * p.v_pad * 4, g.factor = b.factor + local, g.exponents = b.exponents;
-    g.largest = b.count + 1, g.idx = b.idx, g.count = b.count, g.targets = targets, g.dlogp = dlogp;
+    g.largest = b.count + 1, g.idx = b.idx, g.count = b.count, g.targets = b.idx + t, g.dlogp = dlogp, g.tag = p.tag;
     g.scale = b.scale, g.col_top = col_top, g.out = packed_dlogits, g.ld = (long)p.chunk, g.v16 = (int)(p.v_pad / 16);
     g.t16 = (int)(up(rows, 32) / 16), g.j0 = (int)(j0 + local), g.chunk = (int)rows, g.vocab = (int)vocab;
     hipError_t e = launch_fill_zero(reinterpret_cast<float*>(col_top), vocab, st);
@@ -813,14 +830,14 @@ hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, const int6
     HeadArgs h{};
     h.a = packed_dlogits, h.b = b.rows_back + (j0 + local) / 16 * 2 * kFrag, h.ka = g.t16, h.kb = (int)(p.t_pad / 16);
     h.mt = (int)(p.v_pad / 256), h.nt = (int)((d + kBN - 1) / kBN), h.count = b.count, h.j0 = g.j0, h.chunk = g.chunk;
-    h.vocab = (int)vocab, h.col_top = col_top, h.dhead = dhead, h.d = (int)d, h.acc = acc;
+    h.tag = p.tag, h.vocab = (int)vocab, h.col_top = col_top, h.dhead = dhead, h.d = (int)d, h.acc = acc;
     hipLaunchKernelGGL((head_gemm_kernel<4, Product::kHead>), dim3(kWgs), dim3(256), 0, st, h);
     return hipGetLastError();
 }
 
-hipError_t launch_head_zero_rows(const int64_t* targets, size_t t, size_t vocab, float* dhn, size_t d,
+hipError_t launch_head_zero_rows(const HeadPlan& p, const HeadBuffers& b, size_t t, float* dhn, size_t d,
                                  hipStream_t st) {
-    hipLaunchKernelGGL(head_zero_rows_kernel, dim3((unsigned)t), dim3(256), 0, st, targets, (long)vocab, dhn, (int)d);
+    hipLaunchKernelGGL(head_zero_rows_kernel, dim3((unsigned)t), dim3(256), 0, st, b.idx, b.count, p.tag, dhn, (int)d);
     return hipGetLastError();
 }
 

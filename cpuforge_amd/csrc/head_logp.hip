@@ -23,12 +23,13 @@ __device__ __forceinline__ MaxSum merge(const MaxSum& a, const MaxSum& b) {
     return {m, sa + sb};
 }
 
-// The scored rows (targets within the vocabulary): idx[0..n) in row order, n
-// at *count; the result's counts; logp and lse of the other rows, 0 where the
+// The scored rows (targets within the vocabulary) and their targets: idx[0..n) and
+// idx[rows..rows + n) in row order, n and the caller's tag at count[0] and
+// count[2]; the result's counts; logp and lse of the other rows, 0 where the
 // target is ignored and NaN where it is out of range.  One workgroup: 1024
 // targets a round, their places from a scan.
 __global__ __launch_bounds__(1024) void logp_select_kernel(const int64_t* __restrict__ targets, long rows, long vocab,
-                                                           int* __restrict__ idx, int* __restrict__ count,
+                                                           int* __restrict__ idx, int* __restrict__ count, int tag,
                                                            float* __restrict__ logp, float* __restrict__ lse,
                                                            CeMisc* __restrict__ misc) {
     __shared__ int wave_n[16], bad_row;
@@ -53,7 +54,11 @@ __global__ __launch_bounds__(1024) void logp_select_kernel(const int64_t* __rest
             at += w < wave ? wave_n[w] : 0;
             n += wave_n[w];
         }
-        if (scored) idx[at + __popcll(m & ((1ull << lane) - 1))] = (int)r;
+        if (scored) {
+            at += __popcll(m & ((1ull << lane) - 1));
+            idx[at] = (int)r;
+            idx[rows + at] = (int)t;
+        }
         __syncthreads();
     }
 #pragma unroll
@@ -63,6 +68,7 @@ __global__ __launch_bounds__(1024) void logp_select_kernel(const int64_t* __rest
     if (threadIdx.x == 0) {
         count[0] = n;
         count[1] = INT_MIN;  // the largest exponent that head_gemm.hip's pack finds
+        count[2] = tag;
         if (misc) {
             int all = 0;
             for (int w = 0; w < 16; w++) all += wave_n[w];
@@ -259,10 +265,10 @@ __global__ __launch_bounds__(1024) void logp_finish_kernel(const int64_t* __rest
 
 }  // namespace
 
-hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, float* logp,
-                              float* lse, void* misc, hipStream_t st) {
+hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, int tag,
+                              float* logp, float* lse, void* misc, hipStream_t st) {
     hipLaunchKernelGGL(logp_select_kernel, dim3(1), dim3(1024), 0, st, targets, (long)rows, (long)vocab, idx, count,
-                       logp, lse, static_cast<CeMisc*>(misc));
+                       tag, logp, lse, static_cast<CeMisc*>(misc));
     return hipGetLastError();
 }
 hipError_t launch_logp_gather(const float* hn, const int* idx, const int* count, float* out, size_t rows, size_t d,

@@ -427,6 +427,8 @@ def policy_loss(logp, old_logp, ref_logp, advantages, targets, offsets, dlogp, r
     sequences.  No host wait."""
     ctx = ctx or default_context()
     rows, seqs = logp.numel(), offsets.numel() - 1
+    if seqs < 0:
+        raise _lib.ShapeError(_lib.ERR_SHAPE, "offsets of sequences have one entry more than those, got none")
     if reduction not in POLICY_REDUCTIONS:
         raise ValueError(f"unknown reduction {reduction!r}")
     if per_token is None:

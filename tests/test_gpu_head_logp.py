@@ -179,6 +179,36 @@ def test_a_row_that_is_not_finite_stays_alone(t):
     assert torch.equal(logp[keep], logp2[keep]) and torch.equal(dhn[keep], dhn2[keep])
 
 
+def test_what_another_forward_kept_gives_nan():
+    """A keep of another shape is not followed; one whose targets have changed
+    since is the forward's."""
+    from cpuforge_amd import ops as P
+    hn, head, tg, g = inputs(300, 64, 900, 20)
+    _, lse, _ = forward(hn, head, tg)
+    other = kept(*inputs(700, 64, 1300, 21)[:3])
+    assert other.numel() >= P.lm_head_logprobs_keep_bytes(300, 64, 900)
+    for acc in (True, False):
+        dhn, dhead = backward(hn, head, tg, lse, g, keep=other, acc=acc)
+        assert bool(torch.isnan(dhn).all()) and bool(torch.isnan(dhead).all())
+    keep = kept(hn, head, tg)
+    want = backward(hn, head, tg, lse, g, keep=keep)
+    got = backward(hn, head, tg + 10 ** 6, lse, g, keep=keep)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+def test_sizes_past_the_limits_are_refused():
+    from cpuforge_amd import ops as P
+    from cpuforge_amd.attention import default_context
+    ctx, res = default_context(), P.ce_result_buffer(DEV)
+    f, b = ctx._lib.cfops_lm_head_logprobs, ctx._lib.cfops_lm_head_logprobs_backward
+    for t, d, vocab in ((1 << 24, 8, 8), (8, 1 << 31, 8), (8, 8, 1 << 26)):
+        assert f(ctx.handle, None, None, None, t, d, vocab, None, None, res.data_ptr(), None, 0,
+                 None) == _lib.ERR_UNSUPPORTED
+        assert b(ctx.handle, None, None, None, None, None, t, d, vocab, None, None, 1, None, 0,
+                 None) == _lib.ERR_UNSUPPORTED
+        assert P.lm_head_logprobs_keep_bytes(t, d, vocab) == 0
+
+
 def test_no_rows():
     from cpuforge_amd import ops as P
     e = torch.empty(0, device=DEV)

@@ -267,6 +267,10 @@ def test_refusals():
             P.policy_loss(x, x, None, rew, None, o, x, res, **kw)
     with pytest.raises(_lib.ShapeError):
         P.policy_loss(x, x, None, torch.zeros(3, device=DEV), None, o, x, res, clip_low=0.1, clip_high=0.1)
+    for f in (lambda o: P.policy_loss(x, x, None, x, None, o, x, res, clip_low=0.1, clip_high=0.1),
+              lambda o: P.preference_loss(x, x, None, o, x, rew, res, beta=0.1)):
+        with pytest.raises(_lib.ShapeError):
+            f(o[:0])
 
 
 def test_captured_losses_replay():
