@@ -775,7 +775,7 @@ int cfops_preference_loss(cfattn_ctx* c, const float* logp, const float* ref_log
         return fail(c, CFATTN_ERR_ARG, "label_smoothing must be in [0, 1), and 0 for the hinge and squared forms");
     CF_TRY(check_sequences(c, rows, pairs));
     int rc = CFATTN_OK;
-    void* scratch = slot(c, cfattn_ctx::OPS_SEQ, cfattn::preference_scratch_bytes(pairs), &rc);
+    void* scratch = slot(c, cfattn_ctx::OPS_SEQ, cfattn::preference_scratch_bytes(rows, pairs), &rc);
     if (!scratch) return rc;
     cfattn::PreferenceArgs a{};
     a.logp = logp, a.ref_logp = ref_logp, a.targets = targets, a.offsets = offsets, a.rows = (long)rows;
@@ -800,7 +800,7 @@ int cfops_policy_loss(cfattn_ctx* c, const float* logp, const float* old_logp, c
         return fail(c, CFATTN_ERR_ARG, "unknown reduction %d", reduction);
     CF_TRY(check_sequences(c, rows, seqs));
     int rc = CFATTN_OK;
-    void* scratch = slot(c, cfattn_ctx::OPS_SEQ, cfattn::policy_scratch_bytes(seqs), &rc);
+    void* scratch = slot(c, cfattn_ctx::OPS_SEQ, cfattn::policy_scratch_bytes(rows, seqs), &rc);
     if (!scratch) return rc;
     cfattn::PolicyArgs a{};
     a.logp = logp, a.old_logp = old_logp, a.ref_logp = ref_logp, a.advantages = advantages, a.targets = targets;

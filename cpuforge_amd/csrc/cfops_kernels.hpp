@@ -155,9 +155,11 @@ struct PreferenceArgs {
     double beta, margin, label_smoothing;
     float *dlogp, *rewards;
     PreferenceResult* result;
-    double* terms;  // set by launch_preference
+    // set by launch_preference: each part's sum and scored rows, parts to a sequence
+    double2* terms;
+    int parts;
 };
-size_t preference_scratch_bytes(size_t pairs);
+size_t preference_scratch_bytes(size_t rows, size_t pairs);
 hipError_t launch_preference(PreferenceArgs a, void* scratch, hipStream_t st);
 
 struct PolicyResult {
@@ -172,10 +174,11 @@ struct PolicyArgs {
     double low, high, log_low, log_high, kl_coef;  // the ratio's borders and their logarithms
     float* dlogp;
     PolicyResult* result;
-    double* terms;  // set by launch_policy, as counts
-    int* counts;
+    // set by launch_policy: each part's terms and scored rows, parts to a sequence
+    double* terms;
+    int *counts, parts;
 };
-size_t policy_scratch_bytes(size_t seqs);
+size_t policy_scratch_bytes(size_t rows, size_t seqs);
 hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st);
 
 // Log-probabilities of the targets (head_logp.hip).  Rows whose target is within

@@ -9,6 +9,12 @@
 // that a ratio falls on (a difference against the border's logarithm, to f64).
 // Offsets that do not rise within [0, rows] are not followed: their sequence is
 // empty, the loss is NaN and the result names it.
+//
+// A pass over a sequence needs what another pass summed over it (a pair's rewards;
+// the rows or sequences that a mean is over), so there are two or three launches, each
+// with `parts` workgroups to a sequence: long ones are split, and a part's sums are
+// added in order by whoever needs them.  Bound by those launches: 400 pairs of 2 x 1024
+// rows (13 MB) 9.3 us, 1024 rollouts of 1100 (32 MB) 21 us.
 #include <limits.h>
 
 #include <algorithm>
@@ -59,6 +65,15 @@ __device__ __forceinline__ bool is_scored(const int64_t* __restrict__ targets, l
 }
 
 constexpr int kRows = 2;  // rows of a lane whose loads are in flight together
+constexpr int kWaves = 4;  // of a part's workgroup
+constexpr size_t kWgs = 1024;
+
+// Part p of a sequence's rows.
+__device__ __forceinline__ Span part_of(const Span& s, long p, int parts) {
+    const unsigned n = (unsigned)(s.hi - s.lo);
+    const long size = (n + (unsigned)parts - 1) / (unsigned)parts;
+    return {s.lo + min(size * p, (long)n), s.lo + min(size * (p + 1), (long)n), s.bad};
+}
 
 // log(1 + exp(x)).
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
@@ -79,53 +94,70 @@ __device__ __forceinline__ void preference_term(const PreferenceArgs& a, double 
     }
 }
 
-// One pair, by NW waves (of a workgroup of as many, or each on its own with NW == 1).
+// The sum over rows [s.lo, s.hi) of logp - ref_logp and the scored rows, by NW waves from
+// lane `tid` on.
 template <int NW>
-__device__ __forceinline__ void one_pair(const PreferenceArgs& a, long pair, double* red) {
-    const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const Span s[2] = {span(a.offsets, 2 * pair, a.rows), span(a.offsets, 2 * pair + 1, a.rows)};
-    double sums[4] = {};  // of either sequence, and its scored rows
+__device__ __forceinline__ void preference_rows(const PreferenceArgs& a, const Span& s, int tid, double (&sums)[2],
+                                                double* red) {
+    sums[0] = sums[1] = 0.0;
+    for (long r0 = s.lo + tid; r0 < s.hi; r0 += kRows * 64 * NW) {
+        float x[kRows], y[kRows];
+        bool use[kRows];
 #pragma unroll
-    for (int k = 0; k < 2; k++)
-        for (long r0 = s[k].lo + tid; r0 < s[k].hi; r0 += kRows * 64 * NW) {
-            float x[kRows], y[kRows];
-            bool use[kRows];
-#pragma unroll
-            for (int i = 0; i < kRows; i++) {
-                const long r = r0 + i * 64 * NW, at = min(r, s[k].hi - 1);
-                use[i] = is_scored(a.targets, at) && r < s[k].hi;
-                x[i] = a.logp[at];
-                y[i] = a.ref_logp ? a.ref_logp[at] : 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < kRows; i++)
-                if (use[i]) {
-                    sums[k] += (double)x[i] - (double)y[i];
-                    sums[2 + k] += 1.0;
-                }
+        for (int i = 0; i < kRows; i++) {
+            const long r = r0 + i * 64 * NW, at = min(r, s.hi - 1);
+            use[i] = is_scored(a.targets, at) && r < s.hi;
+            x[i] = a.logp[at];
+            y[i] = a.ref_logp ? a.ref_logp[at] : 0.0f;
         }
+#pragma unroll
+        for (int i = 0; i < kRows; i++)
+            if (use[i]) {
+                sums[0] += (double)x[i] - (double)y[i];
+                sums[1] += 1.0;
+            }
+    }
     group_sums<NW>(sums, red);
-    double reward[2], share[2];
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        share[k] = a.length_mean ? a.beta / fmax(sums[2 + k], 1.0) : a.beta;
-        reward[k] = sums[k] * share[k];
+}
+
+// A sequence's reward and what a row's log-probability moves it by, from its parts'
+// sums: lane `lane` of `lanes` (a power of two).
+struct Reward {
+    double value, share;
+};
+__device__ __forceinline__ Reward reward_of(const PreferenceArgs& a, long seq, int lane, int lanes) {
+    double x = 0.0, n = 0.0;
+    for (int i = lane; i < a.parts; i += lanes) {
+        const double2 t = a.terms[seq * a.parts + i];
+        x += t.x, n += t.y;
     }
-    double l, dz;
-    preference_term(a, reward[0] - reward[1] - a.margin, l, dz);
-    dz /= (double)a.pairs;
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const float d = (float)(k ? -dz * share[k] : dz * share[k]);
+    for (int o = lanes >> 1; o >= 1; o >>= 1) x += __shfl_xor(x, o), n += __shfl_xor(n, o);
+    const double share = a.length_mean ? a.beta / fmax(n, 1.0) : a.beta;
+    return {x * share, share};
+}
+
+struct Pair {
+    Reward chosen, rejected;
+    double loss, dz;
+};
+__device__ __forceinline__ Pair one_pair(const PreferenceArgs& a, long pair, int lane, int lanes) {
+    Pair p;
+    p.chosen = reward_of(a, 2 * pair, lane, lanes);
+    p.rejected = reward_of(a, 2 * pair + 1, lane, lanes);
+    preference_term(a, p.chosen.value - p.rejected.value - a.margin, p.loss, p.dz);
+    return p;
+}
+
+// The gradient of sequence `seq` of the pair in rows [s.lo, s.hi), and its reward.
+template <int NW>
+__device__ __forceinline__ void preference_grad(const PreferenceArgs& a, const Pair& p, long seq, const Span& s, int tid,
+                                                bool first) {
+    const double dz = p.dz / (double)a.pairs, up = dz * p.chosen.share, down = -dz * p.rejected.share;
+    const float d = seq & 1 ? (float)down : (float)up;
 #pragma unroll 4
-        for (long r = s[k].lo + tid; r < s[k].hi; r += 64 * NW) a.dlogp[r] = is_scored(a.targets, r) ? d : 0.0f;
-    }
-    if (tid == 0) {
-        a.rewards[2 * pair] = (float)reward[0];
-        a.rewards[2 * pair + 1] = (float)reward[1];
-        a.terms[2 * pair] = s[0].bad || s[1].bad ? __builtin_nan("") : l;
-        a.terms[2 * pair + 1] = reward[0] - reward[1];
-    }
+    for (long r = s.lo + tid; r < s.hi; r += 64 * NW) a.dlogp[r] = is_scored(a.targets, r) ? d : 0.0f;
+    const float chosen = (float)p.chosen.value, rejected = (float)p.rejected.value;
+    if (first && tid == 0) a.rewards[seq] = seq & 1 ? rejected : chosen;
 }
 
 // The first sequence whose offsets do not rise within the rows, by a workgroup of NW
@@ -141,37 +173,63 @@ __device__ __forceinline__ int first_bad(const int64_t* __restrict__ offsets, lo
     return first;
 }
 
-// The result from the pairs' terms, by one workgroup of NW waves.
+// The result, by one workgroup of NW waves.
 template <int NW>
 __device__ __forceinline__ void preference_result(const PreferenceArgs& a, double* red) {
+    int lanes = 1;  // to a pair
+    while (lanes < min(a.parts, 64)) lanes *= 2;
+    const int lane = threadIdx.x & (lanes - 1);
     double sums[3] = {};
-    for (long i = threadIdx.x; i < a.pairs; i += 64 * NW) {
-        sums[0] += a.terms[2 * i];
-        sums[1] += a.terms[2 * i + 1] > 0.0;
-        sums[2] += a.terms[2 * i + 1];
+    for (long i = threadIdx.x / lanes; i < a.pairs; i += 64 * NW / lanes) {
+        const Pair p = one_pair(a, i, lane, lanes);
+        if (lane) continue;
+        sums[0] += p.loss;
+        const double more = p.chosen.value - p.rejected.value;
+        sums[1] += more > 0.0;
+        sums[2] += more;
     }
     const int bad = first_bad<NW>(a.offsets, 2 * a.pairs, a.rows);
     group_sums<NW>(sums, red);
     if (threadIdx.x == 0) {
         const double n = (double)a.pairs;
-        *a.result = {bad, (float)(sums[0] / n), (float)(sums[1] / n), (float)(sums[2] / n)};
+        *a.result = {bad, bad == INT_MAX ? (float)(sums[0] / n) : __builtin_nanf(""), (float)(sums[1] / n),
+                     (float)(sums[2] / n)};
     }
 }
 
+// A wave to a sequence, then to its gradient: one workgroup, parts == 1.
 __global__ __launch_bounds__(1024) void preference_small_kernel(const PreferenceArgs a) {
     __shared__ double red[3 * 16];
-    for (long pair = threadIdx.x >> 6; pair < a.pairs; pair += 16) one_pair<1>(a, pair, red);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (long i = wave; i < 2 * a.pairs; i += 16) {
+        double sums[2];
+        preference_rows<1>(a, span(a.offsets, i, a.rows), lane, sums, red);
+        if (lane == 0) a.terms[i] = make_double2(sums[0], sums[1]);
+    }
     __threadfence_block();
     __syncthreads();
+    for (long i = wave; i < 2 * a.pairs; i += 16)
+        preference_grad<1>(a, one_pair(a, i / 2, 0, 1), i, span(a.offsets, i, a.rows), lane, true);
     preference_result<16>(a, red);
 }
-__global__ __launch_bounds__(512) void preference_pair_kernel(const PreferenceArgs a) {
-    __shared__ double red[4 * 8];
-    one_pair<8>(a, blockIdx.x, red);
+__global__ __launch_bounds__(64 * kWaves) void preference_sum_kernel(const PreferenceArgs a) {
+    __shared__ double red[2 * kWaves];
+    const long seq = blockIdx.x / (unsigned)a.parts;
+    const int part = (int)(blockIdx.x % (unsigned)a.parts);
+    double sums[2];
+    preference_rows<kWaves>(a, part_of(span(a.offsets, seq, a.rows), part, a.parts), threadIdx.x, sums, red);
+    if (threadIdx.x == 0) a.terms[blockIdx.x] = make_double2(sums[0], sums[1]);
 }
-__global__ __launch_bounds__(1024) void preference_finish_kernel(const PreferenceArgs a) {
-    __shared__ double red[3 * 16];
-    preference_result<16>(a, red);
+// The first workgroup has the result, the others a part's gradient each.
+__global__ __launch_bounds__(64 * kWaves) void preference_grad_kernel(const PreferenceArgs a) {
+    __shared__ double red[3 * kWaves];
+    if (blockIdx.x == 0) return preference_result<kWaves>(a, red);
+    const unsigned b = blockIdx.x - 1;
+    const long seq = b / (unsigned)a.parts;
+    const int part = (int)(b % (unsigned)a.parts);
+    const bool one = a.parts == 1;
+    const Pair p = one_pair(a, seq / 2, one ? 0 : threadIdx.x & 63, one ? 1 : 64);
+    preference_grad<kWaves>(a, p, seq, part_of(span(a.offsets, seq, a.rows), part, a.parts), threadIdx.x, part == 0);
 }
 
 // ------------------------------------------------------------------- policy
@@ -190,20 +248,32 @@ __device__ __forceinline__ double count_rows(const PolicyArgs& a, const Span& s,
     group_sums<NW>(n, red);
     return n[0];
 }
-__global__ __launch_bounds__(256) void policy_count_kernel(const PolicyArgs a) {
-    __shared__ double red[4];
-    const double n = count_rows<4>(a, span(a.offsets, blockIdx.x, a.rows), threadIdx.x, red);
+__global__ __launch_bounds__(64 * kWaves) void policy_count_kernel(const PolicyArgs a) {
+    __shared__ double red[kWaves];
+    const Span s = span(a.offsets, blockIdx.x / (unsigned)a.parts, a.rows);
+    const double n = count_rows<kWaves>(a, part_of(s, blockIdx.x % (unsigned)a.parts, a.parts), threadIdx.x, red);
     if (threadIdx.x == 0) a.counts[blockIdx.x] = (int)n;
 }
 
-// N, the scored rows, and M, the sequences with any, by a workgroup of NW waves.
+// N, the scored rows, and, for means over sequences, M, those with any, by a workgroup
+// of NW waves.
 template <int NW>
 __device__ __forceinline__ void totals(const PolicyArgs& a, double& n, double& m, double* red) {
     double x[2] = {};
-    for (long i = threadIdx.x; i < a.seqs; i += 64 * NW) {
-        const int c = a.counts[i];
-        x[0] += c;
-        x[1] += c > 0;
+    if (a.sequence_mean) {
+        int lanes = 1;  // to a sequence
+        while (lanes < min(a.parts, 64)) lanes *= 2;
+        const int lane = threadIdx.x & (lanes - 1);
+        for (long i = threadIdx.x / lanes; i < a.seqs; i += 64 * NW / lanes) {
+            int c = 0;
+            for (int p = lane; p < a.parts; p += lanes) c += a.counts[i * a.parts + p];
+            for (int o = lanes >> 1; o >= 1; o >>= 1) c += __shfl_xor(c, o);
+            if (lane) continue;
+            x[0] += c;
+            x[1] += c > 0;
+        }
+    } else {
+        for (long i = threadIdx.x; i < a.seqs * a.parts; i += 64 * NW) x[0] += a.counts[i];
     }
     group_sums<NW>(x, red);
     n = x[0], m = x[1];
@@ -258,8 +328,11 @@ __device__ __forceinline__ void policy_rows(const PolicyArgs& a, long seq, const
 }
 
 __device__ __forceinline__ double row_weight(const PolicyArgs& a, long seq, double n, double m) {
-    const double c = fmax((double)a.counts[seq], 1.0);
-    return a.sequence_mean ? 1.0 / (c * fmax(m, 1.0)) : 1.0 / fmax(n, 1.0);
+    if (!a.sequence_mean) return 1.0 / fmax(n, 1.0);
+    int c = 0;
+    for (int p = threadIdx.x & 63; p < a.parts; p += 64) c += a.counts[seq * a.parts + p];
+    for (int o = 32; o >= 1; o >>= 1) c += __shfl_xor(c, o);
+    return 1.0 / (fmax((double)c, 1.0) * fmax(m, 1.0));
 }
 
 template <int NW>
@@ -271,7 +344,7 @@ __device__ __forceinline__ void policy_result(const PolicyArgs& a, double (&sums
                      (float)(sums[2] / fmax(n, 1.0))};
 }
 
-// A wave to a sequence, one workgroup for all.
+// A wave to a sequence, one workgroup for all, parts == 1.
 __global__ __launch_bounds__(1024) void policy_small_kernel(const PolicyArgs a) {
     __shared__ double red[3 * 16];
     const int lane = threadIdx.x & 63;
@@ -288,21 +361,22 @@ __global__ __launch_bounds__(1024) void policy_small_kernel(const PolicyArgs a) 
     policy_result<16>(a, sums, n, red);
 }
 
-// A workgroup to a sequence: its terms go to `terms`.
-__global__ __launch_bounds__(256) void policy_seq_kernel(const PolicyArgs a) {
-    __shared__ double red[3 * 4];
+// A part's gradient; its terms go to `terms`.
+__global__ __launch_bounds__(64 * kWaves) void policy_part_kernel(const PolicyArgs a) {
+    __shared__ double red[3 * kWaves];
     double n, m, sums[3] = {};
-    totals<4>(a, n, m, red);
-    const long i = blockIdx.x;
-    policy_rows<4>(a, i, span(a.offsets, i, a.rows), row_weight(a, i, n, m), threadIdx.x, sums);
-    group_sums<4>(sums, red);
-    if (threadIdx.x < 3) a.terms[3 * i + threadIdx.x] = threadIdx.x == 0 ? sums[0] : threadIdx.x == 1 ? sums[1] : sums[2];
+    totals<kWaves>(a, n, m, red);
+    const long seq = blockIdx.x / (unsigned)a.parts;
+    const Span s = part_of(span(a.offsets, seq, a.rows), blockIdx.x % (unsigned)a.parts, a.parts);
+    policy_rows<kWaves>(a, seq, s, row_weight(a, seq, n, m), threadIdx.x, sums);
+    group_sums<kWaves>(sums, red);
+    if (threadIdx.x < 3) a.terms[3l * blockIdx.x + threadIdx.x] = threadIdx.x == 0 ? sums[0] : threadIdx.x == 1 ? sums[1] : sums[2];
 }
 __global__ __launch_bounds__(1024) void policy_finish_kernel(const PolicyArgs a) {
     __shared__ double red[3 * 16];
     double n, m, sums[3] = {};
     totals<16>(a, n, m, red);
-    for (long i = threadIdx.x; i < a.seqs; i += 1024)
+    for (long i = threadIdx.x; i < a.seqs * a.parts; i += 1024)
 #pragma unroll
         for (int k = 0; k < 3; k++) sums[k] += a.terms[3 * i + k];
     policy_result<16>(a, sums, n, red);
@@ -310,35 +384,56 @@ __global__ __launch_bounds__(1024) void policy_finish_kernel(const PolicyArgs a)
 
 }  // namespace
 
-size_t preference_scratch_bytes(size_t pairs) { return 2 * std::max<size_t>(pairs, 1) * sizeof(double); }
-size_t policy_scratch_bytes(size_t seqs) {
-    return std::max<size_t>(seqs, 1) * (3 * sizeof(double) + sizeof(int));
+// One workgroup, a wave to a sequence, where that is a few reads long: it is bound by
+// latency, and so is a second launch.  Us of a captured call (of one from the host, which
+// a launch takes longer to issue than to run), against the form for many:
+//   preference: 8 sequences, 1024 rows 7.1 (7.4) and 5.9 (10.0); 2 of 1000 9.6 and 6.5;
+//   policy:     8 sequences, 1024 rows 8.2 (8.3) and 12 (13.5);  1 of 1000 16.7 and 12.
+static bool small(size_t rows, size_t seqs) { return seqs <= 16 && rows <= 1024 && rows <= 256 * seqs; }
+// Workgroups to a sequence: with few long sequences as many as fill the card, of no
+// fewer than two rows a lane on average.  (One of 65536 rows: preference 61 and policy
+// 195 us by one workgroup, 6.8 and 12.6 by 128.  As many to every sequence, 128 of 128
+// rows by 8 each: 22 where one takes 6.)
+static int parts_of(size_t rows, size_t seqs) {
+    if (small(rows, seqs)) return 1;
+    return (int)std::max<size_t>(1, std::min(kWgs / seqs, rows / (seqs * kRows * 64 * kWaves)));
+}
+
+size_t preference_scratch_bytes(size_t rows, size_t pairs) {
+    return 2 * pairs * parts_of(rows, 2 * pairs) * sizeof(double2);
+}
+size_t policy_scratch_bytes(size_t rows, size_t seqs) {
+    return seqs * parts_of(rows, seqs) * (3 * sizeof(double) + sizeof(int));
 }
 
 hipError_t launch_preference(PreferenceArgs a, void* scratch, hipStream_t st) {
-    a.terms = static_cast<double*>(scratch);
-    if (a.rows <= 16384 && a.pairs <= 64) {
+    a.terms = static_cast<double2*>(scratch);
+    a.parts = parts_of(a.rows, 2 * a.pairs);
+    if (small(a.rows, 2 * a.pairs)) {
         hipLaunchKernelGGL(preference_small_kernel, dim3(1), dim3(1024), 0, st, a);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)a.pairs), dim3(512), 0, st, a);
+    const unsigned wgs = (unsigned)(2 * a.pairs * a.parts);
+    hipLaunchKernelGGL(preference_sum_kernel, dim3(wgs), dim3(64 * kWaves), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(preference_finish_kernel, dim3(1), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(preference_grad_kernel, dim3(wgs + 1), dim3(64 * kWaves), 0, st, a);
     return hipGetLastError();
 }
 
 hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st) {
+    a.parts = parts_of(a.rows, a.seqs);
     a.terms = static_cast<double*>(scratch);
-    a.counts = reinterpret_cast<int*>(a.terms + 3 * std::max<size_t>(a.seqs, 1));
-    if (a.rows <= 16384 && a.seqs <= 64) {
+    a.counts = reinterpret_cast<int*>(a.terms + 3 * a.seqs * a.parts);
+    if (small(a.rows, a.seqs)) {
         hipLaunchKernelGGL(policy_small_kernel, dim3(1), dim3(1024), 0, st, a);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL(policy_count_kernel, dim3((unsigned)a.seqs), dim3(256), 0, st, a);
+    const unsigned wgs = (unsigned)(a.seqs * a.parts);
+    hipLaunchKernelGGL(policy_count_kernel, dim3(wgs), dim3(64 * kWaves), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(policy_seq_kernel, dim3((unsigned)a.seqs), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(policy_part_kernel, dim3(wgs), dim3(64 * kWaves), 0, st, a);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(1024), 0, st, a);

@@ -229,6 +229,43 @@ def test_policy_gradient_against_differences():
 
 BAD = [[0, 5, 4, 9, 12], [0, 5, 8, 9, 13], [-1, 5, 8, 9, 12], [0, 5, 8, 2 ** 40, 12], [-2 ** 62, 2 ** 62, 3, 4, 5]]
 
+# Few long sequences, whose rows many workgroups share, beside ones with nothing.
+SPLIT = [[40000, 3], [1500, 1700, 0, 1600, 1, 2500, 1200, 900], [8192] * 6, [1023, 1025, 4097, 511, 513, 0, 7000, 2]]
+
+
+@pytest.mark.parametrize("lengths", SPLIT, ids=lambda x: f"{len(x)}x{max(x)}")
+def test_sequences_of_many_workgroups(lengths):
+    off, tg, logp, ref, old = seqs(lengths, sum(lengths), lead=5, tail=4)
+    tg[off[-2]:off[-1]] = IGN
+    for form, mean in (("sigmoid", True), ("squared", False)):
+        got = run_preference(off, tg, logp, ref, beta=0.2, form=form, length_mean=mean)
+        check_preference(got, preference(off, tg, logp, ref, 0.2, form, 0.0, 0.0, mean), logp, off, 0.2)
+    for reduction in ("token", "sequence"):
+        for per_token in (True, False):
+            adv = np.random.RandomState(5).randn(len(logp) if per_token else len(lengths)).astype(np.float32)
+            got = run_policy(off, tg, logp, old, ref, adv, clip_low=0.2, clip_high=0.3, kl_coef=0.05,
+                             per_token=per_token, reduction=reduction)
+            check_policy(got, policy(off, tg, logp, old, ref, adv, per_token, 0.2, 0.3, 0.05, reduction), 20.0)
+
+
+def test_bad_offsets_among_many_workgroups():
+    off, tg, logp, ref, old = seqs([5000] * 4, 8)
+    off[2] = len(logp) + 1  # sequences 1 and 2 do not rise within the rows
+    from cpuforge_amd import ops as P
+    t = lambda x: torch.from_numpy(x).to(DEV)  # noqa: E731
+    d, rew = torch.full((len(logp),), 77.0, device=DEV), torch.empty(4, device=DEV)
+    res = torch.empty(P.PREFERENCE_RESULT_WORDS, dtype=torch.int32, device=DEV)
+    P.preference_loss(t(logp), t(ref), t(tg), t(off), d, rew, res, beta=0.1)
+    with pytest.raises(_lib.CfattnError, match="sequence 1"):
+        P.preference_check(res)
+    assert P.preference_result(res).loss.isnan() and (d[5000:15000] == 77.0).all()
+    pres = torch.empty(P.POLICY_RESULT_WORDS, dtype=torch.int32, device=DEV)
+    d.fill_(77.0)
+    P.policy_loss(t(logp), t(old), None, torch.ones(4, device=DEV), t(tg), t(off), d, pres, clip_low=0.2, clip_high=0.2)
+    with pytest.raises(_lib.CfattnError, match="sequence 1"):
+        P.policy_check(pres)
+    assert P.policy_result(pres).loss.isnan() and (d[5000:15000] == 77.0).all()
+
 
 @pytest.mark.parametrize("off", BAD)
 def test_offsets_that_do_not_rise_are_not_followed(off):
