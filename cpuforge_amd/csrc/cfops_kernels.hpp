@@ -228,7 +228,7 @@ hipError_t launch_logp_few(const float* hn, const float* head, const int64_t* ta
 // What a forward of other sizes kept (count[2] is not the plan's tag) counts as no
 // scored row, and gives NaN gradients.
 struct HeadPlan {
-    int k16, splits_max, tag;  // 16-k steps of a row
+    int k16, splits_max, back_mb, tag;  // 16-k steps of a row
     size_t t_pad, v_pad, d_pad, chunk;
     size_t rows_bytes, head_bytes, back_bytes, stats_bytes, keep_bytes, factor_bytes, rows_back_bytes, part_bytes;
 };

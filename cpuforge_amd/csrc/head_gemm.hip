@@ -262,13 +262,16 @@ struct HeadArgs {
 // XCDs, so that one XCD's L2 holds what its workgroups share.  The one with the
 // least rounds of an XCD's share over its 64 workgroups times its length; a split's
 // partial sums cost their way through memory.
-__device__ __forceinline__ int splits_of(int tiles, int k16, int splits_max) {
-    int best = 8;
-    float least = INFINITY;
+struct Splits {
+    int count;
+    float cost;  // in steps of a tile
+};
+__host__ __device__ __forceinline__ Splits splits_of(int tiles, int k16, int splits_max) {
+    Splits best{8, INFINITY};
     for (int s = 8; s <= splits_max; s += 8) {
         const int rounds = (tiles * (s / 8) + kWgs / 8 - 1) / (kWgs / 8);
         const float cost = rounds * ((k16 + s - 1) / s + 24.0f) + 0.35f * tiles * s / 64.0f;
-        if (cost < least) least = cost, best = s;
+        if (cost < best.cost) best = {s, cost};
     }
     return best;
 }
@@ -292,7 +295,7 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
     const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
     int outer = g.mt, inner = nt;
     if constexpr (ROWS) {
-        outer = wave_uniform(splits_of(g.mt * nt, g.ka, g.splits_max));
+        outer = wave_uniform(splits_of(g.mt * nt, g.ka, g.splits_max).count);
         inner = g.mt * nt;
     }
     const int o0 = (int)((long)outer * xcd / 8), o1 = (int)((long)outer * (xcd + 1) / 8);
@@ -585,7 +588,7 @@ __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __re
     const long at = (long)blockIdx.x * 256 + threadIdx.x;
     const int col = (int)(at / quads), i0 = (int)(at % quads) * 4;
     if (col >= n) return;
-    const int splits = splits_of(mt * ((n + kBN - 1) / kBN), k16, splits_max);  // (a multiple of 8)
+    const int splits = splits_of(mt * ((n + kBN - 1) / kBN), k16, splits_max).count;  // (a multiple of 8)
     const float* p = part + (long)col * rows + i0;
     const long step = (long)chunk * rows;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -712,9 +715,6 @@ __global__ __launch_bounds__(256) void head_zero_rows_kernel(const int* __restri
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 size_t up(size_t x, size_t to) { return (x + to - 1) / to * to; }
 
-// Blocks of 32 columns of the head of a wave in the gradient's product (its sums
-// take twice the registers): three where that pads little, else two.
-int back_mb(size_t d) { return 10 * up(d, 192) <= 11 * up(d, 128) ? 3 : 2; }
 constexpr int kSplitsMax = 32;
 
 }  // namespace
@@ -725,11 +725,23 @@ HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes) {
     p.k16 = (int)((d + 15) / 16);
     p.v_pad = up(vocab, 256);
     p.t_pad = up(t, kBN);
-    p.d_pad = up(d, 64 * back_mb(d));
     p.chunk = std::min(std::max<size_t>(chunk_bytes / (p.v_pad * 4) / kBN * kBN, kBN), p.t_pad);
-    p.splits_max = (int)std::min<size_t>(
-        kSplitsMax, std::max<size_t>(8, ((size_t)256 << 20) / (p.chunk * p.d_pad * sizeof(float)) / 8 * 8));
-    p.splits_max = (int)std::min<size_t>(p.splits_max, std::max<size_t>(8, p.v_pad / 256 / 8 * 8));
+    // Blocks of 32 columns of the head of a wave in the rows' gradient (whose sums take
+    // twice the registers): two or three, by which the tiles fill the card better, were
+    // all rows scored.  (Us of the product by three and by two: 500 x 2048 x 49152 372 and
+    // 306, 300 x 576 x 49152 97 and 78, 1000 x 768 x 32000 159 and 183, 2000 x 129 x 49152
+    // 143 and 168.)
+    float least = INFINITY;
+    for (int mb = 3; mb >= 2; mb--) {
+        const size_t d_pad = up(d, 64 * mb);
+        const size_t most = std::min(((size_t)256 << 20) / (p.chunk * d_pad * sizeof(float)), p.v_pad / 256) / 8 * 8;
+        const int splits_max = (int)std::min<size_t>(std::max<size_t>(most, 8), kSplitsMax);
+        const Splits s = splits_of((int)(d_pad / (64 * mb) * (p.chunk / kBN)), (int)(p.v_pad / 16), splits_max);
+        const float cost = (mb == 3 ? 2.9f : 2.0f) * s.cost;
+        if (cost >= least) continue;
+        least = cost;
+        p.back_mb = mb, p.d_pad = d_pad, p.splits_max = splits_max;
+    }
     p.rows_bytes = p.t_pad * p.k16 * 64;
     p.head_bytes = p.v_pad * p.k16 * 64;
     p.back_bytes = p.d_pad * p.v_pad * 4;
@@ -794,7 +806,7 @@ hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, size_t t, 
 
 hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* head,
                            const float* dlogp, size_t j0, size_t d, float* dhn, hipStream_t st) {
-    const int mb = back_mb(d);
+    const int mb = p.back_mb;
     HeadArgs g{};
     g.a = b.back, g.b = b.keep, g.ka = g.kb = (int)(p.v_pad / 16), g.mt = (int)(p.d_pad / (64 * mb)), g.count = b.count;
     g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.factor = b.factor, g.part = b.part;
