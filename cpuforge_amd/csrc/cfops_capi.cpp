@@ -558,7 +558,7 @@ void keep_at(const cfattn::HeadPlan& p, size_t t, char* base, cfattn::HeadBuffer
 }
 
 // The forward's scratch; with no keep, the small parts of it are scratch too.
-int head_scratch(cfattn_ctx* c, const cfattn::HeadPlan& p, size_t t, cfattn::HeadBuffers& b) {
+int head_scratch(cfattn_ctx* c, const cfattn::HeadPlan& p, size_t t, cfattn::HeadBuffers& b, bool mid = false) {
     char *rows = nullptr, *stats = nullptr;
     CF_TRY(take(c, cfattn_ctx::OPS_ROWS, p.rows_bytes + p.t_pad * sizeof(float), rows));
     b.rows = rows;
@@ -566,7 +566,7 @@ int head_scratch(cfattn_ctx* c, const cfattn::HeadPlan& p, size_t t, cfattn::Hea
     CF_TRY(take(c, cfattn_ctx::OPS_STATS, p.stats_bytes + p.chunk * sizeof(float), stats));
     b.stats = stats;
     b.xt = reinterpret_cast<float*>(stats + p.stats_bytes);
-    CF_TRY(take(c, cfattn_ctx::OPS_HEAD, p.head_bytes, b.packed));
+    if (!mid) CF_TRY(take(c, cfattn_ctx::OPS_HEAD, p.head_bytes, b.packed));
     if (b.count) return CFATTN_OK;
     CF_TRY(take(c, cfattn_ctx::OPS_IDX, (4 + 2 * t + p.v_pad / 32) * sizeof(int), b.count));
     b.idx = b.count + 4;
@@ -589,10 +589,15 @@ int logprobs_many(cfattn_ctx* c, const float* hn, const float* head, const int64
         CF_TRY(check_keep(c, keep, keep_bytes, keep_layout(p, t).bytes));
         keep_at(p, t, static_cast<char*>(keep), b);
     }
-    CF_TRY(head_scratch(c, p, t, b));
+    const bool mid = !keep && cfattn::logp_takes_mid(t, d, head);
+    CF_TRY(head_scratch(c, p, t, b, mid));
     CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, b.idx, b.count, p.tag, logp, lse, result, st),
            "log-probability launch");
-    CF_HIP(c, cfattn::launch_head_pack(p, b, hn, head, d, vocab, st), "log-probability launch");
+    CF_HIP(c, cfattn::launch_head_pack(p, b, hn, mid ? nullptr : head, d, vocab, st), "log-probability launch");
+    if (mid) {
+        CF_HIP(c, cfattn::launch_head_mid(p, b, head, t, d, vocab, logp, lse, st), "log-probability launch");
+        return CFATTN_OK;
+    }
     CF_HIP(c, cfattn::launch_head_stats(p, b, t, 0, vocab, logp, lse, st), "log-probability launch");
     return CFATTN_OK;
 }
@@ -710,13 +715,14 @@ int cfops_lm_head_logprobs(cfattn_ctx* c, const float* hn, const float* head, co
         CF_HIP(c, cfattn::launch_ce_begin(targets, 0, result, st), "log-probability launch");
         return CFATTN_OK;
     }
-    if (t <= cfattn::kLogpFew) {
+    if (cfattn::logp_takes_few(t, vocab)) {
         char* scratch = nullptr;
         CF_TRY(take(c, cfattn_ctx::OPS_STATS, cfattn::logp_few_bytes(t, vocab), scratch));
         CF_HIP(c, cfattn::launch_logp_few(hn, head, targets, t, d, vocab, logp, lse, result, scratch, st),
                "log-probability launch");
         return CFATTN_OK;
     }
+    if (t <= cfattn::kLogpFew) keep = nullptr;
     CF_TRY(logprobs_many(c, hn, head, targets, t, d, vocab, logp, lse, result, keep, keep_bytes, st));
     CF_HIP(c, cfattn::launch_logp_finish(targets, logp, t, result, st), "log-probability launch");
     return CFATTN_OK;

@@ -203,11 +203,21 @@ hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const in
                                  hipStream_t st);
 hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t rows, void* misc, hipStream_t st);
 // All of the forward for at most kLogpFew rows in two launches, in scratch of
-// logp_few_bytes(t, vocab).  (us against the packed operands, 576 x 49152 and 2048 x
-// 128256: 32 rows 56 and 83, 415 and 631; 48 rows 88 and 85, 754 and 632; the
-// gradients' f32 products against theirs 128 and 183, 682 and 1167 at 32 rows, with
-// the forward's part of keeping 182 and 186, 1084 and 1176.)
+// logp_few_bytes(t, vocab).  Up to as many rows nothing is kept for the gradients, whose
+// f32 products take, against those over packed operands with what the forward keeps for
+// them, at 32 rows 182 and 186 us (576 x 49152), 1084 and 1176 (2048 x 128256).
 constexpr size_t kLogpFew = 32;
+// Which form takes the forward, us of a call by either (rows, d x vocab):
+//   few or mid: 16 rows 576 x 49152 37 and 43, 2048 x 128256 267 and 249; 17 rows 46 and
+//   44, 319 and 252; where mid's workgroups of 128 rows of the head do not fill half of the
+//   card it has the latency of d for itself: 32 rows 2048 x 1000 55 and 90;
+//   mid or packed: 256 rows 576 x 49152 82 and 93, 2048 x 128256 512 and 744, 384 rows 115
+//   and 115, 726 and 906, 512 rows 129 and 123, 961 and 1066; with rows of the head that are
+//   read value by value 128 rows 129 x 49152 39 and 38, 256 rows 49 and 44.
+inline bool logp_takes_few(size_t t, size_t vocab) { return t <= 16 || (t <= kLogpFew && vocab <= 16384); }
+inline bool logp_takes_mid(size_t t, size_t d, const float* head) {
+    return t <= (d % 4 == 0 && (uintptr_t)head % 16 == 0 ? 384 : 128);
+}
 size_t logp_few_bytes(size_t t, size_t vocab);
 hipError_t launch_logp_few(const float* hn, const float* head, const int64_t* targets, size_t t, size_t d, size_t vocab,
                            float* logp, float* lse, void* misc, void* scratch, hipStream_t st);
@@ -241,6 +251,8 @@ struct HeadBuffers {
 HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes);
 hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float* hn, const float* head, size_t d,
                             size_t vocab, hipStream_t st);
+hipError_t launch_head_mid(const HeadPlan& p, const HeadBuffers& b, const float* head, size_t t, size_t d, size_t vocab,
+                           float* logp, float* lse, hipStream_t st);
 hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, size_t t, size_t j0, size_t vocab,
                              float* logp, float* lse, hipStream_t st);
 hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* head,

@@ -535,6 +535,156 @@ __device__ __forceinline__ float2 join(const float2& a, const float2& b) {
     return make_float2(t, (a.y == 0.0f ? 0.0f : a.y * exp2f(a.x - t)) + (b.y == 0.0f ? 0.0f : b.y * exp2f(b.x - t)));
 }
 
+struct MidArgs {
+    const float* head;
+    const char* rows;     // packed
+    const int *count, *targets;  // targets: of scored rows
+    const float* scale;
+    float2* stats;        // [128 rows of the head][ld]
+    float* xt;
+    long ld;
+    int vocab, d, k16, tag, groups, tiles, vec;
+};
+constexpr int kMidK = 4;  // 16-k steps of a chunk
+
+// Statistics of a few hundred rows at most, the head split into pieces on its way from
+// memory: where it is used by few tiles of tokens, packing it first costs more than its
+// products (2048 x 128256 408 us).  128 rows of the head and 32 NB tokens to a workgroup, 32
+// rows to a wave, whose pieces stay in registers; the tokens' operands go through LDS for
+// all four waves.  The power of two of a wave's rows is that of the largest value so far:
+// where a chunk has one that f16 does not hold, the sums are scaled down (rarely: after the
+// first chunk one bit of room is left).  So it ends no higher than the packed head's.
+// Bound by reading the head up to 64 rows (2048 x 128256 in all 250 us, 1.05 GB at 4.8 TB/s
+// 220), by splitting it again for every 128 rows from there on.
+template <int NB>
+__global__ __launch_bounds__(256, 2) void head_mid_kernel(const MidArgs g) {
+    constexpr int CHUNK = NB * kMidK * 2 * kFrag;  // bytes of a chunk's operands of the tokens
+    __shared__ __attribute__((aligned(1024))) char lds[2 * CHUNK];
+    __shared__ float2 red[4][32 * NB];
+    const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6), l32 = lane & 31, hh = lane >> 5;
+    const int n = wave_uniform(scored_rows(g.count, g.tag, 0, INT_MAX));
+    // The tiles of tokens of 128 rows of the head follow one another on one XCD.
+    const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
+    const int group = local / g.tiles * 8 + xcd, col0 = local % g.tiles * 32 * NB;
+    if (group >= g.groups || col0 >= n) return;
+    const int m0 = group * 128 + wave * 32;
+    const float* row = g.head + (long)min(m0 + l32, g.vocab - 1) * g.d;
+    const uint32_t lds0 = lds_offset(lds), voff = lane * 16;
+    const int chunks = (g.k16 + kMidK - 1) / kMidK;
+    auto load_head = [&](float (&x)[kMidK][8], int c) {
+        const int k = c * 16 * kMidK + 8 * hh;
+        if (g.vec && (c + 1) * 16 * kMidK <= g.d) {
+#pragma unroll
+            for (int s = 0; s < kMidK; s++) load8(x[s], row, k + 16 * s, INT_MAX, true);
+        } else {
+#pragma unroll
+            for (int s = 0; s < kMidK; s++) load8(x[s], row, k + 16 * s, g.d, g.vec);
+        }
+    };
+    auto load_rows = [&](int c) {
+        const int steps = min(kMidK, g.k16 - c * kMidK);
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            const int at = 2 * NB * wave + i, j = at / (2 * kMidK), s = at % (2 * kMidK);  // block, KiB of it
+            if (s / 2 < steps)
+                lds_load16_so(g.rows + (((long)(col0 / 32 + j) * g.k16 + c * kMidK) * 2 + s) * kFrag, voff,
+                              lds0 + (c & 1) * CHUNK + at * kFrag);
+        }
+    };
+    f32x16 acc[NB];
+#pragma unroll
+    for (int j = 0; j < NB; j++) acc[j] = zero16();
+    float x[kMidK][8], next[kMidK][8];
+    int e = -112;
+    load_rows(0);
+    load_head(x, 0);
+    for (int c = 0; c < chunks; c++) {
+        // The chunk's operands are there, and no wave reads the other buffer any more.
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (c + 1 < chunks) {
+            load_rows(c + 1);
+            load_head(next, c + 1);
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kMidK; s++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[s][i]));
+        if (__any(top * exp2i(-e) > 65504.0f)) {
+            top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kMidK; s++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, finite_abs(x[s][i]));
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+            const int more = wave_uniform(max(e, group_exponent(top)));
+            const float down = pow2_clamped(e - more);
+            e = more;
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+                for (int q = 0; q < 16; q++) acc[j][q] *= down;
+        }
+        const float sc = exp2i(-e);
+        const char* b = lds + (c & 1) * CHUNK + voff;
+#pragma unroll
+        for (int s = 0; s < kMidK; s++) {
+            if (c * kMidK + s >= g.k16) break;
+            const Pieces a = split8(x[s], sc);
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                const f16x8 h = *reinterpret_cast<const f16x8*>(b + ((j * kMidK + s) * 2) * kFrag);
+                const f16x8 l = *reinterpret_cast<const f16x8*>(b + ((j * kMidK + s) * 2 + 1) * kFrag);
+                acc[j] = mfma_f16(a.l, h, acc[j]);
+                acc[j] = mfma_f16(a.h, l, acc[j]);
+                acc[j] = mfma_f16(a.h, h, acc[j]);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < kMidK; s++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[s][i] = next[s][i];
+    }
+    const int live = g.vocab - m0;  // rows of the head of this wave
+#pragma unroll
+    for (int j = 0; j < NB; j++) {
+        const int col = col0 + 32 * j + l32;
+        const int et = (int)(__builtin_bit_cast(uint32_t, g.scale[col]) >> 23) - 127;
+        const int target = (col < n ? g.targets[col] : -1) - m0;
+        const int at = (target >= 0 && target < 32 ? target : -1000) - 4 * hh;
+        float t = 0.0f;
+        bool hit = false;
+#pragma unroll
+        for (int q = 0; q < 16; q++) {
+            const int r = 8 * (q >> 2) + (q & 3);
+            hit |= r == at;
+            t = r == at ? acc[j][q] : t;
+            if (r + 4 * hh >= live) acc[j][q] = -INFINITY;
+        }
+        if (hit) g.xt[col] = t * pow2_clamped(e + et);
+        const float c = pow2_clamped(e + et) * kLog2e;
+        float m = acc[j][0];
+#pragma unroll
+        for (int q = 1; q < 16; q++) m = fmaxf(m, acc[j][q]);
+        m = max_halves(m * c);
+        float sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 16; q++) sum += __builtin_amdgcn_exp2f(fmaf(acc[j][q], c, -m));
+        sum = sum_halves(sum);
+        if (hh == 0) red[wave][32 * j + l32] = live > 0 ? make_float2(m, sum) : make_float2(-INFINITY, 0.0f);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32 * NB && col0 + (int)threadIdx.x < n) {
+        float2 a = red[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < 4; w++) a = join(a, red[w][threadIdx.x]);
+        g.stats[(long)group * g.ld + col0 + threadIdx.x] = a;
+    }
+}
+
 // lse and logp (or null) of scored rows [j0, ..) from their parts' maxima and sums,
 // and what the gradient scales a part by (or null).  16 rows to a workgroup, lane l
 // has row l % 16, so that a part's are read side by side.
@@ -801,6 +951,23 @@ hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, size_t t, 
     hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)(p.chunk / 16)), dim3(1024), 0, st, g.stats, g.ld,
                        (int)((vocab + 127) / 128), (int)(p.v_pad / 128), b.xt, b.idx, b.count, p.tag, (int)j0,
                        (int)p.chunk, logp, lse, b.keep ? b.factor : nullptr);
+    return hipGetLastError();
+}
+
+hipError_t launch_head_mid(const HeadPlan& p, const HeadBuffers& b, const float* head, size_t t, size_t d, size_t vocab,
+                           float* logp, float* lse, hipStream_t st) {
+    MidArgs g{};
+    g.head = head, g.rows = b.rows, g.count = b.count, g.targets = b.idx + t, g.scale = b.scale;
+    g.stats = static_cast<float2*>(b.stats), g.xt = b.xt, g.ld = (long)p.chunk, g.vocab = (int)vocab, g.d = (int)d;
+    g.k16 = p.k16, g.tag = p.tag, g.groups = (int)((vocab + 127) / 128), g.vec = d % 4 == 0 && aligned16(head);
+    const bool two = t <= 64;
+    g.tiles = (int)((t + (two ? 63 : 127)) / (two ? 64 : 128));
+    hipLaunchKernelGGL(two ? head_mid_kernel<2> : head_mid_kernel<4>, dim3((unsigned)((g.groups + 7) / 8 * 8 * g.tiles)),
+                       dim3(256), 0, st, g);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)(p.chunk / 16)), dim3(1024), 0, st, g.stats, g.ld, g.groups,
+                       g.groups, b.xt, b.idx, b.count, p.tag, 0, (int)p.chunk, logp, lse, nullptr);
     return hipGetLastError();
 }
 

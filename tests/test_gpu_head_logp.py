@@ -113,6 +113,58 @@ def test_log_probabilities_and_gradients_match_64_bits(t, d, vocab):
     check(*inputs(t, d, vocab, t + d + vocab))
 
 
+def check_forward(hn, head, tg):
+    """The forward alone, without and, where there is one, with a keep."""
+    from cpuforge_amd import ops as P
+    vocab = head.shape[0]
+    w_logp, w_lse, _, _, _, off, x = reference(hn, head, tg, torch.zeros(hn.shape[0], device=DEV))
+    tol = off + U * (vocab / 512 + 32 + (x.amax(1) - x.amin(1)).clamp(max=104.0) + w_lse.abs() * 2)
+    tol = torch.where(tg != IGN, tol, 0.0)
+    n = P.lm_head_logprobs_keep_bytes(*hn.shape, vocab)
+    for keep in (None, torch.empty(n, dtype=torch.uint8, device=DEV) if n else None):
+        logp, lse, _ = forward(hn, head, tg, keep=keep)
+        assert bool(((lse - w_lse).abs() <= tol).all()), (lse - w_lse).abs().max()
+        assert bool(((logp - w_logp).abs() <= tol + off + U * (w_logp.abs() + 2 * w_lse.abs())).all())
+
+
+# The forms of the forward by rows (to 16, to 384, more) and alignment, at their borders.
+FORWARD = [(16, 64, 16385), (17, 64, 16385), (32, 500, 20000), (33, 8, 127), (64, 129, 1000), (65, 577, 3001),
+           (128, 129, 129), (129, 129, 257), (384, 576, 4097), (385, 576, 4097), (200, 2050, 1025), (100, 64, 1),
+           (97, 1, 300), (383, 68, 20000)]
+
+
+@pytest.mark.parametrize("t,d,vocab", FORWARD)
+@pytest.mark.parametrize("masked", [0.0, 0.9])
+def test_forward_of_every_form(t, d, vocab, masked):
+    print(t, d, vocab, masked, flush=True)
+    check_forward(*inputs(t, d, vocab, t * d + vocab, masked)[:3])
+
+
+@pytest.mark.parametrize("d", [256, 257])
+def test_forward_of_a_head_off_its_alignment(d):
+    hn, head, tg, _ = inputs(80, d, 900, 31)
+    off = torch.empty(900 * d + 1, device=DEV)[1:].view(900, d)
+    check_forward(hn, off.copy_(head), tg)
+
+
+@pytest.mark.parametrize("t", [40, 200, 500])
+def test_forward_where_later_columns_are_larger(t):
+    """Weights that grow by 2^10 along a row, whose power of two follows the
+    largest value met so far.  (What their pieces lose, 2^-39 of the largest
+    |hn| 2^2 times the largest |head| 2^9 in each of 600 products, 2^-19 in all, is
+    within the bound of f32 products, 2^-22 of a sum of 20 or more.)"""
+    hn, head, tg, _ = inputs(t, 600, 700, 33)
+    assert (hn.abs() @ head.abs().T).amin() > 20
+    up = torch.exp2(torch.arange(600, device=DEV) / 60)
+    check_forward(hn / up, head * up, tg)
+    check_forward(hn * up, head / up, tg)
+    head[:, 599] *= 3e4
+    check_forward(hn, head, tg)
+    head[300:310] *= 1e-30
+    head[310:320] = 0.0
+    check_forward(hn, head, tg)
+
+
 @pytest.mark.parametrize("masked", [0.0, 0.97, 1.0])
 @pytest.mark.parametrize("t", [9, 400])
 def test_masks(t, masked):
