@@ -301,10 +301,12 @@ def lm_head_logprobs(hn, head, targets):
 
 def preference_loss(logp, ref_logp, targets, offsets, **kw):
     """(loss, rewards [2 * pairs], result block) of ops.preference_loss, whose
-    keywords it takes; logp's gradient is the loss's."""
+    keywords it takes.  The loss's gradient flows to logp alone: ref_logp is a
+    constant, and the rewards carry none."""
     return PreferenceLossFn.apply(logp, ref_logp, targets, offsets, kw)
 
 
 def policy_loss(logp, old_logp, ref_logp, advantages, targets, offsets, **kw):
-    """(loss, result block) of ops.policy_loss, whose keywords it takes."""
+    """(loss, result block) of ops.policy_loss, whose keywords it takes.  The
+    loss's gradient flows to logp alone."""
     return PolicyLossFn.apply(logp, old_logp, ref_logp, advantages, targets, offsets, kw)

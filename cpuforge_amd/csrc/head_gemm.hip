@@ -46,7 +46,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kFrag = 1024;        // bytes of an operand of one MFMA
 constexpr int kBN = 128;           // tokens of a tile
 constexpr int kWgs = 512;          // two workgroups to a CU
-constexpr int kStages = 3;
+constexpr int kStages = 3;           // two workgroups' stages fill 147 of 160 KiB
 constexpr int kGroup = 8;          // token tiles
 constexpr float kTop = 32768.0f;   // of a dlogit over dlogp
 
@@ -278,6 +278,12 @@ __host__ __device__ __forceinline__ Splits splits_of(int tiles, int k16, int spl
 
 // A tile of 64 MB rows and kBN columns to a workgroup of four waves, each 32 MB x 64;
 // two workgroups to a CU: one's epilogue runs beside the other's products.
+// Bound by the power of the products: statistics of 2048 rows x 576 x 49152 297 us (three
+// times 116 GFLOP on f16, 1.17 PFLOP/s, where a library's f16 product of 8192^3 has 1.16),
+// MFMAs busy in 65% of the cycles at 1.8 GHz, no bank conflicts; 3686 rows with what the
+// gradients need kept 609, their gradient's product 639.  Not faster: 256 x 256 tiles of
+// eight waves, waves of 128 x 128 with a SIMD each (593 us where this took 403), a branch
+// for each 32 columns of a last tile (its registers spill).
 template <int MB, Product P>
 __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
     constexpr bool ROWS = P == Product::kRows;
@@ -687,7 +693,8 @@ __global__ __launch_bounds__(256, 2) void head_mid_kernel(const MidArgs g) {
 
 // lse and logp (or null) of scored rows [j0, ..) from their parts' maxima and sums,
 // and what the gradient scales a part by (or null).  16 rows to a workgroup, lane l
-// has row l % 16, so that a part's are read side by side.
+// has row l % 16, so that a part's are read side by side.  Bound by the latency of a
+// thread's parts: 7 us for 384 of them, 14 for 1002.
 __global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restrict__ stats, long ld, int parts,
                                                            int all_parts, const float* __restrict__ xt,
                                                            const int* __restrict__ idx, const int* __restrict__ count,
@@ -723,7 +730,8 @@ __global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restr
 }
 
 // dhn of scored rows [j0, ..): dlogp (head[target] - the splits' sums in order).
-// Four columns to a thread, eight splits' sums in flight.
+// Four columns to a thread, eight splits' sums in flight: bound by memory, 3686 x 576 with
+// 16 splits (136 MB) 27 us.
 __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __restrict__ part, int chunk, int rows,
                                                                int mt, int k16, int splits_max,
                                                                const int* __restrict__ idx,
@@ -773,7 +781,8 @@ struct DlogitsArgs {
 // A bound of every column's dlogits times their rows' 2^e: a column's power of two is
 // its own, since a token that is rarely likely has gradients far below the others',
 // which an optimizer that divides by their size scales up.  From the upper pieces
-// (f16, to 2^-11): 128 columns and every 8th 32 rows to a workgroup.
+// (f16, to 2^-11): 128 columns and every 8th 32 rows to a workgroup.  819 rows x 50001: 27 us
+// for 82 MB in pieces of 1 KiB of every other one.
 __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
     const int n = scored_rows(g.count, g.tag, g.j0, g.chunk);
@@ -808,7 +817,8 @@ __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) 
 }
 
 // The dlogits times their rows' 2^e as operands by columns: 32 rows and 128 columns
-// to a workgroup, turned round in LDS.
+// to a workgroup, turned round in LDS.  Bound by memory: 819 x 50001, read and written,
+// (328 MB) 57 us.
 __global__ __launch_bounds__(256) void head_pack_dlogits_kernel(const DlogitsArgs g) {
     __shared__ float tile[32][129];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
