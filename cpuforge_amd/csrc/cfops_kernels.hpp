@@ -211,12 +211,13 @@ constexpr size_t kLogpFew = 32;
 //   few or mid: 16 rows 576 x 49152 37 and 43, 2048 x 128256 267 and 249; 17 rows 46 and
 //   44, 319 and 252; where mid's workgroups of 128 rows of the head do not fill half of the
 //   card it has the latency of d for itself: 32 rows 2048 x 1000 55 and 90;
-//   mid or packed: 256 rows 576 x 49152 82 and 93, 2048 x 128256 512 and 744, 384 rows 115
-//   and 115, 726 and 906, 512 rows 129 and 123, 961 and 1066; with rows of the head that are
-//   read value by value 128 rows 129 x 49152 39 and 38, 256 rows 49 and 44.
+//   mid or packed: 256 rows 576 x 49152 77 and 96, 512 rows 133 and 128, 1024 rows 210 and
+//   209; 512 rows 2048 x 128256 860 and 1118, 2048 x 32000 250 and 299, 1024 rows 1669 and
+//   1818, 443 and 474, 1536 rows (2048 x 49152) 987 and 969; with rows of the head that are
+//   read value by value 256 rows 129 x 49152 44 and 45, 384 rows 59 and 52.
 inline bool logp_takes_few(size_t t, size_t vocab) { return t <= 16 || (t <= kLogpFew && vocab <= 16384); }
 inline bool logp_takes_mid(size_t t, size_t d, const float* head) {
-    return t <= (d % 4 == 0 && (uintptr_t)head % 16 == 0 ? 384 : 128);
+    return t <= (d % 4 || (uintptr_t)head % 16 ? 256 : d < 1024 ? 512 : 1024);
 }
 size_t logp_few_bytes(size_t t, size_t vocab);
 hipError_t launch_logp_few(const float* hn, const float* head, const int64_t* targets, size_t t, size_t d, size_t vocab,

@@ -551,20 +551,19 @@ struct MidArgs {
     long ld;
     int vocab, d, k16, tag, groups, tiles, vec;
 };
-constexpr int kMidK = 4;  // 16-k steps of a chunk
-
-// Statistics of a few hundred rows at most, the head split into pieces on its way from
-// memory: where it is used by few tiles of tokens, packing it first costs more than its
-// products (2048 x 128256 408 us).  128 rows of the head and 32 NB tokens to a workgroup, 32
+// Statistics of a thousand rows at most, the head split into pieces on its way from
+// memory: where it is used by few tiles of tokens, packing it first costs more than
+// splitting it for each (2048 x 128256 408 us).  128 rows of the head and 32 NB tokens to a workgroup, 32
 // rows to a wave, whose pieces stay in registers; the tokens' operands go through LDS for
 // all four waves.  The power of two of a wave's rows is that of the largest value so far:
 // where a chunk has one that f16 does not hold, the sums are scaled down (rarely: after the
 // first chunk one bit of room is left).  So it ends no higher than the packed head's.
 // Bound by reading the head up to 64 rows (2048 x 128256 in all 250 us, 1.05 GB at 4.8 TB/s
-// 220), by splitting it again for every 128 rows from there on.
-template <int NB>
+// 220), then by the matrix cores beside the splitting (1024 rows, 538 GFLOP in three
+// products, 1.6 ms, 1.0 PFLOP/s).
+template <int NB, int K>
 __global__ __launch_bounds__(256, 2) void head_mid_kernel(const MidArgs g) {
-    constexpr int CHUNK = NB * kMidK * 2 * kFrag;  // bytes of a chunk's operands of the tokens
+    constexpr int CHUNK = NB * K * 2 * kFrag;  // bytes of a chunk's operands of the tokens
     __shared__ __attribute__((aligned(1024))) char lds[2 * CHUNK];
     __shared__ float2 red[4][32 * NB];
     const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6), l32 = lane & 31, hh = lane >> 5;
@@ -573,34 +572,35 @@ __global__ __launch_bounds__(256, 2) void head_mid_kernel(const MidArgs g) {
     const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
     const int group = local / g.tiles * 8 + xcd, col0 = local % g.tiles * 32 * NB;
     if (group >= g.groups || col0 >= n) return;
+    const bool upper = col0 + 16 * NB < n;  // tokens in the second half of the tile
     const int m0 = group * 128 + wave * 32;
     const float* row = g.head + (long)min(m0 + l32, g.vocab - 1) * g.d;
     const uint32_t lds0 = lds_offset(lds), voff = lane * 16;
-    const int chunks = (g.k16 + kMidK - 1) / kMidK;
-    auto load_head = [&](float (&x)[kMidK][8], int c) {
-        const int k = c * 16 * kMidK + 8 * hh;
-        if (g.vec && (c + 1) * 16 * kMidK <= g.d) {
+    const int chunks = (g.k16 + K - 1) / K;
+    auto load_head = [&](float (&x)[K][8], int c) {
+        const int k = c * 16 * K + 8 * hh;
+        if (g.vec && (c + 1) * 16 * K <= g.d) {
 #pragma unroll
-            for (int s = 0; s < kMidK; s++) load8(x[s], row, k + 16 * s, INT_MAX, true);
+            for (int s = 0; s < K; s++) load8(x[s], row, k + 16 * s, INT_MAX, true);
         } else {
 #pragma unroll
-            for (int s = 0; s < kMidK; s++) load8(x[s], row, k + 16 * s, g.d, g.vec);
+            for (int s = 0; s < K; s++) load8(x[s], row, k + 16 * s, g.d, g.vec);
         }
     };
     auto load_rows = [&](int c) {
-        const int steps = min(kMidK, g.k16 - c * kMidK);
+        const int steps = min(K, g.k16 - c * K);
 #pragma unroll
-        for (int i = 0; i < 2 * NB; i++) {
-            const int at = 2 * NB * wave + i, j = at / (2 * kMidK), s = at % (2 * kMidK);  // block, KiB of it
-            if (s / 2 < steps)
-                lds_load16_so(g.rows + (((long)(col0 / 32 + j) * g.k16 + c * kMidK) * 2 + s) * kFrag, voff,
+        for (int i = 0; i < NB * K / 2; i++) {
+            const int at = NB * K / 2 * wave + i, j = at / (2 * K), s = at % (2 * K);  // block, KiB of it
+            if (s / 2 < steps && (upper || j < NB / 2))
+                lds_load16_so(g.rows + (((long)(col0 / 32 + j) * g.k16 + c * K) * 2 + s) * kFrag, voff,
                               lds0 + (c & 1) * CHUNK + at * kFrag);
         }
     };
     f32x16 acc[NB];
 #pragma unroll
     for (int j = 0; j < NB; j++) acc[j] = zero16();
-    float x[kMidK][8], next[kMidK][8];
+    float x[K][8], next[K][8];
     int e = -112;
     load_rows(0);
     load_head(x, 0);
@@ -615,13 +615,13 @@ __global__ __launch_bounds__(256, 2) void head_mid_kernel(const MidArgs g) {
         }
         float top = 0.0f;
 #pragma unroll
-        for (int s = 0; s < kMidK; s++)
+        for (int s = 0; s < K; s++)
 #pragma unroll
             for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[s][i]));
         if (__any(top * exp2i(-e) > 65504.0f)) {
             top = 0.0f;
 #pragma unroll
-            for (int s = 0; s < kMidK; s++)
+            for (int s = 0; s < K; s++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = fmaxf(top, finite_abs(x[s][i]));
 #pragma unroll
@@ -637,26 +637,31 @@ __global__ __launch_bounds__(256, 2) void head_mid_kernel(const MidArgs g) {
         const float sc = exp2i(-e);
         const char* b = lds + (c & 1) * CHUNK + voff;
 #pragma unroll
-        for (int s = 0; s < kMidK; s++) {
-            if (c * kMidK + s >= g.k16) break;
+        for (int s = 0; s < K; s++) {
+            if (c * K + s >= g.k16) break;
             const Pieces a = split8(x[s], sc);
 #pragma unroll
-            for (int j = 0; j < NB; j++) {
-                const f16x8 h = *reinterpret_cast<const f16x8*>(b + ((j * kMidK + s) * 2) * kFrag);
-                const f16x8 l = *reinterpret_cast<const f16x8*>(b + ((j * kMidK + s) * 2 + 1) * kFrag);
-                acc[j] = mfma_f16(a.l, h, acc[j]);
-                acc[j] = mfma_f16(a.h, l, acc[j]);
-                acc[j] = mfma_f16(a.h, h, acc[j]);
+            for (int half = 0; half < 2; half++) {
+                if (half && !upper) break;
+#pragma unroll
+                for (int j = half * NB / 2; j < (half + 1) * NB / 2; j++) {
+                    const f16x8 h = *reinterpret_cast<const f16x8*>(b + ((j * K + s) * 2) * kFrag);
+                    const f16x8 l = *reinterpret_cast<const f16x8*>(b + ((j * K + s) * 2 + 1) * kFrag);
+                    acc[j] = mfma_f16(a.l, h, acc[j]);
+                    acc[j] = mfma_f16(a.h, l, acc[j]);
+                    acc[j] = mfma_f16(a.h, h, acc[j]);
+                }
             }
         }
 #pragma unroll
-        for (int s = 0; s < kMidK; s++)
+        for (int s = 0; s < K; s++)
 #pragma unroll
             for (int i = 0; i < 8; i++) x[s][i] = next[s][i];
     }
     const int live = g.vocab - m0;  // rows of the head of this wave
 #pragma unroll
     for (int j = 0; j < NB; j++) {
+        if (j >= NB / 2 && !upper) break;
         const int col = col0 + 32 * j + l32;
         const int et = (int)(__builtin_bit_cast(uint32_t, g.scale[col]) >> 23) - 127;
         const int target = (col < n ? g.targets[col] : -1) - m0;
@@ -970,10 +975,15 @@ hipError_t launch_head_mid(const HeadPlan& p, const HeadBuffers& b, const float*
     g.head = head, g.rows = b.rows, g.count = b.count, g.targets = b.idx + t, g.scale = b.scale;
     g.stats = static_cast<float2*>(b.stats), g.xt = b.xt, g.ld = (long)p.chunk, g.vocab = (int)vocab, g.d = (int)d;
     g.k16 = p.k16, g.tag = p.tag, g.groups = (int)((vocab + 127) / 128), g.vec = d % 4 == 0 && aligned16(head);
-    const bool two = t <= 64;
-    g.tiles = (int)((t + (two ? 63 : 127)) / (two ? 64 : 128));
-    hipLaunchKernelGGL(two ? head_mid_kernel<2> : head_mid_kernel<4>, dim3((unsigned)((g.groups + 7) / 8 * 8 * g.tiles)),
-                       dim3(256), 0, st, g);
+    // Tiles of 256 tokens, which split the head half as often, take 1.75 times as long as
+    // ones of 128: the ones with less time in rounds of two workgroups to a CU.  (Us by 128
+    // and by 256: 200 rows 2048 x 32000 139 and 184, 2048 x 49152 238 and 218, 400 rows 252
+    // and 234, 371 and 392.)
+    auto rounds = [&](size_t tile) { return (g.groups * ((t + tile - 1) / tile) + kWgs - 1) / kWgs; };
+    const int nb = t <= 64 ? 2 : 4 * rounds(128) <= 7 * rounds(256) ? 4 : 8;
+    g.tiles = (int)((t + 32 * nb - 1) / (32 * nb));
+    hipLaunchKernelGGL((nb == 2 ? head_mid_kernel<2, 4> : nb == 4 ? head_mid_kernel<4, 4> : head_mid_kernel<8, 2>),
+                       dim3((unsigned)((g.groups + 7) / 8 * 8 * g.tiles)), dim3(256), 0, st, g);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)(p.chunk / 16)), dim3(1024), 0, st, g.stats, g.ld, g.groups,

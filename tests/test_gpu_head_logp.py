@@ -127,10 +127,13 @@ def check_forward(hn, head, tg):
         assert bool(((logp - w_logp).abs() <= tol + off + U * (w_logp.abs() + 2 * w_lse.abs())).all())
 
 
-# The forms of the forward by rows (to 16, to 384, more) and alignment, at their borders.
+# The forms of the forward by rows (to 16, to 256, 512 or 1024, more), alignment and the
+# rounds of workgroups that its tiles of tokens make, at their borders.
 FORWARD = [(16, 64, 16385), (17, 64, 16385), (32, 500, 20000), (33, 8, 127), (64, 129, 1000), (65, 577, 3001),
            (128, 129, 129), (129, 129, 257), (384, 576, 4097), (385, 576, 4097), (200, 2050, 1025), (100, 64, 1),
-           (97, 1, 300), (383, 68, 20000)]
+           (97, 1, 300), (383, 68, 20000), (200, 64, 33000), (129, 36, 40000), (257, 40, 66000), (385, 577, 33000),
+           (512, 128, 33000), (513, 128, 33000), (1024, 1028, 20000), (1025, 1028, 20000), (256, 257, 33000),
+           (257, 257, 33000)]
 
 
 @pytest.mark.parametrize("t,d,vocab", FORWARD)
