@@ -280,7 +280,7 @@ __host__ __device__ __forceinline__ Splits splits_of(int tiles, int k16, int spl
 // two workgroups to a CU: one's epilogue runs beside the other's products.
 // Bound by the power of the products: statistics of 2048 rows x 576 x 49152 297 us (three
 // times 116 GFLOP on f16, 1.17 PFLOP/s, where a library's f16 product of 8192^3 has 1.16),
-// MFMAs busy in 65% of the cycles at 1.8 GHz, no bank conflicts; 3686 rows with what the
+// MFMAs busy in 62% of the cycles at 1.76 GHz, no bank conflicts; 3686 rows with what the
 // gradients need kept 609, their gradient's product 639.  Not faster: 256 x 256 tiles of
 // eight waves, waves of 128 x 128 with a SIMD each (593 us where this took 403), a branch
 // for each 32 columns of a last tile (its registers spill).
@@ -560,7 +560,8 @@ struct MidArgs {
 // first chunk one bit of room is left).  So it ends no higher than the packed head's.
 // Bound by reading the head up to 64 rows (2048 x 128256 in all 250 us, 1.05 GB at 4.8 TB/s
 // 220), then by the matrix cores beside the splitting (1024 rows, 538 GFLOP in three
-// products, 1.6 ms, 1.0 PFLOP/s).
+// products, 1.6 ms, 1.0 PFLOP/s; MFMAs busy in half of the cycles).  The head's values two
+// chunks ahead are not faster: 3% at 1024 rows, but 5% slower at 128 of 576 columns.
 template <int NB, int K>
 __global__ __launch_bounds__(256, 2) void head_mid_kernel(const MidArgs g) {
     constexpr int CHUNK = NB * K * 2 * kFrag;  // bytes of a chunk's operands of the tokens
@@ -643,14 +644,19 @@ __global__ __launch_bounds__(256, 2) void head_mid_kernel(const MidArgs g) {
 #pragma unroll
             for (int half = 0; half < 2; half++) {
                 if (half && !upper) break;
+                f16x8 h[NB / 2], l[NB / 2];
+                const int j0 = half * NB / 2;
 #pragma unroll
-                for (int j = half * NB / 2; j < (half + 1) * NB / 2; j++) {
-                    const f16x8 h = *reinterpret_cast<const f16x8*>(b + ((j * K + s) * 2) * kFrag);
-                    const f16x8 l = *reinterpret_cast<const f16x8*>(b + ((j * K + s) * 2 + 1) * kFrag);
-                    acc[j] = mfma_f16(a.l, h, acc[j]);
-                    acc[j] = mfma_f16(a.h, l, acc[j]);
-                    acc[j] = mfma_f16(a.h, h, acc[j]);
+                for (int j = 0; j < NB / 2; j++) {
+                    h[j] = *reinterpret_cast<const f16x8*>(b + (((j0 + j) * K + s) * 2) * kFrag);
+                    l[j] = *reinterpret_cast<const f16x8*>(b + (((j0 + j) * K + s) * 2 + 1) * kFrag);
                 }
+#pragma unroll
+                for (int j = 0; j < NB / 2; j++) acc[j0 + j] = mfma_f16(a.l, h[j], acc[j0 + j]);
+#pragma unroll
+                for (int j = 0; j < NB / 2; j++) acc[j0 + j] = mfma_f16(a.h, l[j], acc[j0 + j]);
+#pragma unroll
+                for (int j = 0; j < NB / 2; j++) acc[j0 + j] = mfma_f16(a.h, h[j], acc[j0 + j]);
             }
         }
 #pragma unroll
