@@ -168,6 +168,27 @@ def test_forward_where_later_columns_are_larger(t):
     check_forward(hn, head, tg)
 
 
+@pytest.mark.parametrize("t,d", [(30, 96), (90, 96), (700, 96), (700, 1024), (1200, 96)])
+def test_what_is_not_scored_or_not_finite_stays_alone_in_every_form(t, d):
+    hn, head, tg, _ = inputs(t, d, 20000, 40 + t)
+    logp, lse, _ = forward(hn, head, tg)
+    off = tg == IGN
+    hn2, tg2 = hn.clone(), tg.clone()
+    hn2[off] = float("nan")
+    first, second, third = (~off).nonzero()[:3, 0].tolist()
+    hn2[first, 7], hn2[second, 3], tg2[third] = float("nan"), float("-inf"), 20000
+    logp2, lse2, res = forward(hn2, head, tg2, check=False)
+    assert int(res[0]) == int((~off).sum()) and int(res[1]) == third
+    odd = torch.tensor([first, second, third], device=DEV)
+    assert not bool(torch.isfinite(logp2[odd]).any())
+    rest = torch.ones(t, dtype=torch.bool, device=DEV)
+    rest[odd] = False
+    assert torch.equal(logp2[rest], logp[rest]) and torch.equal(lse2[rest], lse[rest])
+    # A row of the head that is not finite is in every row's sum.
+    head[19990, d - 1] = float("nan")
+    assert bool(torch.isnan(forward(hn, head, tg)[1][~off]).all())
+
+
 @pytest.mark.parametrize("masked", [0.0, 0.97, 1.0])
 @pytest.mark.parametrize("t", [9, 400])
 def test_masks(t, masked):
