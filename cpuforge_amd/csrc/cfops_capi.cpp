@@ -697,7 +697,7 @@ int adamw8_multi(cfattn_ctx* c, size_t count, const cfops_adamw_tensor* tensors,
 }  // namespace
 
 size_t cfops_lm_head_logprobs_keep_bytes(size_t t, size_t d, size_t vocab) {
-    if (t <= cfattn::kLogpFew || t >= (size_t)1 << 24 || d == 0 || vocab == 0 || !fits_int(d) ||
+    if (t <= cfattn::kLogpUnkept || t >= (size_t)1 << 24 || d == 0 || vocab == 0 || !fits_int(d) ||
         vocab >= (size_t)1 << 26)
         return 0;
     return keep_layout(cfattn::head_plan(t, d, vocab, SIZE_MAX), t).bytes;
@@ -722,7 +722,7 @@ int cfops_lm_head_logprobs(cfattn_ctx* c, const float* hn, const float* head, co
                "log-probability launch");
         return CFATTN_OK;
     }
-    if (t <= cfattn::kLogpFew) keep = nullptr;
+    if (t <= cfattn::kLogpUnkept) keep = nullptr;
     CF_TRY(logprobs_many(c, hn, head, targets, t, d, vocab, logp, lse, result, keep, keep_bytes, st));
     CF_HIP(c, cfattn::launch_logp_finish(targets, logp, t, result, st), "log-probability launch");
     return CFATTN_OK;
@@ -738,7 +738,7 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
     if (t == 0 || (!dhn && !dhead)) return CFATTN_OK;
     if (!hn || !head || !targets || !lse || !dlogp) return fail(c, CFATTN_ERR_ARG, "null buffer");
     const hipStream_t st = to_stream(stream);
-    if (t > cfattn::kLogpFew)
+    if (t > cfattn::kLogpUnkept)
         return logprobs_backward_many(c, hn, head, targets, dlogp, t, d, vocab, dhn, dhead, acc != 0, keep, keep_bytes,
                                       st);
     LogpRows rows{};

@@ -203,10 +203,15 @@ hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const in
                                  hipStream_t st);
 hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t rows, void* misc, hipStream_t st);
 // All of the forward for at most kLogpFew rows in two launches, in scratch of
-// logp_few_bytes(t, vocab).  Up to as many rows nothing is kept for the gradients, whose
-// f32 products take, against those over packed operands with what the forward keeps for
-// them, at 32 rows 182 and 186 us (576 x 49152), 1084 and 1176 (2048 x 128256).
+// logp_few_bytes(t, vocab).
 constexpr size_t kLogpFew = 32;
+// Up to as many rows a forward keeps nothing, and the gradients are f32 products over
+// logits formed again.  Forward and dhn so, and over packed operands with what the forward
+// keeps for them, us: 64 rows 576 x 49152 170 and 170, 2048 x 49152 377 and 467, 2048 x
+// 128256 917 and 1107, 500 x 50001 176 and 162; 96 rows 220 and 176, 500 and 471, 1173 and
+// 1122, 216 and 164.  With the head's gradient 64 rows 227 and 260, 584 and 688, 1489 and
+// 1654, 230 and 260.
+constexpr size_t kLogpUnkept = 64;
 // Which form takes the forward, us of a call by either (rows, d x vocab):
 //   few or mid: 16 rows 576 x 49152 37 and 43, 2048 x 128256 267 and 249; 17 rows 46 and
 //   44, 319 and 252; where mid's workgroups of 128 rows of the head do not fill half of the
