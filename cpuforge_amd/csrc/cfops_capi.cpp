@@ -741,14 +741,18 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
     if (t > cfattn::kLogpUnkept)
         return logprobs_backward_many(c, hn, head, targets, dlogp, t, d, vocab, dhn, dhead, acc != 0, keep, keep_bytes,
                                       st);
+    // With zeros in the rows behind the last one the head's gradient sums over whole steps of
+    // 32 (us with 2048 x 128256, as they are and so: 24 rows 1586 and 1352, 49 rows 1805 and
+    // 1516; 8 rows 1538 and 1504, but 1 row 1253 and 1463).
+    const size_t padded = dhead && t > 16 ? (t + 31) / 32 * 32 : t;
     LogpRows rows{};
-    CF_TRY(logp_rows(c, t, d, vocab, rows));
+    CF_TRY(logp_rows(c, padded, d, vocab, rows));
     CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, 0, nullptr, nullptr, nullptr,
                                               st),
            "log-probability launch");
-    CF_HIP(c, cfattn::launch_logp_gather(hn, rows.idx, rows.count, rows.hn, t, d, st), "log-probability launch");
-    for (size_t j0 = 0; j0 < t; j0 += rows.chunk) {
-        const size_t nr = std::min(t - j0, rows.chunk);
+    CF_HIP(c, cfattn::launch_logp_gather(hn, rows.idx, rows.count, rows.hn, padded, d, st), "log-probability launch");
+    for (size_t j0 = 0; j0 < padded; j0 += rows.chunk) {
+        const size_t nr = std::min(padded - j0, rows.chunk);
         float* h = rows.hn + j0 * d;
         CF_TRY(gemm(c, CFOPS_NT, h, head, rows.logits, nr, d, vocab, false, st));
         CF_HIP(c, cfattn::launch_logp_grad_rows(rows.logits, targets, rows.idx, rows.count, lse, dlogp, j0, nr, vocab,
