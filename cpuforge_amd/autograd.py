@@ -193,14 +193,14 @@ class LMHeadLogprobsFn(torch.autograd.Function):
     that ops.ce_check reads (ops.lm_head_logprobs)."""
 
     @staticmethod
-    def forward(ctx, hn, head, targets):
+    def forward(ctx, hn, head, targets, keeps: bool):
         d = hn.shape[-1]
         h2, head2, tg = _flat(hn, d), head.contiguous(), targets.contiguous().view(-1)
         t, vocab = h2.shape[0], head2.shape[0]
         logp, lse = _empty(tg, tg)
         result = P.ce_result_buffer(hn.device)
         keep = None
-        if any(ctx.needs_input_grad):
+        if keeps:
             n = P.lm_head_logprobs_keep_bytes(t, d, vocab)
             if 0 < n <= LOGPROBS_KEEP_LIMIT:
                 keep = torch.empty(n, dtype=torch.uint8, device=hn.device)
@@ -216,12 +216,12 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         h2, head, tg, lse, keep = ctx.saved_tensors
         need_hn, need_head = ctx.needs_input_grad[:2]
         if g is None or not (need_hn or need_head):
-            return None, None, None
+            return None, None, None, None
         dhn = torch.empty_like(h2) if need_hn else None
         dhead = torch.empty_like(head) if need_head else None
         P.lm_head_logprobs_backward(h2, head, tg, lse, g.contiguous().view(-1), h2.shape[0], h2.shape[1],
                                     head.shape[0], dhn, dhead, keep, acc=False)
-        return None if dhn is None else dhn.view(ctx.shape), dhead, None
+        return None if dhn is None else dhn.view(ctx.shape), dhead, None, None
 
 
 class PreferenceLossFn(torch.autograd.Function):
@@ -295,8 +295,13 @@ def lm_head_ce_dev(hn, head, targets):
 
 def lm_head_logprobs(hn, head, targets):
     """(log-probabilities of the targets, shaped as they are; 0 where the target
-    is ops.IGNORE_INDEX, and the block whose target check ops.ce_check runs)."""
-    return LMHeadLogprobsFn.apply(hn, head, targets)
+    is ops.IGNORE_INDEX, and the block whose target check ops.ce_check runs).
+    Where a backward may follow, its forward keeps what that reads, up to
+    LOGPROBS_KEEP_LIMIT."""
+    # (A function's forward runs without a gradient mode, and its needs_input_grad
+    # names what requires a gradient in any mode: whether one can follow shows here.)
+    keeps = torch.is_grad_enabled() and (hn.requires_grad or head.requires_grad)
+    return LMHeadLogprobsFn.apply(hn, head, targets, keeps)
 
 
 def preference_loss(logp, ref_logp, targets, offsets, **kw):
