@@ -17,12 +17,17 @@
 //
 // The hidden states' gradient, dlogp (head[target] - sum_v P_v head[v]), takes P
 // from the forward: beside its statistics that keeps, for each token and 128
-// rows of the head, exp(x - m) with m their largest logit, as pieces in the order
+// rows of the head, exp(x - m) with m their largest logit, in f32 and in the order
 // of the gradient's product (4 bytes a logit).  The product adds 128 rows at a time
-// and scales their sum by exp(m - lse), a factor of the result's own column:
-// nothing is rounded again, and no exponential or product is formed twice.  (The
-// logits formed again in the backward instead, 3686 x 576 x 49152: 0.81 ms, where
-// keeping them takes 0.2.)
+// and scales their sum by exp(m - lse), a factor of the result's own column: no
+// exponential or product is formed twice.  (The logits formed again in the backward
+// instead, 3686 x 576 x 49152: 0.81 ms, where keeping them takes 0.2.)  The waves of
+// that product split the exponentials, which reach them as they are kept; kept as
+// pieces already they would serve no other sum: pieces hold what lies 2^-40 below the
+// largest of 128, enough beside it in the hidden states' gradient, but the head's
+// gradient of a rare token is a sum of its own over tokens, in which nothing larger
+// hides what they lack (a token e^-20 below the others had 4e-3 of its row's gradient
+// wrong, at e^-25 nothing right).
 //
 // Packed operands: both are first written as MFMA operands (1 KiB: a lane's eight
 // f16, 64 lanes) of 32 rows and 16 k, the two pieces side by side, so a
@@ -48,7 +53,7 @@ constexpr int kBN = 128;           // tokens of a tile
 constexpr int kWgs = 512;          // two workgroups to a CU
 constexpr int kStages = 3;           // two workgroups' stages fill 147 of 160 KiB
 constexpr int kGroup = 8;          // token tiles
-constexpr float kTop = 32768.0f;   // of a dlogit over dlogp
+constexpr float kTop = 32768.0f;   // of a kept exponential in a product
 
 __device__ __forceinline__ float exp2i(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 // 2^e within f32's normal range.
@@ -65,6 +70,9 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a < INFINITY ? a : 0.0f;
 }
 
+// Memory that the whole launch only reads.
+typedef const __attribute__((address_space(4))) int* ScalarInts;
+
 __device__ __forceinline__ f32x16 mfma_f16(const f16x8& a, const f16x8& b, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
@@ -72,6 +80,7 @@ __device__ __forceinline__ f32x16 mfma_f16(const f16x8& a, const f16x8& b, const
 struct Pieces {
     f16x8 h, l;
 };
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ Pieces split8(const float (&x)[8], float scale) {
 #pragma clang fp contract(off)
     Pieces p;
@@ -80,6 +89,17 @@ __device__ __forceinline__ Pieces split8(const float (&x)[8], float scale) {
         const float y = x[i] * scale;
         p.h[i] = (_Float16)y;
         p.l[i] = (_Float16)(y - (float)p.h[i]);
+    }
+    return p;
+}
+// The same by one fused operation a piece.
+__device__ __forceinline__ Pieces split8(const f32x4& a, const f32x4& b, float scale) {
+    Pieces p;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float x = i < 4 ? a[i] : b[i - 4];
+        p.h[i] = (_Float16)fmaf(x, scale, 0.0f);
+        p.l[i] = (_Float16)fmaf(x, scale, -(float)p.h[i]);
     }
     return p;
 }
@@ -247,9 +267,9 @@ struct HeadArgs {
     int vocab, v16;
     float2* stats;      // [128 rows of the head][ld]: max and sum of exp2, in log2 units
     float* xt;          // the targets' logits
-    char* keep;         // [32 tokens][v16][piece], or null
+    char* keep;         // [32 tokens][v16][half of a lane's eight values], or null
     // the rows' gradient: a is the head by columns, b what statistics kept
-    const float* factor;  // [128 rows of the head][ld]
+    const float* factor;  // [128 rows of the head][ld]; exponents and largest as above
     float* part;          // [split][chunk][64 MB mt]
     int splits_max;
     // the head's gradient: a is the dlogits by columns, b the rows by columns
@@ -358,6 +378,11 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
         // (they would count among the loads waited for below).
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
+        // (Through the scalar cache: a vector load's wait would be one for the stages' too.)
+        const ScalarInts exponents = ROWS ? (ScalarInts)(uintptr_t)g.exponents : nullptr;
+        const int big = ROWS ? *(ScalarInts)(uintptr_t)g.largest : 0;
+        int exponent = ROWS && k0 < k1 ? exponents[k0 / 2] : 0;
+        float kept = 1.0f;
         uint32_t cur = 0, nxt = 2 * STAGE;
         if (k0 < k1) load(0);  // (more splits than runs: some have none)
         if (k0 + 1 < k1) load(STAGE);
@@ -370,18 +395,33 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
             asm volatile("" ::: "memory");
             if (k + 2 < k1) load(nxt);
             nxt = nxt == (kStages - 1) * STAGE ? 0 : nxt + STAGE;
+            if constexpr (ROWS) {
+                // The exponentials meet 32 rows of the head, with their power of two.
+                if (k % 2 == 0) {
+                    kept = kTop * pow2_clamped(exponent - big);
+                    exponent = exponents[min(k + 2, k1 - 1) / 2];
+                }
+            }
             const char* s = lds + cur;
             cur = cur == (kStages - 1) * STAGE ? 0 : cur + STAGE;
             f16x8 a[MB][2], b[2][2];
 #pragma unroll
-            for (int p = 0; p < 2; p++) {
+            for (int j = 0; j < 2; j++) {
+                const char* at = s + (2 * MB + wn * 2 + j) * 2 * kFrag + voff;
+                if constexpr (ROWS) {
+                    const Pieces x = split8(*reinterpret_cast<const f32x4*>(at),
+                                            *reinterpret_cast<const f32x4*>(at + kFrag), kept);
+                    b[j][0] = x.h, b[j][1] = x.l;
+                } else {
+                    b[j][0] = *reinterpret_cast<const f16x8*>(at);
+                    b[j][1] = *reinterpret_cast<const f16x8*>(at + kFrag);
+                }
+            }
 #pragma unroll
-                for (int j = 0; j < 2; j++)
-                    b[j][p] = *reinterpret_cast<const f16x8*>(s + ((2 * MB + wn * 2 + j) * 2 + p) * kFrag + voff);
+            for (int p = 0; p < 2; p++)
 #pragma unroll
                 for (int i = 0; i < MB; i++)
                     a[i][p] = *reinterpret_cast<const f16x8*>(s + ((wm * MB + i) * 2 + p) * kFrag + voff);
-            }
             // (The order that shares an operand from one to the next: 1% less time.)
             constexpr int pa[3] = {1, 0, 0}, pb[3] = {0, 0, 1};
             if (live_cols)
@@ -419,7 +459,8 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
 #pragma unroll
                 for (int q = 0; q < 16; q++) {
                     const int v = min(v0 + 8 * (q >> 2) + (q & 3), g.vocab - 1);
-                    u[q] = other ? __builtin_nanf("") : exp2i(group_exponent(__builtin_bit_cast(float, g.col_top[v])));
+                    u[q] = other ? __builtin_nanf("")
+                                 : exp2i(group_exponent(__builtin_bit_cast(float, g.col_top[v]))) * (1.0f / 16384.0f);
                 }
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
@@ -460,7 +501,6 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
             int e[MB];
 #pragma unroll
             for (int i = 0; i < MB; i++) e[i] = wave_uniform(g.exponents[m0 / 32 + i]);
-            const int big = g.keep ? wave_uniform(*g.largest) : 0;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int col = col0 + 32 * j + l32;
@@ -516,15 +556,11 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
                         __builtin_amdgcn_sched_barrier(0);  // (all at once take more registers than there are)
                     }
                     if (!g.keep) continue;
-                    const float f = scored ? kTop * pow2_clamped(e[i] - big) : 0.0f;
+                    char* to = g.keep + ((long)(col0 / 32 + j) * g.v16 + m0 / 16 + 2 * i) * 2 * kFrag + lane * 16;
 #pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        float x[8];
-#pragma unroll
-                        for (int z = 0; z < 8; z++) x[z] = y[8 * q + z];
-                        store_pieces(g.keep + ((long)(col0 / 32 + j) * g.v16 + m0 / 16 + 2 * i + q) * 2 * kFrag, lane,
-                                     split8(x, f));
-                        __builtin_amdgcn_sched_barrier(0);
+                    for (int q = 0; q < 16; q += 4) {
+                        const f32x4 x = {y[q], y[q + 1], y[q + 2], y[q + 3]};
+                        *reinterpret_cast<f32x4*>(to + q / 4 * kFrag) = scored ? x : f32x4{};
                     }
                 }
                 sum = sum_halves(sum);
@@ -781,7 +817,7 @@ __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __re
 struct DlogitsArgs {
     const char* keep;     // from row j0 on
     const float* factor;
-    const int *exponents, *largest, *idx, *targets, *count;
+    const int *idx, *targets, *count;
     const float *dlogp, *scale;
     unsigned* col_top;
     char* out;            // [32 columns][t16][piece]
@@ -789,27 +825,31 @@ struct DlogitsArgs {
     int v16, t16, tag, j0, chunk, vocab;
 };
 
-// A bound of every column's dlogits times their rows' 2^e: a column's power of two is
-// its own, since a token that is rarely likely has gradients far below the others',
-// which an optimizer that divides by their size scales up.  From the upper pieces
-// (f16, to 2^-11): 128 columns and every 8th 32 rows to a workgroup.  819 rows x 50001: 27 us
-// for 82 MB in pieces of 1 KiB of every other one.
+// 2^14 and the power of two of a row of hn: a power of two near its largest value, so
+// that a dlogit times it is as large as what the row adds to the head's gradient.
+__device__ __forceinline__ float row_top(float scale) { return scale * 16384.0f; }
+
+// The largest of every column's dlogits times their rows' row_top: a column's power of
+// two is its own, since a token that is rarely likely has gradients far below the
+// others', which an optimizer that divides by their size scales up.  128 columns and
+// every 8th 32 rows to a workgroup.  (The probability beside 1 at a target counts as 1.)
 __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
     const int n = scored_rows(g.count, g.tag, g.j0, g.chunk);
     float top[2][8] = {};
-    const float u = pow2_clamped(*g.largest - g.exponents[blockIdx.x * 4 + wave] - 15);
     for (int t0 = 32 * blockIdx.y; t0 < n; t0 += 32 * gridDim.y) {
         const int j = t0 + l32;
         if (j >= n) continue;
-        const float row = fabsf(g.dlogp[g.idx[g.j0 + j]]) * g.scale[g.j0 + j];
-        const float f = g.factor[blockIdx.x * g.ld + j] * u * row;
+        const float row = fabsf(g.dlogp[g.idx[g.j0 + j]] * row_top(g.scale[g.j0 + j]));
+        const float f = g.factor[blockIdx.x * g.ld + j];
 #pragma unroll
         for (int q = 0; q < 2; q++) {
-            const f16x8 h = *reinterpret_cast<const f16x8*>(
+            const f32x4* y = reinterpret_cast<const f32x4*>(
                 g.keep + ((long)(t0 / 32) * g.v16 + blockIdx.x * 8 + 2 * wave + q) * 2 * kFrag + lane * 16);
+            const f32x4 a = y[0], b = y[kFrag / 16];
 #pragma unroll
-            for (int i = 0; i < 8; i++) top[q][i] = fmaxf(top[q][i], finite_abs((float)h[i] * f));
+            for (int i = 0; i < 8; i++)
+                top[q][i] = fmaxf(top[q][i], finite_abs((i < 4 ? a[i] : b[i - 4]) * f * row));
         }
         // (One workgroup of the columns sees to a row's target.)
         if (blockIdx.x == 0 && wave == 0 && hh == 0)
@@ -827,7 +867,7 @@ __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) 
         }
 }
 
-// The dlogits times their rows' 2^e as operands by columns: 32 rows and 128 columns
+// The dlogits times their rows' row_top as operands by columns: 32 rows and 128 columns
 // to a workgroup, turned round in LDS.  Bound by memory: 819 x 50001, read and written,
 // (328 MB) 57 us.
 __global__ __launch_bounds__(256) void head_pack_dlogits_kernel(const DlogitsArgs g) {
@@ -837,19 +877,20 @@ __global__ __launch_bounds__(256) void head_pack_dlogits_kernel(const DlogitsArg
     if (t0 >= n) return;
     const bool scored = j < n;
     const long r = scored ? g.idx[g.j0 + j] : 0;
-    const float row = scored ? g.dlogp[r] * g.scale[g.j0 + j] : 0.0f;
-    const float f = scored ? g.factor[blockIdx.x * g.ld + j] * pow2_clamped(*g.largest - g.exponents[blockIdx.x * 4 + wave] - 15) : 0.0f;
+    const float row = scored ? g.dlogp[r] * row_top(g.scale[g.j0 + j]) : 0.0f;
+    const float f = scored ? g.factor[blockIdx.x * g.ld + j] : 0.0f;
     const int target = scored ? g.targets[g.j0 + j] - (int)blockIdx.x * 128 : -1;
 #pragma unroll
     for (int q = 0; q < 2; q++) {
         const int s = 2 * wave + q;  // 16 columns
-        const char* p = g.keep + ((long)blockIdx.y * g.v16 + blockIdx.x * 8 + s) * 2 * kFrag + lane * 16;
-        const f16x8 h = *reinterpret_cast<const f16x8*>(p), l = *reinterpret_cast<const f16x8*>(p + kFrag);
+        const f32x4* y = reinterpret_cast<const f32x4*>(
+            g.keep + ((long)blockIdx.y * g.v16 + blockIdx.x * 8 + s) * 2 * kFrag + lane * 16);
+        const f32x4 a = y[0], b = y[kFrag / 16];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int c = 16 * s + 8 * (i >> 2) + 4 * hh + (i & 3);
             // (Rows from n on are zeros, whatever their factor.)
-            tile[l32][c] = scored ? row * ((c == target ? 1.0f : 0.0f) - ((float)h[i] + (float)l[i]) * f) : 0.0f;
+            tile[l32][c] = scored ? row * ((c == target ? 1.0f : 0.0f) - (i < 4 ? a[i] : b[i - 4]) * f) : 0.0f;
         }
     }
     __syncthreads();
@@ -964,7 +1005,7 @@ hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, size_t t, 
     HeadArgs g{};
     g.a = b.packed, g.b = b.rows + j0 / 32 * p.k16 * 2 * kFrag, g.ka = g.kb = p.k16, g.mt = (int)(p.v_pad / 256);
     g.count = b.count, g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.exponents = b.exponents;
-    g.largest = b.count + 1, g.targets = b.idx + t, g.scale = b.scale, g.tag = p.tag, g.vocab = (int)vocab;
+    g.targets = b.idx + t, g.scale = b.scale, g.tag = p.tag, g.vocab = (int)vocab;
     g.v16 = (int)(p.v_pad / 16), g.stats = static_cast<float2*>(b.stats), g.xt = b.xt, g.keep = b.keep;
     hipLaunchKernelGGL((head_gemm_kernel<4, Product::kStats>), dim3(kWgs), dim3(256), 0, st, g);
     hipError_t e = hipGetLastError();
@@ -1003,7 +1044,7 @@ hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, co
     HeadArgs g{};
     g.a = b.back, g.b = b.keep, g.ka = g.kb = (int)(p.v_pad / 16), g.mt = (int)(p.d_pad / (64 * mb)), g.count = b.count;
     g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.factor = b.factor, g.part = b.part;
-    g.splits_max = p.splits_max, g.tag = p.tag;
+    g.splits_max = p.splits_max, g.tag = p.tag, g.exponents = b.exponents, g.largest = b.count + 1;
     if (mb == 3)
         hipLaunchKernelGGL((head_gemm_kernel<3, Product::kRows>), dim3(kWgs), dim3(256), 0, st, g);
     else
@@ -1021,8 +1062,8 @@ hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, size_t t, 
                              size_t j0, size_t local, size_t rows, size_t d, size_t vocab, char* packed_dlogits,
                              unsigned* col_top, float* dhead, int acc, hipStream_t st) {
     DlogitsArgs g{};
-    g.keep = b.keep + local * p.v_pad * 4, g.factor = b.factor + local, g.exponents = b.exponents;
-    g.largest = b.count + 1, g.idx = b.idx, g.count = b.count, g.targets = b.idx + t, g.dlogp = dlogp, g.tag = p.tag;
+    g.keep = b.keep + local * p.v_pad * 4, g.factor = b.factor + local;
+    g.idx = b.idx, g.count = b.count, g.targets = b.idx + t, g.dlogp = dlogp, g.tag = p.tag;
     g.scale = b.scale, g.col_top = col_top, g.out = packed_dlogits, g.ld = (long)p.chunk, g.v16 = (int)(p.v_pad / 16);
     g.t16 = (int)(up(rows, 32) / 16), g.j0 = (int)(j0 + local), g.chunk = (int)rows, g.vocab = (int)vocab;
     hipError_t e = launch_fill_zero(reinterpret_cast<float*>(col_top), vocab, st);
