@@ -186,8 +186,8 @@ hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st);
 // order, and the kernels below work on scored rows [j0, j0 + nrows), of which
 // `logits` holds the logits; those at or past *count are zeros in what they
 // write, or not written.  The other arrays are indexed by row.
-//   select:    idx and, from idx + rows on, their targets; count[0], INT_MIN in
-//              count[1], tag in count[2]; the result block (CeMisc; or null), and logp
+//   select:    idx and, from idx + rows on, their targets; count[0], tag in count[1]; the
+//              result block (CeMisc; or null), and logp
 //              and lse (or null) of the rows that are not scored;
 //   gather:    the scored rows of hn side by side;   scatter: back, other rows 0;
 //   grad_rows: the logits become their gradients;
@@ -231,9 +231,8 @@ hipError_t launch_logp_few(const float* hn, const float* head, const int64_t* ta
 // The same for many rows, on packed f16 operands (head_gemm.hip), the logits only
 // in registers.  A plan holds the sizes of the buffers, of which rows are in
 // chunks: those of stats, xt, keep and factor begin at the chunk's first scored row.
-//   pack:      rows, scale, packed and exponents, and with back non-null also that
-//              and count[1] (which select has reset); with rows_back non-null that
-//              too; with head null only what is of rows (rows may be null then);
+//   pack:      rows, scale, packed and exponents, and with back non-null also that, with
+//              rows_back non-null that too; with head null only what is of rows (rows may be null then);
 //   stats:     logp and lse (or null) of scored rows [j0, j0 + chunk), j0 a
 //              multiple of chunk; with keep non-null (and back packed) also that and
 //              factor, from which
@@ -241,7 +240,7 @@ hipError_t launch_logp_few(const float* hn, const float* head, const int64_t* ta
 //   dhead:     what `rows` of them from `local` (a multiple of 128) on add to dhead
 //              (acc 0: give as dhead), in scratch of up(rows, 32) v_pad 4 bytes and vocab words;
 //   zero_rows: dhn of the rows that are not scored.
-// What a forward of other sizes kept (count[2] is not the plan's tag) counts as no
+// What a forward of other sizes kept (count[1] is not the plan's tag) counts as no
 // scored row, and gives NaN gradients.
 struct HeadPlan {
     int k16, splits_max, back_mb, tag;  // 16-k steps of a row

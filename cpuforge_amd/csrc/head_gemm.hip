@@ -19,15 +19,16 @@
 // from the forward: beside its statistics that keeps, for each token and 128
 // rows of the head, exp(x - m) with m their largest logit, in f32 and in the order
 // of the gradient's product (4 bytes a logit).  The product adds 128 rows at a time
-// and scales their sum by exp(m - lse), a factor of the result's own column: no
-// exponential or product is formed twice.  (The logits formed again in the backward
-// instead, 3686 x 576 x 49152: 0.81 ms, where keeping them takes 0.2.)  The waves of
-// that product split the exponentials, which reach them as they are kept; kept as
-// pieces already they would serve no other sum: pieces hold what lies 2^-40 below the
-// largest of 128, enough beside it in the hidden states' gradient, but the head's
-// gradient of a rare token is a sum of its own over tokens, in which nothing larger
-// hides what they lack (a token e^-20 below the others had 4e-3 of its row's gradient
-// wrong, at e^-25 nothing right).
+// and scales their sum by exp(m - lse), a factor of the result's own column, and by the
+// power of two of those rows of the head; where that changes by more than kRun from 32
+// rows to the next, a sum ends there.  No exponential or product is formed twice.  (The
+// logits formed again in the backward instead, 3686 x 576 x 49152: 0.81 ms, where keeping
+// them takes 0.2.)
+// The exponentials are kept in f32 and split by the waves of that product (4% of its
+// time with the forward's).  As pieces, whose last bit is 2^-34 of the largest of 128, they
+// would be exact enough for the hidden states' gradient, where that largest one stands in
+// the same sum, but not for the head's: there a rare token's row is a sum of its own over
+// tokens (e^-20 below the others it lost 4e-3 of itself, at e^-25 all).
 //
 // Packed operands: both are first written as MFMA operands (1 KiB: a lane's eight
 // f16, 64 lanes) of 32 rows and 16 k, the two pieces side by side, so a
@@ -53,7 +54,8 @@ constexpr int kBN = 128;           // tokens of a tile
 constexpr int kWgs = 512;          // two workgroups to a CU
 constexpr int kStages = 3;           // two workgroups' stages fill 147 of 160 KiB
 constexpr int kGroup = 8;          // token tiles
-constexpr float kTop = 32768.0f;   // of a kept exponential in a product
+constexpr float kTop = 4096.0f;    // of a kept exponential in a product
+constexpr int kRun = 3;            // powers of two between the rows of the head of a run
 
 __device__ __forceinline__ float exp2i(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 // 2^e within f32's normal range.
@@ -121,7 +123,7 @@ __device__ __forceinline__ void load8(float (&x)[8], const float* row, int k, in
 
 // Scored rows of [j0, j0 + chunk); none where `count` is another plan's.
 __device__ __forceinline__ int scored_rows(const int* __restrict__ count, int tag, int j0, int chunk) {
-    return count[2] == tag ? max(min(count[0] - j0, chunk), 0) : 0;
+    return count[1] == tag ? max(min(count[0] - j0, chunk), 0) : 0;
 }
 
 struct PackArgs {
@@ -129,7 +131,7 @@ struct PackArgs {
     const int *idx, *count;
     char *rows, *packed, *back, *rows_back;  // rows and rows_back may be null
     float* scale;
-    int *exponents, *largest;
+    int* exponents;
     int row_blocks, vocab, d, k16, v16, t16, vec_rows, vec_head, tag;
 };
 
@@ -196,10 +198,7 @@ __global__ __launch_bounds__(64 * NW) void pack_kernel(const PackArgs g) {
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     const int e = group_exponent(top);
-    if (is_head && threadIdx.x == 0) {
-        g.exponents[blk] = e;
-        if (BACK) atomicMax(g.largest, e);
-    }
+    if (is_head && threadIdx.x == 0) g.exponents[blk] = e;
     if (!is_head && threadIdx.x < 32) g.scale[r] = exp2i(e);
     const float sc = exp2i(-e);
     char* out = is_head ? g.packed : g.rows;
@@ -262,14 +261,14 @@ struct HeadArgs {
     int j0, chunk;      // this launch's: [j0, min(j0 + chunk, count)); b, stats, keep and part start at j0
     long ld;            // of stats, xt and factor
     // statistics: a is the head
-    const int *exponents, *largest, *targets;  // targets: of scored rows
+    const int *exponents, *targets;  // targets: of scored rows
     const float* scale;
     int vocab, v16;
     float2* stats;      // [128 rows of the head][ld]: max and sum of exp2, in log2 units
     float* xt;          // the targets' logits
     char* keep;         // [32 tokens][v16][half of a lane's eight values], or null
     // the rows' gradient: a is the head by columns, b what statistics kept
-    const float* factor;  // [128 rows of the head][ld]; exponents and largest as above
+    const float* factor;  // [128 rows of the head][ld]; exponents as above
     float* part;          // [split][chunk][64 MB mt]
     int splits_max;
     // the head's gradient: a is the dlogits by columns, b the rows by columns
@@ -313,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
     const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1, l32 = lane & 31, hh = lane >> 5;
     const int n = wave_uniform(scored_rows(g.count, g.tag, g.j0, g.chunk));
-    const bool other = P == Product::kHead && wave_uniform(g.count[2]) != g.tag;
+    const bool other = P == Product::kHead && wave_uniform(g.count[1]) != g.tag;
     if (n == 0 && !(P == Product::kHead && (!g.acc || other))) return;
     const int nt = P == Product::kHead ? g.nt : (n + kBN - 1) / kBN;
     // Items of an XCD: a contiguous run of the tiles along a (of the splits), every
@@ -380,8 +379,7 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
         __builtin_amdgcn_s_barrier();
         // (Through the scalar cache: a vector load's wait would be one for the stages' too.)
         const ScalarInts exponents = ROWS ? (ScalarInts)(uintptr_t)g.exponents : nullptr;
-        const int big = ROWS ? *(ScalarInts)(uintptr_t)g.largest : 0;
-        int exponent = ROWS && k0 < k1 ? exponents[k0 / 2] : 0;
+        int exponent = ROWS && k0 < k1 ? exponents[k0 / 2] : 0, run = exponent;
         float kept = 1.0f;
         uint32_t cur = 0, nxt = 2 * STAGE;
         if (k0 < k1) load(0);  // (more splits than runs: some have none)
@@ -396,9 +394,10 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
             if (k + 2 < k1) load(nxt);
             nxt = nxt == (kStages - 1) * STAGE ? 0 : nxt + STAGE;
             if constexpr (ROWS) {
-                // The exponentials meet 32 rows of the head, with their power of two.
+                // The exponentials meet 32 rows of the head, whose power of two is within
+                // kRun of that of the sums.
                 if (k % 2 == 0) {
-                    kept = kTop * pow2_clamped(exponent - big);
+                    kept = kTop * exp2i(exponent - run);
                     exponent = exponents[min(k + 2, k1 - 1) / 2];
                 }
             }
@@ -435,11 +434,13 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
                             acc[i][j] = mfma_f16(a[i][pa[q]], b[j][pb[q]], acc[i][j]);
                         }
             if constexpr (ROWS) {
-                if (k % 8 != 7) continue;
+                if (k % 8 != 7 && (k % 2 == 0 || abs(exponent - run) <= kRun)) continue;
+                const float unit = exp2i(run) * (1.0f / kTop);
+                run = exponent;
                 const float* f = reinterpret_cast<const float*>(s + CH * kFrag + wave * 256);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const float fj = f[32 * j + l32];
+                    const float fj = f[32 * j + l32] * unit;
 #pragma unroll
                     for (int i = 0; i < MB; i++) {
 #pragma unroll
@@ -786,7 +787,6 @@ __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __re
                                                                const int* __restrict__ count, int tag, int j0,
                                                                const float* __restrict__ head,
                                                                const float* __restrict__ dlogp,
-                                                               const int* __restrict__ largest,
                                                                float* __restrict__ dhn, int d) {
     const int n = scored_rows(count, tag, j0, chunk);
     const int quads = (d + 3) / 4;
@@ -807,10 +807,10 @@ __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __re
     const long r = idx[j0 + col];
     const float* w = head + (long)targets[j0 + col] * d + i0;
     float* out = dhn + r * d + i0;
-    const float f = dlogp[r], u = pow2_clamped(*largest - 15), t[4] = {s.x, s.y, s.z, s.w};
+    const float f = dlogp[r], t[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (i0 + i < d) out[i] = f * (w[i] - t[i] * u);
+        if (i0 + i < d) out[i] = f * (w[i] - t[i]);
 }
 
 // What the head's gradient takes of what statistics kept, for scored rows [j0, ..).
@@ -920,7 +920,7 @@ __global__ __launch_bounds__(256) void head_zero_rows_kernel(const int* __restri
             hi = mid;
     }
     if (lo < n && idx[lo] == r) return;
-    const float x = count[2] == tag ? 0.0f : __builtin_nanf("");
+    const float x = count[1] == tag ? 0.0f : __builtin_nanf("");
     for (int i = threadIdx.x; i < d; i += 256) dhn[(long)r * d + i] = x;
 }
 
@@ -970,7 +970,7 @@ hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float
     PackArgs g{};
     g.hn = hn, g.head = head, g.idx = b.idx, g.count = b.count, g.rows = b.rows, g.packed = b.packed, g.back = b.back;
     g.rows_back = b.rows_back, g.t16 = (int)(p.t_pad / 16);
-    g.scale = b.scale, g.exponents = b.exponents, g.largest = b.count + 1, g.row_blocks = (int)(p.t_pad / 32);
+    g.scale = b.scale, g.exponents = b.exponents, g.row_blocks = (int)(p.t_pad / 32);
     g.vocab = (int)vocab, g.d = (int)d, g.k16 = p.k16, g.v16 = (int)(p.v_pad / 16);
     g.vec_rows = d % 4 == 0 && aligned16(hn), g.vec_head = d % 4 == 0 && aligned16(head);
     g.tag = p.tag;
@@ -1044,7 +1044,7 @@ hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, co
     HeadArgs g{};
     g.a = b.back, g.b = b.keep, g.ka = g.kb = (int)(p.v_pad / 16), g.mt = (int)(p.d_pad / (64 * mb)), g.count = b.count;
     g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.factor = b.factor, g.part = b.part;
-    g.splits_max = p.splits_max, g.tag = p.tag, g.exponents = b.exponents, g.largest = b.count + 1;
+    g.splits_max = p.splits_max, g.tag = p.tag, g.exponents = b.exponents;
     if (mb == 3)
         hipLaunchKernelGGL((head_gemm_kernel<3, Product::kRows>), dim3(kWgs), dim3(256), 0, st, g);
     else
@@ -1054,7 +1054,7 @@ hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, co
     const size_t quads = p.chunk * ((d + 3) / 4);
     hipLaunchKernelGGL(head_grad_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, b.part, (int)p.chunk,
                        (int)p.d_pad, g.mt, g.ka, g.splits_max, b.idx, b.idx + t, b.count, p.tag, (int)j0, head,
-                       dlogp, b.count + 1, dhn, (int)d);
+                       dlogp, dhn, (int)d);
     return hipGetLastError();
 }
 

@@ -25,7 +25,7 @@ __device__ __forceinline__ MaxSum merge(const MaxSum& a, const MaxSum& b) {
 
 // The scored rows (targets within the vocabulary) and their targets: idx[0..n) and
 // idx[rows..rows + n) in row order, n and the caller's tag at count[0] and
-// count[2]; the result's counts; logp and lse of the other rows, 0 where the
+// count[1]; the result's counts; logp and lse of the other rows, 0 where the
 // target is ignored and NaN where it is out of range.  One workgroup: 1024
 // targets a round, their places from a scan (4096 targets 5.6 us, latency).
 __global__ __launch_bounds__(1024) void logp_select_kernel(const int64_t* __restrict__ targets, long rows, long vocab,
@@ -67,8 +67,7 @@ __global__ __launch_bounds__(1024) void logp_select_kernel(const int64_t* __rest
     __syncthreads();
     if (threadIdx.x == 0) {
         count[0] = n;
-        count[1] = INT_MIN;  // the largest exponent that head_gemm.hip's pack finds
-        count[2] = tag;
+        count[1] = tag;
         if (misc) {
             int all = 0;
             for (int w = 0; w < 16; w++) all += wave_n[w];

@@ -76,7 +76,8 @@ class Exact:
         group = torch.nn.functional.pad(self.P, (0, -v % 128)).view(len(self.h), -1, 128).amax(2)
         group = group.repeat_interleave(128, 1)[:, :v] * self.p.amax(1, keepdim=True).clamp(max=1e30)
         return (self.p * self.rel) @ self.w + U * (v / 64 + 32) * (self.p @ self.w) \
-            + 2.0 ** -33 * (group @ group_top(self.w).expand_as(self.w)) + U * self.dhn.abs() + 2.0 ** -126
+            + 2.0 ** -33 * (group @ self.w) + self.p @ torch.minimum(self.w, 2.0 ** -39 * group_top(self.w)) \
+            + U * self.dhn.abs() + 2.0 ** -126
 
 
 def report(name, err, bound, want):
@@ -166,3 +167,29 @@ def test_heads_gradient_of_small_and_large_hidden_states(t, keeps, scale):
     hn, head, tg, g = inputs(t, 64, 1500, 9)
     hn[5] *= 1e-8
     check(hn * scale, head / scale, tg, g, keeps)
+
+
+@pytest.mark.parametrize("t,keeps", FORMS)
+@pytest.mark.parametrize("row", [0, 500, 1499])
+def test_hidden_states_gradient_beside_one_large_row(t, keeps, row):
+    """One row of the head 2^25 times the others, alone in its group of 32, with a
+    logit of -32: it moves its own column alone."""
+    hn, head, tg, g = inputs(t, 64, 1500, 8)
+    hn[:, 0] = -2.0 ** -20
+    head[:, 0] = 0.0
+    head[row // 32 * 32:row // 32 * 32 + 32] = 0.0
+    head[row, 0] = 2.0 ** 25
+    tg[tg == row] = 700
+    check(hn, head, tg, g, keeps)
+
+
+@pytest.mark.parametrize("t,keeps", FORMS)
+def test_gradients_where_the_heads_size_changes_from_row_to_row(t, keeps):
+    """Groups of 32 rows of the head 2^-60 to 1 times the others, in any order, so
+    that sums over the vocabulary end and begin in among 128 rows."""
+    hn, head, tg, g = inputs(t, 64, 1500, 10)
+    size = torch.randint(-60, 1, (47,), generator=torch.Generator().manual_seed(3)).to(DEV)
+    head *= torch.exp2(size.float()).repeat_interleave(32)[:1500, None]
+    check(hn, head, tg, g, keeps)
+    head *= 2.0 ** -90
+    check(hn * 2.0 ** 45, head * 2.0 ** 45, tg, g, keeps)
