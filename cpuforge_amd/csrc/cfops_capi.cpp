@@ -647,8 +647,9 @@ int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, co
         if (!keep)
             CF_HIP(c, cfattn::launch_head_stats(p, b, t, j0, vocab, nullptr, nullptr, st),
                    "log-probability launch");
-        if (dhn)
-            CF_HIP(c, cfattn::launch_head_dhn(p, b, t, head, dlogp, j0, d, dhn, st), "log-probability launch");
+        for (size_t i = 0; dhn && i < p.chunk && j0 + i < t; i += p.pass)
+            CF_HIP(c, cfattn::launch_head_dhn(p, b, t, head, dlogp, j0, i, std::min(p.chunk - i, p.pass), d, dhn, st),
+                   "log-probability launch");
         for (size_t i = 0; dhead && i < p.chunk && j0 + i < t; i += pass)
             CF_HIP(c, cfattn::launch_head_dhead(p, b, t, dlogp, j0, i, std::min({t - j0 - i, p.chunk - i, pass}),
                                                 d, vocab, dlogits, col_top, dhead, acc || j0 + i, st),

@@ -236,15 +236,15 @@ hipError_t launch_logp_few(const float* hn, const float* head, const int64_t* ta
 //   stats:     logp and lse (or null) of scored rows [j0, j0 + chunk), j0 a
 //              multiple of chunk; with keep non-null (and back packed) also that and
 //              factor, from which
-//   dhn:       their rows of dhn, and
-//   dhead:     what `rows` of them from `local` (a multiple of 128) on add to dhead
+//   dhn:       `rows` of dhn, at most a pass, from `local` (a multiple of 128) on, and
+//   dhead:     what so many rows add to dhead
 //              (acc 0: give as dhead), in scratch of up(rows, 32) v_pad 4 bytes and vocab words;
 //   zero_rows: dhn of the rows that are not scored.
 // What a forward of other sizes kept (count[1] is not the plan's tag) counts as no
 // scored row, and gives NaN gradients.
 struct HeadPlan {
     int k16, splits_max, back_mb, tag;  // 16-k steps of a row
-    size_t t_pad, v_pad, d_pad, chunk;
+    size_t t_pad, v_pad, d_pad, chunk, pass;  // pass: rows of a dhn
     size_t rows_bytes, head_bytes, back_bytes, stats_bytes, keep_bytes, factor_bytes, rows_back_bytes, part_bytes;
 };
 struct HeadBuffers {
@@ -261,7 +261,8 @@ hipError_t launch_head_mid(const HeadPlan& p, const HeadBuffers& b, const float*
 hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, size_t t, size_t j0, size_t vocab,
                              float* logp, float* lse, hipStream_t st);
 hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* head,
-                           const float* dlogp, size_t j0, size_t d, float* dhn, hipStream_t st);
+                           const float* dlogp, size_t j0, size_t local, size_t rows, size_t d, float* dhn,
+                           hipStream_t st);
 hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* dlogp,
                              size_t j0, size_t local, size_t rows, size_t d, size_t vocab, char* packed_dlogits,
                              unsigned* col_top, float* dhead, int acc, hipStream_t st);

@@ -269,7 +269,7 @@ struct HeadArgs {
     char* keep;         // [32 tokens][v16][half of a lane's eight values], or null
     // the rows' gradient: a is the head by columns, b what statistics kept
     const float* factor;  // [128 rows of the head][ld]; exponents as above
-    float* part;          // [split][chunk][64 MB mt]
+    float* part;          // [split][chunk][64 MB mt], chunk a pass's rows
     int splits_max;
     // the head's gradient: a is the dlogits by columns, b the rows by columns
     const unsigned* col_top;  // [vocab]: a bound of the dlogits of a column, as f32 bits
@@ -928,6 +928,20 @@ inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 size_t up(size_t x, size_t to) { return (x + to - 1) / to * to; }
 
 constexpr int kSplitsMax = 32;
+constexpr size_t kPartBytes = (size_t)512 << 20;
+
+// Rows of a pass of their gradient: those whose sums, by eight splits (of which there are
+// no fewer), fit kPartBytes, and of them those that fill whole rounds of an XCD's workgroups
+// with their tiles (mt to 128 rows).  (Us of the gradient in such passes, in ones of half
+// the bytes and in one: 20000 x 1024 x 32000 4930, 4810 and 4940, 32768 x 2048 x 16000 7240,
+// 7250 and 7480, 65536 x 576 x 8000 2390, 2400 and 2360, 16384 x 4096 x 32000 14830, 17240 and
+// 15660; the third in passes of half the bytes that fill no whole rounds 3010.)
+size_t pass_rows(size_t d_pad, size_t mt, size_t chunk) {
+    const size_t fit = std::max<size_t>(kPartBytes / (8 * d_pad * sizeof(float) * kBN), 1);
+    if (fit * kBN >= chunk) return chunk;
+    const size_t round = kWgs / 8, tiles = mt * fit / round * round;
+    return kBN * (tiles ? tiles / mt : fit);
+}
 
 }  // namespace
 
@@ -946,13 +960,14 @@ HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes) {
     float least = INFINITY;
     for (int mb = 3; mb >= 2; mb--) {
         const size_t d_pad = up(d, 64 * mb);
-        const size_t most = std::min(((size_t)256 << 20) / (p.chunk * d_pad * sizeof(float)), p.v_pad / 256) / 8 * 8;
+        const size_t pass = pass_rows(d_pad, d_pad / (64 * mb), p.chunk);
+        const size_t most = std::min(kPartBytes / 2 / (pass * d_pad * sizeof(float)), p.v_pad / 256) / 8 * 8;
         const int splits_max = (int)std::min<size_t>(std::max<size_t>(most, 8), kSplitsMax);
-        const Splits s = splits_of((int)(d_pad / (64 * mb) * (p.chunk / kBN)), (int)(p.v_pad / 16), splits_max);
-        const float cost = (mb == 3 ? 2.9f : 2.0f) * s.cost;
+        const Splits s = splits_of((int)(d_pad / (64 * mb) * (pass / kBN)), (int)(p.v_pad / 16), splits_max);
+        const float cost = (mb == 3 ? 2.9f : 2.0f) * s.cost / pass;
         if (cost >= least) continue;
         least = cost;
-        p.back_mb = mb, p.d_pad = d_pad, p.splits_max = splits_max;
+        p.back_mb = mb, p.d_pad = d_pad, p.splits_max = splits_max, p.pass = pass;
     }
     p.rows_bytes = p.t_pad * p.k16 * 64;
     p.head_bytes = p.v_pad * p.k16 * 64;
@@ -961,7 +976,7 @@ HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes) {
     p.keep_bytes = p.chunk * p.v_pad * 4;
     p.factor_bytes = (p.v_pad / 128) * p.chunk * sizeof(float);
     p.rows_back_bytes = up(d, kBN) * p.t_pad * 4;
-    p.part_bytes = (size_t)p.splits_max * p.chunk * p.d_pad * sizeof(float);
+    p.part_bytes = (size_t)p.splits_max * p.pass * p.d_pad * sizeof(float);
     return p;
 }
 
@@ -1039,11 +1054,13 @@ hipError_t launch_head_mid(const HeadPlan& p, const HeadBuffers& b, const float*
 }
 
 hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* head,
-                           const float* dlogp, size_t j0, size_t d, float* dhn, hipStream_t st) {
+                           const float* dlogp, size_t j0, size_t local, size_t rows, size_t d, float* dhn,
+                           hipStream_t st) {
     const int mb = p.back_mb;
     HeadArgs g{};
-    g.a = b.back, g.b = b.keep, g.ka = g.kb = (int)(p.v_pad / 16), g.mt = (int)(p.d_pad / (64 * mb)), g.count = b.count;
-    g.j0 = (int)j0, g.chunk = (int)p.chunk, g.ld = (long)p.chunk, g.factor = b.factor, g.part = b.part;
+    g.a = b.back, g.b = b.keep + local * p.v_pad * 4, g.ka = g.kb = (int)(p.v_pad / 16);
+    g.mt = (int)(p.d_pad / (64 * mb)), g.count = b.count, g.j0 = (int)(j0 + local), g.chunk = (int)rows;
+    g.ld = (long)p.chunk, g.factor = b.factor + local, g.part = b.part;
     g.splits_max = p.splits_max, g.tag = p.tag, g.exponents = b.exponents;
     if (mb == 3)
         hipLaunchKernelGGL((head_gemm_kernel<3, Product::kRows>), dim3(kWgs), dim3(256), 0, st, g);
@@ -1051,9 +1068,9 @@ hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, co
         hipLaunchKernelGGL((head_gemm_kernel<2, Product::kRows>), dim3(kWgs), dim3(256), 0, st, g);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const size_t quads = p.chunk * ((d + 3) / 4);
-    hipLaunchKernelGGL(head_grad_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, b.part, (int)p.chunk,
-                       (int)p.d_pad, g.mt, g.ka, g.splits_max, b.idx, b.idx + t, b.count, p.tag, (int)j0, head,
+    const size_t quads = rows * ((d + 3) / 4);
+    hipLaunchKernelGGL(head_grad_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, b.part, g.chunk,
+                       (int)p.d_pad, g.mt, g.ka, g.splits_max, b.idx, b.idx + t, b.count, p.tag, g.j0, head,
                        dlogp, dhn, (int)d);
     return hipGetLastError();
 }

@@ -193,3 +193,28 @@ def test_gradients_where_the_heads_size_changes_from_row_to_row(t, keeps):
     check(hn, head, tg, g, keeps)
     head *= 2.0 ** -90
     check(hn * 2.0 ** 45, head * 2.0 ** 45, tg, g, keeps)
+
+
+@pytest.mark.parametrize("keeps", [True, False])
+def test_scratch_of_the_hidden_states_gradient_is_bounded(keeps):
+    """Many rows of a small vocabulary: 512 MiB for the product's partial sums (and,
+    with nothing kept, 4 bytes a value of the hidden states and a chunk of the logits),
+    their gradient right in every pass."""
+    from cpuforge_amd import ops as P
+    from cpuforge_amd.attention import Context
+    t, d, vocab = 20000, 2048, 300
+    hn, head, tg, g = inputs(t, d, vocab, 11)
+    want = Exact(hn, head, tg, g)
+    bound, exact = want.dhn_bound(), want.dhn
+    del want
+    _, lse, keep = forward(hn, head, tg, keeps)
+    dhn = torch.empty_like(hn)
+    ctx = Context(0)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    P.lm_head_logprobs_backward(hn, head, tg, lse, g, t, d, vocab, dhn, None, keep, ctx=ctx)
+    torch.cuda.synchronize()
+    took = free - torch.cuda.mem_get_info()[0]
+    print(took >> 20, "MiB", flush=True)
+    assert took <= (560 << 20) + (0 if keeps else 4 * t * (d + 512))
+    assert bool(((dhn.double() - exact).abs() <= bound).all())
