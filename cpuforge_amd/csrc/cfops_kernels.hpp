@@ -174,8 +174,9 @@ struct PolicyArgs {
     double low, high, log_low, log_high, kl_coef;  // the ratio's borders and their logarithms
     float* dlogp;
     PolicyResult* result;
-    // set by launch_policy: each part's terms and scored rows, parts to a sequence
-    double* terms;
+    // set by launch_policy: each part's terms and scored rows, parts to a sequence; with
+    // many of them the scored rows and the sequences that have any, else null
+    double *terms, *totals;
     int *counts, parts;
 };
 size_t policy_scratch_bytes(size_t rows, size_t seqs);

@@ -11,7 +11,7 @@
 // empty, the loss is NaN and the result names it.
 //
 // A pass over a sequence needs what another pass summed over it (a pair's rewards;
-// the rows or sequences that a mean is over), so there are two or three launches, each
+// the rows or sequences that a mean is over), so there are two to four launches, most
 // with `parts` workgroups to a sequence: long ones are split, and a part's sums are
 // added in order by whoever needs them.  Bound by those launches: 400 pairs of 2 x 1024
 // rows (13 MB) 9.3 us, 1024 rollouts of 1100 (32 MB) 21 us.
@@ -67,6 +67,12 @@ __device__ __forceinline__ bool is_scored(const int64_t* __restrict__ targets, l
 constexpr int kRows = 2;  // rows of a lane whose loads are in flight together
 constexpr int kWaves = 4;  // of a part's workgroup
 constexpr size_t kWgs = 1024;
+// Workgroups of the policy loss up to which each adds all counts for itself, which saves a
+// launch: beyond, their reads grow with the square of the sequences.  (Us of a captured
+// call, each for itself and once for all: 1024 sequences of 1100 rows 20.8 and 20.4, 2048 of
+// 100 21.7 and 19.2, 4096 of 400 38.3 and 30.3, 16384 of 50 162 and 66, 131072 of 4 5900 and
+// 499.)
+constexpr unsigned kTotalsWgs = 1024;
 
 // Part p of a sequence's rows.
 __device__ __forceinline__ Span part_of(const Span& s, long p, int parts) {
@@ -279,6 +285,14 @@ __device__ __forceinline__ void totals(const PolicyArgs& a, double& n, double& m
     n = x[0], m = x[1];
 }
 
+// The same once for all workgroups.
+__global__ __launch_bounds__(1024) void policy_totals_kernel(const PolicyArgs a) {
+    __shared__ double red[2 * 16];
+    double n, m;
+    totals<16>(a, n, m, red);
+    if (threadIdx.x == 0) a.totals[0] = n, a.totals[1] = m;
+}
+
 // One row's gradient, its terms added to the lane's sums (loss, KL, cut rows).
 __device__ __forceinline__ float policy_row(const PolicyArgs& a, double w, double lp, double old, double ref, double adv,
                                             double (&sums)[3]) {
@@ -365,7 +379,10 @@ __global__ __launch_bounds__(1024) void policy_small_kernel(const PolicyArgs a) 
 __global__ __launch_bounds__(64 * kWaves) void policy_part_kernel(const PolicyArgs a) {
     __shared__ double red[3 * kWaves];
     double n, m, sums[3] = {};
-    totals<kWaves>(a, n, m, red);
+    if (a.totals)
+        n = a.totals[0], m = a.totals[1];
+    else
+        totals<kWaves>(a, n, m, red);
     const long seq = blockIdx.x / (unsigned)a.parts;
     const Span s = part_of(span(a.offsets, seq, a.rows), blockIdx.x % (unsigned)a.parts, a.parts);
     policy_rows<kWaves>(a, seq, s, row_weight(a, seq, n, m), threadIdx.x, sums);
@@ -375,7 +392,10 @@ __global__ __launch_bounds__(64 * kWaves) void policy_part_kernel(const PolicyAr
 __global__ __launch_bounds__(1024) void policy_finish_kernel(const PolicyArgs a) {
     __shared__ double red[3 * 16];
     double n, m, sums[3] = {};
-    totals<16>(a, n, m, red);
+    if (a.totals)
+        n = a.totals[0];
+    else
+        totals<16>(a, n, m, red);
     for (long i = threadIdx.x; i < a.seqs * a.parts; i += 1024)
 #pragma unroll
         for (int k = 0; k < 3; k++) sums[k] += a.terms[3 * i + k];
@@ -403,7 +423,7 @@ size_t preference_scratch_bytes(size_t rows, size_t pairs) {
     return 2 * pairs * parts_of(rows, 2 * pairs) * sizeof(double2);
 }
 size_t policy_scratch_bytes(size_t rows, size_t seqs) {
-    return seqs * parts_of(rows, seqs) * (3 * sizeof(double) + sizeof(int));
+    return 2 * sizeof(double) + seqs * parts_of(rows, seqs) * (3 * sizeof(double) + sizeof(int));
 }
 
 hipError_t launch_preference(PreferenceArgs a, void* scratch, hipStream_t st) {
@@ -423,7 +443,8 @@ hipError_t launch_preference(PreferenceArgs a, void* scratch, hipStream_t st) {
 
 hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st) {
     a.parts = parts_of(a.rows, a.seqs);
-    a.terms = static_cast<double*>(scratch);
+    a.totals = nullptr;
+    a.terms = static_cast<double*>(scratch) + 2;
     a.counts = reinterpret_cast<int*>(a.terms + 3 * a.seqs * a.parts);
     if (small(a.rows, a.seqs)) {
         hipLaunchKernelGGL(policy_small_kernel, dim3(1), dim3(1024), 0, st, a);
@@ -433,6 +454,11 @@ hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st) {
     hipLaunchKernelGGL(policy_count_kernel, dim3(wgs), dim3(64 * kWaves), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    if (wgs > kTotalsWgs) {
+        a.totals = static_cast<double*>(scratch);
+        hipLaunchKernelGGL(policy_totals_kernel, dim3(1), dim3(1024), 0, st, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     hipLaunchKernelGGL(policy_part_kernel, dim3(wgs), dim3(64 * kWaves), 0, st, a);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
