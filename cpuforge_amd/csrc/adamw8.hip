@@ -102,7 +102,9 @@ __device__ __forceinline__ uint32_t max16(uint32_t x) {
     return x;
 }
 
-// Two rounds of a 32-bit multiplicative mix.
+// Two rounds of a 32-bit multiplicative mix.  (Its odd multipliers have no meaning of
+// their own; that the bits are uniform, and those of neighbours, of steps and of m and v
+// uncorrelated, is tested.)
 __device__ __forceinline__ uint32_t mix(uint32_t x) {
     x = (x ^ (x >> 16)) * 0xA511E9B3u;
     x = (x ^ (x >> 15)) * 0x63D83595u;
@@ -143,8 +145,16 @@ __device__ __forceinline__ void store4(float* p, long i, long n, bool vec, const
     if (i + 3 < n) p[i + 3] = x.w;
 }
 
+// Rounding thresholds of a value's m and v, 17 bits each.
+struct Thresholds {
+    uint32_t m, v;
+};
+constexpr Thresholds kNearest{1u << 16, 1u << 16};  // (the middle goes up)
+// From 32 bits: the two share two of them.
+__device__ __forceinline__ Thresholds thresholds(uint32_t r) { return {r & 0x1ffff, r >> 15}; }
+
 // Codes of a block's 16 values of this lane, four to a word, from their high words
-// (m with its sign); threshold(e) are the 32 bits of value e.
+// (m with its sign); threshold(e) are the Thresholds of value e.
 template <typename F>
 __device__ __forceinline__ void encode_block(const uint32_t (&m)[16], const uint32_t (&v)[16], F threshold,
                                              uint32_t (&cm)[4], uint32_t (&cv)[4], int& em, int& ev) {
@@ -165,11 +175,12 @@ __device__ __forceinline__ void encode_block(const uint32_t (&m)[16], const uint
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int e = 4 * j + k;
-            const uint32_t r = threshold(e), hm = m[e] & 0x7fffffff;
-            uint32_t c = odd(hm) ? 0x7fu : encode(hm, lm, r & 0x1ffff);
+            const Thresholds r = threshold(e);
+            const uint32_t hm = m[e] & 0x7fffffff;
+            uint32_t c = odd(hm) ? 0x7fu : encode(hm, lm, r.m);
             c |= (m[e] >> 31) << 7;
             cm[j] |= c << (8 * k);
-            c = odd(v[e]) ? 0xffu : encode(v[e], lv, r >> 15);
+            c = odd(v[e]) ? 0xffu : encode(v[e], lv, r.v);
             cv[j] |= max(c, v[e] ? 1u : 0u) << (8 * k);
         }
     }
@@ -234,7 +245,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Args<N> a) {
     }
     int em, ev;
     encode_block(
-        m, v, [&](int e) { return mix((uint32_t)(i0 + 64 * (e / 4) + e % 4) + a.key); }, cm, cv, em, ev);
+        m, v, [&](int e) { return thresholds(mix((uint32_t)(i0 + 64 * (e / 4) + e % 4) + a.key)); }, cm, cv, em, ev);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         *reinterpret_cast<uint32_t*>(s.m + i0 + 64 * j) = cm[j];
@@ -269,7 +280,7 @@ __global__ __launch_bounds__(256) void adamw8_convert_kernel(const Args<N> a) {
         }
         int em, ev;
         encode_block(
-            m, v, [](int) { return 1u << 16 | 1u << 31; }, cm, cv, em, ev);
+            m, v, [](int) { return kNearest; }, cm, cv, em, ev);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             *reinterpret_cast<uint32_t*>(s.m + i0 + 64 * j) = cm[j];
