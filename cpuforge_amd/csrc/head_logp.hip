@@ -202,8 +202,10 @@ __global__ __launch_bounds__(1024) void logp_few_finish_kernel(const MaxSum* __r
             for (int p = lane; p < parts; p += 64) s = merge(s, stats[(long)r * parts + p]);
 #pragma unroll
             for (int o = 32; o >= 1; o >>= 1) s = merge(s, {__shfl_xor(s.m, o), __shfl_xor(s.s, o)});
-            l = s.m + logf(s.s);
-            lp = xt[r] - l;
+            // (In f64: logp of a likely target is far below an lse, whose rounding it would have.)
+            const double sum = (double)s.m + log((double)s.s);
+            l = (float)sum;
+            lp = (float)((double)xt[r] - sum);
         }
         if (lane == 0) {
             lse[r] = l;
