@@ -88,7 +88,8 @@ __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log
 __device__ __forceinline__ void preference_term(const PreferenceArgs& a, double z, double& l, double& dz) {
     if (a.form == 0) {
         const double s = 1.0 / (1.0 + exp(-fabs(z))), sig = z >= 0.0 ? s : exp(-fabs(z)) * s;
-        l = (1.0 - a.label_smoothing) * softplus(-z) + a.label_smoothing * softplus(z);
+        l = (1.0 - a.label_smoothing) * softplus(-z);
+        if (a.label_smoothing != 0.0) l += a.label_smoothing * softplus(z);  // (0 times infinity is no term)
         dz = (1.0 - a.label_smoothing) * (sig - 1.0) + a.label_smoothing * sig;
     } else if (a.form == 1) {
         l = fmax(1.0 - z, 0.0);
