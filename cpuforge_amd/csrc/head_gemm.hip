@@ -749,7 +749,7 @@ __global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restr
                                                            int tag, int j0, int chunk, float* __restrict__ logp,
                                                            float* __restrict__ lse, float* __restrict__ factor) {
     __shared__ float2 red[16][16];
-    __shared__ float lse2[16];
+    __shared__ float2 all[16];
     const int c = threadIdx.x & 15, p0 = threadIdx.x >> 4, j = blockIdx.x * 16 + c;
     const int n = scored_rows(count, tag, j0, chunk);
     if ((int)blockIdx.x * 16 >= (n + kBN - 1) / kBN * kBN) return;
@@ -762,7 +762,7 @@ __global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restr
     __syncthreads();
     if (p0 == 0) {
         for (int w = 1; w < 16; w++) a = join(a, red[w][c]);
-        lse2[c] = a.x + log2f(a.y);
+        all[c] = make_float2(a.x, 1.0f / a.y);
         if (j < n && logp) {
             // Units of kLog2e as rounded: the quotient has the largest logit's own bits.
             const double l = (double)a.x / (double)kLog2e + log((double)a.y);
@@ -773,8 +773,10 @@ __global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restr
     }
     if (!factor) return;
     __syncthreads();
+    // (By the largest logit and the sum: an lse in f32 is off by 2^-24 of itself, and so would
+    // be every probability; 1 - P of a likely token is much less.)
     for (int p = p0; p < all_parts; p += 64)
-        factor[p * ld + j] = j < n && p < parts ? exp2f(stats[p * ld + j].x - lse2[c]) : 0.0f;
+        factor[p * ld + j] = j < n && p < parts ? exp2f(stats[p * ld + j].x - all[c].x) * all[c].y : 0.0f;
 }
 
 // dhn of scored rows [j0, ..): dlogp (head[target] - the splits' sums in order).
