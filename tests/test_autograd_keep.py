@@ -65,3 +65,40 @@ def test_a_trainable_head_without_a_gradient_takes_a_frozen_ones_memory():
             return torch.cuda.max_memory_allocated() - before, logp
     (frozen, want), (trains, got) = peak(False), peak(True)
     assert trains == frozen and want.shape == got.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,keeps", [((4, 15), False), ((4, 35), True), ((2, 5, 70), True)])
+def test_gradients_are_those_of_the_calls_with_what_the_forward_keeps(rows, keeps):
+    """Bit for bit, of hidden states and head together and of either alone; and they
+    are the 64-bit gradients to f32 products (2^-20 of the largest)."""
+    t, d, vocab = torch.Size(rows).numel(), 48, 500
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    hn = torch.randn(*rows, d, generator=gen, device="cuda").requires_grad_()
+    head = (torch.randn(vocab, d, generator=gen, device="cuda") * 0.3).requires_grad_()
+    tg = torch.randint(0, vocab, rows, generator=gen, device="cuda")
+    tg.view(-1)[::5] = P.IGNORE_INDEX
+    g = torch.randn(*rows, generator=gen, device="cuda")
+
+    n = P.lm_head_logprobs_keep_bytes(t, d, vocab)
+    assert (n > 0) == keeps
+    keep = torch.empty(n, dtype=torch.uint8, device="cuda") if n else None
+    logp, lse = torch.empty(t, device="cuda"), torch.empty(t, device="cuda")
+    flat = (hn.detach().view(t, d), head.detach(), tg.view(-1))
+    P.lm_head_logprobs(*flat, t, d, vocab, logp, lse, P.ce_result_buffer("cuda"), keep)
+    dhn, dhead = torch.empty(t, d, device="cuda"), torch.empty(vocab, d, device="cuda")
+    P.lm_head_logprobs_backward(*flat, lse, g.view(-1), t, d, vocab, dhn, dhead, keep, acc=False)
+
+    got, _ = A.lm_head_logprobs(hn, head, tg)
+    assert got.shape == tg.shape and torch.equal(got.view(-1), logp)
+    both = torch.autograd.grad(got, (hn, head), g)
+    assert torch.equal(both[0].view(t, d), dhn) and torch.equal(both[1], dhead)
+    (one,) = torch.autograd.grad(A.lm_head_logprobs(hn, head.detach(), tg)[0], hn, g)
+    (other,) = torch.autograd.grad(A.lm_head_logprobs(hn.detach(), head, tg)[0], head, g)
+    assert torch.equal(one, both[0]) and torch.equal(other, both[1])
+
+    h, w = hn.detach().double().view(t, d), head.detach().double()
+    hot = torch.zeros(t, vocab, dtype=torch.float64, device="cuda").scatter_(1, tg.view(-1, 1).clamp(min=0), 1.0)
+    D = (hot - torch.softmax(h @ w.T, 1)) * ((tg != P.IGNORE_INDEX) * g).double().view(t, 1)
+    for x, want in ((dhn, D @ w), (dhead, D.T @ h)):
+        assert bool(((x.double() - want).abs() <= 2.0 ** -20 * want.abs().max()).all())
