@@ -24,8 +24,8 @@
 // rows to the next, a sum ends there.  No exponential or product is formed twice.  (The
 // logits formed again in the backward instead, 3686 x 576 x 49152: 0.81 ms, where keeping
 // them takes 0.2.)
-// The exponentials are kept in f32 and split by the waves of that product (4% of its
-// time with the forward's).  As pieces, whose last bit is 2^-34 of the largest of 128, they
+// The exponentials are kept in f32 and split by the waves of that product (2 to 4% of the
+// time of both).  As pieces, whose last bit is 2^-34 of the largest of 128, they
 // would be exact enough for the hidden states' gradient, where that largest one stands in
 // the same sum, but not for the head's: there a rare token's row is a sum of its own over
 // tokens (e^-20 below the others it lost 4e-3 of itself, at e^-25 all).
@@ -295,22 +295,27 @@ __host__ __device__ __forceinline__ Splits splits_of(int tiles, int k16, int spl
     return best;
 }
 
-// A tile of 64 MB rows and kBN columns to a workgroup of four waves, each 32 MB x 64;
-// two workgroups to a CU: one's epilogue runs beside the other's products.
+// A tile of 64 MB rows and kBN columns to a workgroup of four waves, each 32 MB x 64, or, in
+// the rows' gradient, 64 MB x 32, so that no two split the same exponentials (32 MB x 64
+// there: 668 us where this takes 650, 182 where 171); two workgroups to a CU: one's epilogue
+// runs beside the other's products.
 // Bound by the power of the products: statistics of 2048 rows x 576 x 49152 297 us (three
 // times 116 GFLOP on f16, 1.17 PFLOP/s, where a library's f16 product of 8192^3 has 1.16),
 // MFMAs busy in 62% of the cycles at 1.76 GHz, no bank conflicts; 3686 rows with what the
-// gradients need kept 609, their gradient's product 639.  Not faster: 256 x 256 tiles of
+// gradients need kept 583, their gradient's product 650 (603 of operands that need no
+// splitting).  Not faster: 256 x 256 tiles of
 // eight waves, waves of 128 x 128 with a SIMD each (593 us where this took 403), a branch
 // for each 32 columns of a last tile (its registers spill).
 template <int MB, Product P>
 __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
     constexpr bool ROWS = P == Product::kRows;
+    // Blocks of 32 rows and columns of a wave's part of the tile.
+    constexpr int RB = ROWS ? 2 * MB : MB, CB = ROWS ? 1 : 2;
     constexpr int BM = 64 * MB, CH = 4 * MB + 8, PER = CH / 4 + ROWS, STAGE = CH * kFrag + ROWS * 1024;
     static_assert(CH % 4 == 0, "whole loads a wave");
     __shared__ __attribute__((aligned(1024))) char lds[kStages * STAGE];
     const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
-    const int wm = wave >> 1, wn = wave & 1, l32 = lane & 31, hh = lane >> 5;
+    const int wm = ROWS ? 0 : wave >> 1, wn = ROWS ? wave : wave & 1, l32 = lane & 31, hh = lane >> 5;
     const int n = wave_uniform(scored_rows(g.count, g.tag, g.j0, g.chunk));
     const bool other = P == Product::kHead && wave_uniform(g.count[1]) != g.tag;
     if (n == 0 && !(P == Product::kHead && (!g.acc || other))) return;
@@ -351,8 +356,8 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
                                             : g.b + ((long)(tt * 4 + blk - 2 * MB) * g.kb + k0) * 2 * kFrag;
             src[i] = base + (c % 2) * kFrag;
         }
-        const int col0 = tt * kBN + wn * 64;  // this wave's first column
-        int kl = k0;                          // the next stage's k
+        const int col0 = tt * kBN + wn * 32 * CB;  // this wave's first column
+        int kl = k0;                               // the next stage's k
         auto load = [&](uint32_t stage) {
 #pragma unroll
             for (int i = 0; i < CH / 4; i++) {
@@ -361,18 +366,20 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
             }
             if constexpr (ROWS) {
                 // The factors of the stage's 128 rows for the wave's tokens.
-                lds_load4_so(g.factor + (long)(kl / 8) * g.ld + col0, lane * 4, lds0 + stage + CH * kFrag + wave * 256);
+                lds_load4_so(g.factor + (long)(kl / 8) * g.ld + col0, l32 * 4, lds0 + stage + CH * kFrag + wave * 256);
                 kl++;
             }
         };
         // (A wave of a last tile whose columns all lie behind the last one forms nothing.)
         const bool live_cols = P == Product::kHead || col0 < n;
-        f32x16 acc[MB][2], tot[ROWS ? MB : 1][2];
+        f32x16 acc[RB][CB], tot[ROWS ? RB : 1][CB];
 #pragma unroll
-        for (int i = 0; i < MB; i++) {
-            acc[i][0] = acc[i][1] = zero16();
-            if constexpr (ROWS) tot[i][0] = tot[i][1] = zero16();
-        }
+        for (int i = 0; i < RB; i++)
+#pragma unroll
+            for (int j = 0; j < CB; j++) {
+                acc[i][j] = zero16();
+                if constexpr (ROWS) tot[i][j] = zero16();
+            }
         // Every wave is done with the LDS of the item before, and with its stores
         // (they would count among the loads waited for below).
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -403,34 +410,40 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
             }
             const char* s = lds + cur;
             cur = cur == (kStages - 1) * STAGE ? 0 : cur + STAGE;
-            f16x8 a[MB][2], b[2][2];
+            f16x8 a[RB][2], b[CB][2];
+            f32x4 kept_b[2];
+            if constexpr (ROWS) {
+                kept_b[0] = *reinterpret_cast<const f32x4*>(s + (2 * MB + wn) * 2 * kFrag + voff);
+                kept_b[1] = *reinterpret_cast<const f32x4*>(s + ((2 * MB + wn) * 2 + 1) * kFrag + voff);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const char* at = s + (2 * MB + wn * 2 + j) * 2 * kFrag + voff;
-                if constexpr (ROWS) {
-                    const Pieces x = split8(*reinterpret_cast<const f32x4*>(at),
-                                            *reinterpret_cast<const f32x4*>(at + kFrag), kept);
-                    b[j][0] = x.h, b[j][1] = x.l;
-                } else {
-                    b[j][0] = *reinterpret_cast<const f16x8*>(at);
-                    b[j][1] = *reinterpret_cast<const f16x8*>(at + kFrag);
-                }
+                for (int p = 0; p < 2; p++)
+#pragma unroll
+                    for (int j = 0; j < CB; j++)
+                        b[j][p] = *reinterpret_cast<const f16x8*>(s + ((2 * MB + wn * CB + j) * 2 + p) * kFrag + voff);
             }
 #pragma unroll
-            for (int p = 0; p < 2; p++)
+            for (int p = 1; p >= 0; p--) {
 #pragma unroll
-                for (int i = 0; i < MB; i++)
-                    a[i][p] = *reinterpret_cast<const f16x8*>(s + ((wm * MB + i) * 2 + p) * kFrag + voff);
+                for (int i = 0; i < RB; i++)
+                    a[i][p] = *reinterpret_cast<const f16x8*>(s + ((wm * RB + i) * 2 + p) * kFrag + voff);
+                // (The first products' operands are read together.)
+                if (ROWS && (p == 1 || MB == 2)) __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (ROWS) {
+                const Pieces x = split8(kept_b[0], kept_b[1], kept);
+                b[0][0] = x.h, b[0][1] = x.l;
+            }
             // (The order that shares an operand from one to the next: 1% less time.)
             constexpr int pa[3] = {1, 0, 0}, pb[3] = {0, 0, 1};
             if (live_cols)
 #pragma unroll
                 for (int q = 0; q < 3; q++)
 #pragma unroll
-                    for (int i = 0; i < MB; i++)
+                    for (int i = 0; i < RB; i++)
 #pragma unroll
-                        for (int jj = 0; jj < 2; jj++) {
-                            const int j = (i + q) & 1 ? 1 - jj : jj;
+                        for (int jj = 0; jj < CB; jj++) {
+                            const int j = (i + q) & 1 ? CB - 1 - jj : jj;
                             acc[i][j] = mfma_f16(a[i][pa[q]], b[j][pb[q]], acc[i][j]);
                         }
             if constexpr (ROWS) {
@@ -439,10 +452,10 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
                 run = exponent;
                 const float* f = reinterpret_cast<const float*>(s + CH * kFrag + wave * 256);
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
+                for (int j = 0; j < CB; j++) {
                     const float fj = f[32 * j + l32] * unit;
 #pragma unroll
-                    for (int i = 0; i < MB; i++) {
+                    for (int i = 0; i < RB; i++) {
 #pragma unroll
                         for (int q = 0; q < 16; q++) tot[i][j][q] = fmaf(acc[i][j][q], fj, tot[i][j][q]);
                         acc[i][j] = zero16();
@@ -451,7 +464,7 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
             }
         }
 
-        const int m0 = tm * BM + wm * 32 * MB;  // this wave's first row
+        const int m0 = tm * BM + wm * 32 * RB;  // this wave's first row
         if constexpr (P == Product::kHead) {
 #pragma unroll
             for (int i = 0; i < MB; i++) {
@@ -484,12 +497,12 @@ __global__ __launch_bounds__(256, 2) void head_gemm_kernel(const HeadArgs g) {
         } else if constexpr (ROWS) {
             const int rows = g.mt * BM;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < CB; j++) {
                 const int col = col0 + 32 * j + l32;
                 float* out = g.part + ((long)o * g.chunk + col) * rows + m0 + 4 * hh;
                 if (col < n)
 #pragma unroll
-                    for (int i = 0; i < MB; i++)
+                    for (int i = 0; i < RB; i++)
 #pragma unroll
                         for (int q = 0; q < 4; q++)
                             *reinterpret_cast<float4*>(out + 32 * i + 8 * q) =
