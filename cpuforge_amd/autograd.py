@@ -190,17 +190,18 @@ LOGPROBS_KEEP_LIMIT = 8 << 30
 
 class LMHeadLogprobsFn(torch.autograd.Function):
     """The targets' log-probabilities under logits = hn head^T and the block
-    that ops.ce_check reads (ops.lm_head_logprobs)."""
+    that ops.ce_check reads (ops.lm_head_logprobs).  `keeps`: whether to keep
+    what a backward reads (None: where an input requires a gradient)."""
 
     @staticmethod
-    def forward(ctx, hn, head, targets, keeps: bool):
+    def forward(ctx, hn, head, targets, keeps: bool | None = None):
         d = hn.shape[-1]
         h2, head2, tg = _flat(hn, d), head.contiguous(), targets.contiguous().view(-1)
         t, vocab = h2.shape[0], head2.shape[0]
         logp, lse = _empty(tg, tg)
         result = P.ce_result_buffer(hn.device)
         keep = None
-        if keeps:
+        if any(ctx.needs_input_grad) if keeps is None else keeps:
             n = P.lm_head_logprobs_keep_bytes(t, d, vocab)
             if 0 < n <= LOGPROBS_KEEP_LIMIT:
                 keep = torch.empty(n, dtype=torch.uint8, device=hn.device)

@@ -39,6 +39,14 @@ def test_a_forward_keeps_for_its_backward(keeps, hn_grad, head_grad):
     assert keeps == [4 * 5 * 7] and logp.requires_grad and not block.requires_grad
 
 
+def test_the_function_itself_takes_three_arguments(keeps, monkeypatch):
+    monkeypatch.setattr(P, "lm_head_logprobs_backward", lambda hn, head, *a, acc: (a[6].fill_(1.0), a[7].fill_(2.0)))
+    hn, head = torch.zeros(5, 3, requires_grad=True), torch.zeros(7, 3, requires_grad=True)
+    logp, _ = A.LMHeadLogprobsFn.apply(hn, head, torch.zeros(5, dtype=torch.int64))
+    logp.sum().backward()
+    assert keeps == [4 * 5 * 7] and bool((hn.grad == 1.0).all()) and bool((head.grad == 2.0).all())
+
+
 def test_frozen_operands_keep_nothing(keeps):
     logp, _ = call(False, False)
     assert keeps == [None] and not logp.requires_grad
