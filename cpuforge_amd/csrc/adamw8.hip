@@ -233,8 +233,10 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Args<N> a) {
             const double md = fma(d1, gd, b1 * decode_m(cm[j] >> (8 * k) & 0xff, um));
             const double vd = fma(d2 * gd, gd, b2 * decode_v(cv[j] >> (8 * k) & 0xff, uv));
             const float mf = (float)md, vf = (float)vd;
-            // (The instructions' square root and reciprocal, to a step of f32: what they are
-            // off by is 2^-23 of an update that is itself a thousandth of p or less.)
+            // (The instructions' square root and reciprocal, to a step of f32 each: 2^-22 of the
+            // update.  2-norm of the error of p against 64 bits, so and correctly rounded, both in
+            // f32: 2.54e-8 and 2.54e-8 where the update is a thousandth of p, 2.72e-8 and 2.63e-8
+            // where it is a twentieth, 7.3e-8 and 6.7e-8 where p starts from zeros.)
             const float den = fmaf(__builtin_amdgcn_sqrtf(vf), a.c2, a.eps);
             const float upd = fmaf(mf * a.c1, __builtin_amdgcn_rcpf(den), t.weight_decay * p[e]);
             p[e] = fmaf(-a.lr, upd, p[e]);

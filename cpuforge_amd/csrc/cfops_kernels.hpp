@@ -208,10 +208,10 @@ hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t 
 constexpr size_t kLogpFew = 32;
 // Up to as many rows a forward keeps nothing, and the gradients are f32 products over
 // logits formed again.  Forward and dhn so, and over packed operands with what the forward
-// keeps for them, us: 64 rows 576 x 49152 170 and 170, 2048 x 49152 377 and 467, 2048 x
-// 128256 917 and 1107, 500 x 50001 176 and 162; 96 rows 220 and 176, 500 and 471, 1173 and
-// 1122, 216 and 164.  With the head's gradient 64 rows 227 and 260, 584 and 688, 1489 and
-// 1654, 230 and 260.
+// keeps for them, us: 64 rows 576 x 49152 177 and 182, 2048 x 49152 390 and 469, 2048 x
+// 128256 913 and 1109, 500 x 50001 179 and 173; 96 rows 225 and 183, 511 and 475, 1191 and
+// 1121, 219 and 175.  With the head's gradient 64 rows 232 and 269, 590 and 689, 1488 and
+// 1664, 231 and 265.
 constexpr size_t kLogpUnkept = 64;
 // Which form takes the forward, us of a call by either (rows, d x vocab):
 //   few or mid: 16 rows 576 x 49152 37 and 43, 2048 x 128256 267 and 249; 17 rows 46 and

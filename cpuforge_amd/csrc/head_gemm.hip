@@ -794,7 +794,7 @@ __global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restr
 
 // dhn of scored rows [j0, ..): dlogp (head[target] - the splits' sums in order).
 // Four columns to a thread, eight splits' sums in flight: bound by memory, 3686 x 576 with
-// 16 splits (136 MB) 27 us.
+// 16 splits (136 MB) 29 us.
 __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __restrict__ part, int chunk, int rows,
                                                                int mt, int k16, int splits_max,
                                                                const int* __restrict__ idx,
@@ -847,7 +847,8 @@ __device__ __forceinline__ float row_top(float scale) { return scale * 16384.0f;
 // The largest of every column's dlogits times their rows' row_top: a column's power of
 // two is its own, since a token that is rarely likely has gradients far below the
 // others', which an optimizer that divides by their size scales up.  128 columns and
-// every 8th 32 rows to a workgroup.  (The probability beside 1 at a target counts as 1.)
+// every 8th 32 rows to a workgroup: 819 rows x 50001 (180 MB) 31 us.  (At a target 1 - P
+// counts as 1.)
 __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
     const int n = scored_rows(g.count, g.tag, g.j0, g.chunk);
@@ -884,7 +885,7 @@ __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) 
 
 // The dlogits times their rows' row_top as operands by columns: 32 rows and 128 columns
 // to a workgroup, turned round in LDS.  Bound by memory: 819 x 50001, read and written,
-// (328 MB) 57 us.
+// (328 MB) 54 us.
 __global__ __launch_bounds__(256) void head_pack_dlogits_kernel(const DlogitsArgs g) {
     __shared__ float tile[32][129];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
@@ -969,9 +970,9 @@ HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes) {
     p.chunk = std::min(std::max<size_t>(chunk_bytes / (p.v_pad * 4) / kBN * kBN, kBN), p.t_pad);
     // Blocks of 32 columns of the head of a wave in the rows' gradient (whose sums take
     // twice the registers): two or three, by which the tiles fill the card better, were
-    // all rows scored.  (Us of the product by three and by two: 500 x 2048 x 49152 372 and
-    // 306, 300 x 576 x 49152 97 and 78, 1000 x 768 x 32000 159 and 183, 2000 x 129 x 49152
-    // 143 and 168.)
+    // all rows of a pass scored.  (Us of the gradient by three and by two: 500 x 2048 x 49152
+    // 417 and 394, 300 x 576 x 49152 107 and 98, 1000 x 768 x 32000 174 and 206, 2000 x 129 x
+    // 49152 145 and 191.)
     float least = INFINITY;
     for (int mb = 3; mb >= 2; mb--) {
         const size_t d_pad = up(d, 64 * mb);

@@ -414,7 +414,8 @@ static bool small(size_t rows, size_t seqs) { return seqs <= 16 && rows <= 1024 
 // Workgroups to a sequence: with few long sequences as many as fill the card, of no
 // fewer than two rows a lane on average.  (One of 65536 rows: preference 61 and policy
 // 195 us by one workgroup, 6.8 and 12.6 by 128.  As many to every sequence, 128 of 128
-// rows by 8 each: 22 where one takes 6.)
+// rows by 8 each: 22 where one takes 6.)  By the mean length: one long sequence beside
+// hundreds of short ones has one workgroup.
 static int parts_of(size_t rows, size_t seqs) {
     if (small(rows, seqs)) return 1;
     return (int)std::max<size_t>(1, std::min(kWgs / seqs, rows / (seqs * kRows * 64 * kWaves)));

@@ -179,7 +179,8 @@ int cfops_adamw_update_multi(cfattn_ctx* ctx, size_t count, float* const* p, con
  * over the scored rows, result->bad_row names the first row whose target is
  * outside [0, vocab) (such a row's logp and lse are NaN), as
  * cfops_lm_head_ce_dev's does.  The logits are never held whole.  d and vocab
- * must be positive, t below 2^24 and vocab below 2^26.
+ * must be positive, t below 2^24 and vocab below 2^26.  What is not finite in a row
+ * of hn stays with that row; in the head it is in every row's sum.
  * `keep` (device memory of keep_bytes, 16-byte aligned, or NULL) takes what a
  * backward reads, so that it need not form the logits again: a buffer of
  * cfops_lm_head_logprobs_keep_bytes(t, d, vocab), about 4 t vocab + 4 d vocab
@@ -194,7 +195,8 @@ int cfops_lm_head_logprobs(cfattn_ctx* ctx, const float* hn, const float* head, 
  * are formed again, a chunk of rows that fit cfops_set_head_chunk_limit at a
  * time; what a forward of other sizes kept gives NaN gradients).  Rows that are
  * not scored, or have a target out of range, have no gradient, and
- * their hn, lse and dlogp do not matter. */
+ * their hn, lse and dlogp do not matter.  Each row of dhead is exact to f32 of its
+ * own size, however small its probabilities (to e^-60) or its row of the head. */
 int cfops_lm_head_logprobs_backward(cfattn_ctx* ctx, const float* hn, const float* head, const int64_t* targets,
                                     const float* lse, const float* dlogp, size_t t, size_t d, size_t vocab,
                                     float* dhn, float* dhead, int acc, const void* keep, size_t keep_bytes,
