@@ -968,7 +968,7 @@ HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes) {
     p.v_pad = up(vocab, 256);
     p.t_pad = up(t, kBN);
     p.chunk = std::min(std::max<size_t>(chunk_bytes / (p.v_pad * 4) / kBN * kBN, kBN), p.t_pad);
-    // Blocks of 32 columns of the head of a wave in the rows' gradient (whose sums take
+    // Half the blocks of 32 columns of the head of a wave in the rows' gradient (whose sums take
     // twice the registers): two or three, by which the tiles fill the card better, were
     // all rows of a pass scored.  (Us of the gradient by three and by two: 500 x 2048 x 49152
     // 417 and 394, 300 x 576 x 49152 107 and 98, 1000 x 768 x 32000 174 and 206, 2000 x 129 x

@@ -218,3 +218,46 @@ def test_scratch_of_the_hidden_states_gradient_is_bounded(keeps):
     print(took >> 20, "MiB", flush=True)
     assert took <= (560 << 20) + (0 if keeps else 4 * t * (d + 512))
     assert bool(((dhn.double() - exact).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("keeps", [True, False])
+@pytest.mark.parametrize("masked", [0.0, 0.7, 1.0])
+def test_passes_with_few_or_no_scored_rows(keeps, masked):
+    """Three passes of rows, of which the scored ones fill three, one or none."""
+    hn, head, tg, g = inputs(5000, 8192, 300, 12, masked)
+    want = Exact(hn, head, tg, g)
+    dhn, dhead = gradients(hn, head, tg, g, keeps)
+    assert bool(((dhn - want.dhn).abs() <= want.dhn_bound()).all()) and not dhn[tg == IGN].any()
+    assert bool(((dhead - want.dhead).abs() <= want.dhead_bound()).all())
+
+
+@pytest.mark.parametrize("t,d", [(60, 96), (700, 96), (5000, 8192)])
+def test_captured_gradients_replay_with_what_the_forward_keeps(t, d):
+    """Forward and both gradients in one graph, whose keep is written anew by every
+    replay, with eager calls of the same context between the replays."""
+    from cpuforge_amd import ops as P
+    hn, head, tg, g = inputs(t, d, 300, 13)
+    n = P.lm_head_logprobs_keep_bytes(t, d, 300)
+
+    def bufs():
+        keep = torch.zeros(n, dtype=torch.uint8, device=DEV) if n else None
+        return torch.zeros(t, device=DEV), torch.zeros(t, device=DEV), torch.zeros_like(hn), torch.zeros_like(head), keep
+
+    def step(b):
+        logp, lse, dhn, dhead, keep = b
+        P.lm_head_logprobs(hn, head, tg, t, d, 300, logp, lse, res, keep)
+        P.lm_head_logprobs_backward(hn, head, tg, lse, g, t, d, 300, dhn, dhead, keep, acc=False)
+    res = P.ce_result_buffer(DEV)
+    a, b = bufs(), bufs()
+    step(b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(a)
+    for i in range(4):
+        hn.mul_(0.99)
+        tg.copy_(tg.roll(7))
+        graph.replay()
+        torch.cuda.synchronize()
+        step(b)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(a[:4], b[:4])), i

@@ -70,3 +70,40 @@ def test_policys_time_grows_no_faster_than_its_sequences():
     few, many = least(40000), least(160000)
     print(few, many, flush=True)
     assert many < 8 * few
+
+
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_captured_policy_of_many_sequences_replays(reduction):
+    from cpuforge_amd import ops as P
+    off, _, tg, lp, ref, old, g = batch(3000, 20, 2)
+    adv = torch.randn(3000, generator=g, device=DEV)
+
+    def step(d, res):
+        P.policy_loss(lp, old, ref, adv, tg, off, d, res, clip_low=0.2, clip_high=0.3, kl_coef=0.1, reduction=reduction)
+
+    def bufs():
+        return torch.zeros_like(lp), torch.zeros(P.POLICY_RESULT_WORDS, dtype=torch.int32, device=DEV)
+    a, b = bufs(), bufs()
+    step(*b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*a)
+    for i in range(4):
+        lp.add_(0.01)
+        tg.copy_(tg.roll(1))
+        graph.replay()
+        torch.cuda.synchronize()
+        step(*b)
+        assert all(torch.equal(x, y) for x, y in zip(a, b)), i
+
+
+def test_bad_offsets_among_many_sequences():
+    from cpuforge_amd import _lib
+    from cpuforge_amd import ops as P
+    off, _, tg, lp, ref, old, g = batch(3000, 20, 3)
+    off[2001] = lp.numel() + 7  # sequences 2000 and 2001 do not rise within the rows
+    d, res = torch.full_like(lp, 77.0), torch.zeros(P.POLICY_RESULT_WORDS, dtype=torch.int32, device=DEV)
+    P.policy_loss(lp, old, ref, torch.ones(3000, device=DEV), tg, off, d, res, clip_low=0.2, clip_high=0.3)
+    with pytest.raises(_lib.CfattnError, match="sequence 2000 "):
+        P.policy_check(res)
+    assert P.policy_result(res).loss.isnan() and bool((d[off[2000]:off[2002]] == 77.0).all())
