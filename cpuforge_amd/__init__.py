@@ -22,6 +22,6 @@ from .attention import (  # noqa: F401
     flops_fwd_bwd,
     set_mode,
 )
-from .rope import Llama3Scaling, RopeCache  # noqa: F401
+from .rope import LinearScaling, Llama3Scaling, NtkScaling, RopeCache, YarnScaling  # noqa: F401
 
 __version__ = "0.1.0"

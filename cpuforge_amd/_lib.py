@@ -33,6 +33,13 @@ class Llama3ScalingC(C.Structure):
                 ("original_max_position", C.c_double)]
 
 
+class RopeScalingC(C.Structure):
+    """`cfattn_rope_scaling` (include/cfattn.h)."""
+    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("low_freq_factor", C.c_double),
+                ("high_freq_factor", C.c_double), ("original_max_position", C.c_double), ("beta_fast", C.c_double),
+                ("beta_slow", C.c_double), ("attention_factor", C.c_double)]
+
+
 class PrologueC(C.Structure):
     _fields_ = [("cos", _vp), ("sin", _vp), ("max_pos", _sz), ("pos0", _sz), ("q_norm", _vp), ("k_norm", _vp),
                 ("eps", C.c_float)]
@@ -48,6 +55,11 @@ class AdamwTensorC(C.Structure):
     """`cfops_adamw_tensor` (include/cfops.h)."""
     _fields_ = [("p", _vp), ("g", _vp), ("m", _vp), ("v", _vp), ("state8", _vp), ("n", _sz),
                 ("weight_decay", C.c_float)]
+
+
+class RotaryTensorC(C.Structure):
+    """`cfops_rotary_tensor` (include/cfops.h)."""
+    _fields_ = [("x", _vp), ("y", _vp), ("heads", _sz), ("x_stride", C.c_int64 * 3), ("y_stride", C.c_int64 * 3)]
 
 
 SIGNATURES = {
@@ -73,6 +85,7 @@ SIGNATURES = {
     "cfattn_fused_bwd": (C.c_int, [_vp, Shape, _sz, C.c_int, C.POINTER(PrologueC)] + [_vp] * 16),
     "cfattn_fused_bwd_grad": (C.c_int, [_vp, Shape, _sz, C.c_int, C.POINTER(PrologueC)] + [_vp] * 16),
     "cfattn_rope_table": (C.c_int, [_sz, _sz, C.c_double, C.POINTER(Llama3ScalingC), _vp, _vp]),
+    "cfattn_rope_table_scaled": (C.c_int, [_sz, _sz, C.c_double, C.POINTER(RopeScalingC), _vp, _vp]),
     "cfattn_llama3_scale": (C.c_double, [C.POINTER(Llama3ScalingC), C.c_double]),
     "cfattn_f32_to_bf16": (C.c_int, [_vp, _vp, _vp, _sz, _vp]),
     "cfattn_set_ds_limit": (C.c_int, [_vp, _sz]),
@@ -93,6 +106,10 @@ SIGNATURES = {
     "cfops_rmsnorm_forward": (C.c_int, [_vp] * 5 + [_sz, _sz, C.c_float, _vp]),
     "cfops_rmsnorm_backward": (C.c_int, [_vp] * 7 + [_sz, _sz, _vp]),
     "cfops_rmsnorm_grad": (C.c_int, [_vp] * 7 + [_sz, _sz, C.c_int, _vp]),
+    "cfops_layernorm_forward": (C.c_int, [_vp, C.c_int] + [_vp] * 6 + [_sz, _sz, C.c_float, _vp]),
+    "cfops_layernorm_backward": (C.c_int, [_vp, C.c_int] + [_vp] * 8 + [_sz, _sz, C.c_int, _vp]),
+    "cfops_rotary": (C.c_int, [_vp, C.POINTER(RotaryTensorC), _sz, C.c_int, C.c_int] + [_sz] * 4 + [_vp] * 2
+                     + [_sz, _vp, _sz, C.c_int, C.c_int, _vp]),
     "cfops_silu_mul_grad": (C.c_int, [_vp] * 6 + [_sz, C.c_int, _vp]),
     "cfops_silu_mul_forward": (C.c_int, [_vp] * 4 + [_sz, _vp]),
     "cfops_silu_mul_backward": (C.c_int, [_vp] * 6 + [_sz, _vp]),
@@ -142,6 +159,7 @@ CFIO_DTYPES = ["BOOL", "F4", "F6_E2M3", "F6_E3M2", "U8", "I8", "F8_E5M2", "F8_E4
 
 # matmul kinds of cfops_matmul (include/cfops.h)
 NN, NT, TN = 0, 1, 2
+ROTARY_MAX = 4  # CFOPS_ROTARY_MAX
 IGNORE_INDEX = -100
 
 _lib = None

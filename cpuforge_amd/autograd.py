@@ -47,6 +47,57 @@ class RMSNormFn(torch.autograd.Function):
         return dx.view(dy.shape), dw, None
 
 
+class LayerNormFn(torch.autograd.Function):
+    """y = layernorm(x, w, b) over the last dim (ops.layernorm_forward); x f32 or
+    bf16, b may be None."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, eps: float):
+        dim = x.shape[-1]
+        x2 = x.contiguous().view(x.numel() // dim if dim else 0, dim)
+        w, b = w.contiguous(), None if b is None else b.contiguous()
+        rows = x2.shape[0]
+        y = torch.empty_like(x2)
+        mean, rstd = torch.empty(2, rows, device=x.device, dtype=torch.float32).unbind()
+        P.layernorm_forward(x2, w, b, y, mean, rstd, rows, dim, eps)
+        ctx.save_for_backward(x2, w, mean, rstd)
+        return y.view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2, w, mean, rstd = ctx.saved_tensors
+        rows, dim = x2.shape
+        dx = torch.empty_like(x2)
+        dw, db = (torch.empty_like(w) if need else None for need in ctx.needs_input_grad[1:3])
+        P.layernorm_backward(dy.contiguous().view(rows, dim), x2, w, mean, rstd, dx, dw, db, rows, dim, acc=False)
+        return dx.view(dy.shape), dw, db, None
+
+
+class RotaryFn(torch.autograd.Function):
+    """ops.rotary into new tensors of `dtype` (None: each of its own type)."""
+
+    @staticmethod
+    def forward(ctx, cos, sin, positions, pos0, interleaved, dtype, *xs):
+        ys = tuple(torch.empty(x.shape, device=x.device, dtype=dtype or x.dtype) for x in xs)
+        kw = dict(pos0=pos0, interleaved=interleaved)
+        P.rotary(tuple(_rows(x) for x in xs), ys, cos, sin, positions, **kw)
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.kw, ctx.dtypes = kw, [x.dtype for x in xs]
+        return ys
+
+    @staticmethod
+    def backward(ctx, *dys):
+        cos, sin, positions = ctx.saved_tensors
+        dxs = tuple(torch.empty(dy.shape, device=dy.device, dtype=t) for dy, t in zip(dys, ctx.dtypes))
+        P.rotary(tuple(_rows(dy) for dy in dys), dxs, cos, sin, positions, inverse=True, **ctx.kw)
+        return (None,) * 6 + dxs
+
+
+def _rows(x):
+    """x itself, or a copy where a head's values do not lie side by side."""
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
 class SiluMulFn(torch.autograd.Function):
     """h = silu(g) * u (crates/core/src/ops/swiglu.rs)."""
 
@@ -268,6 +319,19 @@ def _c(t):
 
 def rmsnorm(x, w, eps):
     return RMSNormFn.apply(x, w, eps)
+
+
+def layer_norm(x, w, b, eps):
+    """Layer norm over the last dim, w and b float32 (b may be None)."""
+    return LayerNormFn.apply(x, w, b, eps)
+
+
+def rotary(xs, cos, sin, positions=None, *, pos0=0, interleaved=False, dtype=None):
+    """ops.rotary of a tensor or several (q and k, [B, S, H, D] of one type), into
+    new ones of `dtype` (None: theirs): a tensor, or a tuple of as many."""
+    one = isinstance(xs, torch.Tensor)
+    ys = RotaryFn.apply(cos, sin, positions, pos0, interleaved, dtype, *((xs,) if one else xs))
+    return ys[0] if one else ys
 
 
 def silu_mul(g, u):

@@ -694,6 +694,53 @@ int cfattn_rope_table(size_t head_dim, size_t max_pos, double theta, const cfatt
     return CFATTN_OK;
 }
 
+int cfattn_rope_table_scaled(size_t head_dim, size_t max_pos, double theta, const cfattn_rope_scaling* sc,
+                             float* cos_out, float* sin_out) {
+    if (head_dim % 2 != 0) return CFATTN_ERR_SHAPE;
+    if ((!cos_out || !sin_out) && max_pos * head_dim > 0) return CFATTN_ERR_ARG;
+    if (!sc || sc->kind < CFATTN_ROPE_LINEAR || sc->kind > CFATTN_ROPE_YARN || !(sc->factor > 0.0) ||
+        !(sc->attention_factor >= 0.0) || !(theta > 0.0))
+        return CFATTN_ERR_ARG;
+    const size_t half = head_dim / 2;
+    const double dim = (double)head_dim;
+    double first = 0.0, last = 0.0, size = 1.0;
+    if (sc->kind == CFATTN_ROPE_NTK) {
+        // (One pair has the frequency 1 whatever theta is.)
+        if (head_dim > 2) theta *= std::pow(sc->factor, dim / (dim - 2.0));
+    } else if (sc->kind == CFATTN_ROPE_YARN) {
+        if (!(sc->original_max_position > 0.0) || !(sc->beta_fast >= sc->beta_slow) || !(sc->beta_slow > 0.0) ||
+            !(theta > 1.0))
+            return CFATTN_ERR_ARG;
+        // The pair, as a real number, that turns so many times in the trained positions.
+        auto pair = [&](double turns) {
+            return dim * std::log(sc->original_max_position / (turns * 2.0 * 3.14159265358979323846)) /
+                   (2.0 * std::log(theta));
+        };
+        first = std::max(std::floor(pair(sc->beta_fast)), 0.0);
+        last = std::min(std::ceil(pair(sc->beta_slow)), dim - 1.0);
+        size = 0.1 * std::log(sc->factor) + 1.0;
+    }
+    if (sc->attention_factor > 0.0) size = sc->attention_factor;
+    const cfattn_llama3_scaling l3 = {sc->factor, sc->low_freq_factor, sc->high_freq_factor,
+                                      sc->original_max_position};
+    for (size_t i = 0; i < half; i++) {
+        double inv_freq = std::pow(theta, -(2.0 * (double)i) / dim);
+        if (sc->kind == CFATTN_ROPE_LINEAR) inv_freq /= sc->factor;
+        if (sc->kind == CFATTN_ROPE_LLAMA3) inv_freq = cfattn_llama3_scale(&l3, inv_freq);
+        if (sc->kind == CFATTN_ROPE_YARN) {
+            const double slow =
+                std::min(std::max(((double)i - first) / (last > first ? last - first : 1e-3), 0.0), 1.0);
+            inv_freq = inv_freq / sc->factor * slow + inv_freq * (1.0 - slow);
+        }
+        for (size_t pos = 0; pos < max_pos; pos++) {
+            const double angle = (double)pos * inv_freq;
+            cos_out[pos * half + i] = (float)(std::cos(angle) * size);
+            sin_out[pos * half + i] = (float)(std::sin(angle) * size);
+        }
+    }
+    return CFATTN_OK;
+}
+
 int cfattn_f32_to_bf16(cfattn_ctx* c, const float* src, uint16_t* dst, size_t n, void* stream) {
     if (!c) return CFATTN_ERR_ARG;
     if (n == 0) return CFATTN_OK;

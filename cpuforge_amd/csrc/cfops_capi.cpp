@@ -2,7 +2,7 @@
 //
 // Host-side plumbing only: argument checks, scratch from the context's pool
 // and dispatch to the gfx950 kernels of gemm_f32.hip, lora.hip, layer_ops.hip,
-// head_logp.hip, seq_loss.hip and adamw8.hip.  There is no CPU compute path.
+// layer_norm.hip, rotary.hip, head_logp.hip, seq_loss.hip and adamw8.hip.  There is no CPU compute path.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -280,6 +280,89 @@ int cfops_rmsnorm_grad(cfattn_ctx* c, const float* dy, const float* x, const flo
     }
     CF_HIP(c, cfattn::launch_rmsnorm_bwd(dy, x, w, rstd, dx, dw, partial, rows, dim, acc != 0, to_stream(stream)),
            "rmsnorm backward launch");
+    return CFATTN_OK;
+}
+
+static int check_layernorm(cfattn_ctx* c, int dtype, size_t rows, size_t dim) {
+    if (dtype != CFATTN_F32 && dtype != CFATTN_BF16) return fail(c, CFATTN_ERR_ARG, "unknown dtype %d", dtype);
+    // (Columns are numbered beside up to 16 KiB of others.)
+    if (rows > (size_t)INT_MAX || dim > (size_t)INT_MAX - 65536)
+        return fail(c, CFATTN_ERR_UNSUPPORTED, "rows=%zu or dim=%zu too large", rows, dim);
+    return CFATTN_OK;
+}
+
+int cfops_layernorm_forward(cfattn_ctx* c, int dtype, const void* x, const float* w, const float* b, void* y,
+                            float* mean, float* rstd, size_t rows, size_t dim, float eps, void* stream) {
+    CF_LOCK(c, stream);
+    CF_TRY(check_layernorm(c, dtype, rows, dim));
+    if (rows == 0 || dim == 0) return CFATTN_OK;
+    if (!x || !w || !y || !mean || !rstd) return fail(c, CFATTN_ERR_ARG, "null buffer");
+    CF_HIP(c, cfattn::launch_layernorm_fwd(dtype == CFATTN_BF16, x, w, b, y, mean, rstd, rows, dim, eps,
+                                           to_stream(stream)),
+           "layer norm launch");
+    return CFATTN_OK;
+}
+
+int cfops_layernorm_backward(cfattn_ctx* c, int dtype, const void* dy, const void* x, const float* w,
+                             const float* mean, const float* rstd, void* dx, float* dw, float* db, size_t rows,
+                             size_t dim, int acc, void* stream) {
+    CF_LOCK(c, stream);
+    CF_TRY(check_layernorm(c, dtype, rows, dim));
+    if (rows == 0 && !acc) {
+        CF_TRY(zero_grad(c, dw, dim, to_stream(stream)));
+        return zero_grad(c, db, dim, to_stream(stream));
+    }
+    if (rows == 0 || dim == 0) return CFATTN_OK;
+    if (!dy || !x || !w || !mean || !rstd || !dx) return fail(c, CFATTN_ERR_ARG, "null buffer");
+    float* partial = nullptr;
+    if (dw || db)
+        CF_TRY(take(c, cfattn_ctx::OPS_PARTIAL, cfattn::layernorm_partial_floats(rows, dim) * sizeof(float), partial));
+    CF_HIP(c, cfattn::launch_layernorm_bwd(dtype == CFATTN_BF16, dy, x, w, mean, rstd, dx, dw, db, partial, rows, dim,
+                                           acc != 0, to_stream(stream)),
+           "layer norm backward launch");
+    return CFATTN_OK;
+}
+
+int cfops_rotary(cfattn_ctx* c, const cfops_rotary_tensor* tensors, size_t n, int x_dtype, int y_dtype, size_t batch,
+                 size_t seq, size_t head_dim, size_t half, const float* cos, const float* sin, size_t max_pos,
+                 const int64_t* positions, size_t pos0, int interleaved, int inverse, void* stream) {
+    static_assert(CFOPS_ROTARY_MAX == cfattn::kRotaryTensors, "the tensors of a launch");
+    CF_LOCK(c, stream);
+    for (int dtype : {x_dtype, y_dtype})
+        if (dtype != CFATTN_F32 && dtype != CFATTN_BF16) return fail(c, CFATTN_ERR_ARG, "unknown dtype %d", dtype);
+    if (n > CFOPS_ROTARY_MAX) return fail(c, CFATTN_ERR_ARG, "%zu tensors, at most %d", n, CFOPS_ROTARY_MAX);
+    if (n && !tensors) return fail(c, CFATTN_ERR_ARG, "null array");
+    if (half == 0 || half > head_dim / 2)
+        return fail(c, CFATTN_ERR_SHAPE, "%zu pairs of a head of %zu values", half, head_dim);
+    if (!positions && (max_pos < seq || pos0 > max_pos - seq))
+        return fail(c, CFATTN_ERR_SHAPE, "positions %zu..%zu exceed max_pos %zu", pos0, pos0 + seq, max_pos);
+    if (!fits_int(batch) || !fits_int(seq)) return fail(c, CFATTN_ERR_UNSUPPORTED, "batch=%zu, seq=%zu", batch, seq);
+    cfattn::RotaryArgs g{};
+    size_t heads = 0;
+    for (size_t i = 0; i < n; i++) {
+        const cfops_rotary_tensor& t = tensors[i];
+        if (t.heads > 65536) return fail(c, CFATTN_ERR_UNSUPPORTED, "heads=%zu above 65536", t.heads);
+        if (t.heads == 0) continue;
+        cfattn::RotaryTensor& r = g.t[g.count++];
+        r.x = t.x, r.y = t.y, r.head0 = (int)heads;
+        std::copy(t.x_stride, t.x_stride + 3, r.xs);
+        std::copy(t.y_stride, t.y_stride + 3, r.ys);
+        const bool same = std::equal(t.x_stride, t.x_stride + 3, t.y_stride);
+        if (batch && seq && (!t.x || !t.y)) return fail(c, CFATTN_ERR_ARG, "null buffer");
+        if (t.x == t.y && batch && seq && (x_dtype != y_dtype || !same))
+            return fail(c, CFATTN_ERR_ARG, "in place needs one type and one set of strides");
+        r.copy = t.x != t.y && 2 * half < head_dim;
+        heads += t.heads;
+    }
+    if (batch == 0 || seq == 0 || heads == 0) return CFATTN_OK;
+    if (!cos || !sin) return fail(c, CFATTN_ERR_ARG, "null table");
+    if (!cfattn::rotary_fits(batch * seq, heads, head_dim))
+        return fail(c, CFATTN_ERR_UNSUPPORTED, "%zu tokens of %zu heads of %zu values", batch * seq, heads, head_dim);
+    g.cos = cos, g.sin = sin, g.positions = positions, g.max_pos = (long)max_pos, g.pos0 = (long)pos0;
+    g.tokens = (unsigned)(batch * seq), g.seq = (unsigned)seq, g.heads = (int)heads, g.head_dim = (int)head_dim;
+    g.half = (int)half, g.interleaved = interleaved != 0, g.inverse = inverse != 0;
+    CF_HIP(c, cfattn::launch_rotary(g, x_dtype == CFATTN_BF16, y_dtype == CFATTN_BF16, to_stream(stream)),
+           "rotary launch");
     return CFATTN_OK;
 }
 

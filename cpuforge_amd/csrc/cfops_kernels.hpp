@@ -17,6 +17,42 @@ size_t rmsnorm_bwd_partial_floats(size_t rows, size_t dim);
 hipError_t launch_rmsnorm_bwd(const float* dy, const float* x, const float* w, const float* rstd, float* dx, float* dw,
                               float* partial, size_t rows, size_t dim, int acc, hipStream_t st);
 
+// Layer norm (layer_norm.hip); x, y, dy and dx are f32 or bf16, b may be null.  Forward
+// overwrites y, mean and rstd.  Backward adds to (acc) or overwrites dx and, where
+// non-null, dw and db, with `partial` scratch of layernorm_partial_floats(rows, dim)
+// floats for those.  rows and dim are positive, dim below 2^31.
+hipError_t launch_layernorm_fwd(bool bf16, const void* x, const float* w, const float* b, void* y, float* mean,
+                                float* rstd, size_t rows, size_t dim, float eps, hipStream_t st);
+size_t layernorm_partial_floats(size_t rows, size_t dim);
+hipError_t launch_layernorm_bwd(bool bf16, const void* dy, const void* x, const float* w, const float* mean,
+                                const float* rstd, void* dx, float* dw, float* db, float* partial, size_t rows,
+                                size_t dim, int acc, hipStream_t st);
+
+// Rotary positions of up to kRotaryTensors tensors (rotary.hip).  Strides are in values, of
+// sequences, tokens and heads; rotary_fits says whether a launch takes the sizes.
+constexpr int kRotaryTensors = 4;
+struct RotaryTensor {
+    const void* x;
+    void* y;
+    long xs[3], ys[3];
+    int head0;  // heads of the tensors before
+    int copy;   // whether the values behind the turned ones are written
+};
+struct RotaryArgs {
+    RotaryTensor t[kRotaryTensors];
+    const float *cos, *sin;    // [max_pos][half]
+    const int64_t* positions;  // of every token, or null: pos0 + its place in its sequence
+    long max_pos, pos0;
+    unsigned tokens, seq;
+    int count, heads, head_dim, half, interleaved, inverse;
+    // set by launch_rotary: pieces of a head that are turned, and all; of a token; to a
+    // workgroup
+    int turned, pieces;
+    unsigned per_token, per_token_rcp, pieces_rcp, tokens_wg, parts, part, token0;
+};
+bool rotary_fits(size_t tokens, size_t heads, size_t head_dim);
+hipError_t launch_rotary(RotaryArgs g, bool x_bf16, bool y_bf16, hipStream_t st);
+
 // SwiGLU gate (crates/core/src/ops/swiglu.rs:10-30): forward overwrites h,
 // backward adds to (acc) or overwrites dg and du.
 hipError_t launch_silu_mul_fwd(const float* g, const float* u, float* h, size_t n, hipStream_t st);

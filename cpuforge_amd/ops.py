@@ -15,7 +15,12 @@ the holder of device memory and the current HIP stream:
     adamw_update                        crates/train/src/optim.rs:9-30
       (adamw_update_multi: many tensors, optim.rs:48-61)
 
-Training on preferences and rewards has no reference counterpart:
+Layers of other decoders have no reference counterpart:
+
+    layernorm_forward / layernorm_backward
+    rotary                              q and k at given positions, either layout
+
+nor has training on preferences and rewards:
 
     lm_head_logprobs(_backward)         the targets' log-probabilities
     preference_loss, policy_loss        losses over them, with their gradients
@@ -55,6 +60,36 @@ def _f32(t: torch.Tensor, name: str, numel: int | None = None) -> int:
         raise ValueError(f"{name} must be contiguous")
     raise _lib.ShapeError(_lib.ERR_SHAPE,
                           f"assertion `left == right` failed: {name}.len() = {t.numel()}, expected {numel}")
+
+
+_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+def _on(t: torch.Tensor, name: str, ctx: Context, dtypes=(torch.float32,), numel: int | None = None) -> int:
+    """The address of a contiguous tensor of one of `dtypes` on the context's
+    device."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.get_device() == ctx.device \
+            and t.is_contiguous() and (numel is None or t.numel() == numel):
+        return t.data_ptr()
+    _check_on(t, name, ctx, dtypes)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    raise _lib.ShapeError(_lib.ERR_SHAPE,
+                          f"assertion `left == right` failed: {name}.len() = {t.numel()}, expected {numel}")
+
+
+def _check_on(t, name, ctx, dtypes) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a device tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {t.dtype}")
+    if t.get_device() != ctx.device:
+        raise ValueError(f"{name} is on device {t.get_device()}, the context on device {ctx.device}")
+
+
+def _stream_of(ctx: Context) -> int:
+    """The current stream of the context's device, whichever device is current."""
+    return torch._C._cuda_getCurrentRawStream(ctx.device)
 
 
 def _opt(t, name, numel=None):
@@ -112,6 +147,77 @@ def rmsnorm_backward(dy, x, w, rstd, dx, dw, rows, dim, ctx: Context | None = No
     ctx = ctx or default_context()
     _call(ctx, "cfops_rmsnorm_grad", _f32(dy, "dy", rows * dim), _f32(x, "x", rows * dim), _f32(w, "w", dim),
           _f32(rstd, "rstd", rows), _f32(dx, "dx", rows * dim), _opt(dw, "dw", dim), rows, dim, int(acc), _stream())
+
+
+# ------------------------------------------------------------ layer norm
+def layernorm_forward(x, w, b, y, mean, rstd, rows, dim, eps, ctx: Context | None = None):
+    """y = (x - mean) rstd w + b per row of `dim` (b None: no bias), mean and
+    rstd = 1 / sqrt(var + eps): overwrites y [rows, dim], mean and rstd [rows].
+    x and y are float32 or bfloat16, the others float32."""
+    ctx = ctx or default_context()
+    n = rows * dim
+    _call(ctx, "cfops_layernorm_forward", _code(x), _on(x, "x", ctx, _CODES, n), _on(w, "w", ctx, numel=dim),
+          None if b is None else _on(b, "b", ctx, numel=dim), _on(y, "y", ctx, (x.dtype,), n),
+          _on(mean, "mean", ctx, numel=rows), _on(rstd, "rstd", ctx, numel=rows), rows, dim, float(eps),
+          _stream_of(ctx))
+
+
+def layernorm_backward(dy, x, w, mean, rstd, dx, dw, db, rows, dim, ctx: Context | None = None, acc: bool = True):
+    """Accumulates into dx (of x's type, as dy), dw and db (None: frozen), or
+    overwrites them with acc=False."""
+    ctx = ctx or default_context()
+    n = rows * dim
+    _call(ctx, "cfops_layernorm_backward", _code(x), _on(dy, "dy", ctx, (x.dtype,), n), _on(x, "x", ctx, _CODES, n),
+          _on(w, "w", ctx, numel=dim), _on(mean, "mean", ctx, numel=rows), _on(rstd, "rstd", ctx, numel=rows),
+          _on(dx, "dx", ctx, (x.dtype,), n), None if dw is None else _on(dw, "dw", ctx, numel=dim),
+          None if db is None else _on(db, "db", ctx, numel=dim), rows, dim, int(acc), _stream_of(ctx))
+
+
+def _code(t) -> int:
+    """(A type that the argument checks refuse gets any.)"""
+    return _CODES.get(getattr(t, "dtype", None), _lib.F32)
+
+
+# ------------------------------------------------------ rotary positions
+def rotary(xs, ys, cos, sin, positions=None, *, pos0: int = 0, interleaved: bool = False, inverse: bool = False,
+           ctx: Context | None = None):
+    """Turns tensors xs of heads [B, S, H, D] (one, or up to 4 of the same B, S and
+    D, as q and k) into ys (the same shapes; a y may be its x, else they share no
+    memory): pair i of a head's first 2 * cos.shape[1] values by cos[p, i] and
+    sin[p, i] of the token's position p, (a, b) -> (a c - b s, b c + a s) (inverse:
+    s negated, the gradient's way); the values behind them are copied.  The pairs
+    are (i, i + half), as in the fused prologue, or (2 i, 2 i + 1) with
+    `interleaved`.  positions [B, S] (int64) or pos0, pos0 + 1, ..; a position
+    that the tables [max_pos, half] do not hold turns the values to NaN.  xs and ys
+    are float32 or bfloat16 with any strides whose last one is 1."""
+    ctx = ctx or default_context()
+    if isinstance(xs, torch.Tensor):
+        xs, ys = (xs,), (ys,)
+    if len(xs) != len(ys) or not 1 <= len(xs) <= _lib.ROTARY_MAX:
+        raise ValueError(f"{len(xs)} xs and {len(ys)} ys: as many of either, and 1 to {_lib.ROTARY_MAX}")
+    table = (_lib.RotaryTensorC * len(xs))()
+    shape = tuple(xs[0].shape)
+    for c, x, y in zip(table, xs, ys):
+        for t, name, of in ((x, "x", xs[0]), (y, "y", ys[0])):
+            _check_on(t, name, ctx, _CODES if t is of else (of.dtype,))
+            if t.dim() != 4 or t.shape != x.shape or (*t.shape[:2], t.shape[3]) != (*shape[:2], shape[3]):
+                raise _lib.ShapeError(_lib.ERR_SHAPE, f"{name} has shape {tuple(t.shape)} beside {shape} "
+                                                      "([B, S, H, D], the same but for H)")
+            if t.shape[3] > 1 and t.stride(3) != 1:
+                raise ValueError(f"{name}'s last stride must be 1")
+        if any(n > 1 and st == 0 for n, st in zip(y.shape, y.stride())):
+            raise ValueError("y must not be expanded")
+        c.x, c.y, c.heads = x.data_ptr(), y.data_ptr(), x.shape[2]
+        c.x_stride[:], c.y_stride[:] = x.stride()[:3], y.stride()[:3]
+    batch, seq, _, dim = shape
+    pp = _on(cos, "cos", ctx), _on(sin, "sin", ctx, numel=cos.numel())
+    if cos.dim() != 2:
+        raise _lib.ShapeError(_lib.ERR_SHAPE, f"cos has shape {tuple(cos.shape)}, expected [max_pos, half]")
+    at = None if positions is None else _on(positions, "positions", ctx, (torch.int64,), batch * seq)
+    if pos0 < 0:
+        raise ValueError("pos0 must not be negative")
+    _call(ctx, "cfops_rotary", table, len(xs), _CODES[xs[0].dtype], _CODES[ys[0].dtype], batch, seq, dim, cos.shape[1],
+          *pp, cos.shape[0], at, int(pos0), int(interleaved), int(inverse), _stream_of(ctx))
 
 
 # --------------------------------------------------------------- SwiGLU

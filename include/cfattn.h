@@ -199,6 +199,27 @@ int cfattn_fused_bwd_grad(cfattn_ctx* ctx, cfattn_shape s, size_t batch, int dty
  * buffers.  scaling may be NULL (plain RoPE).  head_dim must be even. */
 int cfattn_rope_table(size_t head_dim, size_t max_pos, double theta, const cfattn_llama3_scaling* scaling,
                       float* cos_out, float* sin_out);
+/* No reference counterpart: the table with the frequencies of one of the scalings
+ * for contexts longer than a model was trained on (kind), each f64 until the
+ * table is rounded, and cos and sin multiplied by attention_factor (0: the kind's
+ * own, 1 except for YARN's 0.1 ln(factor) + 1):
+ *   LINEAR  inv_freq / factor
+ *   NTK     theta * factor^(head_dim / (head_dim - 2)) in theta's place
+ *   LLAMA3  cfattn_llama3_scale
+ *   YARN    of d pairs, those that turn at most beta_slow times in
+ *           original_max_position positions get inv_freq / factor, those that turn
+ *           beta_fast times or more keep theirs, a line over the pairs in between */
+enum { CFATTN_ROPE_LINEAR = 1, CFATTN_ROPE_NTK = 2, CFATTN_ROPE_LLAMA3 = 3, CFATTN_ROPE_YARN = 4 };
+typedef struct cfattn_rope_scaling {
+    int kind;
+    double factor;
+    double low_freq_factor, high_freq_factor; /* LLAMA3 */
+    double original_max_position;             /* LLAMA3, YARN */
+    double beta_fast, beta_slow;              /* YARN */
+    double attention_factor;
+} cfattn_rope_scaling;
+int cfattn_rope_table_scaled(size_t head_dim, size_t max_pos, double theta, const cfattn_rope_scaling* scaling,
+                             float* cos_out, float* sin_out);
 /* Llama3Scaling::apply (core/src/ops/rope.rs:26-38). */
 double cfattn_llama3_scale(const cfattn_llama3_scaling* scaling, double inv_freq);
 /* Device f32 -> bf16 (round to nearest even) conversion on `stream`. */

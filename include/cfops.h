@@ -61,6 +61,45 @@ int cfops_rmsnorm_backward(cfattn_ctx* ctx, const float* dy, const float* x, con
 int cfops_rmsnorm_grad(cfattn_ctx* ctx, const float* dy, const float* x, const float* w, const float* rstd, float* dx,
                        float* dw, size_t rows, size_t dim, int acc, void* stream);
 
+/* ---- other decoders' layers ------------------------------------------------
+ * No reference counterpart (its layers are RMSNorm and half-layout RoPE). */
+
+/* Layer norm over rows of `dim`: mean = sum x / dim, rstd = 1 / sqrt(sum (x - mean)^2 /
+ * dim + eps), y = (x - mean) rstd w + b (b NULL: no bias).  x and y [rows, dim] are
+ * of `dtype` (CFATTN_F32 or CFATTN_BF16); w, b [dim], mean and rstd [rows] are f32;
+ * y, mean and rstd are overwritten.  Sums and statistics are f32; y is rounded
+ * once.  What is not finite in a row stays with that row. */
+int cfops_layernorm_forward(cfattn_ctx* ctx, int dtype, const void* x, const float* w, const float* b, void* y,
+                            float* mean, float* rstd, size_t rows, size_t dim, float eps, void* stream);
+/* From dy: dx (of `dtype`, as dy and x) and, where non-null, dw = sum dy (x - mean)
+ * rstd and db = sum dy over the rows (f32), each added to what is there (acc
+ * == 0: overwritten).  Rows are summed in an order that their number alone decides. */
+int cfops_layernorm_backward(cfattn_ctx* ctx, int dtype, const void* dy, const void* x, const float* w,
+                             const float* mean, const float* rstd, void* dx, float* dw, float* db, size_t rows,
+                             size_t dim, int acc, void* stream);
+
+/* Rotary positions of tensors of heads [batch, seq, heads, head_dim], with any strides
+ * (in values; a head's values lie side by side): of a head's first 2 `half` values pair
+ * i is turned by the angle of position p, (a, b) -> (a c - b s, b c + a s) with c =
+ * cos[p][i] and s = sin[p][i] ([max_pos][half], f32; inverse != 0: s negated, the
+ * gradient's way).  The pairs are (i, i + half), as cfattn_prologue_fwd's, or
+ * (interleaved != 0) (2 i, 2 i + 1); the values behind them are copied.  A token's
+ * position is positions[batch][seq] (int64), or, with positions NULL, pos0 plus its
+ * place in its sequence; one outside [0, max_pos) turns the values to NaN.  All x are of
+ * x_dtype and all y of y_dtype (rounded once).  A y may be its own x (same pointer,
+ * strides and type); it shares no memory with any x otherwise, nor with another y. */
+typedef struct cfops_rotary_tensor {
+    const void* x;
+    void* y;
+    size_t heads;
+    int64_t x_stride[3]; /* of sequences, tokens and heads */
+    int64_t y_stride[3];
+} cfops_rotary_tensor;
+enum { CFOPS_ROTARY_MAX = 4 };
+int cfops_rotary(cfattn_ctx* ctx, const cfops_rotary_tensor* tensors, size_t n, int x_dtype, int y_dtype, size_t batch,
+                 size_t seq, size_t head_dim, size_t half, const float* cos, const float* sin, size_t max_pos,
+                 const int64_t* positions, size_t pos0, int interleaved, int inverse, void* stream);
+
 /* silu_mul_forward / _backward (swiglu.rs:10-30): h = silu(g) * u
  * (overwritten); the backward accumulates into dg and du. */
 int cfops_silu_mul_forward(cfattn_ctx* ctx, const float* g, const float* u, float* h, size_t n, void* stream);
