@@ -33,21 +33,27 @@ struct Pack<bf16_bits> {
     typedef uint16_t vec __attribute__((ext_vector_type(8), aligned(2)));
 };
 
-// Values [0, N) of p, those at or past n zero (and not read).
+// Values [0, N) of p as they lie in memory, those at or past n zero (and not read).
+template <typename T>
+__device__ __forceinline__ typename Pack<T>::vec load_raw(const T* p, int n) {
+    typedef typename Pack<T>::vec Vec;
+    if (n >= Pack<T>::N) return *reinterpret_cast<const Vec*>(p);
+    Vec v = {};
+#pragma unroll
+    for (int i = 0; i < Pack<T>::N; i++)
+        if (i < n) v[i] = p[i];
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ float value(const typename Pack<T>::vec& v, int i) {
+    const T e = v[i];
+    return to_f32<T>(e);
+}
 template <typename T>
 __device__ __forceinline__ void load_chunk(float (&x)[Pack<T>::N], const T* p, int n) {
-    constexpr int N = Pack<T>::N;
-    if (n >= N) {
-        const typename Pack<T>::vec v = *reinterpret_cast<const typename Pack<T>::vec*>(p);
+    const typename Pack<T>::vec v = load_raw<T>(p, n);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const T e = v[i];
-            x[i] = to_f32<T>(e);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = i < n ? to_f32<T>(p[i]) : 0.0f;
-    }
+    for (int i = 0; i < Pack<T>::N; i++) x[i] = value<T>(v, i);
 }
 template <typename T>
 __device__ __forceinline__ void store_chunk(T* p, const float (&x)[Pack<T>::N], int n) {
@@ -111,48 +117,58 @@ __device__ __forceinline__ void row_sums(float (&x)[K], float (*red)[K], int wav
     }
 }
 
-// 4 rows to a workgroup with NW == 1, else one.
-template <typename T, int NW, int V>
+// R rows to NW waves (4 such to a workgroup with NW == 1, else one), which share the
+// weights' loads and the barriers.
+template <typename T, int NW, int V, int R>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void layernorm_fwd_kernel(
     const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b, T* __restrict__ y,
     float* __restrict__ mean, float* __restrict__ rstd, long rows, int dim, float eps) {
-    constexpr int N = Pack<T>::N;
-    __shared__ float red[2][NW][1];
+    constexpr int N = Pack<T>::N, STEP = 64 * NW * N, ROWS = R * (NW == 1 ? 4 : 1);
+    __shared__ float red[2][NW][R];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int c0 = (NW == 1 ? lane : (int)threadIdx.x) * N;
     // (With NW > 1 all waves of a workgroup have the same rows, and pass its barriers together.)
-    constexpr int ROWS = NW == 1 ? 4 : 1;
-    for (long r = (long)blockIdx.x * ROWS + (NW == 1 ? wave : 0); r < rows; r += (long)gridDim.x * ROWS) {
-        const T* xr = x + r * dim;
-        float v[V][N];
+    for (long r0 = (long)blockIdx.x * ROWS + (NW == 1 ? wave * R : 0); r0 < rows; r0 += (long)gridDim.x * ROWS) {
+        typename Pack<T>::vec v[R][V];
 #pragma unroll
-        for (int i = 0; i < V; i++) load_chunk<T>(v[i], xr + c0 + i * 64 * NW * N, dim - c0 - i * 64 * NW * N);
-        float s[1] = {0.0f};
+        for (int k = 0; k < R; k++)
 #pragma unroll
-        for (int i = 0; i < V; i++)
+            for (int i = 0; i < V; i++)
+                v[k][i] = load_raw<T>(x + (r0 + k) * dim + c0 + i * STEP, r0 + k < rows ? dim - c0 - i * STEP : 0);
+        float mu[R], rs[R];
 #pragma unroll
-            for (int k = 0; k < N; k++) s[0] += v[i][k];
-        row_sums<NW, 1>(s, red[0], wave);
-        const float mu = s[0] / (float)dim;
-        float q[1] = {0.0f};
+        for (int k = 0; k < R; k++) {
+            mu[k] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; i++)
+            for (int i = 0; i < V; i++)
 #pragma unroll
-            for (int k = 0; k < N; k++) {
-                const float d = c0 + i * 64 * NW * N + k < dim ? v[i][k] - mu : 0.0f;
-                v[i][k] = d;
-                q[0] = fmaf(d, d, q[0]);
-            }
-        row_sums<NW, 1>(q, red[1], wave);
-        const float rs = 1.0f / sqrtf(q[0] / (float)dim + eps);
-        if (c0 == 0) {
-            mean[r] = mu;
-            rstd[r] = rs;
+                for (int e = 0; e < N; e++) mu[k] += value<T>(v[k][i], e);
         }
-        T* yr = y + r * dim;
+        row_sums<NW, R>(mu, red[0], wave);
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            mu[k] /= (float)dim;
+            rs[k] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; i++)
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const float d = c0 + i * STEP + e < dim ? value<T>(v[k][i], e) - mu[k] : 0.0f;
+                    rs[k] = fmaf(d, d, rs[k]);
+                }
+        }
+        row_sums<NW, R>(rs, red[1], wave);
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            rs[k] = 1.0f / sqrtf(rs[k] / (float)dim + eps);
+            if (c0 == 0 && r0 + k < rows) {
+                mean[r0 + k] = mu[k];
+                rstd[r0 + k] = rs[k];
+            }
+        }
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const int c = c0 + i * 64 * NW * N;
+            const int c = c0 + i * STEP;
             if (c >= dim) break;
             float ww[N], bb[N];
             load_floats<N>(ww, w + c, dim - c);
@@ -160,72 +176,84 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void layernorm_fwd_kernel(
                 load_floats<N>(bb, b + c, dim - c);
             else
 #pragma unroll
-                for (int k = 0; k < N; k++) bb[k] = 0.0f;
+                for (int e = 0; e < N; e++) bb[e] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < N; k++) v[i][k] = fmaf(v[i][k] * rs, ww[k], bb[k]);
-            store_chunk<T>(yr + c, v[i], dim - c);
+            for (int k = 0; k < R; k++) {
+                float o[N];
+#pragma unroll
+                for (int e = 0; e < N; e++) o[e] = fmaf((value<T>(v[k][i], e) - mu[k]) * rs[k], ww[e], bb[e]);
+                if (r0 + k < rows) store_chunk<T>(y + (r0 + k) * dim + c, o, dim - c);
+            }
         }
     }
 }
 
 // dx of rows g, g + G, .. to the g-th of G groups of NW waves over the grid, whose sums of
-// dy xh and dy over their rows stay in registers; a workgroup of 8 waves adds up its
-// groups' in LDS and writes them to partial[block][2][dim].
+// dy xh and dy over their rows stay in registers; the next row's values are on their way
+// while one is formed.  A workgroup of 8 waves adds up its groups' sums in LDS (dw's, then
+// db's) and writes them to partial[block][2][dim].
 constexpr int kBwdThreads = 512;
 template <typename T, int NW, int V>
-__global__ __launch_bounds__(kBwdThreads) void layernorm_bwd_kernel(
+__global__ __launch_bounds__(kBwdThreads, V == 1 ? 4 : 2) void layernorm_bwd_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ mean,
     const float* __restrict__ rstd, T* dx, float* __restrict__ partial, int want_b, long rows, int dim, int acc) {
-    constexpr int N = Pack<T>::N, GROUPS = 8 / NW;
+    constexpr int N = Pack<T>::N, GROUPS = 8 / NW, STEP = 64 * NW * N;
+    typedef typename Pack<T>::vec Vec;
     __shared__ float red[2][GROUPS][NW][2];
-    extern __shared__ float sums[];  // [dim]
+    extern __shared__ float sums[];  // [GROUPS][dim]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = wave / NW;
     const int c0 = (lane + 64 * (wave % NW)) * N;
     float aw[V][N], ab[V][N], ww[V][N];
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        load_floats<N>(ww[i], w + c0 + i * 64 * NW * N, dim - c0 - i * 64 * NW * N);
+        load_floats<N>(ww[i], w + c0 + i * STEP, dim - c0 - i * STEP);
 #pragma unroll
         for (int k = 0; k < N; k++) aw[i][k] = ab[i][k] = 0.0f;
     }
     const float inv_dim = 1.0f / (float)dim;
-    int turn = 0;
-    // (The groups of a workgroup pass the barriers of row_sums together.)
-    for (long r0 = (long)blockIdx.x * GROUPS; r0 < rows; r0 += (long)gridDim.x * GROUPS, turn ^= 1) {
-        const long r = r0 + group;
+    const long stride = (long)gridDim.x * GROUPS;
+    Vec xn[V], gn[V];
+    float mn = 0.0f, rn = 0.0f;
+    auto load = [&](long r) {
         const bool live = r < rows;
-        const int n = live ? dim : 0;
-        const T *xr = x + (live ? r : 0) * dim, *gr = dy + (live ? r : 0) * dim;
-        float xv[V][N], gv[V][N];
+        const long at = live ? r : 0;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const int c = c0 + i * 64 * NW * N;
-            load_chunk<T>(xv[i], xr + c, n - c);
-            load_chunk<T>(gv[i], gr + c, n - c);
+            const int n = live ? dim - c0 - i * STEP : 0;
+            xn[i] = load_raw<T>(x + at * dim + c0 + i * STEP, n);
+            gn[i] = load_raw<T>(dy + at * dim + c0 + i * STEP, n);
         }
-        const float mu = live ? mean[r] : 0.0f, rs = live ? rstd[r] : 0.0f;
+        mn = live ? mean[at] : 0.0f, rn = live ? rstd[at] : 0.0f;
+    };
+    int turn = 0;
+    load((long)blockIdx.x * GROUPS + group);
+    // (The groups of a workgroup pass the barriers of row_sums together.)
+    for (long r0 = (long)blockIdx.x * GROUPS; r0 < rows; r0 += stride, turn ^= 1) {
+        const long r = r0 + group;
+        Vec xv[V], gv[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) xv[i] = xn[i], gv[i] = gn[i];
+        const float mu = mn, rs = rn;
+        if (r0 + stride < rows) load(r + stride);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < V; i++)
 #pragma unroll
             for (int k = 0; k < N; k++) {
                 // (Past the row's end dy is 0, and so is what x's deviation meets.)
-                const float h = (xv[i][k] - mu) * rs, g = gv[i][k];
+                const float h = (value<T>(xv[i], k) - mu) * rs, g = value<T>(gv[i], k);
                 aw[i][k] = fmaf(g, h, aw[i][k]);
                 ab[i][k] += g;
-                const float gw = g * ww[i][k];
-                s[0] += gw;
-                s[1] = fmaf(gw, h, s[1]);
-                xv[i][k] = h;
-                gv[i][k] = gw;
+                s[0] = fmaf(g, ww[i][k], s[0]);
+                s[1] = fmaf(g * ww[i][k], h, s[1]);
             }
         row_sums<NW, 2>(s, red[turn][group], wave % NW);
         const float m0 = s[0] * inv_dim, m1 = s[1] * inv_dim;
-        if (!live) continue;
+        if (r >= rows) continue;
         T* dr = dx + r * dim;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const int c = c0 + i * 64 * NW * N;
+            const int c = c0 + i * STEP;
             if (c >= dim) break;
             float o[N];
             if (acc)
@@ -234,29 +262,39 @@ __global__ __launch_bounds__(kBwdThreads) void layernorm_bwd_kernel(
 #pragma unroll
                 for (int k = 0; k < N; k++) o[k] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < N; k++) o[k] += rs * (gv[i][k] - m0 - xv[i][k] * m1);
+            for (int k = 0; k < N; k++) {
+                const float h = (value<T>(xv[i], k) - mu) * rs;
+                o[k] += rs * (fmaf(value<T>(gv[i], k), ww[i][k], -m0) - h * m1);
+            }
             store_chunk<T>(dr + c, o, dim - c);
         }
     }
     if (!partial) return;
     float* out = partial + (long)blockIdx.x * 2 * dim;
-    for (int which = 0; which < (want_b ? 2 : 1); which++) {
-        for (int g = 0; g < GROUPS; g++) {
-            if (group == g) {
 #pragma unroll
-                for (int i = 0; i < V; i++)
+    for (int which = 0; which < 2; which++) {
+        if (which && !want_b) return;
+        if (GROUPS > 1 && which) __syncthreads();
 #pragma unroll
-                    for (int k = 0; k < N; k++) {
-                        const int c = c0 + i * 64 * NW * N + k;
-                        if (c >= dim) continue;
-                        const float a = (which ? ab[i][k] : aw[i][k]) + (g ? sums[c] : 0.0f);
-                        if (g + 1 < GROUPS)
-                            sums[c] = a;
-                        else
-                            out[which * dim + c] = a;
-                    }
+        for (int i = 0; i < V; i++) {
+            const int c = c0 + i * STEP;
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                if (c + k >= dim) break;
+                if constexpr (GROUPS > 1)
+                    sums[group * dim + c + k] = which ? ab[i][k] : aw[i][k];
+                else
+                    out[which * dim + c + k] = which ? ab[i][k] : aw[i][k];
             }
-            if (GROUPS > 1) __syncthreads();
+        }
+        if constexpr (GROUPS > 1) {
+            __syncthreads();
+            for (int c = threadIdx.x; c < dim; c += kBwdThreads) {
+                float t = sums[c];
+#pragma unroll
+                for (int g = 1; g < GROUPS; g++) t += sums[g * dim + c];
+                out[which * dim + c] = t;
+            }
         }
     }
 }
@@ -401,62 +439,78 @@ __global__ __launch_bounds__(256) void layernorm_columns_kernel(const T* __restr
     out[c] = sw, out[dim + c] = sb;
 }
 
-// How a row lies in registers: the fewest waves whose lanes hold it in up to four chunks
-// each (eight of f32 in the widest form).  0 waves: it does not fit.
+// How a row lies in registers: waves, and chunks of a lane.  0 waves: it does not fit.
 struct Form {
     int nw, v;
 };
-template <typename T>
-Form form_of(size_t dim) {
-    const size_t chunks = (dim + Pack<T>::N - 1) / Pack<T>::N;
+// The forward: the fewest waves whose lanes hold the row in up to four chunks each.
+Form fwd_form(size_t chunks) {
     for (int nw : {1, 4, 8})
-        for (int v = 1; v <= (nw == 8 && sizeof(T) == 4 ? 8 : 4); v++)
-            if (chunks <= (size_t)64 * nw * v) return {nw, nw == 8 && v > 4 ? 8 : nw == 1 ? v : std::max(v, 2)};
+        if (chunks <= (size_t)256 * nw) return {nw, (int)((chunks + 64 * nw - 1) / (64 * nw))};
     return {0, 0};
+}
+// The backward, whose lanes hold the weight and two sums of each column too: one wave while it
+// holds the row in three chunks, then the most that have one, and up to four in eight waves.
+// (Us in one chunk of several waves and in four of one, or two of four: 8192 x 2048 bf16 20 and
+// 30, 16384 x 4096 bf16 80 and 98, 999 x 1001 f32 5.1 and 8.6; but 65536 x 576 f32, which three
+// chunks of a wave hold and four waves' not whole, 144 and 91.)
+Form bwd_form(size_t chunks) {
+    if (chunks <= 192) return {1, (int)((chunks + 63) / 64)};
+    if (chunks <= 256) return {4, 1};
+    if (chunks <= 2048) return {8, (int)((chunks + 511) / 512)};
+    return {0, 0};
+}
+template <typename T>
+size_t chunks_of(size_t dim) {
+    return (dim + Pack<T>::N - 1) / Pack<T>::N;
 }
 
 // A grid of as many workgroups, or of fewer that take several rows each (a launch has fewer
 // than 2^32 threads).
 unsigned blocks_of(size_t n) { return (unsigned)std::min<size_t>(n, (size_t)1 << 21); }
 
-// The persistent grid of the backward, and slices of rows of the wide one.
-constexpr size_t kBwdBlocks = 512, kSlices = 32;
+// The backward's persistent grid by waves of a row (half of the workgroups, and of the
+// partial sums, cost nothing where eight waves share a row: 16384 x 4096 bf16 80 us and 85; 65536
+// x 576 f32 95 and 91), and slices of rows of the wide one.
+size_t bwd_blocks(int nw) { return nw == 1 ? 512 : 256; }
+constexpr size_t kSlices = 32;
 
 template <typename T>
 hipError_t fwd(const T* x, const float* w, const float* b, T* y, float* mean, float* rstd, size_t rows, size_t dim,
                float eps, hipStream_t st) {
-    const Form f = form_of<T>(dim);
+    const Form f = fwd_form(chunks_of<T>(dim));
     if (f.nw == 0) {
         hipLaunchKernelGGL(layernorm_fwd_wide_kernel<T>, dim3(blocks_of(rows)), dim3(kWide), 0, st, x, w, b, y, mean,
                            rstd, (long)rows, (int)dim, eps);
         return hipGetLastError();
     }
-    auto go = [&](auto kernel, int nw) {
-        hipLaunchKernelGGL(kernel, dim3(blocks_of(nw == 1 ? (rows + 3) / 4 : rows)), dim3(nw == 1 ? 256 : 64 * nw), 0,
-                           st, x, w, b, y, mean, rstd, (long)rows, (int)dim, eps);
+    auto go = [&](auto kernel, size_t per) {
+        hipLaunchKernelGGL(kernel, dim3(blocks_of((rows + per - 1) / per)), dim3(f.nw == 1 ? 256 : 64 * f.nw), 0, st, x,
+                           w, b, y, mean, rstd, (long)rows, (int)dim, eps);
         return hipGetLastError();
     };
     if (f.nw == 1) {
-        if (f.v == 1) return go(layernorm_fwd_kernel<T, 1, 1>, 1);
-        if (f.v == 2) return go(layernorm_fwd_kernel<T, 1, 2>, 1);
-        if (f.v == 3) return go(layernorm_fwd_kernel<T, 1, 3>, 1);
-        return go(layernorm_fwd_kernel<T, 1, 4>, 1);
+        if (f.v == 1) return go(layernorm_fwd_kernel<T, 1, 1, 1>, 4);
+        if (f.v == 2) return go(layernorm_fwd_kernel<T, 1, 2, 1>, 4);
+        if (f.v == 3) return go(layernorm_fwd_kernel<T, 1, 3, 1>, 4);
+        return go(layernorm_fwd_kernel<T, 1, 4, 1>, 4);
     }
+    // Two rows at a time where that leaves every CU eight workgroups (16384 x 4096 bf16 54 us and
+    // 63; a wave that has a row alone gains nothing, 4096 x 2048 bf16 9.6 and 9.3).
+    const bool two = rows >= 4096;
     if (f.nw == 4) {
-        if (f.v == 2) return go(layernorm_fwd_kernel<T, 4, 2>, 4);
-        if (f.v == 3) return go(layernorm_fwd_kernel<T, 4, 3>, 4);
-        return go(layernorm_fwd_kernel<T, 4, 4>, 4);
+        if (f.v == 2) return two ? go(layernorm_fwd_kernel<T, 4, 2, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 2, 1>, 1);
+        if (f.v == 3) return two ? go(layernorm_fwd_kernel<T, 4, 3, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 3, 1>, 1);
+        return two ? go(layernorm_fwd_kernel<T, 4, 4, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 4, 1>, 1);
     }
-    if constexpr (sizeof(T) == 4)
-        if (f.v == 8) return go(layernorm_fwd_kernel<T, 8, 8>, 8);
-    if (f.v == 3) return go(layernorm_fwd_kernel<T, 8, 3>, 8);
-    return go(layernorm_fwd_kernel<T, 8, 4>, 8);
+    if (f.v == 3) return two ? go(layernorm_fwd_kernel<T, 8, 3, 2>, 2) : go(layernorm_fwd_kernel<T, 8, 3, 1>, 1);
+    return two ? go(layernorm_fwd_kernel<T, 8, 4, 2>, 2) : go(layernorm_fwd_kernel<T, 8, 4, 1>, 1);
 }
 
 template <typename T>
 hipError_t bwd(const T* dy, const T* x, const float* w, const float* mean, const float* rstd, T* dx, float* dw,
                float* db, float* partial, size_t rows, size_t dim, int acc, hipStream_t st) {
-    const Form f = form_of<T>(dim);
+    const Form f = bwd_form(chunks_of<T>(dim));
     const bool sums = dw || db;
     size_t parts;
     hipError_t e;
@@ -470,23 +524,24 @@ hipError_t bwd(const T* dy, const T* x, const float* w, const float* mean, const
         if ((e = hipGetLastError()) != hipSuccess) return e;
     } else {
         const size_t groups = 8 / f.nw;
-        parts = std::min(kBwdBlocks, (rows + groups - 1) / groups);
+        parts = std::min(bwd_blocks(f.nw), (rows + groups - 1) / groups);
         auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)parts), dim3(kBwdThreads),
-                               sums && groups > 1 ? dim * sizeof(float) : 0, st, dy, x, w, mean, rstd, dx,
+                               sums && groups > 1 ? groups * dim * sizeof(float) : 0, st, dy, x, w, mean, rstd, dx,
                                sums ? partial : nullptr, db != nullptr, (long)rows, (int)dim, acc);
             return hipGetLastError();
         };
-        e = f.nw == 1   ? f.v == 1   ? go(layernorm_bwd_kernel<T, 1, 1>)
-                          : f.v == 2 ? go(layernorm_bwd_kernel<T, 1, 2>)
-                          : f.v == 3 ? go(layernorm_bwd_kernel<T, 1, 3>)
-                                     : go(layernorm_bwd_kernel<T, 1, 4>)
-            : f.nw == 4 ? f.v == 2   ? go(layernorm_bwd_kernel<T, 4, 2>)
-                          : f.v == 3 ? go(layernorm_bwd_kernel<T, 4, 3>)
-                                     : go(layernorm_bwd_kernel<T, 4, 4>)
-            : f.v == 3  ? go(layernorm_bwd_kernel<T, 8, 3>)
-            : f.v == 4  ? go(layernorm_bwd_kernel<T, 8, 4>)
-                        : go(layernorm_bwd_kernel<T, 8, sizeof(T) == 4 ? 8 : 4>);
+        if (f.nw == 1)
+            e = f.v == 1   ? go(layernorm_bwd_kernel<T, 1, 1>)
+                : f.v == 2 ? go(layernorm_bwd_kernel<T, 1, 2>)
+                           : go(layernorm_bwd_kernel<T, 1, 3>);
+        else if (f.nw == 4)
+            e = go(layernorm_bwd_kernel<T, 4, 1>);
+        else
+            e = f.v == 1   ? go(layernorm_bwd_kernel<T, 8, 1>)
+                : f.v == 2 ? go(layernorm_bwd_kernel<T, 8, 2>)
+                : f.v == 3 ? go(layernorm_bwd_kernel<T, 8, 3>)
+                           : go(layernorm_bwd_kernel<T, 8, 4>);
         if (e != hipSuccess || !sums) return e;
     }
     hipLaunchKernelGGL(layernorm_reduce_kernel, dim3((unsigned)((dim + 15) / 16), 2), dim3(256), 0, st, partial, dw, db,
@@ -496,7 +551,7 @@ hipError_t bwd(const T* dy, const T* x, const float* w, const float* mean, const
 
 }  // namespace
 
-size_t layernorm_partial_floats(size_t rows, size_t dim) { return std::min(kBwdBlocks, rows) * 2 * dim; }
+size_t layernorm_partial_floats(size_t rows, size_t dim) { return std::min(bwd_blocks(1), rows) * 2 * dim; }
 
 hipError_t launch_layernorm_fwd(bool bf16, const void* x, const float* w, const float* b, void* y, float* mean,
                                 float* rstd, size_t rows, size_t dim, float eps, hipStream_t st) {
