@@ -338,13 +338,14 @@ int cfops_rotary(cfattn_ctx* c, const cfops_rotary_tensor* tensors, size_t n, in
         return fail(c, CFATTN_ERR_SHAPE, "positions %zu..%zu exceed max_pos %zu", pos0, pos0 + seq, max_pos);
     if (!fits_int(batch) || !fits_int(seq)) return fail(c, CFATTN_ERR_UNSUPPORTED, "batch=%zu, seq=%zu", batch, seq);
     cfattn::RotaryArgs g{};
-    size_t heads = 0;
     for (size_t i = 0; i < n; i++) {
         const cfops_rotary_tensor& t = tensors[i];
-        if (t.heads > 65536) return fail(c, CFATTN_ERR_UNSUPPORTED, "heads=%zu above 65536", t.heads);
         if (t.heads == 0) continue;
+        if (!fits_int(batch * seq) || !cfattn::rotary_fits(batch * seq, t.heads, head_dim))
+            return fail(c, CFATTN_ERR_UNSUPPORTED, "%zu tokens of %zu heads of %zu values", batch * seq, t.heads,
+                        head_dim);
         cfattn::RotaryTensor& r = g.t[g.count++];
-        r.x = t.x, r.y = t.y, r.head0 = (int)heads;
+        r.x = t.x, r.y = t.y, r.heads = (int)t.heads;
         std::copy(t.x_stride, t.x_stride + 3, r.xs);
         std::copy(t.y_stride, t.y_stride + 3, r.ys);
         const bool same = std::equal(t.x_stride, t.x_stride + 3, t.y_stride);
@@ -352,14 +353,11 @@ int cfops_rotary(cfattn_ctx* c, const cfops_rotary_tensor* tensors, size_t n, in
         if (t.x == t.y && batch && seq && (x_dtype != y_dtype || !same))
             return fail(c, CFATTN_ERR_ARG, "in place needs one type and one set of strides");
         r.copy = t.x != t.y && 2 * half < head_dim;
-        heads += t.heads;
     }
-    if (batch == 0 || seq == 0 || heads == 0) return CFATTN_OK;
+    if (batch == 0 || seq == 0 || g.count == 0) return CFATTN_OK;
     if (!cos || !sin) return fail(c, CFATTN_ERR_ARG, "null table");
-    if (!cfattn::rotary_fits(batch * seq, heads, head_dim))
-        return fail(c, CFATTN_ERR_UNSUPPORTED, "%zu tokens of %zu heads of %zu values", batch * seq, heads, head_dim);
     g.cos = cos, g.sin = sin, g.positions = positions, g.max_pos = (long)max_pos, g.pos0 = (long)pos0;
-    g.tokens = (unsigned)(batch * seq), g.seq = (unsigned)seq, g.heads = (int)heads, g.head_dim = (int)head_dim;
+    g.tokens = (unsigned)(batch * seq), g.seq = (unsigned)seq, g.head_dim = (int)head_dim;
     g.half = (int)half, g.interleaved = interleaved != 0, g.inverse = inverse != 0;
     CF_HIP(c, cfattn::launch_rotary(g, x_dtype == CFATTN_BF16, y_dtype == CFATTN_BF16, to_stream(stream)),
            "rotary launch");

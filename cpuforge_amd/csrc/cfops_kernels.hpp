@@ -35,23 +35,24 @@ struct RotaryTensor {
     const void* x;
     void* y;
     long xs[3], ys[3];
-    int head0;  // heads of the tensors before
+    int heads;  // not 0
     int copy;   // whether the values behind the turned ones are written
+    // set by launch_rotary: pieces of a head and of a token, tokens to a workgroup or
+    // workgroups to a token and its pieces of each, the first workgroup
+    int pieces;
+    unsigned per_token, per_token_rcp, pieces_rcp, tokens_wg, parts, part, block0;
 };
 struct RotaryArgs {
     RotaryTensor t[kRotaryTensors];
     const float *cos, *sin;    // [max_pos][half]
     const int64_t* positions;  // of every token, or null: pos0 + its place in its sequence
     long max_pos, pos0;
-    unsigned tokens, seq;
-    int count, heads, head_dim, half, interleaved, inverse;
-    // set by launch_rotary: pieces of a head that are turned, and all; of a token; to a
-    // workgroup
-    int turned, pieces;
-    unsigned per_token, per_token_rcp, pieces_rcp, tokens_wg, parts, part, token0;
+    unsigned tokens, seq, token0;  // token0 set by launch_rotary, as
+    int turned;                    // pieces of a head that are turned
+    int count, head_dim, half, interleaved, inverse;
 };
 bool rotary_fits(size_t tokens, size_t heads, size_t head_dim);
-hipError_t launch_rotary(RotaryArgs g, bool x_bf16, bool y_bf16, hipStream_t st);
+hipError_t launch_rotary(const RotaryArgs& g, bool x_bf16, bool y_bf16, hipStream_t st);
 
 // SwiGLU gate (crates/core/src/ops/swiglu.rs:10-30): forward overwrites h,
 // backward adds to (acc) or overwrites dg and du.
