@@ -127,6 +127,9 @@ SIGNATURES = {
     "cfops_lm_head_logprobs_keep_bytes": (_sz, [_sz] * 3),
     "cfops_lm_head_logprobs": (C.c_int, [_vp] * 4 + [_sz] * 3 + [_vp] * 4 + [_sz, _vp]),
     "cfops_lm_head_logprobs_backward": (C.c_int, [_vp] * 6 + [_sz] * 3 + [_vp] * 2 + [C.c_int, _vp, _sz, _vp]),
+    "cfops_lm_head_distill_keep_bytes": (_sz, [_sz] * 4),
+    "cfops_lm_head_distill": (C.c_int, [_vp] * 6 + [_sz] * 4 + [C.c_double] + [_vp] * 3 + [_sz, _vp]),
+    "cfops_lm_head_distill_backward": (C.c_int, [_vp] * 7 + [_sz] * 4 + [C.c_double, _vp, _vp, C.c_int, _vp, _sz, _vp]),
     "cfops_preference_loss": (C.c_int, [_vp] * 4 + [_sz, _vp, _sz, C.c_int] + [C.c_double] * 3 + [C.c_int]
                               + [_vp] * 4),
     "cfops_policy_loss": (C.c_int, [_vp] * 6 + [_sz, _vp, _sz, C.c_int] + [C.c_double] * 3 + [C.c_int] + [_vp] * 3),

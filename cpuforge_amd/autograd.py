@@ -276,6 +276,43 @@ class LMHeadLogprobsFn(torch.autograd.Function):
         return None if dhn is None else dhn.view(ctx.shape), dhead, None, None
 
 
+class LMHeadDistillFn(torch.autograd.Function):
+    """The rows' losses against a teacher's top logits and the block that
+    ops.distill_check reads (ops.lm_head_distill)."""
+
+    @staticmethod
+    def forward(ctx, hn, head, ids, teacher, teacher_lse, temperature: float, keeps: bool):
+        d, k = hn.shape[-1], ids.shape[-1]
+        h2, head2 = _flat(hn, d), head.contiguous()
+        ids2, z, lse = ids.contiguous().view(-1, k), _c(teacher).view(-1, k), _c(teacher_lse)
+        t, vocab = h2.shape[0], head2.shape[0]
+        loss = torch.empty(t, device=hn.device, dtype=torch.float32)
+        result = P.ce_result_buffer(hn.device)
+        keep = None
+        if keeps:
+            n = P.lm_head_distill_keep_bytes(t, d, vocab, k)
+            if 0 < n <= LOGPROBS_KEEP_LIMIT:
+                keep = torch.empty(n, dtype=torch.uint8, device=hn.device)
+        P.lm_head_distill(h2, head2, ids2, z, t, d, vocab, k, loss, result, lse, temperature, keep)
+        ctx.save_for_backward(h2, head2, ids2, z, lse, keep)
+        ctx.shape, ctx.temperature = hn.shape, temperature
+        ctx.mark_non_differentiable(result)
+        ctx.set_materialize_grads(False)
+        return loss.view(hn.shape[:-1]), result
+
+    @staticmethod
+    def backward(ctx, g, _g_result):
+        h2, head, ids, z, lse, keep = ctx.saved_tensors
+        need_hn, need_head = ctx.needs_input_grad[:2]
+        if g is None or not (need_hn or need_head):
+            return (None,) * 7
+        dhn = torch.empty_like(h2) if need_hn else None
+        dhead = torch.empty_like(head) if need_head else None
+        P.lm_head_distill_backward(h2, head, ids, z, g.contiguous().view(-1), h2.shape[0], h2.shape[1], head.shape[0],
+                                   ids.shape[1], dhn, dhead, lse, ctx.temperature, keep, acc=False)
+        return (None if dhn is None else dhn.view(ctx.shape), dhead, *(None,) * 5)
+
+
 class PreferenceLossFn(torch.autograd.Function):
     """ops.preference_loss; its forward already forms dlogp."""
 
@@ -367,6 +404,15 @@ def lm_head_logprobs(hn, head, targets):
     # names what requires a gradient in any mode: whether one can follow shows here.)
     keeps = torch.is_grad_enabled() and (hn.requires_grad or head.requires_grad)
     return LMHeadLogprobsFn.apply(hn, head, targets, keeps)
+
+
+def lm_head_distill(hn, head, ids, teacher, teacher_lse=None, temperature=1.0):
+    """(losses of hn's rows, shaped as hn without its last dim, and the block whose
+    check ops.distill_check runs) of ops.lm_head_distill, ids and teacher [.., k].
+    The losses' gradient flows to hn and head: the teacher is a constant.  It
+    keeps as lm_head_logprobs does."""
+    keeps = torch.is_grad_enabled() and (hn.requires_grad or head.requires_grad)
+    return LMHeadDistillFn.apply(hn, head, ids, teacher, teacher_lse, float(temperature), keeps)
 
 
 def preference_loss(logp, ref_logp, targets, offsets, **kw):

@@ -113,7 +113,7 @@ struct cfattn_ctx {
         Q, K, V, O, LSE, DO_, DQ, DK, DV, QB, KB, VB, DOB, DELTA, PARTIAL, DQROT, DKROT, DS, FWD_SPLIT,
         // layer ops (cfops_capi.cpp)
         OPS_PARTIAL, OPS_ROWLOSS, OPS_MISC, OPS_LOGITS, OPS_DXA, OPS_WS, OPS_LORA, OPS_SEQ, OPS_IDX, OPS_ROWS, OPS_HEAD, OPS_BACK,
-        OPS_STATS, OPS_PART, OPS_DLOGITS, OPS_ROWS_BACK,
+        OPS_STATS, OPS_PART, OPS_DLOGITS, OPS_ROWS_BACK, OPS_ENTRIES,
         // on-disk formats (cfio_capi.cpp): the two device staging chunks
         IO_STAGE,
         NSLOT

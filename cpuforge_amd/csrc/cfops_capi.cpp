@@ -683,6 +683,46 @@ int logprobs_many(cfattn_ctx* c, const float* hn, const float* head, const int64
     return CFATTN_OK;
 }
 
+// Scratch of the head's gradient, which goes through dlogits that fit the head's limit (and a
+// launch with a row of workgroups to 32 rows).  With what a forward kept the rows are packed here.
+struct HeadGrad {
+    size_t pass;
+    char* dlogits;
+    unsigned* col_top;
+};
+int head_grad_scratch(cfattn_ctx* c, const cfattn::HeadPlan& p, size_t t, size_t d, size_t vocab, const float* hn,
+                      const float* dhead, bool kept, cfattn::HeadBuffers& b, HeadGrad& h, hipStream_t st) {
+    h.pass = std::min({p.chunk, (size_t)1 << 20,
+                       std::max<size_t>(c->head_chunk_bytes / (p.v_pad * sizeof(float)) / 128 * 128, 128)});
+    if (!dhead) return CFATTN_OK;
+    CF_TRY(take(c, cfattn_ctx::OPS_DLOGITS, h.pass * p.v_pad * sizeof(float) + vocab * sizeof(unsigned), h.dlogits));
+    h.col_top = reinterpret_cast<unsigned*>(h.dlogits + h.pass * p.v_pad * sizeof(float));
+    char* rows = nullptr;
+    CF_TRY(take(c, cfattn_ctx::OPS_ROWS_BACK, p.rows_back_bytes + p.t_pad * sizeof(float), rows));
+    b.rows_back = rows;
+    if (kept) {
+        // (A pack of the rows alone; their exponents come out the same.)
+        b.scale = reinterpret_cast<float*>(rows + p.rows_back_bytes);
+        cfattn::HeadBuffers only = b;
+        only.back = nullptr;
+        CF_HIP(c, cfattn::launch_head_pack(p, only, hn, nullptr, d, vocab, st), "head gradient launch");
+    }
+    return CFATTN_OK;
+}
+// The gradients of the chunk of scored rows from j0 on.
+int head_grads(cfattn_ctx* c, const cfattn::HeadPlan& p, const cfattn::HeadBuffers& b, size_t t, const float* head,
+               const float* dlogp, const cfattn::HeadEntries* entries, size_t j0, size_t d, size_t vocab, float* dhn,
+               float* dhead, bool acc, const HeadGrad& h, hipStream_t st) {
+    for (size_t i = 0; dhn && i < p.chunk && j0 + i < t; i += p.pass)
+        CF_HIP(c, cfattn::launch_head_dhn(p, b, t, head, dlogp, entries, j0, i, std::min(p.chunk - i, p.pass), d, dhn, st),
+               "head gradient launch");
+    for (size_t i = 0; dhead && i < p.chunk && j0 + i < t; i += h.pass)
+        CF_HIP(c, cfattn::launch_head_dhead(p, b, t, dlogp, entries, j0, i, std::min({t - j0 - i, p.chunk - i, h.pass}),
+                                            d, vocab, h.dlogits, h.col_top, dhead, acc || j0 + i, st),
+               "head gradient launch");
+    return CFATTN_OK;
+}
+
 int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, const int64_t* targets,
                            const float* dlogp, size_t t, size_t d, size_t vocab, float* dhn, float* dhead,
                            bool acc, const void* keep, size_t keep_bytes, hipStream_t st) {
@@ -699,26 +739,8 @@ int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, co
         CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, b.idx, b.count, p.tag, nullptr, nullptr, nullptr, st),
                "log-probability launch");
     }
-    // The head's gradient goes through dlogits that fit the head's limit (and a launch
-    // with a row of workgroups to 32 rows).
-    const size_t pass = std::min({p.chunk, (size_t)1 << 20,
-                                  std::max<size_t>(c->head_chunk_bytes / (p.v_pad * sizeof(float)) / 128 * 128, 128)});
-    char* dlogits = nullptr;
-    unsigned* col_top = nullptr;
-    if (dhead) {
-        CF_TRY(take(c, cfattn_ctx::OPS_DLOGITS, pass * p.v_pad * sizeof(float) + vocab * sizeof(unsigned), dlogits));
-        col_top = reinterpret_cast<unsigned*>(dlogits + pass * p.v_pad * sizeof(float));
-        char* rows = nullptr;
-        CF_TRY(take(c, cfattn_ctx::OPS_ROWS_BACK, p.rows_back_bytes + p.t_pad * sizeof(float), rows));
-        b.rows_back = rows;
-        if (keep) {
-            // (A pack of the rows alone; their exponents come out the same.)
-            b.scale = reinterpret_cast<float*>(rows + p.rows_back_bytes);
-            cfattn::HeadBuffers only = b;
-            only.back = nullptr;
-            CF_HIP(c, cfattn::launch_head_pack(p, only, hn, nullptr, d, vocab, st), "log-probability launch");
-        }
-    }
+    HeadGrad h{};
+    CF_TRY(head_grad_scratch(c, p, t, d, vocab, hn, dhead, keep != nullptr, b, h, st));
     if (!keep) CF_HIP(c, cfattn::launch_head_pack(p, b, hn, head, d, vocab, st), "log-probability launch");
     if (dhn) {
         CF_TRY(take(c, cfattn_ctx::OPS_PART, p.part_bytes, b.part));
@@ -728,14 +750,179 @@ int logprobs_backward_many(cfattn_ctx* c, const float* hn, const float* head, co
         if (!keep)
             CF_HIP(c, cfattn::launch_head_stats(p, b, t, j0, vocab, nullptr, nullptr, st),
                    "log-probability launch");
-        for (size_t i = 0; dhn && i < p.chunk && j0 + i < t; i += p.pass)
-            CF_HIP(c, cfattn::launch_head_dhn(p, b, t, head, dlogp, j0, i, std::min(p.chunk - i, p.pass), d, dhn, st),
-                   "log-probability launch");
-        for (size_t i = 0; dhead && i < p.chunk && j0 + i < t; i += pass)
-            CF_HIP(c, cfattn::launch_head_dhead(p, b, t, dlogp, j0, i, std::min({t - j0 - i, p.chunk - i, pass}),
-                                                d, vocab, dlogits, col_top, dhead, acc || j0 + i, st),
-                   "log-probability launch");
+        CF_TRY(head_grads(c, p, b, t, head, dlogp, nullptr, j0, d, vocab, dhn, dhead, acc, h, st));
     }
+    return CFATTN_OK;
+}
+
+// Distillation: the rows' entries by rising token, in scratch, and what a backward reads of
+// them, where the caller keeps it behind what the head's products keep.
+struct Distill {
+    const int64_t* ids;
+    const float *teacher, *teacher_lse;
+    size_t t, d, vocab, k;
+    double inv_t;
+    float mul;
+};
+struct Entries {
+    int64_t* target;
+    double2* row;
+    float *z, *none;  // none: lse of the rows that are put aside
+    int *ids, *count;
+    float *dl, *a;
+};
+cfattn::HeadPlan distill_plan(const Distill& q, size_t chunk_bytes) {
+    cfattn::HeadPlan p = cfattn::head_plan(q.t, q.d, q.vocab, chunk_bytes);
+    p.tag = (int)((uint32_t)p.tag ^ (uint32_t)q.k * 0x27D4EB2Fu ^ 0x64697374u);
+    return p;
+}
+size_t distill_kept_bytes(size_t t, size_t k) { return 2 * align_up(t * k * sizeof(int)) + align_up(2 * t * sizeof(int)); }
+void entries_at(size_t t, size_t k, char* base, Entries& e) {
+    e.ids = reinterpret_cast<int*>(base);
+    e.dl = reinterpret_cast<float*>(base + align_up(t * k * sizeof(int)));
+    e.count = reinterpret_cast<int*>(base + 2 * align_up(t * k * sizeof(int)));
+    e.a = reinterpret_cast<float*>(e.count + t);
+}
+int distill_entries(cfattn_ctx* c, const Distill& q, char* keep, Entries& e, hipStream_t st) {
+    const size_t own = align_up(q.t * sizeof(double2)) + align_up(q.t * sizeof(int64_t)) +
+                       align_up(q.t * q.k * sizeof(float)) + align_up(q.t * sizeof(float));
+    char* base = nullptr;
+    CF_TRY(take(c, cfattn_ctx::OPS_ENTRIES, own + (keep ? 0 : distill_kept_bytes(q.t, q.k)), base));
+    e.row = reinterpret_cast<double2*>(base);
+    e.target = reinterpret_cast<int64_t*>(base + align_up(q.t * sizeof(double2)));
+    e.z = reinterpret_cast<float*>(reinterpret_cast<char*>(e.target) + align_up(q.t * sizeof(int64_t)));
+    e.none = reinterpret_cast<float*>(reinterpret_cast<char*>(e.z) + align_up(q.t * q.k * sizeof(float)));
+    entries_at(q.t, q.k, keep ? keep : base + own, e);
+    cfattn::DistillEntries g{};
+    g.raw_ids = q.ids, g.teacher = q.teacher, g.teacher_lse = q.teacher_lse, g.t = (long)q.t, g.vocab = (long)q.vocab;
+    g.k = (int)q.k, g.inv_t = q.inv_t, g.ids = e.ids, g.count = e.count, g.z = e.z, g.row = e.row, g.target = e.target;
+    CF_HIP(c, cfattn::launch_distill_entries(g, st), "distillation launch");
+    return CFATTN_OK;
+}
+
+// Few rows: logits in memory, a chunk of rows at a time; the loss or (dhn or dhead) the gradients.
+int distill_few(cfattn_ctx* c, const Distill& q, const float* hn, const float* head, float* loss, void* result,
+                const float* dloss, float* dhn, float* dhead, bool acc, hipStream_t st) {
+    const bool grad = dhn || dhead;
+    Entries e{};
+    CF_TRY(distill_entries(c, q, nullptr, e, st));
+    // (Whole steps of 32 rows, as lm_head_logprobs' gradient of the head takes.)
+    const size_t padded = dhead && q.t > 16 ? (q.t + 31) / 32 * 32 : q.t;
+    LogpRows rows{};
+    CF_TRY(logp_rows(c, padded, q.d, q.vocab, rows));
+    CF_HIP(c, cfattn::launch_logp_select(e.target, q.t, q.vocab, rows.idx, rows.count, 0, loss, e.none, result, st),
+           "distillation launch");
+    CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, rows.idx, rows.count, rows.hn, padded, q.d, st),
+           "distillation launch");
+    cfattn::DistillRows g{};
+    g.ids = e.ids, g.count = e.count, g.z = e.z, g.row = e.row, g.k = (int)q.k, g.inv_t = q.inv_t;
+    g.idx = rows.idx, g.scored = rows.count, g.vocab = (long)q.vocab, g.dloss = dloss, g.loss = loss;
+    for (size_t j0 = 0; j0 < padded; j0 += rows.chunk) {
+        const size_t nr = std::min(padded - j0, rows.chunk);
+        float* h = rows.hn + j0 * q.d;
+        g.j0 = (int)j0;
+        CF_TRY(gemm(c, CFOPS_NT, h, head, rows.logits, nr, q.d, q.vocab, false, st));
+        CF_HIP(c, cfattn::launch_distill_logits(rows.logits, nr, grad, g, st), "distillation launch");
+        if (dhead) CF_TRY(gemm(c, CFOPS_TN, rows.logits, h, dhead, q.vocab, nr, q.d, acc || j0, st));
+        if (dhn) CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, h, nr, q.vocab, q.d, false, st));
+    }
+    if (dhn)
+        CF_HIP(c, cfattn::launch_logp_scatter(rows.hn, q.mul, rows.idx, rows.count, dhn, q.t, q.d, st),
+               "distillation launch");
+    if (!grad)
+        CF_HIP(c, cfattn::launch_logp_finish(e.target, loss, 1.0, q.t, result, st), "distillation launch");
+    return CFATTN_OK;
+}
+
+// Many rows, over the head's products and what those keep: in `keep`, or of a chunk of
+// rows at a time in scratch.
+int distill_rows(cfattn_ctx* c, const Distill& q, const cfattn::HeadPlan& p, const cfattn::HeadBuffers& b,
+                 const Entries& e, const float* hn, const float* head, size_t j0, float* loss, bool grad,
+                 hipStream_t st) {
+    CF_HIP(c, cfattn::launch_head_stats(p, b, q.t, j0, q.vocab, nullptr, nullptr, st), "distillation launch");
+    cfattn::DistillKept g{};
+    g.ids = e.ids, g.count = e.count, g.z = e.z, g.row = e.row, g.k = (int)q.k, g.inv_t = q.inv_t;
+    g.idx = b.idx, g.scored = b.count, g.tag = p.tag, g.j0 = (int)j0, g.chunk = (int)p.chunk;
+    g.parts = (int)((q.vocab + 127) / 128), g.vocab = (int)q.vocab, g.v16 = (int)(p.v_pad / 16), g.d = (int)q.d;
+    g.ld = (long)p.chunk, g.stats = static_cast<const float2*>(b.stats), g.keep = b.keep, g.factor = b.factor;
+    g.hn = hn, g.head = head, g.mul = q.mul, g.loss = loss, g.dl = grad ? e.dl : nullptr, g.a = grad ? e.a : nullptr;
+    CF_HIP(c, cfattn::launch_distill_kept(g, st), "distillation launch");
+    return CFATTN_OK;
+}
+int distill_scratch(cfattn_ctx* c, const Distill& q, const cfattn::HeadPlan& p, bool back, cfattn::HeadBuffers& b) {
+    CF_TRY(take(c, cfattn_ctx::OPS_LOGITS, p.keep_bytes, b.keep));
+    char* base = nullptr;
+    CF_TRY(take(c, cfattn_ctx::OPS_BACK, (back ? p.back_bytes : 0) + p.factor_bytes, base));
+    b.back = back ? base : nullptr;
+    b.factor = reinterpret_cast<float*>(base + (back ? p.back_bytes : 0));
+    return CFATTN_OK;
+}
+
+int distill_many(cfattn_ctx* c, const Distill& q, const float* hn, const float* head, float* loss, void* result,
+                 void* keep, size_t keep_bytes, hipStream_t st) {
+    const cfattn::HeadPlan p = distill_plan(q, keep ? SIZE_MAX : c->head_chunk_bytes);
+    cfattn::HeadBuffers b{};
+    b.mul = q.mul;
+    char* entries = nullptr;
+    if (keep) {
+        const size_t products = keep_layout(p, q.t).bytes;
+        CF_TRY(check_keep(c, keep, keep_bytes, products + distill_kept_bytes(q.t, q.k)));
+        keep_at(p, q.t, static_cast<char*>(keep), b);
+        entries = static_cast<char*>(keep) + products;
+    } else {
+        CF_TRY(distill_scratch(c, q, p, false, b));
+    }
+    CF_TRY(head_scratch(c, p, q.t, b));
+    Entries e{};
+    CF_TRY(distill_entries(c, q, entries, e, st));
+    CF_HIP(c, cfattn::launch_logp_select(e.target, q.t, q.vocab, b.idx, b.count, p.tag, loss, e.none, result, st),
+           "distillation launch");
+    CF_HIP(c, cfattn::launch_head_pack(p, b, hn, head, q.d, q.vocab, st), "distillation launch");
+    for (size_t j0 = 0; j0 < q.t; j0 += p.chunk)
+        CF_TRY(distill_rows(c, q, p, b, e, hn, head, j0, loss, keep != nullptr, st));
+    CF_HIP(c, cfattn::launch_logp_finish(e.target, loss, 1.0, q.t, result, st), "distillation launch");
+    return CFATTN_OK;
+}
+
+int distill_backward_many(cfattn_ctx* c, const Distill& q, const float* hn, const float* head, const float* dloss,
+                          float* dhn, float* dhead, bool acc, const void* keep, size_t keep_bytes, hipStream_t st) {
+    const cfattn::HeadPlan p = distill_plan(q, keep ? SIZE_MAX : c->head_chunk_bytes);
+    cfattn::HeadBuffers b{};
+    b.mul = q.mul;
+    Entries e{};
+    if (keep) {
+        const size_t products = keep_layout(p, q.t).bytes;
+        CF_TRY(check_keep(c, keep, keep_bytes, products + distill_kept_bytes(q.t, q.k)));
+        keep_at(p, q.t, static_cast<char*>(const_cast<void*>(keep)), b);
+        entries_at(q.t, q.k, static_cast<char*>(const_cast<void*>(keep)) + products, e);
+    } else {
+        CF_TRY(distill_scratch(c, q, p, true, b));
+        CF_TRY(head_scratch(c, p, q.t, b));
+        CF_TRY(distill_entries(c, q, nullptr, e, st));
+        CF_HIP(c, cfattn::launch_logp_select(e.target, q.t, q.vocab, b.idx, b.count, p.tag, nullptr, nullptr, nullptr, st),
+               "distillation launch");
+    }
+    const cfattn::HeadEntries he{e.ids, e.count, e.dl, e.a, (int)q.k};
+    HeadGrad h{};
+    CF_TRY(head_grad_scratch(c, p, q.t, q.d, q.vocab, hn, dhead, keep != nullptr, b, h, st));
+    if (!keep) CF_HIP(c, cfattn::launch_head_pack(p, b, hn, head, q.d, q.vocab, st), "distillation launch");
+    if (dhn) {
+        CF_TRY(take(c, cfattn_ctx::OPS_PART, p.part_bytes, b.part));
+        CF_HIP(c, cfattn::launch_head_zero_rows(p, b, q.t, dhn, q.d, st), "distillation launch");
+    }
+    for (size_t j0 = 0; j0 < q.t; j0 += p.chunk) {
+        if (!keep) CF_TRY(distill_rows(c, q, p, b, e, hn, head, j0, nullptr, true, st));
+        CF_TRY(head_grads(c, p, b, q.t, head, dloss, &he, j0, q.d, q.vocab, dhn, dhead, acc, h, st));
+    }
+    return CFATTN_OK;
+}
+
+int check_distill(cfattn_ctx* c, const Distill& q, double temperature) {
+    CF_TRY(check_logprobs(c, q.t, q.d, q.vocab));
+    if (q.k == 0 || q.k > cfattn::kDistillMost)
+        return fail(c, CFATTN_ERR_UNSUPPORTED, "k=%zu entries of a row, 1 to %zu are", q.k, cfattn::kDistillMost);
+    if (!(temperature > 0.0) || !std::isfinite(temperature) || !std::isfinite(q.mul) || !(q.mul > 0.0f))
+        return fail(c, CFATTN_ERR_ARG, "the temperature must be positive and finite");
     return CFATTN_OK;
 }
 
@@ -806,7 +993,7 @@ int cfops_lm_head_logprobs(cfattn_ctx* c, const float* hn, const float* head, co
     }
     if (t <= cfattn::kLogpUnkept) keep = nullptr;
     CF_TRY(logprobs_many(c, hn, head, targets, t, d, vocab, logp, lse, result, keep, keep_bytes, st));
-    CF_HIP(c, cfattn::launch_logp_finish(targets, logp, t, result, st), "log-probability launch");
+    CF_HIP(c, cfattn::launch_logp_finish(targets, logp, -1.0, t, result, st), "log-probability launch");
     return CFATTN_OK;
 }
 
@@ -832,7 +1019,7 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
     CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, 0, nullptr, nullptr, nullptr,
                                               st),
            "log-probability launch");
-    CF_HIP(c, cfattn::launch_logp_gather(hn, rows.idx, rows.count, rows.hn, padded, d, st), "log-probability launch");
+    CF_HIP(c, cfattn::launch_logp_gather(hn, 1.0f, rows.idx, rows.count, rows.hn, padded, d, st), "log-probability launch");
     for (size_t j0 = 0; j0 < padded; j0 += rows.chunk) {
         const size_t nr = std::min(padded - j0, rows.chunk);
         float* h = rows.hn + j0 * d;
@@ -844,8 +1031,48 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
         if (dhn) CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, h, nr, vocab, d, false, st));
     }
     if (dhn)
-        CF_HIP(c, cfattn::launch_logp_scatter(rows.hn, rows.idx, rows.count, dhn, t, d, st), "log-probability launch");
+        CF_HIP(c, cfattn::launch_logp_scatter(rows.hn, 1.0f, rows.idx, rows.count, dhn, t, d, st), "log-probability launch");
     return CFATTN_OK;
+}
+
+size_t cfops_lm_head_distill_keep_bytes(size_t t, size_t d, size_t vocab, size_t k) {
+    const size_t products = cfops_lm_head_logprobs_keep_bytes(t, d, vocab);
+    if (products == 0 || k == 0 || k > cfattn::kDistillMost) return 0;
+    return products + distill_kept_bytes(t, k);
+}
+
+int cfops_lm_head_distill(cfattn_ctx* c, const float* hn, const float* head, const int64_t* ids, const float* teacher,
+                          const float* teacher_lse, size_t t, size_t d, size_t vocab, size_t k, double temperature,
+                          float* loss, cfops_ce_result* result, void* keep, size_t keep_bytes, void* stream) {
+    CF_LOCK(c, stream);
+    if (!result) return fail(c, CFATTN_ERR_ARG, "null result");
+    const Distill q{ids, teacher, teacher_lse, t, d, vocab, k, 1.0 / temperature, (float)(1.0 / temperature)};
+    CF_TRY(check_distill(c, q, temperature));
+    if (!head || (t && (!hn || !ids || !teacher || !loss))) return fail(c, CFATTN_ERR_ARG, "null buffer");
+    const hipStream_t st = to_stream(stream);
+    if (t == 0) {
+        CF_HIP(c, cfattn::launch_ce_begin(nullptr, 0, result, st), "distillation launch");
+        return CFATTN_OK;
+    }
+    if (t <= cfattn::kLogpUnkept)
+        return distill_few(c, q, hn, head, loss, result, nullptr, nullptr, nullptr, false, st);
+    return distill_many(c, q, hn, head, loss, result, keep, keep_bytes, st);
+}
+
+int cfops_lm_head_distill_backward(cfattn_ctx* c, const float* hn, const float* head, const int64_t* ids,
+                                   const float* teacher, const float* teacher_lse, const float* dloss, size_t t,
+                                   size_t d, size_t vocab, size_t k, double temperature, float* dhn, float* dhead,
+                                   int acc, const void* keep, size_t keep_bytes, void* stream) {
+    CF_LOCK(c, stream);
+    const Distill q{ids, teacher, teacher_lse, t, d, vocab, k, 1.0 / temperature, (float)(1.0 / temperature)};
+    CF_TRY(check_distill(c, q, temperature));
+    if (t == 0 && !acc) return zero_grad(c, dhead, vocab * d, to_stream(stream));
+    if (t == 0 || (!dhn && !dhead)) return CFATTN_OK;
+    if (!hn || !head || !ids || !teacher || !dloss) return fail(c, CFATTN_ERR_ARG, "null buffer");
+    const hipStream_t st = to_stream(stream);
+    if (t <= cfattn::kLogpUnkept)
+        return distill_few(c, q, hn, head, nullptr, nullptr, dloss, dhn, dhead, acc != 0, st);
+    return distill_backward_many(c, q, hn, head, dloss, dhn, dhead, acc != 0, keep, keep_bytes, st);
 }
 
 static_assert(sizeof(cfops_preference_result) == sizeof(cfattn::PreferenceResult) &&

@@ -227,19 +227,20 @@ hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st);
 //   select:    idx and, from idx + rows on, their targets; count[0], tag in count[1]; the
 //              result block (CeMisc; or null), and logp
 //              and lse (or null) of the rows that are not scored;
-//   gather:    the scored rows of hn side by side;   scatter: back, other rows 0;
+//   gather:    the scored rows of hn side by side, times mul;   scatter: back, other rows 0;
 //   grad_rows: the logits become their gradients;
-//   finish:    the mean of -logp, summed in f64 in a fixed order.
+//   finish:    the mean of sign logp, summed in f64 in a fixed order.
 hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, int tag,
                               float* logp, float* lse, void* misc, hipStream_t st);
-hipError_t launch_logp_gather(const float* hn, const int* idx, const int* count, float* out, size_t rows, size_t d,
-                              hipStream_t st);
-hipError_t launch_logp_scatter(const float* in, const int* idx, const int* count, float* dhn, size_t rows, size_t d,
-                               hipStream_t st);
+hipError_t launch_logp_gather(const float* hn, float mul, const int* idx, const int* count, float* out, size_t rows,
+                              size_t d, hipStream_t st);
+hipError_t launch_logp_scatter(const float* in, float mul, const int* idx, const int* count, float* dhn, size_t rows,
+                               size_t d, hipStream_t st);
 hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const int* idx, const int* count,
                                  const float* lse, const float* dlogp, size_t j0, size_t nrows, size_t vocab,
                                  hipStream_t st);
-hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t rows, void* misc, hipStream_t st);
+hipError_t launch_logp_finish(const int64_t* targets, const float* logp, double sign, size_t rows, void* misc,
+                              hipStream_t st);
 // All of the forward for at most kLogpFew rows in two launches, in scratch of
 // logp_few_bytes(t, vocab).
 constexpr size_t kLogpFew = 32;
@@ -290,6 +291,14 @@ struct HeadBuffers {
     char *rows, *packed, *back, *keep, *rows_back;  // operands
     float *scale, *xt, *factor, *part;   // scale [t_pad], xt [chunk]
     void* stats;
+    float mul = 1.0f;                    // of hn
+};
+// In a target's place k entries of each row (distill.hip), whose kept exponentials are zeros: dlogits
+// are dloss (a q_v + dl of the entry that v is); dhn is times mul.
+struct HeadEntries {
+    const int *ids, *count;  // [t][k] rising, and how many
+    const float *dl, *a;     // [t][k], [t]
+    int k;
 };
 HeadPlan head_plan(size_t t, size_t d, size_t vocab, size_t chunk_bytes);
 hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float* hn, const float* head, size_t d,
@@ -299,12 +308,60 @@ hipError_t launch_head_mid(const HeadPlan& p, const HeadBuffers& b, const float*
 hipError_t launch_head_stats(const HeadPlan& p, const HeadBuffers& b, size_t t, size_t j0, size_t vocab,
                              float* logp, float* lse, hipStream_t st);
 hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* head,
-                           const float* dlogp, size_t j0, size_t local, size_t rows, size_t d, float* dhn,
-                           hipStream_t st);
+                           const float* dlogp, const HeadEntries* entries, size_t j0, size_t local, size_t rows,
+                           size_t d, float* dhn, hipStream_t st);
 hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* dlogp,
-                             size_t j0, size_t local, size_t rows, size_t d, size_t vocab, char* packed_dlogits,
-                             unsigned* col_top, float* dhead, int acc, hipStream_t st);
+                             const HeadEntries* entries, size_t j0, size_t local, size_t rows, size_t d, size_t vocab,
+                             char* packed_dlogits, unsigned* col_top, float* dhead, int acc, hipStream_t st);
 hipError_t launch_head_zero_rows(const HeadPlan& p, const HeadBuffers& b, size_t t, float* dhn, size_t d,
                                  hipStream_t st);
+
+// Distillation from a teacher's top logits (distill.hip).  entries: the rows' entries by
+// rising token, what the teacher's distribution is, and a `target` by which launch_logp_select
+// takes rows (kept, of which the head's products kept statistics and exponentials) or puts
+// them aside; logits: the scored rows [j0, j0 + nrows), whose logits are in memory.
+constexpr size_t kDistillMost = 1024;  // entries of a row
+struct DistillEntries {
+    const int64_t* raw_ids;
+    const float *teacher, *teacher_lse;  // teacher_lse may be null
+    long t, vocab;
+    int k;
+    double inv_t;
+    int *ids, *count;  // [t][k], [t]
+    float* z;          // [t][k]
+    double2* row;      // [t]: the entries' log-sum-exp or the teacher's, p_rest (negative: no rest)
+    int64_t* target;   // [t]
+};
+hipError_t launch_distill_entries(const DistillEntries& g, hipStream_t st);
+struct DistillKept {
+    const int *ids, *count;
+    const float* z;
+    const double2* row;
+    int k;
+    double inv_t;
+    const int *idx, *scored;  // scored rows, how many and the plan's tag
+    int tag, j0, chunk, parts, vocab, v16, d;
+    long ld;
+    const float2* stats;
+    char* keep;
+    float* factor;
+    const float *hn, *head;
+    float mul;
+    float *loss, *dl, *a;  // loss may be null; dl and a may be, together
+};
+hipError_t launch_distill_kept(const DistillKept& g, hipStream_t st);
+struct DistillRows {
+    const int *ids, *count;
+    const float* z;
+    const double2* row;
+    int k;
+    double inv_t;
+    const int *idx, *scored;
+    int j0;
+    long vocab;
+    const float* dloss;  // grad
+    float* loss;         // else
+};
+hipError_t launch_distill_logits(float* logits, size_t nrows, bool grad, const DistillRows& g, hipStream_t st);
 
 }  // namespace cfattn

@@ -83,6 +83,7 @@ struct Pieces {
     f16x8 h, l;
 };
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ Pieces split8(const float (&x)[8], float scale) {
 #pragma clang fp contract(off)
     Pieces p;
@@ -133,6 +134,7 @@ struct PackArgs {
     float* scale;
     int* exponents;
     int row_blocks, vocab, d, k16, v16, t16, vec_rows, vec_head, tag;
+    float mul;  // of hn
 };
 
 // 32 rows to a workgroup, as operands [32 rows][16 k][piece]: first the scored rows
@@ -161,6 +163,7 @@ __global__ __launch_bounds__(64 * NW) void pack_kernel(const PackArgs g) {
         if (r < n) row = g.hn + (long)g.idx[r] * d;
     }
     const bool v = (is_head ? g.vec_head : g.vec_rows) && row;
+    const float mul = is_head ? 1.0f : g.mul;
     const int c = 8 * (lane >> 5), pairs = (k16 + 1) / 2;
     float top = 0.0f, x[U ? U : 1][2][8];
     auto load = [&](float (&y)[2][8], int s) {
@@ -170,7 +173,14 @@ __global__ __launch_bounds__(64 * NW) void pack_kernel(const PackArgs g) {
             load8(y[q], in ? row : nullptr, 16 * (2 * s + q) + c, d, v && in);
         }
     };
-    auto widen = [&](const float (&y)[2][8]) {
+    auto times = [&](float (&y)[2][8]) {
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[q][i] *= mul;
+    };
+    auto widen = [&](float (&y)[2][8]) {
+        times(y);
 #pragma unroll
         for (int q = 0; q < 2; q++)
 #pragma unroll
@@ -243,6 +253,7 @@ __global__ __launch_bounds__(64 * NW) void pack_kernel(const PackArgs g) {
     } else {
         for (int s = wave; s < pairs; s += NW) {
             load(x[0], s);
+            times(x[0]);
             store(x[0], s);
         }
     }
@@ -792,9 +803,11 @@ __global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restr
         factor[p * ld + j] = j < n && p < parts ? exp2f(stats[p * ld + j].x - all[c].x) * all[c].y : 0.0f;
 }
 
-// dhn of scored rows [j0, ..): dlogp (head[target] - the splits' sums in order).
+// dhn of scored rows [j0, ..): dlogp (head[target] - the splits' sums in order), or, with
+// entries, mul dloss (a times those sums + the sum of the entries' dl head).
 // Four columns to a thread, eight splits' sums in flight: bound by memory, 3686 x 576 with
-// 16 splits (136 MB) 29 us.
+// 16 splits (136 MB) 29 us; with 64 entries of each row (543 MB of the head, in the caches) TODO.
+template <bool ENTRIES>
 __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __restrict__ part, int chunk, int rows,
                                                                int mt, int k16, int splits_max,
                                                                const int* __restrict__ idx,
@@ -802,7 +815,8 @@ __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __re
                                                                const int* __restrict__ count, int tag, int j0,
                                                                const float* __restrict__ head,
                                                                const float* __restrict__ dlogp,
-                                                               float* __restrict__ dhn, int d) {
+                                                               float* __restrict__ dhn, int d, const HeadEntries en,
+                                                               float mul) {
     const int n = scored_rows(count, tag, j0, chunk);
     const int quads = (d + 3) / 4;
     const long at = (long)blockIdx.x * 256 + threadIdx.x;
@@ -820,12 +834,37 @@ __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __re
         for (int z = 0; z < 8; z++) s.x += x[z].x, s.y += x[z].y, s.z += x[z].z, s.w += x[z].w;
     }
     const long r = idx[j0 + col];
-    const float* w = head + (long)targets[j0 + col] * d + i0;
     float* out = dhn + r * d + i0;
     const float f = dlogp[r], t[4] = {s.x, s.y, s.z, s.w};
+    if constexpr (ENTRIES) {
+        float sum[4] = {};
+        const int m = en.count[r];
+        const int* ids = en.ids + r * en.k;
+        const float* dl = en.dl + r * en.k;
+        if (i0 + 4 <= d) {
+#pragma unroll 8
+            for (int k = 0; k < m; k++) {
+                const f32x4u w = *reinterpret_cast<const f32x4u*>(head + (long)ids[k] * d + i0);
+                const float g = dl[k];
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (i0 + i < d) out[i] = f * (w[i] - t[i]);
+                for (int i = 0; i < 4; i++) sum[i] = fmaf(g, w[i], sum[i]);
+            }
+        } else {
+            for (int k = 0; k < m; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (i0 + i < d) sum[i] = fmaf(dl[k], head[(long)ids[k] * d + i0 + i], sum[i]);
+        }
+        const float a = en.a[r];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i0 + i < d) out[i] = mul * f * fmaf(a, t[i], sum[i]);
+    } else {
+        const float* w = head + (long)targets[j0 + col] * d + i0;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i0 + i < d) out[i] = f * (w[i] - t[i]);
+    }
 }
 
 // What the head's gradient takes of what statistics kept, for scored rows [j0, ..).
@@ -838,6 +877,7 @@ struct DlogitsArgs {
     char* out;            // [32 columns][t16][piece]
     long ld;
     int v16, t16, tag, j0, chunk, vocab;
+    HeadEntries en;
 };
 
 // 2^14 and the power of two of a row of hn: a power of two near its largest value, so
@@ -849,6 +889,7 @@ __device__ __forceinline__ float row_top(float scale) { return scale * 16384.0f;
 // others', which an optimizer that divides by their size scales up.  128 columns and
 // every 8th 32 rows to a workgroup: 819 rows x 50001 (180 MB) 31 us.  (At a target 1 - P
 // counts as 1.)
+template <bool ENTRIES>
 __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
     const int n = scored_rows(g.count, g.tag, g.j0, g.chunk);
@@ -856,7 +897,9 @@ __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) 
     for (int t0 = 32 * blockIdx.y; t0 < n; t0 += 32 * gridDim.y) {
         const int j = t0 + l32;
         if (j >= n) continue;
-        const float row = fabsf(g.dlogp[g.idx[g.j0 + j]] * row_top(g.scale[g.j0 + j]));
+        const long r = g.idx[g.j0 + j];
+        float row = fabsf(g.dlogp[r] * row_top(g.scale[g.j0 + j]));
+        if constexpr (ENTRIES) row *= fabsf(g.en.a[r]);
         const float f = g.factor[blockIdx.x * g.ld + j];
 #pragma unroll
         for (int q = 0; q < 2; q++) {
@@ -868,7 +911,7 @@ __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) 
                 top[q][i] = fmaxf(top[q][i], finite_abs((i < 4 ? a[i] : b[i - 4]) * f * row));
         }
         // (One workgroup of the columns sees to a row's target.)
-        if (blockIdx.x == 0 && wave == 0 && hh == 0)
+        if (!ENTRIES && blockIdx.x == 0 && wave == 0 && hh == 0)
             atomicMax(g.col_top + g.targets[g.j0 + j], __builtin_bit_cast(unsigned, finite_abs(row)));
     }
 #pragma unroll
@@ -883,9 +926,21 @@ __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) 
         }
 }
 
+// The same of the rows' entries, a wave to a row.
+__global__ __launch_bounds__(256) void head_entries_top_kernel(const DlogitsArgs g) {
+    const int j = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (j >= scored_rows(g.count, g.tag, g.j0, g.chunk)) return;
+    const long r = g.idx[g.j0 + j];
+    const float row = g.dlogp[r] * row_top(g.scale[g.j0 + j]);
+    for (int k = threadIdx.x & 63; k < g.en.count[r]; k += 64)
+        atomicMax(g.col_top + g.en.ids[r * g.en.k + k],
+                  __builtin_bit_cast(unsigned, finite_abs(row * g.en.dl[r * g.en.k + k])));
+}
+
 // The dlogits times their rows' row_top as operands by columns: 32 rows and 128 columns
 // to a workgroup, turned round in LDS.  Bound by memory: 819 x 50001, read and written,
 // (328 MB) 54 us.
+template <bool ENTRIES>
 __global__ __launch_bounds__(256) void head_pack_dlogits_kernel(const DlogitsArgs g) {
     __shared__ float tile[32][129];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, hh = lane >> 5;
@@ -894,8 +949,8 @@ __global__ __launch_bounds__(256) void head_pack_dlogits_kernel(const DlogitsArg
     const bool scored = j < n;
     const long r = scored ? g.idx[g.j0 + j] : 0;
     const float row = scored ? g.dlogp[r] * row_top(g.scale[g.j0 + j]) : 0.0f;
-    const float f = scored ? g.factor[blockIdx.x * g.ld + j] : 0.0f;
-    const int target = scored ? g.targets[g.j0 + j] - (int)blockIdx.x * 128 : -1;
+    const float f = (scored ? g.factor[blockIdx.x * g.ld + j] : 0.0f) * (ENTRIES && scored ? -g.en.a[r] : 1.0f);
+    const int target = !ENTRIES && scored ? g.targets[g.j0 + j] - (int)blockIdx.x * 128 : -1;
 #pragma unroll
     for (int q = 0; q < 2; q++) {
         const int s = 2 * wave + q;  // 16 columns
@@ -910,6 +965,21 @@ __global__ __launch_bounds__(256) void head_pack_dlogits_kernel(const DlogitsArg
         }
     }
     __syncthreads();
+    if constexpr (ENTRIES) {
+        // Eight threads to a row look through its entries for these columns'.
+        const int jr = t0 + (threadIdx.x >> 3);
+        if (jr < n) {
+            const long rr = g.idx[g.j0 + jr];
+            const float top = g.dlogp[rr] * row_top(g.scale[g.j0 + jr]);
+            const int m = g.en.count[rr];
+#pragma unroll 8
+            for (int k = threadIdx.x & 7; k < m; k += 8) {
+                const int c = g.en.ids[rr * g.en.k + k] - (int)blockIdx.x * 128;
+                if (c >= 0 && c < 128) tile[threadIdx.x >> 3][c] = top * g.en.dl[rr * g.en.k + k];
+            }
+        }
+        __syncthreads();
+    }
     const int v = blockIdx.x * 128 + 32 * wave + l32;
     const float sc = exp2i(-group_exponent(v < g.vocab ? __builtin_bit_cast(float, g.col_top[v]) : 0.0f));
 #pragma unroll
@@ -1004,7 +1074,7 @@ hipError_t launch_head_pack(const HeadPlan& p, const HeadBuffers& b, const float
     g.scale = b.scale, g.exponents = b.exponents, g.row_blocks = (int)(p.t_pad / 32);
     g.vocab = (int)vocab, g.d = (int)d, g.k16 = p.k16, g.v16 = (int)(p.v_pad / 16);
     g.vec_rows = d % 4 == 0 && aligned16(hn), g.vec_head = d % 4 == 0 && aligned16(head);
-    g.tag = p.tag;
+    g.tag = p.tag, g.mul = b.mul;
     const size_t blocks = (p.t_pad + (head ? p.v_pad : 0)) / 32;
     const int pairs = (p.k16 + 1) / 2;
     auto pack = [&](auto back, auto nw, auto u) {
@@ -1070,8 +1140,8 @@ hipError_t launch_head_mid(const HeadPlan& p, const HeadBuffers& b, const float*
 }
 
 hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* head,
-                           const float* dlogp, size_t j0, size_t local, size_t rows, size_t d, float* dhn,
-                           hipStream_t st) {
+                           const float* dlogp, const HeadEntries* entries, size_t j0, size_t local, size_t rows,
+                           size_t d, float* dhn, hipStream_t st) {
     const int mb = p.back_mb;
     HeadArgs g{};
     g.a = b.back, g.b = b.keep + local * p.v_pad * 4, g.ka = g.kb = (int)(p.v_pad / 16);
@@ -1085,15 +1155,16 @@ hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, co
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const size_t quads = rows * ((d + 3) / 4);
-    hipLaunchKernelGGL(head_grad_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, b.part, g.chunk,
-                       (int)p.d_pad, g.mt, g.ka, g.splits_max, b.idx, b.idx + t, b.count, p.tag, g.j0, head,
-                       dlogp, dhn, (int)d);
+    hipLaunchKernelGGL((entries ? head_grad_reduce_kernel<true> : head_grad_reduce_kernel<false>),
+                       dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, b.part, g.chunk, (int)p.d_pad, g.mt, g.ka,
+                       g.splits_max, b.idx, b.idx + t, b.count, p.tag, g.j0, head, dlogp, dhn, (int)d,
+                       entries ? *entries : HeadEntries{}, b.mul);
     return hipGetLastError();
 }
 
 hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, size_t t, const float* dlogp,
-                             size_t j0, size_t local, size_t rows, size_t d, size_t vocab, char* packed_dlogits,
-                             unsigned* col_top, float* dhead, int acc, hipStream_t st) {
+                             const HeadEntries* entries, size_t j0, size_t local, size_t rows, size_t d, size_t vocab,
+                             char* packed_dlogits, unsigned* col_top, float* dhead, int acc, hipStream_t st) {
     DlogitsArgs g{};
     g.keep = b.keep + local * p.v_pad * 4, g.factor = b.factor + local;
     g.idx = b.idx, g.count = b.count, g.targets = b.idx + t, g.dlogp = dlogp, g.tag = p.tag;
@@ -1102,9 +1173,16 @@ hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, size_t t, 
     hipError_t e = launch_fill_zero(reinterpret_cast<float*>(col_top), vocab, st);
     if (e != hipSuccess) return e;
     const unsigned t32 = (unsigned)((rows + 31) / 32), v128 = (unsigned)(p.v_pad / 128);
-    hipLaunchKernelGGL(head_col_top_kernel, dim3(v128, std::min(t32, 8u)), dim3(256), 0, st, g);
+    if (entries) g.en = *entries;
+    hipLaunchKernelGGL((entries ? head_col_top_kernel<true> : head_col_top_kernel<false>), dim3(v128, std::min(t32, 8u)),
+                       dim3(256), 0, st, g);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL(head_pack_dlogits_kernel, dim3(v128, t32), dim3(256), 0, st, g);
+    if (entries) {
+        hipLaunchKernelGGL(head_entries_top_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, g);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((entries ? head_pack_dlogits_kernel<true> : head_pack_dlogits_kernel<false>), dim3(v128, t32),
+                       dim3(256), 0, st, g);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     HeadArgs h{};
     h.a = packed_dlogits, h.b = b.rows_back + (j0 + local) / 16 * 2 * kFrag, h.ka = g.t16, h.kb = (int)(p.t_pad / 16);

@@ -76,19 +76,19 @@ __global__ __launch_bounds__(1024) void logp_select_kernel(const int64_t* __rest
     }
 }
 
-// out[j] = hn[idx[j]], zeros from row n on.
-__global__ __launch_bounds__(256) void logp_gather_kernel(const float* __restrict__ hn, const int* __restrict__ idx,
-                                                          const int* __restrict__ count, float* __restrict__ out,
-                                                          long d) {
+// out[j] = mul hn[idx[j]], zeros from row n on.
+__global__ __launch_bounds__(256) void logp_gather_kernel(const float* __restrict__ hn, float mul,
+                                                          const int* __restrict__ idx, const int* __restrict__ count,
+                                                          float* __restrict__ out, long d) {
     const long j = blockIdx.x;
     const float* x = j < *count ? hn + (long)idx[j] * d : nullptr;
-    for (long i = threadIdx.x; i < d; i += 256) out[j * d + i] = x ? x[i] : 0.0f;
+    for (long i = threadIdx.x; i < d; i += 256) out[j * d + i] = x ? mul * x[i] : 0.0f;
 }
 
-// dhn[idx[j]] = in[j] for j < n, the other rows zeros.
-__global__ __launch_bounds__(256) void logp_scatter_kernel(const float* __restrict__ in, const int* __restrict__ idx,
-                                                           const int* __restrict__ count, float* __restrict__ dhn,
-                                                           long d) {
+// dhn[idx[j]] = mul in[j] for j < n, the other rows zeros.
+__global__ __launch_bounds__(256) void logp_scatter_kernel(const float* __restrict__ in, float mul,
+                                                           const int* __restrict__ idx, const int* __restrict__ count,
+                                                           float* __restrict__ dhn, long d) {
     // The place of row blockIdx.x among the ascending idx.
     const int r = blockIdx.x, n = *count;
     int lo = 0, hi = n;
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256) void logp_scatter_kernel(const float* __restri
             hi = mid;
     }
     const float* x = lo < n && idx[lo] == r ? in + (long)lo * d : nullptr;
-    for (long i = threadIdx.x; i < d; i += 256) dhn[r * d + i] = x ? x[i] : 0.0f;
+    for (long i = threadIdx.x; i < d; i += 256) dhn[r * d + i] = x ? mul * x[i] : 0.0f;
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -264,17 +264,17 @@ __global__ __launch_bounds__(512) void logp_grad_rows_kernel(float* __restrict__
         x[i] = i == t ? -g * expm1f((x[i] - l) - more) : f * expf(x[i] - l);
 }
 
-// The mean of -logp over the scored rows, summed in f64 in a fixed order by one
+// The mean of sign logp over the scored rows, summed in f64 in a fixed order by one
 // workgroup: 4096 rows 5.2 us.
 __global__ __launch_bounds__(1024) void logp_finish_kernel(const int64_t* __restrict__ targets,
-                                                           const float* __restrict__ logp, long rows,
+                                                           const float* __restrict__ logp, double sign, long rows,
                                                            CeMisc* __restrict__ m) {
     __shared__ double red[16];
     double s = 0.0;
 #pragma unroll 4
     for (long r = threadIdx.x; r < rows; r += 1024) {
         const float x = logp[r];
-        s -= targets[r] != kIgnoreIndex ? (double)x : 0.0;
+        s += targets[r] != kIgnoreIndex ? sign * (double)x : 0.0;
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
@@ -296,14 +296,14 @@ hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab,
                        tag, logp, lse, static_cast<CeMisc*>(misc));
     return hipGetLastError();
 }
-hipError_t launch_logp_gather(const float* hn, const int* idx, const int* count, float* out, size_t rows, size_t d,
-                              hipStream_t st) {
-    hipLaunchKernelGGL(logp_gather_kernel, dim3((unsigned)rows), dim3(256), 0, st, hn, idx, count, out, (long)d);
+hipError_t launch_logp_gather(const float* hn, float mul, const int* idx, const int* count, float* out, size_t rows,
+                              size_t d, hipStream_t st) {
+    hipLaunchKernelGGL(logp_gather_kernel, dim3((unsigned)rows), dim3(256), 0, st, hn, mul, idx, count, out, (long)d);
     return hipGetLastError();
 }
-hipError_t launch_logp_scatter(const float* in, const int* idx, const int* count, float* dhn, size_t rows, size_t d,
-                               hipStream_t st) {
-    hipLaunchKernelGGL(logp_scatter_kernel, dim3((unsigned)rows), dim3(256), 0, st, in, idx, count, dhn, (long)d);
+hipError_t launch_logp_scatter(const float* in, float mul, const int* idx, const int* count, float* dhn, size_t rows,
+                               size_t d, hipStream_t st) {
+    hipLaunchKernelGGL(logp_scatter_kernel, dim3((unsigned)rows), dim3(256), 0, st, in, mul, idx, count, dhn, (long)d);
     return hipGetLastError();
 }
 size_t logp_few_bytes(size_t t, size_t vocab) {
@@ -330,8 +330,9 @@ hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const in
                        lse, dlogp, (int)j0, (long)vocab);
     return hipGetLastError();
 }
-hipError_t launch_logp_finish(const int64_t* targets, const float* logp, size_t rows, void* misc, hipStream_t st) {
-    hipLaunchKernelGGL(logp_finish_kernel, dim3(1), dim3(1024), 0, st, targets, logp, (long)rows,
+hipError_t launch_logp_finish(const int64_t* targets, const float* logp, double sign, size_t rows, void* misc,
+                              hipStream_t st) {
+    hipLaunchKernelGGL(logp_finish_kernel, dim3(1), dim3(1024), 0, st, targets, logp, sign, (long)rows,
                        static_cast<CeMisc*>(misc));
     return hipGetLastError();
 }

@@ -20,9 +20,10 @@ Layers of other decoders have no reference counterpart:
     layernorm_forward / layernorm_backward
     rotary                              q and k at given positions, either layout
 
-nor has training on preferences and rewards:
+nor has training on preferences, rewards and a teacher:
 
     lm_head_logprobs(_backward)         the targets' log-probabilities
+    lm_head_distill(_backward)          a loss against a teacher's top logits
     preference_loss, policy_loss        losses over them, with their gradients
     adamw8_update_multi                 AdamW with its moments in 8 bits
 
@@ -437,6 +438,61 @@ def lm_head_logprobs_keep_bytes(t: int, d: int, vocab: int) -> int:
     """Size of lm_head_logprobs' keep (about 4 t vocab + 4 d vocab bytes), 0
     where it uses none."""
     return _lib.lib().cfops_lm_head_logprobs_keep_bytes(int(t), int(d), int(vocab))
+
+
+# ------------------------------ distillation from a teacher's top logits
+def lm_head_distill(hn, head, ids, teacher, t, d, vocab, k, loss, result, teacher_lse=None, temperature=1.0, keep=None,
+                    ctx: Context | None = None) -> None:
+    """The loss [t] (overwritten) of the student's logits x = hn . head^T /
+    temperature (never held whole), q = softmax(x), against a teacher's top
+    logits: of each row k tokens ids [t, k] (int64) and their logits teacher [t, k];
+    those with id IGNORE_INDEX or logit -inf are not there.  With p =
+    exp(teacher / temperature - L)
+        sum p (log p - log q) + p_rest (log p_rest - log q_rest),
+    L = teacher_lse [t], the log-sum-exp of all the teacher's logits / temperature,
+    and the other tokens (the rest) one class; teacher_lse None: L the entries' own,
+    and no rest.  A row without entries has loss 0.  `result` (ce_result_buffer) gets
+    the mean (ce_result_loss) and the first row with a token out of range or
+    twice, or a teacher's value NaN or +inf, which distill_check reports; such a
+    row's loss is NaN.  `keep` (a uint8 tensor of lm_head_distill_keep_bytes, when
+    given) takes what the backward reads.  No host wait."""
+    ctx = ctx or default_context()
+    _call(ctx, "cfops_lm_head_distill", *_distill(hn, head, ids, teacher, teacher_lse, t, d, vocab, k, ctx), t, d, vocab,
+          k, float(temperature), _on(loss, "loss", ctx, numel=t), _result(result, CE_RESULT_WORDS), *_keep(keep),
+          _stream_of(ctx))
+
+
+def lm_head_distill_backward(hn, head, ids, teacher, dloss, t, d, vocab, k, dhn=None, dhead=None, teacher_lse=None,
+                             temperature=1.0, keep=None, ctx: Context | None = None, acc: bool = True) -> None:
+    """From the gradient dloss of loss: dhn (overwritten) and dhead += (acc=False:
+    overwritten), each when given.  The others are the forward's; without keep the
+    logits are formed again."""
+    ctx = ctx or default_context()
+    _call(ctx, "cfops_lm_head_distill_backward", *_distill(hn, head, ids, teacher, teacher_lse, t, d, vocab, k, ctx),
+          _on(dloss, "dloss", ctx, numel=t), t, d, vocab, k, float(temperature),
+          None if dhn is None else _on(dhn, "dhn", ctx, numel=t * d),
+          None if dhead is None else _on(dhead, "dhead", ctx, numel=vocab * d), int(acc), *_keep(keep),
+          _stream_of(ctx))
+
+
+def _distill(hn, head, ids, teacher, lse, t, d, vocab, k, ctx):
+    return (_on(hn, "hn", ctx, numel=t * d), _on(head, "head", ctx, numel=vocab * d),
+            _on(ids, "ids", ctx, (torch.int64,), t * k), _on(teacher, "teacher", ctx, numel=t * k),
+            None if lse is None else _on(lse, "teacher_lse", ctx, numel=t))
+
+
+def lm_head_distill_keep_bytes(t: int, d: int, vocab: int, k: int) -> int:
+    """Size of lm_head_distill's keep, 0 where it uses none."""
+    return _lib.lib().cfops_lm_head_distill_keep_bytes(int(t), int(d), int(vocab), int(k))
+
+
+def distill_check(result: torch.Tensor) -> None:
+    """Waits for `result` and raises for a row whose entries lm_head_distill does
+    not take."""
+    bad = int(result[1].item())
+    if bad != _NO_BAD_ROW:
+        raise _lib.CfattnError(_lib.ERR_ARG, f"row {bad} names a token out of range or twice, or a value of the "
+                                             "teacher's is not finite")
 
 
 # ------------------------------------------- losses over packed sequences

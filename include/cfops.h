@@ -241,6 +241,35 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* ctx, const float* hn, const floa
                                     float* dhn, float* dhead, int acc, const void* keep, size_t keep_bytes,
                                     void* stream);
 
+/* Distillation from a teacher's top logits.  Row r of hn has k entries: tokens ids[r]
+ * (int64, [t, k], in any order) and the teacher's logits teacher[r] of them; one whose
+ * id is CFOPS_IGNORE_INDEX or whose logit is -inf is not there.  With the logits
+ * x = hn . head^T / temperature, never held whole, q = softmax(x) and the teacher's
+ * p_k = exp(teacher_k / temperature - L):
+ *   loss[r] = sum_k p_k (log p_k - log q_k) + p_rest (log p_rest - log q_rest),
+ * with L = teacher_lse[r], log sum_v exp(teacher_v / temperature) over its whole
+ * vocabulary, and the tokens that are no entry (the rest) as one more class, of
+ * probability 1 - sum p; or, with teacher_lse NULL, L the entries' own and p_rest = 0.  (A
+ * teacher_lse below the entries' own counts as that, and where every token is an
+ * entry it is not read.)  A row without entries is not scored: loss 0, no gradient. A bad row has
+ * a token outside [0, vocab) or twice, or a teacher's value that is NaN or +inf: its
+ * loss is NaN, it has no gradient, and result->bad_row names the first one.
+ * result->loss is the mean over the rows with entries.  k is 1 to 1024; d, vocab and t as
+ * cfops_lm_head_logprobs's, as is keep, of cfops_lm_head_distill_keep_bytes. */
+size_t cfops_lm_head_distill_keep_bytes(size_t t, size_t d, size_t vocab, size_t k);
+int cfops_lm_head_distill(cfattn_ctx* ctx, const float* hn, const float* head, const int64_t* ids,
+                          const float* teacher, const float* teacher_lse, size_t t, size_t d, size_t vocab, size_t k,
+                          double temperature, float* loss, cfops_ce_result* result, void* keep, size_t keep_bytes,
+                          void* stream);
+/* From the gradient dloss [t] of loss: dhn [t, d] (overwritten; NULL: not wanted) and,
+ * when dhead is non-null, dhead [vocab, d] += (acc == 0: =), as
+ * cfops_lm_head_logprobs_backward; the other arguments are the forward's.  dloss of rows
+ * that are not scored, or bad, is not read. */
+int cfops_lm_head_distill_backward(cfattn_ctx* ctx, const float* hn, const float* head, const int64_t* ids,
+                                   const float* teacher, const float* teacher_lse, const float* dloss, size_t t,
+                                   size_t d, size_t vocab, size_t k, double temperature, float* dhn, float* dhead,
+                                   int acc, const void* keep, size_t keep_bytes, void* stream);
+
 /* Rows of packed sequences: sequence i is rows [offsets[i], offsets[i + 1]) of
  * logp (int64 in device memory, rising within [0, rows]).  A row whose target
  * is CFOPS_IGNORE_INDEX is not scored (targets NULL: every row is): its inputs
