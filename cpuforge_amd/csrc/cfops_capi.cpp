@@ -604,13 +604,15 @@ struct LogpRows {
     float *hn, *logits;
     size_t chunk;
 };
-int logp_rows(cfattn_ctx* c, size_t t, size_t d, size_t vocab, LogpRows& r) {
+// (all: the logits of all rows are in the caller's memory.)
+int logp_rows(cfattn_ctx* c, size_t t, size_t d, size_t vocab, LogpRows& r, bool all = false) {
     // A chunk's logits fit the head's limit, its rows a launch of workgroups.
     r.chunk = std::min<size_t>(c->head_chunk_bytes / (vocab * sizeof(float)), (size_t)1 << 22);
-    r.chunk = std::min(std::max<size_t>(r.chunk, 1), t);
+    r.chunk = all ? t : std::min(std::max<size_t>(r.chunk, 1), t);
     CF_TRY(take(c, cfattn_ctx::OPS_IDX, (4 + 2 * t) * sizeof(int), r.count));
     r.idx = r.count + 4;
     CF_TRY(take(c, cfattn_ctx::OPS_ROWS, t * d * sizeof(float), r.hn));
+    if (all) return CFATTN_OK;
     return take(c, cfattn_ctx::OPS_LOGITS, r.chunk * vocab * sizeof(float), r.logits);
 }
 
@@ -766,8 +768,8 @@ struct Distill {
 };
 struct Entries {
     int64_t* target;
-    double2* row;
-    float *z, *none;  // none: lse of the rows that are put aside
+    cfattn::TeacherRow* row;
+    float *z, *e, *none;  // none: lse of the rows that are put aside
     int *ids, *count;
     float *dl, *a;
 };
@@ -784,53 +786,106 @@ void entries_at(size_t t, size_t k, char* base, Entries& e) {
     e.a = reinterpret_cast<float*>(e.count + t);
 }
 int distill_entries(cfattn_ctx* c, const Distill& q, char* keep, Entries& e, hipStream_t st) {
-    const size_t own = align_up(q.t * sizeof(double2)) + align_up(q.t * sizeof(int64_t)) +
-                       align_up(q.t * q.k * sizeof(float)) + align_up(q.t * sizeof(float));
+    const size_t rows = align_up(q.t * sizeof(cfattn::TeacherRow)), targets = align_up(q.t * sizeof(int64_t));
+    const size_t values = align_up(q.t * q.k * sizeof(float));
+    const size_t own = rows + targets + 2 * values + align_up(q.t * sizeof(float));
     char* base = nullptr;
     CF_TRY(take(c, cfattn_ctx::OPS_ENTRIES, own + (keep ? 0 : distill_kept_bytes(q.t, q.k)), base));
-    e.row = reinterpret_cast<double2*>(base);
-    e.target = reinterpret_cast<int64_t*>(base + align_up(q.t * sizeof(double2)));
-    e.z = reinterpret_cast<float*>(reinterpret_cast<char*>(e.target) + align_up(q.t * sizeof(int64_t)));
-    e.none = reinterpret_cast<float*>(reinterpret_cast<char*>(e.z) + align_up(q.t * q.k * sizeof(float)));
+    e.row = reinterpret_cast<cfattn::TeacherRow*>(base);
+    e.target = reinterpret_cast<int64_t*>(base + rows);
+    e.z = reinterpret_cast<float*>(base + rows + targets);
+    e.e = reinterpret_cast<float*>(base + rows + targets + values);
+    e.none = reinterpret_cast<float*>(base + rows + targets + 2 * values);
     entries_at(q.t, q.k, keep ? keep : base + own, e);
     cfattn::DistillEntries g{};
     g.raw_ids = q.ids, g.teacher = q.teacher, g.teacher_lse = q.teacher_lse, g.t = (long)q.t, g.vocab = (long)q.vocab;
-    g.k = (int)q.k, g.inv_t = q.inv_t, g.ids = e.ids, g.count = e.count, g.z = e.z, g.row = e.row, g.target = e.target;
+    g.k = (int)q.k, g.inv_t = q.inv_t, g.ids = e.ids, g.count = e.count, g.z = e.z, g.e = e.e, g.row = e.row, g.target = e.target;
     CF_HIP(c, cfattn::launch_distill_entries(g, st), "distillation launch");
     return CFATTN_OK;
 }
 
-// Few rows: logits in memory, a chunk of rows at a time; the loss or (dhn or dhead) the gradients.
+// Few rows: logits in memory, a chunk of rows at a time, which become the gradients of dloss = 1; the
+// rows of dhn, and in dhead those of hn, are times theirs.  What a forward keeps is those
+// gradients of all rows.
+int distill_tag(const Distill& q) { return distill_plan(q, SIZE_MAX).tag; }
+// (Whole steps of 32 rows, as lm_head_logprobs' gradient of the head takes.)
+size_t few_padded(size_t t) { return t > 16 ? (t + 31) / 32 * 32 : t; }
+size_t few_index_bytes(size_t t) { return align_up((4 + 2 * few_padded(t)) * sizeof(int)); }
+size_t few_keep_bytes(size_t t, size_t vocab) { return few_index_bytes(t) + few_padded(t) * vocab * sizeof(float); }
+
+int distill_few_logits(cfattn_ctx* c, const Distill& q, const float* head, const Entries& e, const LogpRows& rows,
+                       size_t j0, size_t nr, float* loss, bool grad, hipStream_t st) {
+    cfattn::DistillRows g{};
+    g.ids = e.ids, g.count = e.count, g.z = e.z, g.e = e.e, g.row = e.row, g.k = (int)q.k, g.inv_t = q.inv_t;
+    g.idx = rows.idx, g.scored = rows.count, g.j0 = (int)j0, g.vocab = (long)q.vocab, g.loss = loss;
+    CF_TRY(gemm(c, CFOPS_NT, rows.hn + j0 * q.d, head, rows.logits, nr, q.d, q.vocab, false, st));
+    CF_HIP(c, cfattn::launch_distill_logits(rows.logits, nr, grad, g, st), "distillation launch");
+    return CFATTN_OK;
+}
+
 int distill_few(cfattn_ctx* c, const Distill& q, const float* hn, const float* head, float* loss, void* result,
-                const float* dloss, float* dhn, float* dhead, bool acc, hipStream_t st) {
-    const bool grad = dhn || dhead;
+                void* keep, size_t keep_bytes, hipStream_t st) {
     Entries e{};
     CF_TRY(distill_entries(c, q, nullptr, e, st));
-    // (Whole steps of 32 rows, as lm_head_logprobs' gradient of the head takes.)
-    const size_t padded = dhead && q.t > 16 ? (q.t + 31) / 32 * 32 : q.t;
+    const size_t padded = few_padded(q.t);
     LogpRows rows{};
-    CF_TRY(logp_rows(c, padded, q.d, q.vocab, rows));
-    CF_HIP(c, cfattn::launch_logp_select(e.target, q.t, q.vocab, rows.idx, rows.count, 0, loss, e.none, result, st),
+    CF_TRY(logp_rows(c, padded, q.d, q.vocab, rows, keep != nullptr));
+    if (keep) {
+        CF_TRY(check_keep(c, keep, keep_bytes, few_keep_bytes(q.t, q.vocab)));
+        rows.count = static_cast<int*>(keep);
+        rows.idx = rows.count + 4;
+        rows.logits = reinterpret_cast<float*>(static_cast<char*>(keep) + few_index_bytes(q.t));
+    }
+    CF_HIP(c, cfattn::launch_logp_select(e.target, q.t, q.vocab, rows.idx, rows.count, distill_tag(q), loss, e.none,
+                                         result, st),
            "distillation launch");
-    CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, rows.idx, rows.count, rows.hn, padded, q.d, st),
+    CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, nullptr, rows.idx, rows.count, distill_tag(q), rows.hn, padded, q.d,
+                                         st),
            "distillation launch");
-    cfattn::DistillRows g{};
-    g.ids = e.ids, g.count = e.count, g.z = e.z, g.row = e.row, g.k = (int)q.k, g.inv_t = q.inv_t;
-    g.idx = rows.idx, g.scored = rows.count, g.vocab = (long)q.vocab, g.dloss = dloss, g.loss = loss;
+    const size_t all = keep ? padded : q.t;
+    for (size_t j0 = 0; j0 < all; j0 += rows.chunk)
+        CF_TRY(distill_few_logits(c, q, head, e, rows, j0, std::min(all - j0, rows.chunk), loss, keep != nullptr, st));
+    CF_HIP(c, cfattn::launch_logp_finish(e.target, loss, 1.0, q.t, result, st), "distillation launch");
+    return CFATTN_OK;
+}
+
+int distill_backward_few(cfattn_ctx* c, const Distill& q, const float* hn, const float* head, const float* dloss,
+                         float* dhn, float* dhead, bool acc, const void* keep, size_t keep_bytes, hipStream_t st) {
+    const size_t padded = dhead ? few_padded(q.t) : q.t;
+    const int tag = distill_tag(q);
+    Entries e{};
+    LogpRows rows{};
+    CF_TRY(logp_rows(c, padded, q.d, q.vocab, rows, keep != nullptr));
+    if (keep) {
+        CF_TRY(check_keep(c, keep, keep_bytes, few_keep_bytes(q.t, q.vocab)));
+        rows.count = static_cast<int*>(const_cast<void*>(keep));
+        rows.idx = rows.count + 4;
+        rows.logits = reinterpret_cast<float*>(static_cast<char*>(const_cast<void*>(keep)) + few_index_bytes(q.t));
+    } else {
+        CF_TRY(distill_entries(c, q, nullptr, e, st));
+        CF_HIP(c, cfattn::launch_logp_select(e.target, q.t, q.vocab, rows.idx, rows.count, tag, nullptr, nullptr,
+                                             nullptr, st),
+               "distillation launch");
+        CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, nullptr, rows.idx, rows.count, tag, rows.hn, padded, q.d, st),
+               "distillation launch");
+    }
+    float *scaled = nullptr, *sums = nullptr;  // rows of hn times dloss, and of dhn before it
+    if (dhead) {
+        CF_TRY(take(c, cfattn_ctx::OPS_ROWS_BACK, padded * q.d * sizeof(float), scaled));
+        CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, dloss, rows.idx, rows.count, tag, scaled, padded, q.d, st),
+               "distillation launch");
+    }
+    if (dhn) CF_TRY(take(c, cfattn_ctx::OPS_PART, padded * q.d * sizeof(float), sums));
     for (size_t j0 = 0; j0 < padded; j0 += rows.chunk) {
         const size_t nr = std::min(padded - j0, rows.chunk);
-        float* h = rows.hn + j0 * q.d;
-        g.j0 = (int)j0;
-        CF_TRY(gemm(c, CFOPS_NT, h, head, rows.logits, nr, q.d, q.vocab, false, st));
-        CF_HIP(c, cfattn::launch_distill_logits(rows.logits, nr, grad, g, st), "distillation launch");
-        if (dhead) CF_TRY(gemm(c, CFOPS_TN, rows.logits, h, dhead, q.vocab, nr, q.d, acc || j0, st));
-        if (dhn) CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, h, nr, q.vocab, q.d, false, st));
+        if (!keep) CF_TRY(distill_few_logits(c, q, head, e, rows, j0, nr, nullptr, true, st));
+        if (dhead)
+            CF_TRY(gemm(c, CFOPS_TN, rows.logits, scaled + j0 * q.d, dhead, q.vocab, nr, q.d, acc || j0, st));
+        if (dhn) CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, sums + j0 * q.d, nr, q.vocab, q.d, false, st));
     }
     if (dhn)
-        CF_HIP(c, cfattn::launch_logp_scatter(rows.hn, q.mul, rows.idx, rows.count, dhn, q.t, q.d, st),
+        CF_HIP(c, cfattn::launch_logp_scatter(sums, q.mul, dloss, rows.idx, rows.count, tag, dhn, q.t, q.d, st),
                "distillation launch");
-    if (!grad)
-        CF_HIP(c, cfattn::launch_logp_finish(e.target, loss, 1.0, q.t, result, st), "distillation launch");
     return CFATTN_OK;
 }
 
@@ -841,7 +896,7 @@ int distill_rows(cfattn_ctx* c, const Distill& q, const cfattn::HeadPlan& p, con
                  hipStream_t st) {
     CF_HIP(c, cfattn::launch_head_stats(p, b, q.t, j0, q.vocab, nullptr, nullptr, st), "distillation launch");
     cfattn::DistillKept g{};
-    g.ids = e.ids, g.count = e.count, g.z = e.z, g.row = e.row, g.k = (int)q.k, g.inv_t = q.inv_t;
+    g.ids = e.ids, g.count = e.count, g.z = e.z, g.e = e.e, g.row = e.row, g.k = (int)q.k, g.inv_t = q.inv_t;
     g.idx = b.idx, g.scored = b.count, g.tag = p.tag, g.j0 = (int)j0, g.chunk = (int)p.chunk;
     g.parts = (int)((q.vocab + 127) / 128), g.vocab = (int)q.vocab, g.v16 = (int)(p.v_pad / 16), g.d = (int)q.d;
     g.ld = (long)p.chunk, g.stats = static_cast<const float2*>(b.stats), g.keep = b.keep, g.factor = b.factor;
@@ -1019,7 +1074,7 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
     CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, 0, nullptr, nullptr, nullptr,
                                               st),
            "log-probability launch");
-    CF_HIP(c, cfattn::launch_logp_gather(hn, 1.0f, rows.idx, rows.count, rows.hn, padded, d, st), "log-probability launch");
+    CF_HIP(c, cfattn::launch_logp_gather(hn, 1.0f, nullptr, rows.idx, rows.count, 0, rows.hn, padded, d, st), "log-probability launch");
     for (size_t j0 = 0; j0 < padded; j0 += rows.chunk) {
         const size_t nr = std::min(padded - j0, rows.chunk);
         float* h = rows.hn + j0 * d;
@@ -1031,14 +1086,16 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
         if (dhn) CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, h, nr, vocab, d, false, st));
     }
     if (dhn)
-        CF_HIP(c, cfattn::launch_logp_scatter(rows.hn, 1.0f, rows.idx, rows.count, dhn, t, d, st), "log-probability launch");
+        CF_HIP(c, cfattn::launch_logp_scatter(rows.hn, 1.0f, nullptr, rows.idx, rows.count, 0, dhn, t, d, st), "log-probability launch");
     return CFATTN_OK;
 }
 
 size_t cfops_lm_head_distill_keep_bytes(size_t t, size_t d, size_t vocab, size_t k) {
-    const size_t products = cfops_lm_head_logprobs_keep_bytes(t, d, vocab);
-    if (products == 0 || k == 0 || k > cfattn::kDistillMost) return 0;
-    return products + distill_kept_bytes(t, k);
+    if (t == 0 || t >= (size_t)1 << 24 || d == 0 || vocab == 0 || !fits_int(d) || vocab >= (size_t)1 << 26 || k == 0 ||
+        k > cfattn::kDistillMost)
+        return 0;
+    if (t <= cfattn::kLogpUnkept) return few_keep_bytes(t, vocab);
+    return keep_layout(cfattn::head_plan(t, d, vocab, SIZE_MAX), t).bytes + distill_kept_bytes(t, k);
 }
 
 int cfops_lm_head_distill(cfattn_ctx* c, const float* hn, const float* head, const int64_t* ids, const float* teacher,
@@ -1055,7 +1112,7 @@ int cfops_lm_head_distill(cfattn_ctx* c, const float* hn, const float* head, con
         return CFATTN_OK;
     }
     if (t <= cfattn::kLogpUnkept)
-        return distill_few(c, q, hn, head, loss, result, nullptr, nullptr, nullptr, false, st);
+        return distill_few(c, q, hn, head, loss, result, keep, keep_bytes, st);
     return distill_many(c, q, hn, head, loss, result, keep, keep_bytes, st);
 }
 
@@ -1071,7 +1128,7 @@ int cfops_lm_head_distill_backward(cfattn_ctx* c, const float* hn, const float* 
     if (!hn || !head || !ids || !teacher || !dloss) return fail(c, CFATTN_ERR_ARG, "null buffer");
     const hipStream_t st = to_stream(stream);
     if (t <= cfattn::kLogpUnkept)
-        return distill_few(c, q, hn, head, nullptr, nullptr, dloss, dhn, dhead, acc != 0, st);
+        return distill_backward_few(c, q, hn, head, dloss, dhn, dhead, acc != 0, keep, keep_bytes, st);
     return distill_backward_many(c, q, hn, head, dloss, dhn, dhead, acc != 0, keep, keep_bytes, st);
 }
 

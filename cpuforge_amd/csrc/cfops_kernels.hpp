@@ -227,15 +227,16 @@ hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st);
 //   select:    idx and, from idx + rows on, their targets; count[0], tag in count[1]; the
 //              result block (CeMisc; or null), and logp
 //              and lse (or null) of the rows that are not scored;
-//   gather:    the scored rows of hn side by side, times mul;   scatter: back, other rows 0;
+//   gather:    the scored rows of hn side by side, times mul and the row's `by` (or null);
+//   scatter:   back, other rows 0; either gives NaN where the tag is another;
 //   grad_rows: the logits become their gradients;
 //   finish:    the mean of sign logp, summed in f64 in a fixed order.
 hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, int tag,
                               float* logp, float* lse, void* misc, hipStream_t st);
-hipError_t launch_logp_gather(const float* hn, float mul, const int* idx, const int* count, float* out, size_t rows,
-                              size_t d, hipStream_t st);
-hipError_t launch_logp_scatter(const float* in, float mul, const int* idx, const int* count, float* dhn, size_t rows,
-                               size_t d, hipStream_t st);
+hipError_t launch_logp_gather(const float* hn, float mul, const float* by, const int* idx, const int* count, int tag,
+                              float* out, size_t rows, size_t d, hipStream_t st);
+hipError_t launch_logp_scatter(const float* in, float mul, const float* by, const int* idx, const int* count, int tag,
+                               float* dhn, size_t rows, size_t d, hipStream_t st);
 hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const int* idx, const int* count,
                                  const float* lse, const float* dlogp, size_t j0, size_t nrows, size_t vocab,
                                  hipStream_t st);
@@ -293,10 +294,10 @@ struct HeadBuffers {
     void* stats;
     float mul = 1.0f;                    // of hn
 };
-// In a target's place k entries of each row (distill.hip), whose kept exponentials are zeros: dlogits
-// are dloss (a q_v + dl of the entry that v is); dhn is times mul.
+// In a target's place up to k entries of each row (distill.hip), whose kept exponentials are zeros:
+// dlogits are dloss (a q_v + dl of the entry that v is); dhn is times mul.
 struct HeadEntries {
-    const int *ids, *count;  // [t][k] rising, and how many
+    const int *ids, *count;  // [t][k], and how many
     const float *dl, *a;     // [t][k], [t]
     int k;
 };
@@ -321,6 +322,9 @@ hipError_t launch_head_zero_rows(const HeadPlan& p, const HeadBuffers& b, size_t
 // takes rows (kept, of which the head's products kept statistics and exponentials) or puts
 // them aside; logits: the scored rows [j0, j0 + nrows), whose logits are in memory.
 constexpr size_t kDistillMost = 1024;  // entries of a row
+struct TeacherRow {
+    double l, p_rest, scale;  // the log-sum-exp that it takes, p_rest (negative: no rest), p / e
+};
 struct DistillEntries {
     const int64_t* raw_ids;
     const float *teacher, *teacher_lse;  // teacher_lse may be null
@@ -328,15 +332,15 @@ struct DistillEntries {
     int k;
     double inv_t;
     int *ids, *count;  // [t][k], [t]
-    float* z;          // [t][k]
-    double2* row;      // [t]: the entries' log-sum-exp or the teacher's, p_rest (negative: no rest)
+    float *z, *e;      // [t][k]: logits, exp((z - the row's largest) inv_t)
+    TeacherRow* row;   // [t]
     int64_t* target;   // [t]
 };
 hipError_t launch_distill_entries(const DistillEntries& g, hipStream_t st);
 struct DistillKept {
-    const int *ids, *count;
-    const float* z;
-    const double2* row;
+    int *ids, *count;  // with dl and a, left as those of HeadEntries
+    const float *z, *e;
+    const TeacherRow* row;
     int k;
     double inv_t;
     const int *idx, *scored;  // scored rows, how many and the plan's tag
@@ -352,15 +356,14 @@ struct DistillKept {
 hipError_t launch_distill_kept(const DistillKept& g, hipStream_t st);
 struct DistillRows {
     const int *ids, *count;
-    const float* z;
-    const double2* row;
+    const float *z, *e;
+    const TeacherRow* row;
     int k;
     double inv_t;
     const int *idx, *scored;
     int j0;
     long vocab;
-    const float* dloss;  // grad
-    float* loss;         // else
+    float* loss;  // may be null
 };
 hipError_t launch_distill_logits(float* logits, size_t nrows, bool grad, const DistillRows& g, hipStream_t st);
 

@@ -31,8 +31,8 @@ __device__ __forceinline__ float max_wave(float x) {
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
-// A row's entries by rising token, a wave to a row: ids and z [t][k] (count of them), L and
-// p_rest (negative: no rest); target is a token of the row, kIgnoreIndex without entries, -1 where
+// A row's entries by rising token, a wave to a row: ids, z and e [t][k] (count of them), their
+// exponentials below the largest's; the row's L, p_rest (negative: no rest) and p / e; target is a token of the row, kIgnoreIndex without entries, -1 where
 // the row is bad: a token out of the vocabulary or named twice, or a value of the teacher's that
 // is not finite.  (An entry whose id is kIgnoreIndex or whose logit is -inf is not there.)
 // Places are counts of smaller tokens: 4096 x 64 entries TODO us.
@@ -79,9 +79,11 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const DistillEntri
         if (v == INT_MAX) continue;
         // (Twice the same token: two entries in one place, of which nothing is read.)
         g.ids[r * g.k + place] = v;
+        const double e = exp(((double)z[k] - (double)top) * g.inv_t);
         g.z[r * g.k + place] = z[k];
+        g.e[r * g.k + place] = (float)e;
         least = min(least, v);
-        sum += exp(((double)z[k] - (double)top) * g.inv_t);
+        sum += e;
     }
     sum = sum_wave(sum);
 #pragma unroll
@@ -97,7 +99,7 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const DistillEntri
     const bool any_bad = __any(bad);
     if (lane) return;
     g.count[r] = any_bad ? 0 : n;
-    g.row[r] = make_double2(whole, p_rest);
+    g.row[r] = {whole, p_rest, exp(own - whole) / sum};
     g.target[r] = any_bad ? -1 : n == 0 ? kIgnoreIndex : least;
 }
 
@@ -114,29 +116,37 @@ __device__ __forceinline__ int lower_bound(const int* tokens, int n, int v) {
     return lo;
 }
 
-// What the entries and the rest make of a row, given the logarithms of its probabilities.
-struct RowLoss {
-    double l, p_rest, loss, ratio;  // ratio: p_rest / q_rest
-    __device__ __forceinline__ RowLoss(double2 row, double log_q_rest) : l(row.x), p_rest(row.y), loss(0.0), ratio(0.0) {
+// What the rest makes of a row's loss, given the logarithm of its probability.
+struct Rest {
+    double loss = 0.0, ratio = 0.0;  // ratio: p_rest / q_rest
+    __device__ __forceinline__ Rest(double p_rest, double log_q_rest) {
         if (!(p_rest > 0.0)) return;
         const double log_p = log(p_rest);
         loss = p_rest * (log_p - log_q_rest);
         ratio = exp(log_p - log_q_rest);
     }
-    // An entry's part, and in dl the gradient of its logit.
-    __device__ __forceinline__ double entry(double z, double log_q, double inv_t, double& dl) const {
-        const double log_p = z * inv_t - l, p = exp(log_p);
-        dl = exp(log_q) - p;
-        return p * (log_p - log_q);
-    }
 };
+// An entry's part of the loss, and in dl the gradient of its logit.
+__device__ __forceinline__ double entry_loss(const TeacherRow& row, float z, float e, double inv_t, double q,
+                                             double log_q, double& dl) {
+    const double p = (double)e * row.scale;
+    dl = q - p;
+    return p * ((double)z * inv_t - row.l - log_q);
+}
+
+// 2^x; the f32 instruction where f32 holds it.
+__device__ __forceinline__ double pow2(double x) { return x > -120.0 ? (double)__builtin_amdgcn_exp2f((float)x) : exp2(x); }
 
 // Rows whose product kept exp2(y - m) of 128 logits each (y in units of log2, m the largest):
 // a wave to a row, 8 rows to a workgroup.  An entry whose exponential is too small, and
 // a rest of 128 that is, are formed again from hidden state and head.  Where the entries hold
-// all but little of such 128, the rest of them is summed, not left over.  For the gradients the
-// entries' exponentials become zeros: they have gradients of their own (dl), and a
-// confident student's a q would cancel in them (a is -p_rest / q_rest then).
+// all but little of such 128, the rest of them is summed, not left over.
+//
+// For the gradients an entry's exponential becomes what the product has to find there for its
+// own gradient, dl / (a factor), so that the product adds it up with the others'; where that is
+// much larger than its 128's largest (a near 0, a student that holds the token for unlikely), or
+// the rest is far below the entry, it becomes 0 and the entry stays in ids and dl (count of them).
+// (A sure student's a q would cancel in the entries: a is -p_rest / q_rest then.)
 // 3686 rows of 64 entries, 49152 tokens: TODO us, latency.
 __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) {
     extern __shared__ int tokens[];  // [8][k]
@@ -149,14 +159,18 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
     int* mine = tokens + wave * g.k;
     for (int k = lane; k < n; k += 64) mine[k] = g.ids[r * g.k + k];
     __builtin_amdgcn_wave_barrier();
-    const double2 row = g.row[r];
-    const bool with_rest = row.y > 0.0;
+    const TeacherRow row = g.row[r];
+    const bool with_rest = row.p_rest > 0.0;
     auto kept = [&](int v) -> float& {
         char* p = g.keep + ((long)(j / 32) * g.v16 + v / 32 * 2) * 2048 + v % 32 / 8 * 1024 +
-                        ((v % 8 / 4) * 32 + j % 32) * 16;
+                  ((v % 8 / 4) * 32 + j % 32) * 16;
         return reinterpret_cast<float*>(p)[v % 4];
     };
     auto stat = [&](int part) { return g.stats[(long)part * g.ld + j]; };
+    auto has_entry = [&](int part) {
+        const int at = lower_bound(mine, n, part * 128);
+        return at < n && mine[at] < part * 128 + 128;
+    };
     // A logit in units of log2, by the whole wave.
     auto logit = [&](int v) {
         const float *h = g.hn + r * g.d, *w = g.head + (long)v * g.d;
@@ -164,18 +178,20 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
         for (int i = lane; i < g.d; i += 64) s += (double)(h[i] * g.mul) * (double)w[i];
         return sum_wave(s) * (double)kLog2e;
     };
-    float m = -INFINITY;
-    for (int p = lane; p < g.parts; p += 64) m = fmaxf(m, stat(p).x);
+    float m = -INFINITY, m_rest = -INFINITY;
+    for (int p = lane; p < g.parts; p += 64) {
+        const float x = stat(p).x;
+        m = fmaxf(m, x);
+        if (with_rest && !has_entry(p)) m_rest = fmaxf(m_rest, x);
+    }
     m = max_wave(m);
+    m_rest = max_wave(m_rest);
     const double top = (double)m;
-    double total = 0.0, rest = 0.0;
+    double total = 0.0, rest = 0.0;  // in units of 2^top
     for (int p = lane; p < g.parts; p += 64) {
         const float2 s = stat(p);
-        const double w = s.y == 0.0f ? 0.0 : (double)s.y * exp2((double)s.x - top);
-        total += w;
-        if (!with_rest) continue;
-        const int at = lower_bound(mine, n, p * 128);
-        if (at == n || mine[at] >= p * 128 + 128) rest += w;
+        total += (double)(s.y * __builtin_amdgcn_exp2f(s.x - m));
+        if (with_rest && !has_entry(p)) rest += (double)(s.y * __builtin_amdgcn_exp2f(s.x - m_rest));
     }
     total = sum_wave(total);
     constexpr float kLost = 0x1p-100f;  // of a kept exponential
@@ -197,6 +213,7 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
     auto is_first = [&](int k) { return k < n && (k == 0 || mine[k - 1] / 128 != mine[k] / 128); };
     if (with_rest) {
         rest = sum_wave(rest);
+        if (rest > 0.0) rest *= exp2((double)m_rest - top);
         // The 128s that have entries, by their first: what is left of their sums, then, where that
         // is not exact enough, the sum of the others.
         double left = 0.0;
@@ -205,7 +222,7 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
             const float2 s = stat(part);
             double x = (double)s.y;
             for (int i = k; i < n && mine[i] / 128 == part; i++) x -= (double)kept(mine[i]);
-            const double scale = exp2((double)s.x - top);
+            const double scale = pow2((double)s.x - top);
             size = (double)s.y * scale;
             return fmax(x, 0.0) * scale;
         };
@@ -246,56 +263,70 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
         rest += sum_wave(left);
     }
     const double log_total = log(total), unit = 1.0 / (double)kLog2e;
-    RowLoss loss(row, log(rest) - log_total);
+    const Rest r_(row.p_rest, log(rest) - log_total);
+    // (A rest so small has no exponentials in f32 either.)
+    const float a = (float)(1.0 - fmin(r_.ratio, 1e30));
     double terms = 0.0;
+    int stay = 0;
     for (int k0 = 0; k0 < n; k0 += 64) {
         const int k = k0 + lane;
         const bool live = k < n;
         const int v = live ? mine[k] : 0;
         const float e = live ? kept(v) : 1.0f;
-        double y = live ? log2((double)e) + (double)stat(v / 128).x : 0.0;
+        const double up = live ? (double)stat(v / 128).x - top : 0.0;
+        double y = log2((double)e) + up, q = (double)e * pow2(up) / total;
         for (unsigned long long todo = __ballot(live && e < kLost); todo; todo &= todo - 1) {
             const int at = __ffsll(todo) - 1;
-            const double x = logit(mine[k0 + at]);
-            if (lane == at) y = x;
+            const double x = logit(mine[k0 + at]) - top;
+            if (lane == at) y = x, q = exp2(x) / total;
         }
-        if (!live) continue;
-        double dl;
-        terms += loss.entry((double)g.z[r * g.k + k], (y - top) * unit - log_total, g.inv_t, dl);
-        if (g.dl) {
-            g.dl[r * g.k + k] = (float)dl;
-            kept(v) = 0.0f;
+        double dl = 0.0;
+        if (live)
+            terms += entry_loss(row, g.z[r * g.k + k], g.e[r * g.k + k], g.inv_t, q, y * unit - log_total, dl);
+        if (!g.dl) continue;
+        const bool far = with_rest && pow2(up) * 0x1p-10 > rest;
+        const float in = live ? (float)dl / (a * g.factor[(long)(v / 128) * g.ld + j]) : 0.0f;
+        // (Up to 2 the product's f16 pieces hold it.)
+        const bool stays = live && (far || !(fabsf(in) <= 1.5f));
+        const unsigned long long staying = __ballot(stays);
+        if (stays) {
+            const int to = stay + __popcll(staying & ((1ull << lane) - 1));
+            g.ids[r * g.k + to] = v;
+            g.dl[r * g.k + to] = (float)dl;
         }
+        if (live) kept(v) = stays ? 0.0f : in;
+        stay += __popcll(staying);
     }
     terms = sum_wave(terms);
     // The gradient's product takes a kept value to 2^-36: where an entry lies so far above the rest
     // that this shows in a q, the others of its 128 are scaled up.
     for (int k0 = 0; g.dl && with_rest && k0 < n; k0 += 64) {
         const int k = k0 + lane;
-        const bool far = is_first(k) && exp2((double)stat(mine[k] / 128).x - top) * 0x1p-10 > rest;
+        const bool far = is_first(k) && pow2((double)stat(mine[k] / 128).x - top) * 0x1p-10 > rest;
         for (unsigned long long todo = __ballot(far); todo; todo &= todo - 1) {
             const int at = k0 + __ffsll(todo) - 1, part = mine[at] / 128;
             float x4[4];
             others(at, x4);
             const float most = max_wave(fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])));
-            const int e = min(max(127 - (int)(__builtin_bit_cast(uint32_t, most) >> 23), 0), 126);
-            if (!(most > 0.0f) || e == 0) continue;
-            const float up = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+            const int up = min(max(127 - (int)(__builtin_bit_cast(uint32_t, most) >> 23), 0), 126);
+            if (!(most > 0.0f) || up == 0) continue;
+            const float times = __builtin_bit_cast(float, (uint32_t)(127 + up) << 23);
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if (lane < 32 && part * 128 + v4 + i < g.vocab) kept(part * 128 + v4 + i) = x4[i] * up;
-            if (lane == 0) g.factor[(long)part * g.ld + j] *= __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+                if (lane < 32 && part * 128 + v4 + i < g.vocab) kept(part * 128 + v4 + i) = x4[i] * times;
+            if (lane == 0) g.factor[(long)part * g.ld + j] *= __builtin_bit_cast(float, (uint32_t)(127 - up) << 23);
         }
     }
     if (lane) return;
-    if (g.loss) g.loss[r] = (float)(loss.loss + terms);
-    // (A rest so small has no exponentials in f32 either.)
-    if (g.a) g.a[r] = (float)(1.0 - fmin(loss.ratio, 1e30));
+    if (g.loss) g.loss[r] = (float)(r_.loss + terms);
+    if (!g.dl) return;
+    g.a[r] = a;
+    g.count[r] = stay;
 }
 
-// Rows of logits in memory, a workgroup to one; with GRAD they become their gradients (zeros from
-// the last scored row on), else loss is written.  The entries are taken out of the row before its
-// sum, so the rest is one of its own.
+// Rows of logits in memory, a workgroup to one: the loss, where it is wanted, and with GRAD the
+// logits become their gradients (zeros from the last scored row on).  The entries are taken out
+// of the row before its sum, so the rest is one of its own.
 template <bool GRAD>
 __global__ __launch_bounds__(512) void distill_logits_kernel(float* __restrict__ logits, const DistillRows g) {
     extern __shared__ char lds[];
@@ -344,26 +375,29 @@ __global__ __launch_bounds__(512) void distill_logits_kernel(float* __restrict__
     for (int k = lane; k < n; k += 64) named += exp((double)xs[k] - (double)top);
     const double shift = rest > 0.0 ? (double)m - (double)top : 0.0;
     const double total = sum_wave(named) + rest * exp(shift), log_total = log(total);
-    RowLoss loss(g.row[r], log(rest) + shift - log_total);
-    if (!GRAD) {
-        if (wave) return;
+    const TeacherRow row = g.row[r];
+    const Rest r_(row.p_rest, log(rest) + shift - log_total);
+    // An entry's part of the loss, and in dl the gradient of its logit.
+    auto entry = [&](int k, double& dl) {
+        const double log_q = (double)xs[k] - (double)top - log_total;
+        return entry_loss(row, g.z[r * g.k + k], g.e[r * g.k + k], g.inv_t, exp(log_q), log_q, dl);
+    };
+    if (g.loss && wave == 0) {
         double terms = 0.0, dl;
-        for (int k = lane; k < n; k += 64)
-            terms += loss.entry((double)g.z[r * g.k + k], (double)xs[k] - (double)top - log_total, g.inv_t, dl);
+        for (int k = lane; k < n; k += 64) terms += entry(k, dl);
         terms = sum_wave(terms);
-        if (lane == 0) g.loss[r] = (float)(loss.loss + terms);
-        return;
+        if (lane == 0) g.loss[r] = (float)(r_.loss + terms);
     }
-    const double dloss = (double)g.dloss[r];
+    if (!GRAD) return;
     // (By the rest's own largest: a q of a confident student's is not small where q is.)
-    const float f = (float)(dloss * (1.0 - loss.ratio) * exp(shift) / total), base = m > -INFINITY ? m : 0.0f;
+    const float f = (float)((1.0 - r_.ratio) * exp(shift) / total), base = m > -INFINITY ? m : 0.0f;
 #pragma unroll 4
     for (long i = threadIdx.x; i < g.vocab; i += 512) x[i] = f * expf(x[i] - base);
     __syncthreads();
     for (int k = threadIdx.x; k < n; k += 512) {
         double dl;
-        loss.entry((double)g.z[r * g.k + k], (double)xs[k] - (double)top - log_total, g.inv_t, dl);
-        x[tokens[k]] = (float)(dloss * dl);
+        entry(k, dl);
+        x[tokens[k]] = (float)dl;
     }
 }
 

@@ -76,21 +76,27 @@ __global__ __launch_bounds__(1024) void logp_select_kernel(const int64_t* __rest
     }
 }
 
-// out[j] = mul hn[idx[j]], zeros from row n on.
+// out[j] = mul by[r] hn[r], r = idx[j], zeros from row n on (by null: 1).
 __global__ __launch_bounds__(256) void logp_gather_kernel(const float* __restrict__ hn, float mul,
-                                                          const int* __restrict__ idx, const int* __restrict__ count,
+                                                          const float* __restrict__ by, const int* __restrict__ idx,
+                                                          const int* __restrict__ count, int tag,
                                                           float* __restrict__ out, long d) {
     const long j = blockIdx.x;
-    const float* x = j < *count ? hn + (long)idx[j] * d : nullptr;
-    for (long i = threadIdx.x; i < d; i += 256) out[j * d + i] = x ? mul * x[i] : 0.0f;
+    const bool known = count[1] == tag;
+    const int r = known && j < *count ? idx[j] : -1;
+    const float* x = r >= 0 ? hn + (long)r * d : nullptr;
+    const float f = x && by ? mul * by[r] : mul, none = known ? 0.0f : __builtin_nanf("");
+    for (long i = threadIdx.x; i < d; i += 256) out[j * d + i] = x ? f * x[i] : none;
 }
 
-// dhn[idx[j]] = mul in[j] for j < n, the other rows zeros.
+// dhn[idx[j]] = mul by in[j] for j < n, the other rows zeros.
 __global__ __launch_bounds__(256) void logp_scatter_kernel(const float* __restrict__ in, float mul,
-                                                           const int* __restrict__ idx, const int* __restrict__ count,
+                                                           const float* __restrict__ by, const int* __restrict__ idx,
+                                                           const int* __restrict__ count, int tag,
                                                            float* __restrict__ dhn, long d) {
     // The place of row blockIdx.x among the ascending idx.
-    const int r = blockIdx.x, n = *count;
+    const bool known = count[1] == tag;
+    const int r = blockIdx.x, n = known ? *count : 0;
     int lo = 0, hi = n;
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
@@ -100,7 +106,8 @@ __global__ __launch_bounds__(256) void logp_scatter_kernel(const float* __restri
             hi = mid;
     }
     const float* x = lo < n && idx[lo] == r ? in + (long)lo * d : nullptr;
-    for (long i = threadIdx.x; i < d; i += 256) dhn[r * d + i] = x ? mul * x[i] : 0.0f;
+    const float f = x && by ? mul * by[r] : mul, none = known ? 0.0f : __builtin_nanf("");
+    for (long i = threadIdx.x; i < d; i += 256) dhn[r * d + i] = x ? f * x[i] : none;
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -296,14 +303,16 @@ hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab,
                        tag, logp, lse, static_cast<CeMisc*>(misc));
     return hipGetLastError();
 }
-hipError_t launch_logp_gather(const float* hn, float mul, const int* idx, const int* count, float* out, size_t rows,
-                              size_t d, hipStream_t st) {
-    hipLaunchKernelGGL(logp_gather_kernel, dim3((unsigned)rows), dim3(256), 0, st, hn, mul, idx, count, out, (long)d);
+hipError_t launch_logp_gather(const float* hn, float mul, const float* by, const int* idx, const int* count, int tag,
+                              float* out, size_t rows, size_t d, hipStream_t st) {
+    hipLaunchKernelGGL(logp_gather_kernel, dim3((unsigned)rows), dim3(256), 0, st, hn, mul, by, idx, count, tag, out,
+                       (long)d);
     return hipGetLastError();
 }
-hipError_t launch_logp_scatter(const float* in, float mul, const int* idx, const int* count, float* dhn, size_t rows,
-                               size_t d, hipStream_t st) {
-    hipLaunchKernelGGL(logp_scatter_kernel, dim3((unsigned)rows), dim3(256), 0, st, in, mul, idx, count, dhn, (long)d);
+hipError_t launch_logp_scatter(const float* in, float mul, const float* by, const int* idx, const int* count, int tag,
+                               float* dhn, size_t rows, size_t d, hipStream_t st) {
+    hipLaunchKernelGGL(logp_scatter_kernel, dim3((unsigned)rows), dim3(256), 0, st, in, mul, by, idx, count, tag, dhn,
+                       (long)d);
     return hipGetLastError();
 }
 size_t logp_few_bytes(size_t t, size_t vocab) {

@@ -482,7 +482,7 @@ def _distill(hn, head, ids, teacher, lse, t, d, vocab, k, ctx):
 
 
 def lm_head_distill_keep_bytes(t: int, d: int, vocab: int, k: int) -> int:
-    """Size of lm_head_distill's keep, 0 where it uses none."""
+    """Size of lm_head_distill's keep."""
     return _lib.lib().cfops_lm_head_distill_keep_bytes(int(t), int(d), int(vocab), int(k))
 
 

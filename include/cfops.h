@@ -255,7 +255,8 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* ctx, const float* hn, const floa
  * a token outside [0, vocab) or twice, or a teacher's value that is NaN or +inf: its
  * loss is NaN, it has no gradient, and result->bad_row names the first one.
  * result->loss is the mean over the rows with entries.  k is 1 to 1024; d, vocab and t as
- * cfops_lm_head_logprobs's, as is keep, of cfops_lm_head_distill_keep_bytes. */
+ * cfops_lm_head_logprobs's, as is keep, of cfops_lm_head_distill_keep_bytes (few rows:
+ * 4 t vocab, the logits' gradients). */
 size_t cfops_lm_head_distill_keep_bytes(size_t t, size_t d, size_t vocab, size_t k);
 int cfops_lm_head_distill(cfattn_ctx* ctx, const float* hn, const float* head, const int64_t* ids,
                           const float* teacher, const float* teacher_lse, size_t t, size_t d, size_t vocab, size_t k,

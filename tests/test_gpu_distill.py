@@ -107,8 +107,6 @@ def forward(hn, head, ids, z, lse, temp, keep=None):
 
 def kept(hn, head, ids, z, lse, temp):
     n = P.lm_head_distill_keep_bytes(*hn.shape, head.shape[0], ids.shape[1])
-    if n == 0:
-        return None
     keep = torch.full((n + 64,), 255, dtype=torch.uint8, device=DEV)
     loss, _ = forward(hn, head, ids, z, lse, temp, keep[:n])
     assert bool((keep[n:] == 255).all())
@@ -138,9 +136,8 @@ def check(hn, head, ids, z, lse, temp, dloss):
     mean = float(w.loss.sum()) / max(n, 1)
     assert abs(float(P.ce_result_loss(res)) - mean) <= float(w.tol_loss.max()) + 2 * U * abs(mean)
     k = kept(hn, head, ids, z, lse, temp)
-    if k is not None:
-        assert torch.equal(k[1], loss)  # (the same products, whether or not they are kept)
-    for keep in (None,) if k is None else (None, k[0]):
+    assert torch.equal(k[1], loss)  # (the same products, whether or not they are kept)
+    for keep in (None, k[0]):
         dhn, dhead = backward(hn, head, ids, z, lse, temp, dloss, keep)
         near(dhn, w.dhn, w.tol_dhn, "dhn")
         assert not dhn[~w.use].any()
@@ -271,7 +268,7 @@ def test_bad_rows(t):
     assert torch.equal(loss[rest], want[rest]) and bool(torch.isfinite(loss[17]))
     dloss[bad] = float("nan")  # (not read)
     keep = kept(hn, head, ids, z, lse, 1.0)
-    for k in (None,) if keep is None else (None, keep[0]):
+    for k in (None, keep[0]):
         dhn, dhead = backward(hn, head, ids, z, lse, 1.0, dloss, k)
         assert not dhn[bad].any() and not dhn[15:17].any() and bool(torch.isfinite(dhead).all())
         off = (dhn[rest] - g_want[rest]).abs()
@@ -290,7 +287,7 @@ def test_rows_that_are_not_finite_stay_alone(t):
     rest = [i for i in range(t) if i not in (2, 4)]
     assert torch.equal(loss[rest], want[rest]) and bool(torch.isnan(loss[[2, 4]]).all())
     keep = kept(hn, head, ids, z, lse, 1.0)
-    for k in (None,) if keep is None else (None, keep[0]):
+    for k in (None, keep[0]):
         dhn, _ = backward(hn, head, ids, z, lse, 1.0, dloss, k, want_head=False)
         assert torch.equal(dhn[rest], g_want[rest])
 
@@ -332,19 +329,23 @@ def test_chunks_of_rows():
         assert bool(((x - y).abs() <= 2.0 ** -20 * x.abs().max()).all())
 
 
-def test_another_forwards_keep_gives_nan():
-    hn, head, ids, z, dloss = inputs(200, 48, 1000, 20, 2)
-    n = P.lm_head_distill_keep_bytes(200, 48, 1000, 20)
+@pytest.mark.parametrize("t", [30, 200])
+def test_another_forwards_keep_gives_nan(t):
+    hn, head, ids, z, dloss = inputs(t, 48, 1000, 20, 2)
+    n = P.lm_head_distill_keep_bytes(t, 48, 1000, 20)
     keep = torch.zeros(n, dtype=torch.uint8, device=DEV)
-    a = inputs(199, 48, 1000, 20, 2)
+
+    def gives_nan():
+        dhn, dhead = backward(hn, head, ids, z, None, 1.0, dloss, keep)
+        assert bool(torch.isnan(dhn).all()) and bool(torch.isnan(dhead).all())
+    gives_nan()  # (no forward has written it)
+    a = inputs(t - 1, 48, 1000, 20, 2)
     forward(*a[:4], None, 1.0, keep)
-    dhn, dhead = backward(hn, head, ids, z, None, 1.0, dloss, keep)
-    assert bool(torch.isnan(dhn).all()) and bool(torch.isnan(dhead).all())
-    # A log-probabilities' keep of the same rows.
-    logp, lse = torch.empty(200, device=DEV), torch.empty(200, device=DEV)
-    P.lm_head_logprobs(hn, head, ids.amax(1).contiguous(), 200, 48, 1000, logp, lse, P.ce_result_buffer(DEV), keep)
-    dhn, dhead = backward(hn, head, ids, z, None, 1.0, dloss, keep)
-    assert bool(torch.isnan(dhn).all()) and bool(torch.isnan(dhead).all())
+    gives_nan()
+    if t > 64:  # a log-probabilities' keep of the same rows
+        logp, lse = torch.empty(t, device=DEV), torch.empty(t, device=DEV)
+        P.lm_head_logprobs(hn, head, ids.amax(1).contiguous(), t, 48, 1000, logp, lse, P.ce_result_buffer(DEV), keep)
+        gives_nan()
 
 
 @pytest.mark.parametrize("rows", [(4, 10), (3, 5, 20)])
@@ -403,7 +404,7 @@ def test_captured_replays_beside_eager_calls():
         hn, head, ids, z, dloss = inputs(t, 64, vocab, 16, t)
         lse = teacher_lse(ids, z, 2.0)
         n = P.lm_head_distill_keep_bytes(t, 64, vocab, 16)
-        keep = torch.empty(n, dtype=torch.uint8, device=DEV) if n else None
+        keep = torch.empty(n, dtype=torch.uint8, device=DEV)
         out = [torch.empty(t, device=DEV), P.ce_result_buffer(DEV), torch.empty_like(hn), torch.empty_like(head)]
 
         def step(hn=hn, head=head, ids=ids, z=z, lse=lse, dloss=dloss, out=out, keep=keep, t=t, vocab=vocab):
@@ -463,7 +464,7 @@ def test_refusals():
     none = torch.empty(80, 0, dtype=torch.int64, device=DEV)
     with pytest.raises(CfattnError, match="k=0"):
         P.lm_head_distill(**{**ok, "ids": none, "teacher": none.float(), "k": 0})
-    assert P.lm_head_distill_keep_bytes(80, 16, 100, 1025) == 0 and P.lm_head_distill_keep_bytes(64, 16, 100, 5) == 0
+    assert P.lm_head_distill_keep_bytes(80, 16, 100, 1025) == 0 and P.lm_head_distill_keep_bytes(0, 16, 100, 5) == 0
     args = dict(hn=hn, head=head, ids=ids, teacher=z, dloss=dloss, t=80, d=16, vocab=100, k=5)
     P.lm_head_distill_backward(**args)  # (wants nothing)
     for change, error in ((dict(dhn=hn[:79].clone()), ShapeError), (dict(dhead=head.half()), TypeError),
