@@ -57,11 +57,6 @@ class AdamwTensorC(C.Structure):
                 ("weight_decay", C.c_float)]
 
 
-class RotaryTensorC(C.Structure):
-    """`cfops_rotary_tensor` (include/cfops.h)."""
-    _fields_ = [("x", _vp), ("y", _vp), ("heads", _sz), ("x_stride", C.c_int64 * 3), ("y_stride", C.c_int64 * 3)]
-
-
 SIGNATURES = {
     "cfattn_create": (C.c_int, [C.c_int, C.POINTER(_vp)]),
     "cfattn_destroy": (C.c_int, [_vp]),
@@ -108,7 +103,7 @@ SIGNATURES = {
     "cfops_rmsnorm_grad": (C.c_int, [_vp] * 7 + [_sz, _sz, C.c_int, _vp]),
     "cfops_layernorm_forward": (C.c_int, [_vp, C.c_int] + [_vp] * 6 + [_sz, _sz, C.c_float, _vp]),
     "cfops_layernorm_backward": (C.c_int, [_vp, C.c_int] + [_vp] * 8 + [_sz, _sz, C.c_int, _vp]),
-    "cfops_rotary": (C.c_int, [_vp, C.POINTER(RotaryTensorC), _sz, C.c_int, C.c_int] + [_sz] * 4 + [_vp] * 2
+    "cfops_rotary": (C.c_int, [_vp, _vp, _sz, C.c_int, C.c_int] + [_sz] * 4 + [_vp] * 2
                      + [_sz, _vp, _sz, C.c_int, C.c_int, _vp]),
     "cfops_silu_mul_grad": (C.c_int, [_vp] * 6 + [_sz, C.c_int, _vp]),
     "cfops_silu_mul_forward": (C.c_int, [_vp] * 4 + [_sz, _vp]),

@@ -818,6 +818,9 @@ int distill_few_logits(cfattn_ctx* c, const Distill& q, const float* head, const
     cfattn::DistillRows g{};
     g.ids = e.ids, g.count = e.count, g.z = e.z, g.e = e.e, g.row = e.row, g.k = (int)q.k, g.inv_t = q.inv_t;
     g.idx = rows.idx, g.scored = rows.count, g.j0 = (int)j0, g.vocab = (long)q.vocab, g.loss = loss;
+    const size_t slices = nr * cfattn::distill_slices(q.vocab);
+    CF_TRY(take(c, cfattn_ctx::OPS_STATS, slices * sizeof(float2) + nr * q.k * sizeof(float), g.slices));
+    g.xs = reinterpret_cast<float*>(g.slices + slices);
     CF_TRY(gemm(c, CFOPS_NT, rows.hn + j0 * q.d, head, rows.logits, nr, q.d, q.vocab, false, st));
     CF_HIP(c, cfattn::launch_distill_logits(rows.logits, nr, grad, g, st), "distillation launch");
     return CFATTN_OK;
@@ -869,23 +872,25 @@ int distill_backward_few(cfattn_ctx* c, const Distill& q, const float* hn, const
         CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, nullptr, rows.idx, rows.count, tag, rows.hn, padded, q.d, st),
                "distillation launch");
     }
-    float *scaled = nullptr, *sums = nullptr;  // rows of hn times dloss, and of dhn before it
+    float *scaled = nullptr, *parts = nullptr;  // rows of hn times dloss, sums of dhn
     if (dhead) {
         CF_TRY(take(c, cfattn_ctx::OPS_ROWS_BACK, padded * q.d * sizeof(float), scaled));
         CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, dloss, rows.idx, rows.count, tag, scaled, padded, q.d, st),
                "distillation launch");
     }
-    if (dhn) CF_TRY(take(c, cfattn_ctx::OPS_PART, padded * q.d * sizeof(float), sums));
+    if (dhn)
+        CF_TRY(take(c, cfattn_ctx::OPS_PART, cfattn::distill_dhn_floats(std::min(q.t, rows.chunk), q.d, q.vocab) * sizeof(float),
+                    parts));
     for (size_t j0 = 0; j0 < padded; j0 += rows.chunk) {
         const size_t nr = std::min(padded - j0, rows.chunk);
         if (!keep) CF_TRY(distill_few_logits(c, q, head, e, rows, j0, nr, nullptr, true, st));
         if (dhead)
             CF_TRY(gemm(c, CFOPS_TN, rows.logits, scaled + j0 * q.d, dhead, q.vocab, nr, q.d, acc || j0, st));
-        if (dhn) CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, sums + j0 * q.d, nr, q.vocab, q.d, false, st));
+        if (dhn && j0 < q.t)
+            CF_HIP(c, cfattn::launch_distill_dhn(rows.logits, j0, std::min(q.t - j0, nr), q.t, q.d, q.vocab, head, q.mul,
+                                                 dloss, rows.idx, rows.count, tag, parts, dhn, st),
+                   "distillation launch");
     }
-    if (dhn)
-        CF_HIP(c, cfattn::launch_logp_scatter(sums, q.mul, dloss, rows.idx, rows.count, tag, dhn, q.t, q.d, st),
-               "distillation launch");
     return CFATTN_OK;
 }
 
@@ -1086,7 +1091,7 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
         if (dhn) CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, h, nr, vocab, d, false, st));
     }
     if (dhn)
-        CF_HIP(c, cfattn::launch_logp_scatter(rows.hn, 1.0f, nullptr, rows.idx, rows.count, 0, dhn, t, d, st), "log-probability launch");
+        CF_HIP(c, cfattn::launch_logp_scatter(rows.hn, rows.idx, rows.count, dhn, t, d, st), "log-probability launch");
     return CFATTN_OK;
 }
 

@@ -227,16 +227,16 @@ hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st);
 //   select:    idx and, from idx + rows on, their targets; count[0], tag in count[1]; the
 //              result block (CeMisc; or null), and logp
 //              and lse (or null) of the rows that are not scored;
-//   gather:    the scored rows of hn side by side, times mul and the row's `by` (or null);
-//   scatter:   back, other rows 0; either gives NaN where the tag is another;
+//   gather:    the scored rows of hn side by side, times mul and the row's `by` (or null), NaN
+//              where the tag is another;   scatter: back, other rows 0;
 //   grad_rows: the logits become their gradients;
 //   finish:    the mean of sign logp, summed in f64 in a fixed order.
 hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, int tag,
                               float* logp, float* lse, void* misc, hipStream_t st);
 hipError_t launch_logp_gather(const float* hn, float mul, const float* by, const int* idx, const int* count, int tag,
                               float* out, size_t rows, size_t d, hipStream_t st);
-hipError_t launch_logp_scatter(const float* in, float mul, const float* by, const int* idx, const int* count, int tag,
-                               float* dhn, size_t rows, size_t d, hipStream_t st);
+hipError_t launch_logp_scatter(const float* in, const int* idx, const int* count, float* dhn, size_t rows, size_t d,
+                               hipStream_t st);
 hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const int* idx, const int* count,
                                  const float* lse, const float* dlogp, size_t j0, size_t nrows, size_t vocab,
                                  hipStream_t st);
@@ -363,8 +363,17 @@ struct DistillRows {
     const int *idx, *scored;
     int j0;
     long vocab;
-    float* loss;  // may be null
+    float* loss;     // may be null
+    float2* slices;  // scratch: [rows][distill_slices(vocab)], and
+    float* xs;       // [rows][k]
 };
+size_t distill_slices(size_t vocab);
 hipError_t launch_distill_logits(float* logits, size_t nrows, bool grad, const DistillRows& g, hipStream_t st);
+// dhn, of t rows, of scored rows [j0, j0 + n), at most 64, and of those that are not, from the gradients
+// [n][vocab] of the logits of dloss = 1, in scratch `part` of distill_dhn_floats(n, d, vocab).
+size_t distill_dhn_floats(size_t n, size_t d, size_t vocab);
+hipError_t launch_distill_dhn(const float* grads, size_t j0, size_t n, size_t t, size_t d, size_t vocab,
+                              const float* head, float mul, const float* dloss, const int* idx, const int* count, int tag,
+                              float* part, float* dhn, hipStream_t st);
 
 }  // namespace cfattn

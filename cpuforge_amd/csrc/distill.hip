@@ -11,6 +11,8 @@
 #include <hip/hip_runtime.h>
 #include <limits.h>
 
+#include <algorithm>
+
 #include "cfattn_common.hpp"
 #include "cfops_kernels.hpp"
 
@@ -103,19 +105,6 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const DistillEntri
     g.target[r] = any_bad ? -1 : n == 0 ? kIgnoreIndex : least;
 }
 
-// The first of n rising tokens that is not below v.
-__device__ __forceinline__ int lower_bound(const int* tokens, int n, int v) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (tokens[mid] < v)
-            lo = mid + 1;
-        else
-            hi = mid;
-    }
-    return lo;
-}
-
 // What the rest makes of a row's loss, given the logarithm of its probability.
 struct Rest {
     double loss = 0.0, ratio = 0.0;  // ratio: p_rest / q_rest
@@ -138,7 +127,7 @@ __device__ __forceinline__ double entry_loss(const TeacherRow& row, float z, flo
 __device__ __forceinline__ double pow2(double x) { return x > -120.0 ? (double)__builtin_amdgcn_exp2f((float)x) : exp2(x); }
 
 // Rows whose product kept exp2(y - m) of 128 logits each (y in units of log2, m the largest):
-// a wave to a row, 8 rows to a workgroup.  An entry whose exponential is too small, and
+// a wave to a row.  An entry whose exponential is too small, and
 // a rest of 128 that is, are formed again from hidden state and head.  Where the entries hold
 // all but little of such 128, the rest of them is summed, not left over.
 //
@@ -147,29 +136,50 @@ __device__ __forceinline__ double pow2(double x) { return x > -120.0 ? (double)_
 // much larger than its 128's largest (a near 0, a student that holds the token for unlikely), or
 // the rest is far below the entry, it becomes 0 and the entry stays in ids and dl (count of them).
 // (A sure student's a q would cancel in the entries: a is -p_rest / q_rest then.)
-// 3686 rows of 64 entries, 49152 tokens: TODO us, latency.
+// 3686 rows of 64 entries, 49152 tokens: TODO us, a chain of a few loads: what a row needs is
+// loaded at once, the entries' to LDS (one by one where it was used 55).
+struct EntryLds {
+    int v;
+    float kept;
+    float2 stat;
+};
+constexpr int kStats = 16;  // of a lane in registers
 __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) {
-    extern __shared__ int tokens[];  // [8][k]
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int j = blockIdx.x * 8 + wave;
+    const int j = blockIdx.x * (blockDim.x >> 6) + wave;
     const int scored = g.scored[1] == g.tag ? min(g.scored[0] - g.j0, g.chunk) : 0;
-    if (j >= scored) return;  // (no barrier follows)
+    if (j >= scored) return;  // (no barrier follows: each wave has its own part of LDS)
     const long r = g.idx[g.j0 + j];
     const int n = g.count[r];
-    int* mine = tokens + wave * g.k;
-    for (int k = lane; k < n; k += 64) mine[k] = g.ids[r * g.k + k];
-    __builtin_amdgcn_wave_barrier();
-    const TeacherRow row = g.row[r];
-    const bool with_rest = row.p_rest > 0.0;
+    EntryLds* mine = reinterpret_cast<EntryLds*>(lds) + wave * g.k;
     auto kept = [&](int v) -> float& {
         char* p = g.keep + ((long)(j / 32) * g.v16 + v / 32 * 2) * 2048 + v % 32 / 8 * 1024 +
                   ((v % 8 / 4) * 32 + j % 32) * 16;
         return reinterpret_cast<float*>(p)[v % 4];
     };
     auto stat = [&](int part) { return g.stats[(long)part * g.ld + j]; };
+    float2 st[kStats];
+#pragma unroll
+    for (int i = 0; i < kStats; i++)
+        st[i] = lane + 64 * i < g.parts ? stat(lane + 64 * i) : make_float2(-INFINITY, 0.0f);
+    for (int k = lane; k < n; k += 64) {
+        const int v = g.ids[r * g.k + k];
+        mine[k] = {v, kept(v), stat(v / 128)};
+    }
+    __builtin_amdgcn_wave_barrier();
+    const TeacherRow row = g.row[r];
+    const bool with_rest = row.p_rest > 0.0;
     auto has_entry = [&](int part) {
-        const int at = lower_bound(mine, n, part * 128);
-        return at < n && mine[at] < part * 128 + 128;
+        int lo = 0, hi = n;  // the first that is not below the 128
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (mine[mid].v < part * 128)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        return lo < n && mine[lo].v < part * 128 + 128;
     };
     // A logit in units of log2, by the whole wave.
     auto logit = [&](int v) {
@@ -178,39 +188,44 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
         for (int i = lane; i < g.d; i += 64) s += (double)(h[i] * g.mul) * (double)w[i];
         return sum_wave(s) * (double)kLog2e;
     };
+    // (Every lane's statistics, those past the registers' from memory again.)
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < kStats; i++)
+            if (lane + 64 * i < g.parts) f(lane + 64 * i, st[i]);
+        for (int p = lane + 64 * kStats; p < g.parts; p += 64) f(p, stat(p));
+    };
     float m = -INFINITY, m_rest = -INFINITY;
-    for (int p = lane; p < g.parts; p += 64) {
-        const float x = stat(p).x;
-        m = fmaxf(m, x);
-        if (with_rest && !has_entry(p)) m_rest = fmaxf(m_rest, x);
-    }
+    each([&](int p, const float2& s) {
+        m = fmaxf(m, s.x);
+        if (with_rest && !has_entry(p)) m_rest = fmaxf(m_rest, s.x);
+    });
     m = max_wave(m);
     m_rest = max_wave(m_rest);
     const double top = (double)m;
     double total = 0.0, rest = 0.0;  // in units of 2^top
-    for (int p = lane; p < g.parts; p += 64) {
-        const float2 s = stat(p);
+    each([&](int p, const float2& s) {
         total += (double)(s.y * __builtin_amdgcn_exp2f(s.x - m));
         if (with_rest && !has_entry(p)) rest += (double)(s.y * __builtin_amdgcn_exp2f(s.x - m_rest));
-    }
+    });
     total = sum_wave(total);
     constexpr float kLost = 0x1p-100f;  // of a kept exponential
     // The kept values of the 128 that entry `at` is the first of, four to each of 32 lanes, without
     // those of entries; the first entry behind them.
     const int v4 = lane % 32 * 4;
     auto others = [&](int at, float (&x4)[4]) {
-        const int part = mine[at] / 128, v0 = part * 128 + v4;
+        const int part = mine[at].v / 128, v0 = part * 128 + v4;
 #pragma unroll
         for (int i = 0; i < 4; i++) x4[i] = lane < 32 && v0 + i < g.vocab ? kept(v0 + i) : 0.0f;
         int last = at;
-        for (; last < n && mine[last] / 128 == part; last++) {
+        for (; last < n && mine[last].v / 128 == part; last++) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if (mine[last] == v0 + i) x4[i] = 0.0f;
+                if (mine[last].v == v0 + i) x4[i] = 0.0f;
         }
         return last;
     };
-    auto is_first = [&](int k) { return k < n && (k == 0 || mine[k - 1] / 128 != mine[k] / 128); };
+    auto is_first = [&](int k) { return k < n && (k == 0 || mine[k - 1].v / 128 != mine[k].v / 128); };
     if (with_rest) {
         rest = sum_wave(rest);
         if (rest > 0.0) rest *= exp2((double)m_rest - top);
@@ -218,10 +233,10 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
         // is not exact enough, the sum of the others.
         double left = 0.0;
         auto left_of = [&](int k, double& size) {
-            const int part = mine[k] / 128;
-            const float2 s = stat(part);
+            const int part = mine[k].v / 128;
+            const float2 s = mine[k].stat;
             double x = (double)s.y;
-            for (int i = k; i < n && mine[i] / 128 == part; i++) x -= (double)kept(mine[i]);
+            for (int i = k; i < n && mine[i].v / 128 == part; i++) x -= (double)mine[i].kept;
             const double scale = pow2((double)s.x - top);
             size = (double)s.y * scale;
             return fmax(x, 0.0) * scale;
@@ -241,17 +256,17 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
             const bool again = first && !(size * 0x1p-22 <= about * 0x1p-18);
             if (!again) left += x;
             for (unsigned long long todo = __ballot(again); todo; todo &= todo - 1) {
-                const int at = k0 + __ffsll(todo) - 1, part = mine[at] / 128;
+                const int at = k0 + __ffsll(todo) - 1, part = mine[at].v / 128;
                 float x4[4];
                 const int last = others(at, x4);
                 const double sum = sum_wave((double)x4[0] + (double)x4[1] + (double)x4[2] + (double)x4[3]);
-                const double scale = exp2((double)stat(part).x - top);
+                const double scale = exp2((double)mine[at].stat.x - top);
                 double exact = sum * scale;
                 if (!(128.0 * kLost * scale <= about * 0x1p-18) && !(sum > 128.0 * kLost * 0x1p18)) {
                     exact = 0.0;
                     const int end = min(part * 128 + 128, g.vocab);
                     for (int v = part * 128, i = at; v < end; v++) {
-                        if (i < last && mine[i] == v)
+                        if (i < last && mine[i].v == v)
                             i++;
                         else
                             exact += exp2(logit(v) - top);
@@ -271,13 +286,14 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
     for (int k0 = 0; k0 < n; k0 += 64) {
         const int k = k0 + lane;
         const bool live = k < n;
-        const int v = live ? mine[k] : 0;
-        const float e = live ? kept(v) : 1.0f;
-        const double up = live ? (double)stat(v / 128).x - top : 0.0;
+        const EntryLds en = live ? mine[k] : EntryLds{0, 1.0f, make_float2(0.0f, 0.0f)};
+        const int v = en.v;
+        const float e = en.kept;
+        const double up = live ? (double)en.stat.x - top : 0.0;
         double y = log2((double)e) + up, q = (double)e * pow2(up) / total;
         for (unsigned long long todo = __ballot(live && e < kLost); todo; todo &= todo - 1) {
             const int at = __ffsll(todo) - 1;
-            const double x = logit(mine[k0 + at]) - top;
+            const double x = logit(mine[k0 + at].v) - top;
             if (lane == at) y = x, q = exp2(x) / total;
         }
         double dl = 0.0;
@@ -302,9 +318,9 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
     // that this shows in a q, the others of its 128 are scaled up.
     for (int k0 = 0; g.dl && with_rest && k0 < n; k0 += 64) {
         const int k = k0 + lane;
-        const bool far = is_first(k) && pow2((double)stat(mine[k] / 128).x - top) * 0x1p-10 > rest;
+        const bool far = is_first(k) && pow2((double)mine[k].stat.x - top) * 0x1p-10 > rest;
         for (unsigned long long todo = __ballot(far); todo; todo &= todo - 1) {
-            const int at = k0 + __ffsll(todo) - 1, part = mine[at] / 128;
+            const int at = k0 + __ffsll(todo) - 1, part = mine[at].v / 128;
             float x4[4];
             others(at, x4);
             const float most = max_wave(fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])));
@@ -324,50 +340,92 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
     g.count[r] = stay;
 }
 
-// Rows of logits in memory, a workgroup to one: the loss, where it is wanted, and with GRAD the
-// logits become their gradients (zeros from the last scored row on).  The entries are taken out
-// of the row before its sum, so the rest is one of its own.
+// Rows of logits in memory, kSlice of them to a workgroup, in two launches: the largest and the sum
+// of exponentials of each slice's tokens that are no entries (so the rest is a sum of its own),
+// and the entries' logits; then the loss, where it is wanted, and with GRAD the logits become
+// their gradients (zeros from the last scored row on).  19 rows of 49152 with their gradients
+// TODO us (a row to a workgroup 27).
+constexpr int kSlice = 4096, kSliceThreads = 512, kPer = kSlice / kSliceThreads;
+
+// Whether value i of a slice is an entry's, for the values of this thread.
+__device__ __forceinline__ void mark_entries(unsigned (&bits)[kSlice / 32], const int* ids, int n, long v0) {
+    if (threadIdx.x < kSlice / 32) bits[threadIdx.x] = 0;
+    __syncthreads();
+    for (int k = threadIdx.x; k < n; k += kSliceThreads) {
+        const long at = ids[k] - v0;
+        if (at >= 0 && at < kSlice) atomicOr(&bits[at / 32], 1u << at % 32);
+    }
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(kSliceThreads) void distill_slices_kernel(const float* __restrict__ logits,
+                                                                       const DistillRows g) {
+    __shared__ unsigned bits[kSlice / 32];
+    __shared__ float red[2][8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.y;
+    if (g.j0 + j >= *g.scored) return;
+    const long r = g.idx[g.j0 + j], v0 = (long)blockIdx.x * kSlice;
+    const int n = g.count[r];
+    const int* ids = g.ids + r * g.k;
+    const float* x = logits + j * g.vocab;
+    mark_entries(bits, ids, n, v0);
+    float v[kPer], m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+        const int at = threadIdx.x + i * kSliceThreads;
+        const bool in = v0 + at < g.vocab && !(bits[at / 32] >> at % 32 & 1);
+        v[i] = in ? x[v0 + at] : -INFINITY;
+        m = fmaxf(m, v[i]);
+    }
+    for (int k = threadIdx.x; k < n; k += kSliceThreads) {
+        const long at = ids[k] - v0;
+        if (at >= 0 && at < kSlice) g.xs[(long)j * g.k + k] = x[ids[k]];
+    }
+    m = max_wave(m);
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; w++) m = fmaxf(m, red[0][w]);
+    float s = 0.0f;
+    // (A slice of entries alone, or of nothing but NaN, has no largest.)
+    const float base = m > -INFINITY ? m : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) s += expf(v[i] - base);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+    if (lane == 0) red[1][wave] = s;
+    __syncthreads();
+    if (threadIdx.x) return;
+    s = 0.0f;
+    for (int w = 0; w < 8; w++) s += red[1][w];
+    g.slices[(long)j * gridDim.x + blockIdx.x] = make_float2(m, s);
+}
+
 template <bool GRAD>
-__global__ __launch_bounds__(512) void distill_logits_kernel(float* __restrict__ logits, const DistillRows g) {
-    extern __shared__ char lds[];
-    int* tokens = reinterpret_cast<int*>(lds);            // [k]
-    float* xs = reinterpret_cast<float*>(tokens + g.k);   // [k]
-    __shared__ double red[2][8];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float* x = logits + (long)blockIdx.x * g.vocab;
-    if (g.j0 + (int)blockIdx.x >= *g.scored) {
+__global__ __launch_bounds__(kSliceThreads) void distill_logits_kernel(float* __restrict__ logits, int slices,
+                                                                       const DistillRows g) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.y;
+    const long v0 = (long)blockIdx.x * kSlice;
+    float* x = logits + j * g.vocab;
+    if (g.j0 + j >= *g.scored) {
         if (GRAD)
-            for (long i = threadIdx.x; i < g.vocab; i += 512) x[i] = 0.0f;
+            for (long v = v0 + threadIdx.x; v < min(v0 + kSlice, g.vocab); v += kSliceThreads) x[v] = 0.0f;
         return;
     }
-    const long r = g.idx[g.j0 + blockIdx.x];
+    const long r = g.idx[g.j0 + j];
     const int n = g.count[r];
-    for (int k = threadIdx.x; k < n; k += 512) {
-        const int v = g.ids[r * g.k + k];
-        tokens[k] = v;
-        xs[k] = x[v];
-        x[v] = -INFINITY;
-    }
-    __syncthreads();
+    const int* ids = g.ids + r * g.k;
+    const float* xs = g.xs + (long)j * g.k;
+    // (Every wave for itself: a few slices and entries a lane.)
     float m = -INFINITY;
-#pragma unroll 4
-    for (long i = threadIdx.x; i < g.vocab; i += 512) m = fmaxf(m, x[i]);
+    for (int p = lane; p < slices; p += 64) m = fmaxf(m, g.slices[(long)j * slices + p].x);
     m = max_wave(m);
-    if (lane == 0) red[0][wave] = (double)m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; w++) m = fmaxf(m, (float)red[0][w]);
-    float s = 0.0f;
-    if (m > -INFINITY)
-#pragma unroll 4
-        for (long i = threadIdx.x; i < g.vocab; i += 512) s += expf(x[i] - m);
-    const double part = sum_wave((double)s);
-    if (lane == 0) red[1][wave] = part;
-    __syncthreads();
     double rest = 0.0;
-#pragma unroll
-    for (int w = 0; w < 8; w++) rest += red[1][w];
-    // (Every wave for itself: a few entries a lane.)
+    for (int p = lane; p < slices; p += 64) {
+        const float2 s = g.slices[(long)j * slices + p];
+        rest += s.y == 0.0f ? 0.0 : (double)s.y * exp((double)s.x - (double)m);
+    }
+    rest = sum_wave(rest);
     float top = m;
     for (int k = lane; k < n; k += 64) top = fmaxf(top, xs[k]);
     top = max_wave(top);
@@ -382,7 +440,7 @@ __global__ __launch_bounds__(512) void distill_logits_kernel(float* __restrict__
         const double log_q = (double)xs[k] - (double)top - log_total;
         return entry_loss(row, g.z[r * g.k + k], g.e[r * g.k + k], g.inv_t, exp(log_q), log_q, dl);
     };
-    if (g.loss && wave == 0) {
+    if (g.loss && blockIdx.x == 0 && wave == 0) {
         double terms = 0.0, dl;
         for (int k = lane; k < n; k += 64) terms += entry(k, dl);
         terms = sum_wave(terms);
@@ -391,14 +449,120 @@ __global__ __launch_bounds__(512) void distill_logits_kernel(float* __restrict__
     if (!GRAD) return;
     // (By the rest's own largest: a q of a confident student's is not small where q is.)
     const float f = (float)((1.0 - r_.ratio) * exp(shift) / total), base = m > -INFINITY ? m : 0.0f;
-#pragma unroll 4
-    for (long i = threadIdx.x; i < g.vocab; i += 512) x[i] = f * expf(x[i] - base);
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+        const long v = v0 + threadIdx.x + i * kSliceThreads;
+        if (v < g.vocab) x[v] = f * expf(x[v] - base);
+    }
     __syncthreads();
-    for (int k = threadIdx.x; k < n; k += 512) {
+    for (int k = threadIdx.x; k < n; k += kSliceThreads) {
+        const long at = ids[k] - v0;
+        if (at < 0 || at >= kSlice) continue;
         double dl;
         entry(k, dl);
-        x[tokens[k]] = (float)dl;
+        x[ids[k]] = (float)dl;
     }
+}
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+// Elements [0, 4) of p, those at or past n zero (and not read).
+__device__ __forceinline__ f32x4 load4(const float* __restrict__ p, long n) {
+    if (n >= 4) return *reinterpret_cast<const f32x4u*>(p);
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < n; i++) v[i] = p[i];
+    return v;
+}
+
+// part[split][row][d] = rows' gradients . head over a split of the vocabulary, for up to 16 TT rows on
+// the f32 MFMA: a workgroup 64 columns of the head, a wave 16 of its tokens at a time (v_mfma_f32_16x16x4:
+// lane l has A[l % 16][l / 16] and B[l / 16][l % 16]; product s of 16 tokens takes 4 (l / 16) + s, product
+// q of 64 columns 4 (l % 16) + q, so that every load is of four values side by side).
+// Bound by reading the head: 24 rows of 49152 x 576 TODO us (split into f16 pieces, by the products of
+// many rows, 55).
+template <int TT>
+__global__ __launch_bounds__(256) void distill_rows_head_kernel(const float* __restrict__ grads, long vocab, int t,
+                                                                const float* __restrict__ head, int d, int blocks,
+                                                                int splits, float* __restrict__ part) {
+    __shared__ f32x4 sum[TT * 16 * 16];  // [row][columns of a lane]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, kq = lane >> 4;
+    // The columns of a split follow one another on one XCD, whose L2 holds its gradients.
+    const int local = blockIdx.x / 8, split = local / blocks * 8 + blockIdx.x % 8, c0 = local % blocks * 64;
+    if (split >= splits) return;
+    const int c = c0 + 4 * l16;
+    const long chunks = (vocab + 15) / 16, end = chunks * (split + 1) / splits;
+    const float* g[TT];
+#pragma unroll
+    for (int i = 0; i < TT; i++) g[i] = grads + min(16 * i + l16, t - 1) * vocab;
+    f32x4 acc[TT][4] = {};
+    constexpr int U = 2;  // chunks whose loads are in flight together
+    for (long k = chunks * split / splits + U * wave; k < end; k += 4 * U) {
+        f32x4 a[U][TT], b[U][4];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long v = (k + u) * 16 + 4 * kq;
+            const long live = k + u < end ? vocab - v : 0;
+#pragma unroll
+            for (int i = 0; i < TT; i++) a[u][i] = load4(g[i] + v, live);
+#pragma unroll
+            for (int s = 0; s < 4; s++) b[u][s] = load4(head + (v + s) * d + c, s < live ? d - c : 0);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+#pragma unroll
+                for (int i = 0; i < TT; i++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        acc[i][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][i][s], b[u][s][q], acc[i][q], 0, 0, 0);
+    }
+    // Row 16 i + 4 kq + e and column 4 l16 + q of the result are in acc[i][q][e]; wave after wave.
+    for (int w = 0; w < 4; w++) {
+        if (wave == w)
+#pragma unroll
+            for (int i = 0; i < TT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    f32x4& to = sum[(16 * i + 4 * kq + e) * 16 + l16];
+                    const f32x4 x = {acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
+                    to = w ? to + x : x;
+                }
+        __syncthreads();
+    }
+    for (int at = threadIdx.x; at < t * 64; at += 256) {
+        const int row = at / 64, col = at % 64;
+        if (c0 + col < d) part[((long)split * t + row) * d + c0 + col] = sum[row * 16 + col / 4][col % 4];
+    }
+}
+
+// dhn of row r, of scored rows [j0, j0 + t), = mul dloss (the sum of its parts), 64 columns to a
+// workgroup, every fourth split to a wave; zeros of rows that are not scored, NaN where the gradients
+// are another forward's.
+__global__ __launch_bounds__(256) void distill_rows_sum_kernel(const float* __restrict__ part, int splits, int j0,
+                                                               int t, int d, float mul, const float* __restrict__ dloss,
+                                                               const int* __restrict__ idx,
+                                                               const int* __restrict__ count, int tag,
+                                                               float* __restrict__ dhn) {
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.y, c = blockIdx.x * 64 + lane;
+    const bool known = count[1] == tag;
+    const int n = known ? *count : 0;
+    int j = -1;  // (few rows: all at once)
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const unsigned long long at = __ballot(i0 + lane < n && idx[i0 + lane] == r);
+        if (at) j = i0 + __ffsll(at) - 1;
+    }
+    if (j >= 0 && (j < j0 || j >= j0 + t)) return;
+    float s = 0.0f;
+    if (j >= 0 && c < d)
+#pragma unroll 8
+        for (int p = wave; p < splits; p += 4) s += part[((long)p * t + j - j0) * d + c];
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave || c >= d) return;
+    const float all = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    dhn[(long)r * d + c] = !known ? __builtin_nanf("") : j >= 0 ? mul * dloss[r] * all : 0.0f;
 }
 
 }  // namespace
@@ -408,14 +572,41 @@ hipError_t launch_distill_entries(const DistillEntries& g, hipStream_t st) {
     return hipGetLastError();
 }
 hipError_t launch_distill_kept(const DistillKept& g, hipStream_t st) {
-    hipLaunchKernelGGL(distill_kept_kernel, dim3((unsigned)((g.chunk + 7) / 8)), dim3(512), 8 * g.k * sizeof(int), st,
-                       g);
+    const int waves = g.k <= 256 ? 8 : 2;  // (32 KiB of LDS)
+    hipLaunchKernelGGL(distill_kept_kernel, dim3((unsigned)((g.chunk + waves - 1) / waves)), dim3(64 * waves),
+                       waves * g.k * sizeof(EntryLds), st, g);
     return hipGetLastError();
 }
+size_t distill_slices(size_t vocab) { return (vocab + kSlice - 1) / kSlice; }
 hipError_t launch_distill_logits(float* logits, size_t nrows, bool grad, const DistillRows& g, hipStream_t st) {
-    const size_t lds = g.k * (sizeof(int) + sizeof(float));
-    hipLaunchKernelGGL((grad ? distill_logits_kernel<true> : distill_logits_kernel<false>), dim3((unsigned)nrows),
-                       dim3(512), lds, st, logits, g);
+    const unsigned slices = (unsigned)distill_slices((size_t)g.vocab);
+    hipLaunchKernelGGL(distill_slices_kernel, dim3(slices, (unsigned)nrows), dim3(kSliceThreads), 0, st, logits, g);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((grad ? distill_logits_kernel<true> : distill_logits_kernel<false>),
+                       dim3(grad ? slices : 1, (unsigned)nrows), dim3(kSliceThreads), 0, st, logits, (int)slices, g);
+    return hipGetLastError();
+}
+
+// Workgroups of the product: four to a CU, of 16 tokens and more.
+static size_t rows_head_splits(size_t d, size_t vocab) {
+    const size_t blocks = (d + 63) / 64;
+    return std::max<size_t>(std::min((1024 + blocks - 1) / blocks, (vocab + 63) / 64), 1);
+}
+size_t distill_dhn_floats(size_t t, size_t d, size_t vocab) { return rows_head_splits(d, vocab) * t * d; }
+hipError_t launch_distill_dhn(const float* grads, size_t j0, size_t n, size_t t, size_t d, size_t vocab,
+                              const float* head, float mul, const float* dloss, const int* idx, const int* count, int tag,
+                              float* part, float* dhn, hipStream_t st) {
+    const unsigned blocks = (unsigned)((d + 63) / 64), splits = (unsigned)rows_head_splits(d, vocab);
+    const auto kernel = n <= 16   ? distill_rows_head_kernel<1>
+                        : n <= 32 ? distill_rows_head_kernel<2>
+                                  : distill_rows_head_kernel<4>;
+    hipLaunchKernelGGL(kernel, dim3((splits + 7) / 8 * 8 * blocks), dim3(256), 0, st, grads, (long)vocab, (int)n, head,
+                       (int)d, (int)blocks, (int)splits, part);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(distill_rows_sum_kernel, dim3(blocks, (unsigned)t), dim3(256), 0, st, part, (int)splits, (int)j0,
+                       (int)n, (int)d, mul, dloss, idx, count, tag, dhn);
     return hipGetLastError();
 }
 

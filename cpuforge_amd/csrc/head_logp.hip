@@ -89,14 +89,12 @@ __global__ __launch_bounds__(256) void logp_gather_kernel(const float* __restric
     for (long i = threadIdx.x; i < d; i += 256) out[j * d + i] = x ? f * x[i] : none;
 }
 
-// dhn[idx[j]] = mul by in[j] for j < n, the other rows zeros.
-__global__ __launch_bounds__(256) void logp_scatter_kernel(const float* __restrict__ in, float mul,
-                                                           const float* __restrict__ by, const int* __restrict__ idx,
-                                                           const int* __restrict__ count, int tag,
-                                                           float* __restrict__ dhn, long d) {
+// dhn[idx[j]] = in[j] for j < n, the other rows zeros.
+__global__ __launch_bounds__(256) void logp_scatter_kernel(const float* __restrict__ in, const int* __restrict__ idx,
+                                                           const int* __restrict__ count, float* __restrict__ dhn,
+                                                           long d) {
     // The place of row blockIdx.x among the ascending idx.
-    const bool known = count[1] == tag;
-    const int r = blockIdx.x, n = known ? *count : 0;
+    const int r = blockIdx.x, n = *count;
     int lo = 0, hi = n;
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
@@ -106,8 +104,7 @@ __global__ __launch_bounds__(256) void logp_scatter_kernel(const float* __restri
             hi = mid;
     }
     const float* x = lo < n && idx[lo] == r ? in + (long)lo * d : nullptr;
-    const float f = x && by ? mul * by[r] : mul, none = known ? 0.0f : __builtin_nanf("");
-    for (long i = threadIdx.x; i < d; i += 256) dhn[r * d + i] = x ? f * x[i] : none;
+    for (long i = threadIdx.x; i < d; i += 256) dhn[r * d + i] = x ? x[i] : 0.0f;
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -309,10 +306,9 @@ hipError_t launch_logp_gather(const float* hn, float mul, const float* by, const
                        (long)d);
     return hipGetLastError();
 }
-hipError_t launch_logp_scatter(const float* in, float mul, const float* by, const int* idx, const int* count, int tag,
-                               float* dhn, size_t rows, size_t d, hipStream_t st) {
-    hipLaunchKernelGGL(logp_scatter_kernel, dim3((unsigned)rows), dim3(256), 0, st, in, mul, by, idx, count, tag, dhn,
-                       (long)d);
+hipError_t launch_logp_scatter(const float* in, const int* idx, const int* count, float* dhn, size_t rows, size_t d,
+                               hipStream_t st) {
+    hipLaunchKernelGGL(logp_scatter_kernel, dim3((unsigned)rows), dim3(256), 0, st, in, idx, count, dhn, (long)d);
     return hipGetLastError();
 }
 size_t logp_few_bytes(size_t t, size_t vocab) {

@@ -33,6 +33,7 @@ library failures raise `CfattnError`.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import NamedTuple
 
 import torch
@@ -194,31 +195,44 @@ def rotary(xs, ys, cos, sin, positions=None, *, pos0: int = 0, interleaved: bool
     ctx = ctx or default_context()
     if isinstance(xs, torch.Tensor):
         xs, ys = (xs,), (ys,)
-    if len(xs) != len(ys) or not 1 <= len(xs) <= _lib.ROTARY_MAX:
-        raise ValueError(f"{len(xs)} xs and {len(ys)} ys: as many of either, and 1 to {_lib.ROTARY_MAX}")
-    table = (_lib.RotaryTensorC * len(xs))()
-    shape = tuple(xs[0].shape)
-    for c, x, y in zip(table, xs, ys):
-        for t, name, of in ((x, "x", xs[0]), (y, "y", ys[0])):
-            _check_on(t, name, ctx, _CODES if t is of else (of.dtype,))
-            if t.dim() != 4 or t.shape != x.shape or (*t.shape[:2], t.shape[3]) != (*shape[:2], shape[3]):
-                raise _lib.ShapeError(_lib.ERR_SHAPE, f"{name} has shape {tuple(t.shape)} beside {shape} "
-                                                      "([B, S, H, D], the same but for H)")
-            if t.shape[3] > 1 and t.stride(3) != 1:
-                raise ValueError(f"{name}'s last stride must be 1")
-        if any(n > 1 and st == 0 for n, st in zip(y.shape, y.stride())):
+    n = len(xs)
+    if n != len(ys) or not 1 <= n <= _lib.ROTARY_MAX:
+        raise ValueError(f"{n} xs and {len(ys)} ys: as many of either, and 1 to {_lib.ROTARY_MAX}")
+    dev, table = ctx.device, []
+    x_type, y_type = getattr(xs[0], "dtype", None), getattr(ys[0], "dtype", None)
+    batch = seq = dim = -1
+    for x, y in zip(xs, ys):
+        if not (isinstance(x, torch.Tensor) and isinstance(y, torch.Tensor) and x.dtype is x_type and y.dtype is y_type
+                and x_type in _CODES and y_type in _CODES and x.get_device() == dev and y.get_device() == dev):
+            _check_on(xs[0], "x", ctx, _CODES)
+            _check_on(ys[0], "y", ctx, _CODES)
+            _check_on(x, "x", ctx, (x_type,))
+            _check_on(y, "y", ctx, (y_type,))
+        shape = x.shape
+        if batch < 0 and len(shape) == 4:
+            batch, seq, _, dim = shape
+        if y.shape != shape or len(shape) != 4 or shape[0] != batch or shape[1] != seq or shape[3] != dim:
+            raise _lib.ShapeError(_lib.ERR_SHAPE, f"x and y have shapes {tuple(shape)} and {tuple(y.shape)} beside "
+                                                  f"{tuple(xs[0].shape)} ([B, S, H, D], the same but for H)")
+        x0, x1, x2, x3 = x.stride()
+        y0, y1, y2, y3 = y.stride()
+        if dim > 1 and (x3 != 1 or y3 != 1):
+            raise ValueError("the last stride of x and y must be 1")
+        if (y0 == 0 and batch > 1) or (y1 == 0 and seq > 1) or (y2 == 0 and shape[2] > 1):
             raise ValueError("y must not be expanded")
-        c.x, c.y, c.heads = x.data_ptr(), y.data_ptr(), x.shape[2]
-        c.x_stride[:], c.y_stride[:] = x.stride()[:3], y.stride()[:3]
-    batch, seq, _, dim = shape
-    pp = _on(cos, "cos", ctx), _on(sin, "sin", ctx, numel=cos.numel())
+        table.append(_ROTARY_TENSOR.pack(x.data_ptr(), y.data_ptr(), shape[2], x0, x1, x2, y0, y1, y2))
+    pc, ps = _on(cos, "cos", ctx), _on(sin, "sin", ctx, numel=cos.numel())
     if cos.dim() != 2:
         raise _lib.ShapeError(_lib.ERR_SHAPE, f"cos has shape {tuple(cos.shape)}, expected [max_pos, half]")
     at = None if positions is None else _on(positions, "positions", ctx, (torch.int64,), batch * seq)
     if pos0 < 0:
         raise ValueError("pos0 must not be negative")
-    _call(ctx, "cfops_rotary", table, len(xs), _CODES[xs[0].dtype], _CODES[ys[0].dtype], batch, seq, dim, cos.shape[1],
-          *pp, cos.shape[0], at, int(pos0), int(interleaved), int(inverse), _stream_of(ctx))
+    max_pos, half = cos.shape
+    _call(ctx, "cfops_rotary", b"".join(table), n, _CODES[x_type], _CODES[y_type], batch, seq, dim, half, pc, ps,
+          max_pos, at, pos0, interleaved, inverse, _stream_of(ctx))
+
+
+_ROTARY_TENSOR = struct.Struct("@PPN6q")  # cfops_rotary_tensor
 
 
 # --------------------------------------------------------------- SwiGLU
