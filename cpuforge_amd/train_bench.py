@@ -38,6 +38,7 @@ import torch
 import torch.nn.functional as F
 
 from . import autograd as A
+from . import device as D
 from .layer import LayerRope, layer_attention
 from .rope import RopeCache
 from .st import FormatError
@@ -90,6 +91,17 @@ def rmsnorm(x, w, eps):
     return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + eps) * w
 
 
+def rotary(x, cos, sin, positions, interleaved):
+    """ops.rotary of x [B, S, H, D] in torch operations."""
+    at = torch.arange(x.shape[1], device=x.device) if positions is None else positions
+    c, s = cos[at].unsqueeze(-2), sin[at].unsqueeze(-2)
+    half = cos.shape[1]
+    turned, rest = x[..., :2 * half], x[..., 2 * half:]
+    a, b = (turned[..., 0::2], turned[..., 1::2]) if interleaved else (turned[..., :half], turned[..., half:])
+    pair = (a * c - b * s, b * c + a * s)
+    return torch.cat([torch.stack(pair, -1).flatten(-2) if interleaved else torch.cat(pair, -1), rest], -1)
+
+
 @dataclass
 class LoraConfig:
     """crates/model/src/model.rs:45-49."""
@@ -106,7 +118,12 @@ class SmolLM:
     """`rank` > 0 attaches adapters (alpha 2·rank) to every projection, as
     `cpuforge bench-train` does; `train` is the TrainSpec: "lora" trains the
     adapters only (LORA_ONLY), "full" every parameter (FULL).  `config`
-    overrides entries of SMOLLM_135M (a smaller model for tests)."""
+    overrides entries of SMOLLM_135M (a smaller model for tests), or gives it
+    another decoder's layers: norm="layer" (layer norms with a bias in the place of
+    RMSNorm), rotary=dict(dim=.., interleaved=..) (the first `dim` values of
+    each head turn, all by default, in halves or as pairs side by side: ops.rotary
+    before the attention instead of the fused prologue, at positions of the
+    caller's), rope_scaling (a scaling of RopeCache)."""
 
     def __init__(self, layers: int = 30, seq: int = 512, rank: int = 16, dtype=torch.float32, device="cuda",
                  seed: int = 1, attn_dtype=None, backend: str = "cfops", config: dict | None = None,
@@ -117,7 +134,10 @@ class SmolLM:
             raise ValueError("the cfops backend runs the reference's f32 arithmetic")
         if train not in ("lora", "full"):
             raise ValueError(f"unknown train spec {train!r}")
-        c = dict(SMOLLM_135M, **(config or {}))
+        c = dict(SMOLLM_135M, norm="rms", rotary=None, rope_scaling=None)
+        c.update(config or {})
+        if c["norm"] not in ("rms", "layer"):
+            raise ValueError(f"unknown norm {c['norm']!r}")
         self.c, self.dtype, self.layers_n, self.backend, self.train = c, dtype, layers, backend, train
         self.attn_dtype = attn_dtype or dtype
         self.device = device
@@ -126,12 +146,15 @@ class SmolLM:
         d, f, hd = c["d"], c["ffn"], c["head_dim"]
         qd, kvd = c["heads"] * hd, c["kv_heads"] * hd
         lin = lambda o, i: LoRALinear(o, i, 0.02, gen, dtype, device)  # noqa: E731
-        self.layers = [dict(attn_norm=torch.ones(d, device=device, dtype=dtype), wq=lin(qd, d), wk=lin(kvd, d),
-                            wv=lin(kvd, d), wo=lin(d, qd), mlp_norm=torch.ones(d, device=device, dtype=dtype),
-                            gate=lin(f, d), up=lin(f, d), down=lin(d, f)) for _ in range(layers)]
+        ones = lambda: torch.ones(d, device=device, dtype=dtype)  # noqa: E731
+        zeros = lambda: torch.zeros(d, device=device, dtype=dtype) if c["norm"] == "layer" else None  # noqa: E731
+        self.layers = [dict(attn_norm=ones(), attn_norm_b=zeros(), wq=lin(qd, d), wk=lin(kvd, d), wv=lin(kvd, d),
+                            wo=lin(d, qd), mlp_norm=ones(), mlp_norm_b=zeros(), gate=lin(f, d), up=lin(f, d),
+                            down=lin(d, f)) for _ in range(layers)]
         self.embed = (torch.randn(c["vocab"], d, generator=gen, device=device) * 0.02).to(dtype)
-        self.final_norm = torch.ones(d, device=device, dtype=dtype)
-        self.rope = LayerRope(RopeCache(hd, seq, c["theta"]), device)
+        self.final_norm, self.final_norm_b = ones(), zeros()
+        turned = (c["rotary"] or {}).get("dim", hd)
+        self.rope = LayerRope(RopeCache(turned, seq, c["theta"], c["rope_scaling"]), device)
         self.attention = layer_attention  # (q_pre, k_pre, v, LayerRope) -> o
         # With ce_on_device the cfops loss leaves its value on the device
         # (no host wait: a step that can be captured in a HIP graph) and the
@@ -167,23 +190,62 @@ class SmolLM:
         for i, layer in enumerate(self.layers):
             p = f"model.layers.{i}"
             yield f"{p}.input_layernorm.weight", layer["attn_norm"]
+            if layer["attn_norm_b"] is not None:
+                yield f"{p}.input_layernorm.bias", layer["attn_norm_b"]
             yield from layer["wq"].named(f"{p}.self_attn.q_proj")
             yield from layer["wk"].named(f"{p}.self_attn.k_proj")
             yield from layer["wv"].named(f"{p}.self_attn.v_proj")
             yield from layer["wo"].named(f"{p}.self_attn.o_proj")
             yield f"{p}.post_attention_layernorm.weight", layer["mlp_norm"]
+            if layer["mlp_norm_b"] is not None:
+                yield f"{p}.post_attention_layernorm.bias", layer["mlp_norm_b"]
             yield from layer["gate"].named(f"{p}.mlp.gate_proj")
             yield from layer["up"].named(f"{p}.mlp.up_proj")
             yield from layer["down"].named(f"{p}.mlp.down_proj")
         yield "model.norm.weight", self.final_norm
+        if self.final_norm_b is not None:
+            yield "model.norm.bias", self.final_norm_b
 
     def params(self):
         """The parameters that train (TrainSpec)."""
         return [p for _, p in self.named_params() if p.requires_grad]
 
-    def hidden(self, tokens):
-        """The final norm's output [B, S, d]."""
-        return self._hidden_cfops(tokens) if self.backend == "cfops" else self._hidden_torch(tokens)
+    def hidden(self, tokens, positions=None):
+        """The final norm's output [B, S, d].  positions [B, S] (int64; with
+        config rotary): the tokens' own, where several documents share a row."""
+        return self._hidden_cfops(tokens, positions) if self.backend == "cfops" else \
+            self._hidden_torch(tokens, positions)
+
+    def _attend(self, q, k, v, positions):
+        """Layer::forward's q_pre, k_pre, v -> attn_o; with config rotary, turned by
+        ops.rotary and through the attention alone."""
+        if self.c["rotary"] is None:
+            if positions is not None:
+                raise ValueError("positions need a model with config rotary")
+            return self.attention(q, k, v.to(self.attn_dtype), self.rope)
+        pr, interleaved = self.rope.pr, bool(self.c["rotary"].get("interleaved"))
+        if self.backend == "cfops":
+            q, k = A.rotary((q, k), pr.cos, pr.sin, positions, interleaved=interleaved, dtype=self.attn_dtype)
+        else:
+            q, k = (rotary(x.float(), pr.cos, pr.sin, positions, interleaved).to(self.attn_dtype) for x in (q, k))
+        return D.attention(q, k, v.to(self.attn_dtype))
+
+    def _norm(self, x, w, b):
+        if b is None:
+            return (A.rmsnorm if self.backend == "cfops" else rmsnorm)(x, w, self.c["eps"])
+        if self.backend == "cfops":
+            return A.layer_norm(x, w, b, self.c["eps"])
+        return F.layer_norm(x, x.shape[-1:], w, b, self.c["eps"])
+
+    def distill(self, tokens, ids, teacher, teacher_lse=None, temperature=1.0, positions=None):
+        """The rows' losses [B, S] against a teacher's top logits (A.lm_head_distill;
+        ids and teacher [B, S, k], teacher_lse [B, S] or None; cfops backend, no host
+        wait: check_targets() reports entries that it does not take)."""
+        if self.backend != "cfops":
+            raise ValueError("distillation needs the cfops backend")
+        loss, res = A.lm_head_distill(self.hidden(tokens, positions), self.embed, ids, teacher, teacher_lse, temperature)
+        self._ce = (res, None)
+        return loss
 
     def logprobs(self, tokens, targets):
         """The targets' log-probabilities [B, S], 0 where a target is
@@ -202,22 +264,22 @@ class SmolLM:
         logits = self.hidden(tokens) @ self.embed.t()
         return F.cross_entropy(logits.view(-1, self.c["vocab"]).float(), targets.view(-1))
 
-    def _hidden_torch(self, tokens):
+    def _hidden_torch(self, tokens, positions=None):
         c = self.c
         B, S = tokens.shape
         x = self.embed[tokens]
         for layer in self.layers:
-            n1 = rmsnorm(x, layer["attn_norm"], c["eps"])
+            n1 = self._norm(x, layer["attn_norm"], layer["attn_norm_b"])
             q = layer["wq"](n1).view(B, S, c["heads"], c["head_dim"])
             k = layer["wk"](n1).view(B, S, c["kv_heads"], c["head_dim"])
             v = layer["wv"](n1).view(B, S, c["kv_heads"], c["head_dim"])
-            o = self.attention(q.float(), k.float(), v.to(self.attn_dtype), self.rope)
+            o = self._attend(q.float(), k.float(), v, positions)
             x = x + layer["wo"](o.view(B, S, -1).to(self.dtype))
-            n2 = rmsnorm(x, layer["mlp_norm"], c["eps"])
+            n2 = self._norm(x, layer["mlp_norm"], layer["mlp_norm_b"])
             x = x + layer["down"](F.silu(layer["gate"](n2)) * layer["up"](n2))
-        return rmsnorm(x, self.final_norm, c["eps"])
+        return self._norm(x, self.final_norm, self.final_norm_b)
 
-    def _hidden_cfops(self, tokens):
+    def _hidden_cfops(self, tokens, positions=None):
         """Layer::forward (crates/model/src/layer.rs:90-143) per layer, then the
         final norm, every op but the gather and the residual adds in
         libcfattn.so."""
@@ -225,17 +287,17 @@ class SmolLM:
         B, S = tokens.shape
         x = self.embed[tokens]
         for layer in self.layers:
-            n1 = A.rmsnorm(x, layer["attn_norm"], c["eps"])
+            n1 = self._norm(x, layer["attn_norm"], layer["attn_norm_b"])
             q, k, v = A.shared_input_linears(n1, [layer[n].spec() for n in ("wq", "wk", "wv")])
             q = q.view(B, S, c["heads"], c["head_dim"])
             k = k.view(B, S, c["kv_heads"], c["head_dim"])
             v = v.view(B, S, c["kv_heads"], c["head_dim"])
-            o = self.attention(q, k, v.to(self.attn_dtype), self.rope)
+            o = self._attend(q, k, v, positions)
             x = x + layer["wo"](o.view(B, S, -1), cf)
-            n2 = A.rmsnorm(x, layer["mlp_norm"], c["eps"])
+            n2 = self._norm(x, layer["mlp_norm"], layer["mlp_norm_b"])
             g, u = A.shared_input_linears(n2, [layer[n].spec() for n in ("gate", "up")])
             x = x + layer["down"](A.silu_mul(g, u), cf)
-        return A.rmsnorm(x, self.final_norm, c["eps"])
+        return self._norm(x, self.final_norm, self.final_norm_b)
 
     def _loss_cfops(self, tokens, targets):
         """The tied LM head with its loss (model.rs:436-442)."""
@@ -250,9 +312,12 @@ class SmolLM:
         """Raises, as the loss would have, if the last device-side loss met
         a target out of range (waits for it)."""
         if self._ce is not None:
-            from .ops import ce_check
+            from .ops import ce_check, distill_check
             res, targets = self._ce
-            ce_check(res, targets, self.c["vocab"])
+            if targets is None:
+                distill_check(res)
+            else:
+                ce_check(res, targets, self.c["vocab"])
 
 
 def capture_step(model: SmolLM, tokens, targets, warmup: int = 2):
