@@ -35,9 +35,8 @@ class Llama3ScalingC(C.Structure):
 
 class RopeScalingC(C.Structure):
     """`cfattn_rope_scaling` (include/cfattn.h)."""
-    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("low_freq_factor", C.c_double),
-                ("high_freq_factor", C.c_double), ("original_max_position", C.c_double), ("beta_fast", C.c_double),
-                ("beta_slow", C.c_double), ("attention_factor", C.c_double)]
+    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("original_max_position", C.c_double),
+                ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("attention_factor", C.c_double)]
 
 
 class PrologueC(C.Structure):

@@ -721,12 +721,9 @@ int cfattn_rope_table_scaled(size_t head_dim, size_t max_pos, double theta, cons
         size = 0.1 * std::log(sc->factor) + 1.0;
     }
     if (sc->attention_factor > 0.0) size = sc->attention_factor;
-    const cfattn_llama3_scaling l3 = {sc->factor, sc->low_freq_factor, sc->high_freq_factor,
-                                      sc->original_max_position};
     for (size_t i = 0; i < half; i++) {
         double inv_freq = std::pow(theta, -(2.0 * (double)i) / dim);
         if (sc->kind == CFATTN_ROPE_LINEAR) inv_freq /= sc->factor;
-        if (sc->kind == CFATTN_ROPE_LLAMA3) inv_freq = cfattn_llama3_scale(&l3, inv_freq);
         if (sc->kind == CFATTN_ROPE_YARN) {
             const double slow =
                 std::min(std::max(((double)i - first) / (last > first ? last - first : 1e-3), 0.0), 1.0);

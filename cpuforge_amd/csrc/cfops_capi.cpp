@@ -285,9 +285,9 @@ int cfops_rmsnorm_grad(cfattn_ctx* c, const float* dy, const float* x, const flo
 
 static int check_layernorm(cfattn_ctx* c, int dtype, size_t rows, size_t dim) {
     if (dtype != CFATTN_F32 && dtype != CFATTN_BF16) return fail(c, CFATTN_ERR_ARG, "unknown dtype %d", dtype);
-    // (Columns are numbered beside up to 16 KiB of others.)
-    if (rows > (size_t)INT_MAX || dim > (size_t)INT_MAX - 65536)
-        return fail(c, CFATTN_ERR_UNSUPPORTED, "rows=%zu or dim=%zu too large", rows, dim);
+    // (A launch with 16 threads to a column has fewer than 2^32.)
+    if (!fits_int(rows) || dim >= (size_t)1 << 26)
+        return fail(c, CFATTN_ERR_UNSUPPORTED, "rows=%zu above 2^31 or dim=%zu not below 2^26", rows, dim);
     return CFATTN_OK;
 }
 

@@ -169,7 +169,7 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
     }
     __builtin_amdgcn_wave_barrier();
     const TeacherRow row = g.row[r];
-    const bool with_rest = row.p_rest > 0.0;
+    bool with_rest = row.p_rest > 0.0;
     auto has_entry = [&](int part) {
         int lo = 0, hi = n;  // the first that is not below the 128
         while (lo < hi) {
@@ -209,6 +209,8 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
         if (with_rest && !has_entry(p)) rest += (double)(s.y * __builtin_amdgcn_exp2f(s.x - m_rest));
     });
     total = sum_wave(total);
+    // (A row that is not finite has a loss of NaN, whatever its rest.)
+    with_rest = with_rest && total < INFINITY;
     constexpr float kLost = 0x1p-100f;  // of a kept exponential
     // The kept values of the 128 that entry `at` is the first of, four to each of 32 lanes, without
     // those of entries; the first entry behind them.

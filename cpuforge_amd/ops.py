@@ -221,9 +221,10 @@ def rotary(xs, ys, cos, sin, positions=None, *, pos0: int = 0, interleaved: bool
         if (y0 == 0 and batch > 1) or (y1 == 0 and seq > 1) or (y2 == 0 and shape[2] > 1):
             raise ValueError("y must not be expanded")
         table.append(_ROTARY_TENSOR.pack(x.data_ptr(), y.data_ptr(), shape[2], x0, x1, x2, y0, y1, y2))
-    pc, ps = _on(cos, "cos", ctx), _on(sin, "sin", ctx, numel=cos.numel())
-    if cos.dim() != 2:
-        raise _lib.ShapeError(_lib.ERR_SHAPE, f"cos has shape {tuple(cos.shape)}, expected [max_pos, half]")
+    pc, ps = _on(cos, "cos", ctx), _on(sin, "sin", ctx)
+    if cos.dim() != 2 or sin.shape != cos.shape:
+        raise _lib.ShapeError(_lib.ERR_SHAPE, f"cos and sin have shapes {tuple(cos.shape)} and {tuple(sin.shape)}, "
+                                              "expected [max_pos, half]")
     at = None if positions is None else _on(positions, "positions", ctx, (torch.int64,), batch * seq)
     if pos0 < 0:
         raise ValueError("pos0 must not be negative")
@@ -472,8 +473,8 @@ def lm_head_distill(hn, head, ids, teacher, t, d, vocab, k, loss, result, teache
     given) takes what the backward reads.  No host wait."""
     ctx = ctx or default_context()
     _call(ctx, "cfops_lm_head_distill", *_distill(hn, head, ids, teacher, teacher_lse, t, d, vocab, k, ctx), t, d, vocab,
-          k, float(temperature), _on(loss, "loss", ctx, numel=t), _result(result, CE_RESULT_WORDS), *_keep(keep),
-          _stream_of(ctx))
+          k, float(temperature), _on(loss, "loss", ctx, numel=t), _result(_here(result, ctx), CE_RESULT_WORDS),
+          *_keep(_here(keep, ctx)), _stream_of(ctx))
 
 
 def lm_head_distill_backward(hn, head, ids, teacher, dloss, t, d, vocab, k, dhn=None, dhead=None, teacher_lse=None,
@@ -485,8 +486,15 @@ def lm_head_distill_backward(hn, head, ids, teacher, dloss, t, d, vocab, k, dhn=
     _call(ctx, "cfops_lm_head_distill_backward", *_distill(hn, head, ids, teacher, teacher_lse, t, d, vocab, k, ctx),
           _on(dloss, "dloss", ctx, numel=t), t, d, vocab, k, float(temperature),
           None if dhn is None else _on(dhn, "dhn", ctx, numel=t * d),
-          None if dhead is None else _on(dhead, "dhead", ctx, numel=vocab * d), int(acc), *_keep(keep),
+          None if dhead is None else _on(dhead, "dhead", ctx, numel=vocab * d), int(acc), *_keep(_here(keep, ctx)),
           _stream_of(ctx))
+
+
+def _here(t, ctx):
+    """t, or its error where it is a tensor of another device than the context's."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != ctx.device:
+        raise ValueError(f"a buffer is on device {t.get_device()}, the context on device {ctx.device}")
+    return t
 
 
 def _distill(hn, head, ids, teacher, lse, t, d, vocab, k, ctx):

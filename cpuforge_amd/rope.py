@@ -68,7 +68,7 @@ class YarnScaling:
     def c(self) -> _lib.RopeScalingC:
         if self.attention_factor is not None and not self.attention_factor > 0:
             raise ValueError("attention_factor must be positive")
-        return _lib.RopeScalingC(kind=4, factor=self.factor, original_max_position=self.original_max_position,
+        return _lib.RopeScalingC(kind=3, factor=self.factor, original_max_position=self.original_max_position,
                                  beta_fast=self.beta_fast, beta_slow=self.beta_slow,
                                  attention_factor=self.attention_factor or 0.0)
 

@@ -205,17 +205,14 @@ int cfattn_rope_table(size_t head_dim, size_t max_pos, double theta, const cfatt
  * own, 1 except for YARN's 0.1 ln(factor) + 1):
  *   LINEAR  inv_freq / factor
  *   NTK     theta * factor^(head_dim / (head_dim - 2)) in theta's place
- *   LLAMA3  cfattn_llama3_scale
  *   YARN    of d pairs, those that turn at most beta_slow times in
  *           original_max_position positions get inv_freq / factor, those that turn
  *           beta_fast times or more keep theirs, a line over the pairs in between */
-enum { CFATTN_ROPE_LINEAR = 1, CFATTN_ROPE_NTK = 2, CFATTN_ROPE_LLAMA3 = 3, CFATTN_ROPE_YARN = 4 };
+enum { CFATTN_ROPE_LINEAR = 1, CFATTN_ROPE_NTK = 2, CFATTN_ROPE_YARN = 3 };
 typedef struct cfattn_rope_scaling {
     int kind;
     double factor;
-    double low_freq_factor, high_freq_factor; /* LLAMA3 */
-    double original_max_position;             /* LLAMA3, YARN */
-    double beta_fast, beta_slow;              /* YARN */
+    double original_max_position, beta_fast, beta_slow; /* YARN */
     double attention_factor;
 } cfattn_rope_scaling;
 int cfattn_rope_table_scaled(size_t head_dim, size_t max_pos, double theta, const cfattn_rope_scaling* scaling,

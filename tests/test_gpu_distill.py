@@ -152,7 +152,9 @@ def check(hn, head, ids, z, lse, temp, dloss):
 SHAPES = [(1, 1, 2, 1), (1, 64, 5, 5), (3, 7, 130, 4), (1, 576, 4097, 32), (16, 100, 1000, 64), (17, 576, 1000, 8),
           (33, 40, 128, 65), (64, 33, 4099, 20), (65, 31, 257, 33), (66, 2100, 300, 3), (70, 1500, 300, 300),
           (130, 100, 257, 130), (256, 64, 512, 64), (300, 65, 50, 70), (513, 576, 8192, 64), (700, 128, 900, 200),
-          (90, 16, 5000, 1024), (5, 16, 5000, 1024), (1000, 16, 20000, 1)]
+          (90, 16, 5000, 1024), (5, 16, 5000, 1024), (1000, 16, 20000, 1),
+          # More parts and slices of the vocabulary than a wave has at once.
+          (70, 16, 140000, 8), (3, 8, 270000, 5)]
 
 
 @pytest.mark.parametrize("rest", [True, False])

@@ -108,7 +108,10 @@ def test_forward_and_backward(rows, dim, dtype):
 
 
 @pytest.mark.parametrize("rows,dim,dtype", [(4099, 576, F32), (5000, 2048, BF16), (1023, 4096, F32), (2050, 8192, BF16),
-                                            (515, 16384, F32), (70, 40000, BF16), (20000, 17, F32)])
+                                            (515, 16384, F32), (70, 40000, BF16), (20000, 17, F32),
+                                            # Two rows at a time, in either number of waves.
+                                            (4097, 1500, F32), (4099, 3001, BF16), (4096, 8001, BF16), (4101, 6000, F32),
+                                            (4097, 16383, BF16), (4098, 4096, F32)])
 def test_many_rows(rows, dim, dtype):
     x, w, b, dy = inputs(rows, dim, dtype, 3)
     want, tol = exact(x, w, b, dy, 1e-5)
@@ -299,6 +302,9 @@ def test_refusals():
     with pytest.raises(CfattnError, match="dtype"):
         P._call(ctx, "cfops_layernorm_forward", 7, x.data_ptr(), w.data_ptr(), None, y.data_ptr(), s.data_ptr(),
                 s.data_ptr(), 4, 8, 1e-5, 0)
+    with pytest.raises(CfattnError, match="2\\^26"):
+        P._call(ctx, "cfops_layernorm_forward", 0, x.data_ptr(), w.data_ptr(), None, y.data_ptr(), s.data_ptr(),
+                s.data_ptr(), 4, 1 << 26, 1e-5, 0)
     with pytest.raises(CfattnError, match="null"):
         P._call(ctx, "cfops_layernorm_forward", 0, None, w.data_ptr(), None, y.data_ptr(), s.data_ptr(), s.data_ptr(),
                 4, 8, 1e-5, 0)
