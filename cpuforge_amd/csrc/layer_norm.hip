@@ -135,6 +135,19 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void layernorm_fwd_kernel(
 #pragma unroll
             for (int i = 0; i < V; i++)
                 v[k][i] = load_raw<T>(x + (r0 + k) * dim + c0 + i * STEP, r0 + k < rows ? dim - c0 - i * STEP : 0);
+        // One row at a time, and registers for it: the weights are on their way beside it (65536 x 576
+        // f32 53 us where this took 62, 999 x 1001 3.9 and 4.5).
+        constexpr int AHEAD = R == 1 && V * N <= 16 ? V : 0;
+        float wa[AHEAD ? AHEAD : 1][N], ba[AHEAD ? AHEAD : 1][N];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            load_floats<N>(wa[i], w + c0 + i * STEP, dim - c0 - i * STEP);
+            if (b)
+                load_floats<N>(ba[i], b + c0 + i * STEP, dim - c0 - i * STEP);
+            else
+#pragma unroll
+                for (int e = 0; e < N; e++) ba[i][e] = 0.0f;
+        }
         float mu[R], rs[R];
 #pragma unroll
         for (int k = 0; k < R; k++) {
@@ -171,12 +184,17 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void layernorm_fwd_kernel(
             const int c = c0 + i * STEP;
             if (c >= dim) break;
             float ww[N], bb[N];
-            load_floats<N>(ww, w + c, dim - c);
-            if (b)
-                load_floats<N>(bb, b + c, dim - c);
-            else
+            if constexpr (AHEAD > 0) {
 #pragma unroll
-                for (int e = 0; e < N; e++) bb[e] = 0.0f;
+                for (int e = 0; e < N; e++) ww[e] = wa[i][e], bb[e] = ba[i][e];
+            } else {
+                load_floats<N>(ww, w + c, dim - c);
+                if (b)
+                    load_floats<N>(bb, b + c, dim - c);
+                else
+#pragma unroll
+                    for (int e = 0; e < N; e++) bb[e] = 0.0f;
+            }
 #pragma unroll
             for (int k = 0; k < R; k++) {
                 float o[N];
@@ -443,10 +461,12 @@ __global__ __launch_bounds__(256) void layernorm_columns_kernel(const T* __restr
 struct Form {
     int nw, v;
 };
-// The forward: the fewest waves whose lanes hold the row in up to four chunks each.
+// The forward: the fewest waves whose lanes hold the row in up to four chunks each, of bf16 three where
+// a wave has it alone (8192 x 2048 bf16 14.5 us of four waves, 18 of one; 30000 x 1001 f32 45 and 40).
+template <typename T>
 Form fwd_form(size_t chunks) {
     for (int nw : {1, 4, 8})
-        if (chunks <= (size_t)256 * nw) return {nw, (int)((chunks + 64 * nw - 1) / (64 * nw))};
+        if (chunks <= (size_t)(nw == 1 && sizeof(T) == 2 ? 192 : 256 * nw)) return {nw, (int)((chunks + 64 * nw - 1) / (64 * nw))};
     return {0, 0};
 }
 // The backward, whose lanes hold the weight and two sums of each column too: one wave while it
@@ -478,7 +498,7 @@ constexpr size_t kSlices = 32;
 template <typename T>
 hipError_t fwd(const T* x, const float* w, const float* b, T* y, float* mean, float* rstd, size_t rows, size_t dim,
                float eps, hipStream_t st) {
-    const Form f = fwd_form(chunks_of<T>(dim));
+    const Form f = fwd_form<T>(chunks_of<T>(dim));
     if (f.nw == 0) {
         hipLaunchKernelGGL(layernorm_fwd_wide_kernel<T>, dim3(blocks_of(rows)), dim3(kWide), 0, st, x, w, b, y, mean,
                            rstd, (long)rows, (int)dim, eps);
@@ -492,13 +512,15 @@ hipError_t fwd(const T* x, const float* w, const float* b, T* y, float* mean, fl
     if (f.nw == 1) {
         if (f.v == 1) return go(layernorm_fwd_kernel<T, 1, 1, 1>, 4);
         if (f.v == 2) return go(layernorm_fwd_kernel<T, 1, 2, 1>, 4);
-        if (f.v == 3) return go(layernorm_fwd_kernel<T, 1, 3, 1>, 4);
-        return go(layernorm_fwd_kernel<T, 1, 4, 1>, 4);
+        if (f.v == 3 || sizeof(T) == 2) return go(layernorm_fwd_kernel<T, 1, 3, 1>, 4);
+        return go(layernorm_fwd_kernel<T, 1, sizeof(T) == 2 ? 3 : 4, 1>, 4);
     }
     // Two rows at a time where that leaves every CU eight workgroups (16384 x 4096 bf16 54 us and
-    // 63; a wave that has a row alone gains nothing, 4096 x 2048 bf16 9.6 and 9.3).
+    // 63; a wave that has a row alone gains nothing).
     const bool two = rows >= 4096;
     if (f.nw == 4) {
+        if constexpr (sizeof(T) == 2)
+            if (f.v == 1) return two ? go(layernorm_fwd_kernel<T, 4, 1, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 1, 1>, 1);
         if (f.v == 2) return two ? go(layernorm_fwd_kernel<T, 4, 2, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 2, 1>, 1);
         if (f.v == 3) return two ? go(layernorm_fwd_kernel<T, 4, 3, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 3, 1>, 1);
         return two ? go(layernorm_fwd_kernel<T, 4, 4, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 4, 1>, 1);
