@@ -716,7 +716,8 @@ int head_grads(cfattn_ctx* c, const cfattn::HeadPlan& p, const cfattn::HeadBuffe
                const float* dlogp, const cfattn::HeadEntries* entries, size_t j0, size_t d, size_t vocab, float* dhn,
                float* dhead, bool acc, const HeadGrad& h, hipStream_t st) {
     for (size_t i = 0; dhn && i < p.chunk && j0 + i < t; i += p.pass)
-        CF_HIP(c, cfattn::launch_head_dhn(p, b, t, head, dlogp, entries, j0, i, std::min(p.chunk - i, p.pass), d, dhn, st),
+        CF_HIP(c, cfattn::launch_head_dhn(p, b, t, head, dlogp, entries, j0, i, std::min(p.chunk - i, p.pass), d, dhn,
+                                          st),
                "head gradient launch");
     for (size_t i = 0; dhead && i < p.chunk && j0 + i < t; i += h.pass)
         CF_HIP(c, cfattn::launch_head_dhead(p, b, t, dlogp, entries, j0, i, std::min({t - j0 - i, p.chunk - i, h.pass}),
@@ -778,7 +779,9 @@ cfattn::HeadPlan distill_plan(const Distill& q, size_t chunk_bytes) {
     p.tag = (int)((uint32_t)p.tag ^ (uint32_t)q.k * 0x27D4EB2Fu ^ 0x64697374u);
     return p;
 }
-size_t distill_kept_bytes(size_t t, size_t k) { return 2 * align_up(t * k * sizeof(int)) + align_up(2 * t * sizeof(int)); }
+size_t distill_kept_bytes(size_t t, size_t k) {
+    return 2 * align_up(t * k * sizeof(int)) + align_up(2 * t * sizeof(int));
+}
 void entries_at(size_t t, size_t k, char* base, Entries& e) {
     e.ids = reinterpret_cast<int*>(base);
     e.dl = reinterpret_cast<float*>(base + align_up(t * k * sizeof(int)));
@@ -799,7 +802,8 @@ int distill_entries(cfattn_ctx* c, const Distill& q, char* keep, Entries& e, hip
     entries_at(q.t, q.k, keep ? keep : base + own, e);
     cfattn::DistillEntries g{};
     g.raw_ids = q.ids, g.teacher = q.teacher, g.teacher_lse = q.teacher_lse, g.t = (long)q.t, g.vocab = (long)q.vocab;
-    g.k = (int)q.k, g.inv_t = q.inv_t, g.ids = e.ids, g.count = e.count, g.z = e.z, g.e = e.e, g.row = e.row, g.target = e.target;
+    g.k = (int)q.k, g.inv_t = q.inv_t, g.ids = e.ids, g.count = e.count, g.z = e.z, g.e = e.e, g.row = e.row;
+    g.target = e.target;
     CF_HIP(c, cfattn::launch_distill_entries(g, st), "distillation launch");
     return CFATTN_OK;
 }
@@ -878,18 +882,28 @@ int distill_backward_few(cfattn_ctx* c, const Distill& q, const float* hn, const
         CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, dloss, rows.idx, rows.count, tag, scaled, padded, q.d, st),
                "distillation launch");
     }
-    if (dhn)
-        CF_TRY(take(c, cfattn_ctx::OPS_PART, cfattn::distill_dhn_floats(std::min(q.t, rows.chunk), q.d, q.vocab) * sizeof(float),
-                    parts));
+    if (dhn) {
+        // (The last chunk's rows may be few enough for parts.)
+        size_t floats = 0;
+        for (size_t n : {std::min(q.t, rows.chunk), std::min({q.t, rows.chunk, cfattn::kDistillRowsHead})})
+            floats = std::max(floats, cfattn::distill_dhn_floats(n, q.d, q.vocab));
+        CF_TRY(take(c, cfattn_ctx::OPS_PART, floats * sizeof(float), parts));
+    }
     for (size_t j0 = 0; j0 < padded; j0 += rows.chunk) {
         const size_t nr = std::min(padded - j0, rows.chunk);
         if (!keep) CF_TRY(distill_few_logits(c, q, head, e, rows, j0, nr, nullptr, true, st));
         if (dhead)
             CF_TRY(gemm(c, CFOPS_TN, rows.logits, scaled + j0 * q.d, dhead, q.vocab, nr, q.d, acc || j0, st));
-        if (dhn && j0 < q.t)
-            CF_HIP(c, cfattn::launch_distill_dhn(rows.logits, j0, std::min(q.t - j0, nr), q.t, q.d, q.vocab, head, q.mul,
-                                                 dloss, rows.idx, rows.count, tag, parts, dhn, st),
+        if (!dhn || j0 >= q.t) continue;
+        const size_t n = std::min(q.t - j0, nr);
+        if (n <= cfattn::kDistillRowsHead)
+            CF_HIP(c, cfattn::launch_distill_rows_head(rows.logits, n, q.d, q.vocab, head, parts, st),
                    "distillation launch");
+        else
+            CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, parts, n, q.vocab, q.d, false, st));
+        CF_HIP(c, cfattn::launch_distill_rows_sum(parts, j0, n, q.t, q.d, q.vocab, q.mul, dloss, rows.idx, rows.count,
+                                                  tag, dhn, st),
+               "distillation launch");
     }
     return CFATTN_OK;
 }
@@ -959,7 +973,8 @@ int distill_backward_many(cfattn_ctx* c, const Distill& q, const float* hn, cons
         CF_TRY(distill_scratch(c, q, p, true, b));
         CF_TRY(head_scratch(c, p, q.t, b));
         CF_TRY(distill_entries(c, q, nullptr, e, st));
-        CF_HIP(c, cfattn::launch_logp_select(e.target, q.t, q.vocab, b.idx, b.count, p.tag, nullptr, nullptr, nullptr, st),
+        CF_HIP(c, cfattn::launch_logp_select(e.target, q.t, q.vocab, b.idx, b.count, p.tag, nullptr, nullptr, nullptr,
+                                             st),
                "distillation launch");
     }
     const cfattn::HeadEntries he{e.ids, e.count, e.dl, e.a, (int)q.k};
@@ -1079,7 +1094,8 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
     CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, 0, nullptr, nullptr, nullptr,
                                               st),
            "log-probability launch");
-    CF_HIP(c, cfattn::launch_logp_gather(hn, 1.0f, nullptr, rows.idx, rows.count, 0, rows.hn, padded, d, st), "log-probability launch");
+    CF_HIP(c, cfattn::launch_logp_gather(hn, 1.0f, nullptr, rows.idx, rows.count, 0, rows.hn, padded, d, st),
+           "log-probability launch");
     for (size_t j0 = 0; j0 < padded; j0 += rows.chunk) {
         const size_t nr = std::min(padded - j0, rows.chunk);
         float* h = rows.hn + j0 * d;

@@ -369,11 +369,16 @@ struct DistillRows {
 };
 size_t distill_slices(size_t vocab);
 hipError_t launch_distill_logits(float* logits, size_t nrows, bool grad, const DistillRows& g, hipStream_t st);
-// dhn, of t rows, of scored rows [j0, j0 + n), at most 64, and of those that are not, from the gradients
-// [n][vocab] of the logits of dloss = 1, in scratch `part` of distill_dhn_floats(n, d, vocab).
+// grads [n][vocab] . head into `part` of distill_dhn_floats(n, d, vocab) floats, in parts for up to
+// kDistillRowsHead rows, else (by launch_gemm_f32) whole: us of either, with the sum, 24 and 40 rows of
+// 49152 x 576 41 and 57, 62 and 56, of 49152 x 2048 112 and 134, 148 and 133.  sum: of t rows of dhn
+// those of scored rows [j0, j0 + n), and those that are not scored.
+constexpr size_t kDistillRowsHead = 32;
 size_t distill_dhn_floats(size_t n, size_t d, size_t vocab);
-hipError_t launch_distill_dhn(const float* grads, size_t j0, size_t n, size_t t, size_t d, size_t vocab,
-                              const float* head, float mul, const float* dloss, const int* idx, const int* count, int tag,
-                              float* part, float* dhn, hipStream_t st);
+hipError_t launch_distill_rows_head(const float* grads, size_t n, size_t d, size_t vocab, const float* head,
+                                    float* part, hipStream_t st);
+hipError_t launch_distill_rows_sum(const float* part, size_t j0, size_t n, size_t t, size_t d, size_t vocab, float mul,
+                                   const float* dloss, const int* idx, const int* count, int tag, float* dhn,
+                                   hipStream_t st);
 
 }  // namespace cfattn

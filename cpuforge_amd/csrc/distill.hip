@@ -34,10 +34,10 @@ __device__ __forceinline__ float max_wave(float x) {
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 // A row's entries by rising token, a wave to a row: ids, z and e [t][k] (count of them), their
-// exponentials below the largest's; the row's L, p_rest (negative: no rest) and p / e; target is a token of the row, kIgnoreIndex without entries, -1 where
-// the row is bad: a token out of the vocabulary or named twice, or a value of the teacher's that
+// exponentials below the largest's; the row's L, p_rest (negative: no rest) and p / e; target is a
+// token of the row, kIgnoreIndex without entries, -1 where the row is bad: a token out of the vocabulary or named twice, or a value of the teacher's that
 // is not finite.  (An entry whose id is kIgnoreIndex or whose logit is -inf is not there.)
-// Places are counts of smaller tokens: 4096 x 64 entries TODO us.
+// Places are counts of smaller tokens: 4096 x 64 entries 10 us.
 __global__ __launch_bounds__(256) void distill_entries_kernel(const DistillEntries g) {
     extern __shared__ int tokens[];  // [4][k]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -124,7 +124,9 @@ __device__ __forceinline__ double entry_loss(const TeacherRow& row, float z, flo
 }
 
 // 2^x; the f32 instruction where f32 holds it.
-__device__ __forceinline__ double pow2(double x) { return x > -120.0 ? (double)__builtin_amdgcn_exp2f((float)x) : exp2(x); }
+__device__ __forceinline__ double pow2(double x) {
+    return x > -120.0 ? (double)__builtin_amdgcn_exp2f((float)x) : exp2(x);
+}
 
 // Rows whose product kept exp2(y - m) of 128 logits each (y in units of log2, m the largest):
 // a wave to a row.  An entry whose exponential is too small, and
@@ -136,8 +138,8 @@ __device__ __forceinline__ double pow2(double x) { return x > -120.0 ? (double)_
 // much larger than its 128's largest (a near 0, a student that holds the token for unlikely), or
 // the rest is far below the entry, it becomes 0 and the entry stays in ids and dl (count of them).
 // (A sure student's a q would cancel in the entries: a is -p_rest / q_rest then.)
-// 3686 rows of 64 entries, 49152 tokens: TODO us, a chain of a few loads: what a row needs is
-// loaded at once, the entries' to LDS (one by one where it was used 55).
+// 3686 rows of 64 entries, 49152 tokens: 45 us, a chain of a few loads, values of a row far apart: what
+// a row needs is loaded at once, the entries' to LDS (one by one where it was used 55).
 struct EntryLds {
     int v;
     float kept;
@@ -345,8 +347,8 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
 // Rows of logits in memory, kSlice of them to a workgroup, in two launches: the largest and the sum
 // of exponentials of each slice's tokens that are no entries (so the rest is a sum of its own),
 // and the entries' logits; then the loss, where it is wanted, and with GRAD the logits become
-// their gradients (zeros from the last scored row on).  19 rows of 49152 with their gradients
-// TODO us (a row to a workgroup 27).
+// their gradients (zeros from the last scored row on).  24 rows of 49152, 16 of them scored, with
+// their gradients 12.5 us (a row to a workgroup 27).
 constexpr int kSlice = 4096, kSliceThreads = 512, kPer = kSlice / kSliceThreads;
 
 // Whether value i of a slice is an entry's, for the values of this thread.
@@ -480,8 +482,8 @@ __device__ __forceinline__ f32x4 load4(const float* __restrict__ p, long n) {
 // the f32 MFMA: a workgroup 64 columns of the head, a wave 16 of its tokens at a time (v_mfma_f32_16x16x4:
 // lane l has A[l % 16][l / 16] and B[l / 16][l % 16]; product s of 16 tokens takes 4 (l / 16) + s, product
 // q of 64 columns 4 (l % 16) + q, so that every load is of four values side by side).
-// Bound by reading the head: 24 rows of 49152 x 576 TODO us (split into f16 pieces, by the products of
-// many rows, 55).
+// Bound by reading the head: 9 rows of 49152 x 576 (113 MB) 23 us, 4.9 TB/s; 24 rows 37, with as many bytes
+// of gradients again from the caches (split into bf16 pieces, by launch_gemm_f32, 55).
 template <int TT>
 __global__ __launch_bounds__(256) void distill_rows_head_kernel(const float* __restrict__ grads, long vocab, int t,
                                                                 const float* __restrict__ head, int d, int blocks,
@@ -497,27 +499,20 @@ __global__ __launch_bounds__(256) void distill_rows_head_kernel(const float* __r
 #pragma unroll
     for (int i = 0; i < TT; i++) g[i] = grads + min(16 * i + l16, t - 1) * vocab;
     f32x4 acc[TT][4] = {};
-    constexpr int U = 2;  // chunks whose loads are in flight together
-    for (long k = chunks * split / splits + U * wave; k < end; k += 4 * U) {
-        f32x4 a[U][TT], b[U][4];
+    for (long k = chunks * split / splits + wave; k < end; k += 4) {
+        const long v = k * 16 + 4 * kq, live = vocab - v;
+        f32x4 a[TT], b[4];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const long v = (k + u) * 16 + 4 * kq;
-            const long live = k + u < end ? vocab - v : 0;
+        for (int i = 0; i < TT; i++) a[i] = load4(g[i] + v, live);
 #pragma unroll
-            for (int i = 0; i < TT; i++) a[u][i] = load4(g[i] + v, live);
+        for (int s = 0; s < 4; s++) b[s] = load4(head + (v + s) * d + c, s < live ? d - c : 0);
 #pragma unroll
-            for (int s = 0; s < 4; s++) b[u][s] = load4(head + (v + s) * d + c, s < live ? d - c : 0);
-        }
+        for (int s = 0; s < 4; s++)
 #pragma unroll
-        for (int u = 0; u < U; u++)
+            for (int i = 0; i < TT; i++)
 #pragma unroll
-            for (int s = 0; s < 4; s++)
-#pragma unroll
-                for (int i = 0; i < TT; i++)
-#pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        acc[i][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][i][s], b[u][s][q], acc[i][q], 0, 0, 0);
+                for (int q = 0; q < 4; q++)
+                    acc[i][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][s], b[s][q], acc[i][q], 0, 0, 0);
     }
     // Row 16 i + 4 kq + e and column 4 l16 + q of the result are in acc[i][q][e]; wave after wave.
     for (int w = 0; w < 4; w++) {
@@ -570,7 +565,8 @@ __global__ __launch_bounds__(256) void distill_rows_sum_kernel(const float* __re
 }  // namespace
 
 hipError_t launch_distill_entries(const DistillEntries& g, hipStream_t st) {
-    hipLaunchKernelGGL(distill_entries_kernel, dim3((unsigned)((g.t + 3) / 4)), dim3(256), 4 * g.k * sizeof(int), st, g);
+    hipLaunchKernelGGL(distill_entries_kernel, dim3((unsigned)((g.t + 3) / 4)), dim3(256), 4 * g.k * sizeof(int), st,
+                       g);
     return hipGetLastError();
 }
 hipError_t launch_distill_kept(const DistillKept& g, hipStream_t st) {
@@ -590,25 +586,30 @@ hipError_t launch_distill_logits(float* logits, size_t nrows, bool grad, const D
     return hipGetLastError();
 }
 
-// Workgroups of the product: four to a CU, of 16 tokens and more.
+// Splits of the product: two workgroups to a CU (us with four, of 9 rows of 49152 x 576 and 24 of them:
+// 23 and 35 where two take 23 and 37, but 64 of 49152 x 1024 111 and 79).
 static size_t rows_head_splits(size_t d, size_t vocab) {
     const size_t blocks = (d + 63) / 64;
-    return std::max<size_t>(std::min((1024 + blocks - 1) / blocks, (vocab + 63) / 64), 1);
+    return std::max<size_t>(std::min((512 + blocks - 1) / blocks, (vocab + 63) / 64), 1);
 }
-size_t distill_dhn_floats(size_t t, size_t d, size_t vocab) { return rows_head_splits(d, vocab) * t * d; }
-hipError_t launch_distill_dhn(const float* grads, size_t j0, size_t n, size_t t, size_t d, size_t vocab,
-                              const float* head, float mul, const float* dloss, const int* idx, const int* count, int tag,
-                              float* part, float* dhn, hipStream_t st) {
+size_t distill_dhn_floats(size_t n, size_t d, size_t vocab) {
+    return (n <= kDistillRowsHead ? rows_head_splits(d, vocab) : 1) * n * d;
+}
+hipError_t launch_distill_rows_head(const float* grads, size_t n, size_t d, size_t vocab, const float* head,
+                                    float* part, hipStream_t st) {
     const unsigned blocks = (unsigned)((d + 63) / 64), splits = (unsigned)rows_head_splits(d, vocab);
-    const auto kernel = n <= 16   ? distill_rows_head_kernel<1>
-                        : n <= 32 ? distill_rows_head_kernel<2>
-                                  : distill_rows_head_kernel<4>;
-    hipLaunchKernelGGL(kernel, dim3((splits + 7) / 8 * 8 * blocks), dim3(256), 0, st, grads, (long)vocab, (int)n, head,
-                       (int)d, (int)blocks, (int)splits, part);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(distill_rows_sum_kernel, dim3(blocks, (unsigned)t), dim3(256), 0, st, part, (int)splits, (int)j0,
-                       (int)n, (int)d, mul, dloss, idx, count, tag, dhn);
+    static_assert(kDistillRowsHead == 32, "the rows of a wave");
+    hipLaunchKernelGGL((n <= 16 ? distill_rows_head_kernel<1> : distill_rows_head_kernel<2>),
+                       dim3((splits + 7) / 8 * 8 * blocks), dim3(256), 0, st, grads, (long)vocab, (int)n, head, (int)d,
+                       (int)blocks, (int)splits, part);
+    return hipGetLastError();
+}
+hipError_t launch_distill_rows_sum(const float* part, size_t j0, size_t n, size_t t, size_t d, size_t vocab, float mul,
+                                   const float* dloss, const int* idx, const int* count, int tag, float* dhn,
+                                   hipStream_t st) {
+    const size_t splits = distill_dhn_floats(n, d, vocab) / (n * d);
+    hipLaunchKernelGGL(distill_rows_sum_kernel, dim3((unsigned)((d + 63) / 64), (unsigned)t), dim3(256), 0, st, part,
+                       (int)splits, (int)j0, (int)n, (int)d, mul, dloss, idx, count, tag, dhn);
     return hipGetLastError();
 }
 

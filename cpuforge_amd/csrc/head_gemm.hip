@@ -806,7 +806,8 @@ __global__ __launch_bounds__(1024) void head_finish_kernel(const float2* __restr
 // dhn of scored rows [j0, ..): dlogp (head[target] - the splits' sums in order), or, with
 // entries, mul dloss (a times those sums + the sum of the entries' dl head).
 // Four columns to a thread, eight splits' sums in flight: bound by memory, 3686 x 576 with
-// 16 splits (136 MB) 29 us; with 64 entries of each row (543 MB of the head, in the caches) TODO.
+// 16 splits (136 MB) 29 us; with up to 64 entries of each row, whose rows of the head are in the
+// caches, 45 (90 with all 64 of each).
 template <bool ENTRIES>
 __global__ __launch_bounds__(256) void head_grad_reduce_kernel(const float* __restrict__ part, int chunk, int rows,
                                                                int mt, int k16, int splits_max,
@@ -1156,8 +1157,8 @@ hipError_t launch_head_dhn(const HeadPlan& p, const HeadBuffers& b, size_t t, co
     if (e != hipSuccess) return e;
     const size_t quads = rows * ((d + 3) / 4);
     hipLaunchKernelGGL((entries ? head_grad_reduce_kernel<true> : head_grad_reduce_kernel<false>),
-                       dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, b.part, g.chunk, (int)p.d_pad, g.mt, g.ka,
-                       g.splits_max, b.idx, b.idx + t, b.count, p.tag, g.j0, head, dlogp, dhn, (int)d,
+                       dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, b.part, g.chunk, (int)p.d_pad, g.mt,
+                       g.ka, g.splits_max, b.idx, b.idx + t, b.count, p.tag, g.j0, head, dlogp, dhn, (int)d,
                        entries ? *entries : HeadEntries{}, b.mul);
     return hipGetLastError();
 }
@@ -1174,8 +1175,8 @@ hipError_t launch_head_dhead(const HeadPlan& p, const HeadBuffers& b, size_t t, 
     if (e != hipSuccess) return e;
     const unsigned t32 = (unsigned)((rows + 31) / 32), v128 = (unsigned)(p.v_pad / 128);
     if (entries) g.en = *entries;
-    hipLaunchKernelGGL((entries ? head_col_top_kernel<true> : head_col_top_kernel<false>), dim3(v128, std::min(t32, 8u)),
-                       dim3(256), 0, st, g);
+    hipLaunchKernelGGL((entries ? head_col_top_kernel<true> : head_col_top_kernel<false>),
+                       dim3(v128, std::min(t32, 8u)), dim3(256), 0, st, g);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     if (entries) {
         hipLaunchKernelGGL(head_entries_top_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, g);

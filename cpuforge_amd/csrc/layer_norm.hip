@@ -466,7 +466,8 @@ struct Form {
 template <typename T>
 Form fwd_form(size_t chunks) {
     for (int nw : {1, 4, 8})
-        if (chunks <= (size_t)(nw == 1 && sizeof(T) == 2 ? 192 : 256 * nw)) return {nw, (int)((chunks + 64 * nw - 1) / (64 * nw))};
+        if (chunks <= (size_t)(nw == 1 && sizeof(T) == 2 ? 192 : 256 * nw))
+            return {nw, (int)((chunks + 64 * nw - 1) / (64 * nw))};
     return {0, 0};
 }
 // The backward, whose lanes hold the weight and two sums of each column too: one wave while it
@@ -520,7 +521,8 @@ hipError_t fwd(const T* x, const float* w, const float* b, T* y, float* mean, fl
     const bool two = rows >= 4096;
     if (f.nw == 4) {
         if constexpr (sizeof(T) == 2)
-            if (f.v == 1) return two ? go(layernorm_fwd_kernel<T, 4, 1, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 1, 1>, 1);
+            if (f.v == 1)
+                return two ? go(layernorm_fwd_kernel<T, 4, 1, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 1, 1>, 1);
         if (f.v == 2) return two ? go(layernorm_fwd_kernel<T, 4, 2, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 2, 1>, 1);
         if (f.v == 3) return two ? go(layernorm_fwd_kernel<T, 4, 3, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 3, 1>, 1);
         return two ? go(layernorm_fwd_kernel<T, 4, 4, 2>, 2) : go(layernorm_fwd_kernel<T, 4, 4, 1>, 1);
@@ -537,8 +539,8 @@ hipError_t bwd(const T* dy, const T* x, const float* w, const float* mean, const
     size_t parts;
     hipError_t e;
     if (f.nw == 0) {
-        hipLaunchKernelGGL(layernorm_bwd_wide_kernel<T>, dim3(blocks_of(rows)), dim3(kWide), 0, st, dy, x, w, mean, rstd,
-                           dx, (long)rows, (int)dim, acc);
+        hipLaunchKernelGGL(layernorm_bwd_wide_kernel<T>, dim3(blocks_of(rows)), dim3(kWide), 0, st, dy, x, w, mean,
+                           rstd, dx, (long)rows, (int)dim, acc);
         if ((e = hipGetLastError()) != hipSuccess || !sums) return e;
         parts = std::min(kSlices, rows);
         hipLaunchKernelGGL(layernorm_columns_kernel<T>, dim3((unsigned)((dim + 255) / 256), (unsigned)parts),

@@ -472,8 +472,8 @@ def lm_head_distill(hn, head, ids, teacher, t, d, vocab, k, loss, result, teache
     row's loss is NaN.  `keep` (a uint8 tensor of lm_head_distill_keep_bytes, when
     given) takes what the backward reads.  No host wait."""
     ctx = ctx or default_context()
-    _call(ctx, "cfops_lm_head_distill", *_distill(hn, head, ids, teacher, teacher_lse, t, d, vocab, k, ctx), t, d, vocab,
-          k, float(temperature), _on(loss, "loss", ctx, numel=t), _result(_here(result, ctx), CE_RESULT_WORDS),
+    _call(ctx, "cfops_lm_head_distill", *_distill(hn, head, ids, teacher, teacher_lse, t, d, vocab, k, ctx), t, d,
+          vocab, k, float(temperature), _on(loss, "loss", ctx, numel=t), _result(_here(result, ctx), CE_RESULT_WORDS),
           *_keep(_here(keep, ctx)), _stream_of(ctx))
 
 

@@ -243,7 +243,8 @@ class SmolLM:
         wait: check_targets() reports entries that it does not take)."""
         if self.backend != "cfops":
             raise ValueError("distillation needs the cfops backend")
-        loss, res = A.lm_head_distill(self.hidden(tokens, positions), self.embed, ids, teacher, teacher_lse, temperature)
+        loss, res = A.lm_head_distill(self.hidden(tokens, positions), self.embed, ids, teacher, teacher_lse,
+                                      temperature)
         self._ce = (res, None)
         return loss
 
