@@ -74,7 +74,8 @@ class Exact:
         some = p_rest > 0
         ratio = torch.where(some, p_rest / log_rest.exp(), 0.0)
         loss = torch.where(named, torch.xlogy(p, p) - p * log_q, 0.0).sum(1)
-        loss = loss + torch.where(some, p_rest * (p_rest.clamp(min=1e-300).log() - torch.where(some, log_rest, 0.0)), 0.0)
+        rest = p_rest * (p_rest.clamp(min=1e-300).log() - torch.where(some, log_rest, 0.0))
+        loss = loss + torch.where(some, rest, 0.0)
         dx = torch.where(named, q - p, q * (1 - ratio)[:, None])
         g = torch.where(self.use, dloss.double(), 0.0)
         self.loss = torch.where(self.use, loss, 0.0)
@@ -450,7 +451,8 @@ def test_refusals():
     loss, res = torch.empty(80, device=DEV), P.ce_result_buffer(DEV)
     ok = dict(hn=hn, head=head, ids=ids, teacher=z, t=80, d=16, vocab=100, k=5, loss=loss, result=res)
     P.lm_head_distill(**ok)
-    for change, error in ((dict(hn=hn.half()), TypeError), (dict(ids=ids.int()), TypeError), (dict(ids=ids.cpu()), TypeError),
+    for change, error in ((dict(hn=hn.half()), TypeError), (dict(ids=ids.int()), TypeError),
+                          (dict(ids=ids.cpu()), TypeError),
                           (dict(teacher=z.double()), TypeError), (dict(t=79), ShapeError), (dict(k=4), ShapeError),
                           (dict(teacher_lse=loss[:70]), ShapeError), (dict(temperature=0.0), CfattnError),
                           (dict(temperature=-1.0), CfattnError), (dict(temperature=math.nan), CfattnError),

@@ -252,7 +252,8 @@ def test_refusals():
     big = tables(10, 9)
     for args, error in (((x, y, *big), ShapeError), ((x, y[:, :4], cos, sin), ShapeError),
                         ((x[0], y[0], cos, sin), ShapeError), ((x.cpu(), y, cos, sin), TypeError),
-                        ((x.half(), y, cos, sin), TypeError), ((x, y, cos, sin[:9]), ShapeError), ((x, y, cos, sin.t().contiguous()), ShapeError),
+                        ((x.half(), y, cos, sin), TypeError), ((x, y, cos, sin[:9]), ShapeError),
+                        ((x, y, cos, sin.t().contiguous()), ShapeError),
                         ((x, y, cos[0], sin[0]), ShapeError), ((x, y, cos.double(), sin), TypeError),
                         ((x.transpose(2, 3), y.transpose(2, 3), cos[:, :1].contiguous(), sin[:, :1].contiguous()),
                          ValueError),
