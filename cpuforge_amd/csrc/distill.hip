@@ -31,6 +31,11 @@ __device__ __forceinline__ float max_wave(float x) {
     for (int o = 32; o >= 1; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
     return x;
 }
+// What a wave's lanes wrote to its LDS is there for the others.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 // A row's entries by rising token, a wave to a row: ids, z and e [t][k] (count of them), their
@@ -66,7 +71,7 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const DistillEntri
         }
         n += __popcll(__ballot(v != INT_MAX));
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     top = max_wave(top);
     double sum = 0.0;
     int least = INT_MAX;
@@ -170,7 +175,7 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
         const int v = g.ids[r * g.k + k];
         mine[k] = {v, kept(v), stat(v / 128)};
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     const TeacherRow row = g.row[r];
     bool with_rest = row.p_rest > 0.0;
     auto has_entry = [&](int part) {
@@ -284,8 +289,14 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
     }
     const double log_total = log(total), unit = 1.0 / (double)kLog2e;
     const Rest r_(row.p_rest, log(rest) - log_total);
-    // (A rest so small has no exponentials in f32 either.)
-    const float a = (float)(1.0 - fmin(r_.ratio, 1e30));
+    // Where the rest is so small that f32 holds neither a nor all of its exponentials, a is 2^-lift
+    // of itself and every factor 2^lift (a part's largest is up to 2^10 above the rest, or its entries
+    // stay in the list and its factor follows below).
+    const double lift = with_rest && rest > 0.0 && rest < 0x1p-60 * total ? floor(log2(total / rest)) : 0.0;
+    const float a = lift > 0.0 ? (float)(exp2(-lift) - exp(log(row.p_rest) - log(rest) + log_total - lift * M_LN2))
+                               : (float)(1.0 - fmin(r_.ratio, 1e30));
+    auto lifted = [&](float x) { return (float)(exp2(fmin((double)x - top + lift, 120.0)) / total); };
+    if (g.dl && lift > 0.0) each([&](int p, const float2& s) { g.factor[(long)p * g.ld + j] = lifted(s.x); });
     double terms = 0.0;
     int stay = 0;
     for (int k0 = 0; k0 < n; k0 += 64) {
@@ -306,7 +317,8 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
             terms += entry_loss(row, g.z[r * g.k + k], g.e[r * g.k + k], g.inv_t, q, y * unit - log_total, dl);
         if (!g.dl) continue;
         const bool far = with_rest && pow2(up) * 0x1p-10 > rest;
-        const float in = live ? (float)dl / (a * g.factor[(long)(v / 128) * g.ld + j]) : 0.0f;
+        const float factor = !live ? 1.0f : lift > 0.0 ? lifted(en.stat.x) : g.factor[(long)(v / 128) * g.ld + j];
+        const float in = live ? (float)dl / (a * factor) : 0.0f;
         // (Up to 2 the product's f16 pieces hold it.)
         const bool stays = live && (far || !(fabsf(in) <= 1.5f));
         const unsigned long long staying = __ballot(stays);
@@ -327,8 +339,42 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
         for (unsigned long long todo = __ballot(far); todo; todo &= todo - 1) {
             const int at = k0 + __ffsll(todo) - 1, part = mine[at].v / 128;
             float x4[4];
-            others(at, x4);
+            const int last = others(at, x4);
             const float most = max_wave(fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])));
+            if (lift > 0.0) {
+                // (By a factor of their own, and formed again where f32 holds too little of them.)
+                double y4[4], y_most = -INFINITY;
+                if (most >= 128.0f * kLost * 0x1p18f) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y4[i] = log2((double)x4[i]) + (double)mine[at].stat.x - top;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y4[i] = -INFINITY;
+                    const int end = min(part * 128 + 128, g.vocab);
+                    for (int v = part * 128, e = at; v < end; v++) {
+                        if (e < last && mine[e].v == v) {
+                            e++;
+                            continue;
+                        }
+                        const double y = logit(v) - top;
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (lane < 32 && v4 + i == v % 128) y4[i] = y;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) y_most = fmax(y_most, y4[i]);
+#pragma unroll
+                for (int o = 32; o >= 1; o >>= 1) y_most = fmax(y_most, __shfl_xor(y_most, o));
+                if (!(y_most > -INFINITY)) continue;
+                y_most = floor(y_most);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (lane < 32 && part * 128 + v4 + i < g.vocab)
+                        kept(part * 128 + v4 + i) = (float)exp2(y4[i] - y_most);
+                if (lane == 0) g.factor[(long)part * g.ld + j] = (float)(exp2(y_most + lift) / total);
+                continue;
+            }
             const int up = min(max(127 - (int)(__builtin_bit_cast(uint32_t, most) >> 23), 0), 126);
             if (!(most > 0.0f) || up == 0) continue;
             const float times = __builtin_bit_cast(float, (uint32_t)(127 + up) << 23);
@@ -452,8 +498,10 @@ __global__ __launch_bounds__(kSliceThreads) void distill_logits_kernel(float* __
         if (lane == 0) g.loss[r] = (float)(r_.loss + terms);
     }
     if (!GRAD) return;
-    // (By the rest's own largest: a q of a confident student's is not small where q is.)
-    const float f = (float)((1.0 - r_.ratio) * exp(shift) / total), base = m > -INFINITY ? m : 0.0f;
+    // a q of the others by their own largest: a q of a sure student's is not small where q is (and
+    // p_rest / q_rest may be past what f64 holds).
+    const float f = (float)(exp(shift) / total - (row.p_rest > 0.0 ? row.p_rest / rest : 0.0));
+    const float base = m > -INFINITY ? m : 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
         const long v = v0 + threadIdx.x + i * kSliceThreads;

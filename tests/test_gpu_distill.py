@@ -180,8 +180,7 @@ def test_students_from_uniform_to_sure(t, sharp, share):
 def test_a_rest_far_below_the_entries(t):
     """One token of each row holds all but e^-40 of the student's probability, so every
     rest is formed from exponentials far below 2^-24 of the sums they stand in; at e^-120
-    from logits formed again, where f32 holds no exponential (loss alone: its gradient
-    along such a rest is not held either)."""
+    and below from logits formed again, where f32 holds no exponential and no p_rest / q_rest."""
     g = torch.Generator(device=DEV).manual_seed(t)
     d, vocab = 64, 700
     head = torch.randn(vocab, d, generator=g, device=DEV) * 0.05
@@ -192,15 +191,26 @@ def test_a_rest_far_below_the_entries(t):
     dloss = torch.randn(t, generator=g, device=DEV)
     lse = teacher_lse(ids, z, 1.0, share=0.2)
     own = head[ids[:, 0]]
-    for far in (40.0, 120.0):
-        lifted = hn + far / (own * own).sum(1, keepdim=True) * own
-        if far < 80:
-            check(lifted, head, ids, z, lse, 1.0, dloss)
-            continue
-        want = Exact(lifted, head, ids, z, lse, 1.0, dloss)
-        loss, res = forward(lifted, head, ids, z, lse, 1.0)
-        P.distill_check(res)
-        near(loss, want.loss, want.tol_loss, "loss")
+    for far in (40.0, 60.0, 120.0, 400.0):
+        check(hn + far / (own * own).sum(1, keepdim=True) * own, head, ids, z, lse, 1.0, dloss)
+
+
+@pytest.mark.parametrize("t", [20, 150])
+def test_a_rest_far_below_entries_in_every_part(t):
+    """As above with entries in each 128 tokens, some far above, some among the others: no
+    part of the vocabulary is of the rest alone."""
+    g = torch.Generator(device=DEV).manual_seed(t)
+    d, vocab = 64, 300
+    head = torch.randn(vocab, d, generator=g, device=DEV) * 0.05
+    ids = (torch.tensor([5, 100, 130, 200, 290], device=DEV) + torch.arange(t, device=DEV)[:, None] % 5).contiguous()
+    z = torch.randn(t, 5, generator=g, device=DEV)
+    hn = torch.randn(t, d, generator=g, device=DEV)
+    dloss = torch.randn(t, generator=g, device=DEV)
+    head[[5, 6, 7, 8, 9, 130, 131, 132, 133, 134], 0] = 3.0
+    for far in (30.0, 90.0, 200.0):
+        hn[:, 0] = far
+        head[head[:, 0] != 3.0, 0] = 0.0
+        check(hn, head, ids, z, teacher_lse(ids, z, 1.0, share=0.2), 1.0, dloss)
 
 
 @pytest.mark.parametrize("t", [30, 300])
