@@ -604,15 +604,13 @@ struct LogpRows {
     float *hn, *logits;
     size_t chunk;
 };
-// (all: the logits of all rows are in the caller's memory.)
-int logp_rows(cfattn_ctx* c, size_t t, size_t d, size_t vocab, LogpRows& r, bool all = false) {
+int logp_rows(cfattn_ctx* c, size_t t, size_t d, size_t vocab, LogpRows& r) {
     // A chunk's logits fit the head's limit, its rows a launch of workgroups.
     r.chunk = std::min<size_t>(c->head_chunk_bytes / (vocab * sizeof(float)), (size_t)1 << 22);
-    r.chunk = all ? t : std::min(std::max<size_t>(r.chunk, 1), t);
+    r.chunk = std::min(std::max<size_t>(r.chunk, 1), t);
     CF_TRY(take(c, cfattn_ctx::OPS_IDX, (4 + 2 * t) * sizeof(int), r.count));
     r.idx = r.count + 4;
     CF_TRY(take(c, cfattn_ctx::OPS_ROWS, t * d * sizeof(float), r.hn));
-    if (all) return CFATTN_OK;
     return take(c, cfattn_ctx::OPS_LOGITS, r.chunk * vocab * sizeof(float), r.logits);
 }
 
@@ -788,7 +786,9 @@ void entries_at(size_t t, size_t k, char* base, Entries& e) {
     e.count = reinterpret_cast<int*>(base + 2 * align_up(t * k * sizeof(int)));
     e.a = reinterpret_cast<float*>(e.count + t);
 }
-int distill_entries(cfattn_ctx* c, const Distill& q, char* keep, Entries& e, hipStream_t st) {
+// (kept: takes the targets and the tag.)
+int distill_entries(cfattn_ctx* c, const Distill& q, char* keep, Entries& e, hipStream_t st,
+                    const cfattn::DistillScored* kept = nullptr) {
     const size_t rows = align_up(q.t * sizeof(cfattn::TeacherRow)), targets = align_up(q.t * sizeof(int64_t));
     const size_t values = align_up(q.t * q.k * sizeof(float));
     const size_t own = rows + targets + 2 * values + align_up(q.t * sizeof(float));
@@ -804,28 +804,60 @@ int distill_entries(cfattn_ctx* c, const Distill& q, char* keep, Entries& e, hip
     g.raw_ids = q.ids, g.teacher = q.teacher, g.teacher_lse = q.teacher_lse, g.t = (long)q.t, g.vocab = (long)q.vocab;
     g.k = (int)q.k, g.inv_t = q.inv_t, g.ids = e.ids, g.count = e.count, g.z = e.z, g.e = e.e, g.row = e.row;
     g.target = e.target;
+    if (kept) {
+        g.target = const_cast<int64_t*>(kept->target);
+        g.tag_at = const_cast<int*>(kept->tag_at), g.tag = kept->tag;
+    }
     CF_HIP(c, cfattn::launch_distill_entries(g, st), "distillation launch");
     return CFATTN_OK;
 }
 
-// Few rows: logits in memory, a chunk of rows at a time, which become the gradients of dloss = 1; the
-// rows of dhn, and in dhead those of hn, are times theirs.  What a forward keeps is those
-// gradients of all rows.
-int distill_tag(const Distill& q) { return distill_plan(q, SIZE_MAX).tag; }
+// Few rows: products hn . head in memory, a chunk of rows at a time, which become the gradients of
+// dloss = 1; the rows of dhn, and in dhead those of hn, are times theirs.  What a forward keeps is
+// those gradients, and which rows are scored.
+struct FewRows {
+    cfattn::DistillScored scored;
+    float* logits;
+    size_t chunk;
+};
 // (Whole steps of 32 rows, as lm_head_logprobs' gradient of the head takes.)
 size_t few_padded(size_t t) { return t > 16 ? (t + 31) / 32 * 32 : t; }
-size_t few_index_bytes(size_t t) { return align_up((4 + 2 * few_padded(t)) * sizeof(int)); }
+size_t few_index_bytes(size_t t) { return align_up(4 * sizeof(int) + t * sizeof(int64_t)); }
 size_t few_keep_bytes(size_t t, size_t vocab) { return few_index_bytes(t) + few_padded(t) * vocab * sizeof(float); }
 
-int distill_few_logits(cfattn_ctx* c, const Distill& q, const float* head, const Entries& e, const LogpRows& rows,
-                       size_t j0, size_t nr, float* loss, bool grad, hipStream_t st) {
+// Where the rows' products go, `padded` rows with a keep, else a chunk that fits the head's limit; with
+// a forward's keep, what it left there, else this call's entries.
+int distill_few_rows(cfattn_ctx* c, const Distill& q, size_t padded, const void* keep, size_t keep_bytes, bool forward,
+                     Entries& e, FewRows& rows, hipStream_t st) {
+    rows.chunk = padded;
+    rows.scored.t = (int)q.t;
+    if (keep) {
+        CF_TRY(check_keep(c, keep, keep_bytes, few_keep_bytes(q.t, q.vocab)));
+        char* base = static_cast<char*>(const_cast<void*>(keep));
+        rows.scored.tag_at = reinterpret_cast<int*>(base);
+        rows.scored.tag = distill_plan(q, SIZE_MAX).tag;
+        rows.scored.target = reinterpret_cast<int64_t*>(base + 4 * sizeof(int));
+        rows.logits = reinterpret_cast<float*>(base + few_index_bytes(q.t));
+        return forward ? distill_entries(c, q, nullptr, e, st, &rows.scored) : CFATTN_OK;
+    }
+    rows.chunk = std::min(std::max<size_t>(c->head_chunk_bytes / (q.vocab * sizeof(float)), 1), padded);
+    CF_TRY(take(c, cfattn_ctx::OPS_LOGITS, rows.chunk * q.vocab * sizeof(float), rows.logits));
+    CF_TRY(distill_entries(c, q, nullptr, e, st));
+    rows.scored.target = e.target;
+    return CFATTN_OK;
+}
+
+int distill_few_logits(cfattn_ctx* c, const Distill& q, const float* hn, const float* head, const Entries& e,
+                       const FewRows& rows, size_t j0, size_t nr, float* loss, bool grad, hipStream_t st) {
     cfattn::DistillRows g{};
     g.ids = e.ids, g.count = e.count, g.z = e.z, g.e = e.e, g.row = e.row, g.k = (int)q.k, g.inv_t = q.inv_t;
-    g.idx = rows.idx, g.scored = rows.count, g.j0 = (int)j0, g.vocab = (long)q.vocab, g.loss = loss;
+    g.target = rows.scored.target, g.t = (long)q.t, g.j0 = (int)j0, g.vocab = (long)q.vocab, g.mul = q.mul;
+    g.loss = loss;
     const size_t slices = nr * cfattn::distill_slices(q.vocab);
     CF_TRY(take(c, cfattn_ctx::OPS_STATS, slices * sizeof(float2) + nr * q.k * sizeof(float), g.slices));
     g.xs = reinterpret_cast<float*>(g.slices + slices);
-    CF_TRY(gemm(c, CFOPS_NT, rows.hn + j0 * q.d, head, rows.logits, nr, q.d, q.vocab, false, st));
+    if (j0 < q.t)
+        CF_TRY(gemm(c, CFOPS_NT, hn + j0 * q.d, head, rows.logits, std::min(nr, q.t - j0), q.d, q.vocab, false, st));
     CF_HIP(c, cfattn::launch_distill_logits(rows.logits, nr, grad, g, st), "distillation launch");
     return CFATTN_OK;
 }
@@ -833,53 +865,26 @@ int distill_few_logits(cfattn_ctx* c, const Distill& q, const float* head, const
 int distill_few(cfattn_ctx* c, const Distill& q, const float* hn, const float* head, float* loss, void* result,
                 void* keep, size_t keep_bytes, hipStream_t st) {
     Entries e{};
-    CF_TRY(distill_entries(c, q, nullptr, e, st));
-    const size_t padded = few_padded(q.t);
-    LogpRows rows{};
-    CF_TRY(logp_rows(c, padded, q.d, q.vocab, rows, keep != nullptr));
-    if (keep) {
-        CF_TRY(check_keep(c, keep, keep_bytes, few_keep_bytes(q.t, q.vocab)));
-        rows.count = static_cast<int*>(keep);
-        rows.idx = rows.count + 4;
-        rows.logits = reinterpret_cast<float*>(static_cast<char*>(keep) + few_index_bytes(q.t));
-    }
-    CF_HIP(c, cfattn::launch_logp_select(e.target, q.t, q.vocab, rows.idx, rows.count, distill_tag(q), loss, e.none,
-                                         result, st),
-           "distillation launch");
-    CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, nullptr, rows.idx, rows.count, distill_tag(q), rows.hn, padded, q.d,
-                                         st),
-           "distillation launch");
-    const size_t all = keep ? padded : q.t;
+    FewRows rows{};
+    const size_t all = keep ? few_padded(q.t) : q.t;
+    CF_TRY(distill_few_rows(c, q, all, keep, keep_bytes, true, e, rows, st));
     for (size_t j0 = 0; j0 < all; j0 += rows.chunk)
-        CF_TRY(distill_few_logits(c, q, head, e, rows, j0, std::min(all - j0, rows.chunk), loss, keep != nullptr, st));
-    CF_HIP(c, cfattn::launch_logp_finish(e.target, loss, 1.0, q.t, result, st), "distillation launch");
+        CF_TRY(distill_few_logits(c, q, hn, head, e, rows, j0, std::min(all - j0, rows.chunk), loss, keep != nullptr,
+                                  st));
+    CF_HIP(c, cfattn::launch_distill_finish(rows.scored.target, loss, q.t, result, st), "distillation launch");
     return CFATTN_OK;
 }
 
 int distill_backward_few(cfattn_ctx* c, const Distill& q, const float* hn, const float* head, const float* dloss,
                          float* dhn, float* dhead, bool acc, const void* keep, size_t keep_bytes, hipStream_t st) {
     const size_t padded = dhead ? few_padded(q.t) : q.t;
-    const int tag = distill_tag(q);
     Entries e{};
-    LogpRows rows{};
-    CF_TRY(logp_rows(c, padded, q.d, q.vocab, rows, keep != nullptr));
-    if (keep) {
-        CF_TRY(check_keep(c, keep, keep_bytes, few_keep_bytes(q.t, q.vocab)));
-        rows.count = static_cast<int*>(const_cast<void*>(keep));
-        rows.idx = rows.count + 4;
-        rows.logits = reinterpret_cast<float*>(static_cast<char*>(const_cast<void*>(keep)) + few_index_bytes(q.t));
-    } else {
-        CF_TRY(distill_entries(c, q, nullptr, e, st));
-        CF_HIP(c, cfattn::launch_logp_select(e.target, q.t, q.vocab, rows.idx, rows.count, tag, nullptr, nullptr,
-                                             nullptr, st),
-               "distillation launch");
-        CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, nullptr, rows.idx, rows.count, tag, rows.hn, padded, q.d, st),
-               "distillation launch");
-    }
+    FewRows rows{};
+    CF_TRY(distill_few_rows(c, q, padded, keep, keep_bytes, false, e, rows, st));
     float *scaled = nullptr, *parts = nullptr;  // rows of hn times dloss, sums of dhn
     if (dhead) {
         CF_TRY(take(c, cfattn_ctx::OPS_ROWS_BACK, padded * q.d * sizeof(float), scaled));
-        CF_HIP(c, cfattn::launch_logp_gather(hn, q.mul, dloss, rows.idx, rows.count, tag, scaled, padded, q.d, st),
+        CF_HIP(c, cfattn::launch_distill_scaled(hn, q.mul, dloss, rows.scored, padded, q.d, scaled, st),
                "distillation launch");
     }
     if (dhn) {
@@ -891,7 +896,7 @@ int distill_backward_few(cfattn_ctx* c, const Distill& q, const float* hn, const
     }
     for (size_t j0 = 0; j0 < padded; j0 += rows.chunk) {
         const size_t nr = std::min(padded - j0, rows.chunk);
-        if (!keep) CF_TRY(distill_few_logits(c, q, head, e, rows, j0, nr, nullptr, true, st));
+        if (!keep) CF_TRY(distill_few_logits(c, q, hn, head, e, rows, j0, nr, nullptr, true, st));
         if (dhead)
             CF_TRY(gemm(c, CFOPS_TN, rows.logits, scaled + j0 * q.d, dhead, q.vocab, nr, q.d, acc || j0, st));
         if (!dhn || j0 >= q.t) continue;
@@ -901,8 +906,7 @@ int distill_backward_few(cfattn_ctx* c, const Distill& q, const float* hn, const
                    "distillation launch");
         else
             CF_TRY(gemm(c, CFOPS_NN, rows.logits, head, parts, n, q.vocab, q.d, false, st));
-        CF_HIP(c, cfattn::launch_distill_rows_sum(parts, j0, n, q.t, q.d, q.vocab, q.mul, dloss, rows.idx, rows.count,
-                                                  tag, dhn, st),
+        CF_HIP(c, cfattn::launch_distill_rows_sum(parts, j0, n, q.d, q.vocab, q.mul, dloss, rows.scored, dhn, st),
                "distillation launch");
     }
     return CFATTN_OK;
@@ -1094,7 +1098,7 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* c, const float* hn, const float*
     CF_HIP(c, cfattn::launch_logp_select(targets, t, vocab, rows.idx, rows.count, 0, nullptr, nullptr, nullptr,
                                               st),
            "log-probability launch");
-    CF_HIP(c, cfattn::launch_logp_gather(hn, 1.0f, nullptr, rows.idx, rows.count, 0, rows.hn, padded, d, st),
+    CF_HIP(c, cfattn::launch_logp_gather(hn, rows.idx, rows.count, rows.hn, padded, d, st),
            "log-probability launch");
     for (size_t j0 = 0; j0 < padded; j0 += rows.chunk) {
         const size_t nr = std::min(padded - j0, rows.chunk);

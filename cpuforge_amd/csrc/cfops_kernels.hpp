@@ -233,8 +233,8 @@ hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st);
 //   finish:    the mean of sign logp, summed in f64 in a fixed order.
 hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, int tag,
                               float* logp, float* lse, void* misc, hipStream_t st);
-hipError_t launch_logp_gather(const float* hn, float mul, const float* by, const int* idx, const int* count, int tag,
-                              float* out, size_t rows, size_t d, hipStream_t st);
+hipError_t launch_logp_gather(const float* hn, const int* idx, const int* count, float* out, size_t rows, size_t d,
+                              hipStream_t st);
 hipError_t launch_logp_scatter(const float* in, const int* idx, const int* count, float* dhn, size_t rows, size_t d,
                                hipStream_t st);
 hipError_t launch_logp_grad_rows(float* logits, const int64_t* targets, const int* idx, const int* count,
@@ -320,7 +320,7 @@ hipError_t launch_head_zero_rows(const HeadPlan& p, const HeadBuffers& b, size_t
 // Distillation from a teacher's top logits (distill.hip).  entries: the rows' entries by
 // rising token, what the teacher's distribution is, and a `target` by which launch_logp_select
 // takes rows (kept, of which the head's products kept statistics and exponentials) or puts
-// them aside; logits: the scored rows [j0, j0 + nrows), whose logits are in memory.
+// them aside (negative: not scored); logits: few rows [j0, j0 + nrows), whose products are in memory.
 constexpr size_t kDistillMost = 1024;  // entries of a row
 struct TeacherRow {
     double l, p_rest, scale;  // the log-sum-exp that it takes, p_rest (negative: no rest), p / e
@@ -335,6 +335,8 @@ struct DistillEntries {
     float *z, *e;      // [t][k]: logits, exp((z - the row's largest) inv_t)
     TeacherRow* row;   // [t]
     int64_t* target;   // [t]
+    int* tag_at;       // takes the tag (null: none)
+    int tag;
 };
 hipError_t launch_distill_entries(const DistillEntries& g, hipStream_t st);
 struct DistillKept {
@@ -360,9 +362,10 @@ struct DistillRows {
     const TeacherRow* row;
     int k;
     double inv_t;
-    const int *idx, *scored;
+    const int64_t* target;
+    long t, vocab;   // rows from t on: zeros
     int j0;
-    long vocab;
+    float mul;       // of the products
     float* loss;     // may be null
     float2* slices;  // scratch: [rows][distill_slices(vocab)], and
     float* xs;       // [rows][k]
@@ -371,14 +374,21 @@ size_t distill_slices(size_t vocab);
 hipError_t launch_distill_logits(float* logits, size_t nrows, bool grad, const DistillRows& g, hipStream_t st);
 // grads [n][vocab] . head into `part` of distill_dhn_floats(n, d, vocab) floats, in parts for up to
 // kDistillRowsHead rows, else (by launch_gemm_f32) whole: us of either, with the sum, 24 and 40 rows of
-// 49152 x 576 41 and 57, 62 and 56, of 49152 x 2048 112 and 134, 148 and 133.  sum: of t rows of dhn
-// those of scored rows [j0, j0 + n), and those that are not scored.
+// 49152 x 576 41 and 57, 62 and 56, of 49152 x 2048 112 and 134, 148 and 133.  sum: rows [j0, j0 + n) of
+// dhn.  scaled: `padded` rows of hn times mul and dloss.  finish: the result's counts and mean.
+struct DistillScored {
+    const int64_t* target;  // [t]
+    const int* tag_at;      // where the forward left its tag (null: the targets are this call's)
+    int tag, t;
+};
 constexpr size_t kDistillRowsHead = 32;
 size_t distill_dhn_floats(size_t n, size_t d, size_t vocab);
 hipError_t launch_distill_rows_head(const float* grads, size_t n, size_t d, size_t vocab, const float* head,
                                     float* part, hipStream_t st);
-hipError_t launch_distill_rows_sum(const float* part, size_t j0, size_t n, size_t t, size_t d, size_t vocab, float mul,
-                                   const float* dloss, const int* idx, const int* count, int tag, float* dhn,
-                                   hipStream_t st);
+hipError_t launch_distill_rows_sum(const float* part, size_t j0, size_t n, size_t d, size_t vocab, float mul,
+                                   const float* dloss, const DistillScored& g, float* dhn, hipStream_t st);
+hipError_t launch_distill_scaled(const float* hn, float mul, const float* dloss, const DistillScored& g, size_t padded,
+                                 size_t d, float* out, hipStream_t st);
+hipError_t launch_distill_finish(const int64_t* target, const float* loss, size_t t, void* misc, hipStream_t st);
 
 }  // namespace cfattn

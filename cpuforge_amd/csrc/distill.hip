@@ -109,6 +109,7 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const DistillEntri
     g.count[r] = any_bad ? 0 : n;
     g.row[r] = {whole, p_rest, exp(own - whole) / sum};
     g.target[r] = any_bad ? -1 : n == 0 ? kIgnoreIndex : least;
+    if (r == 0 && g.tag_at) *g.tag_at = g.tag;
 }
 
 // What the rest makes of a row's loss, given the logarithm of its probability.
@@ -391,11 +392,11 @@ __global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) 
     g.count[r] = stay;
 }
 
-// Rows of logits in memory, kSlice of them to a workgroup, in two launches: the largest and the sum
-// of exponentials of each slice's tokens that are no entries (so the rest is a sum of its own),
-// and the entries' logits; then the loss, where it is wanted, and with GRAD the logits become
-// their gradients (zeros from the last scored row on).  24 rows of 49152, 16 of them scored, with
-// their gradients 12.5 us (a row to a workgroup 27).
+// Rows of products hn . head in memory (x times mul), kSlice of them to a workgroup, in two
+// launches: the largest and the sum of exponentials of each slice's tokens that are no entries (so
+// the rest is a sum of its own), and the entries' logits; then the loss, where it is wanted, and
+// with GRAD the products become the logits' gradients (zeros in rows that are not scored and from t
+// on).  24 rows of 49152, 16 of them scored, with their gradients 12.5 us (a row to a workgroup 27).
 constexpr int kSlice = 4096, kSliceThreads = 512, kPer = kSlice / kSliceThreads;
 
 // Whether value i of a slice is an entry's, for the values of this thread.
@@ -414,8 +415,8 @@ __global__ __launch_bounds__(kSliceThreads) void distill_slices_kernel(const flo
     __shared__ unsigned bits[kSlice / 32];
     __shared__ float red[2][8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.y;
-    if (g.j0 + j >= *g.scored) return;
-    const long r = g.idx[g.j0 + j], v0 = (long)blockIdx.x * kSlice;
+    const long r = g.j0 + j, v0 = (long)blockIdx.x * kSlice;
+    if (r >= g.t || g.target[r] < 0) return;
     const int n = g.count[r];
     const int* ids = g.ids + r * g.k;
     const float* x = logits + j * g.vocab;
@@ -425,12 +426,12 @@ __global__ __launch_bounds__(kSliceThreads) void distill_slices_kernel(const flo
     for (int i = 0; i < kPer; i++) {
         const int at = threadIdx.x + i * kSliceThreads;
         const bool in = v0 + at < g.vocab && !(bits[at / 32] >> at % 32 & 1);
-        v[i] = in ? x[v0 + at] : -INFINITY;
+        v[i] = in ? g.mul * x[v0 + at] : -INFINITY;
         m = fmaxf(m, v[i]);
     }
     for (int k = threadIdx.x; k < n; k += kSliceThreads) {
         const long at = ids[k] - v0;
-        if (at >= 0 && at < kSlice) g.xs[(long)j * g.k + k] = x[ids[k]];
+        if (at >= 0 && at < kSlice) g.xs[(long)j * g.k + k] = g.mul * x[ids[k]];
     }
     m = max_wave(m);
     if (lane == 0) red[0][wave] = m;
@@ -458,12 +459,15 @@ __global__ __launch_bounds__(kSliceThreads) void distill_logits_kernel(float* __
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.y;
     const long v0 = (long)blockIdx.x * kSlice;
     float* x = logits + j * g.vocab;
-    if (g.j0 + j >= *g.scored) {
+    const long r = g.j0 + j;
+    const bool scored = r < g.t && g.target[r] >= 0;
+    if (!scored) {
+        if (g.loss && r < g.t && blockIdx.x == 0 && threadIdx.x == 0)
+            g.loss[r] = g.target[r] == kIgnoreIndex ? 0.0f : __builtin_nanf("");
         if (GRAD)
             for (long v = v0 + threadIdx.x; v < min(v0 + kSlice, g.vocab); v += kSliceThreads) x[v] = 0.0f;
         return;
     }
-    const long r = g.idx[g.j0 + j];
     const int n = g.count[r];
     const int* ids = g.ids + r * g.k;
     const float* xs = g.xs + (long)j * g.k;
@@ -505,7 +509,7 @@ __global__ __launch_bounds__(kSliceThreads) void distill_logits_kernel(float* __
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
         const long v = v0 + threadIdx.x + i * kSliceThreads;
-        if (v < g.vocab) x[v] = f * expf(x[v] - base);
+        if (v < g.vocab) x[v] = f * expf(g.mul * x[v] - base);
     }
     __syncthreads();
     for (int k = threadIdx.x; k < n; k += kSliceThreads) {
@@ -582,33 +586,56 @@ __global__ __launch_bounds__(256) void distill_rows_head_kernel(const float* __r
     }
 }
 
-// dhn of row r, of scored rows [j0, j0 + t), = mul dloss (the sum of its parts), 64 columns to a
-// workgroup, every fourth split to a wave; zeros of rows that are not scored, NaN where the gradients
-// are another forward's.
-__global__ __launch_bounds__(256) void distill_rows_sum_kernel(const float* __restrict__ part, int splits, int j0,
-                                                               int t, int d, float mul, const float* __restrict__ dloss,
-                                                               const int* __restrict__ idx,
-                                                               const int* __restrict__ count, int tag,
-                                                               float* __restrict__ dhn) {
-    __shared__ float red[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.y, c = blockIdx.x * 64 + lane;
-    const bool known = count[1] == tag;
-    const int n = known ? *count : 0;
-    int j = -1;  // (few rows: all at once)
-    for (int i0 = 0; i0 < n; i0 += 64) {
-        const unsigned long long at = __ballot(i0 + lane < n && idx[i0 + lane] == r);
-        if (at) j = i0 + __ffsll(at) - 1;
+// Few rows' mean and counts, by one wave.
+__global__ __launch_bounds__(64) void distill_finish_kernel(const int64_t* __restrict__ target,
+                                                            const float* __restrict__ loss, int t,
+                                                            CeMisc* __restrict__ m) {
+    double s = 0.0;
+    int n = 0, bad = INT_MAX;
+    for (int r = threadIdx.x; r < t; r += 64) {
+        if (target[r] == kIgnoreIndex) continue;
+        n++;
+        if (target[r] < 0) bad = min(bad, r);
+        s += (double)loss[r];
     }
-    if (j >= 0 && (j < j0 || j >= j0 + t)) return;
+    s = sum_wave(s);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o), bad = min(bad, __shfl_xor(bad, o));
+    if (threadIdx.x == 0) *m = {n, bad, n > 0 ? (float)(s / (double)n) : 0.0f};
+}
+
+// out[r] = mul dloss[r] hn[r] of scored rows, zeros of others and from t on; NaN where what was kept
+// is another forward's.
+__global__ __launch_bounds__(256) void distill_scaled_kernel(const float* __restrict__ hn, float mul,
+                                                             const float* __restrict__ dloss, const DistillScored g,
+                                                             float* __restrict__ out, long d) {
+    const int r = blockIdx.x;
+    const bool known = !g.tag_at || *g.tag_at == g.tag;
+    const bool scored = known && r < g.t && g.target[r] >= 0;
+    const float f = scored ? mul * dloss[r] : 0.0f, none = known ? 0.0f : __builtin_nanf("");
+    for (long i = threadIdx.x; i < d; i += 256) out[r * d + i] = scored ? f * hn[r * d + i] : none;
+}
+
+// dhn of rows r, [j0, j0 + n), = mul dloss (the sum of its parts), 64 columns to a workgroup, every
+// fourth split to a wave; zeros of rows that are not scored, NaN where what was kept is another
+// forward's.
+__global__ __launch_bounds__(256) void distill_rows_sum_kernel(const float* __restrict__ part, int splits, int j0,
+                                                               int n, int d, float mul, const float* __restrict__ dloss,
+                                                               const DistillScored g, float* __restrict__ dhn) {
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.y, r = j0 + j;
+    const int c = blockIdx.x * 64 + lane;
+    const bool known = !g.tag_at || *g.tag_at == g.tag;
+    const bool scored = known && g.target[r] >= 0;
     float s = 0.0f;
-    if (j >= 0 && c < d)
+    if (scored && c < d)
 #pragma unroll 8
-        for (int p = wave; p < splits; p += 4) s += part[((long)p * t + j - j0) * d + c];
+        for (int p = wave; p < splits; p += 4) s += part[((long)p * n + j) * d + c];
     red[wave][lane] = s;
     __syncthreads();
     if (wave || c >= d) return;
     const float all = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-    dhn[(long)r * d + c] = !known ? __builtin_nanf("") : j >= 0 ? mul * dloss[r] * all : 0.0f;
+    dhn[(long)r * d + c] = !known ? __builtin_nanf("") : scored ? mul * dloss[r] * all : 0.0f;
 }
 
 }  // namespace
@@ -653,12 +680,21 @@ hipError_t launch_distill_rows_head(const float* grads, size_t n, size_t d, size
                        (int)blocks, (int)splits, part);
     return hipGetLastError();
 }
-hipError_t launch_distill_rows_sum(const float* part, size_t j0, size_t n, size_t t, size_t d, size_t vocab, float mul,
-                                   const float* dloss, const int* idx, const int* count, int tag, float* dhn,
-                                   hipStream_t st) {
+hipError_t launch_distill_rows_sum(const float* part, size_t j0, size_t n, size_t d, size_t vocab, float mul,
+                                   const float* dloss, const DistillScored& g, float* dhn, hipStream_t st) {
     const size_t splits = distill_dhn_floats(n, d, vocab) / (n * d);
-    hipLaunchKernelGGL(distill_rows_sum_kernel, dim3((unsigned)((d + 63) / 64), (unsigned)t), dim3(256), 0, st, part,
-                       (int)splits, (int)j0, (int)n, (int)d, mul, dloss, idx, count, tag, dhn);
+    hipLaunchKernelGGL(distill_rows_sum_kernel, dim3((unsigned)((d + 63) / 64), (unsigned)n), dim3(256), 0, st, part,
+                       (int)splits, (int)j0, (int)n, (int)d, mul, dloss, g, dhn);
+    return hipGetLastError();
+}
+hipError_t launch_distill_scaled(const float* hn, float mul, const float* dloss, const DistillScored& g, size_t padded,
+                                 size_t d, float* out, hipStream_t st) {
+    hipLaunchKernelGGL(distill_scaled_kernel, dim3((unsigned)padded), dim3(256), 0, st, hn, mul, dloss, g, out, (long)d);
+    return hipGetLastError();
+}
+hipError_t launch_distill_finish(const int64_t* target, const float* loss, size_t t, void* misc, hipStream_t st) {
+    hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(64), 0, st, target, loss, (int)t,
+                       static_cast<CeMisc*>(misc));
     return hipGetLastError();
 }
 

@@ -76,17 +76,13 @@ __global__ __launch_bounds__(1024) void logp_select_kernel(const int64_t* __rest
     }
 }
 
-// out[j] = mul by[r] hn[r], r = idx[j], zeros from row n on (by null: 1).
-__global__ __launch_bounds__(256) void logp_gather_kernel(const float* __restrict__ hn, float mul,
-                                                          const float* __restrict__ by, const int* __restrict__ idx,
-                                                          const int* __restrict__ count, int tag,
-                                                          float* __restrict__ out, long d) {
+// out[j] = hn[idx[j]], zeros from row n on.
+__global__ __launch_bounds__(256) void logp_gather_kernel(const float* __restrict__ hn, const int* __restrict__ idx,
+                                                          const int* __restrict__ count, float* __restrict__ out,
+                                                          long d) {
     const long j = blockIdx.x;
-    const bool known = count[1] == tag;
-    const int r = known && j < *count ? idx[j] : -1;
-    const float* x = r >= 0 ? hn + (long)r * d : nullptr;
-    const float f = x && by ? mul * by[r] : mul, none = known ? 0.0f : __builtin_nanf("");
-    for (long i = threadIdx.x; i < d; i += 256) out[j * d + i] = x ? f * x[i] : none;
+    const float* x = j < *count ? hn + (long)idx[j] * d : nullptr;
+    for (long i = threadIdx.x; i < d; i += 256) out[j * d + i] = x ? x[i] : 0.0f;
 }
 
 // dhn[idx[j]] = in[j] for j < n, the other rows zeros.
@@ -300,10 +296,9 @@ hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab,
                        tag, logp, lse, static_cast<CeMisc*>(misc));
     return hipGetLastError();
 }
-hipError_t launch_logp_gather(const float* hn, float mul, const float* by, const int* idx, const int* count, int tag,
-                              float* out, size_t rows, size_t d, hipStream_t st) {
-    hipLaunchKernelGGL(logp_gather_kernel, dim3((unsigned)rows), dim3(256), 0, st, hn, mul, by, idx, count, tag, out,
-                       (long)d);
+hipError_t launch_logp_gather(const float* hn, const int* idx, const int* count, float* out, size_t rows, size_t d,
+                              hipStream_t st) {
+    hipLaunchKernelGGL(logp_gather_kernel, dim3((unsigned)rows), dim3(256), 0, st, hn, idx, count, out, (long)d);
     return hipGetLastError();
 }
 hipError_t launch_logp_scatter(const float* in, const int* idx, const int* count, float* dhn, size_t rows, size_t d,

@@ -252,8 +252,9 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* ctx, const float* hn, const floa
  * probability 1 - sum p; or, with teacher_lse NULL, L the entries' own and p_rest = 0.  (A
  * teacher_lse below the entries' own counts as that, and where every token is an
  * entry it is not read; q_rest is held down to e^-700.)  A row without entries is not
- * scored: loss 0, no gradient.  A bad row has a token outside [0, vocab) or twice, or a teacher's value that is NaN or +inf: its
- * loss is NaN, it has no gradient, and result->bad_row names the first one.
+ * scored: loss 0, no gradient.  A bad row has a token outside [0, vocab) or twice, or a
+ * teacher's value that is NaN or +inf: its loss is NaN, it has no gradient, and
+ * result->bad_row names the first one.
  * result->loss is the mean over the rows with entries.  k is 1 to 1024; d, vocab and t as
  * cfops_lm_head_logprobs's, as is keep, of cfops_lm_head_distill_keep_bytes (few rows:
  * 4 t vocab, the logits' gradients). */
