@@ -70,8 +70,9 @@ _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 def _on(t: torch.Tensor, name: str, ctx: Context, dtypes=(torch.float32,), numel: int | None = None) -> int:
     """The address of a contiguous tensor of one of `dtypes` on the context's
     device."""
-    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.get_device() == ctx.device \
-            and t.is_contiguous() and (numel is None or t.numel() == numel):
+    # (A host tensor's device is -1.)
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.get_device() == ctx.device and t.is_contiguous() \
+            and (numel is None or t.numel() == numel):
         return t.data_ptr()
     _check_on(t, name, ctx, dtypes)
     if not t.is_contiguous():
@@ -198,42 +199,47 @@ def rotary(xs, ys, cos, sin, positions=None, *, pos0: int = 0, interleaved: bool
     n = len(xs)
     if n != len(ys) or not 1 <= n <= _lib.ROTARY_MAX:
         raise ValueError(f"{n} xs and {len(ys)} ys: as many of either, and 1 to {_lib.ROTARY_MAX}")
-    dev, table = ctx.device, []
+    dev, table = ctx.device, b""
     x_type, y_type = getattr(xs[0], "dtype", None), getattr(ys[0], "dtype", None)
-    batch = seq = dim = -1
+    typed, batch = x_type in _CODES and y_type in _CODES, -1
     for x, y in zip(xs, ys):
-        if not (isinstance(x, torch.Tensor) and isinstance(y, torch.Tensor) and x.dtype is x_type and y.dtype is y_type
-                and x_type in _CODES and y_type in _CODES and x.get_device() == dev and y.get_device() == dev):
+        if not (typed and isinstance(x, torch.Tensor) and isinstance(y, torch.Tensor) and x.dtype is x_type
+                and y.dtype is y_type and x.get_device() == dev and y.get_device() == dev):
             _check_on(xs[0], "x", ctx, _CODES)
             _check_on(ys[0], "y", ctx, _CODES)
             _check_on(x, "x", ctx, (x_type,))
             _check_on(y, "y", ctx, (y_type,))
         shape = x.shape
-        if batch < 0 and len(shape) == 4:
-            batch, seq, _, dim = shape
-        if y.shape != shape or len(shape) != 4 or shape[0] != batch or shape[1] != seq or shape[3] != dim:
+        fits = y.shape == shape and len(shape) == 4
+        if fits:
+            b, l, heads, w = shape
+            if batch < 0:
+                batch, seq, dim = b, l, w
+            fits = b == batch and l == seq and w == dim
+        if not fits:
             raise _lib.ShapeError(_lib.ERR_SHAPE, f"x and y have shapes {tuple(shape)} and {tuple(y.shape)} beside "
                                                   f"{tuple(xs[0].shape)} ([B, S, H, D], the same but for H)")
         x0, x1, x2, x3 = x.stride()
         y0, y1, y2, y3 = y.stride()
-        if dim > 1 and (x3 != 1 or y3 != 1):
+        if (x3 != 1 or y3 != 1) and dim > 1:
             raise ValueError("the last stride of x and y must be 1")
-        if (y0 == 0 and batch > 1) or (y1 == 0 and seq > 1) or (y2 == 0 and shape[2] > 1):
+        if not (y0 and y1 and y2) and ((y0 == 0 and b > 1) or (y1 == 0 and l > 1) or (y2 == 0 and heads > 1)):
             raise ValueError("y must not be expanded")
-        table.append(_ROTARY_TENSOR.pack(x.data_ptr(), y.data_ptr(), shape[2], x0, x1, x2, y0, y1, y2))
+        table += _ROTARY_TENSOR(x.data_ptr(), y.data_ptr(), heads, x0, x1, x2, y0, y1, y2)
     pc, ps = _on(cos, "cos", ctx), _on(sin, "sin", ctx)
-    if cos.dim() != 2 or sin.shape != cos.shape:
+    held = cos.shape
+    if len(held) != 2 or sin.shape != held:
         raise _lib.ShapeError(_lib.ERR_SHAPE, f"cos and sin have shapes {tuple(cos.shape)} and {tuple(sin.shape)}, "
                                               "expected [max_pos, half]")
     at = None if positions is None else _on(positions, "positions", ctx, (torch.int64,), batch * seq)
     if pos0 < 0:
         raise ValueError("pos0 must not be negative")
-    max_pos, half = cos.shape
-    _call(ctx, "cfops_rotary", b"".join(table), n, _CODES[x_type], _CODES[y_type], batch, seq, dim, half, pc, ps,
+    max_pos, half = held
+    _call(ctx, "cfops_rotary", table, n, _CODES[x_type], _CODES[y_type], batch, seq, dim, half, pc, ps,
           max_pos, at, pos0, interleaved, inverse, _stream_of(ctx))
 
 
-_ROTARY_TENSOR = struct.Struct("@PPN6q")  # cfops_rotary_tensor
+_ROTARY_TENSOR = struct.Struct("@PPN6q").pack  # cfops_rotary_tensor
 
 
 # --------------------------------------------------------------- SwiGLU
