@@ -153,7 +153,8 @@ struct EntryLds {
     float2 stat;
 };
 constexpr int kStats = 16;  // of a lane in registers
-__global__ __launch_bounds__(512) void distill_kept_kernel(const DistillKept g) {
+// (Two workgroups to a CU: with 129 registers, which leave one, 57 us.)
+__global__ __launch_bounds__(512, 4) void distill_kept_kernel(const DistillKept g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int j = blockIdx.x * (blockDim.x >> 6) + wave;
