@@ -47,7 +47,7 @@ struct RotaryArgs {
     const float *cos, *sin;    // [max_pos][half]
     const int64_t* positions;  // of every token, or null: pos0 + its place in its sequence
     long max_pos, pos0;
-    unsigned tokens, seq, token0;  // token0 set by launch_rotary, as
+    unsigned tokens, seq, token0;  // a launch has tokens [token0, tokens); set by launch_rotary, as
     int turned;                    // pieces of a head that are turned
     int count, head_dim, half, interleaved, inverse;
 };

@@ -136,9 +136,11 @@ hipError_t go(RotaryArgs g, hipStream_t st) {
         parts += t.parts;
     }
     // (A launch has fewer than 2^32 threads.)
-    const unsigned most = (1u << 23) / parts;
-    for (g.token0 = 0; g.token0 < g.tokens; g.token0 += most) {
-        const unsigned n = std::min(g.tokens - g.token0, most);
+    const unsigned all = g.tokens, most = (1u << 23) / parts;
+    for (g.token0 = 0; g.token0 < all; g.token0 += most) {
+        const unsigned n = std::min(all - g.token0, most);
+        // (The last workgroup of a launch may have room for tokens of the next one, which turns them.)
+        g.tokens = g.token0 + n;
         unsigned blocks = 0;
         for (int i = 0; i < kRotaryTensors; i++) {
             g.t[i].block0 = blocks;
