@@ -41,7 +41,7 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 // A row's entries by rising token, a wave to a row: ids, z and e [t][k] (count of them), their
 // exponentials below the largest's; the row's L, p_rest (negative: no rest) and p / e; target is a
 // token of the row, kIgnoreIndex without entries, -1 where the row is bad: a token out of the
-// vocabulary or named twice, or a value of the teacher's that is not finite.  (An entry whose id
+// vocabulary or named twice, or a value of the teacher's that is NaN or +inf.  (An entry whose id
 // is kIgnoreIndex or whose logit is -inf is not there.)
 // Places are counts of smaller tokens: 4096 x 64 entries 10 us.
 __global__ __launch_bounds__(256) void distill_entries_kernel(const DistillEntries g) {
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const DistillEntri
     double whole = own, p_rest = -1.0;
     if (g.teacher_lse && n > 0 && n < g.vocab) {
         const float l = g.teacher_lse[r];
-        bad |= !finite(l);
+        bad |= !(l < INFINITY);  // (-inf is below the entries' own.)
         whole = fmax(own, (double)l);
         p_rest = -expm1(own - whole);
     }

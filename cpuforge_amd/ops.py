@@ -520,7 +520,7 @@ def distill_check(result: torch.Tensor) -> None:
     bad = int(result[1].item())
     if bad != _NO_BAD_ROW:
         raise _lib.CfattnError(_lib.ERR_ARG, f"row {bad} names a token out of range or twice, or a value of the "
-                                             "teacher's is not finite")
+                                             "teacher's is NaN or +inf")
 
 
 # ------------------------------------------- losses over packed sequences
