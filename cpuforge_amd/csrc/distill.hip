@@ -242,30 +242,31 @@ __global__ __launch_bounds__(512, 4) void distill_kept_kernel(const DistillKept 
         rest = sum_wave(rest);
         if (rest > 0.0) rest *= exp2((double)m_rest - top);
         // The 128s that have entries, by their first: what is left of their sums, then, where that
-        // is not exact enough, the sum of the others.
+        // is not exact enough beside what the rest is at least, the sum of the others.  (f32 sums of
+        // up to 128 and kept values are off by less than 2^-19 of the sum: so much may be left of
+        // entries alone, and counts for nothing in the least.)
         double left = 0.0;
-        auto left_of = [&](int k, double& size) {
+        auto left_of = [&](int k, double& size, bool least) {
             const int part = mine[k].v / 128;
             const float2 s = mine[k].stat;
             double x = (double)s.y;
             for (int i = k; i < n && mine[i].v / 128 == part; i++) x -= (double)mine[i].kept;
             const double scale = pow2((double)s.x - top);
             size = (double)s.y * scale;
-            return fmax(x, 0.0) * scale;
+            return fmax(least ? x - 0x1p-19 * (double)s.y : x, 0.0) * scale;
         };
         for (int k = lane; k < n; k += 64) {
             double size;
-            if (is_first(k)) left += left_of(k, size);
+            if (is_first(k)) left += left_of(k, size, true);
         }
-        const double about = rest + sum_wave(left);
+        const double least = rest + sum_wave(left);
         left = 0.0;
         for (int k0 = 0; k0 < n; k0 += 64) {
             const int k = k0 + lane;
             const bool first = is_first(k);
             double size = 0.0, x = 0.0;
-            if (first) x = left_of(k, size);
-            // (Kept values and their sum are off by some 2^-23 of it.)
-            const bool again = first && !(size * 0x1p-22 <= about * 0x1p-18);
+            if (first) x = left_of(k, size, false);
+            const bool again = first && !(size * 0x1p-22 <= least * 0x1p-18);
             if (!again) left += x;
             for (unsigned long long todo = __ballot(again); todo; todo &= todo - 1) {
                 const int at = k0 + __ffsll(todo) - 1, part = mine[at].v / 128;
@@ -274,7 +275,7 @@ __global__ __launch_bounds__(512, 4) void distill_kept_kernel(const DistillKept 
                 const double sum = sum_wave((double)x4[0] + (double)x4[1] + (double)x4[2] + (double)x4[3]);
                 const double scale = exp2((double)mine[at].stat.x - top);
                 double exact = sum * scale;
-                if (!(128.0 * kLost * scale <= about * 0x1p-18) && !(sum > 128.0 * kLost * 0x1p18)) {
+                if (!(128.0 * kLost * scale <= least * 0x1p-18) && !(sum > 128.0 * kLost * 0x1p18)) {
                     exact = 0.0;
                     const int end = min(part * 128 + 128, g.vocab);
                     for (int v = part * 128, i = at; v < end; v++) {

@@ -48,3 +48,74 @@ def test_a_teacher_sum_of_minus_infinity_counts_as_the_entries_own(t):
         out.append((loss, *backward(hn, head, ids, z, lse, dloss, keep), *backward(hn, head, ids, z, lse, dloss)))
     for a, b in zip(*out):
         assert bool(torch.isfinite(b).all()) and torch.equal(a, b)
+
+
+class Exact:
+    """The loss and the gradients of 1 as temperature, the rest's in logarithms: q_v p_rest /
+    q_rest is p_rest exp(log q_v - log q_rest), whatever q_rest is.  What they may be off: the
+    logits by the rounding of 22-bit operands and f32 sums (`off`); logarithms by 2^-24 of the
+    exponents that they join (the factor from logits to powers of two is an f32) and of some 40
+    values; the rest by 2^-18 for each entry beside which it is summed; a gradient by 2^-36 of
+    its part's and what sums over its terms round."""
+
+    def __init__(self, hn, head, ids, z, lse, dloss):
+        h, w, g = hn.double(), head.double(), dloss.double()[:, None]
+        x = h @ w.T
+        log_q = torch.log_softmax(x, 1)
+        named = torch.zeros_like(x, dtype=torch.bool).scatter_(1, ids, True)
+        p = torch.zeros_like(x).scatter_(1, ids, (z.double() - lse.double()[:, None]).exp())
+        p_rest = -torch.expm1(z.double().logsumexp(1) - lse.double())
+        log_rest = log_q.masked_fill(named, -math.inf).logsumexp(1)
+        self.loss = (torch.xlogy(p, p) - p * log_q).where(named, torch.zeros(())).sum(1) \
+            + p_rest * (p_rest.log() - log_rest)
+        part = torch.where(named, 0.0, p_rest[:, None] * (log_q - log_rest[:, None]).exp())
+        q = log_q.exp()
+        dx = torch.where(named, q - p, q - part) * g
+        self.dhn, self.dhead = dx @ w, dx.T @ h
+        n, vocab, t = ids.shape[1], head.shape[0], hn.shape[0]
+        off = (2.0 ** -22 + 2 * U) * (h.abs() @ w.abs().T).amax(1)
+        spread = x.amax(1) - x.amin(1)
+        tol = off + U * (vocab / 512 + 40 + spread)
+        rest = off + tol + n * 2.0 ** -18
+        self.tol_loss = off + tol + p_rest * rest + U * self.loss.abs()
+        rel = (off + tol + U * (spread + 8))[:, None]
+        e = q * rel + part * rest[:, None] + 2.0 ** -36
+        e = e * g.abs() + dx.abs() * (2.0 ** -21 + U * vocab ** 0.5 + U * n)
+        self.tol_dhn = e @ w.abs()
+        self.tol_dhead = e.T @ h.abs() + U * self.dhead.abs() + U * t ** 0.5 * (dx.abs().T @ h.abs())
+        # How much of dhn is the rest's: what a test of it has to tell from nothing.
+        self.of_rest = (part * g.abs()) @ w.abs()
+
+
+def check(hn, head, ids, z, lse, dloss):
+    w = Exact(hn, head, ids, z, lse, dloss)
+    keep = keep_of(hn, head, ids)
+    loss, res = forward(hn, head, ids, z, lse, keep)
+    P.distill_check(res)
+    assert math.isfinite(float(P.ce_result_loss(res)))
+    for k in (keep, None):
+        dhn, dhead = backward(hn, head, ids, z, lse, dloss, k)
+        for got, want, tol in ((loss, w.loss, w.tol_loss), (dhn, w.dhn, w.tol_dhn), (dhead, w.dhead, w.tol_dhead)):
+            off = (got.double() - want).abs()
+            assert bool((off <= tol).all()), (float((off - tol).max()), float(off.max()))
+    assert bool(((w.tol_dhn < 0.1 * w.of_rest).sum(1) > hn.shape[1] / 2).all())
+
+
+@pytest.mark.parametrize("gap", [45.0, 60.0, 100.0, 300.0])
+@pytest.mark.parametrize("t", [20, 150])
+def test_what_sums_of_entries_round_is_no_rest(t, gap):
+    """Several entries of a like size in one part of the vocabulary, others 16 below them in
+    another and 28 below in a third, and the rest `gap` below: what is left of an f32 sum
+    less its entries is their rounding, 2^-24 of the largest, and far above the rest.  Parts
+    of the rest alone, one of them far below another, and none."""
+    g = torch.Generator(device=DEV).manual_seed(t)
+    d, k = 64, 14
+    dloss = torch.randn(t, generator=g, device=DEV)
+    for vocab in (900, 380):
+        hn, head = torch.randn(t, d, generator=g, device=DEV), torch.randn(vocab, d, generator=g, device=DEV) * 0.05
+        ids = torch.tensor([3, 20, 50, 90, 101, 127, 130, 150, 199, 201, 240, 256, 300, 379], device=DEV)
+        z = torch.randn(t, k, generator=g, device=DEV)
+        lse = (z.double().logsumexp(1) - math.log1p(-0.2)).float()
+        hn[:, 0], head[:, 0], head[500:, 0] = 8.0, 0.0, -2.0
+        head[ids[:6], 0], head[ids[6:11], 0], head[ids[11:], 0] = gap / 8, (gap - 16) / 8, (gap - 28) / 8
+        check(hn, head, ids.expand(t, k).contiguous(), z, lse, dloss)
