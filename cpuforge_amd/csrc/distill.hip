@@ -238,6 +238,23 @@ __global__ __launch_bounds__(512, 4) void distill_kept_kernel(const DistillKept 
         return last;
     };
     auto is_first = [&](int k) { return k < n && (k == 0 || mine[k - 1].v / 128 != mine[k].v / 128); };
+    // The others of the 128 that entry `at` is the first of, as add(y, s): s 2^y of them; from what was
+    // kept, or, where too little of it was to be `enough`, each formed again.
+    auto add_others = [&](int at, bool enough, auto add) {
+        const int part = mine[at].v / 128;
+        float x4[4];
+        const int last = others(at, x4);
+        const double sum = sum_wave((double)x4[0] + (double)x4[1] + (double)x4[2] + (double)x4[3]);
+        if (enough || sum > 128.0 * kLost * 0x1p18) return add((double)mine[at].stat.x, sum);
+        const int end = min(part * 128 + 128, g.vocab);
+        for (int v = part * 128, i = at; v < end; v++) {
+            if (i < last && mine[i].v == v)
+                i++;
+            else
+                add(logit(v), 1.0);
+        }
+    };
+    double low = 0.0;  // log2 of the rest's sum in units of 2^top
     if (with_rest) {
         rest = sum_wave(rest);
         if (rest > 0.0) rest *= exp2((double)m_rest - top);
@@ -269,37 +286,48 @@ __global__ __launch_bounds__(512, 4) void distill_kept_kernel(const DistillKept 
             const bool again = first && !(size * 0x1p-22 <= least * 0x1p-18);
             if (!again) left += x;
             for (unsigned long long todo = __ballot(again); todo; todo &= todo - 1) {
-                const int at = k0 + __ffsll(todo) - 1, part = mine[at].v / 128;
-                float x4[4];
-                const int last = others(at, x4);
-                const double sum = sum_wave((double)x4[0] + (double)x4[1] + (double)x4[2] + (double)x4[3]);
-                const double scale = exp2((double)mine[at].stat.x - top);
-                double exact = sum * scale;
-                if (!(128.0 * kLost * scale <= least * 0x1p-18) && !(sum > 128.0 * kLost * 0x1p18)) {
-                    exact = 0.0;
-                    const int end = min(part * 128 + 128, g.vocab);
-                    for (int v = part * 128, i = at; v < end; v++) {
-                        if (i < last && mine[i].v == v)
-                            i++;
-                        else
-                            exact += exp2(logit(v) - top);
-                    }
-                }
+                const int at = k0 + __ffsll(todo) - 1;
+                double exact = 0.0;
+                add_others(at, 128.0 * kLost * exp2((double)mine[at].stat.x - top) <= least * 0x1p-18,
+                           [&](double y, double s) { exact += s * exp2(y - top); });
                 if (lane == 0) left += exact;
             }
         }
         rest += sum_wave(left);
+        low = log2(rest);
+        // Where f64 holds it no more, all of it again in units of its own largest.
+        if (rest < 0x1p-900) {
+            double unit = -INFINITY;
+            rest = 0.0;
+            auto add = [&](double y, double s) {
+                if (y > unit) rest *= exp2(unit - y), unit = y;
+                rest += s * exp2(y - unit);
+            };
+            if (m_rest > -INFINITY) {
+                double parts = 0.0;
+                for (int p = lane; p < g.parts; p += 64) {
+                    const float2 s = stat(p);
+                    if (!has_entry(p)) parts += (double)(s.y * __builtin_amdgcn_exp2f(s.x - m_rest));
+                }
+                add((double)m_rest, sum_wave(parts));
+            }
+            for (int k0 = 0; k0 < n; k0 += 64)
+                for (unsigned long long todo = __ballot(is_first(k0 + lane)); todo; todo &= todo - 1)
+                    add_others(k0 + __ffsll(todo) - 1, false, add);
+            low = unit - top + log2(rest);
+        }
     }
     const double log_total = log(total), unit = 1.0 / (double)kLog2e;
-    const Rest r_(row.p_rest, log(rest) - log_total);
+    const Rest r_(row.p_rest, low * M_LN2 - log_total);
     // Where the rest is so small that f32 holds neither a nor all of its exponentials, a is 2^-lift
     // of itself and every factor 2^lift (a part's largest is up to 2^10 above the rest, or its entries
     // stay in the list and its factor follows below).
-    const double lift = with_rest && rest > 0.0 && rest < 0x1p-60 * total ? floor(log2(total / rest)) : 0.0;
-    const float a = lift > 0.0 ? (float)(exp2(-lift) - exp(log(row.p_rest) - log(rest) + log_total - lift * M_LN2))
+    const double above = with_rest ? log2(total) - low : 0.0, lift = above > 60.0 ? floor(above) : 0.0;
+    const float a = lift > 0.0 ? (float)(exp2(-lift) - row.p_rest * exp2(above - lift))
                                : (float)(1.0 - fmin(r_.ratio, 1e30));
     auto lifted = [&](float x) { return (float)(exp2(fmin((double)x - top + lift, 120.0)) / total); };
-    if (g.dl && lift > 0.0) each([&](int p, const float2& s) { g.factor[(long)p * g.ld + j] = lifted(s.x); });
+    if (g.dl && lift > 0.0)
+        for (int p = lane; p < g.parts; p += 64) g.factor[(long)p * g.ld + j] = lifted(stat(p).x);
     double terms = 0.0;
     int stay = 0;
     for (int k0 = 0; k0 < n; k0 += 64) {
@@ -319,7 +347,7 @@ __global__ __launch_bounds__(512, 4) void distill_kept_kernel(const DistillKept 
         if (live)
             terms += entry_loss(row, g.z[r * g.k + k], g.e[r * g.k + k], g.inv_t, q, y * unit - log_total, dl);
         if (!g.dl) continue;
-        const bool far = with_rest && pow2(up) * 0x1p-10 > rest;
+        const bool far = with_rest && up - 10.0 > low;
         const float factor = !live ? 1.0f : lift > 0.0 ? lifted(en.stat.x) : g.factor[(long)(v / 128) * g.ld + j];
         const float in = live ? (float)dl / (a * factor) : 0.0f;
         // (Up to 2 the product's f16 pieces hold it.)
@@ -338,7 +366,7 @@ __global__ __launch_bounds__(512, 4) void distill_kept_kernel(const DistillKept 
     // that this shows in a q, the others of its 128 are scaled up.
     for (int k0 = 0; g.dl && with_rest && k0 < n; k0 += 64) {
         const int k = k0 + lane;
-        const bool far = is_first(k) && pow2((double)mine[k].stat.x - top) * 0x1p-10 > rest;
+        const bool far = is_first(k) && (double)mine[k].stat.x - top - 10.0 > low;
         for (unsigned long long todo = __ballot(far); todo; todo &= todo - 1) {
             const int at = k0 + __ffsll(todo) - 1, part = mine[at].v / 128;
             float x4[4];

@@ -251,8 +251,8 @@ int cfops_lm_head_logprobs_backward(cfattn_ctx* ctx, const float* hn, const floa
  * with L = teacher_lse[r], log sum_v exp(teacher_v / temperature) over its whole
  * vocabulary, and the tokens that are no entry (the rest) as one more class, of
  * probability 1 - sum p; or, with teacher_lse NULL, L the entries' own and p_rest = 0.  (A
- * teacher_lse below the entries' own counts as that, and where every token is an
- * entry it is not read; q_rest is held down to e^-700.)  A row without entries is not
+ * teacher_lse below the entries' own, -inf among them, counts as that, and where every
+ * token is an entry it is not read.)  A row without entries is not
  * scored: loss 0, no gradient.  A bad row has a token outside [0, vocab) or twice, or a
  * teacher's value that is NaN or +inf: its loss is NaN, it has no gradient, and
  * result->bad_row names the first one.

@@ -119,3 +119,24 @@ def test_what_sums_of_entries_round_is_no_rest(t, gap):
         hn[:, 0], head[:, 0], head[500:, 0] = 8.0, 0.0, -2.0
         head[ids[:6], 0], head[ids[6:11], 0], head[ids[11:], 0] = gap / 8, (gap - 16) / 8, (gap - 28) / 8
         check(hn, head, ids.expand(t, k).contiguous(), z, lse, dloss)
+
+
+@pytest.mark.parametrize("gap", [600.0, 690.0, 720.0, 1000.0, 4000.0])
+@pytest.mark.parametrize("t", [20, 150])
+def test_a_rest_that_64_bits_do_not_hold(t, gap):
+    """Every entry is `gap` above every other token, two of them in one part of the
+    vocabulary and one in another: the rest is e^-gap and less, and has its share of the loss
+    and all of its gradient, however many rows there are.  With two parts of the rest
+    alone, one of which is far below the other, and with entries in each part."""
+    g = torch.Generator(device=DEV).manual_seed(t)
+    dloss = torch.randn(t, generator=g, device=DEV)
+    for vocab, entries in ((700, [5, 9, 140]), (300, [5, 140, 141, 260, 299])):
+        d, k = 64, len(entries)
+        hn, head = torch.randn(t, d, generator=g, device=DEV), torch.randn(vocab, d, generator=g, device=DEV) * 0.05
+        ids = torch.tensor(entries, device=DEV).expand(t, k).contiguous()
+        z = torch.randn(t, k, generator=g, device=DEV)
+        lse = (z.double().logsumexp(1) - math.log1p(-0.2)).float()
+        hn[:, 0], head[:, 0] = gap / 4, 0.0
+        head[400:, 0] = -0.25
+        head[entries, 0] = 4.0
+        check(hn, head, ids, z, lse, dloss)
