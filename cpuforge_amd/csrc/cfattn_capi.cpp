@@ -699,7 +699,8 @@ int cfattn_rope_table_scaled(size_t head_dim, size_t max_pos, double theta, cons
     if (head_dim % 2 != 0) return CFATTN_ERR_SHAPE;
     if ((!cos_out || !sin_out) && max_pos * head_dim > 0) return CFATTN_ERR_ARG;
     if (!sc || sc->kind < CFATTN_ROPE_LINEAR || sc->kind > CFATTN_ROPE_YARN || !(sc->factor > 0.0) ||
-        !(sc->attention_factor >= 0.0) || !(theta > 0.0))
+        !(sc->attention_factor >= 0.0) || !(theta > 0.0) || !std::isfinite(sc->factor) ||
+        !std::isfinite(sc->attention_factor) || !std::isfinite(theta))
         return CFATTN_ERR_ARG;
     const size_t half = head_dim / 2;
     const double dim = (double)head_dim;
@@ -707,10 +708,13 @@ int cfattn_rope_table_scaled(size_t head_dim, size_t max_pos, double theta, cons
     if (sc->kind == CFATTN_ROPE_NTK) {
         // (One pair has the frequency 1 whatever theta is.)
         if (head_dim > 2) theta *= std::pow(sc->factor, dim / (dim - 2.0));
+        if (!(theta > 0.0) || !std::isfinite(theta)) return CFATTN_ERR_ARG;
     } else if (sc->kind == CFATTN_ROPE_YARN) {
         if (!(sc->original_max_position > 0.0) || !(sc->beta_fast >= sc->beta_slow) || !(sc->beta_slow > 0.0) ||
-            !(theta > 1.0))
+            !(theta > 1.0) || !std::isfinite(sc->original_max_position) || !std::isfinite(sc->beta_fast))
             return CFATTN_ERR_ARG;
+        // (Its own size is of longer contexts: below 1 it falls, and is negative in the end.)
+        if (sc->factor < 1.0 && sc->attention_factor == 0.0) return CFATTN_ERR_ARG;
         // The pair, as a real number, that turns so many times in the trained positions.
         auto pair = [&](double turns) {
             return dim * std::log(sc->original_max_position / (turns * 2.0 * 3.14159265358979323846)) /

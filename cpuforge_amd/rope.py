@@ -58,7 +58,8 @@ class YarnScaling:
     """Pairs that turn at most beta_slow times in original_max_position positions
     turn `factor` times slower, those that turn beta_fast times or more as before,
     a line over the pairs in between; cos and sin are multiplied by
-    attention_factor (None: 0.1 ln(factor) + 1), which the scores have squared."""
+    attention_factor (None: 0.1 ln(factor) + 1, of a factor of 1 or more), which the
+    scores have squared."""
     factor: float
     original_max_position: float
     beta_fast: float = 32.0

@@ -207,7 +207,9 @@ int cfattn_rope_table(size_t head_dim, size_t max_pos, double theta, const cfatt
  *   NTK     theta * factor^(head_dim / (head_dim - 2)) in theta's place
  *   YARN    of d pairs, those that turn at most beta_slow times in
  *           original_max_position positions get inv_freq / factor, those that turn
- *           beta_fast times or more keep theirs, a line over the pairs in between */
+ *           beta_fast times or more keep theirs, a line over the pairs in between; a
+ *           factor below 1 needs an attention_factor
+ * Values that are not finite are refused. */
 enum { CFATTN_ROPE_LINEAR = 1, CFATTN_ROPE_NTK = 2, CFATTN_ROPE_YARN = 3 };
 typedef struct cfattn_rope_scaling {
     int kind;
