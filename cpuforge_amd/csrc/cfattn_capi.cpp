@@ -704,7 +704,7 @@ int cfattn_rope_table_scaled(size_t head_dim, size_t max_pos, double theta, cons
         return CFATTN_ERR_ARG;
     const size_t half = head_dim / 2;
     const double dim = (double)head_dim;
-    double first = 0.0, last = 0.0, size = 1.0;
+    double fastest = 0.0, first = 0.0, last = 0.0, size = 1.0;
     if (sc->kind == CFATTN_ROPE_NTK) {
         // (One pair has the frequency 1 whatever theta is.)
         if (head_dim > 2) theta *= std::pow(sc->factor, dim / (dim - 2.0));
@@ -720,7 +720,8 @@ int cfattn_rope_table_scaled(size_t head_dim, size_t max_pos, double theta, cons
             return dim * std::log(sc->original_max_position / (turns * 2.0 * 3.14159265358979323846)) /
                    (2.0 * std::log(theta));
         };
-        first = std::max(std::floor(pair(sc->beta_fast)), 0.0);
+        fastest = pair(sc->beta_fast);
+        first = std::max(std::floor(fastest), 0.0);
         last = std::min(std::ceil(pair(sc->beta_slow)), dim - 1.0);
         size = 0.1 * std::log(sc->factor) + 1.0;
     }
@@ -729,8 +730,9 @@ int cfattn_rope_table_scaled(size_t head_dim, size_t max_pos, double theta, cons
         double inv_freq = std::pow(theta, -(2.0 * (double)i) / dim);
         if (sc->kind == CFATTN_ROPE_LINEAR) inv_freq /= sc->factor;
         if (sc->kind == CFATTN_ROPE_YARN) {
-            const double slow =
-                std::min(std::max(((double)i - first) / (last > first ? last - first : 1e-3), 0.0), 1.0);
+            // (No pairs in between: those behind the fast ones, all where even the first is slow.)
+            const double slow = last > first ? std::min(std::max(((double)i - first) / (last - first), 0.0), 1.0)
+                                             : (double)i > fastest;
             inv_freq = inv_freq / sc->factor * slow + inv_freq * (1.0 - slow);
         }
         for (size_t pos = 0; pos < max_pos; pos++) {

@@ -36,3 +36,17 @@ def test_a_base_that_is_not_finite_is_refused():
     for theta in (INF, float("nan"), 0.0):
         with pytest.raises(CfattnError):
             RopeCache(64, 10, theta, LinearScaling(2.0))
+
+
+@pytest.mark.parametrize("trained", [1.0, 4.0, 6.0, 2 * math.pi])
+@pytest.mark.parametrize("dim", [2, 10, 64])
+def test_every_pair_of_a_short_context_is_slow(dim, trained):
+    """The first pair turns once in 2 pi positions: in fewer no pair turns more than
+    beta_slow = 1 times, and all are `factor` times slower."""
+    got = RopeCache(dim, 50, 1e4, YarnScaling(4.0, trained, attention_factor=1.0))
+    assert np.array_equal(tables(got), tables(RopeCache(dim, 50, 1e4, LinearScaling(4.0))))
+
+
+def test_every_pair_of_a_long_context_is_fast():
+    got = RopeCache(64, 50, 1e4, YarnScaling(4.0, 1e9, attention_factor=1.0))
+    assert np.array_equal(tables(got), tables(RopeCache(64, 50, 1e4)))
