@@ -363,7 +363,7 @@ __global__ __launch_bounds__(512, 4) void distill_kept_kernel(const DistillKept 
     }
     terms = sum_wave(terms);
     // The gradient's product takes a kept value to 2^-36: where an entry lies so far above the rest
-    // that this shows in a q, the others of its 128 are scaled up.
+    // that this shows in a q, the others of its 128 are scaled up, to at most 1.
     for (int k0 = 0; g.dl && with_rest && k0 < n; k0 += 64) {
         const int k = k0 + lane;
         const bool far = is_first(k) && (double)mine[k].stat.x - top - 10.0 > low;
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(512, 4) void distill_kept_kernel(const DistillKept 
 #pragma unroll
                 for (int o = 32; o >= 1; o >>= 1) y_most = fmax(y_most, __shfl_xor(y_most, o));
                 if (!(y_most > -INFINITY)) continue;
-                y_most = floor(y_most);
+                y_most = floor(y_most) + 1.0;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     if (lane < 32 && part * 128 + v4 + i < g.vocab)
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(512, 4) void distill_kept_kernel(const DistillKept 
                 if (lane == 0) g.factor[(long)part * g.ld + j] = (float)(exp2(y_most + lift) / total);
                 continue;
             }
-            const int up = min(max(127 - (int)(__builtin_bit_cast(uint32_t, most) >> 23), 0), 126);
+            const int up = min(max(126 - (int)(__builtin_bit_cast(uint32_t, most) >> 23), 0), 126);
             if (!(most > 0.0f) || up == 0) continue;
             const float times = __builtin_bit_cast(float, (uint32_t)(127 + up) << 23);
 #pragma unroll

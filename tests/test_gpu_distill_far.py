@@ -140,3 +140,25 @@ def test_a_rest_that_64_bits_do_not_hold(t, gap):
         head[400:, 0] = -0.25
         head[entries, 0] = 4.0
         check(hn, head, ids, z, lse, dloss)
+
+
+@pytest.mark.parametrize("below", [30.0, 59.0, 70.0, 90.0, 200.0])
+def test_values_just_below_a_power_of_two(below):
+    """A part of the vocabulary whose entry is 2^`below` above its largest other token, which is
+    scaled up for the gradient's product, to all but 2^-13 of a power of two; it stands among
+    rows of the head that are 8 times as large as those before them, which the product takes
+    with a scale of their own: the scaled value has to be within what f16 holds."""
+    t, d, vocab = 150, 32, 300
+    g = torch.Generator(device=DEV).manual_seed(7)
+    hn, head = torch.zeros(t, d, device=DEV), torch.rand(vocab, d, generator=g, device=DEV) * 2 - 1
+    head[:, 31] = 1.0  # (the power of two of each 32 rows)
+    head[32:64] *= 8.0
+    hn[:, 0], hn[:, 1] = 256.0, torch.arange(t, device=DEV) % 4  # (rows are alike but for a little)
+    unit = math.log(2.0) / 256
+    head[:, 0], head[:, 1] = -(below + 5) * unit, 0.0
+    head[40, 0], head[40, 1] = -(below + 0.00017) * unit, 0.00002 * 256 * unit
+    head[3, 0] = 0.0
+    ids = torch.full((t, 1), 3, device=DEV)
+    z = torch.zeros(t, 1, device=DEV)
+    lse = torch.full((t,), -math.log1p(-0.2), device=DEV)
+    check(hn, head, ids, z, lse, torch.randn(t, generator=g, device=DEV))
