@@ -227,8 +227,7 @@ hipError_t launch_policy(PolicyArgs a, void* scratch, hipStream_t st);
 //   select:    idx and, from idx + rows on, their targets; count[0], tag in count[1]; the
 //              result block (CeMisc; or null), and logp
 //              and lse (or null) of the rows that are not scored;
-//   gather:    the scored rows of hn side by side, times mul and the row's `by` (or null), NaN
-//              where the tag is another;   scatter: back, other rows 0;
+//   gather:    the scored rows of hn side by side;   scatter: back, other rows 0;
 //   grad_rows: the logits become their gradients;
 //   finish:    the mean of sign logp, summed in f64 in a fixed order.
 hipError_t launch_logp_select(const int64_t* targets, size_t rows, size_t vocab, int* idx, int* count, int tag,
@@ -294,10 +293,11 @@ struct HeadBuffers {
     void* stats;
     float mul = 1.0f;                    // of hn
 };
-// In a target's place up to k entries of each row (distill.hip), whose kept exponentials are zeros:
-// dlogits are dloss (a q_v + dl of the entry that v is); dhn is times mul.
+// In a target's place what distill_kept leaves of a row: dlogits are dloss (a f e_v + dl of the listed
+// entry that v is), f the factor of v's part and e_v its kept value, which is an exponential, or of
+// an entry that is not listed its gradient over a f, of a listed one 0; dhn is times mul.
 struct HeadEntries {
-    const int *ids, *count;  // [t][k], and how many
+    const int *ids, *count;  // [t][k], and how many are listed
     const float *dl, *a;     // [t][k], [t]
     int k;
 };
@@ -340,7 +340,7 @@ struct DistillEntries {
 };
 hipError_t launch_distill_entries(const DistillEntries& g, hipStream_t st);
 struct DistillKept {
-    int *ids, *count;  // with dl and a, left as those of HeadEntries
+    int *ids, *count;  // all entries of a row; with dl and a, left as those of HeadEntries
     const float *z, *e;
     const TeacherRow* row;
     int k;

@@ -156,7 +156,8 @@ def rmsnorm_backward(dy, x, w, rstd, dx, dw, rows, dim, ctx: Context | None = No
 def layernorm_forward(x, w, b, y, mean, rstd, rows, dim, eps, ctx: Context | None = None):
     """y = (x - mean) rstd w + b per row of `dim` (b None: no bias), mean and
     rstd = 1 / sqrt(var + eps): overwrites y [rows, dim], mean and rstd [rows].
-    x and y are float32 or bfloat16, the others float32."""
+    x and y are float32 or bfloat16, the others float32.  What is
+    written shares memory with no other tensor."""
     ctx = ctx or default_context()
     n = rows * dim
     _call(ctx, "cfops_layernorm_forward", _code(x), _on(x, "x", ctx, _CODES, n), _on(w, "w", ctx, numel=dim),
@@ -167,7 +168,7 @@ def layernorm_forward(x, w, b, y, mean, rstd, rows, dim, eps, ctx: Context | Non
 
 def layernorm_backward(dy, x, w, mean, rstd, dx, dw, db, rows, dim, ctx: Context | None = None, acc: bool = True):
     """Accumulates into dx (of x's type, as dy), dw and db (None: frozen), or
-    overwrites them with acc=False."""
+    overwrites them with acc=False.  They share memory with no other tensor."""
     ctx = ctx or default_context()
     n = rows * dim
     _call(ctx, "cfops_layernorm_backward", _code(x), _on(dy, "dy", ctx, (x.dtype,), n), _on(x, "x", ctx, _CODES, n),

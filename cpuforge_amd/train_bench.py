@@ -123,7 +123,8 @@ class SmolLM:
     RMSNorm), rotary=dict(dim=.., interleaved=..) (the first `dim` values of
     each head turn, all by default, in halves or as pairs side by side: ops.rotary
     before the attention instead of the fused prologue, at positions of the
-    caller's), rope_scaling (a scaling of RopeCache)."""
+    caller's; the attention is over the whole row all the same), rope_scaling (a
+    scaling of RopeCache)."""
 
     def __init__(self, layers: int = 30, seq: int = 512, rank: int = 16, dtype=torch.float32, device="cuda",
                  seed: int = 1, attn_dtype=None, backend: str = "cfops", config: dict | None = None,
@@ -212,7 +213,9 @@ class SmolLM:
 
     def hidden(self, tokens, positions=None):
         """The final norm's output [B, S, d].  positions [B, S] (int64; with
-        config rotary): the tokens' own, where several documents share a row."""
+        config rotary): those that q and k turn by.  They do not limit the attention,
+        which is causal over the row: of documents that share a row, a later one
+        attends to those before it."""
         return self._hidden_cfops(tokens, positions) if self.backend == "cfops" else \
             self._hidden_torch(tokens, positions)
 
@@ -239,8 +242,9 @@ class SmolLM:
 
     def distill(self, tokens, ids, teacher, teacher_lse=None, temperature=1.0, positions=None):
         """The rows' losses [B, S] against a teacher's top logits (A.lm_head_distill;
-        ids and teacher [B, S, k], teacher_lse [B, S] or None; cfops backend, no host
-        wait: check_targets() reports entries that it does not take)."""
+        ids and teacher [B, S, k], teacher_lse [B, S] or None; positions as hidden's;
+        cfops backend, no host wait: check_targets() reports entries that it does not
+        take)."""
         if self.backend != "cfops":
             raise ValueError("distillation needs the cfops backend")
         loss, res = A.lm_head_distill(self.hidden(tokens, positions), self.embed, ids, teacher, teacher_lse,

@@ -68,8 +68,8 @@ int cfops_rmsnorm_grad(cfattn_ctx* ctx, const float* dy, const float* x, const f
  * dim + eps), y = (x - mean) rstd w + b (b NULL: no bias).  x and y [rows, dim] are
  * of `dtype` (CFATTN_F32 or CFATTN_BF16); w, b [dim], mean and rstd [rows] are f32;
  * y, mean and rstd are overwritten.  Sums and statistics are f32; y is rounded
- * once.  What is not finite in a row stays with that row.  (No buffer of either call
- * shares memory with another.) */
+ * once.  What is not finite in a row stays with that row.  (A buffer that either call
+ * writes shares memory with no other.) */
 int cfops_layernorm_forward(cfattn_ctx* ctx, int dtype, const void* x, const float* w, const float* b, void* y,
                             float* mean, float* rstd, size_t rows, size_t dim, float eps, void* stream);
 /* From dy: dx (of `dtype`, as dy and x) and, where non-null, dw = sum dy (x - mean)
