@@ -899,9 +899,9 @@ __global__ __launch_bounds__(256) void head_col_top_kernel(const DlogitsArgs g) 
         const int j = t0 + l32;
         if (j >= n) continue;
         const long r = g.idx[g.j0 + j];
-        float row = fabsf(g.dlogp[r] * row_top(g.scale[g.j0 + j]));
-        if constexpr (ENTRIES) row *= fabsf(g.en.a[r]);
-        const float f = g.factor[blockIdx.x * g.ld + j];
+        const float row = fabsf(g.dlogp[r] * row_top(g.scale[g.j0 + j]));
+        // (Multiplied in the order of the dlogits: what underflows there has to here.)
+        const float f = g.factor[blockIdx.x * g.ld + j] * (ENTRIES ? fabsf(g.en.a[r]) : 1.0f);
 #pragma unroll
         for (int q = 0; q < 2; q++) {
             const f32x4* y = reinterpret_cast<const f32x4*>(

@@ -162,3 +162,20 @@ def test_values_just_below_a_power_of_two(below):
     z = torch.zeros(t, 1, device=DEV)
     lse = torch.full((t,), -math.log1p(-0.2), device=DEV)
     check(hn, head, ids, z, lse, torch.randn(t, generator=g, device=DEV))
+
+
+@pytest.mark.parametrize("low", [-104.5, -106.0, -108.0])
+def test_tokens_whose_probabilities_f32_does_not_hold(low):
+    """Tokens of 2^-151 of the largest and less in a part whose largest is 2^-144, beside a rest
+    of 2^-58 whose gradient is 2^55 times as steep: probability times factor is in f32 what
+    the probability alone is not, and the head's gradient takes its scale from the product."""
+    t, d, vocab = 150, 64, 384
+    g = torch.Generator(device=DEV).manual_seed(3)
+    hn, head = torch.randn(t, d, generator=g, device=DEV), torch.randn(vocab, d, generator=g, device=DEV) * 0.01
+    hn[:, 0], head[:, 0] = 8.0, low / 8
+    head[:256, 0], head[256, 0] = -45.0 / 8, -100.0 / 8
+    head[[3, 20], 0] = 0.0
+    ids = torch.tensor([3, 20], device=DEV).expand(t, 2).contiguous()
+    z = torch.randn(t, 2, generator=g, device=DEV)
+    lse = (z.double().logsumexp(1) - math.log1p(-0.2)).float()
+    check(hn, head, ids, z, lse, torch.randn(t, generator=g, device=DEV))
