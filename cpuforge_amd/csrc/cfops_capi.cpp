@@ -352,6 +352,10 @@ int cfops_rotary(cfattn_ctx* c, const cfops_rotary_tensor* tensors, size_t n, in
         if (batch && seq && (!t.x || !t.y)) return fail(c, CFATTN_ERR_ARG, "null buffer");
         if (t.x == t.y && batch && seq && (x_dtype != y_dtype || !same))
             return fail(c, CFATTN_ERR_ARG, "in place needs one type and one set of strides");
+        // (A launch turns all tensors at once.)
+        for (int o = 0; batch && seq && o + 1 < g.count; o++)
+            if (g.t[o].y == t.y || g.t[o].x == t.y || g.t[o].y == t.x)
+                return fail(c, CFATTN_ERR_ARG, "tensor %zu and one before it share an output", i);
         r.copy = t.x != t.y && 2 * half < head_dim;
     }
     if (batch == 0 || seq == 0 || g.count == 0) return CFATTN_OK;

@@ -186,8 +186,8 @@ def _code(t) -> int:
 def rotary(xs, ys, cos, sin, positions=None, *, pos0: int = 0, interleaved: bool = False, inverse: bool = False,
            ctx: Context | None = None):
     """Turns tensors xs of heads [B, S, H, D] (one, or up to 4 of the same B, S and
-    D, as q and k) into ys (the same shapes; a y may be its x, else they share no
-    memory): pair i of a head's first 2 * cos.shape[1] values by cos[p, i] and
+    D, as q and k) into ys (the same shapes; a y may be its x, else it shares no
+    memory with any tensor): pair i of a head's first 2 * cos.shape[1] values by cos[p, i] and
     sin[p, i] of the token's position p, (a, b) -> (a c - b s, b c + a s) (inverse:
     s negated, the gradient's way); the values behind them are copied.  The pairs
     are (i, i + half), as in the fused prologue, or (2 i, 2 i + 1) with

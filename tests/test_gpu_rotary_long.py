@@ -1,8 +1,10 @@
-"""GPU test of ops.rotary over more tokens than one launch takes."""
+"""GPU tests of ops.rotary over more tokens than one launch takes, and of tensors that a
+launch cannot take together."""
 import pytest
 import torch
 
 from cpuforge_amd import ops as P
+from cpuforge_amd._lib import CfattnError
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -24,3 +26,16 @@ def test_each_token_is_turned_once(heads):
         assert torch.equal(y, w)
         wrong = torch.nonzero((x != w).flatten(2).any(-1))
         assert not len(wrong), wrong[:8].tolist()
+
+
+def test_tensors_that_share_an_output_are_refused():
+    """One launch turns all tensors: a y that is another's, or another's x, would have either."""
+    cos, sin = torch.zeros(5, 4, device=DEV), torch.ones(5, 4, device=DEV)
+    a, b, c, d = (torch.randn(1, 5, 2, 8, device=DEV) for _ in range(4))
+    was = [t.clone() for t in (a, b, c, d)]
+    for xs, ys in (((a, b), (c, c)), ((a, b), (b, c)), ((a, b), (c, a)), ((a, a), (a, a)), ((a, b, c), (d, b, d))):
+        with pytest.raises(CfattnError, match="share"):
+            P.rotary(xs, ys, cos, sin)
+    assert all(torch.equal(t, w) for t, w in zip((a, b, c, d), was))
+    P.rotary((a, a), (c, d), cos, sin)  # (two outputs of one input are two)
+    assert torch.equal(c, d)
