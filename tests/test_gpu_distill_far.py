@@ -1,6 +1,7 @@
 """GPU tests of cfops_lm_head_distill at the ends of its values' ranges, against the
 definition in 64 bits, alike for few rows and for many."""
 import math
+import random
 
 import pytest
 import torch
@@ -87,8 +88,32 @@ class Exact:
         self.of_rest = (part * g.abs()) @ w.abs()
 
 
-def check(hn, head, ids, z, lse, dloss):
-    w = Exact(hn, head, ids, z, lse, dloss)
+class Drawn(Exact):
+    """The same where logits are sums of terms of any size, and parts of the rest of any below
+    their entry: the three products of 16 k each round an f32 sum, 2^-24 of the largest each, and
+    an exponential is taken to 2^-36 of its part's largest, 2^-33 where the rows of the head
+    beside it are up to 8 times smaller, times the factor of the rest (2^10 at most of a part that
+    is not scaled up)."""
+
+    def __init__(self, hn, head, ids, z, lse, dloss):
+        super().__init__(hn, head, ids, z, lse, dloss)
+        h, w, g = hn.double(), head.double(), dloss.double()[:, None].abs()
+        x = h @ w.T
+        log_q = torch.log_softmax(x, 1)
+        named = torch.zeros_like(x, dtype=torch.bool).scatter_(1, ids, True)
+        p_rest = -torch.expm1(z.double().logsumexp(1) - lse.double())
+        log_rest = log_q.masked_fill(named, -math.inf).logsumexp(1)
+        part = torch.where(named, 0.0, p_rest[:, None] * (log_q - log_rest[:, None]).exp())
+        more = 2 * 3 * math.ceil(h.shape[1] / 16) * U * (h.abs() @ w.abs().T).amax(1)
+        steep = (p_rest.log() - log_rest).clamp(max=10 * math.log(2.0)).exp()
+        e = ((log_q.exp() + part) * more[:, None] + 2.0 ** -33 * (1 + steep[:, None])) * g
+        self.tol_loss = self.tol_loss + (1 + p_rest) * more
+        self.tol_dhn = self.tol_dhn + e @ w.abs()
+        self.tol_dhead = self.tol_dhead + e.T @ h.abs()
+
+
+def check(hn, head, ids, z, lse, dloss, exact=Exact):
+    w = exact(hn, head, ids, z, lse, dloss)
     keep = keep_of(hn, head, ids)
     loss, res = forward(hn, head, ids, z, lse, keep)
     P.distill_check(res)
@@ -98,6 +123,8 @@ def check(hn, head, ids, z, lse, dloss):
         for got, want, tol in ((loss, w.loss, w.tol_loss), (dhn, w.dhn, w.tol_dhn), (dhead, w.dhead, w.tol_dhead)):
             off = (got.double() - want).abs()
             assert bool((off <= tol).all()), (float((off - tol).max()), float(off.max()))
+    if exact is Drawn:
+        return
     assert bool(((w.tol_dhn < 0.1 * w.of_rest).sum(1) > hn.shape[1] / 2).all())
 
 
@@ -179,3 +206,30 @@ def test_tokens_whose_probabilities_f32_does_not_hold(low):
     z = torch.randn(t, 2, generator=g, device=DEV)
     lse = (z.double().logsumexp(1) - math.log1p(-0.2)).float()
     check(hn, head, ids, z, lse, torch.randn(t, generator=g, device=DEV))
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_drawn_students(seed):
+    """Entries and others at levels up to 500 apart, in parts of any mixture, over rows of the
+    head of one size or of many, with gradients of any size."""
+    rng = random.Random(seed)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    t, d, vocab = rng.choice((20, 64, 65, 150, 300)), rng.choice((16, 33, 64, 200)), rng.choice((130, 300, 700, 5000))
+    k = rng.choice((1, 2, 5, 12, 40, 100))
+    levels = torch.tensor([rng.choice((0.0, 5.0, rng.uniform(0, 60), rng.uniform(30, 160), 500.0)) for _ in range(3)])
+    hn = torch.randn(t, d, generator=g, device=DEV)
+    head = torch.randn(vocab, d, generator=g, device=DEV) * rng.choice((0.05, 0.3, 1.0)) * 4 / d ** 0.5
+    ids = torch.randperm(vocab, generator=g, device=DEV)[:k]
+    if seed % 2:
+        ids = torch.arange(k, device=DEV) + rng.randrange(vocab - k)
+    hn[:, 0], head[:, 0] = 8.0, 0.0
+    head[ids, 0] = levels.to(DEV)[torch.randint(0, 3, (k,), generator=g, device=DEV)] / 8
+    if seed % 3 == 0:
+        head[torch.randperm(vocab, generator=g, device=DEV)[:vocab // 3], 0] -= rng.uniform(0, 20)
+    if seed % 4 == 0:
+        head[:, 1:] *= torch.exp(2 * torch.randn(vocab, 1, generator=g, device=DEV))
+    z = torch.randn(t, k, generator=g, device=DEV) * rng.choice((0.3, 1.0, 5.0))
+    share = rng.choice((1e-5, 0.01, 0.2, 0.9, 0.9999))
+    lse = (z.double().logsumexp(1) - math.log1p(-share)).float()
+    dloss = torch.randn(t, generator=g, device=DEV) * 10.0 ** rng.choice((0, 0, -15, 12))
+    check(hn, head, ids.expand(t, k).contiguous(), z, lse, dloss, Drawn)
